@@ -1,0 +1,270 @@
+// Attention within packed documents: what the forward and backward kernels share. Which keys a query sees, how a
+// workgroup finds its part of a document, and the score's bends (cap, distance bias).
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "element.h"
+
+namespace dllm_hip {
+
+struct DocAttention {
+    const void *q, *k, *v, *out, *dout;  // out: written by the forward, read by the backward
+    void *dq, *dk, *dv;
+    float* lse;  // [heads][tokens]
+    const int64_t *offsets, *prefix;
+    const float* slopes;
+    int64_t q_stride, k_stride, v_stride, out_stride;
+    int tokens, documents, heads, kv_heads, group, head_dim;
+    int causal, window;  // window 0: none
+    float scale, softcap;  // softcap 0: none
+    // backward scratch
+    float* delta;     // [heads][tokens]: dout . out
+    float* dk_part;   // [heads][tokens][head_dim] float32, before the heads of a group are added
+    float* dv_part;
+};
+
+// Token range of a document, and the end of the keys that all its tokens see.
+struct Document {
+    int start, end, prefix_end;
+};
+
+__device__ __forceinline__ int clamp_token(int64_t v, int low, int high) {
+    return v < low ? low : v > high ? high : static_cast<int>(v);
+}
+
+__device__ __forceinline__ Document document_at(const DocAttention& a, int d) {
+    Document r;
+    r.start = clamp_token(a.offsets[d], 0, a.tokens);
+    r.end = clamp_token(a.offsets[d + 1], r.start, a.tokens);
+    r.prefix_end = a.prefix ? r.start + clamp_token(a.prefix[d], 0, r.end - r.start) : r.start;
+    return r;
+}
+
+// The tile-th part of kRows tokens, counted through all documents; each document starts a part of its own, so that what
+// is computed for it does not depend on where it lies. Every lane of the wave returns the same. False past the last part.
+template <int kRows>
+__device__ __forceinline__ bool locate_tile(const DocAttention& a, int64_t tile, Document& doc, int& first) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    int64_t before = 0;
+    for (int base = 0; base < a.documents; base += 64) {
+        const int d = base + lane;
+        Document mine{0, 0, 0};
+        if (d < a.documents) mine = document_at(a, d);
+        const int parts = (mine.end - mine.start + kRows - 1) / kRows;
+        int64_t through = parts;  // parts of the lanes up to this one
+#pragma unroll
+        for (int s = 1; s < 64; s <<= 1) {
+            const int64_t o = __shfl_up(through, s);
+            if (lane >= s) through += o;
+        }
+        const int64_t all = __shfl(through, 63);
+        if (tile < before + all) {
+            const uint64_t past = __ballot(before + through > tile);
+            const int owner = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(past)) - 1);
+            doc.start = __builtin_amdgcn_readlane(mine.start, owner);
+            doc.end = __builtin_amdgcn_readlane(mine.end, owner);
+            doc.prefix_end = __builtin_amdgcn_readlane(mine.prefix_end, owner);
+            const int64_t earlier = __shfl(before + through - parts, owner);
+            first = doc.start + static_cast<int>(tile - earlier) * kRows;
+            first = __builtin_amdgcn_readfirstlane(first);
+            return true;
+        }
+        before += all;
+    }
+    return false;
+}
+
+// The keys that query i sees: [low, high) and [start, prefix_end).
+struct Span {
+    int low, high;
+};
+
+__device__ __forceinline__ Span key_span(const DocAttention& a, const Document& d, int i) {
+    Span s;
+    s.low = a.window && i - d.start >= a.window ? i - a.window + 1 : d.start;
+    s.high = a.causal ? i + 1 : a.window && d.end - i > a.window ? i + a.window : d.end;
+    return s;
+}
+
+// The queries that see key j: one range, since the prefix is seen by all.
+__device__ __forceinline__ Span query_span(const DocAttention& a, const Document& d, int j) {
+    if (j < d.prefix_end) return {d.start, d.end};
+    Span s;
+    s.low = a.causal ? j : a.window && j - d.start >= a.window ? j - a.window + 1 : d.start;
+    s.high = a.window && d.end - j > a.window ? j + a.window : d.end;
+    return s;
+}
+
+__device__ __forceinline__ bool visible(const Document& d, const Span& s, int j) {
+    return (j >= s.low && j < s.high) || (j >= d.start && j < d.prefix_end);
+}
+
+__device__ __forceinline__ float wave_max(float v) {
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) v = fmaxf(v, __shfl_xor(v, s));
+    return v;
+}
+
+__device__ __forceinline__ float wave_add(float v) {
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
+    return v;
+}
+
+// The score of a dot product, and the cap's derivative there.
+__device__ __forceinline__ float bend_score(const DocAttention& a, float slope, float dot, int distance, float& derivative) {
+    float x = dot * a.scale;
+    derivative = 1.0f;
+    if (a.softcap != 0.0f) {
+        const float t = tanhf(x / a.softcap);
+        derivative = 1.0f - t * t;
+        x = a.softcap * t;
+    }
+    return x - slope * static_cast<float>(distance < 0 ? -distance : distance);
+}
+
+template <typename T>
+__device__ __forceinline__ float dot_row(const T* a, const T* b, int n) {
+    float s = 0.0f;
+    for (int d = 0; d < n; ++d) s = fmaf(static_cast<float>(a[d]), static_cast<float>(b[d]), s);
+    return s;
+}
+
+constexpr int kMaxHeadDim = 256;
+constexpr int kLaneDims = kMaxHeadDim / 64;  // head dimensions that a lane of a row's wave holds
+
+// ---- one row by one wave ----
+//
+// Exactly the formula over the visible keys (queries), 64 of them at a time, one per lane. Nothing of a hidden row
+// is touched.
+
+template <typename T>
+__device__ void attention_row(const DocAttention& a, const Document& doc, int head, int i, float (&o)[kLaneDims], float& lse) {
+    const int lane = static_cast<int>(threadIdx.x) & 63, kv = head / a.group;
+    const T* q = static_cast<const T*>(a.q) + i * a.q_stride + static_cast<int64_t>(head) * a.head_dim;
+    const T* k = static_cast<const T*>(a.k) + static_cast<int64_t>(kv) * a.head_dim;
+    const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(kv) * a.head_dim;
+    const float slope = a.slopes ? a.slopes[head] : 0.0f;
+    const Span s = key_span(a, doc, i);
+    const int from = doc.prefix_end > doc.start ? doc.start : s.low;
+    const int to = s.high > doc.prefix_end ? s.high : doc.prefix_end;
+    float m = -INFINITY, l = 0.0f;
+#pragma unroll
+    for (int c = 0; c < kLaneDims; ++c) o[c] = 0.0f;
+    for (int base = from; base < to; base += 64) {
+        const int j = base + lane;
+        const bool see = j < to && visible(doc, s, j);
+        if (!__any(see)) continue;
+        float unused;
+        const float x = see ? bend_score(a, slope, dot_row(q, k + j * a.k_stride, a.head_dim), i - j, unused) : -INFINITY;
+        const float top = fmaxf(m, wave_max(x));
+        const float p = x == -INFINITY ? 0.0f : expf(x - top);
+        const float keep = m == top ? 1.0f : expf(m - top);
+        m = top;
+        l = l * keep + wave_add(p);
+#pragma unroll
+        for (int c = 0; c < kLaneDims; ++c) o[c] *= keep;
+        for (uint64_t left = __ballot(see); left; left &= left - 1) {
+            const int from_lane = __ffsll(static_cast<unsigned long long>(left)) - 1;
+            const float pj = __shfl(p, from_lane);
+            const T* row = v + (base + from_lane) * a.v_stride;
+#pragma unroll
+            for (int c = 0; c < kLaneDims; ++c)
+                if (lane + 64 * c < a.head_dim) o[c] = fmaf(pj, static_cast<float>(row[lane + 64 * c]), o[c]);
+        }
+    }
+#pragma unroll
+    for (int c = 0; c < kLaneDims; ++c) o[c] /= l;
+    lse = m + logf(l);
+}
+
+template <typename T>
+__device__ void attention_row_dq(const DocAttention& a, const Document& doc, int head, int i, float delta, float (&dq)[kLaneDims]) {
+    const int lane = static_cast<int>(threadIdx.x) & 63, kv = head / a.group;
+    const int64_t at = static_cast<int64_t>(head) * a.head_dim;
+    const T* q = static_cast<const T*>(a.q) + i * a.q_stride + at;
+    const T* dout = static_cast<const T*>(a.dout) + i * a.out_stride + at;
+    const T* k = static_cast<const T*>(a.k) + static_cast<int64_t>(kv) * a.head_dim;
+    const T* v = static_cast<const T*>(a.v) + static_cast<int64_t>(kv) * a.head_dim;
+    const float slope = a.slopes ? a.slopes[head] : 0.0f;
+    const float lse = a.lse[static_cast<int64_t>(head) * a.tokens + i];
+    const Span s = key_span(a, doc, i);
+    const int from = doc.prefix_end > doc.start ? doc.start : s.low;
+    const int to = s.high > doc.prefix_end ? s.high : doc.prefix_end;
+#pragma unroll
+    for (int c = 0; c < kLaneDims; ++c) dq[c] = 0.0f;
+    for (int base = from; base < to; base += 64) {
+        const int j = base + lane;
+        const bool see = j < to && visible(doc, s, j);
+        float ds = 0.0f;
+        if (see) {
+            float derivative;
+            const float x = bend_score(a, slope, dot_row(q, k + j * a.k_stride, a.head_dim), i - j, derivative);
+            const float dp = dot_row(dout, v + j * a.v_stride, a.head_dim);
+            ds = expf(x - lse) * (dp - delta) * derivative * a.scale;
+        }
+        for (uint64_t left = __ballot(see); left; left &= left - 1) {
+            const int from_lane = __ffsll(static_cast<unsigned long long>(left)) - 1;
+            const float d = __shfl(ds, from_lane);
+            const T* row = k + (base + from_lane) * a.k_stride;
+#pragma unroll
+            for (int c = 0; c < kLaneDims; ++c)
+                if (lane + 64 * c < a.head_dim) dq[c] = fmaf(d, static_cast<float>(row[lane + 64 * c]), dq[c]);
+        }
+    }
+}
+
+// One head's part of dk and dv of key j.
+template <typename T>
+__device__ void attention_row_dkv(const DocAttention& a, const Document& doc, int head, int j, float (&dk)[kLaneDims],
+                                  float (&dv)[kLaneDims]) {
+    const int lane = static_cast<int>(threadIdx.x) & 63, kv = head / a.group;
+    const int64_t at = static_cast<int64_t>(head) * a.head_dim;
+    const T* q = static_cast<const T*>(a.q) + at;
+    const T* dout = static_cast<const T*>(a.dout) + at;
+    const T* k = static_cast<const T*>(a.k) + j * a.k_stride + static_cast<int64_t>(kv) * a.head_dim;
+    const T* v = static_cast<const T*>(a.v) + j * a.v_stride + static_cast<int64_t>(kv) * a.head_dim;
+    const float slope = a.slopes ? a.slopes[head] : 0.0f;
+    const float* lse = a.lse + static_cast<int64_t>(head) * a.tokens;
+    const float* delta = a.delta + static_cast<int64_t>(head) * a.tokens;
+    const Span s = query_span(a, doc, j);
+#pragma unroll
+    for (int c = 0; c < kLaneDims; ++c) dk[c] = dv[c] = 0.0f;
+    for (int base = s.low; base < s.high; base += 64) {
+        const int i = base + lane;
+        const bool see = i < s.high;
+        float p = 0.0f, ds = 0.0f;
+        if (see) {
+            float derivative;
+            const float x = bend_score(a, slope, dot_row(q + i * a.q_stride, k, a.head_dim), i - j, derivative);
+            const float dp = dot_row(dout + i * a.out_stride, v, a.head_dim);
+            p = expf(x - lse[i]);
+            ds = p * (dp - delta[i]) * derivative * a.scale;
+        }
+        for (uint64_t left = __ballot(see); left; left &= left - 1) {
+            const int from_lane = __ffsll(static_cast<unsigned long long>(left)) - 1;
+            const float pj = __shfl(p, from_lane), dj = __shfl(ds, from_lane);
+            const T* qi = q + (base + from_lane) * a.q_stride;
+            const T* di = dout + (base + from_lane) * a.out_stride;
+#pragma unroll
+            for (int c = 0; c < kLaneDims; ++c)
+                if (lane + 64 * c < a.head_dim) {
+                    dk[c] = fmaf(dj, static_cast<float>(qi[lane + 64 * c]), dk[c]);
+                    dv[c] = fmaf(pj, static_cast<float>(di[lane + 64 * c]), dv[c]);
+                }
+        }
+    }
+}
+
+// A row of head_dim elements from a wave's registers.
+template <typename To>
+__device__ __forceinline__ void store_row(To* to, const float (&v)[kLaneDims], int head_dim) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+#pragma unroll
+    for (int c = 0; c < kLaneDims; ++c)
+        if (lane + 64 * c < head_dim) to[lane + 64 * c] = static_cast<To>(v[c]);
+}
+
+}  // namespace dllm_hip

@@ -1,0 +1,367 @@
+// The end of one block and the start of the next: h = x + scale gate post(y), n = pre(h), and its gradients.
+//
+// With r = 1 / sqrt(mean(x^2) + eps), a norm is x r w, and its gradient for an upstream d is
+//     dx = r w d - x c,  c = r^3 / dim sum(w d x),    dw = sum over rows of d x r.
+// So a row needs, forward, sum y^2 then sum h^2, and backward sum h^2, sum w dn h and sum y^2 together, then (from
+// g = dh + r_h w dn - h c_h) sum w gate scale g y. All sums are float32, each thread's terms in column order, then the
+// threads of a wave and the waves of a workgroup in a fixed tree: a row's bits depend on the row alone.
+//
+// Bound: HBM, each row array read and written once.
+#include <algorithm>
+
+#include "common.h"
+#include "dllm_hip.h"
+#include "element.h"
+#include "workspace.h"
+
+using namespace dllm_hip;
+
+namespace {
+
+struct NormArgs {
+    const void *x, *y, *gate;  // x: the residual stream (forward), h (backward)
+    const float *post_weight, *pre_weight;
+    const void *dh, *dn;
+    void *h, *n;             // forward outputs
+    void *dx, *dy, *dgate;   // backward outputs
+    float *stats;            // [rows][4]: r_h, c_h, r_y, c_y
+    float *partial;          // [3][chunks][dim]: gate, post, pre
+    int64_t rows, dim;
+    int post, pre, gate_kind;
+    float offset;  // 1 with unit_offset
+    float eps, scale, inv_dim;
+    int64_t chunk_rows;
+    int sums;  // bit 0: dgate, 1: dpost_weight, 2: dpre_weight
+};
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
+    return v;
+}
+
+// Sums of a workgroup's values, the waves' added in wave order; every thread gets them. scratch: 16 * N floats.
+template <int N>
+__device__ __forceinline__ void block_sum(float (&v)[N], float* scratch) {
+    const int wave = static_cast<int>(threadIdx.x) >> 6, waves = static_cast<int>(blockDim.x) >> 6;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    if (waves == 1) return;
+    __syncthreads();  // the scratch's readers of the last sum are done
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) scratch[wave * N + i] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        float t = scratch[i];
+        for (int w = 1; w < waves; ++w) t += scratch[w * N + i];
+        v[i] = t;
+    }
+}
+
+__device__ __forceinline__ float weight_at(const float* w, int64_t c, float offset) {
+    return w ? offset + w[c] : 1.0f;
+}
+
+template <typename T>
+__device__ __forceinline__ float gate_at(const NormArgs& a, int64_t row, int64_t c) {
+    if (a.gate_kind == 0) return 1.0f;
+    if (a.gate_kind == 1) return static_cast<const float*>(a.gate)[c];
+    return static_cast<float>(static_cast<const T*>(a.gate)[row * a.dim + c]);
+}
+
+__device__ __forceinline__ float inverse_rms(float sum_squares, const NormArgs& a) {
+    return 1.0f / sqrtf(sum_squares * a.inv_dim + a.eps);
+}
+
+// ---- rows of any size and alignment: one workgroup per row, a pass over it for each sum ----
+
+template <typename T>
+__global__ __launch_bounds__(256) void forward_any_kernel(NormArgs a) {
+    __shared__ float scratch[16];
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* x = static_cast<const T*>(a.x) + row * a.dim;
+        const T* y = static_cast<const T*>(a.y) + row * a.dim;
+        float ry = 1.0f, rh = 1.0f;
+        if (a.post) {
+            float s[1] = {0.0f};
+            for (int64_t c = threadIdx.x; c < a.dim; c += 256) {
+                const float v = static_cast<float>(y[c]);
+                s[0] = fmaf(v, v, s[0]);
+            }
+            block_sum(s, scratch);
+            ry = inverse_rms(s[0], a);
+        }
+        auto new_h = [&](int64_t c) {
+            float z = static_cast<float>(y[c]);
+            if (a.post) z = z * ry * weight_at(a.post_weight, c, a.offset);
+            return fmaf(a.scale, z * gate_at<T>(a, row, c), static_cast<float>(x[c]));
+        };
+        if (a.pre) {
+            float s[1] = {0.0f};
+            for (int64_t c = threadIdx.x; c < a.dim; c += 256) {
+                const float v = new_h(c);
+                s[0] = fmaf(v, v, s[0]);
+            }
+            block_sum(s, scratch);
+            rh = inverse_rms(s[0], a);
+        }
+        for (int64_t c = threadIdx.x; c < a.dim; c += 256) {
+            const float v = new_h(c);  // h may be x: read before it is written, by the same thread
+            static_cast<T*>(a.h)[row * a.dim + c] = static_cast<T>(v);
+            if (a.pre) static_cast<T*>(a.n)[row * a.dim + c] = static_cast<T>(v * rh * weight_at(a.pre_weight, c, a.offset));
+        }
+    }
+}
+
+// The gradient of h through its uses, and the parts of it that the post norm and the gate see, at one element.
+template <typename T>
+struct BackwardElement {
+    float g, y, z, hat_y, w_post, gate, du;
+    __device__ BackwardElement(const NormArgs& a, int64_t row, int64_t c, float rh, float ch, float ry) {
+        const int64_t at = row * a.dim + c;
+        g = a.dh ? static_cast<float>(static_cast<const T*>(a.dh)[at]) : 0.0f;
+        if (a.pre)
+            g += fmaf(rh * weight_at(a.pre_weight, c, a.offset), static_cast<float>(static_cast<const T*>(a.dn)[at]),
+                      -(static_cast<float>(static_cast<const T*>(a.x)[at]) * ch));
+        y = static_cast<float>(static_cast<const T*>(a.y)[at]);
+        hat_y = a.post ? y * ry : y;
+        w_post = a.post ? weight_at(a.post_weight, c, a.offset) : 1.0f;
+        z = hat_y * w_post;
+        gate = gate_at<T>(a, row, c);
+        du = a.scale * g * gate;
+    }
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void backward_stats_any_kernel(NormArgs a) {
+    __shared__ float scratch[16];
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const T* h = static_cast<const T*>(a.x) + row * a.dim;
+        const T* y = static_cast<const T*>(a.y) + row * a.dim;
+        float s[3] = {0.0f, 0.0f, 0.0f};
+        for (int64_t c = threadIdx.x; c < a.dim; c += 256) {
+            if (a.pre) {
+                const float v = static_cast<float>(h[c]);
+                s[0] = fmaf(v, v, s[0]);
+                s[1] = fmaf(weight_at(a.pre_weight, c, a.offset) * static_cast<float>(static_cast<const T*>(a.dn)[row * a.dim + c]),
+                            v, s[1]);
+            }
+            if (a.post) {
+                const float v = static_cast<float>(y[c]);
+                s[2] = fmaf(v, v, s[2]);
+            }
+        }
+        block_sum(s, scratch);
+        const float rh = a.pre ? inverse_rms(s[0], a) : 0.0f;
+        const float ch = a.pre ? rh * rh * rh * a.inv_dim * s[1] : 0.0f;
+        const float ry = a.post ? inverse_rms(s[2], a) : 1.0f;
+        float cy = 0.0f;
+        if (a.post) {
+            float u[1] = {0.0f};
+            for (int64_t c = threadIdx.x; c < a.dim; c += 256) {
+                const BackwardElement<T> e(a, row, c, rh, ch, ry);
+                u[0] = fmaf(e.du * e.w_post, e.y, u[0]);
+            }
+            block_sum(u, scratch);
+            cy = ry * ry * ry * a.inv_dim * u[0];
+        }
+        if (threadIdx.x == 0) {
+            float* st = a.stats + row * 4;
+            st[0] = rh, st[1] = ch, st[2] = ry, st[3] = cy;
+        }
+    }
+}
+
+// partial[k][chunk][c]: the sums over one chunk of rows, in row order.
+template <typename T>
+__global__ __launch_bounds__(256) void backward_columns_any_kernel(NormArgs a) {
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    const int64_t chunk = blockIdx.y, chunks = gridDim.y;
+    if (c >= a.dim) return;
+    const int64_t end = std::min<int64_t>(a.rows, (chunk + 1) * a.chunk_rows);
+    float s[3] = {0.0f, 0.0f, 0.0f};
+    for (int64_t row = chunk * a.chunk_rows; row < end; ++row) {
+        const float* st = a.stats + row * 4;
+        const BackwardElement<T> e(a, row, c, st[0], st[1], st[2]);
+        s[0] = fmaf(a.scale * e.g, e.z, s[0]);
+        s[1] = fmaf(e.du, e.hat_y, s[1]);
+        if (a.pre)
+            s[2] = fmaf(static_cast<float>(static_cast<const T*>(a.dn)[row * a.dim + c]),
+                        static_cast<float>(static_cast<const T*>(a.x)[row * a.dim + c]) * st[0], s[2]);
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+        if (a.sums >> k & 1) a.partial[(k * chunks + chunk) * a.dim + c] = s[k];
+}
+
+template <typename T>
+__global__ __launch_bounds__(256) void backward_rows_any_kernel(NormArgs a) {
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const float* st = a.stats + row * 4;
+        for (int64_t c = threadIdx.x; c < a.dim; c += 256) {
+            const BackwardElement<T> e(a, row, c, st[0], st[1], st[2]);
+            const int64_t at = row * a.dim + c;
+            if (a.dx) static_cast<T*>(a.dx)[at] = static_cast<T>(e.g);  // dx may be dh: read above by the same thread
+            if (a.dgate && a.gate_kind == 2) static_cast<T*>(a.dgate)[at] = static_cast<T>(a.scale * e.g * e.z);
+            if (a.dy) static_cast<T*>(a.dy)[at] = static_cast<T>(a.post ? fmaf(st[2] * e.w_post, e.du, -(e.y * st[3])) : e.du);
+        }
+    }
+}
+
+// out[k][c] = the chunks' sums: 16 rows of threads take every 16th chunk in order, then are added in order.
+__global__ __launch_bounds__(1024) void column_reduce_kernel(const float* __restrict__ partial, float* dgate,
+                                                             float* dpost, float* dpre, int64_t dim, int64_t chunks) {
+    __shared__ float part[16][64];
+    const int col = threadIdx.x & 63, lane_row = threadIdx.x >> 6;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + col;
+    float* const out = blockIdx.y == 0 ? dgate : blockIdx.y == 1 ? dpost : dpre;
+    if (!out) return;
+    const float* p = partial + static_cast<int64_t>(blockIdx.y) * chunks * dim;
+    float s = 0.0f;
+    if (c < dim)
+        for (int64_t k = lane_row; k < chunks; k += 16) s += p[k * dim + c];
+    part[lane_row][col] = s;
+    __syncthreads();
+    if (lane_row || c >= dim) return;
+    for (int r = 1; r < 16; ++r) s += part[r][col];
+    out[c] = s;
+}
+
+constexpr int64_t kMaxGrid = 1 << 16;  // rows beyond it are taken in turn
+
+int64_t any_chunk_rows(int64_t rows) { return std::max<int64_t>(64, ceil_div(rows, 1024)); }
+
+struct BackwardLayout {
+    int64_t chunks;
+    size_t stats, partial, bytes;
+};
+
+BackwardLayout backward_layout(const dllm_hip_residual_norm_shape& sh) {
+    BackwardLayout b;
+    Layout l;
+    b.stats = static_cast<size_t>(sh.rows) * 4;
+    b.chunks = static_cast<int64_t>(ceil_div(sh.rows, any_chunk_rows(sh.rows)));
+    b.partial = static_cast<size_t>(3 * b.chunks * sh.dim);
+    l.add<float>(b.stats);
+    l.add<float>(b.partial);
+    b.bytes = l.bytes;
+    return b;
+}
+
+int check_shape(const dllm_hip_residual_norm_shape* sh) {
+    DLLM_REQUIRE(sh != nullptr, "null shape");
+    DLLM_REQUIRE(sh->dtype >= 0 && sh->dtype <= 2, "dtype must be float32 (0), bfloat16 (1) or float16 (2)");
+    DLLM_REQUIRE(sh->rows >= 0 && sh->rows < (int64_t{1} << 31), "rows must be in [0, 2^31)");
+    DLLM_REQUIRE(sh->dim >= 1 && sh->dim <= (1 << 20), "dim must be in [1, 2^20]");
+    DLLM_REQUIRE(sh->norm_placement >= 0 && sh->norm_placement <= 2, "norm_placement must be pre (0), post (1) or both (2)");
+    DLLM_REQUIRE(sh->gate >= 0 && sh->gate <= 2, "gate must be none (0), per channel (1) or per element (2)");
+    DLLM_REQUIRE(sh->eps >= 0.0, "eps must not be negative");
+    return kOk;
+}
+
+NormArgs arguments(const dllm_hip_residual_norm_shape& sh) {
+    NormArgs a{};
+    a.rows = sh.rows;
+    a.dim = sh.dim;
+    a.post = sh.norm_placement != 0;
+    a.pre = sh.norm_placement != 1;
+    a.gate_kind = static_cast<int>(sh.gate);
+    a.offset = sh.unit_offset ? 1.0f : 0.0f;
+    a.eps = static_cast<float>(sh.eps);
+    a.scale = static_cast<float>(sh.residual_scale);
+    a.inv_dim = 1.0f / static_cast<float>(sh.dim);
+    return a;
+}
+
+template <typename T>
+int launch_forward(const NormArgs& a, hipStream_t stream) {
+    forward_any_kernel<T><<<static_cast<unsigned>(std::min(a.rows, kMaxGrid)), 256, 0, stream>>>(a);
+    return check_launch("residual_norm");
+}
+
+template <typename T>
+int launch_backward(const NormArgs& a, int64_t chunks, float* dpost, float* dpre, hipStream_t stream) {
+    const unsigned rows = static_cast<unsigned>(std::min(a.rows, kMaxGrid));
+    backward_stats_any_kernel<T><<<rows, 256, 0, stream>>>(a);
+    if (a.sums) {
+        const dim3 grid(static_cast<unsigned>(ceil_div(a.dim, 256)), static_cast<unsigned>(chunks));
+        backward_columns_any_kernel<T><<<grid, 256, 0, stream>>>(a);
+        column_reduce_kernel<<<dim3(static_cast<unsigned>(ceil_div(a.dim, 64)), 3), 1024, 0, stream>>>(
+            a.partial, a.sums & 1 ? static_cast<float*>(a.dgate) : nullptr, dpost, dpre, a.dim, chunks);
+    }
+    if (a.dx || a.dy || (a.dgate && a.gate_kind == 2)) backward_rows_any_kernel<T><<<rows, 256, 0, stream>>>(a);
+    return check_launch("residual_norm_backward");
+}
+
+}  // namespace
+
+extern "C" {
+
+int dllm_hip_residual_norm(const dllm_hip_residual_norm_shape* sh, const void* x, const void* y, const void* gate,
+                           const float* post_weight, const float* pre_weight, void* h, void* n, void* stream) {
+    DLLM_TRY(check_shape(sh));
+    if (sh->rows == 0) return kOk;
+    NormArgs a = arguments(*sh);
+    DLLM_REQUIRE(x && y && h && (n || !a.pre) && (gate || a.gate_kind == 0), "null x, y, gate, h or n");
+    const size_t size = element_bytes(sh->dtype);
+    DLLM_REQUIRE(aligned_to(x, size) && aligned_to(y, size) && aligned_to(h, size) && aligned_to(n, size) &&
+                     aligned_to(gate, a.gate_kind == 1 ? 4 : size) && aligned_to(post_weight, 4) &&
+                     aligned_to(pre_weight, 4),
+                 "pointers must be aligned to the element");
+    a.x = x, a.y = y, a.gate = gate, a.post_weight = post_weight, a.pre_weight = pre_weight, a.h = h, a.n = n;
+    auto s = static_cast<hipStream_t>(stream);
+    switch (sh->dtype) {
+        case kFloat32: return launch_forward<float>(a, s);
+        case kBFloat16: return launch_forward<__bf16>(a, s);
+        default: return launch_forward<_Float16>(a, s);
+    }
+}
+
+size_t dllm_hip_residual_norm_backward_workspace(const dllm_hip_residual_norm_shape* sh) {
+    return check_shape(sh) == kOk ? backward_layout(*sh).bytes : 0;
+}
+
+int dllm_hip_residual_norm_backward(const dllm_hip_residual_norm_shape* sh, const void* h, const void* y,
+                                    const void* gate, const float* post_weight, const float* pre_weight,
+                                    const void* dh, const void* dn, void* dx, void* dy, void* dgate,
+                                    float* dpost_weight, float* dpre_weight, void* workspace, size_t workspace_bytes,
+                                    void* stream) {
+    DLLM_TRY(check_shape(sh));
+    NormArgs a = arguments(*sh);
+    DLLM_REQUIRE(a.gate_kind || !dgate, "dgate without a gate");
+    DLLM_REQUIRE((a.post || !dpost_weight) && (a.pre || !dpre_weight), "a weight gradient of a norm that is not there");
+    auto s = static_cast<hipStream_t>(stream);
+    if (sh->rows == 0) {  // sums over no rows
+        for (float* out : {a.gate_kind == 1 ? static_cast<float*>(dgate) : nullptr, dpost_weight, dpre_weight})
+            if (out) column_reduce_kernel<<<dim3(static_cast<unsigned>(ceil_div(a.dim, 64))), 1024, 0, s>>>(nullptr, out, nullptr, nullptr, a.dim, 0);
+        return check_launch("residual_norm_backward");
+    }
+    DLLM_REQUIRE((h || !a.pre) && y && (gate || a.gate_kind == 0) && (dn || !a.pre) && (dh || a.pre),
+                 "null h, y, gate, dh or dn");
+    const size_t size = element_bytes(sh->dtype);
+    for (const void* p : {h, y, dh, dn, static_cast<const void*>(dx), static_cast<const void*>(dy)})
+        DLLM_REQUIRE(aligned_to(p, size), "pointers must be aligned to the element");
+    for (const void* p : {gate, static_cast<const void*>(dgate)})
+        DLLM_REQUIRE(aligned_to(p, a.gate_kind == 1 ? 4 : size), "pointers must be aligned to the element");
+    for (const float* p : {post_weight, pre_weight, static_cast<const float*>(dpost_weight), static_cast<const float*>(dpre_weight)})
+        DLLM_REQUIRE(aligned_to(p, 4), "pointers must be aligned to the element");
+    const BackwardLayout b = backward_layout(*sh);
+    DLLM_REQUIRE(workspace && workspace_bytes >= b.bytes, "workspace too small for residual_norm_backward");
+    DLLM_REQUIRE(aligned_to(workspace, 16), "the workspace must be aligned to 16 bytes");
+    Carve c(workspace, workspace_bytes);
+    a.stats = c.take<float>(b.stats);
+    a.partial = c.take<float>(b.partial);
+    a.x = h, a.y = y, a.gate = gate, a.post_weight = post_weight, a.pre_weight = pre_weight, a.dh = dh, a.dn = dn;
+    a.dx = dx, a.dy = dy, a.dgate = dgate;
+    a.chunk_rows = any_chunk_rows(sh->rows);
+    a.sums = (a.gate_kind == 1 && dgate ? 1 : 0) | (dpost_weight ? 2 : 0) | (dpre_weight ? 4 : 0);
+    switch (sh->dtype) {
+        case kFloat32: return launch_backward<float>(a, b.chunks, dpost_weight, dpre_weight, s);
+        case kBFloat16: return launch_backward<__bf16>(a, b.chunks, dpost_weight, dpre_weight, s);
+        default: return launch_backward<_Float16>(a, b.chunks, dpost_weight, dpre_weight, s);
+    }
+}
+
+}  // extern "C"

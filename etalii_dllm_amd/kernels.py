@@ -18,11 +18,38 @@ import numpy as np
 
 LIBRARY = Path(__file__).resolve().parent / "libdllm_hip.so"
 
+# the activations' types of the packed-layer operators
+DTYPES = {"float32": 0, "bfloat16": 1, "float16": 2}
+
 _f32p = C.POINTER(C.c_float)
 _f64p = C.POINTER(C.c_double)
 _i64p = C.POINTER(C.c_int64)
 _sz = C.c_size_t
 _vp = C.c_void_p
+
+
+class DocumentAttention(C.Structure):
+    """dllm_hip_document_attention_shape; strides in elements, 0 for packed rows."""
+
+    _fields_ = [(n, C.c_int64) for n in ("dtype", "tokens", "documents", "heads", "kv_heads", "head_dim", "causal",
+                                         "window")]
+    _fields_ += [("scale", C.c_double), ("softcap", C.c_double)]
+    _fields_ += [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride", "out_stride")]
+
+
+class RopeAxes(C.Structure):
+    """dllm_hip_rope_axes_shape; strides in elements, 0 for packed rows."""
+
+    _fields_ = [(n, C.c_int64) for n in ("dtype", "tokens", "q_heads", "k_heads", "head_dim", "pairs", "axes",
+                                         "interleaved", "inverse", "q_stride", "k_stride", "q_out_stride",
+                                         "k_out_stride")]
+
+
+class ResidualNorm(C.Structure):
+    """dllm_hip_residual_norm_shape."""
+
+    _fields_ = [(n, C.c_int64) for n in ("dtype", "rows", "dim", "norm_placement", "gate", "unit_offset")]
+    _fields_ += [("eps", C.c_double), ("residual_scale", C.c_double)]
 
 
 def _load() -> C.CDLL:
@@ -92,6 +119,16 @@ def _load() -> C.CDLL:
     lib.dllm_hip_lora_adapter_gradients_workspace.argtypes = [_sz, _sz, _sz]
     lib.dllm_hip_lora_adapter_gradients.argtypes = [_vp, _vp, _vp, _vp, _vp, _sz, _sz, _sz, C.c_double, _vp, _sz,
                                                     _vp]
+    attention, rope, norm = (C.POINTER(t) for t in (DocumentAttention, RopeAxes, ResidualNorm))
+    for name, shape in (("document_attention", attention), ("document_attention_backward", attention),
+                        ("residual_norm_backward", norm)):
+        query = getattr(lib, f"dllm_hip_{name}_workspace")
+        query.restype, query.argtypes = _sz, [shape]
+    lib.dllm_hip_document_attention.argtypes = [attention] + [_vp] * 9 + [_sz, _vp]
+    lib.dllm_hip_document_attention_backward.argtypes = [attention] + [_vp] * 13 + [_sz, _vp]
+    lib.dllm_hip_rope_axes.argtypes = [rope] + [_vp] * 8
+    lib.dllm_hip_residual_norm.argtypes = [norm] + [_vp] * 8
+    lib.dllm_hip_residual_norm_backward.argtypes = [norm] + [_vp] * 13 + [_sz, _vp]
     return lib
 
 
@@ -802,3 +839,169 @@ def rope_attention_factor(scaling) -> float:
 def attention_scale(head_dim: int) -> float:
     """architecture.py:311-312: 1 / sqrt(head_dim)."""
     return 1.0 / math.sqrt(head_dim)
+
+
+# ---- operators of packed layers (no counterpart in cpp/kernels.cpp) ----
+#
+# Activations are float32 or float16 arrays, or uint16 arrays of bfloat16 bits; results have their type.
+
+_ACTIVATIONS = {np.dtype(np.float32): 0, np.dtype(np.uint16): 1, np.dtype(np.float16): 2}
+
+
+def _activation_type(*arrays) -> int:
+    types = {np.asarray(a).dtype for a in arrays if a is not None}
+    if len(types) != 1 or (dtype := types.pop()) not in _ACTIVATIONS:
+        raise ValueError("activations must share one type: float32, float16 or uint16 (bfloat16 bits)")
+    return _ACTIVATIONS[dtype]
+
+
+def _upload(array, dtype=None):
+    """(device copy or None, its pointer)."""
+    if array is None:
+        return None, None
+    d = Device.of(np.ascontiguousarray(array, dtype=dtype))
+    return d, d.ptr
+
+
+def _document_shape(q, k, v, offsets, prefix, slopes, scale, causal, window, softcap):
+    q, k, v = np.asarray(q), np.asarray(k), np.asarray(v)
+    dtype = _activation_type(q, k, v)
+    if q.ndim != 3 or k.ndim != 3 or v.ndim != 3:
+        raise ValueError("q, k and v must be [tokens, heads, head_dim]")
+    if k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError("k and v must have one shape, and q's tokens and head_dim")
+    if k.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError("q heads must be a multiple of kv heads")
+    offsets = np.ascontiguousarray(offsets, dtype=np.int64)
+    if offsets.ndim != 1 or len(offsets) < 1:
+        raise ValueError("offsets must have one value more than there are documents")
+    if offsets[0] < 0 or offsets[-1] > q.shape[0] or np.any(np.diff(offsets) < 0):
+        raise ValueError("offsets must be non-decreasing and within the tokens")
+    if prefix is not None and len(prefix) != len(offsets) - 1:
+        raise ValueError("prefix must have one length per document")
+    if slopes is not None and len(slopes) != q.shape[1]:
+        raise ValueError("slopes must have one value per head")
+    if window < 0 or softcap < 0:
+        raise ValueError("window and softcap must not be negative")
+    shape = DocumentAttention(dtype, q.shape[0], len(offsets) - 1, q.shape[1], k.shape[1], q.shape[2], int(causal),
+                              int(window), float(scale), float(softcap))
+    return q, k, v, offsets, shape
+
+
+def document_attention(q, k, v, offsets, scale, causal=True, window=0, prefix=None, softcap=0.0, slopes=None):
+    """Attention within the documents offsets[d] .. offsets[d + 1] of a packed batch: (out, lse [heads, tokens]). Tokens
+    of no document are zero in both."""
+    q, k, v, offsets, shape = _document_shape(q, k, v, offsets, prefix, slopes, scale, causal, window, softcap)
+    dq, dk, dv, do = Device.of(q), Device.of(k), Device.of(v), Device.of(offsets)
+    dp, prefix_ptr = _upload(prefix, np.int64)
+    ds, slopes_ptr = _upload(slopes, np.float32)
+    out, lse = Device.of(np.zeros_like(q)), Device.of(np.zeros((q.shape[1], q.shape[0]), np.float32))
+    ws = Device(lib.dllm_hip_document_attention_workspace(shape))
+    check(lib.dllm_hip_document_attention(shape, dq.ptr, dk.ptr, dv.ptr, do.ptr, prefix_ptr, slopes_ptr, out.ptr,
+                                          lse.ptr, ws.ptr, ws.nbytes, None))
+    return out.download(q.shape, q.dtype), lse.download((q.shape[1], q.shape[0]))
+
+
+def document_attention_backward(q, k, v, offsets, out, lse, dout, scale, causal=True, window=0, prefix=None, softcap=0.0,
+                                slopes=None):
+    """(dq, dk, dv) of document_attention from its out and lse and the upstream dout."""
+    q, k, v, offsets, shape = _document_shape(q, k, v, offsets, prefix, slopes, scale, causal, window, softcap)
+    out, dout = np.asarray(out), np.asarray(dout)
+    _activation_type(q, out, dout)
+    if out.shape != q.shape or dout.shape != q.shape or np.shape(lse) != (q.shape[1], q.shape[0]):
+        raise ValueError("out and dout must have q's shape, lse [heads, tokens]")
+    ins = [Device.of(x) for x in (q, k, v, offsets, out, _f32(lse), dout)]
+    dp, prefix_ptr = _upload(prefix, np.int64)
+    ds, slopes_ptr = _upload(slopes, np.float32)
+    grads = [Device.of(np.zeros_like(x)) for x in (q, k, v)]
+    ws = Device(lib.dllm_hip_document_attention_backward_workspace(shape))
+    check(lib.dllm_hip_document_attention_backward(
+        shape, ins[0].ptr, ins[1].ptr, ins[2].ptr, ins[3].ptr, prefix_ptr, slopes_ptr, ins[4].ptr, ins[5].ptr,
+        ins[6].ptr, grads[0].ptr, grads[1].ptr, grads[2].ptr, ws.ptr, ws.nbytes, None))
+    return tuple(g.download(x.shape, x.dtype) for g, x in zip(grads, (q, k, v)))
+
+
+def rope_axes(q, k, positions, inv_freq, pair_axis, interleaved=False, inverse=False):
+    """(q, k) [tokens, heads, head_dim] with pair p turned by positions[pair_axis[p]] * inv_freq[p]; k may be None."""
+    q = np.asarray(q)
+    dtype = _activation_type(q, k)
+    if q.ndim != 3 or (k is not None and (np.ndim(k) != 3 or np.shape(k)[0] != q.shape[0] or np.shape(k)[2] != q.shape[2])):
+        raise ValueError("q and k must be [tokens, heads, head_dim] with one number of tokens and one head_dim")
+    pos = np.ascontiguousarray(positions, dtype=np.int64)
+    freqs = np.ascontiguousarray(inv_freq, dtype=np.float64)
+    axis = np.ascontiguousarray(pair_axis, dtype=np.uint8)
+    if pos.ndim != 2 or pos.shape[1] != q.shape[0]:
+        raise ValueError("positions must be [axes, tokens]")
+    if freqs.ndim != 1 or axis.shape != freqs.shape:
+        raise ValueError("inv_freq and pair_axis must have one entry per pair")
+    if 2 * len(freqs) > q.shape[2]:
+        raise ValueError("2 * len(inv_freq) must not exceed head_dim")
+    if len(axis) and axis.max() >= pos.shape[0]:
+        raise ValueError("pair_axis must be below the number of axes")
+    k_heads = 0 if k is None else np.shape(k)[1]
+    shape = RopeAxes(dtype, q.shape[0], q.shape[1], k_heads, q.shape[2], len(freqs), pos.shape[0], int(interleaved),
+                     int(inverse))
+    dq, dp, df, da, q_out = Device.of(q), Device.of(pos), Device.of(freqs), Device.of(axis), Device(q.nbytes)
+    dk, k_ptr = _upload(k)
+    k_out = None if k is None else Device(dk.nbytes)
+    check(lib.dllm_hip_rope_axes(shape, dq.ptr, k_ptr, dp.ptr, df.ptr, da.ptr, q_out.ptr,
+                                 None if k_out is None else k_out.ptr, None))
+    return q_out.download(q.shape, q.dtype), None if k is None else k_out.download(np.shape(k), q.dtype)
+
+
+def _norm_shape(x, y, gate, post_weight, pre_weight, norm_placement, eps, unit_offset, residual_scale):
+    x, y = np.asarray(x), np.asarray(y)
+    dtype = _activation_type(x, y)
+    if x.ndim < 1 or x.shape != y.shape:
+        raise ValueError("the residual stream and the block's output must have one shape")
+    dim = x.shape[-1]
+    kind = 0 if gate is None else 1 if np.ndim(gate) == 1 and x.ndim > 1 else 2
+    if kind == 1 and (np.shape(gate) != (dim,) or np.asarray(gate).dtype != np.float32):
+        raise ValueError("a gate for each channel must be float32 [dim]")
+    if kind == 2 and (np.shape(gate) != x.shape or np.asarray(gate).dtype != x.dtype):
+        raise ValueError("a gate for each element must have the block output's shape and type")
+    for w in (post_weight, pre_weight):
+        if w is not None and np.shape(w) != (dim,):
+            raise ValueError("weight length must equal the last dimension of x")
+    return x, y, kind, ResidualNorm(dtype, _rows(x), dim, int(norm_placement), kind, int(unit_offset), float(eps),
+                                    float(residual_scale))
+
+
+def residual_norm(x, y, gate=None, post_weight=None, pre_weight=None, norm_placement=0, eps=1e-6, unit_offset=False,
+                  residual_scale=1.0):
+    """(h, n): h = x + residual_scale * gate * post(y) and n = pre(h) (None with norm_placement 1). norm_placement 0
+    norms before the next block (pre), 1 after this one (post), 2 both; gate [dim] float32 or like y."""
+    x, y, kind, shape = _norm_shape(x, y, gate, post_weight, pre_weight, norm_placement, eps, unit_offset,
+                                    residual_scale)
+    dx, dy, h, n = Device.of(x), Device.of(y), Device(x.nbytes), Device(x.nbytes)
+    (dg, gate_ptr), (dp, post_ptr), (dw, pre_ptr) = _upload(gate), _upload(post_weight, np.float32), \
+        _upload(pre_weight, np.float32)
+    check(lib.dllm_hip_residual_norm(shape, dx.ptr, dy.ptr, gate_ptr, post_ptr, pre_ptr, h.ptr, n.ptr, None))
+    return h.download(x.shape, x.dtype), n.download(x.shape, x.dtype) if norm_placement != 1 else None
+
+
+def residual_norm_backward(h, y, dh, dn=None, gate=None, post_weight=None, pre_weight=None, norm_placement=0, eps=1e-6,
+                           unit_offset=False, residual_scale=1.0):
+    """(dx, dy, dgate, dpost_weight, dpre_weight) of residual_norm from its h; None for what is not there."""
+    h, y, kind, shape = _norm_shape(h, y, gate, post_weight, pre_weight, norm_placement, eps, unit_offset,
+                                    residual_scale)
+    for d in (dh, dn):
+        if d is not None and (np.shape(d) != h.shape or np.asarray(d).dtype != h.dtype):
+            raise ValueError("dh and dn must have the shape and type of h")
+    if (dn is None) == (norm_placement != 1):
+        raise ValueError("dn belongs to the norm before the next block")
+    ins = [Device.of(h), Device.of(y)]
+    (dg, gate_ptr), (dp, post_ptr), (dw, pre_ptr) = _upload(gate), _upload(post_weight, np.float32), \
+        _upload(pre_weight, np.float32)
+    (d1, dh_ptr), (d2, dn_ptr) = _upload(dh), _upload(dn)
+    dx, dy = Device(h.nbytes), Device(h.nbytes)
+    dgate = None if gate is None else Device(np.asarray(gate).nbytes)
+    dpost = None if post_weight is None else Device(h.shape[-1] * 4)
+    dpre = None if pre_weight is None else Device(h.shape[-1] * 4)
+    ws = Device(lib.dllm_hip_residual_norm_backward_workspace(shape))
+    ptr = [None if d is None else d.ptr for d in (dgate, dpost, dpre)]
+    check(lib.dllm_hip_residual_norm_backward(shape, ins[0].ptr, ins[1].ptr, gate_ptr, post_ptr, pre_ptr, dh_ptr, dn_ptr,
+                                              dx.ptr, dy.ptr, *ptr, ws.ptr, ws.nbytes, None))
+    got = (dgate and dgate.download(np.shape(gate), np.asarray(gate).dtype), dpost and dpost.download((h.shape[-1],)),
+           dpre and dpre.download((h.shape[-1],)))
+    return dx.download(h.shape, h.dtype), dy.download(h.shape, h.dtype), *got

@@ -4,7 +4,8 @@
  *
  * Every result is bit-identical to the reference CPU kernels (cpp/include/dllm/{nn,grad,math}.hpp of EtAlii.Dllm)
  * on the same inputs, for any batch size, row count or CU count: each output keeps the reference's one double
- * accumulation in its fixed order.
+ * accumulation in its fixed order. The operators of packed layers (below) have no counterpart there and state
+ * their own contract.
  *
  * Conventions
  *  - Array arguments are DEVICE pointers (hipMalloc'd or equivalent), C-contiguous, float32 unless stated; sizes are
@@ -261,6 +262,96 @@ size_t dllm_hip_lora_adapter_gradients_workspace(size_t out_features, size_t in_
 int dllm_hip_lora_adapter_gradients(const float* grad, const float* a, const float* b, float* da, float* db,
                                     size_t out_features, size_t in_features, size_t rank, double scale,
                                     void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- operators of packed layers: documents in one batch, 16-bit activations ----
+ *
+ * The parts of a decoder layer around its matmuls for batches that the reference does not have: several documents packed
+ * into one row of tokens, images among the text, activations in bfloat16 or float16. They have no counterpart in the
+ * reference, so no bits to reproduce: sums, softmax statistics and norms are float32 (float32 activations: float32
+ * products too), and each result is rounded to its type once. They keep the library's other promise: results do not
+ * depend on what shares the batch. A document's attention, a token's rotation and a row's norm are the same bits
+ * alone and in any pack, and every call with the same arguments gives the same bits (no atomic additions). Sums over all rows
+ * (the gradients of norm weights and channel gates) depend on the rows alone.
+ *
+ * dtype is the type of the activations and of their gradients: 0 float32, 1 bfloat16, 2 float16. Parameters (norm
+ * weights, channel gates, ALiBi slopes) and their gradients are float32. Activations are aligned to their element; whole
+ * 16-byte chunks (aligned pointers, head_dim, strides and dim in multiples of 16 bytes) are faster.
+ * Calls are asynchronous, take no host memory after they return and allocate nothing, so they can be captured into a graph;
+ * two calls that may run at once need a workspace each. The device that the stream belongs to must be the current one. */
+enum { DLLM_HIP_FLOAT32 = 0, DLLM_HIP_BFLOAT16 = 1, DLLM_HIP_FLOAT16 = 2 };
+
+/* Attention within packed documents. q[tokens, heads, head_dim], k and v[tokens, kv_heads, head_dim], out like q;
+ * token strides in elements (0: heads * head_dim), so q, k and v may be parts of one projection's output. Document d is
+ * tokens offsets[d] .. offsets[d + 1] - 1 (device, documents + 1 values, non-decreasing, in [0, tokens]; empty documents
+ * are allowed). Tokens of no document are neither read nor written. A query at position i of its document sees the key
+ * at position j of the same document if
+ *     (j <= i or not causal) and (|i - j| < window or window is 0),   or   j < prefix[d]
+ * (prefix: device, one length per document, NULL for none: an instruction or image that every token sees). The score is
+ *     s = softcap tanh(scale q.k / softcap) - slopes[head] |i - j|
+ * (softcap 0: scale q.k; slopes: device, one per head, NULL for none; constants, they get no gradient). out = softmax(s) v and
+ * lse[heads, tokens] = log sum exp s, which the backward reads (float32; may be NULL). Keys that a query does not see do
+ * not reach its results, whatever they hold.
+ * Limits: head_dim at most 256, tokens below 2^31, heads a multiple of kv_heads, at most 65535 heads. Out-of-range
+ * offsets and prefixes are clamped to the tokens and the document; documents that then overlap give unspecified values.
+ * The backward takes the forward's out and lse and the upstream gradient dout (out's layout and stride) and writes dq, dk
+ * and dv (q's, k's and v's layouts and strides); dk and dv sum over the heads that share them, in head order. */
+typedef struct {
+    int64_t dtype;
+    int64_t tokens, documents, heads, kv_heads, head_dim;
+    int64_t causal, window;
+    double scale, softcap;
+    int64_t q_stride, k_stride, v_stride, out_stride;
+} dllm_hip_document_attention_shape;
+size_t dllm_hip_document_attention_workspace(const dllm_hip_document_attention_shape* shape);
+int dllm_hip_document_attention(const dllm_hip_document_attention_shape* shape, const void* q, const void* k,
+                                const void* v, const int64_t* offsets, const int64_t* prefix, const float* slopes,
+                                void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+size_t dllm_hip_document_attention_backward_workspace(const dllm_hip_document_attention_shape* shape);
+int dllm_hip_document_attention_backward(const dllm_hip_document_attention_shape* shape, const void* q, const void* k,
+                                         const void* v, const int64_t* offsets, const int64_t* prefix,
+                                         const float* slopes, const void* out, const float* lse, const void* dout,
+                                         void* dq, void* dk, void* dv, void* workspace, size_t workspace_bytes,
+                                         void* stream);
+
+/* Rotary positions of several axes (text: one; images and video: time, height and width), q and k in one call.
+ * positions[axes, tokens] (int64, device); pair p of a head is turned by positions[pair_axis[p]][t] * inv_freq[p]
+ * (pair_axis: uint8, inv_freq: double, both device, `pairs` entries; dllm_hip_rope_inv_freq gives the frequencies; a pair
+ * whose axis is not below `axes` is not turned). Angles are computed in double, so far positions lose nothing. Pair p is
+ * dimensions p and pairs + p, or 2p and 2p + 1 with interleaved; dimensions from 2 * pairs on are copied. inverse turns
+ * back: the gradient of q and k from those of the outputs. k may be NULL with k_heads 0. q_out may be q and k_out may
+ * be k with the same strides (in place); otherwise inputs and outputs do not overlap. Strides as above. At most 256 pairs,
+ * 65535 heads of each and 2^31 - 1 tokens. */
+typedef struct {
+    int64_t dtype;
+    int64_t tokens, q_heads, k_heads, head_dim, pairs, axes;
+    int64_t interleaved, inverse;
+    int64_t q_stride, k_stride, q_out_stride, k_out_stride;
+} dllm_hip_rope_axes_shape;
+int dllm_hip_rope_axes(const dllm_hip_rope_axes_shape* shape, const void* q, const void* k, const int64_t* positions,
+                       const double* inv_freq, const uint8_t* pair_axis, void* q_out, void* k_out, void* stream);
+
+/* The end of one block and the start of the next: h = x + residual_scale * gate * post(y) and n = pre(h), with the
+ * residual stream x[rows, dim], the block's output y[rows, dim] and RMSNorms post and pre (eps; weight, or 1 + weight with
+ * unit_offset). norm_placement 0: pre alone (post(y) = y), 1: post alone (no n), 2: both. gate 0: none, 1: one float32 per
+ * channel (gate[dim], a parameter), 2: one per element (gate[rows, dim] of dtype). The weight of a norm that is there
+ * may be NULL (all ones; with unit_offset too). n is the norm of h before it is rounded. h may be x.
+ * The backward takes h, y, gate and the gradients dh (of h, from its later uses; may be NULL: none) and dn (of n), and
+ * writes dx, dy, dgate (float32[dim] or like gate), dpost_weight and dpre_weight (float32[dim]); each output may be NULL.
+ * dx may be dh. rows below 2^31, dim at most 2^20. */
+typedef struct {
+    int64_t dtype;
+    int64_t rows, dim;
+    int64_t norm_placement, gate, unit_offset;
+    double eps, residual_scale;
+} dllm_hip_residual_norm_shape;
+int dllm_hip_residual_norm(const dllm_hip_residual_norm_shape* shape, const void* x, const void* y, const void* gate,
+                           const float* post_weight, const float* pre_weight, void* h, void* n, void* stream);
+size_t dllm_hip_residual_norm_backward_workspace(const dllm_hip_residual_norm_shape* shape);
+int dllm_hip_residual_norm_backward(const dllm_hip_residual_norm_shape* shape, const void* h, const void* y,
+                                    const void* gate, const float* post_weight, const float* pre_weight,
+                                    const void* dh, const void* dn, void* dx, void* dy, void* dgate,
+                                    float* dpost_weight, float* dpre_weight, void* workspace, size_t workspace_bytes,
+                                    void* stream);
 
 /* ---- the device-resident fine-tuning step ----
  *
