@@ -21,6 +21,7 @@ struct DocAttention {
     float scale, softcap;  // softcap 0: none
     // backward scratch
     float* delta;     // [heads][tokens]: dout . out
+    float* dout_norm; // [heads][tokens]: |dout| (float16)
     float* dk_part;   // [heads][tokens][head_dim] float32, before the heads of a group are added
     float* dv_part;
 };
@@ -43,15 +44,16 @@ __device__ __forceinline__ Document document_at(const DocAttention& a, int d) {
 }
 
 // The tile-th part of kRows tokens, counted through all documents; each document starts a part of its own, so that what
-// is computed for it does not depend on where it lies. Every lane of the wave returns the same. False past the last part.
-template <int kRows>
+// is computed for it does not depend on where it lies. kLast counts from the last document's last part. Every lane of the
+// wave returns the same. False past the last part.
+template <int kRows, bool kLast = false>
 __device__ __forceinline__ bool locate_tile(const DocAttention& a, int64_t tile, Document& doc, int& first) {
     const int lane = static_cast<int>(threadIdx.x) & 63;
     int64_t before = 0;
     for (int base = 0; base < a.documents; base += 64) {
-        const int d = base + lane;
+        const int d = kLast ? a.documents - 1 - base - lane : base + lane;
         Document mine{0, 0, 0};
-        if (d < a.documents) mine = document_at(a, d);
+        if (d >= 0 && d < a.documents) mine = document_at(a, d);
         const int parts = (mine.end - mine.start + kRows - 1) / kRows;
         int64_t through = parts;  // parts of the lanes up to this one
 #pragma unroll
@@ -66,9 +68,9 @@ __device__ __forceinline__ bool locate_tile(const DocAttention& a, int64_t tile,
             doc.start = __builtin_amdgcn_readlane(mine.start, owner);
             doc.end = __builtin_amdgcn_readlane(mine.end, owner);
             doc.prefix_end = __builtin_amdgcn_readlane(mine.prefix_end, owner);
-            const int64_t earlier = __shfl(before + through - parts, owner);
-            first = doc.start + static_cast<int>(tile - earlier) * kRows;
-            first = __builtin_amdgcn_readfirstlane(first);
+            int part = static_cast<int>(tile - __shfl(before + through - parts, owner));
+            if (kLast) part = __shfl(parts, owner) - 1 - part;
+            first = __builtin_amdgcn_readfirstlane(doc.start + part * kRows);
             return true;
         }
         before += all;
@@ -123,6 +125,14 @@ __device__ __forceinline__ float bend_score(const DocAttention& a, float slope, 
         x = a.softcap * t;
     }
     return x - slope * static_cast<float>(distance < 0 ? -distance : distance);
+}
+
+// tanh for the score cap. 16-bit types: 1 - 2 / (1 + e^2x), off by at most about 6 x 2^-24 absolutely, which the weights
+// (rounded to 2^-9 of themselves) do not see. float32: the library's, which is exact to its last bits near zero too.
+template <typename T>
+__device__ __forceinline__ float cap_tanh(float x) {
+    if constexpr (sizeof(T) == 4) return tanhf(x);
+    return fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * 2.8853900817779268f)), 1.0f);
 }
 
 template <typename T>

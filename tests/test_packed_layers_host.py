@@ -35,7 +35,8 @@ ATTENTION = dict(dtype=1, tokens=10, documents=1, heads=4, kv_heads=2, head_dim=
     (dict(documents=-1), "documents"), (dict(documents=1 << 31), "documents"), (dict(heads=3), "multiple of kv heads"),
     (dict(kv_heads=0), "multiple of kv heads"), (dict(heads=0), "multiple of kv heads"), (dict(heads=65536), "65535"),
     (dict(head_dim=0), "head_dim"), (dict(head_dim=257), "head_dim"), (dict(window=-1), "window"),
-    (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"), (dict(q_stride=255), "stride"),
+    (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("inf")), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(softcap=float("inf")), "softcap"), (dict(softcap=-1.0), "softcap"), (dict(softcap=float("nan")), "softcap"), (dict(q_stride=255), "stride"),
     (dict(k_stride=127), "stride"), (dict(v_stride=-128), "stride"), (dict(out_stride=1), "stride"),
     (dict(tokens=(1 << 31) - 1, documents=(1 << 31) - 1), "too many"),
 ])
