@@ -5,9 +5,16 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <initializer_list>
+
+#include "common.h"
 #include "element.h"
 
 namespace dllm_hip {
+
+constexpr int kDocThreads = 256;
+constexpr int kDocTileRows = 128;  // tokens of a workgroup, 32 for each wave
+constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DocAttention {
     const void *q, *k, *v, *out, *dout;  // out: written by the forward, read by the backward
@@ -276,5 +283,26 @@ __device__ __forceinline__ void store_row(To* to, const float (&v)[kLaneDims], i
     for (int c = 0; c < kLaneDims; ++c)
         if (lane + 64 * c < head_dim) to[lane + 64 * c] = static_cast<To>(v[c]);
 }
+
+// Parts of `rows` tokens of all documents, at most.
+inline unsigned doc_tiles(const DocAttention& a, int rows) {
+    return static_cast<unsigned>(ceil_div(a.tokens, rows) + (a.documents < a.tokens ? a.documents : a.tokens));
+}
+
+// Whole 16-byte chunks throughout: rows can be copied to LDS directly.
+template <typename T>
+bool whole_chunks(const DocAttention& a, std::initializer_list<const void*> arrays) {
+    bool whole = a.head_dim % kChunk<T> == 0;
+    for (const int64_t s : {a.q_stride, a.k_stride, a.v_stride, a.out_stride})
+        whole = whole && s % kChunk<T> == 0 && s < (int64_t{1} << 25);  // a copy's lane offsets stay below 2^32 bytes
+    for (const void* p : arrays) whole = whole && aligned_to(p, 16);
+    return whole;
+}
+
+// doc_attention_{f32,bf16,f16}.hip
+template <typename T>
+int launch_document_attention(const DocAttention& a, void* out, hipStream_t stream);
+template <typename T>
+int launch_document_attention_backward(const DocAttention& a, hipStream_t stream);
 
 }  // namespace dllm_hip

@@ -1,0 +1,453 @@
+// Attention within packed documents: the gradients (doc_attention.h: the mask and the score).
+//
+//   p_ij = exp(s_ij - lse_i),  dP = dout v^T,  dS = p (dP - dout . out) cap' scale,
+//   dq = dS k,  dk = dS^T q,  dv = p^T dout
+//
+// Two kernels, each computing scores and dP for itself, so that every gradient is summed by one wave in one order: dq for 128
+// queries of a head over their keys, then dk and dv for 128 keys over the queries of one head that see them. That is
+// seven products instead of five; sums of dq across workgroups by atomic additions would save two and give other bits every time.
+// Heads that share keys leave their dk and dv in float32 and a third kernel adds them in head order.
+#pragma once
+
+#include <float.h>
+
+#include "common.h"
+#include "doc_attention.h"
+#include "doc_tile.h"
+
+namespace dllm_hip {
+
+template <typename T, int kDim>
+constexpr int kStream = kDim * sizeof(T) <= 256 ? 64 : 32;  // rows of a tile that goes through LDS
+
+constexpr int kTogether = 128;
+
+// float16 loses weights below 2^-14 bit by bit, and upstream gradients have any size: p is held times 2^8, and dout relative
+// to a power of two near its norm (the query's own for dq, the largest of the queries that are summed for dk), so dS is
+// at most 2^8 |v|. Other types need none of it.
+template <typename T>
+constexpr float kWeightShift = sizeof(T) == 2 && __is_same(T, _Float16) ? 8.0f : 0.0f;
+
+// The power of two at or above x; 1 for zero, infinities and NaN.
+__device__ __forceinline__ float power_of_two_above(float x) {
+    if (!(x > 0.0f && x < FLT_MAX)) return 1.0f;
+    int e;
+    frexpf(x, &e);
+    return ldexpf(1.0f, e > 126 ? 126 : e < -126 ? -126 : e);
+}
+
+// What a score needs beside X: see the forward kernel.
+template <typename T>
+struct Bend {
+    float unit, cap_in, slope;
+    bool capped, biased;
+    __device__ Bend(const DocAttention& a, int head) {
+        capped = a.softcap != 0.0f;
+        biased = a.slopes != nullptr;
+        unit = (capped ? a.softcap : a.scale) * kLog2E;
+        cap_in = capped ? a.scale / a.softcap : 0.0f;
+        slope = biased ? a.slopes[head] * kLog2E : 0.0f;
+    }
+};
+
+// ---- dq ----
+template <typename T, int kDim, bool kDirect>
+__global__ __launch_bounds__(kDocThreads, kDim <= 128 ? 2 : 1) void dq_kernel(DocAttention a) {
+    using Shape = TileShape<T, kDim>;
+    constexpr int kTile = kStream<T, kDim>;
+    constexpr int kTileBytes = kTile * Shape::kRowBytes;
+    constexpr int kParts = kDim / 32;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];
+
+    const int turn = static_cast<int>(blockIdx.x) % a.heads;
+    const int head = (turn % a.kv_heads) * a.group + turn / a.kv_heads;
+    const int kv = head / a.group;
+    Document doc;
+    int first;
+    if (!locate_tile<kDocTileRows, true>(a, blockIdx.x / a.heads, doc, first)) return;
+
+    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
+    const int wave_first = first + 32 * wave, wave_last = min(wave_first + 31, doc.end - 1);
+    const bool working = wave_first < doc.end;
+    const bool mine = wave_first + (lane & 31) < doc.end;
+    const int i = min(wave_first + (lane & 31), doc.end - 1);
+    const Span span = key_span(a, doc, i);
+    const int64_t head_at = static_cast<int64_t>(head) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens + i;
+
+    const Column<T, kDim, kDirect> q(static_cast<const T*>(a.q) + i * a.q_stride + head_at, a.head_dim);
+    const Column<T, kDim, kDirect> dout(static_cast<const T*>(a.dout) + i * a.out_stride + head_at, a.head_dim);
+    float delta = 0.0f, norm = 0.0f;
+    {
+        const Column<T, kDim, kDirect> out(static_cast<const T*>(a.out) + i * a.out_stride + head_at, a.head_dim);
+#pragma unroll
+        for (int s = 0; s < Shape::kSteps; ++s) {
+            const Chunk<T> o = out[s], d = dout[s];
+#pragma unroll
+            for (int j = 0; j < kChunk<T>; ++j) {
+                delta = fmaf(static_cast<float>(o[j]), static_cast<float>(d[j]), delta);
+                norm = fmaf(static_cast<float>(d[j]), static_cast<float>(d[j]), norm);
+            }
+        }
+    }
+    delta += other_half(delta);
+    float dout_scale = 1.0f;
+    if constexpr (kWeightShift<T> != 0.0f) {
+        norm = sqrtf(norm + other_half(norm));
+        dout_scale = power_of_two_above(norm);
+        if (mine && half == 0) a.dout_norm[stat_at] = norm;
+    }
+    if (mine && half == 0) a.delta[stat_at] = delta;
+    const float into = 1.0f / dout_scale;  // exact
+
+    const int low = key_span(a, doc, first).low;
+    const int high = max(key_span(a, doc, min(first + kDocTileRows, doc.end) - 1).high, doc.prefix_end);
+    const int low_tile = (low - doc.start) / kTile, prefix_tiles = (doc.prefix_end - doc.start + kTile - 1) / kTile;
+    const int tiles = (high - doc.start + kTile - 1) / kTile;
+    const Span first_span = key_span(a, doc, wave_first), last_span = key_span(a, doc, wave_last);
+    const int any_low = first_span.low, any_high = last_span.high, all_low = last_span.low, all_high = first_span.high;
+
+    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_k(a.k, a.k_stride, kv, a.head_dim);
+    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_v(a.v, a.v_stride, kv, a.head_dim);
+    const TileView<T, kDim> view;
+    LdsByte* const buffers = (LdsByte*)lds;
+    const Bend<T> bend(a, head);
+    const float base = a.lse[stat_at] * kLog2E - kWeightShift<T>;
+
+    Acc dq[kParts];
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dq[p][r] = 0.0f;
+
+    auto next_tile = [&](int t) { return t + 1 < prefix_tiles ? t + 1 : max(t + 1, low_tile); };
+    auto fetch = [&](int t, int buffer) {
+        const int from = doc.start + t * kTile;
+        copy_k(from, doc.end - from, buffers + buffer * 2 * kTileBytes);
+        copy_v(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
+    };
+    int t = next_tile(-1);
+    fetch(t, 0);
+    for (int buffer = 0; t < tiles; buffer ^= 1) {
+        tile_barrier();
+        const int next = next_tile(t);
+        if (next < tiles) fetch(next, buffer ^ 1);
+        const LdsByte* const k_tile = buffers + buffer * 2 * kTileBytes;
+        const LdsByte* const v_tile = k_tile + kTileBytes;
+        const int from = doc.start + t * kTile;
+        t = next;
+        if (!working || !((from < any_high && from + kTile > any_low) || from < doc.prefix_end)) continue;
+        const bool all_seen = (from >= all_low && from + kTile <= all_high) || from + kTile <= doc.prefix_end;
+#pragma unroll
+        for (int b = 0; b < kTile / 32; ++b) {
+            Acc x, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
+#pragma unroll
+            for (int step = 0; step < Shape::kSteps; ++step) multiply(view.rows(k_tile, b, step), q[step], x);
+#pragma unroll
+            for (int step = 0; step < Shape::kSteps; ++step) multiply(view.rows(v_tile, b, step), dout[step], dp);
+            float ds[16];
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] = fmaf(dp[r], into, -delta * into);
+            if (bend.capped) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    x[r] = cap_tanh<T>(x[r] * bend.cap_in);
+                    ds[r] *= fmaf(-x[r], x[r], 1.0f);
+                }
+            }
+            if (bend.biased) {
+                const float away = static_cast<float>(i - from - 32 * b - 4 * half);
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    x[r] = fmaf(-bend.slope, fabsf(away - static_cast<float>(8 * (r / 4) + r % 4)), fmaf(x[r], bend.unit, -base));
+            } else {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], bend.unit, -base);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) ds[r] *= __builtin_amdgcn_exp2f(x[r]);
+            if (!all_seen) {
+                const int to_low = span.low - from - 32 * b - 4 * half;
+                const unsigned width = static_cast<unsigned>(span.high - span.low);
+                const int to_prefix = doc.prefix_end - from - 32 * b - 4 * half;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = 8 * (r / 4) + r % 4;
+                    const bool see = static_cast<unsigned>(j - to_low) < width || j < to_prefix;
+                    ds[r] = see ? ds[r] : 0.0f;
+                }
+            }
+            multiply_columns<T, kDim>(view, k_tile, b, ds, dq);
+        }
+    }
+    if (!working) return;
+    bool spoilt = !all_finite(dq);
+    spoilt = (spoilt | __shfl_xor(static_cast<int>(spoilt), 32)) && mine;
+    T* const to = static_cast<T*>(a.dq) + head_at;
+    if (!spoilt && mine)
+        store_column<kDirect>(to + i * a.q_stride, a.head_dim, dq, a.scale * dout_scale * __builtin_amdgcn_exp2f(-kWeightShift<T>));
+    for (uint32_t left = static_cast<uint32_t>(__ballot(spoilt)); left; left &= left - 1) {
+        const int from_lane = __ffs(left) - 1, row = wave_first + from_lane;
+        float value[kLaneDims];
+        attention_row_dq<T>(a, doc, head, row, __shfl(delta, from_lane), value);
+        store_row(to + row * a.q_stride, value, a.head_dim);
+    }
+}
+
+// ---- dk and dv of one head ----
+//
+// kShared: into the float32 parts of heads that share keys. kDk, kDv: which of the two; rows of more than kTogether
+// elements take a launch for each, since the sums of both and a lane's two rows are more than its registers (five products
+// in all instead of four).
+template <typename T, int kDim, bool kDirect, bool kShared, bool kDk, bool kDv>
+__global__ __launch_bounds__(kDocThreads, kDim <= 64 ? 2 : 1) void dkv_kernel(DocAttention a) {
+    using Shape = TileShape<T, kDim>;
+    constexpr int kTile = kStream<T, kDim>;
+    constexpr int kTileBytes = kTile * Shape::kRowBytes;
+    constexpr int kParts = kDim / 32;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];
+    __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // lse in units of log 2, and dout . out, of a tile's queries
+    __shared__ float largest[kDocThreads / 64];
+
+    const int turn = static_cast<int>(blockIdx.x) % a.heads;
+    const int head = (turn % a.kv_heads) * a.group + turn / a.kv_heads;
+    const int kv = head / a.group;
+    Document doc;
+    int first;
+    if (!locate_tile<kDocTileRows>(a, blockIdx.x / a.heads, doc, first)) return;
+
+    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
+    const int wave_first = first + 32 * wave, wave_last = min(wave_first + 31, doc.end - 1);
+    const bool working = wave_first < doc.end;
+    const bool mine = wave_first + (lane & 31) < doc.end;
+    const int j = min(wave_first + (lane & 31), doc.end - 1);
+    const Span span = query_span(a, doc, j);
+    const int64_t kv_at = static_cast<int64_t>(kv) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens;
+
+    const Column<T, kDim, kDirect> k(static_cast<const T*>(a.k) + j * a.k_stride + kv_at, a.head_dim);
+    const Column<T, kDim, kDirect> v(static_cast<const T*>(a.v) + j * a.v_stride + kv_at, a.head_dim);
+
+    // the queries that see any key of the workgroup; keys in the prefix are seen from the document's start on
+    const int last = min(first + kDocTileRows, doc.end) - 1;
+    const int low = query_span(a, doc, first).low;
+    const int high = max(query_span(a, doc, first).high, query_span(a, doc, last).high);
+    const int low_tile = (low - doc.start) / kTile, tiles = (high - doc.start + kTile - 1) / kTile;
+    // the wave's: those that see any of its keys, and all
+    const Span first_span = query_span(a, doc, min(wave_first, doc.end - 1)), last_span = query_span(a, doc, wave_last);
+    const int any_low = first_span.low, any_high = max(first_span.high, last_span.high);
+    // (a wave with keys on both sides of the prefix's end: the first key after it has the earliest end)
+    const int edge = wave_first < doc.prefix_end && wave_last >= doc.prefix_end ? doc.prefix_end : wave_first;
+    const int all_low = last_span.low, all_high = query_span(a, doc, min(edge, doc.end - 1)).high;
+
+    float dout_scale = 1.0f;
+    if constexpr (kWeightShift<T> != 0.0f && kDk) {
+        float top = 0.0f;
+        for (int i = low + static_cast<int>(threadIdx.x); i < high; i += kDocThreads) {
+            const float n = a.dout_norm[stat_at + i];
+            top = n < FLT_MAX ? fmaxf(top, n) : top;
+        }
+        top = wave_max(top);
+        if (lane == 0) largest[wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < kDocThreads / 64; ++w) top = fmaxf(top, largest[w]);
+        dout_scale = power_of_two_above(top);
+    }
+    const float into = 1.0f / dout_scale;
+
+    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_q(a.q, a.q_stride, head, a.head_dim);
+    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_d(a.dout, a.out_stride, head, a.head_dim);
+    const TileView<T, kDim> view;
+    LdsByte* const buffers = (LdsByte*)lds;
+    const Bend<T> bend(a, head);
+
+    Acc dk[kDk ? kParts : 1], dv[kDv ? kParts : 1];
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+#pragma unroll
+        for (int p = 0; p < (kDk ? kParts : 1); ++p) dk[p][r] = 0.0f;
+#pragma unroll
+        for (int p = 0; p < (kDv ? kParts : 1); ++p) dv[p][r] = 0.0f;
+    }
+
+    // a tile's statistics, one value for each of the first 2 kTile threads
+    auto read_stat = [&](int t) {
+        const int which = static_cast<int>(threadIdx.x) / kTile, at = min(doc.start + t * kTile + static_cast<int>(threadIdx.x) % kTile, doc.end - 1);
+        return which == 0 ? a.lse[stat_at + at] * kLog2E - kWeightShift<T> : which == 1 ? a.delta[stat_at + at] * into : 0.0f;
+    };
+    auto write_stat = [&](int buffer, float value) {
+        if (static_cast<int>(threadIdx.x) < 2 * kTile) (&stats[buffer][0][0])[threadIdx.x] = value;
+    };
+    auto fetch = [&](int t, int buffer) {
+        const int from = doc.start + t * kTile;
+        copy_q(from, doc.end - from, buffers + buffer * 2 * kTileBytes);
+        copy_d(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
+    };
+    int t = low_tile;
+    write_stat(0, read_stat(t));
+    fetch(t, 0);
+    for (int buffer = 0; t < tiles; buffer ^= 1, ++t) {
+        tile_barrier();
+        if (t + 1 < tiles) {
+            write_stat(buffer ^ 1, read_stat(t + 1));
+            fetch(t + 1, buffer ^ 1);
+        }
+        const LdsByte* const q_tile = buffers + buffer * 2 * kTileBytes;
+        const LdsByte* const d_tile = q_tile + kTileBytes;
+        const int from = doc.start + t * kTile;
+        if (!working || !(from < any_high && from + kTile > any_low)) continue;
+        const bool all_seen = from >= all_low && from + kTile <= all_high;
+#pragma unroll
+        for (int b = 0; b < kTile / 32; ++b) {
+            Acc x, dp;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
+#pragma unroll
+            for (int step = 0; step < Shape::kSteps; ++step) multiply(view.rows(q_tile, b, step), k[step], x);
+            if constexpr (kDk)
+#pragma unroll
+                for (int step = 0; step < Shape::kSteps; ++step) multiply(view.rows(d_tile, b, step), v[step], dp);
+            float p[16], ds[16];
+            using Four = float __attribute__((ext_vector_type(4)));
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const Four base = *reinterpret_cast<const Four*>(&stats[buffer][0][32 * b + 8 * g + 4 * half]);
+                const Four delta = *reinterpret_cast<const Four*>(&stats[buffer][1][32 * b + 8 * g + 4 * half]);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    p[4 * g + r] = base[r];
+                    ds[4 * g + r] = fmaf(dp[4 * g + r], into, -delta[r]);
+                }
+            }
+            if (bend.capped) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    x[r] = cap_tanh<T>(x[r] * bend.cap_in);
+                    ds[r] *= fmaf(-x[r], x[r], 1.0f);
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) p[r] = fmaf(x[r], bend.unit, -p[r]);
+            if (bend.biased) {
+                const float away = static_cast<float>(from + 32 * b + 4 * half - j);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) p[r] = fmaf(-bend.slope, fabsf(away + static_cast<float>(8 * (r / 4) + r % 4)), p[r]);
+            }
+            if (!all_seen) {
+                const int to_low = span.low - from - 32 * b - 4 * half;
+                const unsigned width = static_cast<unsigned>(span.high - span.low);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const bool see = static_cast<unsigned>(8 * (r / 4) + r % 4 - to_low) < width;
+                    p[r] = see ? p[r] : -INFINITY;
+                    ds[r] = see ? ds[r] : 0.0f;
+                }
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                p[r] = __builtin_amdgcn_exp2f(p[r]);
+                ds[r] *= p[r];
+            }
+            if constexpr (kDv) multiply_columns<T, kDim>(view, d_tile, b, p, dv);
+            if constexpr (kDk) multiply_columns<T, kDim>(view, q_tile, b, ds, dk);
+        }
+    }
+    if (!working) return;
+    const float unshift = __builtin_amdgcn_exp2f(-kWeightShift<T>), dk_factor = a.scale * dout_scale * unshift;
+    bool spoilt = !(all_finite(dk) && all_finite(dv));
+    spoilt = (spoilt | __shfl_xor(static_cast<int>(spoilt), 32)) && mine;
+    // row `at` of dk and dv, by `store` of its place and its factor
+    auto rows_of = [&](int64_t at, auto&& store) {
+        const int64_t part = (stat_at + at) * a.head_dim;
+        if constexpr (kShared)
+            store(a.dk_part + part, a.dv_part + part);
+        else
+            store(static_cast<T*>(a.dk) + at * a.k_stride + kv_at, static_cast<T*>(a.dv) + at * a.v_stride + kv_at);
+    };
+    if (!spoilt && mine)
+        rows_of(j, [&](auto* to_dk, auto* to_dv) {
+            if constexpr (kDk) store_column<kDirect>(to_dk, a.head_dim, dk, dk_factor);
+            if constexpr (kDv) store_column<kDirect>(to_dv, a.head_dim, dv, unshift);
+        });
+    for (uint32_t left = static_cast<uint32_t>(__ballot(spoilt)); left; left &= left - 1) {
+        const int row = wave_first + __ffs(left) - 1;
+        float dk1[kLaneDims], dv1[kLaneDims];
+        attention_row_dkv<T>(a, doc, head, row, dk1, dv1);
+        rows_of(row, [&](auto* to_dk, auto* to_dv) {
+            if constexpr (kDk) store_row(to_dk, dk1, a.head_dim);
+            if constexpr (kDv) store_row(to_dv, dv1, a.head_dim);
+        });
+    }
+}
+
+// dk and dv of the tokens of documents: the group's heads added in order. kWidth elements to a thread.
+template <typename T, int kWidth>
+__global__ __launch_bounds__(kDocThreads) void add_heads_kernel(DocAttention a) {
+    const int per_row = (a.head_dim + kWidth - 1) / kWidth, per_token = a.kv_heads * per_row;
+    Document doc;
+    int first;
+    if (!locate_tile<kDocTileRows>(a, blockIdx.x, doc, first)) return;
+    const int rows = min(kDocTileRows, doc.end - first);
+    for (int64_t e = static_cast<int64_t>(blockIdx.y) * kDocThreads + threadIdx.x; e < static_cast<int64_t>(rows) * per_token;
+         e += static_cast<int64_t>(gridDim.y) * kDocThreads) {
+        const int row = static_cast<int>(e / per_token), in_token = static_cast<int>(e % per_token);
+        const int kv = in_token / per_row, d = in_token % per_row * kWidth;
+        const int64_t j = first + row;
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            const float* part = (which ? a.dv_part : a.dk_part) + (static_cast<int64_t>(kv) * a.group * a.tokens + j) * a.head_dim + d;
+            float sum[kWidth];
+            load_as_float<float, kWidth>(part, sum);
+            for (int g = 1; g < a.group; ++g) {
+                float more[kWidth];
+                load_as_float<float, kWidth>(part + static_cast<int64_t>(g) * a.tokens * a.head_dim, more);
+#pragma unroll
+                for (int c = 0; c < kWidth; ++c) sum[c] += more[c];
+            }
+            T* to = which ? static_cast<T*>(a.dv) + j * a.v_stride : static_cast<T*>(a.dk) + j * a.k_stride;
+            store_from_float<T, kWidth>(to + static_cast<int64_t>(kv) * a.head_dim + d, sum);
+        }
+    }
+}
+
+template <typename T, int kDim, bool kDirect, bool kDk, bool kDv>
+void launch_dkv(const DocAttention& a, dim3 grid, hipStream_t s) {
+    if (a.group == 1)
+        dkv_kernel<T, kDim, kDirect, false, kDk, kDv><<<grid, kDocThreads, 0, s>>>(a);
+    else
+        dkv_kernel<T, kDim, kDirect, true, kDk, kDv><<<grid, kDocThreads, 0, s>>>(a);
+}
+
+template <typename T, int kDim, bool kDirect>
+void launch_kernels(const DocAttention& a, hipStream_t s) {
+    const dim3 grid(doc_tiles(a, kDocTileRows) * a.heads);
+    dq_kernel<T, kDim, kDirect><<<grid, kDocThreads, 0, s>>>(a);
+    if constexpr (kDim <= kTogether) {
+        launch_dkv<T, kDim, kDirect, true, true>(a, grid, s);
+    } else {
+        launch_dkv<T, kDim, kDirect, true, false>(a, grid, s);
+        launch_dkv<T, kDim, kDirect, false, true>(a, grid, s);
+    }
+}
+
+template <typename T>
+int launch_document_attention_backward(const DocAttention& a, hipStream_t s) {
+    const bool direct = whole_chunks<T>(a, {a.q, a.k, a.v, a.out, a.dout, a.dq, a.dk, a.dv});
+    if (a.head_dim <= 64)
+        direct ? launch_kernels<T, 64, true>(a, s) : launch_kernels<T, 64, false>(a, s);
+    else if (a.head_dim <= 128)
+        direct ? launch_kernels<T, 128, true>(a, s) : launch_kernels<T, 128, false>(a, s);
+    else
+        direct ? launch_kernels<T, 256, true>(a, s) : launch_kernels<T, 256, false>(a, s);
+    if (a.group > 1) {
+        const dim3 grid(doc_tiles(a, kDocTileRows), 8);
+        if (direct)
+            add_heads_kernel<T, 4><<<grid, kDocThreads, 0, s>>>(a);
+        else
+            add_heads_kernel<T, 1><<<grid, kDocThreads, 0, s>>>(a);
+    }
+    return check_launch("document_attention_backward");
+}
+
+}  // namespace dllm_hip

@@ -1,0 +1,10 @@
+// Attention within packed documents in bfloat16.
+#include "doc_attention_backward.h"
+#include "doc_attention_forward.h"
+
+namespace dllm_hip {
+
+template int launch_document_attention<__bf16>(const DocAttention&, void*, hipStream_t);
+template int launch_document_attention_backward<__bf16>(const DocAttention&, hipStream_t);
+
+}  // namespace dllm_hip

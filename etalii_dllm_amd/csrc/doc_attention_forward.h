@@ -1,0 +1,203 @@
+// Attention within packed documents: the forward kernel (doc_attention.h: the mask and the score).
+//
+//   out_i = sum_j p_ij v_j,  p_ij = exp(s_ij - lse_i),  lse_i = log sum_j exp s_ij
+#pragma once
+
+#include "common.h"
+#include "doc_attention.h"
+#include "doc_tile.h"
+
+namespace dllm_hip {
+
+template <typename T, int kDim>
+constexpr int kKeys = kDim * sizeof(T) <= 256 ? 64 : 32;  // keys of a tile: K and V twice in at most 64 KB of LDS, or 128 KB
+
+// Forward. A wave's lane owns one query (two lanes: its halves); keys go through LDS in tiles, two buffers deep.
+//
+//   X = K Q^T (32 keys x 32 queries at a time)     s = X scale, capped, biased, in units of log 2
+//   m = running maximum, P = 2^(s - m), l = sum P   O^T += V^T P
+//
+// The running maximum is moved only when some query of the wave has outgrown it by 2^8: until then P stays below 2^8, which
+// float32 sums and 16-bit products hold as well as values below one.
+template <typename T, int kDim, bool kDirect>
+__global__ __launch_bounds__(kDocThreads, 2) void forward_kernel(DocAttention a, T* out) {
+    using Shape = TileShape<T, kDim>;
+    constexpr int kTile = kKeys<T, kDim>;
+    constexpr int kTileBytes = kTile * Shape::kRowBytes;
+    constexpr int kParts = kDim / 32;
+    __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];  // K, V of one buffer, K, V of the other
+
+    // the heads that share keys are 8 workgroups (or a divisor of it) apart: on the same L2
+    const int turn = static_cast<int>(blockIdx.x) % a.heads;
+    const int head = (turn % a.kv_heads) * a.group + turn / a.kv_heads;
+    const int kv = head / a.group;
+    Document doc;
+    int first;
+    if (!locate_tile<kDocTileRows, true>(a, blockIdx.x / a.heads, doc, first)) return;
+
+    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
+    const int wave_first = first + 32 * wave, wave_last = min(wave_first + 31, doc.end - 1);
+    const bool working = wave_first < doc.end;
+    const int i = min(wave_first + (lane & 31), doc.end - 1);
+    const Span span = key_span(a, doc, i);
+
+    const Column<T, kDim, kDirect> q(static_cast<const T*>(a.q) + i * a.q_stride + static_cast<int64_t>(head) * a.head_dim,
+                                     a.head_dim);
+
+    // keys of the workgroup: [low, high) in whole tiles of the document, and the tiles of the prefix before them
+    const int low = key_span(a, doc, first).low;
+    const int high = max(key_span(a, doc, min(first + kDocTileRows, doc.end) - 1).high, doc.prefix_end);
+    const int low_tile = (low - doc.start) / kTile, prefix_tiles = (doc.prefix_end - doc.start + kTile - 1) / kTile;
+    const int tiles = (high - doc.start + kTile - 1) / kTile;
+    // the wave's: keys that all its queries see, and that any sees
+    const Span first_span = key_span(a, doc, wave_first), last_span = key_span(a, doc, wave_last);
+    const int any_low = first_span.low, any_high = last_span.high, all_low = last_span.low, all_high = first_span.high;
+
+    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_k(a.k, a.k_stride, kv, a.head_dim);
+    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_v(a.v, a.v_stride, kv, a.head_dim);
+    const TileView<T, kDim> view;
+    LdsByte* const buffers = (LdsByte*)lds;
+
+    const float unit = (a.softcap != 0.0f ? a.softcap : a.scale) * kLog2E;  // score of X (or of the tanh) in units of log 2
+    const float cap_in = a.softcap != 0.0f ? a.scale / a.softcap : 0.0f;
+    const float slope = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
+
+    Acc o[kParts];
+#pragma unroll
+    for (int p = 0; p < kParts; ++p)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[p][r] = 0.0f;
+    float m = -INFINITY, l = 0.0f;
+
+    auto next_tile = [&](int t) { return t + 1 < prefix_tiles ? t + 1 : max(t + 1, low_tile); };
+    auto fetch = [&](int t, int buffer) {
+        const int from = doc.start + t * kTile;
+        copy_k(from, doc.end - from, buffers + buffer * 2 * kTileBytes);
+        copy_v(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
+    };
+    int t = next_tile(-1);
+    fetch(t, 0);
+    for (int buffer = 0; t < tiles; buffer ^= 1) {
+        tile_barrier();
+        const int next = next_tile(t);
+        if (next < tiles) fetch(next, buffer ^ 1);
+        const LdsByte* const k_tile = buffers + buffer * 2 * kTileBytes;
+        const LdsByte* const v_tile = k_tile + kTileBytes;
+        const int from = doc.start + t * kTile;
+        t = next;
+        const bool in_prefix = from < doc.prefix_end;
+        if (!working || !((from < any_high && from + kTile > any_low) || in_prefix)) continue;
+        const bool all_seen = (from >= all_low && from + kTile <= all_high) || from + kTile <= doc.prefix_end;
+
+        float s[kTile / 32][16];
+#pragma unroll
+        for (int b = 0; b < kTile / 32; ++b) {
+            Acc x;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = 0.0f;
+#pragma unroll
+            for (int step = 0; step < Shape::kSteps; ++step) multiply(view.rows(k_tile, b, step), q[step], x);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = x[r];
+        }
+        float times = unit;
+        if (a.softcap != 0.0f) {
+#pragma unroll
+            for (int b = 0; b < kTile / 32; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[b][r] = cap_tanh<T>(s[b][r] * cap_in);
+        }
+        if (a.slopes) {
+            const float away = static_cast<float>(i - from - 4 * half);
+#pragma unroll
+            for (int b = 0; b < kTile / 32; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    s[b][r] = fmaf(-slope, fabsf(away - static_cast<float>(32 * b + 8 * (r / 4) + r % 4)), s[b][r] * unit);
+            times = 1.0f;
+        }
+        if (!all_seen) {
+            const int to_low = span.low - from - 4 * half;
+            const unsigned width = static_cast<unsigned>(span.high - span.low);
+            const int to_prefix = doc.prefix_end - from - 4 * half;
+#pragma unroll
+            for (int b = 0; b < kTile / 32; ++b)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int j = 32 * b + 8 * (r / 4) + r % 4;
+                    const bool see = static_cast<unsigned>(j - to_low) < width || j < to_prefix;
+                    s[b][r] = see ? s[b][r] : -INFINITY;
+                }
+        }
+        float top = s[0][0];
+#pragma unroll
+        for (int b = 0; b < kTile / 32; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
+        top = fmaxf(top, other_half(top)) * times;
+        if (__any(top > m + 8.0f)) {
+            const float moved = fmaxf(m, top);
+            const float keep = __builtin_amdgcn_exp2f(m - (moved == -INFINITY ? 0.0f : moved));
+            m = moved;
+            l *= keep;
+#pragma unroll
+            for (int p = 0; p < kParts; ++p)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) o[p][r] *= keep;
+        }
+        const float base = m == -INFINITY ? 0.0f : m;
+        float sum = 0.0f;
+#pragma unroll
+        for (int b = 0; b < kTile / 32; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = __builtin_amdgcn_exp2f(fmaf(s[b][r], times, -base));
+                sum += s[b][r];
+            }
+        l += sum;
+#pragma unroll
+        for (int b = 0; b < kTile / 32; ++b) multiply_columns<T, kDim>(view, v_tile, b, s[b], o);
+    }
+    if (!working) return;
+    l += other_half(l);
+
+    // A hidden key counts as zero times its value: where that is infinite or NaN, the row is computed again from the keys
+    // that it sees alone.
+    bool spoilt = !(all_finite(o) && l * 0.0f == 0.0f && m * 0.0f == 0.0f);
+    spoilt = (spoilt | __shfl_xor(static_cast<int>(spoilt), 32)) && wave_first + (lane & 31) < doc.end;
+    if (!spoilt && wave_first + (lane & 31) < doc.end) {
+        store_column<kDirect>(out + i * a.out_stride + static_cast<int64_t>(head) * a.head_dim, a.head_dim, o, 1.0f / l);
+        if (a.lse && half == 0) a.lse[static_cast<int64_t>(head) * a.tokens + i] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+    }
+    for (uint32_t left = static_cast<uint32_t>(__ballot(spoilt)); left; left &= left - 1) {
+        const int row = wave_first + __ffs(left) - 1;
+        float value[kLaneDims], lse;
+        attention_row<T>(a, doc, head, row, value, lse);
+        store_row(out + row * a.out_stride + static_cast<int64_t>(head) * a.head_dim, value, a.head_dim);
+        if (a.lse && lane == 0) a.lse[static_cast<int64_t>(head) * a.tokens + row] = lse;
+    }
+}
+
+template <typename T, int kDim>
+void launch_forward_dim(const DocAttention& a, T* out, bool direct, hipStream_t s) {
+    const dim3 grid(doc_tiles(a, kDocTileRows) * a.heads);
+    if (direct)
+        forward_kernel<T, kDim, true><<<grid, kDocThreads, 0, s>>>(a, out);
+    else
+        forward_kernel<T, kDim, false><<<grid, kDocThreads, 0, s>>>(a, out);
+}
+
+template <typename T>
+int launch_document_attention(const DocAttention& a, void* out, hipStream_t s) {
+    const bool direct = whole_chunks<T>(a, {a.q, a.k, a.v, out});
+    T* const to = static_cast<T*>(out);
+    if (a.head_dim <= 64)
+        launch_forward_dim<T, 64>(a, to, direct, s);
+    else if (a.head_dim <= 128)
+        launch_forward_dim<T, 128>(a, to, direct, s);
+    else
+        launch_forward_dim<T, 256>(a, to, direct, s);
+    return check_launch("document_attention");
+}
+
+}  // namespace dllm_hip

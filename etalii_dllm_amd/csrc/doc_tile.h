@@ -212,28 +212,45 @@ __device__ __forceinline__ void multiply_columns(const TileView<T, kDim>& view, 
     }
 }
 
-// A lane's own row (of B): chunk pair `step`'s chunk of its half, zero past head_dim.
+// A lane's own row, the B operand of products along head_dim: chunk pair `step`'s chunk of its half, zero past head_dim. Held
+// in registers, or read again at each use where it would take more than 64 of them (a step's four float32 products take 256
+// cycles, and the row stays in the caches).
 template <typename T, int kDim, bool kDirect>
-__device__ __forceinline__ void load_column(const T* row, int head_dim, Chunk<T> (&out)[TileShape<T, kDim>::kSteps]) {
-    const int half = (static_cast<int>(threadIdx.x) >> 5) & 1;
-#pragma unroll
-    for (int s = 0; s < TileShape<T, kDim>::kSteps; ++s) {
-        const int d = (2 * s + half) * kChunk<T>;
+struct Column {
+    static constexpr int kSteps = TileShape<T, kDim>::kSteps;
+    static constexpr bool kHeld = sizeof(T) == 2 || kSteps <= 8;
+    const T* row;
+    int head_dim;
+    Chunk<T> held[kHeld ? kSteps : 1];
+
+    __device__ __forceinline__ Chunk<T> read(int step) const {
+        const int d = (2 * step + ((static_cast<int>(threadIdx.x) >> 5) & 1)) * kChunk<T>;
+        Chunk<T> c{};
         if constexpr (kDirect) {
-            const Chunk<T> zero{};
-            out[s] = d < head_dim ? *reinterpret_cast<const Chunk<T>*>(row + d) : zero;
+            if (d < head_dim) c = *reinterpret_cast<const Chunk<T>*>(row + d);
         } else {
 #pragma unroll
-            for (int j = 0; j < kChunk<T>; ++j) out[s][j] = d + j < head_dim ? row[d + j] : static_cast<T>(0.0f);
+            for (int j = 0; j < kChunk<T>; ++j)
+                if (d + j < head_dim) c[j] = row[d + j];
         }
+        return c;
     }
-}
+    __device__ __forceinline__ Column(const T* from, int dim) : row(from), head_dim(dim) {
+        if constexpr (kHeld)
+#pragma unroll
+            for (int s = 0; s < kSteps; ++s) held[s] = read(s);
+    }
+    __device__ __forceinline__ Chunk<T> operator[](int step) const {
+        if constexpr (kHeld) return held[step];
+        return read(step);
+    }
+};
 
 // The other half's value for the same column.
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
 // Column values 32 p + 8 g + 4 half + 0 .. 3 of a lane, times factor, to its row.
-template <typename T, int kParts, bool kDirect>
+template <bool kDirect, typename T, int kParts>
 __device__ __forceinline__ void store_column(T* row, int head_dim, const Acc (&acc)[kParts], float factor) {
     const int half = (static_cast<int>(threadIdx.x) >> 5) & 1;
 #pragma unroll
