@@ -8,10 +8,12 @@
 //
 // Bound: HBM, each row array read and written once.
 #include <algorithm>
+#include <initializer_list>
 
 #include "common.h"
 #include "dllm_hip.h"
 #include "element.h"
+#include "lds_copy.h"
 #include "workspace.h"
 
 using namespace dllm_hip;
@@ -210,6 +212,241 @@ __global__ __launch_bounds__(256) void backward_rows_any_kernel(NormArgs a) {
     }
 }
 
+// ---- rows of whole vectors, held in registers ----
+//
+// A workgroup has a row, a thread kVectors vectors of kWidth consecutive elements, blockDim vectors apart, so that a row is
+// read once and its sums need one barrier each. kWidth is a 16-byte access, or 1 where rows or pointers are not whole ones.
+
+template <typename T, int kWidth>
+struct Vector {
+    Pack<T, kWidth> raw;
+    __device__ __forceinline__ void load(const void* array, int64_t at, bool in) {
+        if (in) raw = *reinterpret_cast<const Pack<T, kWidth>*>(static_cast<const T*>(array) + at);
+        else raw = Pack<T, kWidth>{};
+    }
+    __device__ __forceinline__ float operator[](int i) const { return static_cast<float>(raw.v[i]); }
+};
+
+// A float32 parameter at kWidth channels: offset + value, or ones where there is none.
+template <int kWidth>
+__device__ __forceinline__ void load_weight(const float* w, int64_t c, bool in, float offset, float (&out)[kWidth]) {
+#pragma unroll
+    for (int i = 0; i < kWidth; ++i) out[i] = w ? 0.0f : 1.0f;
+    if (!w || !in) return;
+    constexpr int kPart = kWidth < 4 ? kWidth : 4;
+#pragma unroll
+    for (int p = 0; p < kWidth / kPart; ++p) {
+        float v[kPart];
+        load_as_float<float, kPart>(w + c + p * kPart, v);
+#pragma unroll
+        for (int i = 0; i < kPart; ++i) out[p * kPart + i] = offset + v[i];
+    }
+}
+
+// Sums over the workgroup with one barrier: the caller alternates between two scratch areas.
+template <int N>
+__device__ __forceinline__ void row_sum(float (&v)[N], float* scratch) {
+    const int wave = static_cast<int>(threadIdx.x) >> 6, waves = static_cast<int>(blockDim.x) >> 6;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = wave_sum(v[i]);
+    if (waves == 1) return;
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) scratch[wave * N + i] = v[i];
+    lds_barrier();
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = scratch[i];
+    for (int w = 1; w < waves; ++w)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] += scratch[w * N + i];
+}
+
+constexpr int kRowThreads = 512;  // at most, of a row
+
+template <typename T, int kWidth, int kVectors>
+__global__ __launch_bounds__(kRowThreads) void forward_kernel(NormArgs a) {
+    __shared__ float scratch[2][16];
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        Vector<T, kWidth> x[kVectors], y[kVectors], gate[kVectors];
+        int64_t c[kVectors];
+        bool in[kVectors];
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) {
+            c[k] = (static_cast<int64_t>(k) * blockDim.x + threadIdx.x) * kWidth;
+            in[k] = c[k] < a.dim;
+            x[k].load(a.x, row * a.dim + c[k], in[k]);
+            y[k].load(a.y, row * a.dim + c[k], in[k]);
+            if (a.gate_kind == 2) gate[k].load(a.gate, row * a.dim + c[k], in[k]);
+        }
+        float ry = 1.0f;
+        if (a.post) {
+            float s[1] = {0.0f};
+#pragma unroll
+            for (int k = 0; k < kVectors; ++k)
+#pragma unroll
+                for (int i = 0; i < kWidth; ++i) s[0] = fmaf(y[k][i], y[k][i], s[0]);
+            row_sum(s, scratch[0]);
+            ry = inverse_rms(s[0], a);
+        }
+        float h[kVectors][kWidth], s[1] = {0.0f};
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) {
+            float w[kWidth], g[kWidth];
+            load_weight<kWidth>(a.post ? a.post_weight : nullptr, c[k], in[k], a.offset, w);
+            load_weight<kWidth>(a.gate_kind == 1 ? static_cast<const float*>(a.gate) : nullptr, c[k], in[k], 0.0f, g);
+#pragma unroll
+            for (int i = 0; i < kWidth; ++i) {
+                float z = y[k][i];
+                if (a.post) z = z * ry * w[i];
+                if (a.gate_kind) z *= a.gate_kind == 1 ? g[i] : gate[k][i];
+                h[k][i] = fmaf(a.scale, z, x[k][i]);
+                s[0] = fmaf(h[k][i], h[k][i], s[0]);
+            }
+            if (in[k]) store_from_float<T, kWidth>(static_cast<T*>(a.h) + row * a.dim + c[k], h[k]);
+        }
+        if (!a.pre) continue;
+        row_sum(s, scratch[1]);
+        const float rh = inverse_rms(s[0], a);
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) {
+            float w[kWidth];
+            load_weight<kWidth>(a.pre_weight, c[k], in[k], a.offset, w);
+#pragma unroll
+            for (int i = 0; i < kWidth; ++i) h[k][i] = h[k][i] * rh * w[i];
+            if (in[k]) store_from_float<T, kWidth>(static_cast<T*>(a.n) + row * a.dim + c[k], h[k]);
+        }
+    }
+}
+
+// The gradients of one row after another, the next row's loads in flight while the sums of this one are formed (where two
+// rows fit the registers); a thread keeps its columns' sums of the gate's and the weights' gradients, which are added over
+// the workgroups afterwards.
+template <typename T, int kWidth, int kVectors>
+__global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
+    constexpr bool kAhead = 5 * kVectors * (kWidth * sizeof(T) > 4 ? kWidth * sizeof(T) / 4 : 1) <= 40;
+    __shared__ float first_scratch[3 * 16], second_scratch[16];
+    float sums[3][kVectors][kWidth] = {};
+    int64_t c[kVectors];
+    bool in[kVectors];
+#pragma unroll
+    for (int k = 0; k < kVectors; ++k) {
+        c[k] = (static_cast<int64_t>(k) * blockDim.x + threadIdx.x) * kWidth;
+        in[k] = c[k] < a.dim;
+    }
+    struct Row {
+        Vector<T, kWidth> h[kVectors], y[kVectors], dh[kVectors], dn[kVectors], gate[kVectors];
+    };
+    auto load = [&](Row& to, int64_t row) {
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) {
+            const int64_t at = row * a.dim + c[k];
+            const bool there = in[k] && row < a.rows;
+            to.h[k].load(a.x, at, there && a.pre);
+            to.dn[k].load(a.dn, at, there && a.pre);
+            to.y[k].load(a.y, at, there);
+            to.dh[k].load(a.dh, at, there && a.dh);
+            to.gate[k].load(a.gate, at, there && a.gate_kind == 2);
+        }
+    };
+    // parameters stay in registers where they are few
+    constexpr bool kHeld = kVectors * kWidth <= 8;
+    float held[3][kHeld ? kVectors : 1][kWidth];
+    auto weights = [&](int k, float (&post)[kWidth], float (&pre)[kWidth], float (&gate)[kWidth]) {
+        load_weight<kWidth>(a.post ? a.post_weight : nullptr, c[k], in[k], a.offset, post);
+        load_weight<kWidth>(a.pre ? a.pre_weight : nullptr, c[k], in[k], a.offset, pre);
+        load_weight<kWidth>(a.gate_kind == 1 ? static_cast<const float*>(a.gate) : nullptr, c[k], in[k], 0.0f, gate);
+    };
+    if constexpr (kHeld)
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) weights(k, held[0][k], held[1][k], held[2][k]);
+    auto parameters = [&](int k, float (&post)[kWidth], float (&pre)[kWidth], float (&gate)[kWidth]) {
+        if constexpr (kHeld) {
+#pragma unroll
+            for (int i = 0; i < kWidth; ++i) post[i] = held[0][k][i], pre[i] = held[1][k][i], gate[i] = held[2][k][i];
+        } else {
+            weights(k, post, pre, gate);
+        }
+    };
+
+    Row now, next;
+    if constexpr (kAhead) load(now, blockIdx.x);
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        load(kAhead ? next : now, kAhead ? row + gridDim.x : row);
+        float s[3] = {0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) {
+            float post[kWidth], pre[kWidth], gate[kWidth];
+            parameters(k, post, pre, gate);
+#pragma unroll
+            for (int i = 0; i < kWidth; ++i) {
+                const float h = now.h[k][i], y = now.y[k][i];
+                s[0] = fmaf(h, h, s[0]);
+                s[1] = fmaf(pre[i] * now.dn[k][i], h, s[1]);
+                s[2] = fmaf(y, y, s[2]);
+            }
+        }
+        row_sum(s, first_scratch);
+        const float rh = a.pre ? inverse_rms(s[0], a) : 0.0f;
+        const float ch = a.pre ? rh * rh * rh * a.inv_dim * s[1] : 0.0f;
+        const float ry = a.post ? inverse_rms(s[2], a) : 1.0f;
+        float du[kVectors][kWidth], u[1] = {0.0f};
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) {
+            float post[kWidth], pre[kWidth], gate[kWidth], g[kWidth], dgate[kWidth];
+            parameters(k, post, pre, gate);
+#pragma unroll
+            for (int i = 0; i < kWidth; ++i) {
+                const float h = now.h[k][i], dn = now.dn[k][i], y = now.y[k][i];
+                g[i] = now.dh[k][i] + fmaf(rh * pre[i], dn, -(h * ch));
+                const float hat = y * ry, dz = a.scale * g[i];
+                const float gated = a.gate_kind == 2 ? now.gate[k][i] : gate[i];
+                dgate[i] = dz * (hat * post[i]);
+                du[k][i] = dz * gated;
+                u[0] = fmaf(du[k][i] * post[i], y, u[0]);
+                sums[0][k][i] += dgate[i];
+                sums[1][k][i] = fmaf(du[k][i], hat, sums[1][k][i]);
+                sums[2][k][i] = fmaf(dn, h * rh, sums[2][k][i]);
+            }
+            const int64_t at = row * a.dim + c[k];
+            if (a.dx && in[k]) store_from_float<T, kWidth>(static_cast<T*>(a.dx) + at, g);
+            if (a.dgate && a.gate_kind == 2 && in[k]) store_from_float<T, kWidth>(static_cast<T*>(a.dgate) + at, dgate);
+        }
+        if (a.dy) {
+            float cy = 0.0f;
+            if (a.post) {
+                row_sum(u, second_scratch);
+                cy = ry * ry * ry * a.inv_dim * u[0];
+            }
+#pragma unroll
+            for (int k = 0; k < kVectors; ++k) {
+                float post[kWidth], pre[kWidth], gate[kWidth], dy[kWidth];
+                parameters(k, post, pre, gate);
+#pragma unroll
+                for (int i = 0; i < kWidth; ++i)
+                    dy[i] = a.post ? fmaf(ry * post[i], du[k][i], -(now.y[k][i] * cy)) : du[k][i];
+                if (in[k]) store_from_float<T, kWidth>(static_cast<T*>(a.dy) + row * a.dim + c[k], dy);
+            }
+        }
+        // without the second sum's barrier, the first one's scratch is still being read
+        if (!a.dy || !a.post) lds_barrier();
+        if constexpr (kAhead) now = next;
+    }
+#pragma unroll
+    for (int which = 0; which < 3; ++which)
+        if (a.sums >> which & 1)
+#pragma unroll
+            for (int k = 0; k < kVectors; ++k)
+                if (in[k]) {
+                    float* to = a.partial + (static_cast<int64_t>(which) * gridDim.x + blockIdx.x) * a.dim + c[k];
+                    if constexpr (kWidth == 1) {
+                        to[0] = sums[which][k][0];
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kWidth; i += 4) store_from_float<float, 4>(to + i, *reinterpret_cast<float(*)[4]>(&sums[which][k][i]));
+                    }
+                }
+}
+
 // out[k][c] = the chunks' sums: 16 rows of threads take every 16th chunk in order, then are added in order.
 __global__ __launch_bounds__(1024) void column_reduce_kernel(const float* __restrict__ partial, float* dgate,
                                                              float* dpost, float* dpre, int64_t dim, int64_t chunks) {
@@ -233,6 +470,10 @@ constexpr int64_t kMaxGrid = 1 << 16;  // rows beyond it are taken in turn
 
 int64_t any_chunk_rows(int64_t rows) { return std::max<int64_t>(64, ceil_div(rows, 1024)); }
 
+// Workgroups of the gradient's rows: two to a CU, each with its rows' loads one row ahead. More would add column sums to be
+// written and read again.
+constexpr int64_t kBackwardGroups = 512;
+
 struct BackwardLayout {
     int64_t chunks;
     size_t stats, partial, bytes;
@@ -243,11 +484,24 @@ BackwardLayout backward_layout(const dllm_hip_residual_norm_shape& sh) {
     Layout l;
     b.stats = static_cast<size_t>(sh.rows) * 4;
     b.chunks = static_cast<int64_t>(ceil_div(sh.rows, any_chunk_rows(sh.rows)));
-    b.partial = static_cast<size_t>(3 * b.chunks * sh.dim);
+    b.partial = static_cast<size_t>(3 * std::max(b.chunks, std::min(sh.rows, kBackwardGroups)) * sh.dim);
     l.add<float>(b.stats);
     l.add<float>(b.partial);
     b.bytes = l.bytes;
     return b;
+}
+
+// Threads and vectors of a row of `vectors` vectors: the fewest vectors to a thread that `most` threads can take; 0 where
+// `deepest` to a thread are not enough.
+struct RowShape {
+    int threads, each;
+};
+RowShape row_shape(int64_t vectors, int most, int deepest) {
+    for (int each = 1; each <= deepest; each *= 2) {
+        const int64_t threads = static_cast<int64_t>(round_up(ceil_div(vectors, each), 64));
+        if (threads <= most) return {static_cast<int>(threads), each};
+    }
+    return {0, 0};
 }
 
 int check_shape(const dllm_hip_residual_norm_shape* sh) {
@@ -275,24 +529,69 @@ NormArgs arguments(const dllm_hip_residual_norm_shape& sh) {
     return a;
 }
 
-template <typename T>
-int launch_forward(const NormArgs& a, hipStream_t stream) {
-    forward_any_kernel<T><<<static_cast<unsigned>(std::min(a.rows, kMaxGrid)), 256, 0, stream>>>(a);
-    return check_launch("residual_norm");
+template <typename T, int kWidth>
+bool launch_forward_rows(const NormArgs& a, hipStream_t stream) {
+    const RowShape r = row_shape(a.dim / kWidth, kRowThreads, kWidth == 1 ? 16 : 4);
+    const unsigned grid = static_cast<unsigned>(std::min(a.rows, kMaxGrid));
+    switch (r.each) {
+        case 1: forward_kernel<T, kWidth, 1><<<grid, r.threads, 0, stream>>>(a); return true;
+        case 2: forward_kernel<T, kWidth, 2><<<grid, r.threads, 0, stream>>>(a); return true;
+        case 4: forward_kernel<T, kWidth, 4><<<grid, r.threads, 0, stream>>>(a); return true;
+        case 8:
+            if constexpr (kWidth == 1) forward_kernel<T, 1, 8><<<grid, r.threads, 0, stream>>>(a);
+            return true;
+        case 16:
+            if constexpr (kWidth == 1) forward_kernel<T, 1, 16><<<grid, r.threads, 0, stream>>>(a);
+            return true;
+        default: return false;
+    }
 }
 
 template <typename T>
-int launch_backward(const NormArgs& a, int64_t chunks, float* dpost, float* dpre, hipStream_t stream) {
-    const unsigned rows = static_cast<unsigned>(std::min(a.rows, kMaxGrid));
-    backward_stats_any_kernel<T><<<rows, 256, 0, stream>>>(a);
-    if (a.sums) {
-        const dim3 grid(static_cast<unsigned>(ceil_div(a.dim, 256)), static_cast<unsigned>(chunks));
-        backward_columns_any_kernel<T><<<grid, 256, 0, stream>>>(a);
-        column_reduce_kernel<<<dim3(static_cast<unsigned>(ceil_div(a.dim, 64)), 3), 1024, 0, stream>>>(
-            a.partial, a.sums & 1 ? static_cast<float*>(a.dgate) : nullptr, dpost, dpre, a.dim, chunks);
+int launch_forward(const NormArgs& a, bool whole, hipStream_t stream) {
+    const bool done = whole ? launch_forward_rows<T, kChunk<T>>(a, stream) : launch_forward_rows<T, 1>(a, stream);
+    if (!done) forward_any_kernel<T><<<static_cast<unsigned>(std::min(a.rows, kMaxGrid)), 256, 0, stream>>>(a);
+    return check_launch("residual_norm");
+}
+
+template <typename T, int kWidth>
+bool launch_backward_rows(const NormArgs& a, unsigned grid, hipStream_t stream) {
+    const RowShape r = row_shape(a.dim / kWidth, kRowThreads, kWidth == 1 ? 16 : 4);
+    switch (r.each) {
+        case 1: backward_kernel<T, kWidth, 1><<<grid, r.threads, 0, stream>>>(a); return true;
+        case 2: backward_kernel<T, kWidth, 2><<<grid, r.threads, 0, stream>>>(a); return true;
+        case 4: backward_kernel<T, kWidth, 4><<<grid, r.threads, 0, stream>>>(a); return true;
+        case 8:
+            if constexpr (kWidth == 1) backward_kernel<T, 1, 8><<<grid, r.threads, 0, stream>>>(a);
+            return true;
+        case 16:
+            if constexpr (kWidth == 1) backward_kernel<T, 1, 16><<<grid, r.threads, 0, stream>>>(a);
+            return true;
+        default: return false;
     }
-    if (a.dx || a.dy || (a.dgate && a.gate_kind == 2)) backward_rows_any_kernel<T><<<rows, 256, 0, stream>>>(a);
+}
+
+template <typename T>
+int launch_backward(const NormArgs& a, bool whole, int64_t chunks, float* dpost, float* dpre, hipStream_t stream) {
+    const unsigned groups = static_cast<unsigned>(std::min(a.rows, kBackwardGroups));
+    const bool done = whole ? launch_backward_rows<T, kChunk<T>>(a, groups, stream) : launch_backward_rows<T, 1>(a, groups, stream);
+    const unsigned rows = static_cast<unsigned>(std::min(a.rows, kMaxGrid));
+    if (!done) backward_stats_any_kernel<T><<<rows, 256, 0, stream>>>(a);
+    if (!done && a.sums)
+        backward_columns_any_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(a.dim, 256)), static_cast<unsigned>(chunks)), 256, 0, stream>>>(a);
+    if (a.sums)
+        column_reduce_kernel<<<dim3(static_cast<unsigned>(ceil_div(a.dim, 64)), 3), 1024, 0, stream>>>(
+            a.partial, a.sums & 1 ? static_cast<float*>(a.dgate) : nullptr, dpost, dpre, a.dim, done ? groups : chunks);
+    // after the column sums: dx may be dh, which they read
+    if (!done && (a.dx || a.dy || (a.dgate && a.gate_kind == 2))) backward_rows_any_kernel<T><<<rows, 256, 0, stream>>>(a);
     return check_launch("residual_norm_backward");
+}
+
+// Rows and pointers of whole 16-byte vectors.
+bool whole_vectors(const NormArgs& a, size_t size, std::initializer_list<const void*> arrays) {
+    bool whole = a.dim % static_cast<int64_t>(16 / size) == 0;
+    for (const void* p : arrays) whole = whole && aligned_to(p, 16);
+    return whole;
 }
 
 }  // namespace
@@ -311,11 +610,12 @@ int dllm_hip_residual_norm(const dllm_hip_residual_norm_shape* sh, const void* x
                      aligned_to(pre_weight, 4),
                  "pointers must be aligned to the element");
     a.x = x, a.y = y, a.gate = gate, a.post_weight = post_weight, a.pre_weight = pre_weight, a.h = h, a.n = n;
+    const bool whole = whole_vectors(a, size, {x, y, gate, post_weight, pre_weight, h, n});
     auto s = static_cast<hipStream_t>(stream);
     switch (sh->dtype) {
-        case kFloat32: return launch_forward<float>(a, s);
-        case kBFloat16: return launch_forward<__bf16>(a, s);
-        default: return launch_forward<_Float16>(a, s);
+        case kFloat32: return launch_forward<float>(a, whole, s);
+        case kBFloat16: return launch_forward<__bf16>(a, whole, s);
+        default: return launch_forward<_Float16>(a, whole, s);
     }
 }
 
@@ -357,10 +657,11 @@ int dllm_hip_residual_norm_backward(const dllm_hip_residual_norm_shape* sh, cons
     a.dx = dx, a.dy = dy, a.dgate = dgate;
     a.chunk_rows = any_chunk_rows(sh->rows);
     a.sums = (a.gate_kind == 1 && dgate ? 1 : 0) | (dpost_weight ? 2 : 0) | (dpre_weight ? 4 : 0);
+    const bool whole = whole_vectors(a, size, {h, y, gate, post_weight, pre_weight, dh, dn, dx, dy, dgate});
     switch (sh->dtype) {
-        case kFloat32: return launch_backward<float>(a, b.chunks, dpost_weight, dpre_weight, s);
-        case kBFloat16: return launch_backward<__bf16>(a, b.chunks, dpost_weight, dpre_weight, s);
-        default: return launch_backward<_Float16>(a, b.chunks, dpost_weight, dpre_weight, s);
+        case kFloat32: return launch_backward<float>(a, whole, b.chunks, dpost_weight, dpre_weight, s);
+        case kBFloat16: return launch_backward<__bf16>(a, whole, b.chunks, dpost_weight, dpre_weight, s);
+        default: return launch_backward<_Float16>(a, whole, b.chunks, dpost_weight, dpre_weight, s);
     }
 }
 
