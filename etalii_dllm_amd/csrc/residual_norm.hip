@@ -36,10 +36,20 @@ struct NormArgs {
     int sums;  // bit 0: dgate, 1: dpost_weight, 2: dpre_weight
 };
 
+// The sum of a wave's 64 values, in every lane: rows of 16 lanes by shifts, then across the rows (data-parallel primitives:
+// no trip through LDS).
+template <int kControl>
+__device__ __forceinline__ float shifted(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), kControl, 0xf, 0xf, true));
+}
 __device__ __forceinline__ float wave_sum(float v) {
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) v += __shfl_xor(v, s);
-    return v;
+    v += shifted<0x111>(v);  // row_shr 1, 2, 4, 8
+    v += shifted<0x112>(v);
+    v += shifted<0x114>(v);
+    v += shifted<0x118>(v);
+    v += shifted<0x142>(v);  // each row's last lane to the next row, then lane 31 to the upper half
+    v += shifted<0x143>(v);
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), 63));
 }
 
 // Sums of a workgroup's values, the waves' added in wave order; every thread gets them. scratch: 16 * N floats.
@@ -224,6 +234,22 @@ struct Vector {
         if (in) raw = *reinterpret_cast<const Pack<T, kWidth>*>(static_cast<const T*>(array) + at);
         else raw = Pack<T, kWidth>{};
     }
+    // Without a branch, so that a wait for it does not wait for the loads after it: lanes outside read element 0 of the row.
+    __device__ __forceinline__ void load_all(const T* row, int64_t c) { raw = *reinterpret_cast<const Pack<T, kWidth>*>(row + c); }
+    __device__ __forceinline__ void keep_if(bool in) {
+        constexpr int kWords = (kWidth * sizeof(T) + 3) / 4;
+        if constexpr (kWidth * sizeof(T) % 4 == 0) {
+            union {
+                Pack<T, kWidth> p;
+                uint32_t w[kWords];
+            } u{raw};
+#pragma unroll
+            for (int i = 0; i < kWords; ++i) u.w[i] = in ? u.w[i] : 0u;
+            raw = u.p;
+        } else {
+            raw.v[0] = in ? raw.v[0] : static_cast<T>(0.0f);
+        }
+    }
     __device__ __forceinline__ float operator[](int i) const { return static_cast<float>(raw.v[i]); }
 };
 
@@ -320,10 +346,13 @@ __global__ __launch_bounds__(kRowThreads) void forward_kernel(NormArgs a) {
 
 // The gradients of one row after another, the next row's loads in flight while the sums of this one are formed (where two
 // rows fit the registers); a thread keeps its columns' sums of the gate's and the weights' gradients, which are added over
-// the workgroups afterwards.
+// the workgroups afterwards. kPre: a norm before the next block; kElementGate: a gate for each element.
 template <typename T, int kWidth, int kVectors>
+constexpr bool kRowAhead = 5 * kVectors * (kWidth * sizeof(T) > 4 ? kWidth * sizeof(T) / 4 : 1) <= 40;
+
+template <typename T, int kWidth, int kVectors, bool kPre, bool kElementGate>
 __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
-    constexpr bool kAhead = 5 * kVectors * (kWidth * sizeof(T) > 4 ? kWidth * sizeof(T) / 4 : 1) <= 40;
+    constexpr bool kAhead = kRowAhead<T, kWidth, kVectors>;
     __shared__ float first_scratch[3 * 16], second_scratch[16];
     float sums[3][kVectors][kWidth] = {};
     int64_t c[kVectors];
@@ -336,35 +365,64 @@ __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
     struct Row {
         Vector<T, kWidth> h[kVectors], y[kVectors], dh[kVectors], dn[kVectors], gate[kVectors];
     };
+    const T* const dh_array = static_cast<const T*>(a.dh ? a.dh : a.y);  // something to load where there is none
     auto load = [&](Row& to, int64_t row) {
+        const int64_t at = std::min(row, a.rows - 1) * a.dim;
 #pragma unroll
         for (int k = 0; k < kVectors; ++k) {
-            const int64_t at = row * a.dim + c[k];
-            const bool there = in[k] && row < a.rows;
-            to.h[k].load(a.x, at, there && a.pre);
-            to.dn[k].load(a.dn, at, there && a.pre);
-            to.y[k].load(a.y, at, there);
-            to.dh[k].load(a.dh, at, there && a.dh);
-            to.gate[k].load(a.gate, at, there && a.gate_kind == 2);
+            const int64_t column = in[k] ? c[k] : 0;
+            if constexpr (kPre) to.h[k].load_all(static_cast<const T*>(a.x) + at, column);
+            if constexpr (kPre) to.dn[k].load_all(static_cast<const T*>(a.dn) + at, column);
+            to.y[k].load_all(static_cast<const T*>(a.y) + at, column);
+            to.dh[k].load_all(dh_array + at, column);
+            if constexpr (kElementGate) to.gate[k].load_all(static_cast<const T*>(a.gate) + at, column);
         }
     };
-    // parameters stay in registers where they are few
+    auto mask = [&](Row& r) {
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) {
+            if constexpr (kPre) r.h[k].keep_if(in[k]), r.dn[k].keep_if(in[k]);
+            r.y[k].keep_if(in[k]);
+            r.dh[k].keep_if(in[k] && a.dh);
+            if constexpr (kElementGate) r.gate[k].keep_if(in[k]);
+        }
+    };
+    // Parameters stay in registers where they are few, else in LDS (each thread its own): a load from memory here would be
+    // waited for together with the next row's.
     constexpr bool kHeld = kVectors * kWidth <= 8;
+    extern __shared__ __attribute__((aligned(16))) float parameter_lds[];  // [3][blockDim * kVectors * kWidth], or nothing
     float held[3][kHeld ? kVectors : 1][kWidth];
-    auto weights = [&](int k, float (&post)[kWidth], float (&pre)[kWidth], float (&gate)[kWidth]) {
+    const int area = static_cast<int>(blockDim.x) * kVectors * kWidth;
+    auto in_lds = [&](int which, int k) { return parameter_lds + which * area + static_cast<int>(c[k]); };
+    auto from_memory = [&](int k, float (&post)[kWidth], float (&pre)[kWidth], float (&gate)[kWidth]) {
         load_weight<kWidth>(a.post ? a.post_weight : nullptr, c[k], in[k], a.offset, post);
-        load_weight<kWidth>(a.pre ? a.pre_weight : nullptr, c[k], in[k], a.offset, pre);
+        load_weight<kWidth>(kPre ? a.pre_weight : nullptr, c[k], in[k], a.offset, pre);
         load_weight<kWidth>(a.gate_kind == 1 ? static_cast<const float*>(a.gate) : nullptr, c[k], in[k], 0.0f, gate);
     };
-    if constexpr (kHeld)
+    if constexpr (kHeld) {
 #pragma unroll
-        for (int k = 0; k < kVectors; ++k) weights(k, held[0][k], held[1][k], held[2][k]);
+        for (int k = 0; k < kVectors; ++k) from_memory(k, held[0][k], held[1][k], held[2][k]);
+    } else if constexpr (kAhead) {
+#pragma unroll
+        for (int k = 0; k < kVectors; ++k) {
+            float w[3][kWidth];
+            from_memory(k, w[0], w[1], w[2]);
+#pragma unroll
+            for (int which = 0; which < 3; ++which)
+#pragma unroll
+                for (int i = 0; i < kWidth; ++i) in_lds(which, k)[i] = w[which][i];
+        }
+    }
     auto parameters = [&](int k, float (&post)[kWidth], float (&pre)[kWidth], float (&gate)[kWidth]) {
-        if constexpr (kHeld) {
+        if constexpr (kHeld || kAhead) {
 #pragma unroll
-            for (int i = 0; i < kWidth; ++i) post[i] = held[0][k][i], pre[i] = held[1][k][i], gate[i] = held[2][k][i];
+            for (int i = 0; i < kWidth; ++i) {
+                post[i] = kHeld ? held[0][kHeld ? k : 0][i] : in_lds(0, k)[i];
+                pre[i] = kHeld ? held[1][kHeld ? k : 0][i] : in_lds(1, k)[i];
+                gate[i] = kHeld ? held[2][kHeld ? k : 0][i] : in_lds(2, k)[i];
+            }
         } else {
-            weights(k, post, pre, gate);
+            from_memory(k, post, pre, gate);
         }
     };
 
@@ -372,23 +430,30 @@ __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
     if constexpr (kAhead) load(now, blockIdx.x);
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         load(kAhead ? next : now, kAhead ? row + gridDim.x : row);
-        float s[3] = {0.0f, 0.0f, 0.0f};
+        mask(now);
+        float s[kPre ? 3 : 1] = {};
 #pragma unroll
         for (int k = 0; k < kVectors; ++k) {
             float post[kWidth], pre[kWidth], gate[kWidth];
             parameters(k, post, pre, gate);
 #pragma unroll
             for (int i = 0; i < kWidth; ++i) {
-                const float h = now.h[k][i], y = now.y[k][i];
-                s[0] = fmaf(h, h, s[0]);
-                s[1] = fmaf(pre[i] * now.dn[k][i], h, s[1]);
-                s[2] = fmaf(y, y, s[2]);
+                const float y = now.y[k][i];
+                s[0] = fmaf(y, y, s[0]);
+                if constexpr (kPre) {
+                    const float h = now.h[k][i];
+                    s[1] = fmaf(h, h, s[1]);
+                    s[2] = fmaf(pre[i] * now.dn[k][i], h, s[2]);
+                }
             }
         }
         row_sum(s, first_scratch);
-        const float rh = a.pre ? inverse_rms(s[0], a) : 0.0f;
-        const float ch = a.pre ? rh * rh * rh * a.inv_dim * s[1] : 0.0f;
-        const float ry = a.post ? inverse_rms(s[2], a) : 1.0f;
+        const float ry = a.post ? inverse_rms(s[0], a) : 1.0f;
+        float rh = 0.0f, ch = 0.0f;
+        if constexpr (kPre) {
+            rh = inverse_rms(s[1], a);
+            ch = rh * rh * rh * a.inv_dim * s[2];
+        }
         float du[kVectors][kWidth], u[1] = {0.0f};
 #pragma unroll
         for (int k = 0; k < kVectors; ++k) {
@@ -396,27 +461,31 @@ __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
             parameters(k, post, pre, gate);
 #pragma unroll
             for (int i = 0; i < kWidth; ++i) {
-                const float h = now.h[k][i], dn = now.dn[k][i], y = now.y[k][i];
-                g[i] = now.dh[k][i] + fmaf(rh * pre[i], dn, -(h * ch));
-                const float hat = y * ry, dz = a.scale * g[i];
-                const float gated = a.gate_kind == 2 ? now.gate[k][i] : gate[i];
+                const float y = now.y[k][i], hat = y * ry;
+                g[i] = now.dh[k][i];
+                if constexpr (kPre) {
+                    const float h = now.h[k][i], dn = now.dn[k][i];
+                    g[i] += fmaf(rh * pre[i], dn, -(h * ch));
+                    sums[2][k][i] = fmaf(dn, h * rh, sums[2][k][i]);
+                }
+                const float dz = a.scale * g[i];
+                float gated = gate[i];
+                if constexpr (kElementGate) gated = now.gate[k][i];
                 dgate[i] = dz * (hat * post[i]);
                 du[k][i] = dz * gated;
                 u[0] = fmaf(du[k][i] * post[i], y, u[0]);
                 sums[0][k][i] += dgate[i];
                 sums[1][k][i] = fmaf(du[k][i], hat, sums[1][k][i]);
-                sums[2][k][i] = fmaf(dn, h * rh, sums[2][k][i]);
             }
             const int64_t at = row * a.dim + c[k];
             if (a.dx && in[k]) store_from_float<T, kWidth>(static_cast<T*>(a.dx) + at, g);
-            if (a.dgate && a.gate_kind == 2 && in[k]) store_from_float<T, kWidth>(static_cast<T*>(a.dgate) + at, dgate);
+            if constexpr (kElementGate)
+                if (a.dgate && in[k]) store_from_float<T, kWidth>(static_cast<T*>(a.dgate) + at, dgate);
         }
-        if (a.dy) {
-            float cy = 0.0f;
-            if (a.post) {
-                row_sum(u, second_scratch);
-                cy = ry * ry * ry * a.inv_dim * u[0];
-            }
+        // (also where no dy is asked for: the barrier of this sum frees the first one's scratch)
+        row_sum(u, second_scratch);
+        const float cy = a.post ? ry * ry * ry * a.inv_dim * u[0] : 0.0f;
+        if (a.dy)
 #pragma unroll
             for (int k = 0; k < kVectors; ++k) {
                 float post[kWidth], pre[kWidth], gate[kWidth], dy[kWidth];
@@ -426,9 +495,6 @@ __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
                     dy[i] = a.post ? fmaf(ry * post[i], du[k][i], -(now.y[k][i] * cy)) : du[k][i];
                 if (in[k]) store_from_float<T, kWidth>(static_cast<T*>(a.dy) + row * a.dim + c[k], dy);
             }
-        }
-        // without the second sum's barrier, the first one's scratch is still being read
-        if (!a.dy || !a.post) lds_barrier();
         if constexpr (kAhead) now = next;
     }
 #pragma unroll
@@ -447,21 +513,27 @@ __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
                 }
 }
 
-// out[k][c] = the chunks' sums: 16 rows of threads take every 16th chunk in order, then are added in order.
+// out[c] = the chunks' sums of column c: 64 threads take every 64th chunk in order, then are added in a fixed tree. 16 columns
+// (a 64-byte piece of a row of sums) to a workgroup, so that a few thousand columns fill the CUs.
 __global__ __launch_bounds__(1024) void column_reduce_kernel(const float* __restrict__ partial, float* dgate,
                                                              float* dpost, float* dpre, int64_t dim, int64_t chunks) {
-    __shared__ float part[16][64];
-    const int col = threadIdx.x & 63, lane_row = threadIdx.x >> 6;
-    const int64_t c = static_cast<int64_t>(blockIdx.x) * 64 + col;
+    __shared__ float part[16][16];
     float* const out = blockIdx.y == 0 ? dgate : blockIdx.y == 1 ? dpost : dpre;
     if (!out) return;
+    const int col = threadIdx.x & 15, wave = threadIdx.x >> 6;
+    const int64_t c = static_cast<int64_t>(blockIdx.x) * 16 + col;
     const float* p = partial + static_cast<int64_t>(blockIdx.y) * chunks * dim;
     float s = 0.0f;
-    if (c < dim)
-        for (int64_t k = lane_row; k < chunks; k += 16) s += p[k * dim + c];
-    part[lane_row][col] = s;
+    if (c < dim) {
+#pragma unroll 8
+        for (int64_t k = threadIdx.x >> 4; k < chunks; k += 64) s += p[k * dim + c];
+    }
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+    if ((threadIdx.x & 63) < 16) part[wave][col] = s;
     __syncthreads();
-    if (lane_row || c >= dim) return;
+    if (threadIdx.x >= 16 || c >= dim) return;
+    s = part[0][col];
     for (int r = 1; r < 16; ++r) s += part[r][col];
     out[c] = s;
 }
@@ -554,33 +626,57 @@ int launch_forward(const NormArgs& a, bool whole, hipStream_t stream) {
     return check_launch("residual_norm");
 }
 
+template <typename T, int kWidth, int kVectors, bool kPre, bool kElementGate>
+int launch_backward_kind(const NormArgs& a, dim3 grid, int threads, hipStream_t stream) {
+    const bool lds = kRowAhead<T, kWidth, kVectors> && kVectors * kWidth > 8;
+    const int bytes = lds ? 3 * threads * kVectors * kWidth * 4 : 0;
+    const auto kernel = backward_kernel<T, kWidth, kVectors, kPre, kElementGate>;
+    if (bytes > 60 * 1024)
+        DLLM_TRY(check_hip(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes),
+                           "residual_norm_backward"));
+    kernel<<<grid, threads, bytes, stream>>>(a);
+    return check_launch("residual_norm_backward");
+}
+
+template <typename T, int kWidth, int kVectors>
+int launch_backward_vectors(const NormArgs& a, dim3 grid, int threads, hipStream_t stream) {
+    if (a.pre && a.gate_kind == 2) return launch_backward_kind<T, kWidth, kVectors, true, true>(a, grid, threads, stream);
+    if (a.pre) return launch_backward_kind<T, kWidth, kVectors, true, false>(a, grid, threads, stream);
+    if (a.gate_kind == 2) return launch_backward_kind<T, kWidth, kVectors, false, true>(a, grid, threads, stream);
+    return launch_backward_kind<T, kWidth, kVectors, false, false>(a, grid, threads, stream);
+}
+
+// The rows in registers, with `done`; not where they are too long for it.
 template <typename T, int kWidth>
-bool launch_backward_rows(const NormArgs& a, unsigned grid, hipStream_t stream) {
+int launch_backward_rows(const NormArgs& a, unsigned groups, bool& done, hipStream_t stream) {
     const RowShape r = row_shape(a.dim / kWidth, kRowThreads, kWidth == 1 ? 16 : 4);
+    done = r.each != 0;
     switch (r.each) {
-        case 1: backward_kernel<T, kWidth, 1><<<grid, r.threads, 0, stream>>>(a); return true;
-        case 2: backward_kernel<T, kWidth, 2><<<grid, r.threads, 0, stream>>>(a); return true;
-        case 4: backward_kernel<T, kWidth, 4><<<grid, r.threads, 0, stream>>>(a); return true;
-        case 8:
-            if constexpr (kWidth == 1) backward_kernel<T, 1, 8><<<grid, r.threads, 0, stream>>>(a);
-            return true;
-        case 16:
-            if constexpr (kWidth == 1) backward_kernel<T, 1, 16><<<grid, r.threads, 0, stream>>>(a);
-            return true;
-        default: return false;
+        case 1: return launch_backward_vectors<T, kWidth, 1>(a, groups, r.threads, stream);
+        case 2: return launch_backward_vectors<T, kWidth, 2>(a, groups, r.threads, stream);
+        case 4: return launch_backward_vectors<T, kWidth, 4>(a, groups, r.threads, stream);
     }
+    if constexpr (kWidth == 1) {
+        if (r.each == 8) return launch_backward_vectors<T, 1, 8>(a, groups, r.threads, stream);
+        if (r.each == 16) return launch_backward_vectors<T, 1, 16>(a, groups, r.threads, stream);
+    }
+    return kOk;
 }
 
 template <typename T>
 int launch_backward(const NormArgs& a, bool whole, int64_t chunks, float* dpost, float* dpre, hipStream_t stream) {
     const unsigned groups = static_cast<unsigned>(std::min(a.rows, kBackwardGroups));
-    const bool done = whole ? launch_backward_rows<T, kChunk<T>>(a, groups, stream) : launch_backward_rows<T, 1>(a, groups, stream);
     const unsigned rows = static_cast<unsigned>(std::min(a.rows, kMaxGrid));
+    bool done = false;
+    if (whole)
+        DLLM_TRY((launch_backward_rows<T, kChunk<T>>(a, groups, done, stream)));
+    else
+        DLLM_TRY((launch_backward_rows<T, 1>(a, groups, done, stream)));
     if (!done) backward_stats_any_kernel<T><<<rows, 256, 0, stream>>>(a);
     if (!done && a.sums)
         backward_columns_any_kernel<T><<<dim3(static_cast<unsigned>(ceil_div(a.dim, 256)), static_cast<unsigned>(chunks)), 256, 0, stream>>>(a);
     if (a.sums)
-        column_reduce_kernel<<<dim3(static_cast<unsigned>(ceil_div(a.dim, 64)), 3), 1024, 0, stream>>>(
+        column_reduce_kernel<<<dim3(static_cast<unsigned>(ceil_div(a.dim, 16)), 3), 1024, 0, stream>>>(
             a.partial, a.sums & 1 ? static_cast<float*>(a.dgate) : nullptr, dpost, dpre, a.dim, done ? groups : chunks);
     // after the column sums: dx may be dh, which they read
     if (!done && (a.dx || a.dy || (a.dgate && a.gate_kind == 2))) backward_rows_any_kernel<T><<<rows, 256, 0, stream>>>(a);
@@ -635,7 +731,7 @@ int dllm_hip_residual_norm_backward(const dllm_hip_residual_norm_shape* sh, cons
     auto s = static_cast<hipStream_t>(stream);
     if (sh->rows == 0) {  // sums over no rows
         for (float* out : {a.gate_kind == 1 ? static_cast<float*>(dgate) : nullptr, dpost_weight, dpre_weight})
-            if (out) column_reduce_kernel<<<dim3(static_cast<unsigned>(ceil_div(a.dim, 64))), 1024, 0, s>>>(nullptr, out, nullptr, nullptr, a.dim, 0);
+            if (out) column_reduce_kernel<<<dim3(static_cast<unsigned>(ceil_div(a.dim, 16))), 1024, 0, s>>>(nullptr, out, nullptr, nullptr, a.dim, 0);
         return check_launch("residual_norm_backward");
     }
     DLLM_REQUIRE((h || !a.pre) && y && (gate || a.gate_kind == 0) && (dn || !a.pre) && (dh || a.pre),
