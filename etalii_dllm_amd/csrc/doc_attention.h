@@ -51,14 +51,45 @@ __device__ __forceinline__ Document document_at(const DocAttention& a, int d) {
 }
 
 // The tile-th part of kRows tokens, counted through all documents; each document starts a part of its own, so that what
-// is computed for it does not depend on where it lies. kLast counts from the last document's last part. Every lane of the
-// wave returns the same. False past the last part.
-template <int kRows, bool kLast = false>
+// is computed for it does not depend on where it lies. Every lane of the wave returns the same. False past the last part.
+//
+// Parts come longest first, as far as that is cheap to know, so that the last workgroups to start are short ones: kFromEnd is
+// for work that grows towards a document's end (a causal row's keys), else towards its start (a key's queries). Up to 64
+// causal documents (one to a lane): the parts of the highest level first, of all documents that reach it, where a part's level
+// counts from the end with less work. Else the documents in order, each from the end with more work.
+template <int kRows, bool kFromEnd>
 __device__ __forceinline__ bool locate_tile(const DocAttention& a, int64_t tile, Document& doc, int& first) {
     const int lane = static_cast<int>(threadIdx.x) & 63;
+    auto found = [&](const Document& mine, int owner, int level) {
+        doc.start = __builtin_amdgcn_readlane(mine.start, owner);
+        doc.end = __builtin_amdgcn_readlane(mine.end, owner);
+        doc.prefix_end = __builtin_amdgcn_readlane(mine.prefix_end, owner);
+        const int parts = (doc.end - doc.start + kRows - 1) / kRows;
+        first = doc.start + (kFromEnd ? level : parts - 1 - level) * kRows;
+        return true;
+    };
+    if (a.documents <= 64 && a.causal) {
+        Document mine{0, 0, 0};
+        if (lane < a.documents) mine = document_at(a, lane);
+        const int parts = (mine.end - mine.start + kRows - 1) / kRows;
+        const int bits = 32 - __builtin_clz((a.tokens + kRows - 1) / kRows | 1);
+        auto at_or_above = [&](int level) {  // parts of that level or higher, by the bits of each document's number of them
+            const int n = parts > level ? parts - level : 0;
+            int64_t sum = 0;
+            for (int b = 0; b < bits; ++b) sum += static_cast<int64_t>(__popcll(__ballot(n >> b & 1))) << b;
+            return sum;
+        };
+        if (tile >= at_or_above(0)) return false;
+        int level = 0;
+        for (int b = bits - 1; b >= 0; --b)
+            if (at_or_above(level + (1 << b)) > tile) level += 1 << b;
+        uint64_t reach = __ballot(parts > level);
+        for (int64_t skip = tile - at_or_above(level + 1); skip > 0; --skip) reach &= reach - 1;
+        return found(mine, __builtin_ctzll(reach), level);
+    }
     int64_t before = 0;
     for (int base = 0; base < a.documents; base += 64) {
-        const int d = kLast ? a.documents - 1 - base - lane : base + lane;
+        const int d = kFromEnd ? a.documents - 1 - base - lane : base + lane;
         Document mine{0, 0, 0};
         if (d >= 0 && d < a.documents) mine = document_at(a, d);
         const int parts = (mine.end - mine.start + kRows - 1) / kRows;
@@ -70,15 +101,10 @@ __device__ __forceinline__ bool locate_tile(const DocAttention& a, int64_t tile,
         }
         const int64_t all = __shfl(through, 63);
         if (tile < before + all) {
-            const uint64_t past = __ballot(before + through > tile);
-            const int owner = __builtin_amdgcn_readfirstlane(__ffsll(static_cast<unsigned long long>(past)) - 1);
-            doc.start = __builtin_amdgcn_readlane(mine.start, owner);
-            doc.end = __builtin_amdgcn_readlane(mine.end, owner);
-            doc.prefix_end = __builtin_amdgcn_readlane(mine.prefix_end, owner);
-            int part = static_cast<int>(tile - __shfl(before + through - parts, owner));
-            if (kLast) part = __shfl(parts, owner) - 1 - part;
-            first = __builtin_amdgcn_readfirstlane(doc.start + part * kRows);
-            return true;
+            const int owner = __builtin_ctzll(__ballot(before + through > tile));
+            const int part = static_cast<int>(tile - __shfl(before + through - parts, owner));
+            const int count = __builtin_amdgcn_readlane(parts, owner);
+            return found(mine, owner, __builtin_amdgcn_readfirstlane(count - 1 - part));
         }
         before += all;
     }

@@ -215,7 +215,7 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 64 ? 2 : 1) void dkv_kernel(Do
     const int kv = head / a.group;
     Document doc;
     int first;
-    if (!locate_tile<kDocTileRows>(a, blockIdx.x / a.heads, doc, first)) return;
+    if (!locate_tile<kDocTileRows, false>(a, blockIdx.x / a.heads, doc, first)) return;
 
     const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
     const int wave_first = first + 32 * wave, wave_last = min(wave_first + 31, doc.end - 1);
@@ -387,7 +387,7 @@ __global__ __launch_bounds__(kDocThreads) void add_heads_kernel(DocAttention a) 
     const int per_row = (a.head_dim + kWidth - 1) / kWidth, per_token = a.kv_heads * per_row;
     Document doc;
     int first;
-    if (!locate_tile<kDocTileRows>(a, blockIdx.x, doc, first)) return;
+    if (!locate_tile<kDocTileRows, false>(a, blockIdx.x, doc, first)) return;
     const int rows = min(kDocTileRows, doc.end - first);
     for (int64_t e = static_cast<int64_t>(blockIdx.y) * kDocThreads + threadIdx.x; e < static_cast<int64_t>(rows) * per_token;
          e += static_cast<int64_t>(gridDim.y) * kDocThreads) {
