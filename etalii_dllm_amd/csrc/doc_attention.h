@@ -8,6 +8,7 @@
 #include <initializer_list>
 
 #include "common.h"
+#include "doc_tile.h"
 #include "element.h"
 
 namespace dllm_hip {
@@ -26,6 +27,8 @@ struct DocAttention {
     int tokens, documents, heads, kv_heads, group, head_dim;
     int causal, window;  // window 0: none
     float scale, softcap;  // softcap 0: none
+    bool whole;  // every array's rows are whole 16-byte chunks, aligned to them
+    Source sources[4];  // q, k, v, dout as the matrix cores read them
     // backward scratch
     float* delta;     // [heads][tokens]: dout . out
     float* dout_norm; // [heads][tokens]: |dout| (float16)
@@ -315,20 +318,89 @@ inline unsigned doc_tiles(const DocAttention& a, int rows) {
     return static_cast<unsigned>(ceil_div(a.tokens, rows) + (a.documents < a.tokens ? a.documents : a.tokens));
 }
 
-// Whole 16-byte chunks throughout: rows can be copied to LDS directly.
-template <typename T>
-bool whole_chunks(const DocAttention& a, std::initializer_list<const void*> arrays) {
-    bool whole = a.head_dim % kChunk<T> == 0;
+// Whole 16-byte chunks throughout, and strides that leave a copy's lane offsets below 2^32 bytes.
+inline bool whole_chunks(const DocAttention& a, int64_t chunk, std::initializer_list<const void*> arrays) {
+    bool whole = a.head_dim % chunk == 0;
     for (const int64_t s : {a.q_stride, a.k_stride, a.v_stride, a.out_stride})
-        whole = whole && s % kChunk<T> == 0 && s < (int64_t{1} << 25);  // a copy's lane offsets stay below 2^32 bytes
+        whole = whole && s % chunk == 0 && s < (int64_t{1} << 25);
     for (const void* p : arrays) whole = whole && aligned_to(p, 16);
     return whole;
 }
 
+// Bytes of one token of q, k, v (and dout) as packed sources.
+template <typename T>
+size_t packed_token_bytes(const DocAttention& a, bool backward) {
+    const size_t heads = static_cast<size_t>(a.heads) * (backward ? 2 : 1) + 2 * static_cast<size_t>(a.kv_heads);
+    return heads * round_up(a.head_dim, kPartChunk) * 2 * kPlanes<T>;
+}
+
+struct PackArgs {
+    const void* from[4];
+    int64_t stride[4];
+    Source to[4];
+    int heads[4];
+    int tokens, head_dim;
+};
+
+// Copies arrays into sources: split into planes, heads filled up with zeroes to whole chunks. A thread has a chunk.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
+    const int which = blockIdx.y;
+    const Source to = a.to[which];
+    const int64_t per_token = static_cast<int64_t>(a.heads[which]) * to.chunks;
+    for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < a.tokens * per_token; e += static_cast<int64_t>(gridDim.x) * 256) {
+        const int64_t token = e / per_token, in_token = e % per_token;
+        const int head = static_cast<int>(in_token / to.chunks), chunk = static_cast<int>(in_token % to.chunks);
+        const T* from = static_cast<const T*>(a.from[which]) + token * a.stride[which] + static_cast<int64_t>(head) * a.head_dim;
+        Part<T> parts[kPartChunk][kPlanes<T>];
+#pragma unroll
+        for (int j = 0; j < kPartChunk; ++j) {
+            const int d = chunk * kPartChunk + j;
+            if constexpr (kPlanes<T> == 1)
+                parts[j][0] = d < a.head_dim ? from[d] : static_cast<T>(0.0f);
+            else
+                split<T>(d < a.head_dim ? from[d] : 0.0f, parts[j]);
+        }
+#pragma unroll
+        for (int p = 0; p < kPlanes<T>; ++p) {
+            Pack<Part<T>, kPartChunk> c;
+#pragma unroll
+            for (int j = 0; j < kPartChunk; ++j) c.v[j] = parts[j][p];
+            *reinterpret_cast<Pack<Part<T>, kPartChunk>*>(const_cast<char*>(to.base) + p * to.plane + token * to.stride + head * to.head + chunk * 16) = c;
+        }
+    }
+}
+
+// a's sources: the arrays themselves where they are 16-bit and whole, else copies in the workspace.
+template <typename T>
+void set_sources(DocAttention& a, bool backward, char* packed, hipStream_t stream) {
+    const void* const arrays[4] = {a.q, a.k, a.v, a.dout};
+    const int64_t strides[4] = {a.q_stride, a.k_stride, a.v_stride, a.out_stride};
+    const int heads[4] = {a.heads, a.kv_heads, a.kv_heads, a.heads};
+    const int count = backward ? 4 : 3;
+    const int chunks = static_cast<int>(ceil_div(a.head_dim, kPartChunk));
+    if (kPlanes<T> == 1 && a.whole) {
+        for (int i = 0; i < count; ++i)
+            a.sources[i] = {static_cast<const char*>(arrays[i]), strides[i] * 2, int64_t{a.head_dim} * 2, 0, chunks};
+        return;
+    }
+    PackArgs p{};
+    p.tokens = a.tokens;
+    p.head_dim = a.head_dim;
+    for (int i = 0; i < count; ++i) {
+        const int64_t row = int64_t{heads[i]} * chunks * 16, plane = row * a.tokens;
+        a.sources[i] = {packed, row, int64_t{chunks} * 16, plane, chunks};
+        packed += plane * kPlanes<T>;
+        p.from[i] = arrays[i], p.stride[i] = strides[i], p.to[i] = a.sources[i], p.heads[i] = heads[i];
+    }
+    const size_t blocks = ceil_div(static_cast<size_t>(a.tokens) * a.heads * chunks, 256);
+    pack_kernel<T><<<dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), count), 256, 0, stream>>>(p);
+}
+
 // doc_attention_{f32,bf16,f16}.hip
 template <typename T>
-int launch_document_attention(const DocAttention& a, void* out, hipStream_t stream);
+int launch_document_attention(DocAttention a, void* out, char* packed, hipStream_t stream);
 template <typename T>
-int launch_document_attention_backward(const DocAttention& a, hipStream_t stream);
+int launch_document_attention_backward(DocAttention a, char* packed, hipStream_t stream);
 
 }  // namespace dllm_hip

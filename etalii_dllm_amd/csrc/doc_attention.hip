@@ -6,8 +6,8 @@
 #include <initializer_list>
 
 #include "common.h"
-#include "doc_attention.h"
 #include "dllm_hip.h"
+#include "doc_attention.h"
 #include "workspace.h"
 
 using namespace dllm_hip;
@@ -56,29 +56,35 @@ DocAttention arguments(const dllm_hip_document_attention_shape& sh) {
     return a;
 }
 
-size_t backward_bytes(const DocAttention& a) {
-    Layout l;
-    const size_t stats = static_cast<size_t>(a.heads) * a.tokens, part = a.group > 1 ? stats * a.head_dim : 0;
-    l.add<float>(stats);
-    l.add<float>(stats);
-    l.add<float>(part);
-    l.add<float>(part);
-    return l.bytes;
+size_t token_bytes(const DocAttention& a, int64_t dtype, bool backward) {
+    return dtype == kFloat32 ? packed_token_bytes<float>(a, backward) : packed_token_bytes<__bf16>(a, backward);
 }
+
+// The sources' copies; backward, the rows' statistics and the parts of heads that share keys too.
+struct AttentionLayout {
+    size_t packed, stats, part, bytes;
+    AttentionLayout(const DocAttention& a, int64_t dtype, bool backward) {
+        packed = token_bytes(a, dtype, backward) * static_cast<size_t>(a.tokens);
+        stats = backward ? static_cast<size_t>(a.heads) * a.tokens : 0;
+        part = backward && a.group > 1 ? stats * a.head_dim : 0;
+        Layout l;
+        l.add<char>(packed);
+        for (const size_t n : {stats, stats, part, part}) l.add<float>(n);
+        bytes = l.bytes;
+    }
+};
 
 }  // namespace
 
 extern "C" {
 
 size_t dllm_hip_document_attention_workspace(const dllm_hip_document_attention_shape* sh) {
-    (void)sh;
-    return 0;
+    return check_shape(sh) == kOk ? AttentionLayout(arguments(*sh), sh->dtype, false).bytes : 0;
 }
 
 int dllm_hip_document_attention(const dllm_hip_document_attention_shape* sh, const void* q, const void* k,
                                 const void* v, const int64_t* offsets, const int64_t* prefix, const float* slopes,
                                 void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
-    (void)workspace, (void)workspace_bytes;
     DLLM_TRY(check_shape(sh));
     if (sh->tokens == 0 || sh->documents == 0) return kOk;
     DLLM_REQUIRE(q && k && v && offsets && out, "null q, k, v, offsets or out");
@@ -87,17 +93,21 @@ int dllm_hip_document_attention(const dllm_hip_document_attention_shape* sh, con
                      aligned_to(offsets, 8) && aligned_to(prefix, 8) && aligned_to(slopes, 4) && aligned_to(lse, 4),
                  "pointers must be aligned to the element");
     DocAttention a = arguments(*sh);
+    const AttentionLayout layout(a, sh->dtype, false);
+    DLLM_REQUIRE(workspace && workspace_bytes >= layout.bytes, "workspace too small for document_attention");
+    DLLM_REQUIRE(aligned_to(workspace, 16), "the workspace must be aligned to 16 bytes");
     a.q = q, a.k = k, a.v = v, a.offsets = offsets, a.prefix = prefix, a.slopes = slopes, a.lse = lse;
+    char* const packed = Carve(workspace, workspace_bytes).take<char>(layout.packed);
     auto s = static_cast<hipStream_t>(stream);
     switch (sh->dtype) {
-        case kFloat32: return launch_document_attention<float>(a, out, s);
-        case kBFloat16: return launch_document_attention<__bf16>(a, out, s);
-        default: return launch_document_attention<_Float16>(a, out, s);
+        case kFloat32: return launch_document_attention<float>(a, out, packed, s);
+        case kBFloat16: return launch_document_attention<__bf16>(a, out, packed, s);
+        default: return launch_document_attention<_Float16>(a, out, packed, s);
     }
 }
 
 size_t dllm_hip_document_attention_backward_workspace(const dllm_hip_document_attention_shape* sh) {
-    return check_shape(sh) == kOk ? backward_bytes(arguments(*sh)) : 0;
+    return check_shape(sh) == kOk ? AttentionLayout(arguments(*sh), sh->dtype, true).bytes : 0;
 }
 
 int dllm_hip_document_attention_backward(const dllm_hip_document_attention_shape* sh, const void* q, const void* k,
@@ -115,22 +125,23 @@ int dllm_hip_document_attention_backward(const dllm_hip_document_attention_shape
     DLLM_REQUIRE(aligned_to(offsets, 8) && aligned_to(prefix, 8) && aligned_to(slopes, 4) && aligned_to(lse, 4),
                  "pointers must be aligned to the element");
     DocAttention a = arguments(*sh);
-    DLLM_REQUIRE(workspace && workspace_bytes >= backward_bytes(a), "workspace too small for document_attention_backward");
+    const AttentionLayout layout(a, sh->dtype, true);
+    DLLM_REQUIRE(workspace && workspace_bytes >= layout.bytes, "workspace too small for document_attention_backward");
     DLLM_REQUIRE(aligned_to(workspace, 16), "the workspace must be aligned to 16 bytes");
     a.q = q, a.k = k, a.v = v, a.offsets = offsets, a.prefix = prefix, a.slopes = slopes, a.out = out, a.dout = dout;
     a.lse = const_cast<float*>(lse);
     a.dq = dq, a.dk = dk, a.dv = dv;
     Carve c(workspace, workspace_bytes);
-    const size_t stats = static_cast<size_t>(a.heads) * a.tokens, part = a.group > 1 ? stats * a.head_dim : 0;
-    a.delta = c.take<float>(stats);
-    a.dout_norm = c.take<float>(stats);
-    a.dk_part = c.take<float>(part);
-    a.dv_part = c.take<float>(part);
+    char* const packed = c.take<char>(layout.packed);
+    a.delta = c.take<float>(layout.stats);
+    a.dout_norm = c.take<float>(layout.stats);
+    a.dk_part = c.take<float>(layout.part);
+    a.dv_part = c.take<float>(layout.part);
     auto s = static_cast<hipStream_t>(stream);
     switch (sh->dtype) {
-        case kFloat32: return launch_document_attention_backward<float>(a, s);
-        case kBFloat16: return launch_document_attention_backward<__bf16>(a, s);
-        default: return launch_document_attention_backward<_Float16>(a, s);
+        case kFloat32: return launch_document_attention_backward<float>(a, packed, s);
+        case kBFloat16: return launch_document_attention_backward<__bf16>(a, packed, s);
+        default: return launch_document_attention_backward<_Float16>(a, packed, s);
     }
 }
 

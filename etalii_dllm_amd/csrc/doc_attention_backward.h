@@ -11,14 +11,19 @@
 
 #include <float.h>
 
+#include <type_traits>
+
 #include "common.h"
 #include "doc_attention.h"
 #include "doc_tile.h"
 
 namespace dllm_hip {
 
+// Rows of a tile that goes through LDS, and whether two buffers of two tiles fit it.
 template <typename T, int kDim>
-constexpr int kStream = kDim * sizeof(T) <= 256 ? 64 : 32;  // rows of a tile that goes through LDS
+constexpr int kStream = kPlanes<T> == 1 || kDim <= 64 ? 64 : 32;
+template <typename T, int kDim>
+constexpr int kStreamBuffers = 4 * kStream<T, kDim> * kDim * 2 * kPlanes<T> <= 128 * 1024 ? 2 : 1;
 
 constexpr int kTogether = 128;
 
@@ -51,13 +56,15 @@ struct Bend {
 };
 
 // ---- dq ----
-template <typename T, int kDim, bool kDirect>
-__global__ __launch_bounds__(kDocThreads, kDim <= 128 ? 2 : 1) void dq_kernel(DocAttention a) {
+template <typename T, int kDim>
+__global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1) void dq_kernel(DocAttention a) {
     using Shape = TileShape<T, kDim>;
     constexpr int kTile = kStream<T, kDim>;
-    constexpr int kTileBytes = kTile * Shape::kRowBytes;
+    using Copy = TileCopy<T, kDim, kTile, kDocThreads>;
+    constexpr int kTileBytes = Copy::kBytes;
     constexpr int kParts = kDim / 32;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];
+    constexpr bool kAhead = kStreamBuffers<T, kDim> == 2;
+    __shared__ __attribute__((aligned(1024))) char lds[kStreamBuffers<T, kDim> * 2 * kTileBytes];
 
     const int turn = static_cast<int>(blockIdx.x) % a.heads;
     const int head = (turn % a.kv_heads) * a.group + turn / a.kv_heads;
@@ -74,18 +81,27 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 128 ? 2 : 1) void dq_kernel(Do
     const Span span = key_span(a, doc, i);
     const int64_t head_at = static_cast<int64_t>(head) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens + i;
 
-    const Column<T, kDim, kDirect> q(static_cast<const T*>(a.q) + i * a.q_stride + head_at, a.head_dim);
-    const Column<T, kDim, kDirect> dout(static_cast<const T*>(a.dout) + i * a.out_stride + head_at, a.head_dim);
-    float delta = 0.0f, norm = 0.0f;
+    const Column<T, kDim> q(a.sources[0], head, i), dout(a.sources[3], head, i);
+    float delta = 0.0f, norm = 0.0f;  // this half's part
     {
-        const Column<T, kDim, kDirect> out(static_cast<const T*>(a.out) + i * a.out_stride + head_at, a.head_dim);
+        const T* const out_row = static_cast<const T*>(a.out) + i * a.out_stride + head_at;
+        const T* const dout_row = static_cast<const T*>(a.dout) + i * a.out_stride + head_at;
+        auto add = [&](float o, float d) {
+            delta = fmaf(o, d, delta);
+            norm = fmaf(d, d, norm);
+        };
+        // (both ways take the same elements in the same order)
+        constexpr int kWide = kChunk<T>;
+        for (int d0 = half * kWide; d0 < a.head_dim; d0 += 2 * kWide) {
+            if (a.whole) {
+                float o[kWide], d[kWide];
+                load_as_float<T, kWide>(out_row + d0, o);
+                load_as_float<T, kWide>(dout_row + d0, d);
 #pragma unroll
-        for (int s = 0; s < Shape::kSteps; ++s) {
-            const Chunk<T> o = out[s], d = dout[s];
-#pragma unroll
-            for (int j = 0; j < kChunk<T>; ++j) {
-                delta = fmaf(static_cast<float>(o[j]), static_cast<float>(d[j]), delta);
-                norm = fmaf(static_cast<float>(d[j]), static_cast<float>(d[j]), norm);
+                for (int j = 0; j < kWide; ++j) add(o[j], d[j]);
+            } else {
+                for (int j = 0; j < kWide && d0 + j < a.head_dim; ++j)
+                    add(static_cast<float>(out_row[d0 + j]), static_cast<float>(dout_row[d0 + j]));
             }
         }
     }
@@ -106,9 +122,8 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 128 ? 2 : 1) void dq_kernel(Do
     const Span first_span = key_span(a, doc, wave_first), last_span = key_span(a, doc, wave_last);
     const int any_low = first_span.low, any_high = last_span.high, all_low = last_span.low, all_high = first_span.high;
 
-    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_k(a.k, a.k_stride, kv, a.head_dim);
-    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_v(a.v, a.v_stride, kv, a.head_dim);
-    const TileView<T, kDim> view;
+    const Copy copy_k(a.sources[1], kv), copy_v(a.sources[2], kv);
+    const TileView<T, kDim, kTile> view;
     LdsByte* const buffers = (LdsByte*)lds;
     const Bend<T> bend(a, head);
     const float base = a.lse[stat_at] * kLog2E - kWeightShift<T>;
@@ -126,11 +141,16 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 128 ? 2 : 1) void dq_kernel(Do
         copy_v(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
     };
     int t = next_tile(-1);
-    fetch(t, 0);
-    for (int buffer = 0; t < tiles; buffer ^= 1) {
+    if (kAhead) fetch(t, 0);
+    for (int buffer = 0; t < tiles; buffer ^= kAhead) {
         tile_barrier();
         const int next = next_tile(t);
-        if (next < tiles) fetch(next, buffer ^ 1);
+        if (!kAhead) {
+            fetch(t, 0);
+            tile_barrier();
+        } else if (next < tiles) {
+            fetch(next, buffer ^ 1);
+        }
         const LdsByte* const k_tile = buffers + buffer * 2 * kTileBytes;
         const LdsByte* const v_tile = k_tile + kTileBytes;
         const int from = doc.start + t * kTile;
@@ -143,9 +163,9 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 128 ? 2 : 1) void dq_kernel(Do
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
 #pragma unroll
-            for (int step = 0; step < Shape::kSteps; ++step) multiply(view.rows(k_tile, b, step), q[step], x);
+            for (int step = 0; step < Shape::kSteps; ++step) multiply<T>(view.rows(k_tile, b, step), q[step], x);
 #pragma unroll
-            for (int step = 0; step < Shape::kSteps; ++step) multiply(view.rows(v_tile, b, step), dout[step], dp);
+            for (int step = 0; step < Shape::kSteps; ++step) multiply<T>(view.rows(v_tile, b, step), dout[step], dp);
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] = fmaf(dp[r], into, -delta * into);
@@ -178,7 +198,7 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 128 ? 2 : 1) void dq_kernel(Do
                     ds[r] = see ? ds[r] : 0.0f;
                 }
             }
-            multiply_columns<T, kDim>(view, k_tile, b, ds, dq);
+            multiply_columns<T, kDim, kTile>(view, k_tile, b, Rows16<T>(ds), dq);
         }
     }
     if (!working) return;
@@ -186,7 +206,7 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 128 ? 2 : 1) void dq_kernel(Do
     spoilt = (spoilt | __shfl_xor(static_cast<int>(spoilt), 32)) && mine;
     T* const to = static_cast<T*>(a.dq) + head_at;
     if (!spoilt && mine)
-        store_column<kDirect>(to + i * a.q_stride, a.head_dim, dq, a.scale * dout_scale * __builtin_amdgcn_exp2f(-kWeightShift<T>));
+        store_column<T, kParts>(to + i * a.q_stride, a.head_dim, a.whole, dq, a.scale * dout_scale * __builtin_amdgcn_exp2f(-kWeightShift<T>));
     for (uint32_t left = static_cast<uint32_t>(__ballot(spoilt)); left; left &= left - 1) {
         const int from_lane = __ffs(left) - 1, row = wave_first + from_lane;
         float value[kLaneDims];
@@ -200,13 +220,16 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 128 ? 2 : 1) void dq_kernel(Do
 // kShared: into the float32 parts of heads that share keys. kDk, kDv: which of the two; rows of more than kTogether
 // elements take a launch for each, since the sums of both and a lane's two rows are more than its registers (five products
 // in all instead of four).
-template <typename T, int kDim, bool kDirect, bool kShared, bool kDk, bool kDv>
-__global__ __launch_bounds__(kDocThreads, kDim <= 64 ? 2 : 1) void dkv_kernel(DocAttention a) {
+template <typename T, int kDim, bool kShared, bool kDk, bool kDv>
+__global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1) void dkv_kernel(DocAttention a) {
     using Shape = TileShape<T, kDim>;
-    constexpr int kTile = kStream<T, kDim>;
-    constexpr int kTileBytes = kTile * Shape::kRowBytes;
+    constexpr bool kPipelined = sizeof(T) == 2 && kDim == 128;
+    constexpr int kTile = kPipelined ? 128 : kStream<T, kDim>;
+    using Copy = TileCopy<T, kDim, kTile, kDocThreads>;
+    constexpr int kTileBytes = Copy::kBytes;
     constexpr int kParts = kDim / 32;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];
+    constexpr bool kAhead = kStreamBuffers<T, kDim> == 2;
+    __shared__ __attribute__((aligned(1024))) char lds[(kAhead ? 4 : 2) * kTileBytes];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // lse in units of log 2, and dout . out, of a tile's queries
     __shared__ float largest[kDocThreads / 64];
 
@@ -225,8 +248,7 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 64 ? 2 : 1) void dkv_kernel(Do
     const Span span = query_span(a, doc, j);
     const int64_t kv_at = static_cast<int64_t>(kv) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens;
 
-    const Column<T, kDim, kDirect> k(static_cast<const T*>(a.k) + j * a.k_stride + kv_at, a.head_dim);
-    const Column<T, kDim, kDirect> v(static_cast<const T*>(a.v) + j * a.v_stride + kv_at, a.head_dim);
+    const Column<T, kDim> k(a.sources[1], kv, j), v(a.sources[2], kv, j);
 
     // the queries that see any key of the workgroup; keys in the prefix are seen from the document's start on
     const int last = min(first + kDocTileRows, doc.end) - 1;
@@ -256,9 +278,8 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 64 ? 2 : 1) void dkv_kernel(Do
     }
     const float into = 1.0f / dout_scale;
 
-    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_q(a.q, a.q_stride, head, a.head_dim);
-    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_d(a.dout, a.out_stride, head, a.head_dim);
-    const TileView<T, kDim> view;
+    const Copy copy_q(a.sources[0], head), copy_d(a.sources[3], head);
+    const TileView<T, kDim, kTile> view;
     LdsByte* const buffers = (LdsByte*)lds;
     const Bend<T> bend(a, head);
 
@@ -285,11 +306,17 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 64 ? 2 : 1) void dkv_kernel(Do
         copy_d(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
     };
     int t = low_tile;
-    write_stat(0, read_stat(t));
-    fetch(t, 0);
-    for (int buffer = 0; t < tiles; buffer ^= 1, ++t) {
+    if (kAhead) {
+        write_stat(0, read_stat(t));
+        fetch(t, 0);
+    }
+    for (int buffer = 0; t < tiles; buffer ^= kAhead, ++t) {
         tile_barrier();
-        if (t + 1 < tiles) {
+        if (!kAhead) {
+            write_stat(0, read_stat(t));
+            fetch(t, 0);
+            tile_barrier();
+        } else if (t + 1 < tiles) {
             write_stat(buffer ^ 1, read_stat(t + 1));
             fetch(t + 1, buffer ^ 1);
         }
@@ -298,29 +325,36 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 64 ? 2 : 1) void dkv_kernel(Do
         const int from = doc.start + t * kTile;
         if (!working || !(from < any_high && from + kTile > any_low)) continue;
         const bool all_seen = from >= all_low && from + kTile <= all_high;
-#pragma unroll
-        for (int b = 0; b < kTile / 32; ++b) {
-            Acc x, dp;
+        const float* const tile_base = &stats[buffer][0][4 * half];
+        const float* const tile_delta = &stats[buffer][1][4 * half];
+        using Four = float __attribute__((ext_vector_type(4)));
+
+        // 32 queries' scores and dP ...
+        auto products = [&](int b, Acc& x, Acc& dp) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
 #pragma unroll
-            for (int step = 0; step < Shape::kSteps; ++step) multiply(view.rows(q_tile, b, step), k[step], x);
-            if constexpr (kDk)
-#pragma unroll
-                for (int step = 0; step < Shape::kSteps; ++step) multiply(view.rows(d_tile, b, step), v[step], dp);
-            float p[16], ds[16];
-            using Four = float __attribute__((ext_vector_type(4)));
+            for (int step = 0; step < Shape::kSteps; ++step) {
+                multiply<T>(view.rows(q_tile, b, step), k[step], x);
+                if constexpr (kDk) multiply<T>(view.rows(d_tile, b, step), v[step], dp);
+            }
+        };
+        // ... their weights and dS; kPlain: every key sees them, no cap and no bias ...
+        auto weights = [&](int b, const Acc& x_in, const Acc& dp, auto plain, float (&p)[16], float (&ds)[16]) {
+            constexpr bool kPlain = decltype(plain)::value;
+            float x[16];
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
-                const Four base = *reinterpret_cast<const Four*>(&stats[buffer][0][32 * b + 8 * g + 4 * half]);
-                const Four delta = *reinterpret_cast<const Four*>(&stats[buffer][1][32 * b + 8 * g + 4 * half]);
+                const Four base = *reinterpret_cast<const Four*>(tile_base + 32 * b + 8 * g);
+                const Four delta = *reinterpret_cast<const Four*>(tile_delta + 32 * b + 8 * g);
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     p[4 * g + r] = base[r];
-                    ds[4 * g + r] = fmaf(dp[4 * g + r], into, -delta[r]);
+                    ds[4 * g + r] = kWeightShift<T> != 0.0f ? fmaf(dp[4 * g + r], into, -delta[r]) : dp[4 * g + r] - delta[r];
+                    x[4 * g + r] = x_in[4 * g + r];
                 }
             }
-            if (bend.capped) {
+            if (!kPlain && bend.capped) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     x[r] = cap_tanh<T>(x[r] * bend.cap_in);
@@ -329,12 +363,12 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 64 ? 2 : 1) void dkv_kernel(Do
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) p[r] = fmaf(x[r], bend.unit, -p[r]);
-            if (bend.biased) {
+            if (!kPlain && bend.biased) {
                 const float away = static_cast<float>(from + 32 * b + 4 * half - j);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) p[r] = fmaf(-bend.slope, fabsf(away + static_cast<float>(8 * (r / 4) + r % 4)), p[r]);
             }
-            if (!all_seen) {
+            if (!kPlain && !all_seen) {
                 const int to_low = span.low - from - 32 * b - 4 * half;
                 const unsigned width = static_cast<unsigned>(span.high - span.low);
 #pragma unroll
@@ -349,8 +383,37 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 64 ? 2 : 1) void dkv_kernel(Do
                 p[r] = __builtin_amdgcn_exp2f(p[r]);
                 ds[r] *= p[r];
             }
-            if constexpr (kDv) multiply_columns<T, kDim>(view, d_tile, b, p, dv);
-            if constexpr (kDk) multiply_columns<T, kDim>(view, q_tile, b, ds, dk);
+        };
+        // ... and their part of the sums.
+        auto add = [&](int b, const Rows16<T>& p, const Rows16<T>& ds) {
+            if constexpr (kDv) multiply_columns<T, kDim, kTile>(view, d_tile, b, p, dv);
+            if constexpr (kDk) multiply_columns<T, kDim, kTile>(view, q_tile, b, ds, dk);
+        };
+        constexpr int kBlocks = kTile / 32;
+        if (kPipelined && all_seen && !bend.capped && !bend.biased) {
+            // One wave to a SIMD: the matrix cores work on the next queries' scores and the last ones' sums while the vector
+            // unit has this one's weights.
+            Acc x[2], dp[2];
+            products(0, x[0], dp[0]);
+            float p[16], ds[16];
+            weights(0, x[0], dp[0], std::true_type{}, p, ds);
+            if constexpr (kBlocks > 1) products(1, x[1], dp[1]);
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                const Rows16<T> pb(p), dsb(ds);
+                if (b + 1 < kBlocks) weights(b + 1, x[(b + 1) & 1], dp[(b + 1) & 1], std::true_type{}, p, ds);
+                add(b, pb, dsb);
+                if (b + 2 < kBlocks) products(b + 2, x[b & 1], dp[b & 1]);
+            }
+        } else {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                Acc x, dp;
+                products(b, x, dp);
+                float p[16], ds[16];
+                weights(b, x, dp, std::false_type{}, p, ds);
+                add(b, Rows16<T>(p), Rows16<T>(ds));
+            }
         }
     }
     if (!working) return;
@@ -367,8 +430,8 @@ __global__ __launch_bounds__(kDocThreads, kDim <= 64 ? 2 : 1) void dkv_kernel(Do
     };
     if (!spoilt && mine)
         rows_of(j, [&](auto* to_dk, auto* to_dv) {
-            if constexpr (kDk) store_column<kDirect>(to_dk, a.head_dim, dk, dk_factor);
-            if constexpr (kDv) store_column<kDirect>(to_dv, a.head_dim, dv, unshift);
+            if constexpr (kDk) store_column(to_dk, a.head_dim, a.whole, dk, dk_factor);
+            if constexpr (kDv) store_column(to_dv, a.head_dim, a.whole, dv, unshift);
         });
     for (uint32_t left = static_cast<uint32_t>(__ballot(spoilt)); left; left &= left - 1) {
         const int row = wave_first + __ffs(left) - 1;
@@ -411,38 +474,39 @@ __global__ __launch_bounds__(kDocThreads) void add_heads_kernel(DocAttention a) 
     }
 }
 
-template <typename T, int kDim, bool kDirect, bool kDk, bool kDv>
+template <typename T, int kDim, bool kDk, bool kDv>
 void launch_dkv(const DocAttention& a, dim3 grid, hipStream_t s) {
     if (a.group == 1)
-        dkv_kernel<T, kDim, kDirect, false, kDk, kDv><<<grid, kDocThreads, 0, s>>>(a);
+        dkv_kernel<T, kDim, false, kDk, kDv><<<grid, kDocThreads, 0, s>>>(a);
     else
-        dkv_kernel<T, kDim, kDirect, true, kDk, kDv><<<grid, kDocThreads, 0, s>>>(a);
+        dkv_kernel<T, kDim, true, kDk, kDv><<<grid, kDocThreads, 0, s>>>(a);
 }
 
-template <typename T, int kDim, bool kDirect>
-void launch_kernels(const DocAttention& a, hipStream_t s) {
+template <typename T, int kDim>
+void launch_gradients(const DocAttention& a, hipStream_t s) {
     const dim3 grid(doc_tiles(a, kDocTileRows) * a.heads);
-    dq_kernel<T, kDim, kDirect><<<grid, kDocThreads, 0, s>>>(a);
+    dq_kernel<T, kDim><<<grid, kDocThreads, 0, s>>>(a);
     if constexpr (kDim <= kTogether) {
-        launch_dkv<T, kDim, kDirect, true, true>(a, grid, s);
+        launch_dkv<T, kDim, true, true>(a, grid, s);
     } else {
-        launch_dkv<T, kDim, kDirect, true, false>(a, grid, s);
-        launch_dkv<T, kDim, kDirect, false, true>(a, grid, s);
+        launch_dkv<T, kDim, true, false>(a, grid, s);
+        launch_dkv<T, kDim, false, true>(a, grid, s);
     }
 }
 
 template <typename T>
-int launch_document_attention_backward(const DocAttention& a, hipStream_t s) {
-    const bool direct = whole_chunks<T>(a, {a.q, a.k, a.v, a.out, a.dout, a.dq, a.dk, a.dv});
+int launch_document_attention_backward(DocAttention a, char* packed, hipStream_t s) {
+    a.whole = whole_chunks(a, kChunk<T>, {a.q, a.k, a.v, a.out, a.dout, a.dq, a.dk, a.dv});
+    set_sources<T>(a, true, packed, s);
     if (a.head_dim <= 64)
-        direct ? launch_kernels<T, 64, true>(a, s) : launch_kernels<T, 64, false>(a, s);
+        launch_gradients<T, 64>(a, s);
     else if (a.head_dim <= 128)
-        direct ? launch_kernels<T, 128, true>(a, s) : launch_kernels<T, 128, false>(a, s);
+        launch_gradients<T, 128>(a, s);
     else
-        direct ? launch_kernels<T, 256, true>(a, s) : launch_kernels<T, 256, false>(a, s);
+        launch_gradients<T, 256>(a, s);
     if (a.group > 1) {
         const dim3 grid(doc_tiles(a, kDocTileRows), 8);
-        if (direct)
+        if (a.whole)
             add_heads_kernel<T, 4><<<grid, kDocThreads, 0, s>>>(a);
         else
             add_heads_kernel<T, 1><<<grid, kDocThreads, 0, s>>>(a);

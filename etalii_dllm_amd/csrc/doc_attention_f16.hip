@@ -4,7 +4,7 @@
 
 namespace dllm_hip {
 
-template int launch_document_attention<_Float16>(const DocAttention&, void*, hipStream_t);
-template int launch_document_attention_backward<_Float16>(const DocAttention&, hipStream_t);
+template int launch_document_attention<_Float16>(DocAttention, void*, char*, hipStream_t);
+template int launch_document_attention_backward<_Float16>(DocAttention, char*, hipStream_t);
 
 }  // namespace dllm_hip

@@ -4,7 +4,7 @@
 
 namespace dllm_hip {
 
-template int launch_document_attention<float>(const DocAttention&, void*, hipStream_t);
-template int launch_document_attention_backward<float>(const DocAttention&, hipStream_t);
+template int launch_document_attention<float>(DocAttention, void*, char*, hipStream_t);
+template int launch_document_attention_backward<float>(DocAttention, char*, hipStream_t);
 
 }  // namespace dllm_hip

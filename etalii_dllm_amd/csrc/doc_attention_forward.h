@@ -9,8 +9,11 @@
 
 namespace dllm_hip {
 
+// Keys of a tile, and whether two buffers of K and V tiles fit LDS: 64 or 128 KB for 16-bit types, 96 KB for float32's planes.
 template <typename T, int kDim>
-constexpr int kKeys = kDim * sizeof(T) <= 256 ? 64 : 32;  // keys of a tile: K and V twice in at most 64 KB of LDS, or 128 KB
+constexpr int kKeys = kPlanes<T> == 1 || kDim <= 64 ? 64 : 32;
+template <typename T, int kDim>
+constexpr int kBuffers = 4 * kKeys<T, kDim> * kDim * 2 * kPlanes<T> <= 128 * 1024 ? 2 : 1;
 
 // Forward. A wave's lane owns one query (two lanes: its halves); keys go through LDS in tiles, two buffers deep.
 //
@@ -19,13 +22,15 @@ constexpr int kKeys = kDim * sizeof(T) <= 256 ? 64 : 32;  // keys of a tile: K a
 //
 // The running maximum is moved only when some query of the wave has outgrown it by 2^8: until then P stays below 2^8, which
 // float32 sums and 16-bit products hold as well as values below one.
-template <typename T, int kDim, bool kDirect>
-__global__ __launch_bounds__(kDocThreads, 2) void forward_kernel(DocAttention a, T* out) {
+template <typename T, int kDim>
+__global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1) void forward_kernel(DocAttention a, T* out) {
     using Shape = TileShape<T, kDim>;
     constexpr int kTile = kKeys<T, kDim>;
-    constexpr int kTileBytes = kTile * Shape::kRowBytes;
+    using Copy = TileCopy<T, kDim, kTile, kDocThreads>;
+    constexpr int kTileBytes = Copy::kBytes;
     constexpr int kParts = kDim / 32;
-    __shared__ __attribute__((aligned(1024))) char lds[4 * kTileBytes];  // K, V of one buffer, K, V of the other
+    constexpr bool kAhead = kBuffers<T, kDim> == 2;
+    __shared__ __attribute__((aligned(1024))) char lds[kBuffers<T, kDim> * 2 * kTileBytes];  // K, V of each buffer
 
     // the heads that share keys are 8 workgroups (or a divisor of it) apart: on the same L2
     const int turn = static_cast<int>(blockIdx.x) % a.heads;
@@ -41,8 +46,7 @@ __global__ __launch_bounds__(kDocThreads, 2) void forward_kernel(DocAttention a,
     const int i = min(wave_first + (lane & 31), doc.end - 1);
     const Span span = key_span(a, doc, i);
 
-    const Column<T, kDim, kDirect> q(static_cast<const T*>(a.q) + i * a.q_stride + static_cast<int64_t>(head) * a.head_dim,
-                                     a.head_dim);
+    const Column<T, kDim> q(a.sources[0], head, i);
 
     // keys of the workgroup: [low, high) in whole tiles of the document, and the tiles of the prefix before them
     const int low = key_span(a, doc, first).low;
@@ -53,9 +57,8 @@ __global__ __launch_bounds__(kDocThreads, 2) void forward_kernel(DocAttention a,
     const Span first_span = key_span(a, doc, wave_first), last_span = key_span(a, doc, wave_last);
     const int any_low = first_span.low, any_high = last_span.high, all_low = last_span.low, all_high = first_span.high;
 
-    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_k(a.k, a.k_stride, kv, a.head_dim);
-    const TileCopy<T, kDim, kTile, kDocThreads, kDirect> copy_v(a.v, a.v_stride, kv, a.head_dim);
-    const TileView<T, kDim> view;
+    const Copy copy_k(a.sources[1], kv), copy_v(a.sources[2], kv);
+    const TileView<T, kDim, kTile> view;
     LdsByte* const buffers = (LdsByte*)lds;
 
     const float unit = (a.softcap != 0.0f ? a.softcap : a.scale) * kLog2E;  // score of X (or of the tanh) in units of log 2
@@ -76,11 +79,16 @@ __global__ __launch_bounds__(kDocThreads, 2) void forward_kernel(DocAttention a,
         copy_v(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
     };
     int t = next_tile(-1);
-    fetch(t, 0);
-    for (int buffer = 0; t < tiles; buffer ^= 1) {
+    if (kAhead) fetch(t, 0);
+    for (int buffer = 0; t < tiles; buffer ^= kAhead) {
         tile_barrier();
         const int next = next_tile(t);
-        if (next < tiles) fetch(next, buffer ^ 1);
+        if (!kAhead) {
+            fetch(t, 0);
+            tile_barrier();
+        } else if (next < tiles) {
+            fetch(next, buffer ^ 1);
+        }
         const LdsByte* const k_tile = buffers + buffer * 2 * kTileBytes;
         const LdsByte* const v_tile = k_tile + kTileBytes;
         const int from = doc.start + t * kTile;
@@ -96,7 +104,7 @@ __global__ __launch_bounds__(kDocThreads, 2) void forward_kernel(DocAttention a,
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = 0.0f;
 #pragma unroll
-            for (int step = 0; step < Shape::kSteps; ++step) multiply(view.rows(k_tile, b, step), q[step], x);
+            for (int step = 0; step < Shape::kSteps; ++step) multiply<T>(view.rows(k_tile, b, step), q[step], x);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[b][r] = x[r];
         }
@@ -156,7 +164,7 @@ __global__ __launch_bounds__(kDocThreads, 2) void forward_kernel(DocAttention a,
             }
         l += sum;
 #pragma unroll
-        for (int b = 0; b < kTile / 32; ++b) multiply_columns<T, kDim>(view, v_tile, b, s[b], o);
+        for (int b = 0; b < kTile / 32; ++b) multiply_columns<T, kDim, kTile>(view, v_tile, b, Rows16<T>(s[b]), o);
     }
     if (!working) return;
     l += other_half(l);
@@ -166,7 +174,7 @@ __global__ __launch_bounds__(kDocThreads, 2) void forward_kernel(DocAttention a,
     bool spoilt = !(all_finite(o) && l * 0.0f == 0.0f && m * 0.0f == 0.0f);
     spoilt = (spoilt | __shfl_xor(static_cast<int>(spoilt), 32)) && wave_first + (lane & 31) < doc.end;
     if (!spoilt && wave_first + (lane & 31) < doc.end) {
-        store_column<kDirect>(out + i * a.out_stride + static_cast<int64_t>(head) * a.head_dim, a.head_dim, o, 1.0f / l);
+        store_column<T, kParts>(out + i * a.out_stride + static_cast<int64_t>(head) * a.head_dim, a.head_dim, a.whole, o, 1.0f / l);
         if (a.lse && half == 0) a.lse[static_cast<int64_t>(head) * a.tokens + i] = (m + __builtin_amdgcn_logf(l)) * kLn2;
     }
     for (uint32_t left = static_cast<uint32_t>(__ballot(spoilt)); left; left &= left - 1) {
@@ -178,25 +186,18 @@ __global__ __launch_bounds__(kDocThreads, 2) void forward_kernel(DocAttention a,
     }
 }
 
-template <typename T, int kDim>
-void launch_forward_dim(const DocAttention& a, T* out, bool direct, hipStream_t s) {
-    const dim3 grid(doc_tiles(a, kDocTileRows) * a.heads);
-    if (direct)
-        forward_kernel<T, kDim, true><<<grid, kDocThreads, 0, s>>>(a, out);
-    else
-        forward_kernel<T, kDim, false><<<grid, kDocThreads, 0, s>>>(a, out);
-}
-
 template <typename T>
-int launch_document_attention(const DocAttention& a, void* out, hipStream_t s) {
-    const bool direct = whole_chunks<T>(a, {a.q, a.k, a.v, out});
+int launch_document_attention(DocAttention a, void* out, char* packed, hipStream_t s) {
+    a.whole = whole_chunks(a, kChunk<T>, {a.q, a.k, a.v, out});
+    set_sources<T>(a, false, packed, s);
+    const dim3 grid(doc_tiles(a, kDocTileRows) * a.heads);
     T* const to = static_cast<T*>(out);
     if (a.head_dim <= 64)
-        launch_forward_dim<T, 64>(a, to, direct, s);
+        forward_kernel<T, 64><<<grid, kDocThreads, 0, s>>>(a, to);
     else if (a.head_dim <= 128)
-        launch_forward_dim<T, 128>(a, to, direct, s);
+        forward_kernel<T, 128><<<grid, kDocThreads, 0, s>>>(a, to);
     else
-        launch_forward_dim<T, 256>(a, to, direct, s);
+        forward_kernel<T, 256><<<grid, kDocThreads, 0, s>>>(a, to);
     return check_launch("document_attention");
 }
 

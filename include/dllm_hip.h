@@ -267,8 +267,9 @@ int dllm_hip_lora_adapter_gradients(const float* grad, const float* a, const flo
  *
  * The parts of a decoder layer around its matmuls for batches that the reference does not have: several documents packed
  * into one row of tokens, images among the text, activations in bfloat16 or float16. They have no counterpart in the
- * reference, so no bits to reproduce: sums, softmax statistics and norms are float32 (float32 activations: float32
- * products too), and each result is rounded to its type once. They keep the library's other promise: results do not
+ * reference, so no bits to reproduce: sums, softmax statistics and norms are float32, products of float32 activations are
+ * float32's to its last bits, those of 16-bit activations have their operands in that type, and each result is rounded to
+ * its type once. They keep the library's other promise: results do not
  * depend on what shares the batch. A document's attention, a token's rotation and a row's norm are the same bits
  * alone and in any pack, and every call with the same arguments gives the same bits (no atomic additions). Sums over all rows
  * (the gradients of norm weights and channel gates) depend on the rows alone.
@@ -283,7 +284,7 @@ enum { DLLM_HIP_FLOAT32 = 0, DLLM_HIP_BFLOAT16 = 1, DLLM_HIP_FLOAT16 = 2 };
 /* Attention within packed documents. q[tokens, heads, head_dim], k and v[tokens, kv_heads, head_dim], out like q;
  * token strides in elements (0: heads * head_dim), so q, k and v may be parts of one projection's output. Document d is
  * tokens offsets[d] .. offsets[d + 1] - 1 (device, documents + 1 values, non-decreasing, in [0, tokens]; empty documents
- * are allowed). Tokens of no document are neither read nor written. A query at position i of its document sees the key
+ * are allowed). Tokens of no document count for nothing, and their rows of the outputs are left as they were. A query at position i of its document sees the key
  * at position j of the same document if
  *     (j <= i or not causal) and (|i - j| < window or window is 0),   or   j < prefix[d]
  * (prefix: device, one length per document, NULL for none: an instruction or image that every token sees). The score is
