@@ -25,6 +25,10 @@ constexpr int kStream = kPlanes<T> == 1 || kDim <= 64 ? 64 : 32;
 template <typename T, int kDim>
 constexpr int kStreamBuffers = 4 * kStream<T, kDim> * kDim * 2 * kPlanes<T> <= 128 * 1024 ? 2 : 1;
 
+// Whether a lane holds its rows: not where two of them are 192 registers each (wide float32 heads).
+template <typename T, int kDim>
+constexpr bool kBothHeld = kDim * kPlanes<T> <= 384;
+
 constexpr int kTogether = 128;
 
 // float16 loses weights below 2^-14 bit by bit, and upstream gradients have any size: p is held times 2^8, and dout relative
@@ -81,7 +85,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     const Span span = key_span(a, doc, i);
     const int64_t head_at = static_cast<int64_t>(head) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens + i;
 
-    const Column<T, kDim> q(a.sources[0], head, i), dout(a.sources[3], head, i);
+    const Column<T, kDim, kBothHeld<T, kDim>> q(a.sources[0], head, i), dout(a.sources[3], head, i);
     float delta = 0.0f, norm = 0.0f;  // this half's part
     {
         const T* const out_row = static_cast<const T*>(a.out) + i * a.out_stride + head_at;
@@ -162,10 +166,8 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
             Acc x, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
-#pragma unroll
-            for (int step = 0; step < Shape::kSteps; ++step) multiply<T>(view.rows(k_tile, b, step), q[step], x);
-#pragma unroll
-            for (int step = 0; step < Shape::kSteps; ++step) multiply<T>(view.rows(v_tile, b, step), dout[step], dp);
+            multiply_rows(view, k_tile, b, q, x);
+            multiply_rows(view, v_tile, b, dout, dp);
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] = fmaf(dp[r], into, -delta * into);
@@ -248,7 +250,8 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     const Span span = query_span(a, doc, j);
     const int64_t kv_at = static_cast<int64_t>(kv) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens;
 
-    const Column<T, kDim> k(a.sources[1], kv, j), v(a.sources[2], kv, j);
+    const Column<T, kDim, kBothHeld<T, kDim> || !kDk> k(a.sources[1], kv, j);
+    const Column<T, kDim, kBothHeld<T, kDim>> v(a.sources[2], kv, j);
 
     // the queries that see any key of the workgroup; keys in the prefix are seen from the document's start on
     const int last = min(first + kDocTileRows, doc.end) - 1;
@@ -333,11 +336,8 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
         auto products = [&](int b, Acc& x, Acc& dp) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
-#pragma unroll
-            for (int step = 0; step < Shape::kSteps; ++step) {
-                multiply<T>(view.rows(q_tile, b, step), k[step], x);
-                if constexpr (kDk) multiply<T>(view.rows(d_tile, b, step), v[step], dp);
-            }
+            multiply_rows(view, q_tile, b, k, x);
+            if constexpr (kDk) multiply_rows(view, d_tile, b, v, dp);
         };
         // ... their weights and dS; kPlain: every key sees them, no cap and no bias ...
         auto weights = [&](int b, const Acc& x_in, const Acc& dp, auto plain, float (&p)[16], float (&ds)[16]) {

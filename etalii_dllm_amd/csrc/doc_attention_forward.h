@@ -103,8 +103,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
             Acc x;
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = 0.0f;
-#pragma unroll
-            for (int step = 0; step < Shape::kSteps; ++step) multiply<T>(view.rows(k_tile, b, step), q[step], x);
+            multiply_rows(view, k_tile, b, q, x);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[b][r] = x[r];
         }

@@ -249,11 +249,10 @@ __device__ __forceinline__ void multiply_columns(const TileView<T, kDim, kRows>&
 }
 
 // A lane's own row, the B operand of products along head_dim: chunk pair `step`'s chunk of its half, zero past the head. Held
-// in registers, or read again at each use where it would take more than 96 of them (the row stays in the caches).
-template <typename T, int kDim>
+// in registers, or (kHeld false: where two rows and the sums are more than the registers) read again for every product.
+template <typename T, int kDim, bool kHeld = true>
 struct Column {
     static constexpr int kSteps = TileShape<T, kDim>::kSteps;
-    static constexpr bool kHeld = kSteps * 4 * kPlanes<T> <= 96;
     const char* row;
     int64_t plane;
     int chunks;
@@ -275,11 +274,31 @@ struct Column {
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) held[i] = read(i);
     }
-    __device__ __forceinline__ Chunks<T> operator[](int step) const {
-        if constexpr (kHeld) return held[step];
-        return read(step);
-    }
 };
+
+// acc += (rows 32 block .. of a tile) column
+template <typename T, int kDim, int kRows, bool kHeld>
+__device__ __forceinline__ void multiply_rows(const TileView<T, kDim, kRows>& view, const LdsByte* tile, int block,
+                                              const Column<T, kDim, kHeld>& column, Acc& acc) {
+    constexpr int kSteps = TileShape<T, kDim>::kSteps;
+    if constexpr (kHeld) {
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) multiply<T>(view.rows(tile, block, step), column.held[step], acc);
+    } else {
+        // from the caches, kAhead steps before their use
+        constexpr int kAhead = 4;
+        Chunks<T> next[kAhead];
+#pragma unroll
+        for (int step = 0; step < kAhead; ++step) next[step] = column.read(step);
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+            const Chunks<T> now = next[step % kAhead];
+            if (step + kAhead < kSteps) next[step % kAhead] = column.read(step + kAhead);
+            multiply<T>(view.rows(tile, block, step), now, acc);
+            __builtin_amdgcn_sched_barrier(0);  // the loads stay where they are
+        }
+    }
+}
 
 // The other half's value for the same column.
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
