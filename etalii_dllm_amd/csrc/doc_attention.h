@@ -14,7 +14,7 @@
 namespace dllm_hip {
 
 constexpr int kDocThreads = 256;
-constexpr int kDocTileRows = 128;  // tokens of a workgroup, 32 for each wave
+constexpr int kDocTileRows = 128;  // tokens of a workgroup, 32 for each wave (64 of wide float32 heads)
 constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DocAttention {

@@ -25,10 +25,6 @@ constexpr int kStream = kPlanes<T> == 1 || kDim <= 64 ? 64 : 32;
 template <typename T, int kDim>
 constexpr int kStreamBuffers = 4 * kStream<T, kDim> * kDim * 2 * kPlanes<T> <= 128 * 1024 ? 2 : 1;
 
-// Whether a lane holds its rows: not where two of them are 192 registers each (wide float32 heads).
-template <typename T, int kDim>
-constexpr bool kBothHeld = kDim * kPlanes<T> <= 384;
-
 constexpr int kTogether = 128;
 
 // float16 loses weights below 2^-14 bit by bit, and upstream gradients have any size: p is held times 2^8, and dout relative
@@ -66,26 +62,29 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     constexpr int kTile = kStream<T, kDim>;
     using Copy = TileCopy<T, kDim, kTile, kDocThreads>;
     constexpr int kTileBytes = Copy::kBytes;
-    constexpr int kParts = kDim / 32;
+    constexpr bool kPaired = kPair<T, kDim> == 2;
+    constexpr int kParts = kWaveDim<T, kDim> / 32, kOwn = kBlockRows<T, kDim>;
     constexpr bool kAhead = kStreamBuffers<T, kDim> == 2;
     __shared__ __attribute__((aligned(1024))) char lds[kStreamBuffers<T, kDim> * 2 * kTileBytes];
+    __shared__ __attribute__((aligned(16))) char pair_lds[kPaired ? 2 * 4 * 4096 : 16];
 
     const int turn = static_cast<int>(blockIdx.x) % a.heads;
     const int head = (turn % a.kv_heads) * a.group + turn / a.kv_heads;
     const int kv = head / a.group;
     Document doc;
     int first;
-    if (!locate_tile<kDocTileRows, true>(a, blockIdx.x / a.heads, doc, first)) return;
+    if (!locate_tile<kOwn, true>(a, blockIdx.x / a.heads, doc, first)) return;
 
     const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
-    const int wave_first = first + 32 * wave, wave_last = min(wave_first + 31, doc.end - 1);
+    const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
+    const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
     const bool working = wave_first < doc.end;
     const bool mine = wave_first + (lane & 31) < doc.end;
     const int i = min(wave_first + (lane & 31), doc.end - 1);
     const Span span = key_span(a, doc, i);
     const int64_t head_at = static_cast<int64_t>(head) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens + i;
 
-    const Column<T, kDim, kBothHeld<T, kDim>> q(a.sources[0], head, i), dout(a.sources[3], head, i);
+    const Column<T, kDim> q(a.sources[0], head, i, part), dout(a.sources[3], head, i, part);
     float delta = 0.0f, norm = 0.0f;  // this half's part
     {
         const T* const out_row = static_cast<const T*>(a.out) + i * a.out_stride + head_at;
@@ -114,13 +113,13 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     if constexpr (kWeightShift<T> != 0.0f) {
         norm = sqrtf(norm + other_half(norm));
         dout_scale = power_of_two_above(norm);
-        if (mine && half == 0) a.dout_norm[stat_at] = norm;
+        if (mine && half == 0 && part == 0) a.dout_norm[stat_at] = norm;
     }
-    if (mine && half == 0) a.delta[stat_at] = delta;
+    if (mine && half == 0 && part == 0) a.delta[stat_at] = delta;
     const float into = 1.0f / dout_scale;  // exact
 
     const int low = key_span(a, doc, first).low;
-    const int high = max(key_span(a, doc, min(first + kDocTileRows, doc.end) - 1).high, doc.prefix_end);
+    const int high = max(key_span(a, doc, min(first + kOwn, doc.end) - 1).high, doc.prefix_end);
     const int low_tile = (low - doc.start) / kTile, prefix_tiles = (doc.prefix_end - doc.start + kTile - 1) / kTile;
     const int tiles = (high - doc.start + kTile - 1) / kTile;
     const Span first_span = key_span(a, doc, wave_first), last_span = key_span(a, doc, wave_last);
@@ -159,15 +158,23 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
         const LdsByte* const v_tile = k_tile + kTileBytes;
         const int from = doc.start + t * kTile;
         t = next;
-        if (!working || !((from < any_high && from + kTile > any_low) || from < doc.prefix_end)) continue;
+        const bool idle = !working || !((from < any_high && from + kTile > any_low) || from < doc.prefix_end);
+        if (!kPaired && idle) continue;
         const bool all_seen = (from >= all_low && from + kTile <= all_high) || from + kTile <= doc.prefix_end;
 #pragma unroll
         for (int b = 0; b < kTile / 32; ++b) {
             Acc x, dp;
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
-            multiply_rows(view, k_tile, b, q, x);
-            multiply_rows(view, v_tile, b, dout, dp);
+            if (!kPaired || !idle) {
+                multiply_rows(view, k_tile, b, q, part, x);
+                multiply_rows(view, v_tile, b, dout, part, dp);
+            }
+            if constexpr (kPaired) {
+                static_assert(kTile == 32);
+                exchange({&x, &dp}, (LdsByte*)pair_lds);
+                if (idle) continue;
+            }
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] = fmaf(dp[r], into, -delta * into);
@@ -200,16 +207,17 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
                     ds[r] = see ? ds[r] : 0.0f;
                 }
             }
-            multiply_columns<T, kDim, kTile>(view, k_tile, b, Rows16<T>(ds), dq);
+            multiply_columns<T, kDim, kTile>(view, k_tile, b, Rows16<T>(ds), first_part, dq);
         }
     }
-    if (!working) return;
-    bool spoilt = !all_finite(dq);
-    spoilt = (spoilt | __shfl_xor(static_cast<int>(spoilt), 32)) && mine;
+    if (!kPaired && !working) return;
+    const uint64_t marks = __ballot(!all_finite(dq) && mine);
+    uint32_t spoilt = static_cast<uint32_t>(marks) | static_cast<uint32_t>(marks >> 32);
+    if constexpr (kPaired) spoilt = pair_marks(spoilt, (LdsByte*)pair_lds);
     T* const to = static_cast<T*>(a.dq) + head_at;
-    if (!spoilt && mine)
-        store_column<T, kParts>(to + i * a.q_stride, a.head_dim, a.whole, dq, a.scale * dout_scale * __builtin_amdgcn_exp2f(-kWeightShift<T>));
-    for (uint32_t left = static_cast<uint32_t>(__ballot(spoilt)); left; left &= left - 1) {
+    if (mine && !(spoilt >> (lane & 31) & 1))
+        store_column(to + i * a.q_stride, a.head_dim, a.whole, first_part, dq, a.scale * dout_scale * __builtin_amdgcn_exp2f(-kWeightShift<T>));
+    for (uint32_t left = part == 0 ? spoilt : 0; left; left &= left - 1) {
         const int from_lane = __ffs(left) - 1, row = wave_first + from_lane;
         float value[kLaneDims];
         attention_row_dq<T>(a, doc, head, row, __shfl(delta, from_lane), value);
@@ -229,32 +237,34 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     constexpr int kTile = kPipelined ? 128 : kStream<T, kDim>;
     using Copy = TileCopy<T, kDim, kTile, kDocThreads>;
     constexpr int kTileBytes = Copy::kBytes;
-    constexpr int kParts = kDim / 32;
+    constexpr bool kPaired = kPair<T, kDim> == 2;
+    constexpr int kParts = kWaveDim<T, kDim> / 32, kOwn = kBlockRows<T, kDim>;
     constexpr bool kAhead = kStreamBuffers<T, kDim> == 2;
     __shared__ __attribute__((aligned(1024))) char lds[(kAhead ? 4 : 2) * kTileBytes];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // lse in units of log 2, and dout . out, of a tile's queries
     __shared__ float largest[kDocThreads / 64];
+    __shared__ __attribute__((aligned(16))) char pair_lds[kPaired ? 2 * 4 * 4096 : 16];
 
     const int turn = static_cast<int>(blockIdx.x) % a.heads;
     const int head = (turn % a.kv_heads) * a.group + turn / a.kv_heads;
     const int kv = head / a.group;
     Document doc;
     int first;
-    if (!locate_tile<kDocTileRows, false>(a, blockIdx.x / a.heads, doc, first)) return;
+    if (!locate_tile<kOwn, false>(a, blockIdx.x / a.heads, doc, first)) return;
 
     const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
-    const int wave_first = first + 32 * wave, wave_last = min(wave_first + 31, doc.end - 1);
+    const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
+    const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
     const bool working = wave_first < doc.end;
     const bool mine = wave_first + (lane & 31) < doc.end;
     const int j = min(wave_first + (lane & 31), doc.end - 1);
     const Span span = query_span(a, doc, j);
     const int64_t kv_at = static_cast<int64_t>(kv) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens;
 
-    const Column<T, kDim, kBothHeld<T, kDim> || !kDk> k(a.sources[1], kv, j);
-    const Column<T, kDim, kBothHeld<T, kDim>> v(a.sources[2], kv, j);
+    const Column<T, kDim> k(a.sources[1], kv, j, part), v(a.sources[2], kv, j, part);
 
     // the queries that see any key of the workgroup; keys in the prefix are seen from the document's start on
-    const int last = min(first + kDocTileRows, doc.end) - 1;
+    const int last = min(first + kOwn, doc.end) - 1;
     const int low = query_span(a, doc, first).low;
     const int high = max(query_span(a, doc, first).high, query_span(a, doc, last).high);
     const int low_tile = (low - doc.start) / kTile, tiles = (high - doc.start + kTile - 1) / kTile;
@@ -326,7 +336,8 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
         const LdsByte* const q_tile = buffers + buffer * 2 * kTileBytes;
         const LdsByte* const d_tile = q_tile + kTileBytes;
         const int from = doc.start + t * kTile;
-        if (!working || !(from < any_high && from + kTile > any_low)) continue;
+        const bool idle = !working || !(from < any_high && from + kTile > any_low);
+        if (!kPaired && idle) continue;
         const bool all_seen = from >= all_low && from + kTile <= all_high;
         const float* const tile_base = &stats[buffer][0][4 * half];
         const float* const tile_delta = &stats[buffer][1][4 * half];
@@ -336,8 +347,8 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
         auto products = [&](int b, Acc& x, Acc& dp) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) x[r] = dp[r] = 0.0f;
-            multiply_rows(view, q_tile, b, k, x);
-            if constexpr (kDk) multiply_rows(view, d_tile, b, v, dp);
+            multiply_rows(view, q_tile, b, k, part, x);
+            if constexpr (kDk) multiply_rows(view, d_tile, b, v, part, dp);
         };
         // ... their weights and dS; kPlain: every key sees them, no cap and no bias ...
         auto weights = [&](int b, const Acc& x_in, const Acc& dp, auto plain, float (&p)[16], float (&ds)[16]) {
@@ -386,8 +397,8 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
         };
         // ... and their part of the sums.
         auto add = [&](int b, const Rows16<T>& p, const Rows16<T>& ds) {
-            if constexpr (kDv) multiply_columns<T, kDim, kTile>(view, d_tile, b, p, dv);
-            if constexpr (kDk) multiply_columns<T, kDim, kTile>(view, q_tile, b, ds, dk);
+            if constexpr (kDv) multiply_columns<T, kDim, kTile>(view, d_tile, b, p, first_part, dv);
+            if constexpr (kDk) multiply_columns<T, kDim, kTile>(view, q_tile, b, ds, first_part, dk);
         };
         constexpr int kBlocks = kTile / 32;
         if (kPipelined && all_seen && !bend.capped && !bend.biased) {
@@ -408,18 +419,27 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
         } else {
 #pragma unroll
             for (int b = 0; b < kBlocks; ++b) {
-                Acc x, dp;
-                products(b, x, dp);
+                Acc x{}, dp{};
+                if (!kPaired || !idle) products(b, x, dp);
+                if constexpr (kPaired) {
+                    static_assert(kBlocks == 1);
+                    if constexpr (kDk)
+                        exchange({&x, &dp}, (LdsByte*)pair_lds);
+                    else
+                        exchange({&x}, (LdsByte*)pair_lds);
+                    if (idle) continue;
+                }
                 float p[16], ds[16];
                 weights(b, x, dp, std::false_type{}, p, ds);
                 add(b, Rows16<T>(p), Rows16<T>(ds));
             }
         }
     }
-    if (!working) return;
+    if (!kPaired && !working) return;
     const float unshift = __builtin_amdgcn_exp2f(-kWeightShift<T>), dk_factor = a.scale * dout_scale * unshift;
-    bool spoilt = !(all_finite(dk) && all_finite(dv));
-    spoilt = (spoilt | __shfl_xor(static_cast<int>(spoilt), 32)) && mine;
+    const uint64_t marks = __ballot(!(all_finite(dk) && all_finite(dv)) && mine);
+    uint32_t spoilt = static_cast<uint32_t>(marks) | static_cast<uint32_t>(marks >> 32);
+    if constexpr (kPaired) spoilt = pair_marks(spoilt, (LdsByte*)pair_lds);
     // row `at` of dk and dv, by `store` of its place and its factor
     auto rows_of = [&](int64_t at, auto&& store) {
         const int64_t part = (stat_at + at) * a.head_dim;
@@ -428,12 +448,12 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
         else
             store(static_cast<T*>(a.dk) + at * a.k_stride + kv_at, static_cast<T*>(a.dv) + at * a.v_stride + kv_at);
     };
-    if (!spoilt && mine)
+    if (mine && !(spoilt >> (lane & 31) & 1))
         rows_of(j, [&](auto* to_dk, auto* to_dv) {
-            if constexpr (kDk) store_column(to_dk, a.head_dim, a.whole, dk, dk_factor);
-            if constexpr (kDv) store_column(to_dv, a.head_dim, a.whole, dv, unshift);
+            if constexpr (kDk) store_column(to_dk, a.head_dim, a.whole, first_part, dk, dk_factor);
+            if constexpr (kDv) store_column(to_dv, a.head_dim, a.whole, first_part, dv, unshift);
         });
-    for (uint32_t left = static_cast<uint32_t>(__ballot(spoilt)); left; left &= left - 1) {
+    for (uint32_t left = part == 0 ? spoilt : 0; left; left &= left - 1) {
         const int row = wave_first + __ffs(left) - 1;
         float dk1[kLaneDims], dv1[kLaneDims];
         attention_row_dkv<T>(a, doc, head, row, dk1, dv1);
@@ -484,9 +504,9 @@ void launch_dkv(const DocAttention& a, dim3 grid, hipStream_t s) {
 
 template <typename T, int kDim>
 void launch_gradients(const DocAttention& a, hipStream_t s) {
-    const dim3 grid(doc_tiles(a, kDocTileRows) * a.heads);
+    const dim3 grid(doc_tiles(a, kBlockRows<T, kDim>) * a.heads);
     dq_kernel<T, kDim><<<grid, kDocThreads, 0, s>>>(a);
-    if constexpr (kDim <= kTogether) {
+    if constexpr (kWaveDim<T, kDim> <= kTogether) {
         launch_dkv<T, kDim, true, true>(a, grid, s);
     } else {
         launch_dkv<T, kDim, true, false>(a, grid, s);

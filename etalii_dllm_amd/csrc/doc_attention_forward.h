@@ -28,9 +28,11 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     constexpr int kTile = kKeys<T, kDim>;
     using Copy = TileCopy<T, kDim, kTile, kDocThreads>;
     constexpr int kTileBytes = Copy::kBytes;
-    constexpr int kParts = kDim / 32;
+    constexpr bool kPaired = kPair<T, kDim> == 2;
+    constexpr int kParts = kWaveDim<T, kDim> / 32, kOwn = kBlockRows<T, kDim>;
     constexpr bool kAhead = kBuffers<T, kDim> == 2;
     __shared__ __attribute__((aligned(1024))) char lds[kBuffers<T, kDim> * 2 * kTileBytes];  // K, V of each buffer
+    __shared__ __attribute__((aligned(16))) char pair_lds[kPaired ? kTile / 32 * 4 * 4096 : 16];
 
     // the heads that share keys are 8 workgroups (or a divisor of it) apart: on the same L2
     const int turn = static_cast<int>(blockIdx.x) % a.heads;
@@ -38,19 +40,20 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     const int kv = head / a.group;
     Document doc;
     int first;
-    if (!locate_tile<kDocTileRows, true>(a, blockIdx.x / a.heads, doc, first)) return;
+    if (!locate_tile<kOwn, true>(a, blockIdx.x / a.heads, doc, first)) return;
 
     const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
-    const int wave_first = first + 32 * wave, wave_last = min(wave_first + 31, doc.end - 1);
+    const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
+    const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
     const bool working = wave_first < doc.end;
     const int i = min(wave_first + (lane & 31), doc.end - 1);
     const Span span = key_span(a, doc, i);
 
-    const Column<T, kDim> q(a.sources[0], head, i);
+    const Column<T, kDim> q(a.sources[0], head, i, part);
 
     // keys of the workgroup: [low, high) in whole tiles of the document, and the tiles of the prefix before them
     const int low = key_span(a, doc, first).low;
-    const int high = max(key_span(a, doc, min(first + kDocTileRows, doc.end) - 1).high, doc.prefix_end);
+    const int high = max(key_span(a, doc, min(first + kOwn, doc.end) - 1).high, doc.prefix_end);
     const int low_tile = (low - doc.start) / kTile, prefix_tiles = (doc.prefix_end - doc.start + kTile - 1) / kTile;
     const int tiles = (high - doc.start + kTile - 1) / kTile;
     // the wave's: keys that all its queries see, and that any sees
@@ -94,19 +97,27 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
         const int from = doc.start + t * kTile;
         t = next;
         const bool in_prefix = from < doc.prefix_end;
-        if (!working || !((from < any_high && from + kTile > any_low) || in_prefix)) continue;
+        const bool idle = !working || !((from < any_high && from + kTile > any_low) || in_prefix);
+        if (!kPaired && idle) continue;
         const bool all_seen = (from >= all_low && from + kTile <= all_high) || from + kTile <= doc.prefix_end;
 
-        float s[kTile / 32][16];
+        Acc x[kTile / 32];
 #pragma unroll
         for (int b = 0; b < kTile / 32; ++b) {
-            Acc x;
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x[r] = 0.0f;
-            multiply_rows(view, k_tile, b, q, x);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[b][r] = x[r];
+            for (int r = 0; r < 16; ++r) x[b][r] = 0.0f;
+            if (!kPaired || !idle) multiply_rows(view, k_tile, b, q, part, x[b]);
         }
+        if constexpr (kPaired) {
+            static_assert(kTile == 32);
+            exchange({&x[0]}, (LdsByte*)pair_lds);
+            if (idle) continue;
+        }
+        float s[kTile / 32][16];
+#pragma unroll
+        for (int b = 0; b < kTile / 32; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = x[b][r];
         float times = unit;
         if (a.softcap != 0.0f) {
 #pragma unroll
@@ -163,20 +174,23 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
             }
         l += sum;
 #pragma unroll
-        for (int b = 0; b < kTile / 32; ++b) multiply_columns<T, kDim, kTile>(view, v_tile, b, Rows16<T>(s[b]), o);
+        for (int b = 0; b < kTile / 32; ++b) multiply_columns<T, kDim, kTile>(view, v_tile, b, Rows16<T>(s[b]), first_part, o);
     }
-    if (!working) return;
+    if (!kPaired && !working) return;
     l += other_half(l);
 
     // A hidden key counts as zero times its value: where that is infinite or NaN, the row is computed again from the keys
     // that it sees alone.
-    bool spoilt = !(all_finite(o) && l * 0.0f == 0.0f && m * 0.0f == 0.0f);
-    spoilt = (spoilt | __shfl_xor(static_cast<int>(spoilt), 32)) && wave_first + (lane & 31) < doc.end;
-    if (!spoilt && wave_first + (lane & 31) < doc.end) {
-        store_column<T, kParts>(out + i * a.out_stride + static_cast<int64_t>(head) * a.head_dim, a.head_dim, a.whole, o, 1.0f / l);
-        if (a.lse && half == 0) a.lse[static_cast<int64_t>(head) * a.tokens + i] = (m + __builtin_amdgcn_logf(l)) * kLn2;
+    const bool mine = wave_first + (lane & 31) < doc.end;
+    const bool finite = all_finite(o) && l * 0.0f == 0.0f && m * 0.0f == 0.0f;
+    const uint64_t marks = __ballot(!finite && mine);
+    uint32_t spoilt = static_cast<uint32_t>(marks) | static_cast<uint32_t>(marks >> 32);
+    if constexpr (kPaired) spoilt = pair_marks(spoilt, (LdsByte*)pair_lds);
+    if (mine && !(spoilt >> (lane & 31) & 1)) {
+        store_column(out + i * a.out_stride + static_cast<int64_t>(head) * a.head_dim, a.head_dim, a.whole, first_part, o, 1.0f / l);
+        if (a.lse && half == 0 && part == 0) a.lse[static_cast<int64_t>(head) * a.tokens + i] = (m + __builtin_amdgcn_logf(l)) * kLn2;
     }
-    for (uint32_t left = static_cast<uint32_t>(__ballot(spoilt)); left; left &= left - 1) {
+    for (uint32_t left = part == 0 ? spoilt : 0; left; left &= left - 1) {
         const int row = wave_first + __ffs(left) - 1;
         float value[kLaneDims], lse;
         attention_row<T>(a, doc, head, row, value, lse);
@@ -185,18 +199,22 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     }
 }
 
+template <typename T, int kDim>
+void launch_forward(const DocAttention& a, T* out, hipStream_t s) {
+    forward_kernel<T, kDim><<<doc_tiles(a, kBlockRows<T, kDim>) * a.heads, kDocThreads, 0, s>>>(a, out);
+}
+
 template <typename T>
 int launch_document_attention(DocAttention a, void* out, char* packed, hipStream_t s) {
     a.whole = whole_chunks(a, kChunk<T>, {a.q, a.k, a.v, out});
     set_sources<T>(a, false, packed, s);
-    const dim3 grid(doc_tiles(a, kDocTileRows) * a.heads);
     T* const to = static_cast<T*>(out);
     if (a.head_dim <= 64)
-        forward_kernel<T, 64><<<grid, kDocThreads, 0, s>>>(a, to);
+        launch_forward<T, 64>(a, to, s);
     else if (a.head_dim <= 128)
-        forward_kernel<T, 128><<<grid, kDocThreads, 0, s>>>(a, to);
+        launch_forward<T, 128>(a, to, s);
     else
-        forward_kernel<T, 256><<<grid, kDocThreads, 0, s>>>(a, to);
+        launch_forward<T, 256>(a, to, s);
     return check_launch("document_attention");
 }
 

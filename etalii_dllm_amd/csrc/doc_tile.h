@@ -238,81 +238,104 @@ struct Rows16 {
     }
 };
 
-// acc += (tile's rows, 32 of them from 32 block, as columns 32 part ..)^T x
+// acc += (tile's rows, 32 of them from 32 block, as columns 32 (first + 0 .. kParts - 1) ..)^T x
 template <typename T, int kDim, int kRows, int kParts>
 __device__ __forceinline__ void multiply_columns(const TileView<T, kDim, kRows>& view, const LdsByte* tile, int block,
-                                                 const Rows16<T>& x, Acc (&acc)[kParts]) {
+                                                 const Rows16<T>& x, int first, Acc (&acc)[kParts]) {
 #pragma unroll
     for (int g = 0; g < 2; ++g)
 #pragma unroll
-        for (int p = 0; p < kParts; ++p) multiply<T>(view.columns(tile, block, g, p), x.group[g], acc[p]);
+        for (int p = 0; p < kParts; ++p)
+            multiply<T>(view.columns(tile, block, g, kParts * 32 == kDim ? p : first + p), x.group[g], acc[p]);
 }
 
-// A lane's own row, the B operand of products along head_dim: chunk pair `step`'s chunk of its half, zero past the head. Held
-// in registers, or (kHeld false: where two rows and the sums are more than the registers) read again for every product.
-template <typename T, int kDim, bool kHeld = true>
-struct Column {
-    static constexpr int kSteps = TileShape<T, kDim>::kSteps;
-    const char* row;
-    int64_t plane;
-    int chunks;
-    Chunks<T> held[kHeld ? kSteps : 1];
+// Wide float32 heads: a lane's rows and sums in three planes are more than the registers, so a pair of waves shares 32 rows
+// and takes half of the head's dimensions each. Both then need the sums over all of them: see exchange().
+template <typename T, int kDim>
+constexpr int kPair = kPlanes<T> * kDim > 384 ? 2 : 1;
+template <typename T, int kDim>
+constexpr int kWaveDim = kDim / kPair<T, kDim>;
+template <typename T, int kDim>
+constexpr int kBlockRows = 128 / kPair<T, kDim>;  // of a workgroup's own, 32 for each wave or pair
 
-    __device__ __forceinline__ Chunks<T> read(int step) const {
-        const int chunk = 2 * step + ((static_cast<int>(threadIdx.x) >> 5) & 1);
-        Chunks<T> c;
+// A lane's own row, the B operand of products along head_dim: each chunk pair's chunk of its half, zero past the head; of a
+// wave's part of the dimensions.
+template <typename T, int kDim>
+struct Column {
+    static constexpr int kSteps = kWaveDim<T, kDim> / 16;
+    Chunks<T> held[kSteps];
+    __device__ __forceinline__ Column(const Source& s, int head, int64_t token, int part) {
+        const char* const row = s.base + token * s.stride + head * s.head;
 #pragma unroll
-        for (int p = 0; p < kPlanes<T>; ++p) {
-            c.c[p] = Chunk16{};
-            if (chunk < chunks) c.c[p] = *reinterpret_cast<const Chunk16*>(row + p * plane + chunk * 16);
+        for (int i = 0; i < kSteps; ++i) {
+            const int chunk = 2 * (i + part * kSteps) + ((static_cast<int>(threadIdx.x) >> 5) & 1);
+#pragma unroll
+            for (int p = 0; p < kPlanes<T>; ++p) {
+                held[i].c[p] = Chunk16{};
+                if (chunk < s.chunks) held[i].c[p] = *reinterpret_cast<const Chunk16*>(row + p * s.plane + chunk * 16);
+            }
         }
-        return c;
-    }
-    __device__ __forceinline__ Column(const Source& s, int head, int64_t token)
-        : row(s.base + token * s.stride + head * s.head), plane(s.plane), chunks(s.chunks) {
-        if constexpr (kHeld)
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) held[i] = read(i);
     }
 };
 
-// acc += (rows 32 block .. of a tile) column
-template <typename T, int kDim, int kRows, bool kHeld>
+// acc += (rows 32 block .. of a tile) column, over the wave's part of the dimensions
+template <typename T, int kDim, int kRows>
 __device__ __forceinline__ void multiply_rows(const TileView<T, kDim, kRows>& view, const LdsByte* tile, int block,
-                                              const Column<T, kDim, kHeld>& column, Acc& acc) {
-    constexpr int kSteps = TileShape<T, kDim>::kSteps;
-    if constexpr (kHeld) {
+                                              const Column<T, kDim>& column, int part, Acc& acc) {
+    constexpr int kSteps = Column<T, kDim>::kSteps;
 #pragma unroll
-        for (int step = 0; step < kSteps; ++step) multiply<T>(view.rows(tile, block, step), column.held[step], acc);
-    } else {
-        // from the caches, kAhead steps before their use
-        constexpr int kAhead = 4;
-        Chunks<T> next[kAhead];
+    for (int step = 0; step < kSteps; ++step)
+        multiply<T>(view.rows(tile, block, kPair<T, kDim> == 1 ? step : step + part * kSteps), column.held[step], acc);
+}
+
+// The pair's sums: each wave leaves its own in LDS (4 KB for each 32 x 32), and after the barrier adds the other's. All waves
+// of the workgroup come here. area: kCount * 4 KB for each wave; the next exchange comes after another barrier.
+template <int kCount>
+__device__ __forceinline__ void exchange(Acc* const (&x)[kCount], LdsByte* area) {
+    using Four = float __attribute__((ext_vector_type(4)));
+    using LdsFour = __attribute__((address_space(3))) Four;
+    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63;
+    LdsFour* const mine = (LdsFour*)(area + wave * kCount * 4096) + lane;
+    LdsFour* const other = (LdsFour*)(area + (wave ^ 1) * kCount * 4096) + lane;
 #pragma unroll
-        for (int step = 0; step < kAhead; ++step) next[step] = column.read(step);
+    for (int c = 0; c < kCount; ++c)
 #pragma unroll
-        for (int step = 0; step < kSteps; ++step) {
-            const Chunks<T> now = next[step % kAhead];
-            if (step + kAhead < kSteps) next[step % kAhead] = column.read(step + kAhead);
-            multiply<T>(view.rows(tile, block, step), now, acc);
-            __builtin_amdgcn_sched_barrier(0);  // the loads stay where they are
+        for (int g = 0; g < 4; ++g) mine[(4 * c + g) * 64] = Four{(*x[c])[4 * g], (*x[c])[4 * g + 1], (*x[c])[4 * g + 2], (*x[c])[4 * g + 3]};
+    lds_barrier();
+#pragma unroll
+    for (int c = 0; c < kCount; ++c)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const Four v = other[(4 * c + g) * 64];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) (*x[c])[4 * g + r] += v[r];
         }
-    }
+}
+
+// Which of a wave's rows either wave of the pair has marked. All waves of the workgroup come here.
+__device__ __forceinline__ uint32_t pair_marks(uint32_t marks, LdsByte* area) {
+    using LdsWord = __attribute__((address_space(3))) uint32_t;
+    LdsWord* const words = (LdsWord*)area;
+    const int wave = static_cast<int>(threadIdx.x) >> 6;
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) words[wave] = marks;
+    __syncthreads();
+    return __builtin_amdgcn_readfirstlane(words[wave & ~1] | words[wave | 1]);
 }
 
 // The other half's value for the same column.
 __device__ __forceinline__ float other_half(float v) { return __shfl_xor(v, 32); }
 
-// Column values 32 p + 8 g + 4 half + 0 .. 3 of a lane, times factor, to its row; whole: rows of whole groups of four,
-// aligned to them.
+// Column values 32 (first + p) + 8 g + 4 half + 0 .. 3 of a lane, times factor, to its row; whole: rows of whole groups of
+// four, aligned to them.
 template <typename T, int kParts>
-__device__ __forceinline__ void store_column(T* row, int head_dim, bool whole, const Acc (&acc)[kParts], float factor) {
+__device__ __forceinline__ void store_column(T* row, int head_dim, bool whole, int first, const Acc (&acc)[kParts], float factor) {
     const int half = (static_cast<int>(threadIdx.x) >> 5) & 1;
 #pragma unroll
     for (int p = 0; p < kParts; ++p)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const int d = 32 * p + 8 * g + 4 * half;
+            const int d = 32 * (first + p) + 8 * g + 4 * half;
             float v[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) v[r] = acc[p][4 * g + r] * factor;

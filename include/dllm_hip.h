@@ -293,7 +293,7 @@ enum { DLLM_HIP_FLOAT32 = 0, DLLM_HIP_BFLOAT16 = 1, DLLM_HIP_FLOAT16 = 2 };
  * lse[heads, tokens] = log sum exp s, which the backward reads (float32; may be NULL). Keys that a query does not see do
  * not reach its results, whatever they hold.
  * Limits: scale positive, head_dim at most 256, tokens below 2^31, heads a multiple of kv_heads, at most 65535 heads, and
- * (tokens / 128 + documents) * heads below 2^24. Out-of-range
+ * (tokens / 64 + documents) * heads below 2^24. Out-of-range
  * offsets and prefixes are clamped to the tokens and the document; documents that then overlap give unspecified values.
  * The backward takes the forward's out and lse and the upstream gradient dout (out's layout and stride) and writes dq, dk
  * and dv (q's, k's and v's layouts and strides); dk and dv sum over the heads that share them, in head order. */
