@@ -163,13 +163,28 @@ __device__ __forceinline__ float bend_score(const DocAttention& a, float slope, 
     return x - slope * static_cast<float>(distance < 0 ? -distance : distance);
 }
 
-// tanh for the score cap. 16-bit types: 1 - 2 / (1 + e^2x), off by at most about 6 x 2^-24 absolutely, which the weights
-// (rounded to 2^-9 of themselves) do not see. float32: the library's, which is exact to its last bits near zero too.
+// The score of a product x in units of log 2: bend(x) times + plus, which is x scale without a cap. With one, 16-bit types
+// use tanh z = 1 - 2 / (1 + e^2z), off by at most about 6 x 2^-24 absolutely, which the weights (rounded to 2^-9 of
+// themselves) do not see: bend is -1 / (1 + e^2z), and the rest of it falls into times and plus. float32 uses the library's
+// tanh, exact to its last bits near zero too. bend grows with x, so the largest score is that of the largest bend.
 template <typename T>
-__device__ __forceinline__ float cap_tanh(float x) {
-    if constexpr (sizeof(T) == 4) return tanhf(x);
-    return fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(x * 2.8853900817779268f)), 1.0f);
-}
+struct CapTerms {
+    bool capped;
+    float in, times, plus;
+    __device__ __forceinline__ explicit CapTerms(const DocAttention& a) {
+        capped = a.softcap != 0.0f;
+        const float unit = (capped ? a.softcap : a.scale) * kLog2E;
+        in = capped ? a.scale / a.softcap : 0.0f;
+        times = unit, plus = 0.0f;
+        if (sizeof(T) == 2 && capped) in *= 2.0f * kLog2E, times = 2.0f * unit, plus = unit;
+    }
+    __device__ __forceinline__ float bend(float x) const {
+        if constexpr (sizeof(T) == 4) return tanhf(x * in);
+        return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(x * in));
+    }
+    // bend's tanh, whose square is one minus the cap's derivative
+    __device__ __forceinline__ float tangent(float bent) const { return sizeof(T) == 4 ? bent : fmaf(2.0f, bent, 1.0f); }
+};
 
 template <typename T>
 __device__ __forceinline__ float dot_row(const T* a, const T* b, int n) {

@@ -41,20 +41,6 @@ __device__ __forceinline__ float power_of_two_above(float x) {
     return ldexpf(1.0f, e > 126 ? 126 : e < -126 ? -126 : e);
 }
 
-// What a score needs beside X: see the forward kernel.
-template <typename T>
-struct Bend {
-    float unit, cap_in, slope;
-    bool capped, biased;
-    __device__ Bend(const DocAttention& a, int head) {
-        capped = a.softcap != 0.0f;
-        biased = a.slopes != nullptr;
-        unit = (capped ? a.softcap : a.scale) * kLog2E;
-        cap_in = capped ? a.scale / a.softcap : 0.0f;
-        slope = biased ? a.slopes[head] * kLog2E : 0.0f;
-    }
-};
-
 // ---- dq ----
 template <typename T, int kDim>
 __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1) void dq_kernel(DocAttention a) {
@@ -128,8 +114,9 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     const Copy copy_k(a.sources[1], kv), copy_v(a.sources[2], kv);
     const TileView<T, kDim, kTile> view;
     LdsByte* const buffers = (LdsByte*)lds;
-    const Bend<T> bend(a, head);
-    const float base = a.lse[stat_at] * kLog2E - kWeightShift<T>;
+    const CapTerms<T> cap(a);
+    const float slope = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
+    const float base = a.lse[stat_at] * kLog2E - kWeightShift<T> - cap.plus;
 
     Acc dq[kParts];
 #pragma unroll
@@ -178,21 +165,20 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
             float ds[16];
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] = fmaf(dp[r], into, -delta * into);
-            if (bend.capped) {
+            if (cap.capped) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    x[r] = cap_tanh<T>(x[r] * bend.cap_in);
-                    ds[r] *= fmaf(-x[r], x[r], 1.0f);
+                    x[r] = cap.bend(x[r]);
+                    const float tangent = cap.tangent(x[r]);
+                    ds[r] *= fmaf(-tangent, tangent, 1.0f);
                 }
             }
-            if (bend.biased) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], cap.times, -base);
+            if (a.slopes) {
                 const float away = static_cast<float>(i - from - 32 * b - 4 * half);
 #pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    x[r] = fmaf(-bend.slope, fabsf(away - static_cast<float>(8 * (r / 4) + r % 4)), fmaf(x[r], bend.unit, -base));
-            } else {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) x[r] = fmaf(x[r], bend.unit, -base);
+                for (int r = 0; r < 16; ++r) x[r] = fmaf(-slope, fabsf(away - static_cast<float>(8 * (r / 4) + r % 4)), x[r]);
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) ds[r] *= __builtin_amdgcn_exp2f(x[r]);
@@ -294,7 +280,8 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     const Copy copy_q(a.sources[0], head), copy_d(a.sources[3], head);
     const TileView<T, kDim, kTile> view;
     LdsByte* const buffers = (LdsByte*)lds;
-    const Bend<T> bend(a, head);
+    const CapTerms<T> cap(a);
+    const float slope = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
 
     Acc dk[kDk ? kParts : 1], dv[kDv ? kParts : 1];
 #pragma unroll
@@ -308,7 +295,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     // a tile's statistics, one value for each of the first 2 kTile threads
     auto read_stat = [&](int t) {
         const int which = static_cast<int>(threadIdx.x) / kTile, at = min(doc.start + t * kTile + static_cast<int>(threadIdx.x) % kTile, doc.end - 1);
-        return which == 0 ? a.lse[stat_at + at] * kLog2E - kWeightShift<T> : which == 1 ? a.delta[stat_at + at] * into : 0.0f;
+        return which == 0 ? a.lse[stat_at + at] * kLog2E - kWeightShift<T> - cap.plus : which == 1 ? a.delta[stat_at + at] * into : 0.0f;
     };
     auto write_stat = [&](int buffer, float value) {
         if (static_cast<int>(threadIdx.x) < 2 * kTile) (&stats[buffer][0][0])[threadIdx.x] = value;
@@ -365,19 +352,20 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
                     x[4 * g + r] = x_in[4 * g + r];
                 }
             }
-            if (!kPlain && bend.capped) {
+            if (!kPlain && cap.capped) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    x[r] = cap_tanh<T>(x[r] * bend.cap_in);
-                    ds[r] *= fmaf(-x[r], x[r], 1.0f);
+                    x[r] = cap.bend(x[r]);
+                    const float tangent = cap.tangent(x[r]);
+                    ds[r] *= fmaf(-tangent, tangent, 1.0f);
                 }
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) p[r] = fmaf(x[r], bend.unit, -p[r]);
-            if (!kPlain && bend.biased) {
+            for (int r = 0; r < 16; ++r) p[r] = fmaf(x[r], cap.times, -p[r]);
+            if (!kPlain && a.slopes) {
                 const float away = static_cast<float>(from + 32 * b + 4 * half - j);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) p[r] = fmaf(-bend.slope, fabsf(away + static_cast<float>(8 * (r / 4) + r % 4)), p[r]);
+                for (int r = 0; r < 16; ++r) p[r] = fmaf(-slope, fabsf(away + static_cast<float>(8 * (r / 4) + r % 4)), p[r]);
             }
             if (!kPlain && !all_seen) {
                 const int to_low = span.low - from - 32 * b - 4 * half;
@@ -401,7 +389,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
             if constexpr (kDk) multiply_columns<T, kDim, kTile>(view, q_tile, b, ds, first_part, dk);
         };
         constexpr int kBlocks = kTile / 32;
-        if (kPipelined && all_seen && !bend.capped && !bend.biased) {
+        if (kPipelined && all_seen && !cap.capped && !a.slopes) {
             // One wave to a SIMD: the matrix cores work on the next queries' scores and the last ones' sums while the vector
             // unit has this one's weights.
             Acc x[2], dp[2];

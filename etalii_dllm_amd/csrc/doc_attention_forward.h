@@ -64,8 +64,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     const TileView<T, kDim, kTile> view;
     LdsByte* const buffers = (LdsByte*)lds;
 
-    const float unit = (a.softcap != 0.0f ? a.softcap : a.scale) * kLog2E;  // score of X (or of the tanh) in units of log 2
-    const float cap_in = a.softcap != 0.0f ? a.scale / a.softcap : 0.0f;
+    const CapTerms<T> cap(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
 
     Acc o[kParts];
@@ -118,12 +117,12 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
         for (int b = 0; b < kTile / 32; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[b][r] = x[b][r];
-        float times = unit;
-        if (a.softcap != 0.0f) {
+        float times = cap.times, plus = cap.plus;  // s times + plus: the score in units of log 2
+        if (cap.capped) {
 #pragma unroll
             for (int b = 0; b < kTile / 32; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[b][r] = cap_tanh<T>(s[b][r] * cap_in);
+                for (int r = 0; r < 16; ++r) s[b][r] = cap.bend(s[b][r]);
         }
         if (a.slopes) {
             const float away = static_cast<float>(i - from - 4 * half);
@@ -131,8 +130,8 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
             for (int b = 0; b < kTile / 32; ++b)
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    s[b][r] = fmaf(-slope, fabsf(away - static_cast<float>(32 * b + 8 * (r / 4) + r % 4)), s[b][r] * unit);
-            times = 1.0f;
+                    s[b][r] = fmaf(-slope, fabsf(away - static_cast<float>(32 * b + 8 * (r / 4) + r % 4)), fmaf(s[b][r], times, plus));
+            times = 1.0f, plus = 0.0f;
         }
         if (!all_seen) {
             const int to_low = span.low - from - 4 * half;
@@ -152,7 +151,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
         for (int b = 0; b < kTile / 32; ++b)
 #pragma unroll
             for (int r = 0; r < 16; ++r) top = fmaxf(top, s[b][r]);
-        top = fmaxf(top, other_half(top)) * times;
+        top = fmaf(fmaxf(top, other_half(top)), times, plus);
         if (__any(top > m + 8.0f)) {
             const float moved = fmaxf(m, top);
             const float keep = __builtin_amdgcn_exp2f(m - (moved == -INFINITY ? 0.0f : moved));
@@ -163,7 +162,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
 #pragma unroll
                 for (int r = 0; r < 16; ++r) o[p][r] *= keep;
         }
-        const float base = m == -INFINITY ? 0.0f : m;
+        const float base = (m == -INFINITY ? 0.0f : m) - plus;
         float sum = 0.0f;
 #pragma unroll
         for (int b = 0; b < kTile / 32; ++b)

@@ -238,6 +238,20 @@ struct Rows16 {
     }
 };
 
+// The order that the compiler is asked to keep between LDS reads and products: kFirst reads ahead, then kReads for every
+// kProducts products. Left alone it reads one operand, waits for it and multiplies, which leaves the matrix cores idle for
+// the LDS's latency every time.
+constexpr int kAheadSteps = 2;  // measured: 3, 4 and 6 are no faster, and take registers
+template <int kCount, int kFirst, int kReads, int kProducts>
+__device__ __forceinline__ void reads_ahead() {
+    __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
+#pragma unroll
+    for (int i = 0; i < kCount; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x8, kProducts, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+    }
+}
+
 // acc += (tile's rows, 32 of them from 32 block, as columns 32 (first + 0 .. kParts - 1) ..)^T x
 template <typename T, int kDim, int kRows, int kParts>
 __device__ __forceinline__ void multiply_columns(const TileView<T, kDim, kRows>& view, const LdsByte* tile, int block,
@@ -247,6 +261,7 @@ __device__ __forceinline__ void multiply_columns(const TileView<T, kDim, kRows>&
 #pragma unroll
         for (int p = 0; p < kParts; ++p)
             multiply<T>(view.columns(tile, block, g, kParts * 32 == kDim ? p : first + p), x.group[g], acc[p]);
+    reads_ahead<2 * kParts, 2 * kAheadSteps * kPlanes<T>, 2 * kPlanes<T>, kPlanes<T> == 3 ? 6 : 1>();
 }
 
 // Wide float32 heads: a lane's rows and sums in three planes are more than the registers, so a pair of waves shares 32 rows
@@ -286,6 +301,7 @@ __device__ __forceinline__ void multiply_rows(const TileView<T, kDim, kRows>& vi
 #pragma unroll
     for (int step = 0; step < kSteps; ++step)
         multiply<T>(view.rows(tile, block, kPair<T, kDim> == 1 ? step : step + part * kSteps), column.held[step], acc);
+    reads_ahead<kSteps, kAheadSteps * kPlanes<T>, kPlanes<T>, kPlanes<T> == 3 ? 6 : 1>();
 }
 
 // The pair's sums: each wave leaves its own in LDS (4 KB for each 32 x 32), and after the barrier adds the other's. All waves
