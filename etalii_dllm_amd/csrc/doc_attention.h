@@ -355,33 +355,50 @@ struct PackArgs {
     Source to[4];
     int heads[4];
     int tokens, head_dim;
+    bool whole;
 };
 
-// Copies arrays into sources: split into planes, heads filled up with zeroes to whole chunks. A thread has a chunk.
+// Copies arrays into sources: split into planes, heads filled up with zeroes to whole chunks. A workgroup has some tokens, a
+// thread a chunk of 8 elements at a time.
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const int which = blockIdx.y;
     const Source to = a.to[which];
-    const int64_t per_token = static_cast<int64_t>(a.heads[which]) * to.chunks;
-    for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < a.tokens * per_token; e += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t token = e / per_token, in_token = e % per_token;
-        const int head = static_cast<int>(in_token / to.chunks), chunk = static_cast<int>(in_token % to.chunks);
-        const T* from = static_cast<const T*>(a.from[which]) + token * a.stride[which] + static_cast<int64_t>(head) * a.head_dim;
-        Part<T> parts[kPartChunk][kPlanes<T>];
+    const int per_token = a.heads[which] * to.chunks;
+    const int at_once = per_token < 256 ? 256 / per_token : 1;  // tokens of a turn of the workgroup
+    const int mine = static_cast<int>(threadIdx.x) / per_token, first = static_cast<int>(threadIdx.x) % per_token;
+    if (per_token < 256 && mine >= at_once) return;
+    for (int64_t base = static_cast<int64_t>(blockIdx.x) * at_once; base < a.tokens; base += static_cast<int64_t>(gridDim.x) * at_once) {
+        const int64_t token = base + (per_token < 256 ? mine : 0);
+        if (token >= a.tokens) return;
+        for (int c = per_token < 256 ? first : static_cast<int>(threadIdx.x); c < per_token; c += per_token < 256 ? per_token : 256) {
+            const int head = c / to.chunks, chunk = c - head * to.chunks;
+            const T* from = static_cast<const T*>(a.from[which]) + token * a.stride[which] + static_cast<int64_t>(head) * a.head_dim + chunk * kPartChunk;
+            const int there = a.head_dim - chunk * kPartChunk;  // elements of the head from here on
+            T x[kPartChunk];
+            if (a.whole && there >= kPartChunk) {
 #pragma unroll
-        for (int j = 0; j < kPartChunk; ++j) {
-            const int d = chunk * kPartChunk + j;
-            if constexpr (kPlanes<T> == 1)
-                parts[j][0] = d < a.head_dim ? from[d] : static_cast<T>(0.0f);
-            else
-                split<T>(d < a.head_dim ? from[d] : 0.0f, parts[j]);
-        }
+                for (int h = 0; h < kPartChunk; h += kChunk<T>)
+                    *reinterpret_cast<Pack<T, kChunk<T>>*>(x + h) = *reinterpret_cast<const Pack<T, kChunk<T>>*>(from + h);
+            } else {
 #pragma unroll
-        for (int p = 0; p < kPlanes<T>; ++p) {
-            Pack<Part<T>, kPartChunk> c;
+                for (int j = 0; j < kPartChunk; ++j) x[j] = j < there ? from[j] : static_cast<T>(0.0f);
+            }
+            Pack<Part<T>, kPartChunk> planes[kPlanes<T>];
 #pragma unroll
-            for (int j = 0; j < kPartChunk; ++j) c.v[j] = parts[j][p];
-            *reinterpret_cast<Pack<Part<T>, kPartChunk>*>(const_cast<char*>(to.base) + p * to.plane + token * to.stride + head * to.head + chunk * 16) = c;
+            for (int j = 0; j < kPartChunk; ++j) {
+                Part<T> parts[kPlanes<T>];
+                if constexpr (kPlanes<T> == 1)
+                    parts[0] = x[j];
+                else
+                    split<T>(x[j], parts);
+#pragma unroll
+                for (int p = 0; p < kPlanes<T>; ++p) planes[p].v[j] = parts[p];
+            }
+#pragma unroll
+            for (int p = 0; p < kPlanes<T>; ++p)
+                *reinterpret_cast<Pack<Part<T>, kPartChunk>*>(const_cast<char*>(to.base) + p * to.plane + token * to.stride +
+                                                              head * to.head + chunk * 16) = planes[p];
         }
     }
 }
@@ -402,6 +419,7 @@ void set_sources(DocAttention& a, bool backward, char* packed, hipStream_t strea
     PackArgs p{};
     p.tokens = a.tokens;
     p.head_dim = a.head_dim;
+    p.whole = a.whole;
     for (int i = 0; i < count; ++i) {
         const int64_t row = int64_t{heads[i]} * chunks * 16, plane = row * a.tokens;
         a.sources[i] = {packed, row, int64_t{chunks} * 16, plane, chunks};

@@ -460,10 +460,10 @@ __global__ __launch_bounds__(kDocThreads) void add_heads_kernel(DocAttention a) 
     int first;
     if (!locate_tile<kDocTileRows, false>(a, blockIdx.x, doc, first)) return;
     const int rows = min(kDocTileRows, doc.end - first);
-    for (int64_t e = static_cast<int64_t>(blockIdx.y) * kDocThreads + threadIdx.x; e < static_cast<int64_t>(rows) * per_token;
-         e += static_cast<int64_t>(gridDim.y) * kDocThreads) {
-        const int row = static_cast<int>(e / per_token), in_token = static_cast<int>(e % per_token);
-        const int kv = in_token / per_row, d = in_token % per_row * kWidth;
+    // (128 rows of at most 65535 heads of 64 groups of four: 32 bits)
+    for (int e = static_cast<int>(blockIdx.y * kDocThreads + threadIdx.x); e < rows * per_token; e += static_cast<int>(gridDim.y) * kDocThreads) {
+        const int row = e / per_token, in_token = e - row * per_token;
+        const int kv = in_token / per_row, d = (in_token - kv * per_row) * kWidth;
         const int64_t j = first + row;
 #pragma unroll
         for (int which = 0; which < 2; ++which) {
@@ -513,7 +513,7 @@ int launch_document_attention_backward(DocAttention a, char* packed, hipStream_t
     else
         launch_gradients<T, 256>(a, s);
     if (a.group > 1) {
-        const dim3 grid(doc_tiles(a, kDocTileRows), 8);
+        const dim3 grid(doc_tiles(a, kDocTileRows), 16);
         if (a.whole)
             add_heads_kernel<T, 4><<<grid, kDocThreads, 0, s>>>(a);
         else
