@@ -36,6 +36,11 @@ struct DocAttention {
     float* dv_part;
 };
 
+// 16-bit weights (and dS) are rounded to their type for the second product: each is off by 2^-9 or 2^-12 of itself, which in a
+// sum over many keys adds to about what the result's own rounding is. Documents of so few tokens that such errors do not
+// average out have what the rounding left multiplied too; they are one tile of keys, which that makes a fifth slower.
+constexpr int kFewTokens = 64;
+
 // Token range of a document, and the end of the keys that all its tokens see.
 struct Document {
     int start, end, prefix_end;

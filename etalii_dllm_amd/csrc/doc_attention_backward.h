@@ -61,6 +61,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     int first;
     if (!locate_tile<kOwn, true>(a, blockIdx.x / a.heads, doc, first)) return;
 
+    const bool few = doc.end - doc.start <= kFewTokens;
     const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
     const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
     const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
@@ -194,6 +195,10 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
                 }
             }
             multiply_columns<T, kDim, kTile>(view, k_tile, b, Rows16<T>(ds), first_part, dq);
+            if (kPlanes<T> == 1 && few) {
+                keep_rest<T>(ds);
+                multiply_columns<T, kDim, kTile>(view, k_tile, b, Rows16<T>(ds), first_part, dq);
+            }
         }
     }
     if (!kPaired && !working) return;
@@ -238,6 +243,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     int first;
     if (!locate_tile<kOwn, false>(a, blockIdx.x / a.heads, doc, first)) return;
 
+    const bool few = doc.end - doc.start <= kFewTokens;
     const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
     const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
     const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
@@ -389,7 +395,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
             if constexpr (kDk) multiply_columns<T, kDim, kTile>(view, q_tile, b, ds, first_part, dk);
         };
         constexpr int kBlocks = kTile / 32;
-        if (kPipelined && all_seen && !cap.capped && !a.slopes) {
+        if (kPipelined && all_seen && !cap.capped && !a.slopes && !few) {
             // One wave to a SIMD: the matrix cores work on the next queries' scores and the last ones' sums while the vector
             // unit has this one's weights.
             Acc x[2], dp[2];
@@ -420,6 +426,11 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
                 float p[16], ds[16];
                 weights(b, x, dp, std::false_type{}, p, ds);
                 add(b, Rows16<T>(p), Rows16<T>(ds));
+                if (kPlanes<T> == 1 && few) {
+                    keep_rest<T>(p);
+                    keep_rest<T>(ds);
+                    add(b, Rows16<T>(p), Rows16<T>(ds));
+                }
             }
         }
     }

@@ -23,7 +23,7 @@ constexpr int kBuffers = 4 * kKeys<T, kDim> * kDim * 2 * kPlanes<T> <= 128 * 102
 // The running maximum is moved only when some query of the wave has outgrown it by 2^8: until then P stays below 2^8, which
 // float32 sums and 16-bit products hold as well as values below one.
 template <typename T, int kDim>
-__global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1) void forward_kernel(DocAttention a, T* out) {
+__global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kDim <= 128 ? 2 : 1) : 1) void forward_kernel(DocAttention a, T* out) {
     using Shape = TileShape<T, kDim>;
     constexpr int kTile = kKeys<T, kDim>;
     using Copy = TileCopy<T, kDim, kTile, kDocThreads>;
@@ -42,6 +42,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     int first;
     if (!locate_tile<kOwn, true>(a, blockIdx.x / a.heads, doc, first)) return;
 
+    const bool few = doc.end - doc.start <= kFewTokens;
     const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
     const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
     const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
@@ -174,6 +175,13 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
         l += sum;
 #pragma unroll
         for (int b = 0; b < kTile / 32; ++b) multiply_columns<T, kDim, kTile>(view, v_tile, b, Rows16<T>(s[b]), first_part, o);
+        if (kPlanes<T> == 1 && few) {
+#pragma unroll
+            for (int b = 0; b < kTile / 32; ++b) {
+                keep_rest<T>(s[b]);
+                multiply_columns<T, kDim, kTile>(view, v_tile, b, Rows16<T>(s[b]), first_part, o);
+            }
+        }
     }
     if (!kPaired && !working) return;
     l += other_half(l);

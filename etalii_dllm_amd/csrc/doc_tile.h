@@ -238,6 +238,13 @@ struct Rows16 {
     }
 };
 
+// What the type's rounding leaves of each value.
+template <typename T>
+__device__ __forceinline__ void keep_rest(float (&x)[16]) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] -= static_cast<float>(static_cast<Part<T>>(x[r]));
+}
+
 // The order that the compiler is asked to keep between LDS reads and products: kFirst reads ahead, then kReads for every
 // kProducts products. Left alone it reads one operand, waits for it and multiplies, which leaves the matrix cores idle for
 // the LDS's latency every time.
