@@ -29,16 +29,19 @@ FLAGS = [
     "-ffp-contract=off",
     "-fno-fast-math",
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    # matrix-core accumulators in architectural VGPRs (no AGPR copies around each MFMA)
-    "-mllvm", "-amdgpu-mfma-vgpr-form",
     f"-I{ROOT / 'include'}",
     f"-I{CSRC}",
+    # matrix-core accumulators in architectural VGPRs (no AGPR copies around each MFMA) ...
+    *(VGPR_SUMS := ["-mllvm", "-amdgpu-mfma-vgpr-form"]),
 ]
+# ... but where they take half of a wave's registers
+AGPR_SUMS = {"doc_attention_wide.hip"}
 
 
 def _compile(source: Path) -> Path:
     obj = BUILD / (source.stem + ".o")
-    cmd = [HIPCC, *FLAGS, "-c", str(source), "-o", str(obj)]
+    flags = FLAGS[:-len(VGPR_SUMS)] if source.name in AGPR_SUMS else FLAGS
+    cmd = [HIPCC, *flags, "-c", str(source), "-o", str(obj)]
     result = subprocess.run(cmd, capture_output=True, text=True)
     if result.returncode != 0:
         raise RuntimeError(f"hipcc failed for {source.name}:\n{result.stderr[-4000:]}")

@@ -11,6 +11,7 @@
 
 #include <float.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -71,6 +72,26 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     const Span span = key_span(a, doc, i);
     const int64_t head_at = static_cast<int64_t>(head) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens + i;
 
+    const int low = key_span(a, doc, first).low;
+    const int high = max(key_span(a, doc, min(first + kOwn, doc.end) - 1).high, doc.prefix_end);
+    const int low_tile = (low - doc.start) / kTile, prefix_tiles = (doc.prefix_end - doc.start + kTile - 1) / kTile;
+    const int tiles = (high - doc.start + kTile - 1) / kTile;
+    const Span first_span = key_span(a, doc, wave_first), last_span = key_span(a, doc, wave_last);
+    const int any_low = first_span.low, any_high = last_span.high, all_low = last_span.low, all_high = first_span.high;
+
+    const Copy copy_k(a.sources[1], kv), copy_v(a.sources[2], kv);
+    const TileView<T, kDim, kTile> view;
+    LdsByte* const buffers = (LdsByte*)lds;
+    // the first tile is on its way while the lane's rows are read
+    auto next_tile = [&](int t) { return t + 1 < prefix_tiles ? t + 1 : max(t + 1, low_tile); };
+    auto fetch = [&](int t, int buffer) {
+        const int from = doc.start + t * kTile;
+        copy_k(from, doc.end - from, buffers + buffer * 2 * kTileBytes);
+        copy_v(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
+    };
+    int t = next_tile(-1);
+    if (kAhead) fetch(t, 0);
+
     const Column<T, kDim> q(a.sources[0], head, i, part), dout(a.sources[3], head, i, part);
     float delta = 0.0f, norm = 0.0f;  // this half's part
     {
@@ -80,18 +101,35 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
             delta = fmaf(o, d, delta);
             norm = fmaf(d, d, norm);
         };
-        // (both ways take the same elements in the same order)
-        constexpr int kWide = kChunk<T>;
-        for (int d0 = half * kWide; d0 < a.head_dim; d0 += 2 * kWide) {
-            if (a.whole) {
-                float o[kWide], d[kWide];
-                load_as_float<T, kWide>(out_row + d0, o);
-                load_as_float<T, kWide>(dout_row + d0, d);
+        // (both ways take the same elements in the same order; every load is on its way before the first is used)
+        constexpr int kWide = kChunk<T>, kLoads = kDim / (2 * kWide);
+        if (a.whole) {
+            Pack<T, kWide> o[kLoads], d[kLoads];
 #pragma unroll
-                for (int j = 0; j < kWide; ++j) add(o[j], d[j]);
-            } else {
-                for (int j = 0; j < kWide && d0 + j < a.head_dim; ++j)
-                    add(static_cast<float>(out_row[d0 + j]), static_cast<float>(dout_row[d0 + j]));
+            for (int s = 0; s < kLoads; ++s) {
+                const int d0 = min((2 * s + half) * kWide, a.head_dim - kWide);
+                o[s] = *reinterpret_cast<const Pack<T, kWide>*>(out_row + d0);
+                d[s] = *reinterpret_cast<const Pack<T, kWide>*>(dout_row + d0);
+            }
+#pragma unroll
+            for (int s = 0; s < kLoads; ++s)
+                if ((2 * s + half) * kWide < a.head_dim)
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j) add(static_cast<float>(o[s].v[j]), static_cast<float>(d[s].v[j]));
+        } else {
+#pragma unroll 4
+            for (int d0 = half * kWide; d0 < a.head_dim; d0 += 2 * kWide) {
+                T o[kWide], d[kWide];
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) {
+                    const int at = min(d0 + j, a.head_dim - 1);
+                    o[j] = out_row[at], d[j] = dout_row[at];
+                }
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) {
+                    const bool there = d0 + j < a.head_dim;
+                    add(there ? static_cast<float>(o[j]) : 0.0f, there ? static_cast<float>(d[j]) : 0.0f);
+                }
             }
         }
     }
@@ -105,16 +143,6 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     if (mine && half == 0 && part == 0) a.delta[stat_at] = delta;
     const float into = 1.0f / dout_scale;  // exact
 
-    const int low = key_span(a, doc, first).low;
-    const int high = max(key_span(a, doc, min(first + kOwn, doc.end) - 1).high, doc.prefix_end);
-    const int low_tile = (low - doc.start) / kTile, prefix_tiles = (doc.prefix_end - doc.start + kTile - 1) / kTile;
-    const int tiles = (high - doc.start + kTile - 1) / kTile;
-    const Span first_span = key_span(a, doc, wave_first), last_span = key_span(a, doc, wave_last);
-    const int any_low = first_span.low, any_high = last_span.high, all_low = last_span.low, all_high = first_span.high;
-
-    const Copy copy_k(a.sources[1], kv), copy_v(a.sources[2], kv);
-    const TileView<T, kDim, kTile> view;
-    LdsByte* const buffers = (LdsByte*)lds;
     const CapTerms<T> cap(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
     const float base = a.lse[stat_at] * kLog2E - kWeightShift<T> - cap.plus;
@@ -125,14 +153,6 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
 #pragma unroll
         for (int r = 0; r < 16; ++r) dq[p][r] = 0.0f;
 
-    auto next_tile = [&](int t) { return t + 1 < prefix_tiles ? t + 1 : max(t + 1, low_tile); };
-    auto fetch = [&](int t, int buffer) {
-        const int from = doc.start + t * kTile;
-        copy_k(from, doc.end - from, buffers + buffer * 2 * kTileBytes);
-        copy_v(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
-    };
-    int t = next_tile(-1);
-    if (kAhead) fetch(t, 0);
     for (int buffer = 0; t < tiles; buffer ^= kAhead) {
         tile_barrier();
         const int next = next_tile(t);
@@ -253,8 +273,6 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     const Span span = query_span(a, doc, j);
     const int64_t kv_at = static_cast<int64_t>(kv) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens;
 
-    const Column<T, kDim> k(a.sources[1], kv, j, part), v(a.sources[2], kv, j, part);
-
     // the queries that see any key of the workgroup; keys in the prefix are seen from the document's start on
     const int last = min(first + kOwn, doc.end) - 1;
     const int low = query_span(a, doc, first).low;
@@ -266,6 +284,20 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     // (a wave with keys on both sides of the prefix's end: the first key after it has the earliest end)
     const int edge = wave_first < doc.prefix_end && wave_last >= doc.prefix_end ? doc.prefix_end : wave_first;
     const int all_low = last_span.low, all_high = query_span(a, doc, min(edge, doc.end - 1)).high;
+
+    const Copy copy_q(a.sources[0], head), copy_d(a.sources[3], head);
+    const TileView<T, kDim, kTile> view;
+    LdsByte* const buffers = (LdsByte*)lds;
+    auto fetch = [&](int t, int buffer) {
+        const int from = doc.start + t * kTile;
+        copy_q(from, doc.end - from, buffers + buffer * 2 * kTileBytes);
+        copy_d(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
+    };
+    // the first tile is on its way while the lane's rows are read
+    int t = low_tile;
+    if (kAhead) fetch(t, 0);
+    const Column<T, kDim> k(a.sources[1], kv, j, part), v(a.sources[2], kv, j, part);
+
 
     float dout_scale = 1.0f;
     if constexpr (kWeightShift<T> != 0.0f && kDk) {
@@ -283,9 +315,6 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     }
     const float into = 1.0f / dout_scale;
 
-    const Copy copy_q(a.sources[0], head), copy_d(a.sources[3], head);
-    const TileView<T, kDim, kTile> view;
-    LdsByte* const buffers = (LdsByte*)lds;
     const CapTerms<T> cap(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
 
@@ -306,16 +335,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     auto write_stat = [&](int buffer, float value) {
         if (static_cast<int>(threadIdx.x) < 2 * kTile) (&stats[buffer][0][0])[threadIdx.x] = value;
     };
-    auto fetch = [&](int t, int buffer) {
-        const int from = doc.start + t * kTile;
-        copy_q(from, doc.end - from, buffers + buffer * 2 * kTileBytes);
-        copy_d(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
-    };
-    int t = low_tile;
-    if (kAhead) {
-        write_stat(0, read_stat(t));
-        fetch(t, 0);
-    }
+    if (kAhead) write_stat(0, read_stat(t));
     for (int buffer = 0; t < tiles; buffer ^= kAhead, ++t) {
         tile_barrier();
         if (!kAhead) {
@@ -476,20 +496,18 @@ __global__ __launch_bounds__(kDocThreads) void add_heads_kernel(DocAttention a) 
         const int row = e / per_token, in_token = e - row * per_token;
         const int kv = in_token / per_row, d = (in_token - kv * per_row) * kWidth;
         const int64_t j = first + row;
+        const int64_t at = (static_cast<int64_t>(kv) * a.group * a.tokens + j) * a.head_dim + d, next = static_cast<int64_t>(a.tokens) * a.head_dim;
+        float sum[2][kWidth] = {};  // (of zero and a first part of minus zero: plus zero, as a product's sum would be)
+#pragma unroll 4
+        for (int g = 0; g < a.group; ++g) {
+            float more[2][kWidth];
+            load_as_float<float, kWidth>(a.dk_part + at + g * next, more[0]);
+            load_as_float<float, kWidth>(a.dv_part + at + g * next, more[1]);
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const float* part = (which ? a.dv_part : a.dk_part) + (static_cast<int64_t>(kv) * a.group * a.tokens + j) * a.head_dim + d;
-            float sum[kWidth];
-            load_as_float<float, kWidth>(part, sum);
-            for (int g = 1; g < a.group; ++g) {
-                float more[kWidth];
-                load_as_float<float, kWidth>(part + static_cast<int64_t>(g) * a.tokens * a.head_dim, more);
-#pragma unroll
-                for (int c = 0; c < kWidth; ++c) sum[c] += more[c];
-            }
-            T* to = which ? static_cast<T*>(a.dv) + j * a.v_stride : static_cast<T*>(a.dk) + j * a.k_stride;
-            store_from_float<T, kWidth>(to + static_cast<int64_t>(kv) * a.head_dim + d, sum);
+            for (int c = 0; c < kWidth; ++c) sum[0][c] += more[0][c], sum[1][c] += more[1][c];
         }
+        store_from_float<T, kWidth>(static_cast<T*>(a.dk) + j * a.k_stride + static_cast<int64_t>(kv) * a.head_dim + d, sum[0]);
+        store_from_float<T, kWidth>(static_cast<T*>(a.dv) + j * a.v_stride + static_cast<int64_t>(kv) * a.head_dim + d, sum[1]);
     }
 }
 
@@ -524,7 +542,9 @@ int launch_document_attention_backward(DocAttention a, char* packed, hipStream_t
     else
         launch_gradients<T, 256>(a, s);
     if (a.group > 1) {
-        const dim3 grid(doc_tiles(a, kDocTileRows), 16);
+        // about one turn for each thread, as far as 64 workgroups to a part of a document go
+        const int64_t threads = static_cast<int64_t>(kDocTileRows) * a.kv_heads * a.head_dim / (a.whole ? 4 : 1);
+        const dim3 grid(doc_tiles(a, kDocTileRows), static_cast<unsigned>(std::clamp<int64_t>(threads / kDocThreads, 1, 64)));
         if (a.whole)
             add_heads_kernel<T, 4><<<grid, kDocThreads, 0, s>>>(a);
         else

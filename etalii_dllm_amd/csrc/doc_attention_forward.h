@@ -50,8 +50,6 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kD
     const int i = min(wave_first + (lane & 31), doc.end - 1);
     const Span span = key_span(a, doc, i);
 
-    const Column<T, kDim> q(a.sources[0], head, i, part);
-
     // keys of the workgroup: [low, high) in whole tiles of the document, and the tiles of the prefix before them
     const int low = key_span(a, doc, first).low;
     const int high = max(key_span(a, doc, min(first + kOwn, doc.end) - 1).high, doc.prefix_end);
@@ -65,6 +63,17 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kD
     const TileView<T, kDim, kTile> view;
     LdsByte* const buffers = (LdsByte*)lds;
 
+    // the first tile is on its way while the lane's row is read
+    auto next_tile = [&](int t) { return t + 1 < prefix_tiles ? t + 1 : max(t + 1, low_tile); };
+    auto fetch = [&](int t, int buffer) {
+        const int from = doc.start + t * kTile;
+        copy_k(from, doc.end - from, buffers + buffer * 2 * kTileBytes);
+        copy_v(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
+    };
+    int t = next_tile(-1);
+    if (kAhead) fetch(t, 0);
+    const Column<T, kDim> q(a.sources[0], head, i, part);
+
     const CapTerms<T> cap(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
 
@@ -75,14 +84,6 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kD
         for (int r = 0; r < 16; ++r) o[p][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
-    auto next_tile = [&](int t) { return t + 1 < prefix_tiles ? t + 1 : max(t + 1, low_tile); };
-    auto fetch = [&](int t, int buffer) {
-        const int from = doc.start + t * kTile;
-        copy_k(from, doc.end - from, buffers + buffer * 2 * kTileBytes);
-        copy_v(from, doc.end - from, buffers + buffer * 2 * kTileBytes + kTileBytes);
-    };
-    int t = next_tile(-1);
-    if (kAhead) fetch(t, 0);
     for (int buffer = 0; t < tiles; buffer ^= kAhead) {
         tile_barrier();
         const int next = next_tile(t);
@@ -210,6 +211,10 @@ template <typename T, int kDim>
 void launch_forward(const DocAttention& a, T* out, hipStream_t s) {
     forward_kernel<T, kDim><<<doc_tiles(a, kBlockRows<T, kDim>) * a.heads, kDocThreads, 0, s>>>(a, out);
 }
+
+// doc_attention_wide.hip
+extern template void launch_forward<__bf16, 256>(const DocAttention&, __bf16*, hipStream_t);
+extern template void launch_forward<_Float16, 256>(const DocAttention&, _Float16*, hipStream_t);
 
 template <typename T>
 int launch_document_attention(DocAttention a, void* out, char* packed, hipStream_t s) {
