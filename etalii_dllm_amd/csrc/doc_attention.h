@@ -66,7 +66,7 @@ __device__ __forceinline__ Document document_at(const DocAttention& a, int d) {
 // causal documents (one to a lane): the parts of the highest level first, of all documents that reach it, where a part's level
 // counts from the end with less work. Else the documents in order, each from the end with more work.
 template <int kRows, bool kFromEnd>
-__device__ __forceinline__ bool locate_tile(const DocAttention& a, int64_t tile, Document& doc, int& first) {
+__device__ __forceinline__ bool find_tile(const DocAttention& a, int64_t tile, Document& doc, int& first) {
     const int lane = static_cast<int>(threadIdx.x) & 63;
     auto found = [&](const Document& mine, int owner, int level) {
         doc.start = __builtin_amdgcn_readlane(mine.start, owner);
@@ -118,6 +118,23 @@ __device__ __forceinline__ bool locate_tile(const DocAttention& a, int64_t tile,
     }
     return false;
 }
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
+// find_tile, with its results in scalar registers: what follows from them (loops, branches, addresses) is scalar too.
+template <int kRows, bool kFromEnd>
+__device__ __forceinline__ bool locate_tile(const DocAttention& a, int64_t tile, Document& doc, int& first) {
+    Document d{0, 0, 0};
+    int f = 0;
+    const int found = find_tile<kRows, kFromEnd>(a, tile, d, f);
+    doc.start = uniform(d.start), doc.end = uniform(d.end), doc.prefix_end = uniform(d.prefix_end);
+    first = uniform(f);
+    return uniform(found);
+}
+
+// Waits for the loads issued so far, where the compiler sees it: a load from before a loop that is first used in it is waited
+// for in every turn otherwise, and with it the copies to LDS that the turn has just begun.
+__device__ __forceinline__ void loads_arrived() { __builtin_amdgcn_s_waitcnt(0x0f70); }  // vmcnt(0)
 
 // The keys that query i sees: [low, high) and [start, prefix_end).
 struct Span {

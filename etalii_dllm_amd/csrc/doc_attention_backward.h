@@ -12,7 +12,6 @@
 #include <float.h>
 
 #include <algorithm>
-#include <type_traits>
 
 #include "common.h"
 #include "doc_attention.h"
@@ -63,7 +62,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     if (!locate_tile<kOwn, true>(a, blockIdx.x / a.heads, doc, first)) return;
 
     const bool few = doc.end - doc.start <= kFewTokens;
-    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
+    const int wave = uniform(static_cast<int>(threadIdx.x) >> 6), lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
     const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
     const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
     const bool working = wave_first < doc.end;
@@ -153,6 +152,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
 #pragma unroll
         for (int r = 0; r < 16; ++r) dq[p][r] = 0.0f;
 
+    loads_arrived();
     for (int buffer = 0; t < tiles; buffer ^= kAhead) {
         tile_barrier();
         const int next = next_tile(t);
@@ -244,8 +244,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
 template <typename T, int kDim, bool kShared, bool kDk, bool kDv>
 __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1) void dkv_kernel(DocAttention a) {
     using Shape = TileShape<T, kDim>;
-    constexpr bool kPipelined = sizeof(T) == 2 && kDim == 128;
-    constexpr int kTile = kPipelined ? 128 : kStream<T, kDim>;
+    constexpr int kTile = kStream<T, kDim>;
     using Copy = TileCopy<T, kDim, kTile, kDocThreads>;
     constexpr int kTileBytes = Copy::kBytes;
     constexpr bool kPaired = kPair<T, kDim> == 2;
@@ -264,7 +263,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     if (!locate_tile<kOwn, false>(a, blockIdx.x / a.heads, doc, first)) return;
 
     const bool few = doc.end - doc.start <= kFewTokens;
-    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
+    const int wave = uniform(static_cast<int>(threadIdx.x) >> 6), lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
     const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
     const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
     const bool working = wave_first < doc.end;
@@ -335,17 +334,21 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     auto write_stat = [&](int buffer, float value) {
         if (static_cast<int>(threadIdx.x) < 2 * kTile) (&stats[buffer][0][0])[threadIdx.x] = value;
     };
+    // (read a tile ahead of their writing to LDS, which is a tile ahead of their use)
     if (kAhead) write_stat(0, read_stat(t));
+    float ahead = read_stat(t + (kAhead ? 1 : 0));
+    loads_arrived();
     for (int buffer = 0; t < tiles; buffer ^= kAhead, ++t) {
         tile_barrier();
         if (!kAhead) {
-            write_stat(0, read_stat(t));
+            write_stat(0, ahead);
             fetch(t, 0);
             tile_barrier();
         } else if (t + 1 < tiles) {
-            write_stat(buffer ^ 1, read_stat(t + 1));
-            fetch(t + 1, buffer ^ 1);
+            write_stat(buffer ^ 1, ahead);
         }
+        ahead = read_stat(t + (kAhead ? 2 : 1));
+        if (kAhead && t + 1 < tiles) fetch(t + 1, buffer ^ 1);
         const LdsByte* const q_tile = buffers + buffer * 2 * kTileBytes;
         const LdsByte* const d_tile = q_tile + kTileBytes;
         const int from = doc.start + t * kTile;
@@ -363,10 +366,8 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
             multiply_rows(view, q_tile, b, k, part, x);
             if constexpr (kDk) multiply_rows(view, d_tile, b, v, part, dp);
         };
-        // ... their weights and dS; kPlain: every key sees them, no cap and no bias ...
-        auto weights = [&](int b, const Acc& x_in, const Acc& dp, auto plain, float (&p)[16], float (&ds)[16]) {
-            constexpr bool kPlain = decltype(plain)::value;
-            float x[16];
+        // ... their weights and dS ...
+        auto weights = [&](int b, Acc& x, const Acc& dp, float (&p)[16], float (&ds)[16]) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const Four base = *reinterpret_cast<const Four*>(tile_base + 32 * b + 8 * g);
@@ -375,10 +376,9 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
                 for (int r = 0; r < 4; ++r) {
                     p[4 * g + r] = base[r];
                     ds[4 * g + r] = kWeightShift<T> != 0.0f ? fmaf(dp[4 * g + r], into, -delta[r]) : dp[4 * g + r] - delta[r];
-                    x[4 * g + r] = x_in[4 * g + r];
                 }
             }
-            if (!kPlain && cap.capped) {
+            if (cap.capped) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     x[r] = cap.bend(x[r]);
@@ -388,12 +388,12 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
             }
 #pragma unroll
             for (int r = 0; r < 16; ++r) p[r] = fmaf(x[r], cap.times, -p[r]);
-            if (!kPlain && a.slopes) {
+            if (a.slopes) {
                 const float away = static_cast<float>(from + 32 * b + 4 * half - j);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) p[r] = fmaf(-slope, fabsf(away + static_cast<float>(8 * (r / 4) + r % 4)), p[r]);
             }
-            if (!kPlain && !all_seen) {
+            if (!all_seen) {
                 const int to_low = span.low - from - 32 * b - 4 * half;
                 const unsigned width = static_cast<unsigned>(span.high - span.low);
 #pragma unroll
@@ -415,42 +415,25 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
             if constexpr (kDk) multiply_columns<T, kDim, kTile>(view, q_tile, b, ds, first_part, dk);
         };
         constexpr int kBlocks = kTile / 32;
-        if (kPipelined && all_seen && !cap.capped && !a.slopes && !few) {
-            // One wave to a SIMD: the matrix cores work on the next queries' scores and the last ones' sums while the vector
-            // unit has this one's weights.
-            Acc x[2], dp[2];
-            products(0, x[0], dp[0]);
-            float p[16], ds[16];
-            weights(0, x[0], dp[0], std::true_type{}, p, ds);
-            if constexpr (kBlocks > 1) products(1, x[1], dp[1]);
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                const Rows16<T> pb(p), dsb(ds);
-                if (b + 1 < kBlocks) weights(b + 1, x[(b + 1) & 1], dp[(b + 1) & 1], std::true_type{}, p, ds);
-                add(b, pb, dsb);
-                if (b + 2 < kBlocks) products(b + 2, x[b & 1], dp[b & 1]);
+        for (int b = 0; b < kBlocks; ++b) {
+            Acc x{}, dp{};
+            if (!kPaired || !idle) products(b, x, dp);
+            if constexpr (kPaired) {
+                static_assert(kBlocks == 1);
+                if constexpr (kDk)
+                    exchange({&x, &dp}, (LdsByte*)pair_lds);
+                else
+                    exchange({&x}, (LdsByte*)pair_lds);
+                if (idle) continue;
             }
-        } else {
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                Acc x{}, dp{};
-                if (!kPaired || !idle) products(b, x, dp);
-                if constexpr (kPaired) {
-                    static_assert(kBlocks == 1);
-                    if constexpr (kDk)
-                        exchange({&x, &dp}, (LdsByte*)pair_lds);
-                    else
-                        exchange({&x}, (LdsByte*)pair_lds);
-                    if (idle) continue;
-                }
-                float p[16], ds[16];
-                weights(b, x, dp, std::false_type{}, p, ds);
+            float p[16], ds[16];
+            weights(b, x, dp, p, ds);
+            add(b, Rows16<T>(p), Rows16<T>(ds));
+            if (kPlanes<T> == 1 && few) {
+                keep_rest<T>(p);
+                keep_rest<T>(ds);
                 add(b, Rows16<T>(p), Rows16<T>(ds));
-                if (kPlanes<T> == 1 && few) {
-                    keep_rest<T>(p);
-                    keep_rest<T>(ds);
-                    add(b, Rows16<T>(p), Rows16<T>(ds));
-                }
             }
         }
     }

@@ -43,7 +43,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kD
     if (!locate_tile<kOwn, true>(a, blockIdx.x / a.heads, doc, first)) return;
 
     const bool few = doc.end - doc.start <= kFewTokens;
-    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
+    const int wave = uniform(static_cast<int>(threadIdx.x) >> 6), lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
     const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
     const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
     const bool working = wave_first < doc.end;
@@ -84,6 +84,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kD
         for (int r = 0; r < 16; ++r) o[p][r] = 0.0f;
     float m = -INFINITY, l = 0.0f;
 
+    loads_arrived();
     for (int buffer = 0; t < tiles; buffer ^= kAhead) {
         tile_barrier();
         const int next = next_tile(t);
