@@ -378,13 +378,51 @@ struct PackArgs {
     int heads[4];
     int tokens, head_dim;
     bool whole;
+    const void* out;  // backward: with dout, for
+    float *delta, *dout_norm;
+    int skip;  // arrays that need no copy: all four, or none
 };
 
+// dout . out of every token and head, and float16's norm of dout: 16 lanes to a row, 16 bytes of it to a lane at a time.
+template <typename T>
+__device__ __forceinline__ void row_products(const PackArgs& a) {
+    constexpr int kWide = kChunk<T>, kLanes = 16;
+    const int lane = static_cast<int>(threadIdx.x) % kLanes;
+    for (int64_t token = blockIdx.x; token < a.tokens; token += gridDim.x)
+        for (int head = static_cast<int>(threadIdx.x) / kLanes; head < a.heads[3]; head += 256 / kLanes) {
+            const int64_t at = token * a.stride[3] + static_cast<int64_t>(head) * a.head_dim;
+            const T* const out = static_cast<const T*>(a.out) + at;
+            const T* const dout = static_cast<const T*>(a.from[3]) + at;
+            float sum = 0.0f, squares = 0.0f;
+            for (int d = lane * kWide; d < a.head_dim; d += kLanes * kWide) {
+                float o[kWide] = {}, g[kWide] = {};
+                if (a.whole) {
+                    load_as_float<T, kWide>(out + d, o);
+                    load_as_float<T, kWide>(dout + d, g);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < kWide; ++j)
+                        if (d + j < a.head_dim) o[j] = static_cast<float>(out[d + j]), g[j] = static_cast<float>(dout[d + j]);
+                }
+#pragma unroll
+                for (int j = 0; j < kWide; ++j) sum = fmaf(o[j], g[j], sum), squares = fmaf(g[j], g[j], squares);
+            }
+#pragma unroll
+            for (int s = kLanes / 2; s > 0; s >>= 1) sum += __shfl_xor(sum, s), squares += __shfl_xor(squares, s);
+            if (lane == 0) {
+                const int64_t row = static_cast<int64_t>(head) * a.tokens + token;
+                a.delta[row] = sum;
+                if (a.dout_norm) a.dout_norm[row] = sqrtf(squares);
+            }
+        }
+}
+
 // Copies arrays into sources: split into planes, heads filled up with zeroes to whole chunks. A workgroup has some tokens, a
-// thread a chunk of 8 elements at a time.
+// thread a chunk of 8 elements at a time. float32's gradients have delta from here, too.
 template <typename T>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
-    const int which = blockIdx.y;
+    const int which = static_cast<int>(blockIdx.y) + a.skip;
+    if (which == 4) return row_products<T>(a);
     const Source to = a.to[which];
     const int per_token = a.heads[which] * to.chunks;
     const int at_once = per_token < 256 ? 256 / per_token : 1;  // tokens of a turn of the workgroup
@@ -433,23 +471,27 @@ void set_sources(DocAttention& a, bool backward, char* packed, hipStream_t strea
     const int heads[4] = {a.heads, a.kv_heads, a.kv_heads, a.heads};
     const int count = backward ? 4 : 3;
     const int chunks = static_cast<int>(ceil_div(a.head_dim, kPartChunk));
-    if (kPlanes<T> == 1 && a.whole) {
-        for (int i = 0; i < count; ++i)
-            a.sources[i] = {static_cast<const char*>(arrays[i]), strides[i] * 2, int64_t{a.head_dim} * 2, 0, chunks};
-        return;
-    }
+    const bool as_they_are = kPlanes<T> == 1 && a.whole;
     PackArgs p{};
     p.tokens = a.tokens;
     p.head_dim = a.head_dim;
     p.whole = a.whole;
     for (int i = 0; i < count; ++i) {
         const int64_t row = int64_t{heads[i]} * chunks * 16, plane = row * a.tokens;
-        a.sources[i] = {packed, row, int64_t{chunks} * 16, plane, chunks};
-        packed += plane * kPlanes<T>;
+        if (as_they_are) {
+            a.sources[i] = {static_cast<const char*>(arrays[i]), strides[i] * 2, int64_t{a.head_dim} * 2, 0, chunks};
+        } else {
+            a.sources[i] = {packed, row, int64_t{chunks} * 16, plane, chunks};
+            packed += plane * kPlanes<T>;
+        }
         p.from[i] = arrays[i], p.stride[i] = strides[i], p.to[i] = a.sources[i], p.heads[i] = heads[i];
     }
+    p.out = a.out, p.delta = a.delta, p.dout_norm = a.dout_norm;
+    p.skip = as_they_are ? 4 : 0;
+    const int parts = (as_they_are ? 0 : count) + (backward ? 1 : 0);
+    if (!parts) return;
     const size_t blocks = ceil_div(static_cast<size_t>(a.tokens) * a.heads * chunks, 256);
-    pack_kernel<T><<<dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), count), 256, 0, stream>>>(p);
+    pack_kernel<T><<<dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096), parts), 256, 0, stream>>>(p);
 }
 
 // doc_attention_{f32,bf16,f16}.hip

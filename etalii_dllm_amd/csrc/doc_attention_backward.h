@@ -3,10 +3,15 @@
 //   p_ij = exp(s_ij - lse_i),  dP = dout v^T,  dS = p (dP - dout . out) cap' scale,
 //   dq = dS k,  dk = dS^T q,  dv = p^T dout
 //
-// Two kernels, each computing scores and dP for itself, so that every gradient is summed by one wave in one order: dq for 128
-// queries of a head over their keys, then dk and dv for 128 keys over the queries of one head that see them. That is
-// seven products instead of five; sums of dq across workgroups by atomic additions would save two and give other bits every time.
-// Heads that share keys leave their dk and dv in float32 and a third kernel adds them in head order.
+// dout . out of every row comes first (pack_kernel). Then there are two kinds of workgroups, each computing scores and dP for
+// itself, so that every gradient is summed by one wave in one order: dq for 128 queries of a head over their keys, and dk and
+// dv for 128 keys over the queries of one head that see them. That is seven products instead of five; sums of dq across
+// workgroups by atomic additions would save two and give other bits every time. Heads that share keys leave their dk and dv in
+// float32 and a last kernel adds them in head order.
+//
+// Both kinds run in one launch where that costs neither of them waves per CU (gradients_kernel): each fills the other's ends,
+// and short calls have half the way (4 float32 documents of 256 tokens, 9/3 heads of 64: 71 to 48 us; 2521 tokens of
+// 4/2 heads of 256: 655 to 383 us).
 #pragma once
 
 #include <float.h>
@@ -43,7 +48,7 @@ __device__ __forceinline__ float power_of_two_above(float x) {
 
 // ---- dq ----
 template <typename T, int kDim>
-__global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1) void dq_kernel(DocAttention a) {
+__device__ __forceinline__ void dq_tile(const DocAttention& a, unsigned block, LdsByte* buffers, LdsByte* pair_lds) {
     using Shape = TileShape<T, kDim>;
     constexpr int kTile = kStream<T, kDim>;
     using Copy = TileCopy<T, kDim, kTile, kDocThreads>;
@@ -51,15 +56,13 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     constexpr bool kPaired = kPair<T, kDim> == 2;
     constexpr int kParts = kWaveDim<T, kDim> / 32, kOwn = kBlockRows<T, kDim>;
     constexpr bool kAhead = kStreamBuffers<T, kDim> == 2;
-    __shared__ __attribute__((aligned(1024))) char lds[kStreamBuffers<T, kDim> * 2 * kTileBytes];
-    __shared__ __attribute__((aligned(16))) char pair_lds[kPaired ? 2 * 4 * 4096 : 16];
 
-    const int turn = static_cast<int>(blockIdx.x) % a.heads;
+    const int turn = static_cast<int>(block) % a.heads;
     const int head = (turn % a.kv_heads) * a.group + turn / a.kv_heads;
     const int kv = head / a.group;
     Document doc;
     int first;
-    if (!locate_tile<kOwn, true>(a, blockIdx.x / a.heads, doc, first)) return;
+    if (!locate_tile<kOwn, true>(a, block / a.heads, doc, first)) return;
 
     const bool few = doc.end - doc.start <= kFewTokens;
     const int wave = uniform(static_cast<int>(threadIdx.x) >> 6), lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
@@ -80,7 +83,6 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
 
     const Copy copy_k(a.sources[1], kv), copy_v(a.sources[2], kv);
     const TileView<T, kDim, kTile> view;
-    LdsByte* const buffers = (LdsByte*)lds;
     // the first tile is on its way while the lane's rows are read
     auto next_tile = [&](int t) { return t + 1 < prefix_tiles ? t + 1 : max(t + 1, low_tile); };
     auto fetch = [&](int t, int buffer) {
@@ -92,54 +94,9 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     if (kAhead) fetch(t, 0);
 
     const Column<T, kDim> q(a.sources[0], head, i, part), dout(a.sources[3], head, i, part);
-    float delta = 0.0f, norm = 0.0f;  // this half's part
-    {
-        const T* const out_row = static_cast<const T*>(a.out) + i * a.out_stride + head_at;
-        const T* const dout_row = static_cast<const T*>(a.dout) + i * a.out_stride + head_at;
-        auto add = [&](float o, float d) {
-            delta = fmaf(o, d, delta);
-            norm = fmaf(d, d, norm);
-        };
-        // (both ways take the same elements in the same order; every load is on its way before the first is used)
-        constexpr int kWide = kChunk<T>, kLoads = kDim / (2 * kWide);
-        if (a.whole) {
-            Pack<T, kWide> o[kLoads], d[kLoads];
-#pragma unroll
-            for (int s = 0; s < kLoads; ++s) {
-                const int d0 = min((2 * s + half) * kWide, a.head_dim - kWide);
-                o[s] = *reinterpret_cast<const Pack<T, kWide>*>(out_row + d0);
-                d[s] = *reinterpret_cast<const Pack<T, kWide>*>(dout_row + d0);
-            }
-#pragma unroll
-            for (int s = 0; s < kLoads; ++s)
-                if ((2 * s + half) * kWide < a.head_dim)
-#pragma unroll
-                    for (int j = 0; j < kWide; ++j) add(static_cast<float>(o[s].v[j]), static_cast<float>(d[s].v[j]));
-        } else {
-#pragma unroll 4
-            for (int d0 = half * kWide; d0 < a.head_dim; d0 += 2 * kWide) {
-                T o[kWide], d[kWide];
-#pragma unroll
-                for (int j = 0; j < kWide; ++j) {
-                    const int at = min(d0 + j, a.head_dim - 1);
-                    o[j] = out_row[at], d[j] = dout_row[at];
-                }
-#pragma unroll
-                for (int j = 0; j < kWide; ++j) {
-                    const bool there = d0 + j < a.head_dim;
-                    add(there ? static_cast<float>(o[j]) : 0.0f, there ? static_cast<float>(d[j]) : 0.0f);
-                }
-            }
-        }
-    }
-    delta += other_half(delta);
+    const float delta = a.delta[stat_at];
     float dout_scale = 1.0f;
-    if constexpr (kWeightShift<T> != 0.0f) {
-        norm = sqrtf(norm + other_half(norm));
-        dout_scale = power_of_two_above(norm);
-        if (mine && half == 0 && part == 0) a.dout_norm[stat_at] = norm;
-    }
-    if (mine && half == 0 && part == 0) a.delta[stat_at] = delta;
+    if constexpr (kWeightShift<T> != 0.0f) dout_scale = power_of_two_above(a.dout_norm[stat_at]);
     const float into = 1.0f / dout_scale;  // exact
 
     const CapTerms<T> cap(a);
@@ -180,7 +137,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
             }
             if constexpr (kPaired) {
                 static_assert(kTile == 32);
-                exchange({&x, &dp}, (LdsByte*)pair_lds);
+                exchange({&x, &dp}, pair_lds);
                 if (idle) continue;
             }
             float ds[16];
@@ -224,7 +181,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
     if (!kPaired && !working) return;
     const uint64_t marks = __ballot(!all_finite(dq) && mine);
     uint32_t spoilt = static_cast<uint32_t>(marks) | static_cast<uint32_t>(marks >> 32);
-    if constexpr (kPaired) spoilt = pair_marks(spoilt, (LdsByte*)pair_lds);
+    if constexpr (kPaired) spoilt = pair_marks(spoilt, pair_lds);
     T* const to = static_cast<T*>(a.dq) + head_at;
     if (mine && !(spoilt >> (lane & 31) & 1))
         store_column(to + i * a.q_stride, a.head_dim, a.whole, first_part, dq, a.scale * dout_scale * __builtin_amdgcn_exp2f(-kWeightShift<T>));
@@ -239,10 +196,10 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 128 ? 2 : 1
 // ---- dk and dv of one head ----
 //
 // kShared: into the float32 parts of heads that share keys. kDk, kDv: which of the two; rows of more than kTogether
-// elements take a launch for each, since the sums of both and a lane's two rows are more than its registers (five products
+// elements for a wave take a workgroup for each, since the sums of both and a lane's two rows are more than its registers (five products
 // in all instead of four).
 template <typename T, int kDim, bool kShared, bool kDk, bool kDv>
-__global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1) void dkv_kernel(DocAttention a) {
+__device__ __forceinline__ void dkv_tile(const DocAttention& a, unsigned block, LdsByte* buffers, LdsByte* pair_lds) {
     using Shape = TileShape<T, kDim>;
     constexpr int kTile = kStream<T, kDim>;
     using Copy = TileCopy<T, kDim, kTile, kDocThreads>;
@@ -250,17 +207,15 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     constexpr bool kPaired = kPair<T, kDim> == 2;
     constexpr int kParts = kWaveDim<T, kDim> / 32, kOwn = kBlockRows<T, kDim>;
     constexpr bool kAhead = kStreamBuffers<T, kDim> == 2;
-    __shared__ __attribute__((aligned(1024))) char lds[(kAhead ? 4 : 2) * kTileBytes];
     __shared__ __attribute__((aligned(16))) float stats[2][2][kTile];  // lse in units of log 2, and dout . out, of a tile's queries
     __shared__ float largest[kDocThreads / 64];
-    __shared__ __attribute__((aligned(16))) char pair_lds[kPaired ? 2 * 4 * 4096 : 16];
 
-    const int turn = static_cast<int>(blockIdx.x) % a.heads;
+    const int turn = static_cast<int>(block) % a.heads;
     const int head = (turn % a.kv_heads) * a.group + turn / a.kv_heads;
     const int kv = head / a.group;
     Document doc;
     int first;
-    if (!locate_tile<kOwn, false>(a, blockIdx.x / a.heads, doc, first)) return;
+    if (!locate_tile<kOwn, false>(a, block / a.heads, doc, first)) return;
 
     const bool few = doc.end - doc.start <= kFewTokens;
     const int wave = uniform(static_cast<int>(threadIdx.x) >> 6), lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
@@ -286,7 +241,6 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
 
     const Copy copy_q(a.sources[0], head), copy_d(a.sources[3], head);
     const TileView<T, kDim, kTile> view;
-    LdsByte* const buffers = (LdsByte*)lds;
     auto fetch = [&](int t, int buffer) {
         const int from = doc.start + t * kTile;
         copy_q(from, doc.end - from, buffers + buffer * 2 * kTileBytes);
@@ -296,7 +250,6 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     int t = low_tile;
     if (kAhead) fetch(t, 0);
     const Column<T, kDim> k(a.sources[1], kv, j, part), v(a.sources[2], kv, j, part);
-
 
     float dout_scale = 1.0f;
     if constexpr (kWeightShift<T> != 0.0f && kDk) {
@@ -422,9 +375,9 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
             if constexpr (kPaired) {
                 static_assert(kBlocks == 1);
                 if constexpr (kDk)
-                    exchange({&x, &dp}, (LdsByte*)pair_lds);
+                    exchange({&x, &dp}, pair_lds);
                 else
-                    exchange({&x}, (LdsByte*)pair_lds);
+                    exchange({&x}, pair_lds);
                 if (idle) continue;
             }
             float p[16], ds[16];
@@ -441,7 +394,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     const float unshift = __builtin_amdgcn_exp2f(-kWeightShift<T>), dk_factor = a.scale * dout_scale * unshift;
     const uint64_t marks = __ballot(!(all_finite(dk) && all_finite(dv)) && mine);
     uint32_t spoilt = static_cast<uint32_t>(marks) | static_cast<uint32_t>(marks >> 32);
-    if constexpr (kPaired) spoilt = pair_marks(spoilt, (LdsByte*)pair_lds);
+    if constexpr (kPaired) spoilt = pair_marks(spoilt, pair_lds);
     // row `at` of dk and dv, by `store` of its place and its factor
     auto rows_of = [&](int64_t at, auto&& store) {
         const int64_t part = (stat_at + at) * a.head_dim;
@@ -464,6 +417,51 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
             if constexpr (kDv) store_row(to_dv, dv1, a.head_dim);
         });
     }
+}
+
+// LDS of a workgroup: the tiles, and what a pair of waves exchanges.
+template <typename T, int kDim>
+constexpr int kTilesBytes = kStreamBuffers<T, kDim> * 2 * TileCopy<T, kDim, kStream<T, kDim>, kDocThreads>::kBytes;
+template <typename T, int kDim>
+constexpr int kExchangeBytes = kPair<T, kDim> == 2 ? 2 * 4 * 4096 : 16;
+
+// All gradients at once: dk and dv (blockIdx.y 0; dv 2 where it is on its own), whose workgroups take longer, before dq (1).
+template <typename T, int kDim, bool kShared>
+__global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1) void gradients_kernel(DocAttention a) {
+    __shared__ __attribute__((aligned(1024))) char lds[kTilesBytes<T, kDim>];
+    __shared__ __attribute__((aligned(16))) char exchanged[kExchangeBytes<T, kDim>];
+    LdsByte* const buffers = (LdsByte*)lds;
+    LdsByte* const pair_lds = (LdsByte*)exchanged;
+    const unsigned block = blockIdx.x, turn = blockIdx.y;
+    if constexpr (kWaveDim<T, kDim> <= kTogether) {
+        if (turn == 0) return dkv_tile<T, kDim, kShared, true, true>(a, block, buffers, pair_lds);
+    } else {
+        if (turn == 0) return dkv_tile<T, kDim, kShared, true, false>(a, block, buffers, pair_lds);
+        if (turn == 2) return dkv_tile<T, kDim, kShared, false, true>(a, block, buffers, pair_lds);
+    }
+    dq_tile<T, kDim>(a, block, buffers, pair_lds);
+}
+
+// 16-bit heads of 65 to 128 elements: dq alone fits twice on a CU, dk and dv do not. With more than kFewTiles workgroups of
+// each kind a kernel for each is faster (16/8 heads of 128 in bfloat16, microseconds together and apart: 2048 tokens, 272
+// workgroups, 111 and 163; 3071 tokens, 400, 215 and 234; 4096 tokens, 528, 339 and 329; 8192 tokens, 1040, 1184 and 1045).
+// Both ways run the same code and give the same bits.
+template <typename T, int kDim>
+constexpr bool kApart = kPlanes<T> == 1 && kDim == 128;
+constexpr unsigned kFewTiles = 512;
+
+template <typename T, int kDim>
+__global__ __launch_bounds__(kDocThreads, 2) void dq_kernel(DocAttention a) {
+    static_assert(kApart<T, kDim>);
+    __shared__ __attribute__((aligned(1024))) char lds[kTilesBytes<T, kDim>];
+    dq_tile<T, kDim>(a, blockIdx.x, (LdsByte*)lds, nullptr);
+}
+
+template <typename T, int kDim, bool kShared>
+__global__ __launch_bounds__(kDocThreads, 1) void dkv_kernel(DocAttention a) {
+    static_assert(kApart<T, kDim>);
+    __shared__ __attribute__((aligned(1024))) char lds[kTilesBytes<T, kDim>];
+    dkv_tile<T, kDim, kShared, true, true>(a, blockIdx.x, (LdsByte*)lds, nullptr);
 }
 
 // dk and dv of the tokens of documents: the group's heads added in order. kWidth elements to a thread.
@@ -494,24 +492,25 @@ __global__ __launch_bounds__(kDocThreads) void add_heads_kernel(DocAttention a) 
     }
 }
 
-template <typename T, int kDim, bool kDk, bool kDv>
-void launch_dkv(const DocAttention& a, dim3 grid, hipStream_t s) {
-    if (a.group == 1)
-        dkv_kernel<T, kDim, false, kDk, kDv><<<grid, kDocThreads, 0, s>>>(a);
-    else
-        dkv_kernel<T, kDim, true, kDk, kDv><<<grid, kDocThreads, 0, s>>>(a);
+template <typename T, int kDim, bool kShared>
+void launch_gradients(const DocAttention& a, hipStream_t s) {
+    const unsigned tiles = doc_tiles(a, kBlockRows<T, kDim>) * a.heads;
+    if constexpr (kApart<T, kDim>) {
+        if (tiles > kFewTiles) {
+            dkv_kernel<T, kDim, kShared><<<tiles, kDocThreads, 0, s>>>(a);
+            dq_kernel<T, kDim><<<tiles, kDocThreads, 0, s>>>(a);
+            return;
+        }
+    }
+    gradients_kernel<T, kDim, kShared><<<dim3(tiles, kWaveDim<T, kDim> <= kTogether ? 2 : 3), kDocThreads, 0, s>>>(a);
 }
 
 template <typename T, int kDim>
 void launch_gradients(const DocAttention& a, hipStream_t s) {
-    const dim3 grid(doc_tiles(a, kBlockRows<T, kDim>) * a.heads);
-    dq_kernel<T, kDim><<<grid, kDocThreads, 0, s>>>(a);
-    if constexpr (kWaveDim<T, kDim> <= kTogether) {
-        launch_dkv<T, kDim, true, true>(a, grid, s);
-    } else {
-        launch_dkv<T, kDim, true, false>(a, grid, s);
-        launch_dkv<T, kDim, false, true>(a, grid, s);
-    }
+    if (a.group == 1)
+        launch_gradients<T, kDim, false>(a, s);
+    else
+        launch_gradients<T, kDim, true>(a, s);
 }
 
 template <typename T>

@@ -251,6 +251,35 @@ def test_hidden_values_do_not_matter(K, dtype, value, head_dim):
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize("head_dim", [128, 256])
+def test_hidden_values_do_not_matter_to_wide_heads(K, dtype, head_dim):
+    """float32 heads of 256 are shared by pairs of waves, which have to agree on the rows that are spoilt."""
+    test_hidden_values_do_not_matter(K, dtype, float("nan"), head_dim)
+    test_hidden_values_do_not_matter(K, dtype, float("inf"), head_dim)
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize("head_dim", [64, 120, 128, 256])
+@pytest.mark.parametrize("options", [dict(), dict(causal=False, window=50)])
+def test_a_document_in_a_large_pack(K, dtype, head_dim, options):
+    """A document's bits are the same alone and among as many that the gradients are launched otherwise, or the tiles
+    come in another order."""
+    lengths = [(53 * i) % 211 + 7 for i in range(80)]
+    lengths[40] = 600
+    offsets = np.concatenate([[0], np.cumsum(lengths)]).tolist()
+    p, dout = problem(K, 12, R.DTYPES[dtype], offsets, offsets[-1], 8, 2, head_dim, **options)
+    out, lse = p.forward()
+    grads = p.backward(dout)
+    for d in (0, 17, 40, 79):
+        b, e = offsets[d], offsets[d + 1]
+        s = Attention(K, p.q[b:e].clone(), p.k[b:e].clone(), p.v[b:e].clone(), [0, e - b], **options)
+        out1, lse1 = s.forward()
+        assert torch.equal(out1, out[b:e]) and torch.equal(lse1, lse[:, b:e]), d
+        for got, want in zip(s.backward(dout[b:e].clone()), grads):
+            assert torch.equal(got, want[b:e]), d
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
 @pytest.mark.parametrize(("extra", "shift"), [(0, 0), (8, 0), (3, 0), (0, 1)])
 def test_attention_of_a_fused_projection(K, dtype, extra, shift):
     """q, k and v as parts of one projection's rows; strides and starts that are whole 16-byte chunks or not. The gradients
