@@ -221,7 +221,13 @@ constexpr int kLaneDims = kMaxHeadDim / 64;  // head dimensions that a lane of a
 // ---- one row by one wave ----
 //
 // Exactly the formula over the visible keys (queries), 64 of them at a time, one per lane. Nothing of a hidden row
-// is touched.
+// is touched. A weight that is NaN ends it: whatever follows, the row is NaN (so a batch that is NaN throughout costs each row
+// its first keys).
+
+__device__ __forceinline__ void all_nan(float (&v)[kLaneDims]) {
+#pragma unroll
+    for (int c = 0; c < kLaneDims; ++c) v[c] = NAN;
+}
 
 template <typename T>
 __device__ void attention_row(const DocAttention& a, const Document& doc, int head, int i, float (&o)[kLaneDims], float& lse) {
@@ -242,6 +248,11 @@ __device__ void attention_row(const DocAttention& a, const Document& doc, int he
         if (!__any(see)) continue;
         float unused;
         const float x = see ? bend_score(a, slope, dot_row(q, k + j * a.k_stride, a.head_dim), i - j, unused) : -INFINITY;
+        if (__any(x != x)) {
+            all_nan(o);
+            lse = NAN;
+            return;
+        }
         const float top = fmaxf(m, wave_max(x));
         const float p = x == -INFINITY ? 0.0f : expf(x - top);
         const float keep = m == top ? 1.0f : expf(m - top);
@@ -288,6 +299,7 @@ __device__ void attention_row_dq(const DocAttention& a, const Document& doc, int
             const float dp = dot_row(dout, v + j * a.v_stride, a.head_dim);
             ds = expf(x - lse) * (dp - delta) * derivative * a.scale;
         }
+        if (__any(ds != ds)) return all_nan(dq);
         for (uint64_t left = __ballot(see); left; left &= left - 1) {
             const int from_lane = __ffsll(static_cast<unsigned long long>(left)) - 1;
             const float d = __shfl(ds, from_lane);
@@ -325,6 +337,10 @@ __device__ void attention_row_dkv(const DocAttention& a, const Document& doc, in
             const float dp = dot_row(dout + i * a.out_stride, v, a.head_dim);
             p = expf(x - lse[i]);
             ds = p * (dp - delta[i]) * derivative * a.scale;
+        }
+        if (__any(p != p)) {
+            all_nan(dk), all_nan(dv);
+            return;
         }
         for (uint64_t left = __ballot(see); left; left &= left - 1) {
             const int from_lane = __ffsll(static_cast<unsigned long long>(left)) - 1;

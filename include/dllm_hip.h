@@ -269,10 +269,10 @@ int dllm_hip_lora_adapter_gradients(const float* grad, const float* a, const flo
  * into one row of tokens, images among the text, activations in bfloat16 or float16. They have no counterpart in the
  * reference, so no bits to reproduce: sums, softmax statistics and norms are float32, products of float32 activations are
  * float32's to its last bits, those of 16-bit activations have their operands in that type, and each result is rounded to
- * its type once. They keep the library's other promise: results do not
- * depend on what shares the batch. A document's attention, a token's rotation and a row's norm are the same bits
- * alone and in any pack, and every call with the same arguments gives the same bits (no atomic additions). Sums over all rows
- * (the gradients of norm weights and channel gates) depend on the rows alone.
+ * its type once. They keep the library's other promise: results do not depend on what shares the batch. A document's
+ * attention, a token's rotation and a row's norm are the same bits alone and in any pack, and every call with the same
+ * arguments gives the same bits (no atomic additions). Sums over all rows (the gradients of norm weights and channel
+ * gates) depend on the rows alone.
  *
  * dtype is the type of the activations and of their gradients: 0 float32, 1 bfloat16, 2 float16. Parameters (norm
  * weights, channel gates, ALiBi slopes) and their gradients are float32. Activations are aligned to their element; whole
@@ -284,17 +284,17 @@ enum { DLLM_HIP_FLOAT32 = 0, DLLM_HIP_BFLOAT16 = 1, DLLM_HIP_FLOAT16 = 2 };
 /* Attention within packed documents. q[tokens, heads, head_dim], k and v[tokens, kv_heads, head_dim], out like q;
  * token strides in elements (0: heads * head_dim), so q, k and v may be parts of one projection's output. Document d is
  * tokens offsets[d] .. offsets[d + 1] - 1 (device, documents + 1 values, non-decreasing, in [0, tokens]; empty documents
- * are allowed). Tokens of no document count for nothing, and their rows of the outputs are left as they were. A query at position i of its document sees the key
- * at position j of the same document if
+ * are allowed). Tokens of no document count for nothing, and their rows of the outputs are left as they were. A query at
+ * position i of its document sees the key at position j of the same document if
  *     (j <= i or not causal) and (|i - j| < window or window is 0),   or   j < prefix[d]
  * (prefix: device, one length per document, NULL for none: an instruction or image that every token sees). The score is
  *     s = softcap tanh(scale q.k / softcap) - slopes[head] |i - j|
  * (softcap 0: scale q.k; slopes: device, one per head, NULL for none; constants, they get no gradient). out = softmax(s) v and
  * lse[heads, tokens] = log sum exp s, which the backward reads (float32; may be NULL). Keys that a query does not see do
  * not reach its results, whatever they hold.
- * Limits: scale positive, head_dim at most 256, tokens below 2^31, heads a multiple of kv_heads, at most 65535 heads, and
- * (tokens / 64 + documents) * heads below 2^24. Out-of-range
- * offsets and prefixes are clamped to the tokens and the document; documents that then overlap give unspecified values.
+ * Limits: scale positive, head_dim at most 256, heads a multiple of kv_heads, at most 65535 heads, and (tokens / 64 +
+ * documents) * heads below 2^24. Out-of-range offsets and prefixes are clamped to the tokens and the document; documents
+ * that then overlap give unspecified values. Outputs do not overlap inputs, nor the workspace either.
  * The backward takes the forward's out and lse and the upstream gradient dout (out's layout and stride) and writes dq, dk
  * and dv (q's, k's and v's layouts and strides); dk and dv sum over the heads that share them, in head order. */
 typedef struct {

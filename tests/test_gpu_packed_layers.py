@@ -259,6 +259,20 @@ def test_hidden_values_do_not_matter_to_wide_heads(K, dtype, head_dim):
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize("head_dim", [64, 256])
+def test_a_document_of_nan(K, dtype, head_dim):
+    """Of two documents one is NaN throughout: its results are NaN, the other's are what they were."""
+    n = 300
+    p, dout = problem(K, 13, R.DTYPES[dtype], [0, n, 2 * n], 2 * n, 4, 2, head_dim)
+    want = [t.clone() for t in p.forward()] + [t.clone() for t in p.backward(dout)]
+    for t in (p.q, p.k, p.v, dout):
+        t[:n] = float("nan")
+    out, lse = p.forward()
+    for got, ref in zip([out, lse.T, *p.backward(dout)], [want[0], want[1].T, *want[2:]]):
+        assert bool(torch.isnan(got[:n]).all()) and torch.equal(got[n:], ref[n:])
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
 @pytest.mark.parametrize("head_dim", [64, 120, 128, 256])
 @pytest.mark.parametrize("options", [dict(), dict(causal=False, window=50)])
 def test_a_document_in_a_large_pack(K, dtype, head_dim, options):
