@@ -12,6 +12,10 @@
 // Both kinds run in one launch where that costs neither of them waves per CU (gradients_kernel): each fills the other's ends,
 // and short calls have half the way (4 float32 documents of 256 tokens, 9/3 heads of 64: 71 to 48 us; 2521 tokens of
 // 4/2 heads of 256: 655 to 383 us).
+//
+// Bound: the matrix cores, as the forward is. 8192 tokens, 16/8 heads of 128 in bfloat16: dq 405 us, 1020 TFLOP/s of its three
+// products; dk and dv 605 to 660 us, 830 to 910 of four; all together 1040 us, 660 TFLOP/s of the five that it could not do
+// without. A second order of dk's and dv's products, with the next tile's scores formed before this one's sums, took 816 us.
 #pragma once
 
 #include <float.h>
@@ -464,7 +468,8 @@ __global__ __launch_bounds__(kDocThreads, 1) void dkv_kernel(DocAttention a) {
     dkv_tile<T, kDim, kShared, true, true>(a, blockIdx.x, (LdsByte*)lds, nullptr);
 }
 
-// dk and dv of the tokens of documents: the group's heads added in order. kWidth elements to a thread.
+// dk and dv of the tokens of documents: the group's heads added in order. kWidth elements to a thread. Bound: HBM (8192 tokens,
+// 16/8 heads of 128: 32 us, 5.2 TB/s).
 template <typename T, int kWidth>
 __global__ __launch_bounds__(kDocThreads) void add_heads_kernel(DocAttention a) {
     const int per_row = (a.head_dim + kWidth - 1) / kWidth, per_token = a.kv_heads * per_row;

@@ -1,5 +1,5 @@
 // Attention within packed documents, forward, of 16-bit heads wider than 128: compiled with the sums in accumulation registers
-// (build.py), which leaves the others to operands read ahead (8192 tokens, 8/4 heads of 256: 465 to 430 us).
+// (build.py), which leaves the others to operands read ahead (8192 tokens, 8/4 heads of 256: 438 to 382 us).
 #include "doc_attention_forward.h"
 
 namespace dllm_hip {

@@ -6,7 +6,9 @@
 // g = dh + r_h w dn - h c_h) sum w gate scale g y. All sums are float32, each thread's terms in column order, then the
 // threads of a wave and the waves of a workgroup in a fixed tree: a row's bits depend on the row alone.
 //
-// Bound: HBM, each row array read and written once.
+// Bound: HBM, each row array read and written once. 8192 x 2304 in bfloat16: forward 31.7 us, 4.8 TB/s; gradients 68 us, 3.3 TB/s,
+// where two sums in a row over the workgroup leave gaps that its two or three workgroups on a CU do not fill (8192 x 4096: 87 us,
+// 4.6 TB/s). 4099 x 2048 in float32 with a channel gate: 49 us, 4.1 TB/s.
 #include <algorithm>
 #include <initializer_list>
 
@@ -432,7 +434,8 @@ __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
         }
     };
     // Parameters stay in registers where they are few, else in LDS (each thread its own): a load from memory here would be
-    // waited for together with the next row's.
+    // waited for together with the next row's. (8192 rows of bfloat16, eight elements to a thread, registers and LDS: 4096 wide
+    // 87 and 91 us, 2304 wide 70 and 64, 896 wide 25 and 28.)
     constexpr bool kHeld = kVectors * kWidth <= 8;
     extern __shared__ __attribute__((aligned(16))) float parameter_lds[];  // [3][blockDim * kVectors * kWidth], or nothing
     float held[3][kHeld ? kVectors : 1][kWidth];

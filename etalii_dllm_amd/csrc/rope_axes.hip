@@ -6,7 +6,8 @@
 // at any position. All heads of a token share its angles: a workgroup computes the sines and cosines of its tokens once
 // into LDS, then turns every head of q and k.
 //
-// Bound: HBM, each element read and written once; per element a multiply, an FMA and 4 bytes of LDS.
+// Bound: HBM, each element read and written once; per element a multiply, an FMA and 4 bytes of LDS. 16384 tokens, 12/2 heads of
+// 128 in bfloat16: 28 us, 4.2 TB/s. One token: 7.5 us, the launch.
 #include <math.h>
 
 #include <algorithm>
@@ -175,7 +176,8 @@ extern "C" int dllm_hip_rope_axes(const dllm_hip_rope_axes_shape* sh, const void
     a.axes = static_cast<int>(sh->axes);
     a.inverse = sh->inverse != 0;
     // Tokens of a workgroup: enough for about four items to a thread, as far as their angles fit the table and there are
-    // workgroups for all CUs. (16384 tokens, 12/2 heads of 128 in bfloat16: 31 us with one token each.)
+    // workgroups for all CUs. (16384 tokens, 12/2 heads of 128 in bfloat16: 31 us with one token
+    // each, 28 with these.)
     const int64_t width = wide ? chunk : 1, pair_width = sh->interleaved ? std::max<int64_t>(width / 2, 1) : width;
     const int64_t items = (sh->q_heads + sh->k_heads) * (sh->pairs / pair_width + (sh->head_dim - 2 * sh->pairs) / width);
     const int64_t by_items = 4 * kThreads / std::max<int64_t>(items, 1), by_table = kTableEntries / std::max<int64_t>(sh->pairs, 1);
