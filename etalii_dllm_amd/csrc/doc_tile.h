@@ -245,17 +245,41 @@ __device__ __forceinline__ void keep_rest(float (&x)[16]) {
     for (int r = 0; r < 16; ++r) x[r] -= static_cast<float>(static_cast<Part<T>>(x[r]));
 }
 
-// The order that the compiler is asked to keep between LDS reads and products: kFirst reads ahead, then kReads for every
-// kProducts products. Left alone it reads one operand, waits for it and multiplies, which leaves the matrix cores idle for
-// the LDS's latency every time.
-constexpr int kAheadSteps = 2;  // measured: 3, 4 and 6 are no faster, and take registers
-template <int kCount, int kFirst, int kReads, int kProducts>
-__device__ __forceinline__ void reads_ahead() {
-    __builtin_amdgcn_sched_group_barrier(0x100, kFirst, 0);
+// kSteps products, each of kReads LDS reads that are begun some steps before their use. Left alone the compiler reads an operand,
+// waits for it and multiplies, which leaves the matrix cores idle for the LDS's latency every time.
+//
+// One wave on a SIMD (float32, heads of 256) has no other to fill such waits: the order is held by scheduling barriers that reads
+// and products do not cross. More waves do better where the compiler is only asked for an order (microseconds, asked and held:
+// 4096 float32 tokens of 16/8 heads of 128, gradients 1306 and 1228; 8192 bfloat16 tokens of 8/4 heads of 256, 1400 and
+// 1222; of 16/8 heads of 128, 1154 and 1188; of 64, forward, 175 to 183 both).
+template <typename T, int kDim>
+constexpr bool kOrderHeld = kPlanes<T> == 3 || kDim > 128;
+template <typename T, int kDim>
+constexpr int kAheadSteps = kPlanes<T> == 3 ? 1 : 2;  // measured: one more, two more and four more are no faster, and take registers
+template <typename T, int kDim, int kSteps, int kReads, typename Read, typename Multiply>
+__device__ __forceinline__ void multiply_steps(Read&& read, Multiply&& multiply_step) {
+    constexpr int kAhead = kAheadSteps<T, kDim>;
+    if constexpr (kOrderHeld<T, kDim>) {
+        constexpr int kMayCross = 0x2 | 0x4 | 0x400;  // vector, scalar and transcendental arithmetic
+        decltype(read(0)) held[kAhead + 1];
 #pragma unroll
-    for (int i = 0; i < kCount; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x8, kProducts, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+        for (int i = 0; i < kAhead; ++i) held[i] = read(i);
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+            if (step + kAhead < kSteps) held[(step + kAhead) % (kAhead + 1)] = read(step + kAhead);
+            __builtin_amdgcn_sched_barrier(kMayCross);
+            multiply_step(step, held[step % (kAhead + 1)]);
+            __builtin_amdgcn_sched_barrier(kMayCross);
+        }
+    } else {
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) multiply_step(step, read(step));
+        __builtin_amdgcn_sched_group_barrier(0x100, kAhead * kReads, 0);  // LDS reads, ...
+#pragma unroll
+        for (int step = 0; step < kSteps; ++step) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);  // ... a product, and the reads of a later one
+            __builtin_amdgcn_sched_group_barrier(0x100, kReads, 0);
+        }
     }
 }
 
@@ -263,12 +287,9 @@ __device__ __forceinline__ void reads_ahead() {
 template <typename T, int kDim, int kRows, int kParts>
 __device__ __forceinline__ void multiply_columns(const TileView<T, kDim, kRows>& view, const LdsByte* tile, int block,
                                                  const Rows16<T>& x, int first, Acc (&acc)[kParts]) {
-#pragma unroll
-    for (int g = 0; g < 2; ++g)
-#pragma unroll
-        for (int p = 0; p < kParts; ++p)
-            multiply<T>(view.columns(tile, block, g, kParts * 32 == kDim ? p : first + p), x.group[g], acc[p]);
-    reads_ahead<2 * kParts, 2 * kAheadSteps * kPlanes<T>, 2 * kPlanes<T>, kPlanes<T> == 3 ? 6 : 1>();
+    multiply_steps<T, kDim, 2 * kParts, 2>(
+        [&](int s) { return view.columns(tile, block, s / kParts, kParts * 32 == kDim ? s % kParts : first + s % kParts); },
+        [&](int s, const Chunks<T>& a) { multiply<T>(a, x.group[s / kParts], acc[s % kParts]); });
 }
 
 // Wide float32 heads: a lane's rows and sums in three planes are more than the registers, so a pair of waves shares 32 rows
@@ -307,10 +328,9 @@ template <typename T, int kDim, int kRows>
 __device__ __forceinline__ void multiply_rows(const TileView<T, kDim, kRows>& view, const LdsByte* tile, int block,
                                               const Column<T, kDim>& column, int part, Acc& acc) {
     constexpr int kSteps = Column<T, kDim>::kSteps;
-#pragma unroll
-    for (int step = 0; step < kSteps; ++step)
-        multiply<T>(view.rows(tile, block, kPair<T, kDim> == 1 ? step : step + part * kSteps), column.held[step], acc);
-    reads_ahead<kSteps, kAheadSteps * kPlanes<T>, kPlanes<T>, kPlanes<T> == 3 ? 6 : 1>();
+    multiply_steps<T, kDim, kSteps, 1>(
+        [&](int s) { return view.rows(tile, block, kPair<T, kDim> == 1 ? s : s + part * kSteps); },
+        [&](int s, const Chunks<T>& a) { multiply<T>(a, column.held[s], acc); });
 }
 
 // The pair's sums: each wave leaves its own in LDS (4 KB for each 32 x 32), and after the barrier adds the other's. All waves
