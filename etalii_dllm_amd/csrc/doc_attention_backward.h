@@ -10,12 +10,14 @@
 // float32 and a last kernel adds them in head order.
 //
 // Both kinds run in one launch where that costs neither of them waves per CU (gradients_kernel): each fills the other's ends,
-// and short calls have half the way (4 float32 documents of 256 tokens, 9/3 heads of 64: 71 to 48 us; 2521 tokens of
+// and short calls have half the way (4 float32 documents of 256 tokens, 9/3 heads of 64: 71 to 48 us; 2447 tokens of
 // 4/2 heads of 256: 655 to 383 us).
 //
 // Bound: the matrix cores, as the forward is. 8192 tokens, 16/8 heads of 128 in bfloat16: dq 405 us, 1020 TFLOP/s of its three
-// products; dk and dv 605 to 660 us, 830 to 910 of four; all together 1040 us, 660 TFLOP/s of the five that it could not do
-// without. A second order of dk's and dv's products, with the next tile's scores formed before this one's sums, took 816 us.
+// products; dk and dv 605 to 660 us, 830 to 910 of four; all together 1040 to 1150 us, 600 to 660 TFLOP/s of the five that it
+// could not do without. 8/4 heads of 256, where dk and dv are two kinds of workgroups and eight products in all: 1220 us.
+// Another order of dk's and dv's products, with the next tile's scores formed before this one's sums, took 816 us for heads
+// of 128.
 #pragma once
 
 #include <float.h>

@@ -28,7 +28,7 @@ constexpr int kBuffers = 4 * kKeys<T, kDim> * kDim * 2 * kPlanes<T> <= 128 * 102
 // nothing else. 8192 tokens in bfloat16, of the scores that count: 16/8 heads of 128, 320 to 364 us, 755 to 860 TFLOP/s (567 us
 // and 970 without the causal mask); of 64, 174 us and 790; 8/4 heads of 256, 355 us and 775. float32, 4096 tokens, 16/8 heads of
 // 128: 420 us, of six products 980. Short calls are bound by the way of one workgroup through a row's keys: about 1.1 us a tile
-// of 64 (16-bit), 3.3 us one of 32 (float32).
+// of 64 (16-bit), 3.1 us one of 32 (float32).
 template <typename T, int kDim>
 __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kDim <= 128 ? 2 : 1) : 1) void forward_kernel(DocAttention a, T* out) {
     using Shape = TileShape<T, kDim>;
