@@ -251,16 +251,16 @@ __device__ void attention_row(const DocAttention& a, const Document& doc, int he
         if (!__any(see)) continue;
         float unused;
         const float x = see ? bend_score(a, slope, dot_row(q, k + j * a.k_stride, a.head_dim), i - j, unused) : -INFINITY;
-        if (__any(x != x)) {
-            all_nan(o);
-            lse = NAN;
-            return;
-        }
         const float top = fmaxf(m, wave_max(x));
         const float p = x == -INFINITY ? 0.0f : expf(x - top);
         const float keep = m == top ? 1.0f : expf(m - top);
         m = top;
         l = l * keep + wave_add(p);
+        if (l != l) {  // NaN, or infinity less itself
+            all_nan(o);
+            lse = NAN;
+            return;
+        }
 #pragma unroll
         for (int c = 0; c < kLaneDims; ++c) o[c] *= keep;
         for (uint64_t left = __ballot(see); left; left &= left - 1) {

@@ -273,6 +273,28 @@ def test_a_document_of_nan(K, dtype, head_dim):
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES)
+def test_a_key_of_infinite_score(K, dtype):
+    """The rows that see it are NaN where its score is plus infinity, and do without it where that is minus infinity."""
+    n, hd = 200, 64
+    p, _ = problem(K, 14, R.DTYPES[dtype], [0, n], n, 2, 1, hd)
+    p.q[:, :, 0] = torch.where(torch.arange(n, device="cuda")[:, None] % 2 == 0, 1.0, -1.0).to(p.q.dtype)
+    p.k[0, 0] = 0.0
+    want, want_lse = (t.clone() for t in Attention(K, p.q[1:], p.k[1:], p.v[1:], [0, n - 1]).forward())
+    p.k[0, 0, 0] = float("inf")
+    p.k[0, 0, 1:] = 1e-3
+    out, lse = p.forward()
+    even = torch.arange(n, device="cuda") % 2 == 0
+    assert bool(torch.isnan(out[even]).all()) and bool(torch.isnan(lse[:, even]).all())
+    odd = ~even
+    odd[0] = False
+    eps = torch.finfo(p.q.dtype).eps
+    # the same keys in tiles that start one key earlier: two results within their roundings, and float32's of 200 terms
+    tol = (2 * eps + 200 * 2.0**-22) * p.v.float().abs().max().item()
+    assert float((out[odd].float() - want[odd[1:]].float()).abs().max()) <= tol
+    assert float((lse[:, odd] - want_lse[:, odd[1:]]).abs().max()) <= 200 * 2.0**-22 * 8
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
 @pytest.mark.parametrize("head_dim", [64, 120, 128, 256])
 @pytest.mark.parametrize("options", [dict(), dict(causal=False, window=50)])
 def test_a_document_in_a_large_pack(K, dtype, head_dim, options):
