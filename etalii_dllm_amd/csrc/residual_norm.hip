@@ -1,9 +1,11 @@
 // The end of one block and the start of the next: h = x + scale gate post(y), n = pre(h), and its gradients.
 //
 // With r = 1 / sqrt(mean(x^2) + eps), a norm is x r w, and its gradient for an upstream d is
-//     dx = r w d - x c,  c = r^3 / dim sum(w d x),    dw = sum over rows of d x r.
+//     dx = r w d - (x r) c,  c = r^2 / dim sum(w d x),    dw = sum over rows of d x r.
+// (r^3 is no float32 for rows of size 1e13, or 1e-13 without an eps. r sum / dim is of w d's size for any x, so c is formed as
+// that times r: see projection().)
 // So a row needs, forward, sum y^2 then sum h^2, and backward sum h^2, sum w dn h and sum y^2 together, then (from
-// g = dh + r_h w dn - h c_h) sum w gate scale g y. All sums are float32, each thread's terms in column order, then the
+// g = dh + r_h w dn - h r_h c_h) sum w gate scale g y. All sums are float32, each thread's terms in column order, then the
 // threads of a wave and the waves of a workgroup in a fixed tree: a row's bits depend on the row alone.
 //
 // Bound: HBM, each row array read and written once. 8192 x 2304 in bfloat16: forward 31.7 us, 4.8 TB/s; gradients 68 us, 3.3 TB/s,
@@ -89,6 +91,9 @@ __device__ __forceinline__ float inverse_rms(float sum_squares, const NormArgs& 
     return 1.0f / sqrtf(sum_squares * a.inv_dim + a.eps);
 }
 
+// c of a norm's gradient from r and sum(w d x).
+__device__ __forceinline__ float projection(float r, float sum, const NormArgs& a) { return r * sum * a.inv_dim * r; }
+
 // ---- rows of any size and alignment: one workgroup per row, a pass over it for each sum ----
 
 template <typename T>
@@ -138,7 +143,7 @@ struct BackwardElement {
         g = a.dh ? static_cast<float>(static_cast<const T*>(a.dh)[at]) : 0.0f;
         if (a.pre)
             g += fmaf(rh * weight_at(a.pre_weight, c, a.offset), static_cast<float>(static_cast<const T*>(a.dn)[at]),
-                      -(static_cast<float>(static_cast<const T*>(a.x)[at]) * ch));
+                      -(static_cast<float>(static_cast<const T*>(a.x)[at]) * rh * ch));
         y = static_cast<float>(static_cast<const T*>(a.y)[at]);
         hat_y = a.post ? y * ry : y;
         w_post = a.post ? weight_at(a.post_weight, c, a.offset) : 1.0f;
@@ -169,7 +174,7 @@ __global__ __launch_bounds__(256) void backward_stats_any_kernel(NormArgs a) {
         }
         block_sum(s, scratch);
         const float rh = a.pre ? inverse_rms(s[0], a) : 0.0f;
-        const float ch = a.pre ? rh * rh * rh * a.inv_dim * s[1] : 0.0f;
+        const float ch = a.pre ? projection(rh, s[1], a) : 0.0f;
         const float ry = a.post ? inverse_rms(s[2], a) : 1.0f;
         float cy = 0.0f;
         if (a.post) {
@@ -179,7 +184,7 @@ __global__ __launch_bounds__(256) void backward_stats_any_kernel(NormArgs a) {
                 u[0] = fmaf(e.du * e.w_post, e.y, u[0]);
             }
             block_sum(u, scratch);
-            cy = ry * ry * ry * a.inv_dim * u[0];
+            cy = projection(ry, u[0], a);
         }
         if (threadIdx.x == 0) {
             float* st = a.stats + row * 4;
@@ -219,7 +224,7 @@ __global__ __launch_bounds__(256) void backward_rows_any_kernel(NormArgs a) {
             const int64_t at = row * a.dim + c;
             if (a.dx) static_cast<T*>(a.dx)[at] = static_cast<T>(e.g);  // dx may be dh: read above by the same thread
             if (a.dgate && a.gate_kind == 2) static_cast<T*>(a.dgate)[at] = static_cast<T>(a.scale * e.g * e.z);
-            if (a.dy) static_cast<T*>(a.dy)[at] = static_cast<T>(a.post ? fmaf(st[2] * e.w_post, e.du, -(e.y * st[3])) : e.du);
+            if (a.dy) static_cast<T*>(a.dy)[at] = static_cast<T>(a.post ? fmaf(st[2] * e.w_post, e.du, -(e.hat_y * st[3])) : e.du);
         }
     }
 }
@@ -499,7 +504,7 @@ __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
         float rh = 0.0f, ch = 0.0f;
         if constexpr (kPre) {
             rh = inverse_rms(s[1], a);
-            ch = rh * rh * rh * a.inv_dim * s[2];
+            ch = projection(rh, s[2], a);
         }
         float du[kVectors][kWidth], u[1] = {0.0f};
 #pragma unroll
@@ -512,8 +517,9 @@ __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
                 g[i] = now.dh[k][i];
                 if constexpr (kPre) {
                     const float h = now.h[k][i], dn = now.dn[k][i];
-                    g[i] += fmaf(rh * pre[i], dn, -(h * ch));
-                    sums[2][k][i] = fmaf(dn, h * rh, sums[2][k][i]);
+                    const float hat_h = h * rh;
+                    g[i] += fmaf(rh * pre[i], dn, -(hat_h * ch));
+                    sums[2][k][i] = fmaf(dn, hat_h, sums[2][k][i]);
                 }
                 const float dz = a.scale * g[i];
                 float gated = gate[i];
@@ -531,7 +537,7 @@ __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
         }
         // (also where no dy is asked for: the barrier of this sum frees the first one's scratch)
         row_sum(u, second_scratch);
-        const float cy = a.post ? ry * ry * ry * a.inv_dim * u[0] : 0.0f;
+        const float cy = a.post ? projection(ry, u[0], a) : 0.0f;
         if (a.dy)
 #pragma unroll
             for (int k = 0; k < kVectors; ++k) {
@@ -539,7 +545,7 @@ __global__ __launch_bounds__(kRowThreads) void backward_kernel(NormArgs a) {
                 parameters(k, post, pre, gate);
 #pragma unroll
                 for (int i = 0; i < kWidth; ++i)
-                    dy[i] = a.post ? fmaf(ry * post[i], du[k][i], -(now.y[k][i] * cy)) : du[k][i];
+                    dy[i] = a.post ? fmaf(ry * post[i], du[k][i], -(now.y[k][i] * ry * cy)) : du[k][i];
                 if (in[k]) store_from_float<T, kWidth>(static_cast<T*>(a.dy) + row * a.dim + c[k], dy);
             }
         if constexpr (kAhead) now = next;
