@@ -31,7 +31,6 @@ struct DocAttention {
     Source sources[4];  // q, k, v, dout as the matrix cores read them
     // backward scratch
     float* delta;     // [heads][tokens]: dout . out
-    float* dout_norm; // [heads][tokens]: |dout| (float16)
     float* dk_part;   // [heads][tokens][head_dim] float32, before the heads of a group are added
     float* dv_part;
 };
@@ -398,11 +397,11 @@ struct PackArgs {
     int tokens, head_dim;
     bool whole;
     const void* out;  // backward: with dout, for
-    float *delta, *dout_norm;
+    float* delta;
     int skip;  // arrays that need no copy: all four, or none
 };
 
-// dout . out of every token and head, and float16's norm of dout: 16 lanes to a row, 16 bytes of it to a lane at a time. Bound:
+// dout . out of every token and head: 16 lanes to a row, 16 bytes of it to a lane at a time. Bound:
 // HBM (8192 tokens, 16 heads of 128 in bfloat16: 15 us, 4.5 TB/s).
 template <typename T>
 __device__ __forceinline__ void row_products(const PackArgs& a) {
@@ -413,7 +412,7 @@ __device__ __forceinline__ void row_products(const PackArgs& a) {
             const int64_t at = token * a.stride[3] + static_cast<int64_t>(head) * a.head_dim;
             const T* const out = static_cast<const T*>(a.out) + at;
             const T* const dout = static_cast<const T*>(a.from[3]) + at;
-            float sum = 0.0f, squares = 0.0f;
+            float sum = 0.0f;
             for (int d = lane * kWide; d < a.head_dim; d += kLanes * kWide) {
                 float o[kWide] = {}, g[kWide] = {};
                 if (a.whole) {
@@ -425,15 +424,11 @@ __device__ __forceinline__ void row_products(const PackArgs& a) {
                         if (d + j < a.head_dim) o[j] = static_cast<float>(out[d + j]), g[j] = static_cast<float>(dout[d + j]);
                 }
 #pragma unroll
-                for (int j = 0; j < kWide; ++j) sum = fmaf(o[j], g[j], sum), squares = fmaf(g[j], g[j], squares);
+                for (int j = 0; j < kWide; ++j) sum = fmaf(o[j], g[j], sum);
             }
 #pragma unroll
-            for (int s = kLanes / 2; s > 0; s >>= 1) sum += __shfl_xor(sum, s), squares += __shfl_xor(squares, s);
-            if (lane == 0) {
-                const int64_t row = static_cast<int64_t>(head) * a.tokens + token;
-                a.delta[row] = sum;
-                if (a.dout_norm) a.dout_norm[row] = sqrtf(squares);
-            }
+            for (int s = kLanes / 2; s > 0; s >>= 1) sum += __shfl_xor(sum, s);
+            if (lane == 0) a.delta[static_cast<int64_t>(head) * a.tokens + token] = sum;
         }
 }
 
@@ -507,7 +502,7 @@ void set_sources(DocAttention& a, bool backward, char* packed, hipStream_t strea
         }
         p.from[i] = arrays[i], p.stride[i] = strides[i], p.to[i] = a.sources[i], p.heads[i] = heads[i];
     }
-    p.out = a.out, p.delta = a.delta, p.dout_norm = a.dout_norm;
+    p.out = a.out, p.delta = a.delta;
     p.skip = as_they_are ? 4 : 0;
     const int parts = (as_they_are ? 0 : count) + (backward ? 1 : 0);
     if (!parts) return;

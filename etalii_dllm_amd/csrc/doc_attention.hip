@@ -69,7 +69,7 @@ struct AttentionLayout {
         part = backward && a.group > 1 ? stats * a.head_dim : 0;
         Layout l;
         l.add<char>(packed);
-        for (const size_t n : {stats, stats, part, part}) l.add<float>(n);
+        for (const size_t n : {stats, part, part}) l.add<float>(n);
         bytes = l.bytes;
     }
 };
@@ -134,7 +134,6 @@ int dllm_hip_document_attention_backward(const dllm_hip_document_attention_shape
     Carve c(workspace, workspace_bytes);
     char* const packed = c.take<char>(layout.packed);
     a.delta = c.take<float>(layout.stats);
-    a.dout_norm = c.take<float>(layout.stats);
     a.dk_part = c.take<float>(layout.part);
     a.dv_part = c.take<float>(layout.part);
     auto s = static_cast<hipStream_t>(stream);

@@ -1,14 +1,121 @@
-"""GPU: the packed-layer operators at the ends of their ranges, within the bounds of packed_reference."""
+"""GPU: the packed-layer operators at the ends of their ranges: rows of norms far from one, upstream
+gradients of very different sizes. The bounds are those of packed_reference or, where its are as wide as what is
+looked for, tighter ones of the same kind (u = eps / 2 of the activations' type, F = 2^-24)."""
 
 from __future__ import annotations
+
+import math
 
 import pytest
 import torch
 
 import packed_reference as R
-from test_gpu_packed_layers import K, gen, norm_backward, norm_forward, randn  # noqa: F401  (K: the fixture)
+from packed_reference import F
+from test_gpu_packed_layers import Attention, K, gen, norm_backward, norm_forward, randn  # noqa: F401  (K: the fixture)
 
 pytestmark = pytest.mark.gpu
+
+
+# ---- attention ----
+
+
+def tight(p, out=None, lse=None, dout=None, few=0):
+    """Results and bounds of a problem of one document, forward, or with dout backward. As packed_reference.attention, but
+    - tanh is off by a few F of its value however large the cap is (16-bit types up to a cap of 64: a few F of the cap);
+    - rows that see at most `few` keys (keys that as few queries see) have their 16-bit weights and dS multiplied with what
+      rounding left of them, as far as all 32 rows of their wave do;
+    - float16's p and dS are rounded as multiples of the smallest float16 relative to what the row's (the key's) own largest
+      visible value is: p to 2^-25 forward and 2^-40 backward, dS to 2^-34 of the largest (2^-33 for its own roundings)."""
+    q, k, v, o = p.q.double(), p.k.double(), p.v.double(), p.options
+    dt, n, heads, hd = p.q.dtype, *p.q.shape
+    u, group, cap, half = R.unit(dt), heads // p.k.shape[1], o["softcap"], dt == torch.float16
+    seen = ~R.hidden(n, o["causal"], o["window"], 0 if o["prefix"] is None else o["prefix"][0]).cuda()
+
+    def rounding(counts):  # of 16-bit weights, by how many the rows of a wave have
+        if dt == torch.float32:
+            return torch.zeros(n, dtype=torch.float64, device="cuda")
+        waves = torch.nn.functional.pad(counts, (0, -n % 32)).view(-1, 32).amax(dim=1).repeat_interleave(32)[:n]
+        return torch.where(waves <= few, 2 * u * u, u).double()
+
+    by_row, by_key = rounding(seen.sum(dim=1))[:, None], rounding(seen.sum(dim=0))[None, :]
+    i = torch.arange(n, device="cuda")
+    distance = (i[:, None] - i[None, :]).abs().double()
+    got = {name: torch.zeros(t.shape, dtype=torch.float64, device="cuda") for name, t in
+           (("out", q), ("lse", p.lse), ("dq", q), ("dk", k), ("dv", v))}
+    off = {name: torch.zeros_like(t) for name, t in got.items()}
+    for h in range(heads):
+        Q, Kh, V = q[:, h], k[:, h // group], v[:, h // group]
+        x = Q @ Kh.T * p.scale
+        err = (hd + 4) * F * (Q.abs() @ Kh.abs().T) * p.scale
+        slope = torch.ones_like(x)
+        if cap:
+            t = torch.tanh(x / cap)
+            x, slope = cap * t, 1 - t * t
+            err = err + 8 * F * (cap if dt != torch.float32 and cap <= 64 else x.abs())
+        if o["slopes"] is not None:
+            x = x - float(o["slopes"][h]) * distance
+            err = err + 4 * F * float(o["slopes"][h]) * distance
+        err = (err + 4 * F * x.abs()).masked_fill(~seen, 0.0).amax(dim=1, keepdim=True)
+        x = x.masked_fill(~seen, -math.inf)
+        if dout is None:
+            s = torch.logsumexp(x, dim=1, keepdim=True)
+            w = torch.exp(x - s)
+            got["lse"][h], off["lse"][h] = s[:, 0], (err + 4 * F * s.abs() + (n + 8) * F)[:, 0]
+            got["out"][:, h] = r = w @ V
+            off["out"][:, h] = u * r.abs() + (w @ V.abs()) * (2 * err.expm1() + 2 * by_row + (2 * n + 16) * F) * (1 + u) + \
+                seen.double() @ V.abs() * (2.0 ** -25 if half else 2.0 ** -126)
+            continue
+        s = lse[h].double()[:, None]
+        w = torch.exp(x - s)
+        rel = err.expm1() + 4 * F * s.abs() + 8 * F
+        dO, O = dout[:, h].double(), out[:, h].double()
+        dP, delta = dO @ V.T, (dO * O).sum(dim=1, keepdim=True)
+        size = dO.abs() @ V.abs().T + (dO.abs() * O.abs()).sum(dim=1, keepdim=True)
+        dS = w * (dP - delta) * slope * p.scale
+        dslope = 2 * (8 * F + err / cap) if cap else 0.0
+        eS = w * size * p.scale * (rel + (hd + 16) * F + dslope) + seen * 2.0 ** -126 * (1 + size * p.scale)
+        eP = w * (rel + by_key) + seen * (2.0 ** -40 if half else 2.0 ** -126)
+        both = [eS + dS.abs() * by for by in (by_row, by_key)]  # dq's and dk's
+        if half:
+            both = [e + seen * 2.0 ** -33 * (dS.abs() + eS).amax(dim=d, keepdim=True) for e, d in zip(both, (1, 0))]
+        got["dq"][:, h] = dS @ Kh
+        off["dq"][:, h] = u * got["dq"][:, h].abs() + (both[0] @ Kh.abs() + (2 * n + 8) * F * (dS.abs() @ Kh.abs())) * (1 + u)
+        for name, value, e, rows in (("dk", dS, both[1], Q), ("dv", w, eP, dO)):
+            got[name][:, h // group] += value.T @ rows
+            off[name][:, h // group] += (e.T @ rows.abs() + (2 * n + 8 + heads) * F * (value.abs().T @ rows.abs())) * (1 + u)
+    for name in ("dk", "dv"):
+        off[name] += u * got[name].abs()
+    return {name: (got[name], off[name] + (0.0 if name == "lse" else R.tiny(dt))) for name in got}
+
+
+def check(p, dout, what="", few=0):
+    out, lse = p.forward()
+    want = tight(p, few=few)
+    R.assert_within(out, want["out"], f"{what} out"), R.assert_within(lse, want["lse"], f"{what} lse")
+    want = tight(p, out, lse, dout, few)
+    for name, got in zip(("dq", "dk", "dv"), p.backward(dout)):
+        R.assert_within(got, want[name], f"{what} {name}")
+
+
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("options", [dict(), dict(window=20), dict(causal=False, window=90), dict(prefix=[100])])
+def test_float16_gradients_beside_a_large_one(K, head_dim, options):  # noqa: F811
+    """One query whose upstream gradient is 10^6 to 10^7 times the others': the keys that it does not see keep their bits."""
+    g = gen(72)
+    q, k, v, dout = (randn(g, 256, h, head_dim) for h in (2, 1, 1, 2))
+    for row in (0, 140):
+        d = dout * 1e-3
+        d[row] = dout[row] * 1e4
+        check(Attention(K, q.half(), k.half(), v.half(), [0, 256], **options), d.half(), f"{row}")
+
+
+@pytest.mark.parametrize("head_dim", [64, 128])
+@pytest.mark.parametrize(("size", "spread"), [(1e-3, 1.0), (1e-3, 4.0), (1.0, 4.0), (1e3, 1.0)])
+def test_float16_gradients_of_small_and_large_values(K, head_dim, size, spread):  # noqa: F811
+    """Values far below and above one, and weights from one down to e^-60: dS has the size of both, and keeps its bits."""
+    g = gen(73)
+    q, k, v, dout = (randn(g, 1500, h, head_dim, scale=s).half() for h, s in ((2, spread), (1, spread), (1, size), (2, 1.0)))
+    check(Attention(K, q, k, v, [0, 1500]), dout)
 
 
 # ---- norms ----
