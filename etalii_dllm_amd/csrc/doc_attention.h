@@ -187,12 +187,31 @@ __device__ __forceinline__ float bend_score(const DocAttention& a, float slope, 
     return x - slope * static_cast<float>(distance < 0 ? -distance : distance);
 }
 
-// The score of a product x in units of log 2: bend(x) times + plus, which is x scale without a cap. With one, 16-bit types
-// use tanh z = 1 - 2 / (1 + e^2z), off by at most about 6 x 2^-24 absolutely, which the weights (rounded to 2^-9 of
-// themselves) do not see: bend is -1 / (1 + e^2z), and the rest of it falls into times and plus. float32 uses the library's
-// tanh, exact to its last bits near zero too. bend grows with x, so the largest score is that of the largest bend.
-template <typename T>
+// The score of a product x in units of log 2: bent(x) times + plus, which is x scale without a cap. bent grows with x, so the
+// largest score is that of the largest bent. bent is tanh, as float32 has it from the library, exact to its last bits near zero
+// too. With 16-bit types it is
+// - of caps up to kSmallCap -1 / (1 + e^2z) = (tanh z - 1) / 2, whose rest falls into times and plus. It is off by at most about
+//   6 x 2^-24 of the cap however small the score is: 2^-15 of a weight, which rounds to 2^-9 or 2^-12 of itself.
+// - of larger ones, whose scores may be any part of the cap, tanh again, to about 6 x 2^-24 of itself: z (945 + 105 z^2 + z^4) /
+//   (945 + 420 z^2 + 15 z^4), Lambert's continued fraction cut after five levels, where |z| < 1/2 (off by 2^-27), else
+//   1 - 2 / (1 + e^2|z|).
+// Large caps have kernels of their own: in the same ones, chosen by a branch, they cost other calls registers (8192 tokens of
+// 16/8 heads of 64 in bfloat16, without a cap, 168 and 178 us). Caps of 50 and 100: 8000 + 192 tokens, 8/4 heads of 256, window 4096,
+// 377 and 462 us; gradients of 8192 tokens, 16/8 heads of 128, 1257 and 1830.
+constexpr float kSmallCap = 64.0f;
+
+inline bool large_cap(const DocAttention& a) { return a.softcap > kSmallCap; }
+
+__device__ __forceinline__ float tanh_of_any_size(float z) {
+    const float w = z * z;
+    const float near = z * fmaf(w + 105.0f, w, 945.0f) * __builtin_amdgcn_rcpf(fmaf(fmaf(15.0f, w, 420.0f), w, 945.0f));
+    const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.0f * kLog2E * fabsf(z))), 1.0f);
+    return fabsf(z) < 0.5f ? near : copysignf(far, z);
+}
+
+template <typename T, bool kLargeCap>
 struct CapTerms {
+    static constexpr bool kHalved = sizeof(T) == 2 && !kLargeCap;  // bent is (tanh - 1) / 2
     bool capped;
     float in, times, plus;
     __device__ __forceinline__ explicit CapTerms(const DocAttention& a) {
@@ -200,14 +219,15 @@ struct CapTerms {
         const float unit = (capped ? a.softcap : a.scale) * kLog2E;
         in = capped ? a.scale / a.softcap : 0.0f;
         times = unit, plus = 0.0f;
-        if (sizeof(T) == 2 && capped) in *= 2.0f * kLog2E, times = 2.0f * unit, plus = unit;
+        if (kHalved && capped) in *= 2.0f * kLog2E, times = 2.0f * unit, plus = unit;
     }
     __device__ __forceinline__ float bend(float x) const {
         if constexpr (sizeof(T) == 4) return tanhf(x * in);
+        if constexpr (kLargeCap) return tanh_of_any_size(x * in);
         return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(x * in));
     }
     // bend's tanh, whose square is one minus the cap's derivative
-    __device__ __forceinline__ float tangent(float bent) const { return sizeof(T) == 4 ? bent : fmaf(2.0f, bent, 1.0f); }
+    __device__ __forceinline__ float tangent(float bent) const { return kHalved ? fmaf(2.0f, bent, 1.0f) : bent; }
 };
 
 template <typename T>

@@ -75,7 +75,7 @@ struct ColumnScale {
 };
 
 // ---- dq ----
-template <typename T, int kDim>
+template <typename T, int kDim, bool kLargeCap>
 __device__ __forceinline__ void dq_tile(const DocAttention& a, unsigned block, LdsByte* buffers, LdsByte* pair_lds) {
     using Shape = TileShape<T, kDim>;
     constexpr int kTile = kStream<T, kDim>;
@@ -125,7 +125,7 @@ __device__ __forceinline__ void dq_tile(const DocAttention& a, unsigned block, L
     const float delta = a.delta[stat_at];
     ColumnScale scale;
 
-    const CapTerms<T> cap(a);
+    const CapTerms<T, kLargeCap> cap(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
     const float base = a.lse[stat_at] * kLog2E - cap.plus;
 
@@ -225,7 +225,7 @@ __device__ __forceinline__ void dq_tile(const DocAttention& a, unsigned block, L
 // kShared: into the float32 parts of heads that share keys. kDk, kDv: which of the two; rows of more than kTogether
 // elements for a wave take a workgroup for each, since the sums of both and a lane's two rows are more than its registers (five products
 // in all instead of four).
-template <typename T, int kDim, bool kShared, bool kDk, bool kDv>
+template <typename T, int kDim, bool kLargeCap, bool kShared, bool kDk, bool kDv>
 __device__ __forceinline__ void dkv_tile(const DocAttention& a, unsigned block, LdsByte* buffers, LdsByte* pair_lds) {
     using Shape = TileShape<T, kDim>;
     constexpr int kTile = kStream<T, kDim>;
@@ -279,7 +279,7 @@ __device__ __forceinline__ void dkv_tile(const DocAttention& a, unsigned block, 
 
     ColumnScale scale;
 
-    const CapTerms<T> cap(a);
+    const CapTerms<T, kLargeCap> cap(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
 
     Acc dk[kDk ? kParts : 1], dv[kDv ? kParts : 1];
@@ -443,7 +443,7 @@ template <typename T, int kDim>
 constexpr int kExchangeBytes = kPair<T, kDim> == 2 ? 2 * 4 * 4096 : 16;
 
 // All gradients at once: dk and dv (blockIdx.y 0; dv 2 where it is on its own), whose workgroups take longer, before dq (1).
-template <typename T, int kDim, bool kShared>
+template <typename T, int kDim, bool kLargeCap, bool kShared>
 __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1) void gradients_kernel(DocAttention a) {
     __shared__ __attribute__((aligned(1024))) char lds[kTilesBytes<T, kDim>];
     __shared__ __attribute__((aligned(16))) char exchanged[kExchangeBytes<T, kDim>];
@@ -451,18 +451,18 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 && kDim <= 64 ? 2 : 1)
     LdsByte* const pair_lds = (LdsByte*)exchanged;
     const unsigned block = blockIdx.x, turn = blockIdx.y;
     if constexpr (kWaveDim<T, kDim> <= kTogether) {
-        if (turn == 0) return dkv_tile<T, kDim, kShared, true, true>(a, block, buffers, pair_lds);
+        if (turn == 0) return dkv_tile<T, kDim, kLargeCap, kShared, true, true>(a, block, buffers, pair_lds);
     } else {
-        if (turn == 0) return dkv_tile<T, kDim, kShared, true, false>(a, block, buffers, pair_lds);
-        if (turn == 2) return dkv_tile<T, kDim, kShared, false, true>(a, block, buffers, pair_lds);
+        if (turn == 0) return dkv_tile<T, kDim, kLargeCap, kShared, true, false>(a, block, buffers, pair_lds);
+        if (turn == 2) return dkv_tile<T, kDim, kLargeCap, kShared, false, true>(a, block, buffers, pair_lds);
     }
-    dq_tile<T, kDim>(a, block, buffers, pair_lds);
+    dq_tile<T, kDim, kLargeCap>(a, block, buffers, pair_lds);
 }
 
 // 16-bit heads of 65 to 128 elements: dq alone fits twice on a CU, dk and dv do not. With more than kFewTiles workgroups of
 // each kind a kernel for each is faster (16/8 heads of 128 in bfloat16, microseconds together and apart: 2048 tokens, 272
 // workgroups, 111 and 163; 3071 tokens, 400, 215 and 234; 4096 tokens, 528, 339 and 329; 8192 tokens, 1040, 1184 and 1045).
-// Both ways run the same code and give the same bits.
+// Both ways run the same code and give the same bits; large caps have the one launch alone.
 template <typename T, int kDim>
 constexpr bool kApart = kPlanes<T> == 1 && kDim == 128;
 constexpr unsigned kFewTiles = 512;
@@ -471,14 +471,14 @@ template <typename T, int kDim>
 __global__ __launch_bounds__(kDocThreads, 2) void dq_kernel(DocAttention a) {
     static_assert(kApart<T, kDim>);
     __shared__ __attribute__((aligned(1024))) char lds[kTilesBytes<T, kDim>];
-    dq_tile<T, kDim>(a, blockIdx.x, (LdsByte*)lds, nullptr);
+    dq_tile<T, kDim, false>(a, blockIdx.x, (LdsByte*)lds, nullptr);
 }
 
 template <typename T, int kDim, bool kShared>
 __global__ __launch_bounds__(kDocThreads, 1) void dkv_kernel(DocAttention a) {
     static_assert(kApart<T, kDim>);
     __shared__ __attribute__((aligned(1024))) char lds[kTilesBytes<T, kDim>];
-    dkv_tile<T, kDim, kShared, true, true>(a, blockIdx.x, (LdsByte*)lds, nullptr);
+    dkv_tile<T, kDim, false, kShared, true, true>(a, blockIdx.x, (LdsByte*)lds, nullptr);
 }
 
 // dk and dv of the tokens of documents: the group's heads added in order. kWidth elements to a thread. Bound: HBM (8192 tokens,
@@ -513,6 +513,12 @@ __global__ __launch_bounds__(kDocThreads) void add_heads_kernel(DocAttention a) 
 template <typename T, int kDim, bool kShared>
 void launch_gradients(const DocAttention& a, hipStream_t s) {
     const unsigned tiles = doc_tiles(a, kBlockRows<T, kDim>) * a.heads;
+    const dim3 together(tiles, kWaveDim<T, kDim> <= kTogether ? 2 : 3);
+    if constexpr (sizeof(T) == 2)
+        if (large_cap(a)) {
+            gradients_kernel<T, kDim, true, kShared><<<together, kDocThreads, 0, s>>>(a);
+            return;
+        }
     if constexpr (kApart<T, kDim>) {
         if (tiles > kFewTiles) {
             dkv_kernel<T, kDim, kShared><<<tiles, kDocThreads, 0, s>>>(a);
@@ -520,7 +526,7 @@ void launch_gradients(const DocAttention& a, hipStream_t s) {
             return;
         }
     }
-    gradients_kernel<T, kDim, kShared><<<dim3(tiles, kWaveDim<T, kDim> <= kTogether ? 2 : 3), kDocThreads, 0, s>>>(a);
+    gradients_kernel<T, kDim, false, kShared><<<together, kDocThreads, 0, s>>>(a);
 }
 
 template <typename T, int kDim>

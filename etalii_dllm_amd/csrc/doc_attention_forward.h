@@ -29,7 +29,7 @@ constexpr int kBuffers = 4 * kKeys<T, kDim> * kDim * 2 * kPlanes<T> <= 128 * 102
 // and 970 without the causal mask); of 64, 174 us and 790; 8/4 heads of 256, 355 us and 775. float32, 4096 tokens, 16/8 heads of
 // 128: 420 us, of six products 980. Short calls are bound by the way of one workgroup through a row's keys: about 1.1 us a tile
 // of 64 (16-bit), 3.1 us one of 32 (float32).
-template <typename T, int kDim>
+template <typename T, int kDim, bool kLargeCap>
 __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kDim <= 128 ? 2 : 1) : 1) void forward_kernel(DocAttention a, T* out) {
     using Shape = TileShape<T, kDim>;
     constexpr int kTile = kKeys<T, kDim>;
@@ -81,7 +81,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kD
     if (kAhead) fetch(t, 0);
     const Column<T, kDim> q(a.sources[0], head, i, part);
 
-    const CapTerms<T> cap(a);
+    const CapTerms<T, kLargeCap> cap(a);
     const float slope = a.slopes ? a.slopes[head] * kLog2E : 0.0f;
 
     Acc o[kParts];
@@ -217,7 +217,13 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kD
 
 template <typename T, int kDim>
 void launch_forward(const DocAttention& a, T* out, hipStream_t s) {
-    forward_kernel<T, kDim><<<doc_tiles(a, kBlockRows<T, kDim>) * a.heads, kDocThreads, 0, s>>>(a, out);
+    const unsigned blocks = doc_tiles(a, kBlockRows<T, kDim>) * a.heads;
+    if constexpr (sizeof(T) == 2)
+        if (large_cap(a)) {
+            forward_kernel<T, kDim, true><<<blocks, kDocThreads, 0, s>>>(a, out);
+            return;
+        }
+    forward_kernel<T, kDim, false><<<blocks, kDocThreads, 0, s>>>(a, out);
 }
 
 // doc_attention_wide.hip

@@ -1,5 +1,5 @@
-"""GPU: the packed-layer operators at the ends of their ranges: rows of norms far from one, upstream
-gradients of very different sizes. The bounds are those of packed_reference or, where its are as wide as what is
+"""GPU: the packed-layer operators at the ends of their ranges: rows of norms far from one, caps of any
+size, upstream gradients of very different sizes. The bounds are those of packed_reference or, where its are as wide as what is
 looked for, tighter ones of the same kind (u = eps / 2 of the activations' type, F = 2^-24)."""
 
 from __future__ import annotations
@@ -11,7 +11,7 @@ import torch
 
 import packed_reference as R
 from packed_reference import F
-from test_gpu_packed_layers import Attention, K, gen, norm_backward, norm_forward, randn  # noqa: F401  (K: the fixture)
+from test_gpu_packed_layers import PACK, Attention, K, gen, norm_backward, norm_forward, problem, randn  # noqa: F401  (K: the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -95,6 +95,45 @@ def check(p, dout, what="", few=0):
     want = tight(p, out, lse, dout, few)
     for name, got in zip(("dq", "dk", "dv"), p.backward(dout)):
         R.assert_within(got, want[name], f"{what} {name}")
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("cap", [64.0, 100.0, 1e3, 1e5, 1e8, 1e19])
+def test_caps_of_any_size(K, dtype, head_dim, cap):  # noqa: F811
+    """A cap far above the scores hardly bends them, and costs them no bits; scores above it are bent flat."""
+    g, dt = gen(71), R.DTYPES[dtype]
+    q, k, v, dout = (randn(g, 150, h, head_dim, dtype=dt) for h in (2, 1, 1, 2))
+    check(Attention(K, q, k, v, [0, 150], softcap=cap), dout, "ordinary scores")
+    if cap <= 1e5:
+        check(Attention(K, q, k, v, [0, 150], softcap=cap, scale=cap / 8), dout, "scores about the cap's size")
+    check(Attention(K, q, k, v, [0, 150], softcap=cap, causal=False, slopes=[0.1, 0.0]), dout, "bias")
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize("head_dim", [64, 100, 128, 256])
+def test_documents_with_a_large_cap(K, dtype, head_dim):  # noqa: F811
+    """Masks, hidden NaN and a document's own bits where large caps have kernels of their own."""
+    options = dict(window=65, softcap=1e3, slopes=[1.0, 0.01, 0.0, 0.3])
+    prefix = [1, 0, 3, 64, 100, 1, 0]
+    p, dout = problem(K, 74, R.DTYPES[dtype], PACK, 437, 4, 2, head_dim, prefix=prefix, **options)
+    p.check(dout)
+    want = [t.clone() for t in (*p.forward(), *p.backward(dout))]
+    for d in (3, 6):
+        b, e = PACK[d], PACK[d + 1]
+        s = Attention(K, p.q[b:e].clone(), p.k[b:e].clone(), p.v[b:e].clone(), [0, e - b], prefix=[prefix[d]], **options)
+        got = [*s.forward(), *s.backward(dout[b:e].clone())]
+        assert all(torch.equal(x, (y[:, b:e] if y is want[1] else y[b:e])) for x, y in zip(got, want))
+    # the last document's first key is seen by its first 65 queries alone
+    b, n = PACK[6], PACK[7] - PACK[6]
+    p.k[b], p.v[b] = float("nan"), float("nan")
+    out, _ = p.forward()
+    sees = torch.zeros(437, dtype=torch.bool, device="cuda")
+    sees[b:b + 65] = True
+    assert bool(torch.isnan(out[sees]).all()) and n > 65
+    assert torch.equal(out[:b], want[0][:b]) and torch.equal(out[b + 128:], want[0][b + 128:])
+    clean = R.attention(p.q, torch.nan_to_num(p.k), torch.nan_to_num(p.v), p.offsets, p.scale, prefix=prefix, **options)["out"]
+    R.assert_within(out[~sees], (clean[0][~sees], clean[1][~sees]), "beside NaN")
 
 
 @pytest.mark.parametrize("head_dim", [64, 128, 256])
