@@ -1,7 +1,5 @@
 // Attention within packed documents: the entry points. The kernels are doc_attention_forward.h's and
 // doc_attention_backward.h's, compiled for each type in doc_attention_{f32,bf16,f16}.hip.
-#include <float.h>
-
 #include <algorithm>
 #include <initializer_list>
 
@@ -25,8 +23,9 @@ int check_shape(const dllm_hip_document_attention_shape* sh) {
     DLLM_REQUIRE(sh->heads <= 65535, "at most 65535 heads");
     DLLM_REQUIRE(sh->head_dim >= 1 && sh->head_dim <= kMaxHeadDim, "head_dim must be in [1, 256]");
     DLLM_REQUIRE(sh->window >= 0, "window must not be negative");
-    DLLM_REQUIRE(sh->softcap >= 0.0 && static_cast<float>(sh->softcap) <= FLT_MAX, "softcap must not be negative, nor infinite");
-    DLLM_REQUIRE(static_cast<float>(sh->scale) > 0.0f && static_cast<float>(sh->scale) <= FLT_MAX, "scale must be positive and finite");
+    // in float32 the scale, the cap, their quotient and any of them times 2 / log 2 are then ordinary numbers
+    DLLM_REQUIRE(sh->softcap == 0.0 || (sh->softcap >= 0x1p-64 && sh->softcap <= 0x1p64), "softcap must be 0 or in [2^-64, 2^64]");
+    DLLM_REQUIRE(sh->scale >= 0x1p-60 && sh->scale <= 0x1p60, "scale must be in [2^-60, 2^60]");
     const int64_t q = sh->heads * sh->head_dim, k = sh->kv_heads * sh->head_dim;
     for (const int64_t s : {sh->q_stride, sh->out_stride}) DLLM_REQUIRE(s == 0 || s >= q, "a token stride must be 0 or at least heads * head_dim");
     for (const int64_t s : {sh->k_stride, sh->v_stride}) DLLM_REQUIRE(s == 0 || s >= k, "a token stride must be 0 or at least heads * head_dim");

@@ -292,8 +292,8 @@ enum { DLLM_HIP_FLOAT32 = 0, DLLM_HIP_BFLOAT16 = 1, DLLM_HIP_FLOAT16 = 2 };
  * (softcap 0: scale q.k; slopes: device, one per head, NULL for none; constants, they get no gradient). out = softmax(s) v and
  * lse[heads, tokens] = log sum exp s, which the backward reads (float32; may be NULL). Keys that a query does not see do
  * not reach its results, whatever they hold.
- * Limits: scale positive, head_dim at most 256, heads a multiple of kv_heads, at most 65535 heads, and (tokens / 64 +
- * documents) * heads below 2^24. Out-of-range offsets and prefixes are clamped to the tokens and the document; documents
+ * Limits: scale in [2^-60, 2^60], softcap 0 or in [2^-64, 2^64], head_dim at most 256, heads a multiple of kv_heads, at most 65535
+ * heads, and (tokens / 64 + documents) * heads below 2^24. Out-of-range offsets and prefixes are clamped to the tokens and the document; documents
  * that then overlap give unspecified values. Outputs do not overlap inputs, nor the workspace either.
  * The backward takes the forward's out and lse and the upstream gradient dout (out's layout and stride) and writes dq, dk
  * and dv (q's, k's and v's layouts and strides); dk and dv sum over the heads that share them, in head order. */

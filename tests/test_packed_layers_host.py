@@ -271,3 +271,21 @@ def test_rope_definition_turns_back(interleaved):
     assert (R.rope(there, pos, freq, axis, interleaved, True)[0] - x).abs().max() < 1e-9
     # a rotation keeps lengths; dimensions past the pairs stay
     assert (there.square().sum(-1) - x.square().sum(-1)).abs().max() < 1e-9 and torch.equal(there[..., 8:], x[..., 8:])
+
+
+@needs_library
+def test_attention_refuses_scales_and_caps_that_float32_does_not_hold(K):
+    """A cap that is zero in float32 would be none, and one whose quotient with the scale is no ordinary float32 would bend the
+    scores otherwise than it says."""
+    for change, message in [(dict(softcap=1e-50), "softcap"), (dict(softcap=1e-30), "softcap"), (dict(softcap=1e30), "softcap"),
+                            (dict(softcap=3.4e38), "softcap"), (dict(scale=3e38), "scale"), (dict(scale=1e-40), "scale")]:
+        shape = K.DocumentAttention(**{**ATTENTION, **change})
+        with pytest.raises(ValueError, match=message):
+            K.check(K.lib.dllm_hip_document_attention(shape, *[P] * 9, 1 << 60, None))
+        with pytest.raises(ValueError, match=message):
+            K.check(K.lib.dllm_hip_document_attention_backward(shape, *[P] * 13, 1 << 60, None))
+        assert K.lib.dllm_hip_document_attention_workspace(shape) == 0
+    for scale in (2.0 ** -60, 2.0 ** 60):
+        for softcap in (0.0, 2.0 ** -64, 2.0 ** 64):
+            shape = K.DocumentAttention(**{**ATTENTION, "scale": scale, "softcap": softcap})
+            assert K.lib.dllm_hip_document_attention_workspace(shape) > 0
