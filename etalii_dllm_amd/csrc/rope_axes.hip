@@ -139,8 +139,9 @@ extern "C" int dllm_hip_rope_axes(const dllm_hip_rope_axes_shape* sh, const void
     DLLM_REQUIRE(sh->pairs >= 0 && sh->pairs <= kMaxPairs, "pairs must be in [0, 256]");
     DLLM_REQUIRE(sh->head_dim >= 1 && sh->head_dim <= 65536 && 2 * sh->pairs <= sh->head_dim,
                  "2 * pairs must not exceed head_dim");
-    DLLM_REQUIRE((sh->q_heads + sh->k_heads) * sh->head_dim < (int64_t{1} << 31),
-                 "a token's heads must have fewer than 2^31 elements");
+    // (a thread counts them in steps of a workgroup, past the last)
+    DLLM_REQUIRE((sh->q_heads + sh->k_heads) * sh->head_dim <= INT32_MAX - kThreads,
+                 "a token's heads must have fewer than 2^31 - 256 elements");
     DLLM_REQUIRE(sh->axes >= 1 && sh->axes <= 255, "axes must be in [1, 255]");
     const int64_t heads[2] = {sh->q_heads, sh->k_heads};
     const int64_t in[2] = {sh->q_stride, sh->k_stride}, out[2] = {sh->q_out_stride, sh->k_out_stride};

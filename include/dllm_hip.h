@@ -322,7 +322,7 @@ int dllm_hip_document_attention_backward(const dllm_hip_document_attention_shape
  * dimensions p and pairs + p, or 2p and 2p + 1 with interleaved; dimensions from 2 * pairs on are copied. inverse turns
  * back: the gradient of q and k from those of the outputs. k may be NULL with k_heads 0. q_out may be q and k_out may
  * be k with the same strides (in place); otherwise inputs and outputs do not overlap. Strides as above. At most 256 pairs,
- * 65535 heads of each and 2^31 - 1 tokens. */
+ * 65535 heads of each of at most 65536 elements, fewer than 2^31 - 256 elements in all heads of a token, and 2^31 - 1 tokens. */
 typedef struct {
     int64_t dtype;
     int64_t tokens, q_heads, k_heads, head_dim, pairs, axes;

@@ -289,3 +289,16 @@ def test_attention_refuses_scales_and_caps_that_float32_does_not_hold(K):
         for softcap in (0.0, 2.0 ** -64, 2.0 ** 64):
             shape = K.DocumentAttention(**{**ATTENTION, "scale": scale, "softcap": softcap})
             assert K.lib.dllm_hip_document_attention_workspace(shape) > 0
+
+
+@needs_library
+def test_rope_axes_refuses_tokens_that_a_thread_cannot_count(K):
+    """A thread's count of a token's elements steps 256 past the last, in 32 bits: tokens of up to 2^31 - 257 elements."""
+    for q_heads, k_heads, head_dim in [(32770, 0, 65532), (32769, 0, 65534), (1, 33373, 64346), (65535, 53624, 18022)]:
+        assert 2 ** 31 - 256 <= (q_heads + k_heads) * head_dim < 2 ** 31
+        shape = K.RopeAxes(**{**ROPE, "q_heads": q_heads, "k_heads": k_heads, "head_dim": head_dim})
+        with pytest.raises(ValueError, match="elements"):
+            K.check(K.lib.dllm_hip_rope_axes(shape, *[P] * 7, None))
+    shape = K.RopeAxes(**{**ROPE, "q_heads": 32768, "k_heads": 0, "head_dim": 65535})
+    with pytest.raises(ValueError, match="null"):  # far enough below: its pointers are looked at
+        K.check(K.lib.dllm_hip_rope_axes(shape, None, *[P] * 6, None))
