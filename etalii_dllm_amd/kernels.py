@@ -929,15 +929,16 @@ def rope_axes(q, k, positions, inv_freq, pair_axis, interleaved=False, inverse=F
         raise ValueError("q and k must be [tokens, heads, head_dim] with one number of tokens and one head_dim")
     pos = np.ascontiguousarray(positions, dtype=np.int64)
     freqs = np.ascontiguousarray(inv_freq, dtype=np.float64)
-    axis = np.ascontiguousarray(pair_axis, dtype=np.uint8)
+    axis = np.asarray(pair_axis)
     if pos.ndim != 2 or pos.shape[1] != q.shape[0]:
         raise ValueError("positions must be [axes, tokens]")
     if freqs.ndim != 1 or axis.shape != freqs.shape:
         raise ValueError("inv_freq and pair_axis must have one entry per pair")
     if 2 * len(freqs) > q.shape[2]:
         raise ValueError("2 * len(inv_freq) must not exceed head_dim")
-    if len(axis) and axis.max() >= pos.shape[0]:
+    if len(axis) and not (axis.min() >= 0 and axis.max() < pos.shape[0]):
         raise ValueError("pair_axis must be below the number of axes")
+    axis = np.ascontiguousarray(axis, dtype=np.uint8)
     k_heads = 0 if k is None else np.shape(k)[1]
     shape = RopeAxes(dtype, q.shape[0], q.shape[1], k_heads, q.shape[2], len(freqs), pos.shape[0], int(interleaved),
                      int(inverse))

@@ -302,3 +302,11 @@ def test_rope_axes_refuses_tokens_that_a_thread_cannot_count(K):
     shape = K.RopeAxes(**{**ROPE, "q_heads": 32768, "k_heads": 0, "head_dim": 65535})
     with pytest.raises(ValueError, match="null"):  # far enough below: its pointers are looked at
         K.check(K.lib.dllm_hip_rope_axes(shape, None, *[P] * 6, None))
+
+
+@needs_library
+@pytest.mark.parametrize("axis", [256, 512, -256, -1, 3])
+def test_rope_axes_refuses_axes_that_eight_bits_wrap(K, axis):
+    x = np.zeros((4, 2, 8), np.float32)
+    with pytest.raises(ValueError, match="pair_axis"):
+        K.rope_axes(x, x, np.zeros((3, 4)), np.ones(4), np.array([0, 1, 2, axis]))
