@@ -36,10 +36,11 @@ struct DocAttention {
 };
 
 // 16-bit weights (and dS) are rounded to their type for the second product: each is off by 2^-9 or 2^-12 of itself, which in a
-// sum over many keys adds to about what the result's own rounding is. Documents of so few tokens that such errors do not
-// average out have what the rounding left multiplied too. They are one tile of keys, so that costs little (128 documents of 64
-// tokens, 16/8 heads of 128 in bfloat16: 37.7 to 39.3 us, gradients 193 to 202 us; the error of a document of 37: 1.8e-3 to
-// 1.6e-3, which is the result's own rounding).
+// sum over many keys adds to about what the result's own rounding is. Rows that see so few keys (keys that so few queries see)
+// that such errors do not average out have what the rounding left multiplied too, where that holds for all 32 of a wave: short
+// documents, narrow windows, a long causal document's first queries and last keys. (128 documents of 64 tokens, 16/8 heads of 128
+// in bfloat16: 37.7 to 39.3 us, gradients 193 to 202 us; the error of a document of 37: 1.8e-3 to 1.6e-3, which is the result's own
+// rounding.)
 constexpr int kFewTokens = 64;
 
 // Token range of a document, and the end of the keys that all its tokens see.
@@ -162,6 +163,14 @@ __device__ __forceinline__ Span query_span(const DocAttention& a, const Document
 __device__ __forceinline__ bool visible(const Document& d, const Span& s, int j) {
     return (j >= s.low && j < s.high) || (j >= d.start && j < d.prefix_end);
 }
+
+// Of the 32 queries (keys) of a wave: whether each sees (is seen by) few.
+__device__ __forceinline__ bool all_see_few(const Document& d, const Span& s) {
+    const int before = max(min(d.prefix_end, s.low), d.start) - d.start, after = max(d.prefix_end - s.high, 0);
+    return !__any(s.high - s.low + before + after > kFewTokens);
+}
+
+__device__ __forceinline__ bool all_seen_by_few(const Span& s) { return !__any(s.high - s.low > kFewTokens); }
 
 __device__ __forceinline__ float wave_max(float v) {
 #pragma unroll

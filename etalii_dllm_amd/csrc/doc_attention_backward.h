@@ -92,7 +92,6 @@ __device__ __forceinline__ void dq_tile(const DocAttention& a, unsigned block, L
     int first;
     if (!locate_tile<kOwn, true>(a, block / a.heads, doc, first)) return;
 
-    const bool few = doc.end - doc.start <= kFewTokens;
     const int wave = uniform(static_cast<int>(threadIdx.x) >> 6), lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
     const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
     const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
@@ -100,6 +99,7 @@ __device__ __forceinline__ void dq_tile(const DocAttention& a, unsigned block, L
     const bool mine = wave_first + (lane & 31) < doc.end;
     const int i = min(wave_first + (lane & 31), doc.end - 1);
     const Span span = key_span(a, doc, i);
+    const bool few = kPlanes<T> == 1 && all_see_few(doc, span);
     const int64_t head_at = static_cast<int64_t>(head) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens + i;
 
     const int low = key_span(a, doc, first).low;
@@ -199,7 +199,7 @@ __device__ __forceinline__ void dq_tile(const DocAttention& a, unsigned block, L
             }
             if constexpr (kScaled<T>) scale.keep_in_range(ds, dq);
             multiply_columns<T, kDim, kTile>(view, k_tile, b, Rows16<T>(ds), first_part, dq);
-            if (kPlanes<T> == 1 && few) {
+            if (few) {
                 keep_rest<T>(ds);
                 multiply_columns<T, kDim, kTile>(view, k_tile, b, Rows16<T>(ds), first_part, dq);
             }
@@ -243,7 +243,6 @@ __device__ __forceinline__ void dkv_tile(const DocAttention& a, unsigned block, 
     int first;
     if (!locate_tile<kOwn, false>(a, block / a.heads, doc, first)) return;
 
-    const bool few = doc.end - doc.start <= kFewTokens;
     const int wave = uniform(static_cast<int>(threadIdx.x) >> 6), lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
     const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
     const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
@@ -251,6 +250,7 @@ __device__ __forceinline__ void dkv_tile(const DocAttention& a, unsigned block, 
     const bool mine = wave_first + (lane & 31) < doc.end;
     const int j = min(wave_first + (lane & 31), doc.end - 1);
     const Span span = query_span(a, doc, j);
+    const bool few = kPlanes<T> == 1 && all_seen_by_few(span);
     const int64_t kv_at = static_cast<int64_t>(kv) * a.head_dim, stat_at = static_cast<int64_t>(head) * a.tokens;
 
     // the queries that see any key of the workgroup; keys in the prefix are seen from the document's start on
@@ -400,7 +400,7 @@ __device__ __forceinline__ void dkv_tile(const DocAttention& a, unsigned block, 
                 scale.keep_in_range(ds, dk);
             }
             add(b, Rows16<T>(p), Rows16<T>(ds));
-            if (kPlanes<T> == 1 && few) {
+            if (few) {
                 keep_rest<T>(p);
                 keep_rest<T>(ds);
                 add(b, Rows16<T>(p), Rows16<T>(ds));

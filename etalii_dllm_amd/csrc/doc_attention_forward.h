@@ -49,13 +49,13 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kD
     int first;
     if (!locate_tile<kOwn, true>(a, blockIdx.x / a.heads, doc, first)) return;
 
-    const bool few = doc.end - doc.start <= kFewTokens;
     const int wave = uniform(static_cast<int>(threadIdx.x) >> 6), lane = static_cast<int>(threadIdx.x) & 63, half = lane >> 5;
     const int part = kPaired ? wave & 1 : 0, first_part = part * kParts;  // of the dimensions
     const int wave_first = first + 32 * (kPaired ? wave >> 1 : wave), wave_last = min(wave_first + 31, doc.end - 1);
     const bool working = wave_first < doc.end;
     const int i = min(wave_first + (lane & 31), doc.end - 1);
     const Span span = key_span(a, doc, i);
+    const bool few = kPlanes<T> == 1 && all_see_few(doc, span);
 
     // keys of the workgroup: [low, high) in whole tiles of the document, and the tiles of the prefix before them
     const int low = key_span(a, doc, first).low;
@@ -184,7 +184,7 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kD
         l += sum;
 #pragma unroll
         for (int b = 0; b < kTile / 32; ++b) multiply_columns<T, kDim, kTile>(view, v_tile, b, Rows16<T>(s[b]), first_part, o);
-        if (kPlanes<T> == 1 && few) {
+        if (few) {
 #pragma unroll
             for (int b = 0; b < kTile / 32; ++b) {
                 keep_rest<T>(s[b]);

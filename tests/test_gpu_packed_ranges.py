@@ -1,5 +1,5 @@
 """GPU: the packed-layer operators at the ends of their ranges: rows of norms far from one, caps of any
-size, upstream gradients of very different sizes. The bounds are those of packed_reference or, where its are as wide as what is
+size, upstream gradients of very different sizes, rows that see few keys. The bounds are those of packed_reference or, where its are as wide as what is
 looked for, tighter ones of the same kind (u = eps / 2 of the activations' type, F = 2^-24)."""
 
 from __future__ import annotations
@@ -155,6 +155,22 @@ def test_float16_gradients_of_small_and_large_values(K, head_dim, size, spread):
     g = gen(73)
     q, k, v, dout = (randn(g, 1500, h, head_dim, scale=s).half() for h, s in ((2, spread), (1, spread), (1, size), (2, 1.0)))
     check(Attention(K, q, k, v, [0, 1500]), dout)
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("options", [dict(), dict(window=50), dict(causal=False, window=32), dict(prefix=[40]),
+                                     dict(window=20, prefix=[44]), dict(window=64, softcap=10.0)])
+def test_rows_that_see_few_keys(K, dtype, head_dim, options):  # noqa: F811
+    """Where a wave's rows see at most 64 keys (its keys at most as many queries) the weights' rounding to 16 bits does not reach
+    the results, in a long document as in a short one."""
+    g, dt = gen(75), R.DTYPES[dtype]
+    for n in (320, 333):
+        q, k, v, dout = (randn(g, n, h, head_dim, dtype=dt) for h in (2, 1, 1, 2))
+        p = Attention(K, q, k, v, [0, n], **options)
+        seen = ~R.hidden(n, p.options["causal"], p.options["window"], (p.options["prefix"] or [0])[0])
+        assert bool((seen.sum(dim=1)[:32] <= 64).all()) or bool((seen.sum(dim=0)[288:320] <= 64).all())
+        check(p, dout, f"{n}", few=64)
 
 
 # ---- norms ----
