@@ -124,3 +124,16 @@ def test_the_checkers_find_a_hazard():
     load = "v_readfirstlane_b32 s87, v1\nv_readfirstlane_b32 s86, v0\ns_nop 0\nglobal_load_lds_dwordx4 v191, s[86:87]\n"
     assert sgpr_base_hazards(load)[1]
     assert not sgpr_base_hazards(load.replace("s_nop 0", "s_nop 4"))[1]
+
+
+@pytest.mark.skipif(not Path(B.HIPCC).exists() and shutil.which("hipcc") is None, reason="hipcc not available")
+@pytest.mark.parametrize("source", ["doc_attention_f32.hip", "doc_attention_bf16.hip", "doc_attention_f16.hip", "doc_attention_wide.hip"])
+def test_tile_copies_respect_their_wait_states(tmp_path, source, monkeypatch):
+    """The document attention kernels' tile copies are the same statements, in sources with flags of their own."""
+    if source in B.AGPR_SUMS:
+        monkeypatch.setattr(B, "FLAGS", B.FLAGS[:-len(B.VGPR_SUMS)])
+    asm = _device_asm(tmp_path, source)
+    copies = asm.count("global_load_lds_dwordx4")
+    checked, bad = sgpr_base_hazards(asm)
+    assert not bad, f"{len(bad)} SGPR-base hazards, e.g. {bad[:3]}"
+    assert checked >= copies // 2 > 0
