@@ -11,7 +11,8 @@ import torch
 
 import packed_reference as R
 from packed_reference import F
-from test_gpu_packed_layers import PACK, Attention, K, gen, norm_backward, norm_forward, problem, randn  # noqa: F401  (K: the fixture)
+from test_gpu_packed_layers import (PACK, Attention, K, Layer, gen, norm_backward, norm_forward, problem,  # noqa: F401  (K: the fixture)
+                                    randn)
 
 pytestmark = pytest.mark.gpu
 
@@ -173,6 +174,39 @@ def test_rows_that_see_few_keys(K, dtype, head_dim, options):  # noqa: F811
         check(p, dout, f"{n}", few=64)
 
 
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize(("extra", "shift"), [(8, 0), (16, 8), (3, 0), (0, 1)])
+def test_attention_into_wider_rows(K, dtype, head_dim, extra, shift):  # noqa: F811
+    """out and dout as parts of wider rows, whole 16-byte chunks or not: the bits of packed ones (in 16 bits a copy of the
+    inputs takes the place of the inputs; the products are the same), and what lies between is left as it was. Infinities too,
+    whose rows are computed and written another way."""
+    n, heads = 150, 4
+    p, dout = problem(K, 76, R.DTYPES[dtype], [3, 90, 150], n, heads, 2, head_dim, window=40, prefix=[0, 9])
+    p.k[20], p.v[20], dout[130] = float("inf"), float("inf"), float("inf")
+    width = heads * head_dim + extra
+
+    def wide(t):
+        flat = torch.full((n * width + shift,), 5.0, dtype=t.dtype, device="cuda")
+        part = flat[shift:].view(n, width)[:, :heads * head_dim].unflatten(1, (heads, head_dim))
+        part.copy_(t)
+        return flat, part
+
+    want = [t.clone() for t in (*p.forward(), *p.backward(dout))]
+    flat, out = wide(torch.full_like(p.out, 5.0))
+    _, upstream = wide(dout)
+    p.out = out
+    p.lse.zero_()
+    p.shape.out_stride = width
+    got = [*p.forward(), *p.backward(upstream)]
+    rows = slice(3, 150)
+    assert torch.equal(got[0][rows].nan_to_num(), want[0][rows].nan_to_num()) and bool((got[0][:3] == 5.0).all())
+    assert torch.equal(got[1].nan_to_num(), want[1].nan_to_num())
+    assert all(torch.equal(a.nan_to_num(), b.nan_to_num()) for a, b in zip(got[2:], want[2:]))
+    assert bool(torch.isnan(got[0][20:60]).any()) and bool(torch.isfinite(got[0][3:20]).all())
+    assert bool((flat[shift:].view(n, width)[:, heads * head_dim:] == 5.0).all()) and bool((flat[:shift] == 5.0).all())
+
+
 # ---- norms ----
 
 
@@ -201,3 +235,60 @@ def test_norm_gradients_of_very_large_and_small_rows(K, dtype, size, eps, placem
     assert got.keys() == want.keys()
     for name in want:
         R.assert_within(got[name], want[name], name)
+
+
+# ---- together ----
+
+
+class Rounded(torch.autograd.Function):
+    """A value, and the gradient that comes back to it, rounded to a type as a kernel's result is."""
+
+    @staticmethod
+    def forward(ctx, x, dt):
+        ctx.dt = dt
+        return x.to(dt).double()
+
+    @staticmethod
+    def backward(ctx, g):
+        return g.to(ctx.dt).double(), None
+
+
+def layer(l, dt):
+    """Layer.step in 64 bits, with each result that the step leaves in its type rounded to it (dt None: with none rounded)."""
+    n, hd = l.n, l.hd
+    r = (lambda t: Rounded.apply(t, dt)) if dt is not None else (lambda t: t)
+    d = lambda t: t.detach().double().requires_grad_()  # noqa: E731
+    x, gate, w = d(l.x), d(l.gate), [d(t) for t in l.w]
+    rms = lambda v, s: v / torch.sqrt(v.square().mean(dim=1, keepdim=True) + 1e-5) * s  # noqa: E731
+    exact_h0 = x + l.y0.double()
+    h0, n0 = r(exact_h0), r(rms(exact_h0, w[0]))
+    q, k, v = (r((n0 @ p.double()).view(n, -1, hd)) for p in l.proj[:3])
+    angle = l.pos[l.axis.long()].double().T * l.freq
+    c, s = torch.cos(angle)[:, None], torch.sin(angle)[:, None]
+    q, k = (r(torch.cat([t[..., :32] * c - t[..., 32:] * s, t[..., 32:] * c + t[..., :32] * s], dim=-1)) for t in (q, k))
+    outs = []
+    for i, (b, e) in enumerate(zip(l.offsets, l.offsets[1:])):
+        mask = R.hidden(e - b, True, 0, l.prefix[i]).cuda()
+        heads = []
+        for h in range(l.heads):
+            z = 20.0 * torch.tanh(q[b:e, h] @ k[b:e, h // 2].T / math.sqrt(hd) / 20.0)
+            heads.append(r(torch.softmax(z.masked_fill(mask, -math.inf), dim=1)) @ v[b:e, h // 2])
+        outs.append(torch.cat(heads, dim=1))
+    y1 = r(r(torch.cat(outs)) @ l.proj[3].double())
+    exact_h1 = h0 + 0.5 * gate * rms(y1, w[1])
+    h1, n1 = r(exact_h1), r(rms(exact_h1, w[2]))
+    grads = torch.autograd.grad([h1, n1], [x, w[0], gate, w[1], w[2]], [l.dh.double(), l.dn.double()])
+    return dict(h1=h1.detach(), n1=n1.detach(), **dict(zip(("dx", "dw0", "dgate", "dw1", "dw2"), grads)))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_a_layer_is_off_by_its_roundings(K, dtype):  # noqa: F811
+    """A block of all three operators is off by as much as the same block in 64 bits with its results rounded at the same places:
+    two draws of the same roundings, whose 2-norms over some hundred to some ten thousand values differ by less than a half of
+    themselves. (dS, which the kernels round too, and the rounded h that the norms' gradients read, are one rounding each beside
+    the dozen on the way: the factor of 2 has room for them.)"""
+    l = Layer(K, 42, R.DTYPES[dtype])
+    got, exact, rounded = l.step(), layer(l, None), layer(l, l.dt)
+    for name in exact:
+        off, draw = (float((t[name].double() - exact[name]).norm() / exact[name].norm()) for t in (got, rounded))
+        assert 0 < off <= 2 * draw, (name, off, draw)
