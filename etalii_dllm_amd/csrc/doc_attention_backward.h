@@ -13,9 +13,12 @@
 // and short calls have half the way (4 float32 documents of 256 tokens, 9/3 heads of 64: 71 to 48 us; 2447 tokens of
 // 4/2 heads of 256: 655 to 383 us).
 //
-// Bound: the matrix cores, as the forward is. 8192 tokens, 16/8 heads of 128 in bfloat16: dq 405 us, 1020 TFLOP/s of its three
-// products; dk and dv 605 to 660 us, 830 to 910 of four; all together 1040 to 1150 us, 600 to 660 TFLOP/s of the five that it
-// could not do without. 8/4 heads of 256, where dk and dv are two kinds of workgroups and eight products in all: 1220 us.
+// Bound: as the forward, few waves' way through products, weights and waits in series, and two products more than the five that
+// the gradients could not do without. 8192 tokens, 16/8 heads of 128 in bfloat16: dq 405 us, 1020 TFLOP/s of its three products
+// (matrix cores, vector units and LDS busy 48, 38 and 24%; of its 1.7 waves on a SIMD 34% wait for memory or LDS and 29% for their
+// turn); dk and dv 605 to 660 us, 830 to 910 of four (37, 24 and 23%; 38 and 17% of 0.9 waves); all together 1040 to 1150 us, 600 to
+// 660 TFLOP/s of the five. 8/4 heads of 256, where dk and dv are two kinds of workgroups and eight products in all: 1200 us (38, 22
+// and 21%; 32 and 28% of 0.9). float32, 4096 tokens of 16/8 heads of 128: 1210 us (55, 22 and 15%; 20 and 45% of 0.9).
 // Another order of dk's and dv's products, with the next tile's scores formed before this one's sums, took 816 us for heads
 // of 128.
 #pragma once
@@ -467,6 +470,7 @@ template <typename T, int kDim>
 constexpr bool kApart = kPlanes<T> == 1 && kDim == 128;
 constexpr unsigned kFewTiles = 512;
 
+// (two waves on a SIMD, 256 registers each; float16 keeps one more in scratch memory)
 template <typename T, int kDim>
 __global__ __launch_bounds__(kDocThreads, 2) void dq_kernel(DocAttention a) {
     static_assert(kApart<T, kDim>);

@@ -24,10 +24,13 @@ constexpr int kBuffers = 4 * kKeys<T, kDim> * kDim * 2 * kPlanes<T> <= 128 * 102
 // float32 sums and 16-bit products hold as well as values below one. P is rounded to the type for the second product, as the
 // type's users expect of it; l is the sum of P before that.
 //
-// Bound: the matrix cores, which this card's power holds to about 1540 TFLOP/s of 16-bit products of random numbers and
-// nothing else. 8192 tokens in bfloat16, of the scores that count: 16/8 heads of 128, 320 to 364 us, 755 to 860 TFLOP/s (567 us
-// and 970 without the causal mask); of 64, 174 us and 790; 8/4 heads of 256, 355 us and 775. float32, 4096 tokens, 16/8 heads of
-// 128: 420 us, of six products 980. Short calls are bound by the way of one workgroup through a row's keys: about 1.1 us a tile
+// Bound: the way of few waves through products, softmax and waits in series; no unit is full. 8192 tokens in bfloat16 (matrix
+// cores, vector units and LDS busy; waves waiting for memory or LDS, and for their turn to issue): 16/8 heads of 128, 41, 45 and
+// 21%; 31 and 26% of 1.6 waves on a SIMD; heads of 64, 36, 63 and 19%; 31 and 28% of 2.5; 8/4 heads of 256, 32, 32 and 16%; 26 and
+// 23% of 0.9. float32, 4096 tokens of 16/8 heads of 128: 45, 24 and 11%; 21 and 40% of 0.9. A loop of nothing but 16-bit products of
+// random numbers reaches 1540 TFLOP/s; of the scores that count these are 320 to 364 us, 755 to 860 TFLOP/s, for heads of 128 (567 to
+// 610 us and 900 to 970 without the causal mask), 170 to 197 us and 700 to 810 for 64, 355 to 390 us and 705 to 775 for 256, and
+// 410 to 435 us for float32, of six products 945 to 1000. Short calls are bound by the way of one workgroup through a row's keys: about 1.1 us a tile
 // of 64 (16-bit), 3.1 us one of 32 (float32).
 template <typename T, int kDim, bool kLargeCap>
 __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kDim <= 128 ? 2 : 1) : 1) void forward_kernel(DocAttention a, T* out) {

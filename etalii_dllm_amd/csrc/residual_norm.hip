@@ -10,7 +10,10 @@
 //
 // Bound: HBM, each row array read and written once. 8192 x 2304 in bfloat16: forward 31.7 us, 4.8 TB/s; gradients 68 us, 3.3 TB/s,
 // where two sums in a row over the workgroup leave gaps that its two or three workgroups on a CU do not fill (8192 x 4096: 87 us,
-// 4.6 TB/s). 4099 x 2048 in float32 with a channel gate: 49 us, 4.1 TB/s.
+// 4.6 TB/s). 4099 x 2048 in float32 with a channel gate: 49 us, 4.1 TB/s. Gradients of rows that are more than a thread's registers
+// are far from it: 16-bit rows of 8193 to 16384 elements (121 to 127 registers in scratch memory with a norm before the next
+// block; 4096 x 12288: 596 us, 1.0 TB/s, where 4096 x 8192 has 3.6), rows of 4097 to 8192 that are not whole 16-byte chunks (56 to
+// 62; 4096 x 6001: 306 us, 1.0 TB/s), and longer ones, which are read once for each sum (4096 x 20000: 1.46 ms, 0.7 TB/s).
 #include <algorithm>
 #include <initializer_list>
 
