@@ -237,6 +237,29 @@ def test_norm_gradients_of_very_large_and_small_rows(K, dtype, size, eps, placem
         R.assert_within(got[name], want[name], name)
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_norm_gradients_of_wide_rows_in_a_graph(K, dtype):  # noqa: F811
+    """Rows whose parameters take more LDS than a kernel has without asking, captured at the kernel's first call."""
+    g, dt, rows, dim = gen(77), R.DTYPES[dtype], 300, 8192
+    x, y, dh, dn = (randn(g, rows, dim, dtype=dt) for _ in range(4))
+    post, pre = (1 + randn(g, dim, scale=0.2) for _ in range(2))
+    shape = K.ResidualNorm(K.DTYPES[dtype], rows, dim, 2, 0, 0, 1e-5, 0.5)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = norm_backward(K, shape, x, y, None, post, pre, dh, dn)
+    want = R.residual_norm(x, y, None, post, pre, 2, 1e-5, False, 0.5, dh=dh, dn=dn)
+    eager = norm_backward(K, shape, x, y, None, post, pre, dh, dn)
+    for _ in range(3):
+        for t in held.values():
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        for name in want:
+            R.assert_within(held[name], want[name], name)
+            assert torch.equal(held[name], eager[name])
+
+
 # ---- together ----
 
 
