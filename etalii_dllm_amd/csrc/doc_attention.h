@@ -5,6 +5,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <initializer_list>
 
 #include "common.h"
@@ -60,29 +61,60 @@ __device__ __forceinline__ Document document_at(const DocAttention& a, int d) {
     return r;
 }
 
-// The tile-th part of kRows tokens, counted through all documents; each document starts a part of its own, so that what
-// is computed for it does not depend on where it lies. Every lane of the wave returns the same. False past the last part.
+// The tile-th part of kRows tokens of all documents; each document starts a part of its own, so that what is computed for it
+// does not depend on where it lies. Every lane of the wave returns the same. False where there is no such part: past the last one
+// and, among many documents, in between.
 //
 // Parts come longest first, as far as that is cheap to know, so that the last workgroups to start are short ones: kFromEnd is
 // for work that grows towards a document's end (a causal row's keys), else towards its start (a key's queries). Up to 64
 // causal documents (one to a lane): the parts of the highest level first, of all documents that reach it, where a part's level
 // counts from the end with less work. Else the documents in order, each from the end with more work. (Ten documents of 1 to 2048
 // tokens, 8192 in all, 16/8 heads of 128 in bfloat16: 97 us in their order, 83 by level; gradients 363 and 345.)
+//
+// More documents than lanes are not counted through, which would take every workgroup a time that grows with their number. Part p
+// of document d is tile start / kRows + d + p instead: that gives no tile twice (a document has at most one part more than
+// start / kRows steps on to the next) and leaves some out, and grows with d, which is searched for, 64 documents at once. (5000
+// documents of 10 tokens, 8/4 heads of 64 in bfloat16: counted 1523 us and 8.8 ms for the gradients, searched 256 us and 1.2 ms.)
+constexpr int kFewDocuments = 64;
+
 template <int kRows, bool kFromEnd>
-__device__ __forceinline__ bool find_tile(const DocAttention& a, int64_t tile, Document& doc, int& first) {
+__device__ __forceinline__ bool find_tile_of_many(const DocAttention& a, int tile, Document& doc, int& first) {
     const int lane = static_cast<int>(threadIdx.x) & 63;
-    auto found = [&](const Document& mine, int owner, int level) {
+    const int at = kFromEnd ? (a.tokens + kRows - 1) / kRows + a.documents - 1 - tile : tile;
+    auto first_tile = [&](int d) { return clamp_token(a.offsets[d], 0, a.tokens) / kRows + d; };
+    int low = 0, step;  // document low begins at or before the tile, low + count, if there is one, after it
+    for (int count = a.documents; count > 0; count = step == 1 ? 0 : min(step, count)) {
+        step = (count + 63) / 64;
+        const int off = lane * step;
+        const uint64_t begun = __ballot(off < count && first_tile(low + min(off, count - 1)) <= at);
+        if (!begun) return false;
+        const int last = (__popcll(begun) - 1) * step;
+        low += last, count -= last;
+    }
+    doc = document_at(a, low);
+    const int part = at - first_tile(low);
+    if (part >= (doc.end - doc.start + kRows - 1) / kRows) return false;
+    first = doc.start + part * kRows;
+    return true;
+}
+
+template <int kRows, bool kFromEnd>
+__device__ __forceinline__ bool find_tile(const DocAttention& a, int tile, Document& doc, int& first) {
+    if (a.documents > kFewDocuments) return find_tile_of_many<kRows, kFromEnd>(a, tile, doc, first);
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int d = a.causal || !kFromEnd ? lane : a.documents - 1 - lane;
+    Document mine{0, 0, 0};
+    if (d >= 0 && d < a.documents) mine = document_at(a, d);
+    const int parts = (mine.end - mine.start + kRows - 1) / kRows;
+    auto found = [&](int owner, int level) {
         doc.start = __builtin_amdgcn_readlane(mine.start, owner);
         doc.end = __builtin_amdgcn_readlane(mine.end, owner);
         doc.prefix_end = __builtin_amdgcn_readlane(mine.prefix_end, owner);
-        const int parts = (doc.end - doc.start + kRows - 1) / kRows;
-        first = doc.start + (kFromEnd ? level : parts - 1 - level) * kRows;
+        const int all = (doc.end - doc.start + kRows - 1) / kRows;
+        first = doc.start + (kFromEnd ? level : all - 1 - level) * kRows;
         return true;
     };
-    if (a.documents <= 64 && a.causal) {
-        Document mine{0, 0, 0};
-        if (lane < a.documents) mine = document_at(a, lane);
-        const int parts = (mine.end - mine.start + kRows - 1) / kRows;
+    if (a.causal) {
         const int bits = 32 - __builtin_clz((a.tokens + kRows - 1) / kRows | 1);
         auto at_or_above = [&](int level) {  // parts of that level or higher, by the bits of each document's number of them
             const int n = parts > level ? parts - level : 0;
@@ -96,40 +128,28 @@ __device__ __forceinline__ bool find_tile(const DocAttention& a, int64_t tile, D
             if (at_or_above(level + (1 << b)) > tile) level += 1 << b;
         uint64_t reach = __ballot(parts > level);
         for (int64_t skip = tile - at_or_above(level + 1); skip > 0; --skip) reach &= reach - 1;
-        return found(mine, __builtin_ctzll(reach), level);
+        return found(__builtin_ctzll(reach), level);
     }
-    int64_t before = 0;
-    for (int base = 0; base < a.documents; base += 64) {
-        const int d = kFromEnd ? a.documents - 1 - base - lane : base + lane;
-        Document mine{0, 0, 0};
-        if (d >= 0 && d < a.documents) mine = document_at(a, d);
-        const int parts = (mine.end - mine.start + kRows - 1) / kRows;
-        int64_t through = parts;  // parts of the lanes up to this one
+    int64_t through = parts;  // parts of the lanes up to this one
 #pragma unroll
-        for (int s = 1; s < 64; s <<= 1) {
-            const int64_t o = __shfl_up(through, s);
-            if (lane >= s) through += o;
-        }
-        const int64_t all = __shfl(through, 63);
-        if (tile < before + all) {
-            const int owner = __builtin_ctzll(__ballot(before + through > tile));
-            const int part = static_cast<int>(tile - __shfl(before + through - parts, owner));
-            const int count = __builtin_amdgcn_readlane(parts, owner);
-            return found(mine, owner, __builtin_amdgcn_readfirstlane(count - 1 - part));
-        }
-        before += all;
+    for (int s = 1; s < 64; s <<= 1) {
+        const int64_t o = __shfl_up(through, s);
+        if (lane >= s) through += o;
     }
-    return false;
+    if (tile >= __shfl(through, 63)) return false;
+    const int owner = __builtin_ctzll(__ballot(through > tile));
+    const int part = static_cast<int>(tile - __shfl(through - parts, owner));
+    return found(owner, __builtin_amdgcn_readfirstlane(__builtin_amdgcn_readlane(parts, owner) - 1 - part));
 }
 
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 
 // find_tile, with its results in scalar registers: what follows from them (loops, branches, addresses) is scalar too.
 template <int kRows, bool kFromEnd>
-__device__ __forceinline__ bool locate_tile(const DocAttention& a, int64_t tile, Document& doc, int& first) {
+__device__ __forceinline__ bool locate_tile(const DocAttention& a, unsigned tile, Document& doc, int& first) {
     Document d{0, 0, 0};
     int f = 0;
-    const int found = find_tile<kRows, kFromEnd>(a, tile, d, f);
+    const int found = find_tile<kRows, kFromEnd>(a, static_cast<int>(tile), d, f);
     doc.start = uniform(d.start), doc.end = uniform(d.end), doc.prefix_end = uniform(d.prefix_end);
     first = uniform(f);
     return uniform(found);
@@ -397,9 +417,10 @@ __device__ __forceinline__ void store_row(To* to, const float (&v)[kLaneDims], i
         if (lane + 64 * c < head_dim) to[lane + 64 * c] = static_cast<To>(v[c]);
 }
 
-// Parts of `rows` tokens of all documents, at most.
+// Tiles that find_tile gives parts of `rows` tokens, at most.
 inline unsigned doc_tiles(const DocAttention& a, int rows) {
-    return static_cast<unsigned>(ceil_div(a.tokens, rows) + (a.documents < a.tokens ? a.documents : a.tokens));
+    const int parts_begun = a.documents > kFewDocuments ? a.documents : std::min(a.documents, a.tokens);
+    return static_cast<unsigned>(ceil_div(a.tokens, rows) + parts_begun);
 }
 
 // Whole 16-byte chunks throughout, and strides that leave a copy's lane offsets below 2^32 bytes.

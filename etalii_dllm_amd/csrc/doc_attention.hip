@@ -30,7 +30,7 @@ int check_shape(const dllm_hip_document_attention_shape* sh) {
     for (const int64_t s : {sh->q_stride, sh->out_stride}) DLLM_REQUIRE(s == 0 || s >= q, "a token stride must be 0 or at least heads * head_dim");
     for (const int64_t s : {sh->k_stride, sh->v_stride}) DLLM_REQUIRE(s == 0 || s >= k, "a token stride must be 0 or at least heads * head_dim");
     // a grid's x extent times its workgroup is below 2^32
-    DLLM_REQUIRE((static_cast<int64_t>(ceil_div(sh->tokens, kDocTileRows / 2)) + std::min(sh->documents, sh->tokens)) * sh->heads < (1 << 24),
+    DLLM_REQUIRE((static_cast<int64_t>(ceil_div(sh->tokens, kDocTileRows / 2)) + sh->documents) * sh->heads < (1 << 24),
                  "too many tokens and documents for one call");
     return kOk;
 }

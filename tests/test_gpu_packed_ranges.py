@@ -207,6 +207,34 @@ def test_attention_into_wider_rows(K, dtype, head_dim, extra, shift):  # noqa: F
     assert bool((flat[shift:].view(n, width)[:, heads * head_dim:] == 5.0).all()) and bool((flat[:shift] == 5.0).all())
 
 
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize("options", [dict(), dict(causal=False, window=70)])
+@pytest.mark.parametrize("repeats", [2, 3, 500])
+def test_many_documents_repeat_a_few(K, dtype, options, repeats):  # noqa: F811
+    """A pack of 40 documents, empty ones and ends of tiles among them, over and over: each time the bits of the one pack, whose
+    documents a wave finds another way; prefixes of their own, and tokens of none before and after."""
+    lengths = [0, 1, 2, 127, 128, 129, 0, 0, 64, 65, 200, 1, 63, 3, 17, 256] + [(7 * i) % 23 for i in range(24)]
+    prefix = [(5 * i) % 40 for i in range(40)]
+    n = sum(lengths)
+    offsets = [0]
+    for length in lengths:
+        offsets.append(offsets[-1] + length)
+    one, dout = problem(K, 78, R.DTYPES[dtype], offsets, n, 2, 1, 64, prefix=prefix, **options)
+    want = [t.clone() for t in (*one.forward(), *one.backward(dout))]
+
+    def tiled(t):  # 5 tokens of no document, the pack again and again, 9 more
+        return torch.cat([t[:5], *[t] * repeats, t[:9]])
+
+    ends = [5 + r * n + o for r in range(repeats) for o in offsets[:-1]] + [5 + repeats * n]
+    p = Attention(K, tiled(one.q), tiled(one.k), tiled(one.v), ends, prefix=prefix * repeats, **options)
+    got = [*p.forward(), *p.backward(tiled(dout))]
+    got[1], want[1] = got[1].T, want[1].T
+    for x, y in zip(got, want):
+        inside = x[5:5 + repeats * n].reshape(repeats, *y.shape)
+        assert torch.equal(inside, y.expand(repeats, *y.shape))
+        assert bool((x[:5] == 0).all()) and bool((x[5 + repeats * n:] == 0).all())
+
+
 # ---- norms ----
 
 

@@ -310,3 +310,15 @@ def test_rope_axes_refuses_axes_that_eight_bits_wrap(K, axis):
     x = np.zeros((4, 2, 8), np.float32)
     with pytest.raises(ValueError, match="pair_axis"):
         K.rope_axes(x, x, np.zeros((3, 4)), np.ones(4), np.array([0, 1, 2, axis]))
+
+
+@needs_library
+def test_attention_refuses_more_empty_documents_than_tiles(K):
+    """A launch has a tile for each document, empty ones too: their number is limited whatever the number of tokens."""
+    for change in (dict(documents=(1 << 31) - 1), dict(documents=1 << 22)):
+        shape = K.DocumentAttention(**{**ATTENTION, **change})
+        with pytest.raises(ValueError, match="too many"):
+            K.check(K.lib.dllm_hip_document_attention(shape, *[P] * 9, 1 << 60, None))
+        with pytest.raises(ValueError, match="too many"):
+            K.check(K.lib.dllm_hip_document_attention_backward(shape, *[P] * 13, 1 << 60, None))
+    assert K.lib.dllm_hip_document_attention_workspace(K.DocumentAttention(**{**ATTENTION, "documents": (1 << 22) - 2})) > 0
