@@ -226,16 +226,18 @@ __device__ __forceinline__ float bend_score(const DocAttention& a, float slope, 
 //   1 - 2 / (1 + e^2|z|).
 // Large caps have kernels of their own: in the same ones, chosen by a branch, they cost other calls registers (8192 tokens of
 // 16/8 heads of 64 in bfloat16, without a cap, 168 and 178 us). Caps of 50 and 100: 8000 + 192 tokens, 8/4 heads of 256, window 4096,
-// 377 and 462 us; gradients of 8192 tokens, 16/8 heads of 128, 1257 and 1830.
+// 377 and 462 us; gradients of 8192 tokens, 16/8 heads of 128, 1323 and 1925.
 constexpr float kSmallCap = 64.0f;
 
 inline bool large_cap(const DocAttention& a) { return a.softcap > kSmallCap; }
 
-__device__ __forceinline__ float tanh_of_any_size(float z) {
+__device__ __forceinline__ float tanh_of_any_size(float z, float& derivative) {
     const float w = z * z;
     const float near = z * fmaf(w + 105.0f, w, 945.0f) * __builtin_amdgcn_rcpf(fmaf(fmaf(15.0f, w, 420.0f), w, 945.0f));
-    const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.0f * kLog2E * fabsf(z))), 1.0f);
-    return fabsf(z) < 0.5f ? near : copysignf(far, z);
+    const float tail = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.0f * kLog2E * fabsf(z)));  // (1 - tanh |z|) / 2
+    const bool is_near = fabsf(z) < 0.5f;
+    derivative = is_near ? fmaf(-near, near, 1.0f) : 4.0f * fmaf(-tail, tail, tail);
+    return is_near ? near : copysignf(fmaf(-2.0f, tail, 1.0f), z);
 }
 
 template <typename T, bool kLargeCap>
@@ -250,13 +252,19 @@ struct CapTerms {
         times = unit, plus = 0.0f;
         if (kHalved && capped) in *= 2.0f * kLog2E, times = 2.0f * unit, plus = unit;
     }
-    __device__ __forceinline__ float bend(float x) const {
-        if constexpr (sizeof(T) == 4) return tanhf(x * in);
-        if constexpr (kLargeCap) return tanh_of_any_size(x * in);
-        return __builtin_amdgcn_rcpf(-1.0f - __builtin_amdgcn_exp2f(x * in));
+    // bent, and the cap's derivative: of a halved one 4 e b^2 with e = e^2z, which is right to its last bits where the cap is nearly
+    // reached on either side (one minus the square of a tanh near one is not; float32 has it as any float32 evaluation would)
+    __device__ __forceinline__ float bend(float x, float& derivative) const {
+        if constexpr (kLargeCap) return tanh_of_any_size(x * in, derivative);
+        if constexpr (sizeof(T) == 4) {
+            const float t = tanhf(x * in);
+            derivative = fmaf(-t, t, 1.0f);
+            return t;
+        }
+        const float e = __builtin_amdgcn_exp2f(x * in), b = __builtin_amdgcn_rcpf(-1.0f - e);
+        derivative = fminf(e, 0x1p126f) * b * (4.0f * b);
+        return b;
     }
-    // bend's tanh, whose square is one minus the cap's derivative
-    __device__ __forceinline__ float tangent(float bent) const { return kHalved ? fmaf(2.0f, bent, 1.0f) : bent; }
 };
 
 template <typename T>

@@ -175,9 +175,9 @@ __device__ __forceinline__ void dq_tile(const DocAttention& a, unsigned block, L
             if (cap.capped) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    x[r] = cap.bend(x[r]);
-                    const float tangent = cap.tangent(x[r]);
-                    ds[r] *= fmaf(-tangent, tangent, 1.0f);
+                    float derivative;
+                    x[r] = cap.bend(x[r], derivative);
+                    ds[r] *= derivative;
                 }
             }
 #pragma unroll
@@ -349,9 +349,9 @@ __device__ __forceinline__ void dkv_tile(const DocAttention& a, unsigned block, 
             if (cap.capped) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    x[r] = cap.bend(x[r]);
-                    const float tangent = cap.tangent(x[r]);
-                    ds[r] *= fmaf(-tangent, tangent, 1.0f);
+                    float derivative;
+                    x[r] = cap.bend(x[r], derivative);
+                    ds[r] *= derivative;
                 }
             }
 #pragma unroll

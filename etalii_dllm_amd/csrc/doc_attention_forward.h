@@ -132,10 +132,11 @@ __global__ __launch_bounds__(kDocThreads, kPlanes<T> == 1 ? (kDim <= 64 ? 3 : kD
             for (int r = 0; r < 16; ++r) s[b][r] = x[b][r];
         float times = cap.times, plus = cap.plus;  // s times + plus: the score in units of log 2
         if (cap.capped) {
+            float unused;
 #pragma unroll
             for (int b = 0; b < kTile / 32; ++b)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) s[b][r] = cap.bend(s[b][r]);
+                for (int r = 0; r < 16; ++r) s[b][r] = cap.bend(s[b][r], unused);
         }
         if (a.slopes) {
             const float away = static_cast<float>(i - from - 4 * half);

@@ -1,5 +1,5 @@
 """GPU: the packed-layer operators at the ends of their ranges: rows of norms far from one, caps of any
-size, upstream gradients of very different sizes, rows that see few keys. The bounds are those of packed_reference or, where its are as wide as what is
+size and scores that reach them, upstream gradients of very different sizes, rows that see few keys. The bounds are those of packed_reference or, where its are as wide as what is
 looked for, tighter ones of the same kind (u = eps / 2 of the activations' type, F = 2^-24)."""
 
 from __future__ import annotations
@@ -109,6 +109,48 @@ def test_caps_of_any_size(K, dtype, head_dim, cap):  # noqa: F811
     if cap <= 1e5:
         check(Attention(K, q, k, v, [0, 150], softcap=cap, scale=cap / 8), dout, "scores about the cap's size")
     check(Attention(K, q, k, v, [0, 150], softcap=cap, causal=False, slopes=[0.1, 0.0]), dout, "bias")
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("head_dim", [64, 128, 256])
+@pytest.mark.parametrize("cap", [1.0, 30.0, 100.0])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_gradients_of_scores_near_the_cap(K, dtype, head_dim, cap, sign):  # noqa: F811
+    """Scores of 3 to 9 times the cap are bent almost flat: their small derivatives, 1e-2 to 1e-7, are right to the type."""
+    g, dt, n = gen(79), R.DTYPES[dtype], 100
+    q, k = ((0.75 + 0.5 * torch.rand(n, h, head_dim, generator=g, device="cuda")).to(dt) for h in (2, 1))
+    q, v, dout = q * sign, randn(g, n, 1, head_dim, dtype=dt), randn(g, n, 2, head_dim, dtype=dt)
+    # of the scores' sizes: q.k is head_dim times 0.6 to 1.5
+    p = Attention(K, q, k, v, [0, n], softcap=cap, scale=6 * cap / head_dim)
+    if dtype == "float16":
+        dout = dout * 1000  # (results of 1e-6 would be subnormal)
+    out, lse = p.forward()
+    dq, dk, _ = p.backward(dout)
+    seen = ~R.hidden(n, True, 0, 0).cuda()
+    u, bounds = R.unit(dt), dict(dk=[0.0, 0.0])
+    for h in range(2):
+        Q, Kh, V, dO, O = (t.double() for t in (q[:, h], k[:, 0], v[:, 0], dout[:, h], out[:, h]))
+        z = Q @ Kh.T * (p.scale / cap)
+        ez = (head_dim + 8) * F * z.abs()  # (every term has one sign)
+        assert float(z[seen].abs().min()) > 2.5 and float(z[seen].abs().max()) < 9.5
+        t = torch.tanh(z)
+        slope = torch.cosh(z) ** -2
+        # e^2z's relative error is 2 ez and its own roundings': so are those of 1 - tanh and of the derivative
+        eslope = slope * (2 * ez + 8 * F * (1 + z.abs()))
+        w = torch.exp(cap * t - lse[h].double()[:, None]).masked_fill(~seen, 0.0)
+        ew = w * (cap * (slope * ez + 8 * F) + 4 * F * (1 + cap) + 8 * F)
+        dP, delta = dO @ V.T, (dO * O).sum(dim=1, keepdim=True)
+        size = dO.abs() @ V.abs().T + (dO.abs() * O.abs()).sum(dim=1, keepdim=True)
+        dS = w * (dP - delta) * slope * p.scale
+        eS = p.scale * (size * (w * eslope + ew * slope + w * slope * (head_dim + 16) * F)) + dS.abs() * u
+        grown = [2.0 ** -33 * (dS.abs() + eS).amax(dim=d, keepdim=True) * seen * (dtype == "float16") for d in (1, 0)]
+        value = dS @ Kh
+        bound = u * value.abs() + ((eS + grown[0]) @ Kh + 2 * n * F * (dS.abs() @ Kh)) * (1 + u) + R.tiny(dt)
+        R.assert_within(dq[:, h], (value, bound), f"dq {h}")
+        bounds["dk"][0] += dS.T @ Q
+        bounds["dk"][1] += ((eS + grown[1]).T @ Q.abs() + (2 * n + 10) * F * (dS.abs().T @ Q)) * (1 + u)
+    value, bound = bounds["dk"]
+    R.assert_within(dk[:, 0], (value, bound + u * value.abs() + R.tiny(dt)), "dk")
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES)
