@@ -1,6 +1,7 @@
-"""GPU: the packed-layer operators at the ends of their ranges: rows of norms far from one, caps of any
-size and scores that reach them, upstream gradients of very different sizes, rows that see few keys. The bounds are those of packed_reference or, where its are as wide as what is
-looked for, tighter ones of the same kind (u = eps / 2 of the activations' type, F = 2^-24)."""
+"""GPU: the packed-layer operators at the ends of their ranges: rows of norms far from one, caps of any size and scores that
+reach them, upstream gradients of very different sizes, rows that see few keys, many documents, outputs in wider rows. The
+bounds are those of packed_reference or, where its are as wide as what is looked for, tighter ones of the same kind (u = eps / 2
+of the activations' type, F = 2^-24)."""
 
 from __future__ import annotations
 
