@@ -40,6 +40,14 @@ int check_launch(const char* what);
 inline size_t ceil_div(size_t a, size_t b) { return (a + b - 1) / b; }
 inline size_t round_up(size_t a, size_t b) { return ceil_div(a, b) * b; }
 
+// A grid of `blocks` workgroups (below 2^36) in two extents, since one extent times its workgroup is below 2^32; block_id() counts
+// them, those past the last too.
+inline dim3 grid_of(size_t blocks) {
+    const size_t x = blocks < (size_t{1} << 20) ? (blocks > 0 ? blocks : 1) : size_t{1} << 20;
+    return dim3(static_cast<unsigned>(x), static_cast<unsigned>(ceil_div(blocks > 0 ? blocks : 1, x)));
+}
+__device__ __forceinline__ int64_t block_id() { return static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x; }
+
 // Wave size of CDNA: every kernel here is written for 64-wide wavefronts.
 constexpr int kWave = 64;
 

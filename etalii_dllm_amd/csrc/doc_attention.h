@@ -11,12 +11,12 @@
 #include "common.h"
 #include "doc_tile.h"
 #include "element.h"
+#include "softcap.h"
 
 namespace dllm_hip {
 
 constexpr int kDocThreads = 256;
 constexpr int kDocTileRows = 128;  // tokens of a workgroup, 32 for each wave (64 of wide float32 heads)
-constexpr float kLog2E = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 struct DocAttention {
     const void *q, *k, *v, *out, *dout;  // out: written by the forward, read by the backward
@@ -221,24 +221,13 @@ __device__ __forceinline__ float bend_score(const DocAttention& a, float slope, 
 // too. With 16-bit types it is
 // - of caps up to kSmallCap -1 / (1 + e^2z) = (tanh z - 1) / 2, whose rest falls into times and plus. It is off by at most about
 //   6 x 2^-24 of the cap however small the score is: 2^-15 of a weight, which rounds to 2^-9 or 2^-12 of itself.
-// - of larger ones, whose scores may be any part of the cap, tanh again, to about 6 x 2^-24 of itself: z (945 + 105 z^2 + z^4) /
-//   (945 + 420 z^2 + 15 z^4), Lambert's continued fraction cut after five levels, where |z| < 1/2 (off by 2^-27), else
-//   1 - 2 / (1 + e^2|z|).
+// - of larger ones, whose scores may be any part of the cap, tanh again (softcap.h).
 // Large caps have kernels of their own: in the same ones, chosen by a branch, they cost other calls registers (8192 tokens of
 // 16/8 heads of 64 in bfloat16, without a cap, 168 and 178 us). Caps of 50 and 100: 8000 + 192 tokens, 8/4 heads of 256, window 4096,
 // 377 and 462 us; gradients of 8192 tokens, 16/8 heads of 128, 1323 and 1925.
 constexpr float kSmallCap = 64.0f;
 
 inline bool large_cap(const DocAttention& a) { return a.softcap > kSmallCap; }
-
-__device__ __forceinline__ float tanh_of_any_size(float z, float& derivative) {
-    const float w = z * z;
-    const float near = z * fmaf(w + 105.0f, w, 945.0f) * __builtin_amdgcn_rcpf(fmaf(fmaf(15.0f, w, 420.0f), w, 945.0f));
-    const float tail = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(2.0f * kLog2E * fabsf(z)));  // (1 - tanh |z|) / 2
-    const bool is_near = fabsf(z) < 0.5f;
-    derivative = is_near ? fmaf(-near, near, 1.0f) : 4.0f * fmaf(-tail, tail, tail);
-    return is_near ? near : copysignf(fmaf(-2.0f, tail, 1.0f), z);
-}
 
 template <typename T, bool kLargeCap>
 struct CapTerms {

@@ -1,0 +1,443 @@
+// The sort and the sums of token_rows.h.
+//
+// Sort: least significant digits first, 9 bits at a time (a vocabulary of 2^18 takes two passes). A position's place is the
+// number of smaller digits, the same digits in earlier waves (counts of each wave and digit, scanned), and those before it
+// in its own wave, which 9 ballots per 64 positions give without any atomic operation, so the sort is stable and its result
+// the same every time. Up to 16384 positions stay in one workgroup's LDS for all passes; more go through memory, each
+// pass three launches. 16384 tokens of 2^18: see the figures at sort_kernel.
+//
+// Sums: a wave takes 16 sorted positions and 16 bytes of columns to a lane, reads all 16 rows at once and adds them in order.
+// A token whose positions lie within the 16 is done; the sums of others are float32 parts, added in their order by a second
+// launch. Nothing depends on when a wave runs.
+#include "token_rows.h"
+
+#include <algorithm>
+#include <initializer_list>
+
+namespace dllm_hip {
+
+namespace {
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortWaves = kSortThreads / kWave;
+constexpr int kSortRounds = 16;  // positions of a thread
+constexpr int kSortBlock = kSortThreads * kSortRounds;
+constexpr int kDigitBits = 9;
+constexpr int kDigits = 1 << kDigitBits;
+
+struct SortCounts {
+    uint16_t wave[kSortWaves][kDigits];
+    uint32_t digit[kDigits];
+    uint32_t carry[kDigits / kWave];
+};
+
+// The items of a workgroup lie wave by wave, `rounds` times 64 to a wave.
+__device__ __forceinline__ int sort_item(int rounds, int r) {
+    return ((static_cast<int>(threadIdx.x) >> 6) * rounds + r) * kWave + (static_cast<int>(threadIdx.x) & 63);
+}
+
+// rank[i]: how many items with item i's digit come before it in its wave; then counts.wave: those in earlier waves;
+// counts.digit: the items with smaller digits.
+__device__ __forceinline__ void rank_digits(const uint32_t* keys, int rounds, int n, int shift, SortCounts& counts, uint16_t* ranks) {
+    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63;
+    for (int i = threadIdx.x; i < kSortWaves * kDigits; i += kSortThreads) (&counts.wave[0][0])[i] = 0;
+    __syncthreads();
+    volatile uint16_t* const mine = counts.wave[wave];
+    for (int r = 0; r < rounds; ++r) {
+        const int i = sort_item(rounds, r);
+        const bool valid = i < n;
+        const uint32_t d = valid ? (keys[i] >> shift) & (kDigits - 1) : 0;
+        uint64_t same = __ballot(valid);
+#pragma unroll
+        for (int b = 0; b < kDigitBits; ++b) {
+            const uint64_t set = __ballot((d >> b) & 1);
+            same &= (d >> b) & 1 ? set : ~set;
+        }
+        const int before = __popcll(same & ((uint64_t{1} << lane) - 1));
+        const int old = mine[d];
+        __builtin_amdgcn_wave_barrier();
+        if (valid) {
+            ranks[i] = static_cast<uint16_t>(old + before);
+            if (before == 0) mine[d] = static_cast<uint16_t>(old + __popcll(same));
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+    __syncthreads();
+    uint32_t total = 0, sum = 0;
+    if (threadIdx.x < kDigits) {
+#pragma unroll
+        for (int w = 0; w < kSortWaves; ++w) {
+            const uint32_t c = counts.wave[w][threadIdx.x];
+            counts.wave[w][threadIdx.x] = static_cast<uint16_t>(total);
+            total += c;
+        }
+        sum = total;
+#pragma unroll
+        for (int s = 1; s < kWave; s *= 2) {
+            const uint32_t o = __shfl_up(sum, s);
+            if (lane >= s) sum += o;
+        }
+        if (lane == kWave - 1) counts.carry[wave] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x < kDigits) {
+        uint32_t before = 0;
+        for (int w = 0; w < wave; ++w) before += counts.carry[w];
+        counts.digit[threadIdx.x] = before + sum - total;
+    }
+    __syncthreads();
+}
+
+__device__ __forceinline__ uint32_t token_key(int64_t token, int64_t vocabulary) {
+    return static_cast<uint32_t>(token >= 0 && token < vocabulary ? token : vocabulary);
+}
+
+// word to every word of `bytes` bytes at `at` (aligned to 2), by workgroups `block` of `blocks`
+__device__ __forceinline__ void fill_part(char* at, size_t bytes, uint32_t word, size_t block, size_t blocks) {
+    const size_t head = min(bytes, (16 - reinterpret_cast<uintptr_t>(at) % 16) % 16), chunks = (bytes - head) / 16;
+    uint4* const body = reinterpret_cast<uint4*>(at + head);
+    for (size_t i = block * blockDim.x + threadIdx.x; i < chunks; i += blocks * blockDim.x) body[i] = make_uint4(word, word, word, word);
+    const size_t tail = head + chunks * 16;
+    if (block == 0) {
+        for (size_t i = 2 * threadIdx.x; i + 2 <= head; i += 2 * blockDim.x) *reinterpret_cast<uint16_t*>(at + i) = static_cast<uint16_t>(word);
+        for (size_t i = tail + 2 * threadIdx.x; i + 2 <= bytes; i += 2 * blockDim.x)
+            *reinterpret_cast<uint16_t*>(at + i) = static_cast<uint16_t>(word);
+    }
+}
+
+__global__ __launch_bounds__(256) void fill_kernel(char* at, size_t bytes, uint32_t word) {
+    fill_part(at, bytes, word, blockIdx.x, gridDim.x);
+}
+
+// Workgroup 0 sorts, the others fill.
+__global__ __launch_bounds__(kSortThreads) void sort_kernel(const int64_t* __restrict__ tokens, int n, int64_t vocabulary, int passes,
+                                                            TokenOrder order, char* fill_at, size_t fill_bytes, uint32_t fill) {
+    __shared__ SortCounts counts;
+    __shared__ uint32_t keys[kSortBlock];
+    __shared__ uint16_t positions[kSortBlock], ranks[kSortBlock];
+    if (blockIdx.x > 0) {
+        fill_part(fill_at, fill_bytes, fill, blockIdx.x - 1, gridDim.x - 1);
+        return;
+    }
+    const int rounds = (n + kSortThreads - 1) / kSortThreads;
+    for (int i = threadIdx.x; i < n; i += kSortThreads) {
+        keys[i] = token_key(tokens[i], vocabulary);
+        positions[i] = static_cast<uint16_t>(i);
+    }
+    __syncthreads();
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * kDigitBits, wave = static_cast<int>(threadIdx.x) >> 6;
+        rank_digits(keys, rounds, n, shift, counts, ranks);
+        uint32_t key[kSortRounds], to[kSortRounds];
+        uint16_t position[kSortRounds];
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r) {
+            const int i = sort_item(rounds, r);
+            if (r < rounds && i < n) {
+                key[r] = keys[i], position[r] = positions[i];
+                const uint32_t d = (key[r] >> shift) & (kDigits - 1);
+                to[r] = counts.digit[d] + counts.wave[wave][d] + ranks[i];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int r = 0; r < kSortRounds; ++r)
+            if (r < rounds && sort_item(rounds, r) < n) keys[to[r]] = key[r], positions[to[r]] = position[r];
+        __syncthreads();
+    }
+    const uint32_t outside = static_cast<uint32_t>(vocabulary);
+    for (int i = threadIdx.x; i < n; i += kSortThreads) {
+        const uint32_t key = keys[i];
+        order.token[i] = key;
+        order.position[i] = positions[i];
+        if (key != outside && (i == n - 1 || keys[i + 1] == outside)) *order.kept = i + 1;
+        if (i == 0 && key == outside) *order.kept = 0;
+    }
+}
+
+// One pass over more positions: this workgroup's number of each digit, by digit and workgroup ...
+__global__ __launch_bounds__(kSortThreads) void digit_counts_kernel(const int64_t* __restrict__ tokens, const uint32_t* __restrict__ key,
+                                                                    int64_t n, int64_t vocabulary, int shift, uint32_t* __restrict__ counts) {
+    __shared__ uint32_t of[kDigits];
+    for (int i = threadIdx.x; i < kDigits; i += kSortThreads) of[i] = 0;
+    __syncthreads();
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortBlock, end = min(n, first + kSortBlock);
+    for (int64_t i = first + threadIdx.x; i < end; i += kSortThreads)
+        atomicAdd(&of[((key ? key[i] : token_key(tokens[i], vocabulary)) >> shift) & (kDigits - 1)], 1u);
+    __syncthreads();
+    for (int i = threadIdx.x; i < kDigits; i += kSortThreads) counts[static_cast<size_t>(i) * gridDim.x + blockIdx.x] = of[i];
+}
+
+// ... their sums before each, by one workgroup ...
+__global__ __launch_bounds__(kSortThreads) void scan_kernel(uint32_t* __restrict__ counts, int64_t n) {
+    __shared__ uint32_t carry[kSortWaves];
+    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63;
+    uint32_t before = 0;
+    for (int64_t base = 0; base < n; base += kSortThreads) {
+        const int64_t i = base + threadIdx.x;
+        const uint32_t c = i < n ? counts[i] : 0;
+        uint32_t sum = c;
+#pragma unroll
+        for (int s = 1; s < kWave; s *= 2) {
+            const uint32_t o = __shfl_up(sum, s);
+            if (lane >= s) sum += o;
+        }
+        if (lane == kWave - 1) carry[wave] = sum;
+        __syncthreads();
+        uint32_t earlier = 0, all = 0;
+        for (int w = 0; w < kSortWaves; ++w) {
+            if (w < wave) earlier += carry[w];
+            all += carry[w];
+        }
+        if (i < n) counts[i] = before + earlier + sum - c;
+        before += all;
+        __syncthreads();
+    }
+}
+
+// ... and the positions to their places.
+__global__ __launch_bounds__(kSortThreads) void scatter_kernel(const int64_t* __restrict__ tokens, const uint32_t* __restrict__ key_in,
+                                                               const uint32_t* __restrict__ position_in, int64_t n, int64_t vocabulary,
+                                                               int shift, const uint32_t* __restrict__ before, uint32_t* __restrict__ key_out,
+                                                               uint32_t* __restrict__ position_out) {
+    __shared__ SortCounts counts;
+    __shared__ uint32_t keys[kSortBlock];
+    __shared__ uint16_t ranks[kSortBlock];
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortBlock;
+    const int here = static_cast<int>(min(n - first, static_cast<int64_t>(kSortBlock)));
+    for (int i = threadIdx.x; i < here; i += kSortThreads) keys[i] = key_in ? key_in[first + i] : token_key(tokens[first + i], vocabulary);
+    __syncthreads();
+    rank_digits(keys, kSortRounds, here, shift, counts, ranks);
+    for (int i = threadIdx.x; i < here; i += kSortThreads) {
+        const uint32_t key = keys[i], d = (key >> shift) & (kDigits - 1);
+        const int wave = i / (kWave * kSortRounds);  // the one that ranked it
+        const uint32_t to = before[static_cast<size_t>(d) * gridDim.x + blockIdx.x] + counts.wave[wave][d] + ranks[i];
+        key_out[to] = key;
+        position_out[to] = position_in ? position_in[first + i] : static_cast<uint32_t>(first + i);
+    }
+}
+
+__global__ __launch_bounds__(256) void kept_kernel(const uint32_t* __restrict__ token, int64_t n, uint32_t outside, uint32_t* __restrict__ kept) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+    if (i >= n) return;
+    if (token[i] != outside && (i == n - 1 || token[i + 1] == outside)) *kept = static_cast<uint32_t>(i + 1);
+    if (i == 0 && token[0] == outside) *kept = 0;
+}
+
+// ---- sums ----
+
+constexpr int kSumRows = 16;  // sorted positions of a wave
+
+struct SumArgs {
+    const uint32_t* token;
+    const uint32_t* position;
+    int64_t n, dim, stride, blocks;
+    uint32_t outside;
+    const float* coefficient;
+    float scale;
+    float* part;
+    bool accumulate;
+    float* sums;
+    int32_t* first;
+};
+
+template <typename T, int kWidth>
+__device__ __forceinline__ void finish_sum(const SumArgs& a, T* table, uint32_t token, int64_t index, int64_t column, float (&acc)[kWidth]) {
+#pragma unroll
+    for (int j = 0; j < kWidth; ++j) acc[j] *= a.scale;
+    if (a.sums) {
+        if (column == 0) a.first[token] = static_cast<int32_t>(index);
+        store_from_float<float, kWidth>(a.sums + index * a.dim + column, acc);
+        return;
+    }
+    T* const row = table + static_cast<int64_t>(token) * a.dim + column;
+    if (a.accumulate) {
+        float old[kWidth];
+        load_as_float<T, kWidth>(row, old);
+#pragma unroll
+        for (int j = 0; j < kWidth; ++j) acc[j] += old[j];
+    }
+    store_from_float<T, kWidth>(row, acc);
+}
+
+// part[block][0]: what the block's first token has here, if it began earlier; part[block][1]: what its last one has here, if it
+// begins here and goes on.
+template <typename T, int kWidth>
+__global__ __launch_bounds__(256) void token_sums_kernel(const T* __restrict__ rows, T* __restrict__ table, SumArgs a) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int64_t block = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)));
+    if (block >= a.blocks) return;
+    const int64_t first = block * kSumRows, column = (static_cast<int64_t>(blockIdx.y) * kWave + lane) * kWidth;
+    const int count = static_cast<int>(min(a.n - first, static_cast<int64_t>(kSumRows)));
+    // lane 0: the position before; lanes 1 .. count: the block's; lane count + 1: the one after
+    uint32_t token = a.outside, position = 0;
+    const int64_t at = first + lane - 1;
+    if (lane <= count + 1 && at >= 0 && at < a.n) token = a.token[at], position = a.position[at];
+    float mine = 1.0f;
+    if (a.coefficient && lane >= 1 && lane <= count && token != a.outside) mine = a.coefficient[position];
+    const bool inside = column < a.dim;
+    Pack<T, kWidth> row[kSumRows] = {};
+#pragma unroll
+    for (int i = 0; i < kSumRows; ++i) {
+        const uint32_t t = __builtin_amdgcn_readlane(token, i + 1);
+        const uint32_t p = __builtin_amdgcn_readlane(position, i + 1);
+        if (i < count && t != a.outside && inside)
+            row[i] = *reinterpret_cast<const Pack<T, kWidth>*>(rows + static_cast<int64_t>(p) * a.stride + column);
+    }
+    // (all lanes stay: the tokens are read from lanes whose columns are past the row too)
+    float acc[kWidth] = {};
+    int begin = 0;
+    bool earlier = false;
+#pragma unroll
+    for (int i = 0; i < kSumRows; ++i) {
+        const uint32_t t = __builtin_amdgcn_readlane(token, i + 1), previous = __builtin_amdgcn_readlane(token, i),
+                       next = __builtin_amdgcn_readlane(token, i + 2);
+        if (i >= count || t == a.outside) break;
+        if (i == 0) earlier = previous == t && first > 0;
+        const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), i + 1));
+#pragma unroll
+        for (int j = 0; j < kWidth; ++j) acc[j] = fmaf(c, static_cast<float>(row[i].v[j]), acc[j]);
+        const bool last = i == count - 1, goes_on = next == t;
+        if (!last && goes_on) continue;
+        if (inside) {
+            if (!earlier && !goes_on)
+                finish_sum<T, kWidth>(a, table, t, first + begin, column, acc);
+            else
+                store_from_float<float, kWidth>(a.part + (2 * block + (earlier ? 0 : 1)) * a.dim + column, acc);
+        }
+#pragma unroll
+        for (int j = 0; j < kWidth; ++j) acc[j] = 0.0f;
+        begin = i + 1;
+        earlier = false;
+    }
+}
+
+// Adds the parts of a token whose positions begin in this block and go on.
+template <typename T, int kWidth>
+__global__ __launch_bounds__(256) void token_parts_kernel(T* __restrict__ table, SumArgs a) {
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int64_t block = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)));
+    if (block >= a.blocks - 1) return;  // the last block's tokens end there
+    const int64_t first = block * kSumRows, end = first + kSumRows;
+    const uint32_t t = a.token[end - 1];
+    if (t == a.outside || a.token[end] != t) return;
+    if (a.token[first] == t && first > 0 && a.token[first - 1] == t) return;  // began earlier
+    // the sorted index of its first position
+    const uint64_t same = __ballot(lane < kSumRows && a.token[first + (lane < kSumRows ? lane : 0)] == t);
+    const int64_t index = first + (__ffsll(static_cast<unsigned long long>(same)) - 1);
+    // further blocks that it reaches into
+    int64_t more = 0;
+    for (int64_t b = block + 1;; b += kWave) {
+        const int64_t last = (b + lane + 1) * kSumRows;  // the position after block b + lane
+        const bool goes_on = last < a.n && a.token[last - 1] == t && a.token[last] == t;
+        const uint64_t stops = ~__ballot(goes_on);
+        if (stops) {
+            more += __ffsll(static_cast<unsigned long long>(stops));
+            break;
+        }
+        more += kWave;
+    }
+    const int64_t column = (static_cast<int64_t>(blockIdx.y) * kWave + lane) * kWidth;
+    if (column >= a.dim) return;
+    float acc[kWidth];
+    load_as_float<float, kWidth>(a.part + (2 * block + 1) * a.dim + column, acc);
+    const float* part = a.part + 2 * (block + 1) * a.dim + column;
+    int64_t i = 0;
+    constexpr int kAhead = 8;
+    for (; i + kAhead <= more; i += kAhead) {
+        float v[kAhead][kWidth];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) load_as_float<float, kWidth>(part + 2 * (i + k) * a.dim, v[k]);
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+            for (int j = 0; j < kWidth; ++j) acc[j] += v[k][j];
+    }
+    for (; i < more; ++i) {
+        float v[kWidth];
+        load_as_float<float, kWidth>(part + 2 * i * a.dim, v);
+#pragma unroll
+        for (int j = 0; j < kWidth; ++j) acc[j] += v[j];
+    }
+    finish_sum<T, kWidth>(a, table, t, index, column, acc);
+}
+
+template <typename T, int kWidth>
+int launch_sums(const TokenSums& s, const SumArgs& a, hipStream_t stream) {
+    const dim3 grid(static_cast<unsigned>(ceil_div(a.blocks, 4)), static_cast<unsigned>(ceil_div(a.dim, kWave * kWidth)));
+    token_sums_kernel<T, kWidth><<<grid, 256, 0, stream>>>(static_cast<const T*>(s.rows), static_cast<T*>(s.table), a);
+    if (a.blocks > 1) token_parts_kernel<T, kWidth><<<grid, 256, 0, stream>>>(static_cast<T*>(s.table), a);
+    return check_launch("token_sums");
+}
+
+template <typename T>
+int launch_sums_of(const TokenSums& s, hipStream_t stream) {
+    SumArgs a{};
+    a.token = s.order.token, a.position = s.order.position;
+    a.n = s.n, a.dim = s.dim, a.stride = s.stride;
+    a.blocks = static_cast<int64_t>(ceil_div(s.n, kSumRows));
+    a.outside = static_cast<uint32_t>(s.vocabulary);
+    a.coefficient = s.coefficient, a.scale = s.scale, a.part = s.part;
+    a.accumulate = s.accumulate, a.sums = s.sums, a.first = s.first;
+    constexpr int kWide = kChunk<T>;
+    const bool wide = s.dim % kWide == 0 && s.stride % kWide == 0 && aligned_to(s.rows, 16) && aligned_to(s.table, 16);
+    return wide ? launch_sums<T, kWide>(s, a, stream) : launch_sums<T, 1>(s, a, stream);
+}
+
+}  // namespace
+
+TokenOrderSizes::TokenOrderSizes(int64_t tokens) : n(static_cast<size_t>(tokens)) {
+    const size_t blocks = ceil_div(n, kSortBlock);
+    spare = blocks > 1 ? n : 0;
+    counts = blocks > 1 ? blocks * kDigits : 0;
+}
+
+int fill_words(void* at, size_t bytes, uint32_t word, hipStream_t stream) {
+    const size_t blocks = std::min<size_t>(ceil_div(bytes, 256 * 16), 2048);
+    fill_kernel<<<static_cast<unsigned>(blocks), 256, 0, stream>>>(static_cast<char*>(at), bytes, word);
+    return check_launch("fill_words");
+}
+
+int sort_tokens(const int64_t* tokens, int64_t n, int64_t vocabulary, const TokenOrder& o, void* fill_at, size_t fill_bytes, uint32_t fill,
+                hipStream_t stream) {
+    int bits = 1;
+    while (bits < 32 && vocabulary >> bits) ++bits;
+    const int passes = (bits + kDigitBits - 1) / kDigitBits;
+    char* const to = static_cast<char*>(fill_at);
+    if (n <= kSortBlock) {
+        const size_t fills = std::min<size_t>(ceil_div(fill_bytes, kSortThreads * 16), 255);
+        sort_kernel<<<static_cast<unsigned>(1 + fills), kSortThreads, 0, stream>>>(tokens, static_cast<int>(n), vocabulary, passes, o, to,
+                                                                                    fill_bytes, fill);
+        return check_launch("sort_tokens");
+    }
+    if (fill_bytes) DLLM_TRY(fill_words(fill_at, fill_bytes, fill, stream));
+    const unsigned blocks = static_cast<unsigned>(ceil_div(n, kSortBlock));
+    // the last pass ends in the order's own arrays
+    uint32_t *key_in = nullptr, *position_in = nullptr;
+    for (int pass = 0; pass < passes; ++pass) {
+        const bool own = (passes - 1 - pass) % 2 == 0;
+        uint32_t *const key_out = own ? o.token : o.spare_token, *const position_out = own ? o.position : o.spare_position;
+        const int shift = pass * kDigitBits;
+        digit_counts_kernel<<<blocks, kSortThreads, 0, stream>>>(tokens, key_in, n, vocabulary, shift, o.counts);
+        scan_kernel<<<1, kSortThreads, 0, stream>>>(o.counts, static_cast<int64_t>(blocks) * kDigits);
+        scatter_kernel<<<blocks, kSortThreads, 0, stream>>>(tokens, key_in, position_in, n, vocabulary, shift, o.counts, key_out, position_out);
+        key_in = key_out, position_in = position_out;
+    }
+    kept_kernel<<<static_cast<unsigned>(ceil_div(n, 256)), 256, 0, stream>>>(o.token, n, static_cast<uint32_t>(vocabulary), o.kept);
+    return check_launch("sort_tokens");
+}
+
+size_t token_sums_part_floats(int64_t n, int64_t dim) {
+    const size_t blocks = ceil_div(static_cast<size_t>(n), kSumRows);
+    return blocks > 1 ? 2 * blocks * static_cast<size_t>(dim) : 0;
+}
+
+int launch_token_sums(const TokenSums& a, int64_t dtype, hipStream_t stream) {
+    switch (dtype) {
+        case kFloat32: return launch_sums_of<float>(a, stream);
+        case kBFloat16: return launch_sums_of<__bf16>(a, stream);
+        default: return launch_sums_of<_Float16>(a, stream);
+    }
+}
+
+}  // namespace dllm_hip

@@ -1,0 +1,823 @@
+// The loss over the vocabulary from the last hidden states, and its gradients, without keeping the logits.
+//
+//   x = scale h.w     z = cap tanh(x / cap)     lse = log sum exp z     loss = lse - z[target]
+//   g = (exp(z - lse) - onehot) dloss scale (1 - tanh^2)     dh = g W     dW = g^T h
+//
+// Only rows that count (a target inside the vocabulary) are worked on: they are listed first, and their hidden states gathered
+// into whole 16-byte chunks (float32 as three planes of bfloat16 parts), zeroes behind.
+//
+// Forward: tiles of logits on the matrix cores, vocabulary by rows, so that a lane owns a row of the batch; a tile leaves each
+// row's largest logit and sum of exponentials of 128 of the vocabulary, which a second launch joins in a fixed order, and
+// the target's logit.
+//
+// Backward, a piece of the vocabulary at a time: the logits again, whose epilogue stores the softmax's part of g in the product's
+// type; then its products with the weights and with the hidden states. dh is added up in float32 over units of 8192 of the
+// vocabulary, whatever the batch, so a row's bits are its own. The target's element c = expm1(z - lse) ... stays out of the
+// 16-bit products: p - 1 is what is left of two near numbers where the model is sure, and with a uniform dloss its rounding would
+// not average out. c W[target] is added to dh in float32, and the sums of c h by target (token_rows.h) to dW in the epilogue.
+#include <math.h>
+
+#include <algorithm>
+
+#include "common.h"
+#include "dllm_hip.h"
+#include "element.h"
+#include "softcap.h"
+#include "tile_product.h"
+#include "token_rows.h"
+#include "workspace.h"
+
+using namespace dllm_hip;
+
+namespace {
+
+constexpr int64_t kUnit = 8192;       // of the vocabulary: one addition to dh
+constexpr int64_t kPackPiece = 16384;  // of the vocabulary: weights packed at once, where they are
+constexpr int kStatRows = 128;        // of the vocabulary: one maximum and sum
+constexpr size_t kPieceBytes = size_t{1} << 28;
+constexpr int kHalfShift = 14;  // float16 holds the softmax's part of g times 2^14, relative to the row's weight
+
+struct LossShape {
+    int64_t rows, vocabulary, dim, padded;  // padded: dim in whole chunks
+    int64_t hidden_stride, dhidden_stride;
+    float scale, softcap;
+};
+
+// ---- which rows count ----
+
+// list[0 .. count): the rows whose target is inside, ascending; zeroes for the others.
+__global__ __launch_bounds__(1024) void keep_rows_kernel(const int64_t* __restrict__ targets, int64_t n, int64_t vocabulary,
+                                                         uint32_t* __restrict__ list, uint32_t* __restrict__ count, float* __restrict__ loss,
+                                                         float* __restrict__ lse) {
+    __shared__ uint32_t of_wave[16];
+    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63;
+    uint32_t before = 0;
+    for (int64_t base = 0; base < n; base += 1024) {
+        const int64_t i = base + threadIdx.x;
+        const bool inside = i < n && targets[i] >= 0 && targets[i] < vocabulary;
+        const uint64_t mask = __ballot(inside);
+        if (lane == 0) of_wave[wave] = __popcll(mask);
+        __syncthreads();
+        uint32_t at = before;
+        for (int w = 0; w < 16; ++w) {
+            if (w < wave) at += of_wave[w];
+            before += of_wave[w];
+        }
+        if (inside) list[at + __popcll(mask & ((uint64_t{1} << lane) - 1))] = static_cast<uint32_t>(i);
+        if (i < n && !inside) {
+            if (loss) loss[i] = 0.0f;
+            if (lse) lse[i] = 0.0f;
+        }
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) *count = before;
+}
+
+// ---- packing ----
+
+// Row list[j] (j itself without a list) of src as chunks of 8 parts, in kPlanes<T> planes; zeroes past dim. exponent: row j times
+// 2^(exponent[j] - *largest), as float16 allows.
+struct PackArgs {
+    const uint32_t *list, *count;
+    int64_t n, dim, stride, chunks, plane;
+    const int32_t *exponent, *largest;
+};
+
+template <typename T, bool kWhole>
+__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, Part<T>* __restrict__ dst, PackArgs a) {
+    const int64_t i = block_id() * 256 + threadIdx.x;
+    const int64_t j = i / a.chunks, c = i - j * a.chunks;
+    if (j >= (a.count ? static_cast<int64_t>(*a.count) : a.n)) return;
+    const T* const row = src + (a.list ? static_cast<int64_t>(a.list[j]) : j) * a.stride + c * 8;
+    float v[8];
+    if constexpr (kWhole) {
+#pragma unroll
+        for (int p = 0; p < 8; p += kChunk<T>) {
+            float w[kChunk<T>];
+            load_as_float<T, kChunk<T>>(row + p, w);
+#pragma unroll
+            for (int e = 0; e < kChunk<T>; ++e) v[p + e] = w[e];
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = c * 8 + e < a.dim ? static_cast<float>(row[e]) : 0.0f;
+    }
+    if (a.exponent) {
+        const int by = a.exponent[j] - *a.largest;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], by);
+    }
+    using V = Part<T> __attribute__((ext_vector_type(8)));
+    V out[kPlanes<T>];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        Part<T> parts[kPlanes<T>];
+        split<T>(v[e], parts);
+#pragma unroll
+        for (int p = 0; p < kPlanes<T>; ++p) out[p][e] = parts[p];
+    }
+#pragma unroll
+    for (int p = 0; p < kPlanes<T>; ++p) *reinterpret_cast<V*>(dst + p * a.plane + i * 8) = out[p];
+}
+
+template <typename T>
+int launch_pack(const T* src, Part<T>* dst, const PackArgs& args, hipStream_t stream) {
+    PackArgs a = args;
+    a.chunks = static_cast<int64_t>(ceil_div(a.dim, 8));
+    const bool whole = a.dim % 8 == 0 && a.stride % kChunk<T> == 0 && aligned_to(src, 16);
+    const dim3 grid = grid_of(ceil_div(a.n * a.chunks, 256));
+    if (whole)
+        pack_kernel<T, true><<<grid, 256, 0, stream>>>(src, dst, a);
+    else
+        pack_kernel<T, false><<<grid, 256, 0, stream>>>(src, dst, a);
+    return check_launch("vocabulary_loss packing");
+}
+
+// ---- logits ----
+
+// A logit from its product, and the cap's derivative.
+struct Cap {
+    float scale, softcap, in;
+    __device__ __forceinline__ explicit Cap(const LossShape& s) : scale(s.scale), softcap(s.softcap), in(0.0f) {
+        if (softcap != 0.0f) in = scale / softcap;
+    }
+    template <bool kCapped>
+    __device__ __forceinline__ float logit(float x, float& derivative) const {
+        derivative = 1.0f;
+        if constexpr (!kCapped) return x * scale;
+        return softcap * tanh_of_any_size(x * in, derivative);
+    }
+};
+
+// ---- forward ----
+
+struct Stat {
+    float top, sum;  // sum of exp(z - top); top -infinity: none
+};
+
+__device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
+    const float top = fmaxf(a.top, b.top), base = top == -INFINITY ? 0.0f : top;
+    return {top, a.sum * __builtin_amdgcn_exp2f((a.top - base) * kLog2E) + b.sum * __builtin_amdgcn_exp2f((b.top - base) * kLog2E)};
+}
+
+struct ForwardArgs {
+    LossShape s;
+    Operand weight, hidden;
+    int64_t first;  // of the piece, in the vocabulary; weight.count: of the piece
+    const uint32_t *list, *count;
+    const int64_t* targets;
+    Stat* stats;  // [unit of kStatRows][rows]
+    float* at_target;  // [rows]
+};
+
+template <typename T>
+using ForwardTile = TileProduct<Part<T>, kPlanes<T>, 256, 256, 2, 4, false, false>;
+
+template <typename T, bool kCapped>
+__global__ __launch_bounds__(ForwardTile<T>::kThreads) void forward_kernel(ForwardArgs a, int64_t m_tiles, int64_t n_tiles) {
+    using Tile = ForwardTile<T>;
+    static_assert(Tile::kWaveM == kStatRows);
+    __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+    const int64_t count = *a.count;
+    int64_t m, n;
+    if (block_id() >= m_tiles * n_tiles) return;
+    tile_of(block_id(), m_tiles, n_tiles, m, n);
+    if (n * Tile::kN >= count) return;
+    typename Tile::Sums acc;
+    Tile::run(a.weight, a.hidden, m * Tile::kM, n * Tile::kN, a.weight.count, count, a.s.padded, 0, 0, (LdsByte*)lds, acc);
+    const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
+    if (m0 >= a.weight.count) return;
+    const int64_t unit = (a.first + m0) / kStatRows;
+    const int valid = static_cast<int>(min(a.weight.count - m0, static_cast<int64_t>(kStatRows)));
+    const Cap cap(a.s);
+#pragma unroll
+    for (int j = 0; j < Tile::kBlocksN; ++j) {
+        const int64_t row = n0 + 32 * j + lane_column();
+        const int target = row < count ? static_cast<int>(a.targets[a.list[row]] - a.first - m0) : -1;
+        const bool any = __ballot(target >= 0 && target < kStatRows) != 0;
+        float top = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < Tile::kBlocksM; ++i) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                float unused;
+                acc[i][j][r] = cap.logit<kCapped>(acc[i][j][r], unused);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // one block's values at a time: all of them do not fit the registers
+        }
+        if (valid < kStatRows) {
+#pragma unroll
+            for (int i = 0; i < Tile::kBlocksM; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 32 * i + block_row(r) < valid ? acc[i][j][r] : -INFINITY;
+        }
+        if (any) {
+            float wanted = 0.0f;
+#pragma unroll
+            for (int i = 0; i < Tile::kBlocksM; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) wanted = 32 * i + block_row(r) == target ? acc[i][j][r] : wanted;
+            if (target >= 0 && target < kStatRows && lane_half() == (target >> 2 & 1)) a.at_target[row] = wanted;
+        }
+#pragma unroll
+        for (int i = 0; i < Tile::kBlocksM; ++i)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) top = fmaxf(top, acc[i][j][r]);
+        top = fmaxf(top, other_half(top));
+        const float base = top == -INFINITY ? 0.0f : top;
+        float sum = 0.0f;
+#pragma unroll
+        for (int i = 0; i < Tile::kBlocksM; ++i) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sum += __builtin_amdgcn_exp2f((acc[i][j][r] - base) * kLog2E);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        sum += other_half(sum);
+        if (row < count && lane_half() == 0) a.stats[unit * a.s.rows + row] = {top, sum};
+    }
+}
+
+// Joins a row's statistics: 64 threads take every 64th unit, then the threads' in a fixed tree.
+__global__ __launch_bounds__(256) void join_stats_kernel(const Stat* __restrict__ stats, const float* __restrict__ at_target, int64_t units,
+                                                         int64_t rows, const uint32_t* __restrict__ list, const uint32_t* __restrict__ count,
+                                                         float* __restrict__ loss, float* __restrict__ lse) {
+    __shared__ Stat of[64][4];
+    const int64_t n = *count, first = block_id() * 4;
+    if (first >= n) return;
+    const int part = static_cast<int>(threadIdx.x) >> 2, which = static_cast<int>(threadIdx.x) & 3;
+    const int64_t row = min(first + which, n - 1);
+    Stat s = {-INFINITY, 0.0f};
+    for (int64_t u = part; u < units; u += 64) s = join(s, stats[u * rows + row]);
+    of[part][which] = s;
+    for (int step = 32; step > 0; step >>= 1) {
+        __syncthreads();
+        if (part < step) of[part][which] = s = join(s, of[part + step][which]);
+    }
+    if (part == 0 && first + which < n) {
+        const float l = s.top + kLn2 * __builtin_amdgcn_logf(s.sum);
+        if (lse) lse[list[row]] = l;
+        if (loss) loss[list[row]] = l - at_target[row];
+    }
+}
+
+// ---- backward ----
+
+// What a row's gradient is formed from, by its place in the list.
+struct RowTerms {
+    float *lse, *factor;
+    int32_t* target;
+    int32_t* exponent;  // float16: factor holds the weight's mantissa, this the power of two left out
+};
+
+struct TargetArgs {
+    LossShape s;
+    TokenOrder order;
+    const float *lse, *dloss;
+    RowTerms terms;
+    float* coefficient;  // by row
+    int32_t* largest;    // float16: the largest exponent
+};
+
+// factor = mantissa 2^exponent, mantissa in [1, 2); an exponent no other is below, for zero
+__device__ __forceinline__ void take_apart(float factor, float& mantissa, int& exponent) {
+    int e = 0;
+    mantissa = factor;
+    if (factor != 0.0f && isfinite(factor)) mantissa = 2.0f * frexpf(factor, &e), e -= 1;
+    exponent = factor == 0.0f ? -200 : e;
+}
+
+__global__ __launch_bounds__(1024) void largest_exponent_kernel(TargetArgs a) {
+    __shared__ int of_wave[16];
+    int top = -200;
+    const int64_t n = *a.order.kept;
+    for (int64_t j = threadIdx.x; j < n; j += 1024) {
+        float mantissa;
+        int e;
+        take_apart(a.dloss[a.order.position[j]] * a.s.scale, mantissa, e);
+        top = max(top, e);
+    }
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) top = max(top, __shfl_xor(top, s));
+    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) top = max(top, of_wave[w]);
+        *a.largest = top;
+    }
+}
+
+// The target's element of each row's gradient, a wave to a row: the product in float32.
+template <typename T, bool kCapped>
+__global__ __launch_bounds__(256) void target_kernel(const T* __restrict__ hidden, const T* __restrict__ weight, TargetArgs a) {
+    const int64_t j = block_id() * 4 + (threadIdx.x >> 6);
+    if (j >= static_cast<int64_t>(*a.order.kept)) return;
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const int64_t row = a.order.position[j], target = a.order.token[j];
+    const T *const h = hidden + row * a.s.hidden_stride, *const w = weight + target * a.s.dim;
+    float x = 0.0f;
+    for (int64_t d = lane; d < a.s.dim; d += kWave) x = fmaf(static_cast<float>(h[d]), static_cast<float>(w[d]), x);
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
+    float derivative;
+    const float z = Cap(a.s).logit<kCapped>(x, derivative), lse = a.lse[row], factor = a.dloss[row] * a.s.scale;
+    if (lane != 0) return;
+    a.coefficient[row] = expm1f(z - lse) * derivative * factor;
+    a.terms.lse[j] = lse;
+    a.terms.target[j] = static_cast<int32_t>(target);
+    if constexpr (sizeof(Part<T>) == 2 && __is_same(Part<T>, _Float16)) {
+        float mantissa;
+        int e;
+        take_apart(factor, mantissa, e);
+        a.terms.factor[j] = ldexpf(mantissa, kHalfShift);
+        a.terms.exponent[j] = e;
+    } else {
+        a.terms.factor[j] = factor;
+    }
+}
+
+struct SoftmaxArgs {
+    LossShape s;
+    Operand hidden, weight;
+    int64_t first;  // of the piece, in the vocabulary
+    const uint32_t* count;
+    RowTerms terms;
+    char* out;  // [rows][piece] parts, in planes
+    int64_t out_stride, out_plane;
+};
+
+template <typename T>
+using LogitTile = TileProduct<Part<T>, kPlanes<T>, 256, 256, 2, 4, false, false>;
+
+template <typename T, bool kCapped>
+__global__ __launch_bounds__(LogitTile<T>::kThreads) void softmax_kernel(SoftmaxArgs a, int64_t m_tiles, int64_t n_tiles) {
+    using Tile = LogitTile<T>;
+    __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+    const int64_t count = *a.count;
+    int64_t m, n;
+    if (block_id() >= m_tiles * n_tiles) return;
+    tile_of(block_id(), m_tiles, n_tiles, m, n);
+    if (m * Tile::kM >= count) return;
+    typename Tile::Sums acc;
+    Tile::run(a.hidden, a.weight, m * Tile::kM, n * Tile::kN, count, a.weight.count, a.s.padded, 0, 0, (LdsByte*)lds, acc);
+    const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
+    const Cap cap(a.s);
+#pragma unroll
+    for (int i = 0; i < Tile::kBlocksM; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int64_t row = m0 + 32 * i + 8 * g + 4 * lane_half();  // the arrays are padded to whole tiles
+            const float4 lse = *reinterpret_cast<const float4*>(a.terms.lse + row);
+            const float4 factor = *reinterpret_cast<const float4*>(a.terms.factor + row);
+            const int4 target = *reinterpret_cast<const int4*>(a.terms.target + row);
+            const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, fs[4] = {factor.x, factor.y, factor.z, factor.w};
+            const int ts[4] = {target.x, target.y, target.z, target.w};
+#pragma unroll
+            for (int j = 0; j < Tile::kBlocksN; ++j) {
+                const int64_t column = n0 + 32 * j + lane_column();
+                const bool inside = column < a.weight.count;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float derivative;
+                    const float z = cap.logit<kCapped>(acc[i][j][4 * g + r], derivative);
+                    float p = __builtin_amdgcn_exp2f((z - ls[r]) * kLog2E) * fs[r];
+                    if constexpr (kCapped) p *= derivative;
+                    if (!inside || a.first + column == ts[r]) p = 0.0f;
+                    if (row + r >= count) continue;
+                    Part<T> parts[kPlanes<T>];
+                    split<T>(p, parts);
+#pragma unroll
+                    for (int q = 0; q < kPlanes<T>; ++q)
+                        *reinterpret_cast<Part<T>*>(a.out + q * a.out_plane + (row + r) * a.out_stride + column * 2) = parts[q];
+                }
+            }
+        }
+}
+
+struct HiddenArgs {
+    Operand softmax, weight;  // batch: units
+    const uint32_t* count;
+    int64_t k;  // of the piece
+    float* part;  // [unit][rows][dim]
+    int64_t rows, dim;
+};
+
+template <typename T>
+using HiddenTile = TileProduct<Part<T>, kPlanes<T>, 256, 256, 2, 4, false, true>;
+
+template <typename T>
+__global__ __launch_bounds__(HiddenTile<T>::kThreads) void hidden_kernel(HiddenArgs a, int64_t m_tiles, int64_t n_tiles, int64_t units) {
+    using Tile = HiddenTile<T>;
+    __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+    const int64_t count = *a.count;
+    if (block_id() >= m_tiles * n_tiles * units) return;
+    const int64_t unit = block_id() / (m_tiles * n_tiles);
+    int64_t m, n;
+    tile_of(block_id() - unit * m_tiles * n_tiles, m_tiles, n_tiles, m, n);
+    if (m * Tile::kM >= count) return;
+    typename Tile::Sums acc;
+    Tile::run(a.softmax, a.weight, m * Tile::kM, n * Tile::kN, count, a.dim, min(kUnit, a.k - unit * kUnit), unit, unit, (LdsByte*)lds, acc);
+    const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
+    float* const part = a.part + unit * a.rows * a.dim;
+#pragma unroll
+    for (int i = 0; i < Tile::kBlocksM; ++i)
+#pragma unroll
+        for (int j = 0; j < Tile::kBlocksN; ++j) {
+            const int64_t column = n0 + 32 * j + lane_column();
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int64_t row = m0 + 32 * i + block_row(r);
+                if (row < count && column < a.dim) part[row * a.dim + column] = acc[i][j][r];
+            }
+        }
+}
+
+// total (+)= the units' parts, in their order
+__global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, float* __restrict__ total, const uint32_t* __restrict__ count,
+                                                        int64_t rows, int64_t dim, int units, bool first) {
+    const int64_t n = static_cast<int64_t>(*count) * dim;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
+        float v = first ? part[i] : total[i] + part[i];
+        for (int u = 1; u < units; ++u) v += part[u * rows * dim + i];
+        total[i] = v;
+    }
+}
+
+struct FinishArgs {
+    LossShape s;
+    TokenOrder order;
+    RowTerms terms;
+    const float *total, *coefficient;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void finish_hidden_kernel(const T* __restrict__ weight, T* __restrict__ dhidden, FinishArgs a) {
+    const int64_t j = block_id();
+    if (j >= a.s.rows) return;
+    const int64_t row = a.order.position[j];
+    T* const out = dhidden + row * a.s.dhidden_stride;
+    if (j >= static_cast<int64_t>(*a.order.kept)) {
+        for (int64_t d = threadIdx.x; d < a.s.dim; d += 256) out[d] = static_cast<T>(0.0f);
+        return;
+    }
+    const T* const w = weight + static_cast<int64_t>(a.order.token[j]) * a.s.dim;
+    const float c = a.coefficient[row];
+    const int by = __is_same(T, _Float16) ? a.terms.exponent[j] - kHalfShift : 0;
+    for (int64_t d = threadIdx.x; d < a.s.dim; d += 256) {
+        float v = a.total[j * a.s.dim + d];
+        if constexpr (__is_same(T, _Float16)) v = ldexpf(v, by);
+        out[d] = static_cast<T>(fmaf(c, static_cast<float>(w[d]), v));
+    }
+}
+
+struct WeightArgs {
+    Operand softmax, hidden;
+    const uint32_t* count;
+    int64_t first, rows, dim;  // rows: of the piece
+    const float* sums;         // the targets' part, by the index in `at`
+    const int32_t* at;         // by token, -1: none
+    const int32_t* largest;    // float16: the power of two left out
+    bool accumulate;
+};
+
+template <typename T>
+using WeightTile = TileProduct<Part<T>, kPlanes<T>, 256, 256, 2, 4, true, true>;
+
+template <typename T>
+__global__ __launch_bounds__(WeightTile<T>::kThreads) void weight_kernel(T* __restrict__ dweight, WeightArgs a, int64_t m_tiles, int64_t n_tiles) {
+    using Tile = WeightTile<T>;
+    __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+    int64_t m, n;
+    if (block_id() >= m_tiles * n_tiles) return;
+    tile_of(block_id(), m_tiles, n_tiles, m, n);
+    typename Tile::Sums acc;
+    Tile::run(a.softmax, a.hidden, m * Tile::kM, n * Tile::kN, a.rows, a.dim, *a.count, 0, 0, (LdsByte*)lds, acc);
+    const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
+    const int by = __is_same(T, _Float16) ? *a.largest - kHalfShift : 0;
+#pragma unroll
+    for (int i = 0; i < Tile::kBlocksM; ++i)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const int64_t row = m0 + 32 * i + block_row(r);
+            if (row >= a.rows) continue;
+            const int64_t at = a.at[a.first + row];
+#pragma unroll
+            for (int j = 0; j < Tile::kBlocksN; ++j) {
+                const int64_t column = n0 + 32 * j + lane_column();
+                if (column >= a.dim) continue;
+                float v = acc[i][j][r];
+                if constexpr (__is_same(T, _Float16)) v = ldexpf(v, by);
+                if (at >= 0) v += a.sums[at * a.dim + column];
+                T* const out = dweight + (a.first + row) * a.dim + column;
+                if (a.accumulate) v += static_cast<float>(*out);
+                *out = static_cast<T>(v);
+            }
+        }
+}
+
+// ---- workspaces ----
+
+int check_shape(const dllm_hip_vocabulary_loss_shape* sh) {
+    DLLM_REQUIRE(sh != nullptr, "null shape");
+    DLLM_REQUIRE(sh->dtype >= 0 && sh->dtype <= 2, "dtype must be float32 (0), bfloat16 (1) or float16 (2)");
+    DLLM_REQUIRE(sh->rows >= 0 && sh->rows < kMaxSortTokens, "rows must be in [0, 2^27)");
+    DLLM_REQUIRE(sh->vocabulary >= 1 && sh->vocabulary < (int64_t{1} << 31), "vocabulary must be in [1, 2^31)");
+    DLLM_REQUIRE(sh->dim >= 1 && sh->dim <= (1 << 16), "dim must be in [1, 2^16]");
+    DLLM_REQUIRE(sh->rows * sh->vocabulary < (int64_t{1} << 48), "rows * vocabulary must be below 2^48");
+    // in float32 the scale, the cap and their quotient are then ordinary numbers
+    DLLM_REQUIRE(sh->softcap == 0.0 || (sh->softcap >= 0x1p-64 && sh->softcap <= 0x1p64), "softcap must be 0 or in [2^-64, 2^64]");
+    DLLM_REQUIRE(sh->scale >= 0x1p-60 && sh->scale <= 0x1p60, "scale must be in [2^-60, 2^60]");
+    for (const int64_t s : {sh->hidden_stride, sh->dhidden_stride}) DLLM_REQUIRE(s == 0 || s >= sh->dim, "a row stride must be 0 or at least dim");
+    return kOk;
+}
+
+LossShape loss_shape(const dllm_hip_vocabulary_loss_shape& sh) {
+    LossShape s;
+    s.rows = sh.rows, s.vocabulary = sh.vocabulary, s.dim = sh.dim;
+    s.padded = static_cast<int64_t>(round_up(sh.dim, 8));
+    s.hidden_stride = sh.hidden_stride ? sh.hidden_stride : sh.dim;
+    s.dhidden_stride = sh.dhidden_stride ? sh.dhidden_stride : sh.dim;
+    s.scale = static_cast<float>(sh.scale), s.softcap = static_cast<float>(sh.softcap);
+    return s;
+}
+
+int planes_of(int64_t dtype) { return dtype == kFloat32 ? 3 : 1; }
+
+// Units of the backward's piece: as many as keep its softmax within kPieceBytes, at least one.
+int64_t piece_units(const LossShape& s, int64_t dtype) {
+    const size_t unit = static_cast<size_t>(s.rows) * kUnit * 2 * planes_of(dtype);
+    const int64_t all = static_cast<int64_t>(ceil_div(s.vocabulary, kUnit));
+    return std::clamp<int64_t>(static_cast<int64_t>(kPieceBytes / std::max<size_t>(unit, 1)), 1, all);
+}
+
+struct LossLayout {
+    size_t hidden, scaled, weight, list, stats, at_target;                  // forward
+    size_t terms, softmax, part, total, sums, sum_parts, at, coefficient;   // backward
+    int64_t units;
+    size_t bytes;
+    LossLayout(const LossShape& s, int64_t dtype, bool backward) {
+        const size_t rows = static_cast<size_t>(s.rows), planes = planes_of(dtype), dim = static_cast<size_t>(s.dim);
+        units = piece_units(s, dtype);
+        const size_t piece = backward ? std::min<size_t>(units * kUnit, s.vocabulary) : std::min<size_t>(kPackPiece, s.vocabulary);
+        hidden = rows * s.padded * planes;
+        scaled = backward && dtype == kFloat16 ? hidden : 0;
+        weight = piece * s.padded * planes;
+        list = backward ? 0 : rows;
+        stats = backward ? 0 : ceil_div(s.vocabulary, kStatRows) * rows;
+        at_target = backward ? 0 : rows;
+        terms = backward ? round_up(rows, 256) : 0;
+        softmax = backward ? rows * units * kUnit * planes : 0;
+        part = backward ? units * rows * dim : 0;
+        total = backward ? rows * dim : 0;
+        sums = total;
+        sum_parts = backward ? token_sums_part_floats(s.rows, s.dim) : 0;
+        at = backward ? s.vocabulary : 0;
+        coefficient = backward ? rows : 0;
+        Layout l;
+        l.add<uint16_t>(hidden);
+        l.add<uint16_t>(scaled);
+        l.add<uint16_t>(weight);
+        l.add<uint32_t>(list);
+        l.add<uint32_t>(1);
+        l.add<Stat>(stats);
+        l.add<float>(at_target);
+        if (backward) {
+            add_token_order(l, s.rows);
+            for (int i = 0; i < 4; ++i) l.add<float>(terms);
+            l.add<uint16_t>(softmax);
+            for (const size_t n : {part, total, sums, sum_parts, at, coefficient, size_t{1}}) l.add<float>(n);
+        }
+        bytes = l.bytes;
+    }
+};
+
+template <typename T>
+struct Buffers {
+    Part<T>*hidden, *scaled, *weight;
+    uint32_t *list, *count;
+    Stat* stats;
+    float* at_target;
+    TokenOrder order;
+    RowTerms terms;
+    char* softmax;
+    float *part, *total, *sums, *sum_parts;
+    int32_t* at;
+    float* coefficient;
+    int32_t* largest;
+    Buffers(const LossLayout& l, const LossShape& s, bool backward, void* workspace, size_t bytes) {
+        Carve c(workspace, bytes);
+        hidden = c.take<Part<T>>(l.hidden);
+        scaled = c.take<Part<T>>(l.scaled);
+        weight = c.take<Part<T>>(l.weight);
+        list = c.take<uint32_t>(l.list);
+        count = c.take<uint32_t>(1);
+        stats = c.take<Stat>(l.stats);
+        at_target = c.take<float>(l.at_target);
+        if (!backward) return;
+        order = take_token_order(c, s.rows);
+        terms.lse = c.take<float>(l.terms);
+        terms.factor = c.take<float>(l.terms);
+        terms.target = c.take<int32_t>(l.terms);
+        terms.exponent = c.take<int32_t>(l.terms);
+        softmax = reinterpret_cast<char*>(c.take<uint16_t>(l.softmax));
+        part = c.take<float>(l.part);
+        total = c.take<float>(l.total);
+        sums = c.take<float>(l.sums);
+        sum_parts = c.take<float>(l.sum_parts);
+        at = c.take<int32_t>(l.at);
+        coefficient = c.take<float>(l.coefficient);
+        largest = c.take<int32_t>(1);
+    }
+};
+
+// The weights of a piece as an operand: where they are, or packed.
+template <typename T>
+int weight_operand(const LossShape& s, const T* weight, Part<T>* packed, int64_t first, int64_t n, Operand& op, hipStream_t stream) {
+    const bool direct = sizeof(T) == 2 && s.dim % 8 == 0 && aligned_to(weight, 16);
+    op.count = n;
+    op.batch = 0;
+    op.stride = s.padded * 2;
+    op.plane = n * s.padded * 2;
+    if (direct) {
+        op.base = reinterpret_cast<const char*>(weight + first * s.dim);
+        return kOk;
+    }
+    op.base = reinterpret_cast<const char*>(packed);
+    PackArgs p{};
+    p.n = n, p.dim = s.dim, p.stride = s.dim, p.plane = n * s.padded;
+    return launch_pack<T>(weight + first * s.dim, packed, p, stream);
+}
+
+template <typename T>
+Operand hidden_operand(const LossShape& s, const Part<T>* packed) {
+    return {reinterpret_cast<const char*>(packed), s.padded * 2, s.rows * s.padded * 2, 0, s.rows};
+}
+
+template <typename T>
+int run_forward(const LossShape& s, int64_t dtype, const T* hidden, const T* weight, const int64_t* targets, float* loss, float* lse,
+                void* workspace, size_t bytes, hipStream_t stream) {
+    const LossLayout layout(s, dtype, false);
+    const Buffers<T> b(layout, s, false, workspace, bytes);
+    keep_rows_kernel<<<1, 1024, 0, stream>>>(targets, s.rows, s.vocabulary, b.list, b.count, loss, lse);
+    PackArgs p{};
+    p.list = b.list, p.count = b.count, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride, p.plane = s.rows * s.padded;
+    DLLM_TRY(launch_pack<T>(hidden, b.hidden, p, stream));
+    const bool direct = sizeof(T) == 2 && s.dim % 8 == 0 && aligned_to(weight, 16);
+    const int64_t piece = direct ? s.vocabulary : kPackPiece;
+    for (int64_t first = 0; first < s.vocabulary; first += piece) {
+        ForwardArgs a{};
+        a.s = s, a.hidden = hidden_operand<T>(s, b.hidden);
+        DLLM_TRY(weight_operand<T>(s, weight, b.weight, first, std::min(piece, s.vocabulary - first), a.weight, stream));
+        a.first = first, a.list = b.list, a.count = b.count, a.targets = targets, a.stats = b.stats, a.at_target = b.at_target;
+        using Tile = ForwardTile<T>;
+        const int64_t m = ceil_div(a.weight.count, Tile::kM), n = ceil_div(s.rows, Tile::kN);
+        const dim3 grid = grid_of(m * n);
+        if (s.softcap != 0.0f)
+            forward_kernel<T, true><<<grid, Tile::kThreads, 0, stream>>>(a, m, n);
+        else
+            forward_kernel<T, false><<<grid, Tile::kThreads, 0, stream>>>(a, m, n);
+    }
+    join_stats_kernel<<<grid_of(ceil_div(s.rows, 4)), 256, 0, stream>>>(
+        b.stats, b.at_target, static_cast<int64_t>(ceil_div(s.vocabulary, kStatRows)), s.rows, b.list, b.count, loss, lse);
+    return check_launch("vocabulary_loss");
+}
+
+template <typename T>
+int run_backward(const LossShape& s, int64_t dtype, const T* hidden, const T* weight, const int64_t* targets, const float* lse,
+                 const float* dloss, T* dhidden, T* dweight, bool accumulate, void* workspace, size_t bytes, hipStream_t stream) {
+    constexpr bool kHalf = __is_same(T, _Float16);
+    const LossLayout layout(s, dtype, true);
+    const Buffers<T> b(layout, s, true, workspace, bytes);
+    // at: -1 everywhere, until the sums say where they are
+    DLLM_TRY(sort_tokens(targets, s.rows, s.vocabulary, b.order, b.at, dweight ? layout.at * 4 : 0, ~uint32_t{0}, stream));
+    TargetArgs t{};
+    t.s = s, t.order = b.order, t.lse = lse, t.dloss = dloss, t.terms = b.terms, t.coefficient = b.coefficient, t.largest = b.largest;
+    if (kHalf) largest_exponent_kernel<<<1, 1024, 0, stream>>>(t);
+    const dim3 by_rows = grid_of(ceil_div(s.rows, 4));
+    if (s.softcap != 0.0f)
+        target_kernel<T, true><<<by_rows, 256, 0, stream>>>(hidden, weight, t);
+    else
+        target_kernel<T, false><<<by_rows, 256, 0, stream>>>(hidden, weight, t);
+    PackArgs p{};
+    p.list = b.order.position, p.count = b.order.kept, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride, p.plane = s.rows * s.padded;
+    DLLM_TRY(launch_pack<T>(hidden, b.hidden, p, stream));
+    if (kHalf && dweight) {
+        p.exponent = b.terms.exponent, p.largest = b.largest;
+        DLLM_TRY(launch_pack<T>(hidden, b.scaled, p, stream));
+    }
+    if (dweight) {
+        TokenSums sums{};
+        sums.order = b.order, sums.n = s.rows, sums.vocabulary = s.vocabulary, sums.dim = s.dim, sums.stride = s.hidden_stride;
+        sums.rows = hidden, sums.coefficient = b.coefficient, sums.scale = 1.0f, sums.part = b.sum_parts, sums.sums = b.sums, sums.first = b.at;
+        DLLM_TRY(launch_token_sums(sums, dtype, stream));
+    }
+    const int64_t piece = layout.units * kUnit;
+    for (int64_t first = 0; first < s.vocabulary; first += piece) {
+        SoftmaxArgs a{};
+        a.s = s, a.hidden = hidden_operand<T>(s, b.hidden);
+        DLLM_TRY(weight_operand<T>(s, weight, b.weight, first, std::min(piece, s.vocabulary - first), a.weight, stream));
+        a.first = first, a.count = b.order.kept, a.terms = b.terms, a.out = b.softmax;
+        a.out_stride = piece * 2, a.out_plane = s.rows * a.out_stride;
+        const int64_t width = a.weight.count;
+        {
+            using Tile = LogitTile<T>;
+            const int64_t m = ceil_div(s.rows, Tile::kM), n = ceil_div(width, Tile::kN);
+            const dim3 grid = grid_of(m * n);
+            if (s.softcap != 0.0f)
+                softmax_kernel<T, true><<<grid, Tile::kThreads, 0, stream>>>(a, m, n);
+            else
+                softmax_kernel<T, false><<<grid, Tile::kThreads, 0, stream>>>(a, m, n);
+        }
+        const Operand softmax{b.softmax, a.out_stride, a.out_plane, kUnit * 2, s.rows};
+        if (dhidden) {
+            using Tile = HiddenTile<T>;
+            HiddenArgs h{};
+            h.softmax = softmax, h.weight = a.weight, h.weight.batch = kUnit * a.weight.stride;
+            h.count = b.order.kept, h.k = width, h.part = b.part, h.rows = s.rows, h.dim = s.dim;
+            const int64_t m = ceil_div(s.rows, Tile::kM), n = ceil_div(s.dim, Tile::kN), units = ceil_div(width, kUnit);
+            hidden_kernel<T><<<grid_of(m * n * units), Tile::kThreads, 0, stream>>>(h, m, n, units);
+            add_parts_kernel<<<static_cast<unsigned>(std::min<size_t>(ceil_div(s.rows * s.dim, 256), 4096)), 256, 0, stream>>>(
+                b.part, b.total, b.order.kept, s.rows, s.dim, static_cast<int>(units), first == 0);
+        }
+        if (dweight) {
+            using Tile = WeightTile<T>;
+            WeightArgs w{};
+            w.softmax = softmax, w.hidden = hidden_operand<T>(s, kHalf ? b.scaled : b.hidden);
+            w.count = b.order.kept, w.first = first, w.rows = width, w.dim = s.dim, w.sums = b.sums, w.at = b.at, w.largest = b.largest;
+            w.accumulate = accumulate;
+            const int64_t m = ceil_div(width, Tile::kM), n = ceil_div(s.dim, Tile::kN);
+            weight_kernel<T><<<grid_of(m * n), Tile::kThreads, 0, stream>>>(dweight, w, m, n);
+        }
+    }
+    if (dhidden) {
+        FinishArgs f{s, b.order, b.terms, b.total, b.coefficient};
+        finish_hidden_kernel<T><<<grid_of(s.rows), 256, 0, stream>>>(weight, dhidden, f);
+    }
+    return check_launch("vocabulary_loss_backward");
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t dllm_hip_vocabulary_loss_workspace(const dllm_hip_vocabulary_loss_shape* sh) {
+    return check_shape(sh) == kOk ? LossLayout(loss_shape(*sh), sh->dtype, false).bytes : 0;
+}
+
+int dllm_hip_vocabulary_loss(const dllm_hip_vocabulary_loss_shape* sh, const void* hidden, const void* weight, const int64_t* targets,
+                             float* loss, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
+    DLLM_TRY(check_shape(sh));
+    if (sh->rows == 0 || (!loss && !lse)) return kOk;
+    DLLM_REQUIRE(hidden && weight && targets, "null hidden, weight or targets");
+    const size_t size = element_bytes(sh->dtype);
+    DLLM_REQUIRE(aligned_to(hidden, size) && aligned_to(weight, size) && aligned_to(targets, 8) && aligned_to(loss, 4) && aligned_to(lse, 4),
+                 "pointers must be aligned to the element");
+    const LossShape s = loss_shape(*sh);
+    DLLM_REQUIRE(workspace && workspace_bytes >= LossLayout(s, sh->dtype, false).bytes, "workspace too small for vocabulary_loss");
+    DLLM_REQUIRE(aligned_to(workspace, 16), "the workspace must be aligned to 16 bytes");
+    const auto run = [&](auto type) {
+        using T = decltype(type);
+        return run_forward<T>(s, sh->dtype, static_cast<const T*>(hidden), static_cast<const T*>(weight), targets, loss, lse, workspace,
+                              workspace_bytes, static_cast<hipStream_t>(stream));
+    };
+    switch (sh->dtype) {
+        case kFloat32: return run(float{});
+        case kBFloat16: return run(__bf16{});
+        default: return run(_Float16{});
+    }
+}
+
+size_t dllm_hip_vocabulary_loss_backward_workspace(const dllm_hip_vocabulary_loss_shape* sh) {
+    return check_shape(sh) == kOk ? LossLayout(loss_shape(*sh), sh->dtype, true).bytes : 0;
+}
+
+int dllm_hip_vocabulary_loss_backward(const dllm_hip_vocabulary_loss_shape* sh, const void* hidden, const void* weight,
+                                      const int64_t* targets, const float* lse, const float* dloss, void* dhidden, void* dweight,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+    DLLM_TRY(check_shape(sh));
+    const size_t size = element_bytes(sh->dtype);
+    DLLM_REQUIRE(aligned_to(dhidden, size) && aligned_to(dweight, size), "pointers must be aligned to the element");
+    if (!dhidden && !dweight) return kOk;
+    if (sh->rows == 0) {
+        const size_t table = static_cast<size_t>(sh->vocabulary) * sh->dim * size;
+        return dweight && !sh->accumulate ? fill_words(dweight, table, 0, static_cast<hipStream_t>(stream)) : static_cast<int>(kOk);
+    }
+    DLLM_REQUIRE(hidden && weight && targets && lse && dloss, "null hidden, weight, targets, lse or dloss");
+    DLLM_REQUIRE(aligned_to(hidden, size) && aligned_to(weight, size) && aligned_to(targets, 8) && aligned_to(lse, 4) && aligned_to(dloss, 4),
+                 "pointers must be aligned to the element");
+    const LossShape s = loss_shape(*sh);
+    DLLM_REQUIRE(workspace && workspace_bytes >= LossLayout(s, sh->dtype, true).bytes, "workspace too small for vocabulary_loss_backward");
+    DLLM_REQUIRE(aligned_to(workspace, 16), "the workspace must be aligned to 16 bytes");
+    const auto run = [&](auto type) {
+        using T = decltype(type);
+        return run_backward<T>(s, sh->dtype, static_cast<const T*>(hidden), static_cast<const T*>(weight), targets, lse, dloss,
+                               static_cast<T*>(dhidden), static_cast<T*>(dweight), sh->accumulate != 0, workspace, workspace_bytes,
+                               static_cast<hipStream_t>(stream));
+    };
+    switch (sh->dtype) {
+        case kFloat32: return run(float{});
+        case kBFloat16: return run(__bf16{});
+        default: return run(_Float16{});
+    }
+}
+
+}  // extern "C"

@@ -52,6 +52,29 @@ class ResidualNorm(C.Structure):
     _fields_ += [("eps", C.c_double), ("residual_scale", C.c_double)]
 
 
+class TokenEmbedding(C.Structure):
+    """dllm_hip_token_embedding_shape; stride in elements, 0 for packed rows."""
+
+    _fields_ = [(n, C.c_int64) for n in ("dtype", "tokens", "vocabulary", "dim", "accumulate")]
+    _fields_ += [("scale", C.c_double), ("stride", C.c_int64)]
+
+
+class VocabularyLoss(C.Structure):
+    """dllm_hip_vocabulary_loss_shape; strides in elements, 0 for packed rows."""
+
+    _fields_ = [(n, C.c_int64) for n in ("dtype", "rows", "vocabulary", "dim", "accumulate")]
+    _fields_ += [(n, C.c_double) for n in ("scale", "softcap")]
+    _fields_ += [(n, C.c_int64) for n in ("hidden_stride", "dhidden_stride")]
+
+
+class Orthogonalize(C.Structure):
+    """dllm_hip_orthogonalize_shape; strides in elements, 0 for packed rows and matrices."""
+
+    _fields_ = [(n, C.c_int64) for n in ("dtype", "batch", "rows", "cols", "steps")]
+    _fields_ += [(n, C.c_double) for n in ("eps", "scale")]
+    _fields_ += [(n, C.c_int64) for n in ("x_stride", "x_batch_stride", "out_stride", "out_batch_stride")]
+
+
 def _load() -> C.CDLL:
     if not LIBRARY.exists():
         raise ImportError(f"{LIBRARY} is not built; run etalii_dllm_amd/build.py (hipcc, gfx950)")
@@ -129,6 +152,16 @@ def _load() -> C.CDLL:
     lib.dllm_hip_rope_axes.argtypes = [rope] + [_vp] * 8
     lib.dllm_hip_residual_norm.argtypes = [norm] + [_vp] * 8
     lib.dllm_hip_residual_norm_backward.argtypes = [norm] + [_vp] * 13 + [_sz, _vp]
+    embedding, loss, update = (C.POINTER(t) for t in (TokenEmbedding, VocabularyLoss, Orthogonalize))
+    for name, shape in (("token_embedding_backward", embedding), ("vocabulary_loss", loss),
+                        ("vocabulary_loss_backward", loss), ("orthogonalize", update)):
+        query = getattr(lib, f"dllm_hip_{name}_workspace")
+        query.restype, query.argtypes = _sz, [shape]
+    lib.dllm_hip_token_embedding.argtypes = [embedding] + [_vp] * 4
+    lib.dllm_hip_token_embedding_backward.argtypes = [embedding] + [_vp] * 4 + [_sz, _vp]
+    lib.dllm_hip_vocabulary_loss.argtypes = [loss] + [_vp] * 6 + [_sz, _vp]
+    lib.dllm_hip_vocabulary_loss_backward.argtypes = [loss] + [_vp] * 8 + [_sz, _vp]
+    lib.dllm_hip_orthogonalize.argtypes = [update, _f64p] + [_vp] * 3 + [_sz, _vp]
     return lib
 
 
@@ -1006,3 +1039,107 @@ def residual_norm_backward(h, y, dh, dn=None, gate=None, post_weight=None, pre_w
     got = (dgate and dgate.download(np.shape(gate), np.asarray(gate).dtype), dpost and dpost.download((h.shape[-1],)),
            dpre and dpre.download((h.shape[-1],)))
     return dx.download(h.shape, h.dtype), dy.download(h.shape, h.dtype), *got
+
+
+# ---- the ends of a packed step, and its update (no counterpart in cpp/kernels.cpp) ----
+
+
+def _token_ids(tokens, vocabulary: int, name: str) -> np.ndarray:
+    ids = np.ascontiguousarray(tokens, dtype=np.int64)
+    if ids.ndim != 1:
+        raise ValueError(f"{name} must have one dimension")
+    if ids.size and ids.max() >= vocabulary:
+        raise ValueError(f"{name} must be below the vocabulary's size (negative ones count for nothing)")
+    return ids
+
+
+def token_embedding(table, tokens, scale=1.0) -> np.ndarray:
+    """scale * table[tokens]; rows of zeroes for negative tokens (padding)."""
+    table = np.asarray(table)
+    dtype = _activation_type(table)
+    if table.ndim != 2:
+        raise ValueError("table must be [vocabulary, dim]")
+    ids = _token_ids(tokens, table.shape[0], "tokens")
+    shape = TokenEmbedding(dtype, len(ids), *table.shape, 0, float(scale))
+    dt, di, out = Device.of(table), Device.of(ids), Device(len(ids) * table.shape[1] * table.itemsize)
+    check(lib.dllm_hip_token_embedding(shape, dt.ptr, di.ptr, out.ptr, None))
+    return out.download((len(ids), table.shape[1]), table.dtype)
+
+
+def token_embedding_backward(tokens, dout, vocabulary_size, scale=1.0, dtable=None) -> np.ndarray:
+    """The table's gradient from dout [tokens, dim]; added to dtable where that is given (a new array either way)."""
+    dout = np.asarray(dout)
+    dtype = _activation_type(dout, dtable)
+    ids = _token_ids(tokens, vocabulary_size, "tokens")
+    if dout.ndim != 2 or dout.shape[0] != len(ids):
+        raise ValueError("dout must be [tokens, dim]")
+    size = (int(vocabulary_size), dout.shape[1])
+    if dtable is not None and np.shape(dtable) != size:
+        raise ValueError("dtable must be [vocabulary, dim]")
+    shape = TokenEmbedding(dtype, len(ids), *size, int(dtable is not None), float(scale))
+    di, dd = Device.of(ids), Device.of(dout)
+    out = Device(size[0] * size[1] * dout.itemsize) if dtable is None else Device.of(np.asarray(dtable))
+    ws = Device(lib.dllm_hip_token_embedding_backward_workspace(shape))
+    check(lib.dllm_hip_token_embedding_backward(shape, di.ptr, dd.ptr, out.ptr, ws.ptr, ws.nbytes, None))
+    return out.download(size, dout.dtype)
+
+
+def _loss_shape(hidden, weight, targets, scale, softcap, accumulate):
+    hidden, weight = np.asarray(hidden), np.asarray(weight)
+    dtype = _activation_type(hidden, weight)
+    if hidden.ndim != 2 or weight.ndim != 2 or hidden.shape[1] != weight.shape[1]:
+        raise ValueError("hidden must be [rows, dim] and weight [vocabulary, dim]")
+    ids = _token_ids(targets, weight.shape[0], "targets")
+    if len(ids) != hidden.shape[0]:
+        raise ValueError("targets must have one entry per row")
+    if not scale > 0 or softcap < 0:
+        raise ValueError("scale must be positive and softcap not negative")
+    return hidden, weight, ids, VocabularyLoss(dtype, len(ids), *weight.shape, int(accumulate), float(scale), float(softcap))
+
+
+def vocabulary_loss(hidden, weight, targets, scale=1.0, softcap=0.0):
+    """(loss, lse), float32 [rows], of the logits softcap * tanh(scale * hidden @ weight.T / softcap), which are not kept; zero
+    for rows with a negative target."""
+    hidden, weight, ids, shape = _loss_shape(hidden, weight, targets, scale, softcap, False)
+    ins = [Device.of(x) for x in (hidden, weight, ids)]
+    loss, lse = Device(4 * len(ids)), Device(4 * len(ids))
+    ws = Device(lib.dllm_hip_vocabulary_loss_workspace(shape))
+    check(lib.dllm_hip_vocabulary_loss(shape, *(d.ptr for d in ins), loss.ptr, lse.ptr, ws.ptr, ws.nbytes, None))
+    return loss.download((len(ids),)), lse.download((len(ids),))
+
+
+def vocabulary_loss_backward(hidden, weight, targets, lse, dloss, scale=1.0, softcap=0.0, dweight=None):
+    """(dhidden, dweight) of vocabulary_loss from its lse and the upstream dloss [rows]; dweight is added to where it is
+    given (a new array either way)."""
+    hidden, weight, ids, shape = _loss_shape(hidden, weight, targets, scale, softcap, dweight is not None)
+    _activation_type(hidden, dweight)
+    if np.shape(lse) != ids.shape or np.shape(dloss) != ids.shape:
+        raise ValueError("lse and dloss must have one entry per row")
+    if dweight is not None and np.shape(dweight) != weight.shape:
+        raise ValueError("dweight must have the shape of weight")
+    ins = [Device.of(x) for x in (hidden, weight, ids, _f32(lse), _f32(dloss))]
+    dh, dw = Device(hidden.nbytes), Device(weight.nbytes) if dweight is None else Device.of(np.asarray(dweight))
+    ws = Device(lib.dllm_hip_vocabulary_loss_backward_workspace(shape))
+    check(lib.dllm_hip_vocabulary_loss_backward(shape, *(d.ptr for d in ins), dh.ptr, dw.ptr, ws.ptr, ws.nbytes, None))
+    return dh.download(hidden.shape, hidden.dtype), dw.download(weight.shape, weight.dtype)
+
+
+def orthogonalize(x, steps=5, coefficients=None, eps=1e-7, scale=1.0) -> np.ndarray:
+    """scale times the orthogonalised matrices x [rows, cols] or [batch, rows, cols]: Newton-Schulz steps with coefficients
+    [steps, 3] (a, b, c; None: 3.4445, -4.7750, 2.0315 in all of them)."""
+    x = np.asarray(x)
+    dtype = _activation_type(x)
+    if x.ndim not in (2, 3) or x.shape[-1] == 0 or x.shape[-2] == 0:
+        raise ValueError("x must be [rows, cols] or [batch, rows, cols]")
+    host = None
+    if coefficients is not None:
+        host = np.ascontiguousarray(coefficients, dtype=np.float64)
+        if host.shape != (steps, 3):
+            raise ValueError("coefficients must be [steps, 3]")
+    shape = Orthogonalize(dtype, x.shape[0] if x.ndim == 3 else 1, x.shape[-2], x.shape[-1], int(steps), float(eps),
+                          float(scale))
+    dx, out = Device.of(x), Device(x.nbytes)
+    ws = Device(lib.dllm_hip_orthogonalize_workspace(shape))
+    check(lib.dllm_hip_orthogonalize(shape, None if host is None else host.ctypes.data_as(_f64p), dx.ptr, out.ptr, ws.ptr,
+                                     ws.nbytes, None))
+    return out.download(x.shape, x.dtype)

@@ -355,6 +355,83 @@ int dllm_hip_residual_norm_backward(const dllm_hip_residual_norm_shape* shape, c
                                     float* dpost_weight, float* dpre_weight, void* workspace, size_t workspace_bytes,
                                     void* stream);
 
+/* ---- the ends of a packed step, and its update ----
+ *
+ * What lies before the first packed layer and behind the last one, and an update for the matrices between. They keep the
+ * packed layers' contract: dtype is the type of activations, tables and their gradients, sums are float32 or wider, each
+ * result is rounded to its type once, no atomic additions, calls allocate nothing and can be captured into a graph, two
+ * calls that may run at once need a workspace each, and the stream's device must be the current one. */
+
+/* Embedding lookup: out[t] = scale * table[tokens[t]], table[vocabulary, dim], tokens[tokens] (int64, device). A token outside the
+ * vocabulary (padding) gives a row of zeroes. stride: elements between the rows of out, and of dout (0: dim).
+ * The backward: dtable[v] = scale * sum of dout[t] over the t with token v, added in order of t in float32; all other rows are
+ * zero. With accumulate the sum is added to what dtable holds, in float32 before the one rounding (the table of a model
+ * whose embeddings are tied gathers its gradient from both ends), and rows of tokens that do not occur stay as they are.
+ * Tokens outside the vocabulary count for nothing. out or dtable do not overlap inputs.
+ * Limits: tokens below 2^27, vocabulary below 2^31, dim at most 2^20, tokens * dim below 2^40, scale in [-2^60, 2^60]. */
+typedef struct {
+    int64_t dtype;
+    int64_t tokens, vocabulary, dim;
+    int64_t accumulate;
+    double scale;
+    int64_t stride;
+} dllm_hip_token_embedding_shape;
+int dllm_hip_token_embedding(const dllm_hip_token_embedding_shape* shape, const void* table, const int64_t* tokens, void* out,
+                             void* stream);
+size_t dllm_hip_token_embedding_backward_workspace(const dllm_hip_token_embedding_shape* shape);
+int dllm_hip_token_embedding_backward(const dllm_hip_token_embedding_shape* shape, const int64_t* tokens, const void* dout,
+                                      void* dtable, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The loss over the vocabulary from the last hidden states, without keeping the logits: hidden[rows, dim], weight[vocabulary, dim],
+ * targets[rows] (int64, device). With x = scale * hidden.weight and z = softcap tanh(x / softcap) (softcap 0: z = x),
+ *     lse[t] = log sum over v of exp z[t, v],   loss[t] = lse[t] - z[t, targets[t]]   (float32[rows] each).
+ * A row whose target is outside the vocabulary (a prompt's, padding) does not count: its loss and lse are 0, and whatever its
+ * hidden state holds reaches nothing. loss is minus the target's log-probability. Either of loss and lse may be NULL.
+ * The backward takes the forward's lse and the upstream gradients dloss (float32[rows]; the caller's weights, 1 / count for a mean) and
+ * writes dhidden (zero where a row does not count) and dweight; either may be NULL. accumulate adds to what dweight holds, in
+ * float32 before the one rounding. It forms the logits again, a piece of the vocabulary at a time. The softmax's part of a
+ * gradient has the probabilities as operands in dtype, the target's part is float32's. float16 holds the probabilities times each
+ * row's dloss relative to it, so that gradients of any size keep their bits; in dweight, rows whose dloss is below 2^-14
+ * of the largest one's lose some of their softmax's part.
+ * A row's loss, lse and dhidden are the same bits alone and in any batch. hidden_stride and dhidden_stride: elements between rows (0: dim).
+ * Outputs do not overlap inputs. Limits: rows below 2^27, vocabulary below 2^31, their product below 2^48, dim at most 2^16, scale in
+ * [2^-60, 2^60], softcap 0 or in [2^-64, 2^64]. */
+typedef struct {
+    int64_t dtype;
+    int64_t rows, vocabulary, dim;
+    int64_t accumulate;
+    double scale, softcap;
+    int64_t hidden_stride, dhidden_stride;
+} dllm_hip_vocabulary_loss_shape;
+size_t dllm_hip_vocabulary_loss_workspace(const dllm_hip_vocabulary_loss_shape* shape);
+int dllm_hip_vocabulary_loss(const dllm_hip_vocabulary_loss_shape* shape, const void* hidden, const void* weight,
+                             const int64_t* targets, float* loss, float* lse, void* workspace, size_t workspace_bytes,
+                             void* stream);
+size_t dllm_hip_vocabulary_loss_backward_workspace(const dllm_hip_vocabulary_loss_shape* shape);
+int dllm_hip_vocabulary_loss_backward(const dllm_hip_vocabulary_loss_shape* shape, const void* hidden, const void* weight,
+                                      const int64_t* targets, const float* lse, const float* dloss, void* dhidden,
+                                      void* dweight, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Orthogonalises updates, as the Muon optimiser does: `batch` matrices x[rows, cols]. With X = x / (|x| + eps) (Frobenius norm),
+ * `steps` times
+ *     A = X X^T,   X = a X + (b A + c A A) X
+ * (on the transposed matrix where rows exceed cols, which is the same and smaller), and out = scale * X. coefficients: HOST, a, b
+ * and c of each step; NULL: 3.4445, -4.7750, 2.0315 in all of them, which bring the singular values near one in about five
+ * steps. 16-bit updates are multiplied in float16 with X itself held in float32; float32 ones in pairs of float16,
+ * float32's accuracy. Strides in elements between rows and between matrices (0: packed). out may be x with the same strides;
+ * otherwise they do not overlap. Limits: rows and cols at most 2^16, batch at most 65535, steps in [0, 64], eps at least 0,
+ * scale and coefficients finite. */
+typedef struct {
+    int64_t dtype;
+    int64_t batch, rows, cols;
+    int64_t steps;
+    double eps, scale;
+    int64_t x_stride, x_batch_stride, out_stride, out_batch_stride;
+} dllm_hip_orthogonalize_shape;
+size_t dllm_hip_orthogonalize_workspace(const dllm_hip_orthogonalize_shape* shape);
+int dllm_hip_orthogonalize(const dllm_hip_orthogonalize_shape* shape, const double* coefficients, const void* x, void* out,
+                           void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- the device-resident fine-tuning step ----
  *
  * Replaces the Python step the reference runs through those kernels: FineTuner.train_step
