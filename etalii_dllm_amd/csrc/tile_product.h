@@ -29,8 +29,6 @@ struct Operand {
 
 static __device__ const uint4 kZeroChunk = {0, 0, 0, 0};
 
-constexpr int kTileK = 64;
-
 template <int kPlanesOf>
 struct PlanePairs {
     static constexpr int kCount = kPlanesOf == 1 ? 1 : kPlanesOf == 2 ? 3 : 6;
@@ -50,11 +48,12 @@ struct PlanePairs {
 template <int kChunks>
 __device__ __forceinline__ int tile_swizzle(int row) {
     if constexpr (kChunks >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+    if constexpr (kChunks == 4) return (row >> 2) & 3;
     return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
-// One operand's tile of kSize m or n by 64 k: its copy to LDS and its reads.
-template <int kSize, int kThreads, bool kColumns>
+// One operand's tile of kSize m or n by kTileK k: its copy to LDS.
+template <int kSize, int kTileK, int kThreads, bool kColumns>
 struct OperandTile {
     static constexpr int kChunks = kColumns ? kSize / 8 : kTileK / 8;  // of an LDS row
     static constexpr int kRows = kColumns ? kTileK : kSize;
@@ -62,7 +61,7 @@ struct OperandTile {
     static constexpr int kBytes = kRows * kRowBytes;
     static constexpr int kTurns = kRows * kChunks / kThreads;
     static constexpr int kTurnRows = kThreads / kChunks;
-    static_assert(kRows * kChunks % kThreads == 0 && kTurnRows % 16 == 0);
+    static_assert(kRows * kChunks % kThreads == 0 && kThreads % kChunks == 0);
 
     const char* base;  // of the tile's first m or n
     int64_t stride, plane;
@@ -107,7 +106,7 @@ struct OperandTile {
 };
 
 // A lane's reads of blocks of 32 m or n by 16 k from a tile.
-template <int kSize, bool kColumns>
+template <int kSize, int kTileK, bool kColumns>
 struct OperandView {
 
     static constexpr int kRowBytes = (kColumns ? kSize / 8 : kTileK / 8) * 16;
@@ -150,17 +149,25 @@ struct OperandView {
     }
 };
 
-// A tile of kM x kN by kWavesM x kWavesN waves.
-template <typename P, int kPlanesOf, int kM_, int kN_, int kWavesM_, int kWavesN_, bool kAColumns, bool kBColumns>
+// All but kCount of this wave's copies have arrived, and its LDS reads are done; then all waves' are.
+template <int kCount>
+__device__ __forceinline__ void stage_barrier() {
+    static_assert(kCount < 64);
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kCount) : "memory");
+}
+
+// A tile of kM x kN by kWavesM x kWavesN waves, kTileK k to each of kStages buffers.
+template <typename P, int kPlanesOf, int kM_, int kN_, int kWavesM_, int kWavesN_, bool kAColumns, bool kBColumns, int kTileK = 64, int kStages = 2>
 struct TileProduct {
     static constexpr int kM = kM_, kN = kN_, kWavesM = kWavesM_, kWavesN = kWavesN_;
     static constexpr int kThreads = kWavesM * kWavesN * kWave;
     static constexpr int kWaveM = kM / kWavesM, kWaveN = kN / kWavesN;
     static constexpr int kBlocksM = kWaveM / 32, kBlocksN = kWaveN / 32;
-    using ATile = OperandTile<kM, kThreads, kAColumns>;
-    using BTile = OperandTile<kN, kThreads, kBColumns>;
+    using ATile = OperandTile<kM, kTileK, kThreads, kAColumns>;
+    using BTile = OperandTile<kN, kTileK, kThreads, kBColumns>;
     static constexpr int kStage = ATile::kBytes + BTile::kBytes;
-    static constexpr int kLds = 2 * kStage;
+    static constexpr int kLds = kStages * kStage;
+    static constexpr int kCopies = ATile::kTurns + BTile::kTurns;  // of a thread, for one stage
     using Sums = Acc[kBlocksM][kBlocksN];
 
     static __device__ __forceinline__ int wave() { return __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6); }
@@ -174,33 +181,40 @@ struct TileProduct {
         BTile bt;
         at.init(a, m0, a_count, batch_a);
         bt.init(b, n0, b_count, batch_b);
-        const OperandView<kM, kAColumns> av(wave_m());
-        const OperandView<kN, kBColumns> bv(wave_n());
+        const OperandView<kM, kTileK, kAColumns> av(wave_m());
+        const OperandView<kN, kTileK, kBColumns> bv(wave_n());
 #pragma unroll
         for (int i = 0; i < kBlocksM; ++i)
 #pragma unroll
             for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Acc{};
         const int tiles = static_cast<int>((k + kTileK - 1) / kTileK), count = tiles * PlanePairs<kPlanesOf>::kCount;
         if (count == 0) return;
-        int pair = 0, tile = 0;  // of the next copy
-        auto copy = [&](int buffer) {
-            LdsByte* const to = lds + buffer * kStage;
+        int pair = 0, tile = 0, into = 0;  // of the next copy
+        auto copy = [&] {
+            LdsByte* const to = lds + into * kStage;
             at.copy(static_cast<int64_t>(tile) * kTileK, k, PlanePairs<kPlanesOf>::a(pair), to);
             bt.copy(static_cast<int64_t>(tile) * kTileK, k, PlanePairs<kPlanesOf>::b(pair), to + ATile::kBytes);
             if (++tile == tiles) tile = 0, ++pair;
+            into = into + 1 == kStages ? 0 : into + 1;
         };
-        copy(0);
+        for (int i = 0; i < kStages - 1 && i < count; ++i) copy();
+        int from = 0;
         for (int i = 0; i < count; ++i) {
-            tile_barrier();
-            if (i + 1 < count) copy((i + 1) & 1);
-            const LdsByte* const from = lds + (i & 1) * kStage;
+            // stage i has arrived, and the one that the next copy goes to is read
+            if (kStages > 2 && i + kStages - 2 < count)
+                stage_barrier<(kStages - 2) * kCopies>();
+            else
+                stage_barrier<0>();
+            if (i + kStages - 1 < count) copy();
+            const LdsByte* const stage = lds + from * kStage;
+            from = from + 1 == kStages ? 0 : from + 1;
 #pragma unroll
             for (int step = 0; step < kTileK / 16; ++step) {
                 Chunk16 x[kBlocksM], y[kBlocksN];
 #pragma unroll
-                for (int m = 0; m < kBlocksM; ++m) x[m] = av.read(from, m, step);
+                for (int m = 0; m < kBlocksM; ++m) x[m] = av.read(stage, m, step);
 #pragma unroll
-                for (int n = 0; n < kBlocksN; ++n) y[n] = bv.read(from + ATile::kBytes, n, step);
+                for (int n = 0; n < kBlocksN; ++n) y[n] = bv.read(stage + ATile::kBytes, n, step);
 #pragma unroll
                 for (int m = 0; m < kBlocksM; ++m)
 #pragma unroll
@@ -215,6 +229,40 @@ __device__ __forceinline__ int lane_column() { return static_cast<int>(threadIdx
 
 // Row of a 32 x 32 block that a lane holds in element r; its column is lane % 32.
 __device__ __forceinline__ int block_row(int r) { return 8 * (r >> 2) + 4 * lane_half() + (r & 3); }
+
+// A wave's sums by rows: f(row, column, v) with 8 consecutive columns' sums in each lane (row and column within the wave's part), for
+// wide stores. The blocks go through LDS, 32 rows at a time; its 16-byte chunks lie at places that keep both ways free of
+// conflicts on the 64 banks.
+template <typename Tile, typename F>
+__device__ __forceinline__ void by_rows(const typename Tile::Sums& acc, LdsByte* lds, F&& f) {
+    constexpr int kColumns = Tile::kWaveN, kRowBytes = kColumns * 4, kLanes = kColumns / 8, kRowsAtOnce = kWave / kLanes;
+    static_assert(Tile::kThreads / kWave * 32 * kRowBytes <= Tile::kLds);
+    using Four = float __attribute__((ext_vector_type(4)));
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    LdsByte* const area = lds + Tile::wave() * 32 * kRowBytes;
+    const auto at = [](int row, int chunk) { return row * kRowBytes + ((chunk ^ (kColumns >= 64 ? ((row >> 2) & 1) << 3 | (row & 1) : row & 1)) << 4); };
+    __syncthreads();  // the products' stages are read
+#pragma unroll
+    for (int i = 0; i < Tile::kBlocksM; ++i) {
+#pragma unroll
+        for (int j = 0; j < Tile::kBlocksN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const int column = 32 * j + lane_column();
+                *(__attribute__((address_space(3))) float*)(area + at(block_row(r), column >> 2) + (column & 3) * 4) = acc[i][j][r];
+            }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int t = 0; t < 32 / kRowsAtOnce; ++t) {
+            const int row = t * kRowsAtOnce + lane / kLanes, chunk = 2 * (lane % kLanes);
+            const Four one = *(__attribute__((address_space(3))) Four*)(area + at(row, chunk)),
+                       two = *(__attribute__((address_space(3))) Four*)(area + at(row, chunk + 1));
+            float v[8] = {one[0], one[1], one[2], one[3], two[0], two[1], two[2], two[3]};
+            f(32 * i + row, chunk * 4, v);
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
 
 // Workgroup id -> tile, such that each XCD (workgroups are dealt over the 8 in turn) takes a contiguous range of tiles, and those
 // that run at once share panels: 8 tiles of n side by side, m after m.

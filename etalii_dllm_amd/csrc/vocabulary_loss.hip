@@ -11,8 +11,8 @@
 // the target's logit.
 //
 // Backward, a piece of the vocabulary at a time: the logits again, whose epilogue stores the softmax's part of g in the product's
-// type; then its products with the weights and with the hidden states. dh is added up in float32 over units of 8192 of the
-// vocabulary, whatever the batch, so a row's bits are its own. The target's element c = expm1(z - lse) ... stays out of the
+// type; then its products with the weights and with the hidden states. dh is added up in float32 over units of the vocabulary that
+// go by its size alone, whatever the batch, so a row's bits are its own. The target's element c = expm1(z - lse) ... stays out of the
 // 16-bit products: p - 1 is what is left of two near numbers where the model is sure, and with a uniform dloss its rounding would
 // not average out. c W[target] is added to dh in float32, and the sums of c h by target (token_rows.h) to dW in the epilogue.
 #include <math.h>
@@ -31,10 +31,10 @@ using namespace dllm_hip;
 
 namespace {
 
-constexpr int64_t kUnit = 8192;       // of the vocabulary: one addition to dh
 constexpr int64_t kPackPiece = 16384;  // of the vocabulary: weights packed at once, where they are
 constexpr int kStatRows = 128;        // of the vocabulary: one maximum and sum
 constexpr size_t kPieceBytes = size_t{1} << 28;
+constexpr int64_t kStrideSlack = 64;  // elements between the softmax's rows: their stride is no power of two, which would meet on few channels
 constexpr int kHalfShift = 14;  // float16 holds the softmax's part of g times 2^14, relative to the row's weight
 
 struct LossShape {
@@ -133,6 +133,36 @@ int launch_pack(const T* src, Part<T>* dst, const PackArgs& args, hipStream_t st
     return check_launch("vocabulary_loss packing");
 }
 
+// ---- tiles ----
+
+// The products' tiles by the number of rows. 256 x 256 by eight waves, one workgroup to a CU; 128 x 128 by four, two to a CU, where
+// the large ones would leave CUs without work or pad much; and for up to 64 rows, whose products wait for the weights'
+// bytes, tiles of 64 rows. The forward's waves hold kStatRows of the vocabulary in all of them.
+template <typename T, bool kAColumns, bool kBColumns, int kM, int kN, int kWavesM, int kWavesN, int kStages = 2>
+using Product64 = TileProduct<Part<T>, kPlanes<T>, kM, kN, kWavesM, kWavesN, kAColumns, kBColumns, 64, kStages>;
+
+template <typename T>
+struct LargeTiles {
+    using Forward = Product64<T, false, false, 256, 256, 2, 4>;
+    using Logits = Product64<T, false, false, 256, 256, 2, 4>;
+    using Hidden = Product64<T, false, true, 256, 256, 2, 4>;
+    using Weight = Product64<T, true, true, 256, 256, 2, 4>;
+};
+template <typename T>
+struct MiddleTiles {
+    using Forward = Product64<T, false, false, 256, 128, 2, 4>;
+    using Logits = Product64<T, false, false, 128, 128, 2, 2>;
+    using Hidden = Product64<T, false, true, 128, 128, 2, 2>;
+    using Weight = Product64<T, true, true, 128, 128, 2, 2>;
+};
+template <typename T>
+struct SmallTiles {
+    using Forward = Product64<T, false, false, 128, 64, 1, 2>;
+    using Logits = Product64<T, false, false, 64, 256, 1, 4>;
+    using Hidden = Product64<T, false, true, 64, 64, 2, 2, 4>;
+    using Weight = Product64<T, true, true, 128, 128, 2, 2>;
+};
+
 // ---- logits ----
 
 // A logit from its product, and the cap's derivative.
@@ -170,12 +200,8 @@ struct ForwardArgs {
     float* at_target;  // [rows]
 };
 
-template <typename T>
-using ForwardTile = TileProduct<Part<T>, kPlanes<T>, 256, 256, 2, 4, false, false>;
-
-template <typename T, bool kCapped>
-__global__ __launch_bounds__(ForwardTile<T>::kThreads) void forward_kernel(ForwardArgs a, int64_t m_tiles, int64_t n_tiles) {
-    using Tile = ForwardTile<T>;
+template <typename T, bool kCapped, typename Tile>
+__global__ __launch_bounds__(Tile::kThreads) void forward_kernel(ForwardArgs a, int64_t m_tiles, int64_t n_tiles) {
     static_assert(Tile::kWaveM == kStatRows);
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int64_t count = *a.count;
@@ -345,12 +371,9 @@ struct SoftmaxArgs {
     int64_t out_stride, out_plane;
 };
 
-template <typename T>
-using LogitTile = TileProduct<Part<T>, kPlanes<T>, 256, 256, 2, 4, false, false>;
-
-template <typename T, bool kCapped>
-__global__ __launch_bounds__(LogitTile<T>::kThreads) void softmax_kernel(SoftmaxArgs a, int64_t m_tiles, int64_t n_tiles) {
-    using Tile = LogitTile<T>;
+// The softmax's part of g, zero past the vocabulary's end and at the targets.
+template <typename T, bool kCapped, typename Tile>
+__global__ __launch_bounds__(Tile::kThreads) void softmax_kernel(SoftmaxArgs a, int64_t m_tiles, int64_t n_tiles) {
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int64_t count = *a.count;
     int64_t m, n;
@@ -361,82 +384,149 @@ __global__ __launch_bounds__(LogitTile<T>::kThreads) void softmax_kernel(Softmax
     Tile::run(a.hidden, a.weight, m * Tile::kM, n * Tile::kN, count, a.weight.count, a.s.padded, 0, 0, (LdsByte*)lds, acc);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
     const Cap cap(a.s);
+    by_rows<Tile>(acc, (LdsByte*)lds, [&](int in_row, int in_column, float (&v)[8]) {
+        const int64_t row = m0 + in_row, column = n0 + in_column;
+        if (row >= count) return;
+        const float lse = a.terms.lse[row], factor = a.terms.factor[row];
+        const int64_t target = a.terms.target[row] - a.first - column, left = a.weight.count - column;
+        using V = Part<T> __attribute__((ext_vector_type(8)));
+        V out[kPlanes<T>];
 #pragma unroll
-    for (int i = 0; i < Tile::kBlocksM; ++i)
+        for (int e = 0; e < 8; ++e) {
+            float derivative;
+            const float z = cap.logit<kCapped>(v[e], derivative);
+            float p = __builtin_amdgcn_exp2f((z - lse) * kLog2E) * factor;
+            if constexpr (kCapped) p *= derivative;
+            if (e >= left || e == target) p = 0.0f;
+            Part<T> parts[kPlanes<T>];
+            split<T>(p, parts);
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int64_t row = m0 + 32 * i + 8 * g + 4 * lane_half();  // the arrays are padded to whole tiles
-            const float4 lse = *reinterpret_cast<const float4*>(a.terms.lse + row);
-            const float4 factor = *reinterpret_cast<const float4*>(a.terms.factor + row);
-            const int4 target = *reinterpret_cast<const int4*>(a.terms.target + row);
-            const float ls[4] = {lse.x, lse.y, lse.z, lse.w}, fs[4] = {factor.x, factor.y, factor.z, factor.w};
-            const int ts[4] = {target.x, target.y, target.z, target.w};
-#pragma unroll
-            for (int j = 0; j < Tile::kBlocksN; ++j) {
-                const int64_t column = n0 + 32 * j + lane_column();
-                const bool inside = column < a.weight.count;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    float derivative;
-                    const float z = cap.logit<kCapped>(acc[i][j][4 * g + r], derivative);
-                    float p = __builtin_amdgcn_exp2f((z - ls[r]) * kLog2E) * fs[r];
-                    if constexpr (kCapped) p *= derivative;
-                    if (!inside || a.first + column == ts[r]) p = 0.0f;
-                    if (row + r >= count) continue;
-                    Part<T> parts[kPlanes<T>];
-                    split<T>(p, parts);
-#pragma unroll
-                    for (int q = 0; q < kPlanes<T>; ++q)
-                        *reinterpret_cast<Part<T>*>(a.out + q * a.out_plane + (row + r) * a.out_stride + column * 2) = parts[q];
-                }
-            }
+            for (int q = 0; q < kPlanes<T>; ++q) out[q][e] = parts[q];
         }
+#pragma unroll
+        for (int q = 0; q < kPlanes<T>; ++q)
+            *reinterpret_cast<V*>(a.out + q * a.out_plane + row * a.out_stride + column * 2) = out[q];
+    });
 }
 
-struct HiddenArgs {
-    Operand softmax, weight;  // batch: units
+// The products of a piece's softmax: with the weights, for dh, and with the hidden states, for dW, in one launch. Their tiles fill
+// the CUs' rounds together (8192 rows, 16384 of the vocabulary, 1536 dimensions: 192 and 384 tiles, the first twice as long), and the longer ones begin.
+struct GradientArgs {
+    Operand softmax, weight, hidden;  // softmax.batch, weight.batch: a unit
     const uint32_t* count;
-    int64_t k;  // of the piece
-    float* part;  // [unit][rows][dim]
-    int64_t rows, dim;
+    int64_t rows, dim, first, width, unit;  // first and width: of the piece
+    // dh
+    int64_t hidden_blocks, m_tiles, n_tiles;
+    bool in_turn;  // a tile adds its units to the total itself, else each unit has a part
+    bool begin;    // the total begins here
+    float *total, *part;
+    // dW
+    int64_t weight_m_tiles, weight_n_tiles;
+    const float* sums;       // the targets' part, by the index in `at`
+    const int32_t* at;       // by token, -1: none
+    const int32_t* largest;  // float16: the power of two left out
+    bool accumulate;
+    bool whole;  // dW's rows are whole 16-byte chunks
 };
 
-template <typename T>
-using HiddenTile = TileProduct<Part<T>, kPlanes<T>, 256, 256, 2, 4, false, true>;
-
-template <typename T>
-__global__ __launch_bounds__(HiddenTile<T>::kThreads) void hidden_kernel(HiddenArgs a, int64_t m_tiles, int64_t n_tiles, int64_t units) {
-    using Tile = HiddenTile<T>;
-    __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
-    const int64_t count = *a.count;
-    if (block_id() >= m_tiles * n_tiles * units) return;
-    const int64_t unit = block_id() / (m_tiles * n_tiles);
+template <typename Tile>
+__device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, LdsByte* lds) {
+    const int64_t count = *a.count, units = (a.width + a.unit - 1) / a.unit, each = a.m_tiles * a.n_tiles;
+    const int64_t only = a.in_turn ? 0 : id / each, end = a.in_turn ? units : only + 1;
     int64_t m, n;
-    tile_of(block_id() - unit * m_tiles * n_tiles, m_tiles, n_tiles, m, n);
+    tile_of(id - only * each, a.m_tiles, a.n_tiles, m, n);
     if (m * Tile::kM >= count) return;
-    typename Tile::Sums acc;
-    Tile::run(a.softmax, a.weight, m * Tile::kM, n * Tile::kN, count, a.dim, min(kUnit, a.k - unit * kUnit), unit, unit, (LdsByte*)lds, acc);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
-    float* const part = a.part + unit * a.rows * a.dim;
+    float* const out = a.in_turn ? a.total : a.part + only * a.rows * a.dim;
+    for (int64_t unit = only; unit < end; ++unit) {
+        typename Tile::Sums acc;
+        Tile::run(a.softmax, a.weight, m * Tile::kM, n * Tile::kN, count, a.dim, min(a.unit, a.width - unit * a.unit), unit, unit, lds, acc);
+        const bool store = !a.in_turn || (a.begin && unit == 0);
+        by_rows<Tile>(acc, lds, [&](int in_row, int in_column, float (&v)[8]) {
+            const int64_t row = m0 + in_row, column = n0 + in_column;
+            if (row >= count) return;
+            float* const to = out + row * a.dim + column;
+            if (a.dim % 4 == 0) {
 #pragma unroll
-    for (int i = 0; i < Tile::kBlocksM; ++i)
+                for (int q = 0; q < 8; q += 4) {
+                    if (column + q >= a.dim) continue;
+                    float4 w = make_float4(v[q], v[q + 1], v[q + 2], v[q + 3]);
+                    if (!store) {
+                        const float4 old = *reinterpret_cast<const float4*>(to + q);
+                        w = make_float4(old.x + w.x, old.y + w.y, old.z + w.z, old.w + w.w);
+                    }
+                    *reinterpret_cast<float4*>(to + q) = w;
+                }
+            } else {
 #pragma unroll
-        for (int j = 0; j < Tile::kBlocksN; ++j) {
-            const int64_t column = n0 + 32 * j + lane_column();
+                for (int e = 0; e < 8; ++e)
+                    if (column + e < a.dim) to[e] = store ? v[e] : to[e] + v[e];
+            }
+        });
+        if (unit + 1 < end) __syncthreads();  // the next unit's copies go where these rows were
+    }
+}
+
+template <typename T, typename Tile>
+__device__ __forceinline__ void weight_tile(T* __restrict__ dweight, const GradientArgs& a, int64_t id, LdsByte* lds) {
+    int64_t m, n;
+    tile_of(id, a.weight_m_tiles, a.weight_n_tiles, m, n);
+    typename Tile::Sums acc;
+    Tile::run(a.softmax, a.hidden, m * Tile::kM, n * Tile::kN, a.width, a.dim, *a.count, 0, 0, lds, acc);
+    const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
+    const int by = __is_same(T, _Float16) ? *a.largest - kHalfShift : 0;
+    by_rows<Tile>(acc, lds, [&](int in_row, int in_column, float (&v)[8]) {
+        const int64_t row = m0 + in_row, column = n0 + in_column;
+        if (row >= a.width || column >= a.dim) return;
+        const int64_t at = a.at[a.first + row];
+        T* const out = dweight + (a.first + row) * a.dim + column;
+        if constexpr (__is_same(T, _Float16)) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t row = m0 + 32 * i + block_row(r);
-                if (row < count && column < a.dim) part[row * a.dim + column] = acc[i][j][r];
+            for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], by);
+        }
+        if (a.whole) {
+            if (at >= 0) {
+                float w[8];
+                load_as_float<float, 8>(a.sums + at * a.dim + column, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += w[e];
+            }
+            if (a.accumulate) {
+                float w[8];
+                load_as_float<T, 8>(out, w);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] += w[e];
+            }
+            store_from_float<T, 8>(out, v);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                if (column + e >= a.dim) break;
+                if (at >= 0) v[e] += a.sums[at * a.dim + column + e];
+                if (a.accumulate) v[e] += static_cast<float>(out[e]);
+                out[e] = static_cast<T>(v[e]);
             }
         }
+    });
+}
+
+template <typename T, typename HiddenTile, typename WeightTile>
+__global__ __launch_bounds__(HiddenTile::kThreads) void gradient_kernel(T* __restrict__ dweight, GradientArgs a) {
+    static_assert(HiddenTile::kThreads == WeightTile::kThreads);
+    __shared__ __attribute__((aligned(1024))) char lds[HiddenTile::kLds > WeightTile::kLds ? HiddenTile::kLds : WeightTile::kLds];
+    const int64_t id = block_id();
+    if (id < a.hidden_blocks)
+        hidden_tile<HiddenTile>(a, id, (LdsByte*)lds);
+    else if (id < a.hidden_blocks + a.weight_m_tiles * a.weight_n_tiles)
+        weight_tile<T, WeightTile>(dweight, a, id - a.hidden_blocks, (LdsByte*)lds);
 }
 
 // total (+)= the units' parts, in their order
 __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, float* __restrict__ total, const uint32_t* __restrict__ count,
-                                                        int64_t rows, int64_t dim, int units, bool first) {
+                                                        int64_t rows, int64_t dim, int units, bool begin) {
     const int64_t n = static_cast<int64_t>(*count) * dim;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
-        float v = first ? part[i] : total[i] + part[i];
+        float v = begin ? part[i] : total[i] + part[i];
         for (int u = 1; u < units; ++u) v += part[u * rows * dim + i];
         total[i] = v;
     }
@@ -469,51 +559,6 @@ __global__ __launch_bounds__(256) void finish_hidden_kernel(const T* __restrict_
     }
 }
 
-struct WeightArgs {
-    Operand softmax, hidden;
-    const uint32_t* count;
-    int64_t first, rows, dim;  // rows: of the piece
-    const float* sums;         // the targets' part, by the index in `at`
-    const int32_t* at;         // by token, -1: none
-    const int32_t* largest;    // float16: the power of two left out
-    bool accumulate;
-};
-
-template <typename T>
-using WeightTile = TileProduct<Part<T>, kPlanes<T>, 256, 256, 2, 4, true, true>;
-
-template <typename T>
-__global__ __launch_bounds__(WeightTile<T>::kThreads) void weight_kernel(T* __restrict__ dweight, WeightArgs a, int64_t m_tiles, int64_t n_tiles) {
-    using Tile = WeightTile<T>;
-    __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
-    int64_t m, n;
-    if (block_id() >= m_tiles * n_tiles) return;
-    tile_of(block_id(), m_tiles, n_tiles, m, n);
-    typename Tile::Sums acc;
-    Tile::run(a.softmax, a.hidden, m * Tile::kM, n * Tile::kN, a.rows, a.dim, *a.count, 0, 0, (LdsByte*)lds, acc);
-    const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
-    const int by = __is_same(T, _Float16) ? *a.largest - kHalfShift : 0;
-#pragma unroll
-    for (int i = 0; i < Tile::kBlocksM; ++i)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const int64_t row = m0 + 32 * i + block_row(r);
-            if (row >= a.rows) continue;
-            const int64_t at = a.at[a.first + row];
-#pragma unroll
-            for (int j = 0; j < Tile::kBlocksN; ++j) {
-                const int64_t column = n0 + 32 * j + lane_column();
-                if (column >= a.dim) continue;
-                float v = acc[i][j][r];
-                if constexpr (__is_same(T, _Float16)) v = ldexpf(v, by);
-                if (at >= 0) v += a.sums[at * a.dim + column];
-                T* const out = dweight + (a.first + row) * a.dim + column;
-                if (a.accumulate) v += static_cast<float>(*out);
-                *out = static_cast<T>(v);
-            }
-        }
-}
-
 // ---- workspaces ----
 
 int check_shape(const dllm_hip_vocabulary_loss_shape* sh) {
@@ -542,22 +587,27 @@ LossShape loss_shape(const dllm_hip_vocabulary_loss_shape& sh) {
 
 int planes_of(int64_t dtype) { return dtype == kFloat32 ? 3 : 1; }
 
+// Of the vocabulary: one addition to dh. It goes by the vocabulary and type alone, so that a row's bits are its own. Shorter units are
+// more workgroups where rows are few and more additions where they are many; float32's take six times as long.
+int64_t unit_of(const LossShape& s, int64_t dtype) { return dtype == kFloat32 ? 2048 : s.vocabulary <= 65536 ? 4096 : 8192; }
+
 // Units of the backward's piece: as many as keep its softmax within kPieceBytes, at least one.
 int64_t piece_units(const LossShape& s, int64_t dtype) {
-    const size_t unit = static_cast<size_t>(s.rows) * kUnit * 2 * planes_of(dtype);
-    const int64_t all = static_cast<int64_t>(ceil_div(s.vocabulary, kUnit));
-    return std::clamp<int64_t>(static_cast<int64_t>(kPieceBytes / std::max<size_t>(unit, 1)), 1, all);
+    const int64_t unit = unit_of(s, dtype);
+    const size_t bytes = static_cast<size_t>(s.rows) * unit * 2 * planes_of(dtype);
+    const int64_t all = static_cast<int64_t>(ceil_div(s.vocabulary, unit));
+    return std::clamp<int64_t>(static_cast<int64_t>(kPieceBytes / std::max<size_t>(bytes, 1)), 1, all);
 }
 
 struct LossLayout {
     size_t hidden, scaled, weight, list, stats, at_target;                  // forward
     size_t terms, softmax, part, total, sums, sum_parts, at, coefficient;   // backward
-    int64_t units;
+    int64_t unit, units;
     size_t bytes;
     LossLayout(const LossShape& s, int64_t dtype, bool backward) {
         const size_t rows = static_cast<size_t>(s.rows), planes = planes_of(dtype), dim = static_cast<size_t>(s.dim);
-        units = piece_units(s, dtype);
-        const size_t piece = backward ? std::min<size_t>(units * kUnit, s.vocabulary) : std::min<size_t>(kPackPiece, s.vocabulary);
+        unit = unit_of(s, dtype), units = piece_units(s, dtype);
+        const size_t piece = backward ? std::min<size_t>(units * unit, s.vocabulary) : std::min<size_t>(kPackPiece, s.vocabulary);
         hidden = rows * s.padded * planes;
         scaled = backward && dtype == kFloat16 ? hidden : 0;
         weight = piece * s.padded * planes;
@@ -565,7 +615,7 @@ struct LossLayout {
         stats = backward ? 0 : ceil_div(s.vocabulary, kStatRows) * rows;
         at_target = backward ? 0 : rows;
         terms = backward ? round_up(rows, 256) : 0;
-        softmax = backward ? rows * units * kUnit * planes : 0;
+        softmax = backward ? rows * (units * unit + kStrideSlack) * planes : 0;
         part = backward ? units * rows * dim : 0;
         total = backward ? rows * dim : 0;
         sums = total;
@@ -652,6 +702,15 @@ Operand hidden_operand(const LossShape& s, const Part<T>* packed) {
     return {reinterpret_cast<const char*>(packed), s.padded * 2, s.rows * s.padded * 2, 0, s.rows};
 }
 
+template <typename T, typename Tile>
+void launch_forward(const ForwardArgs& a, hipStream_t stream) {
+    const int64_t m = ceil_div(a.weight.count, Tile::kM), n = ceil_div(a.s.rows, Tile::kN);
+    if (a.s.softcap != 0.0f)
+        forward_kernel<T, true, Tile><<<grid_of(m * n), Tile::kThreads, 0, stream>>>(a, m, n);
+    else
+        forward_kernel<T, false, Tile><<<grid_of(m * n), Tile::kThreads, 0, stream>>>(a, m, n);
+}
+
 template <typename T>
 int run_forward(const LossShape& s, int64_t dtype, const T* hidden, const T* weight, const int64_t* targets, float* loss, float* lse,
                 void* workspace, size_t bytes, hipStream_t stream) {
@@ -668,17 +727,75 @@ int run_forward(const LossShape& s, int64_t dtype, const T* hidden, const T* wei
         a.s = s, a.hidden = hidden_operand<T>(s, b.hidden);
         DLLM_TRY(weight_operand<T>(s, weight, b.weight, first, std::min(piece, s.vocabulary - first), a.weight, stream));
         a.first = first, a.list = b.list, a.count = b.count, a.targets = targets, a.stats = b.stats, a.at_target = b.at_target;
-        using Tile = ForwardTile<T>;
-        const int64_t m = ceil_div(a.weight.count, Tile::kM), n = ceil_div(s.rows, Tile::kN);
-        const dim3 grid = grid_of(m * n);
-        if (s.softcap != 0.0f)
-            forward_kernel<T, true><<<grid, Tile::kThreads, 0, stream>>>(a, m, n);
+        if (s.rows <= 64)
+            launch_forward<T, typename SmallTiles<T>::Forward>(a, stream);
+        else if (s.rows <= 128)
+            launch_forward<T, typename MiddleTiles<T>::Forward>(a, stream);
         else
-            forward_kernel<T, false><<<grid, Tile::kThreads, 0, stream>>>(a, m, n);
+            launch_forward<T, typename LargeTiles<T>::Forward>(a, stream);
     }
     join_stats_kernel<<<grid_of(ceil_div(s.rows, 4)), 256, 0, stream>>>(
         b.stats, b.at_target, static_cast<int64_t>(ceil_div(s.vocabulary, kStatRows)), s.rows, b.list, b.count, loss, lse);
     return check_launch("vocabulary_loss");
+}
+
+// Whether 256 x 256 tiles take less time for a piece's products than 128 x 128 ones: a large tile takes as long as four small ones at
+// two to a CU would, or a little less, so rounds and padding decide.
+bool large_tiles(const LossShape& s, const LossLayout& l) {
+    const auto time = [&](int64_t size, int64_t slots, double round) {
+        const int64_t width = std::min(l.units * l.unit, s.vocabulary);
+        const int64_t m = ceil_div(s.rows, size), n = ceil_div(width, size), d = ceil_div(s.dim, size);
+        const double logits = std::ceil(static_cast<double>(m * n) / slots) * s.dim;
+        const double products = std::max(std::ceil(static_cast<double>(m * d * l.units) * l.unit + static_cast<double>(n * d) * s.rows) / slots,
+                                         static_cast<double>(l.unit));
+        return (logits + products) * round;
+    };
+    return time(256, 256, 4.0) <= time(128, 512, 2.1);
+}
+
+template <typename T, typename Tiles>
+int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout, const T* weight, bool dhidden, T* dweight, bool accumulate,
+               hipStream_t stream) {
+    constexpr bool kHalf = __is_same(T, _Float16);
+    using Logits = typename Tiles::Logits;
+    using Hidden = typename Tiles::Hidden;
+    using Weight = typename Tiles::Weight;
+    const int64_t piece = layout.units * layout.unit;
+    for (int64_t first = 0; first < s.vocabulary; first += piece) {
+        SoftmaxArgs a{};
+        a.s = s, a.hidden = hidden_operand<T>(s, b.hidden);
+        DLLM_TRY(weight_operand<T>(s, weight, b.weight, first, std::min(piece, s.vocabulary - first), a.weight, stream));
+        a.first = first, a.count = b.order.kept, a.terms = b.terms, a.out = b.softmax;
+        a.out_stride = (piece + kStrideSlack) * 2, a.out_plane = s.rows * a.out_stride;
+        const int64_t width = a.weight.count, m = ceil_div(s.rows, Logits::kM), n = ceil_div(width, Logits::kN);
+        if (s.softcap != 0.0f)
+            softmax_kernel<T, true, Logits><<<grid_of(m * n), Logits::kThreads, 0, stream>>>(a, m, n);
+        else
+            softmax_kernel<T, false, Logits><<<grid_of(m * n), Logits::kThreads, 0, stream>>>(a, m, n);
+        GradientArgs g{};
+        g.softmax = Operand{b.softmax, a.out_stride, a.out_plane, layout.unit * 2, s.rows};
+        g.weight = a.weight, g.weight.batch = layout.unit * a.weight.stride;
+        g.hidden = hidden_operand<T>(s, kHalf ? b.scaled : b.hidden);
+        g.count = b.order.kept, g.rows = s.rows, g.dim = s.dim, g.first = first, g.width = width, g.unit = layout.unit;
+        const int64_t units = ceil_div(width, layout.unit);
+        if (dhidden) {
+            g.m_tiles = ceil_div(s.rows, Hidden::kM), g.n_tiles = ceil_div(s.dim, Hidden::kN);
+            // with tiles for most CUs a tile takes the units in turn, which saves the parts' way through memory
+            g.in_turn = g.m_tiles * g.n_tiles >= 160 || units == 1;
+            g.hidden_blocks = g.m_tiles * g.n_tiles * (g.in_turn ? 1 : units);
+            g.begin = first == 0, g.total = b.total, g.part = b.part;
+        }
+        if (dweight) {
+            g.weight_m_tiles = ceil_div(width, Weight::kM), g.weight_n_tiles = ceil_div(s.dim, Weight::kN);
+            g.sums = b.sums, g.at = b.at, g.largest = b.largest, g.accumulate = accumulate;
+            g.whole = s.dim % 8 == 0 && aligned_to(dweight, 16);
+        }
+        gradient_kernel<T, Hidden, Weight><<<grid_of(g.hidden_blocks + g.weight_m_tiles * g.weight_n_tiles), Hidden::kThreads, 0, stream>>>(dweight, g);
+        if (dhidden && !g.in_turn)
+            add_parts_kernel<<<static_cast<unsigned>(std::min<size_t>(ceil_div(s.rows * s.dim, 256), 4096)), 256, 0, stream>>>(
+                b.part, b.total, b.order.kept, s.rows, s.dim, static_cast<int>(units), first == 0);
+    }
+    return check_launch("vocabulary_loss_backward");
 }
 
 template <typename T>
@@ -710,44 +827,13 @@ int run_backward(const LossShape& s, int64_t dtype, const T* hidden, const T* we
         sums.rows = hidden, sums.coefficient = b.coefficient, sums.scale = 1.0f, sums.part = b.sum_parts, sums.sums = b.sums, sums.first = b.at;
         DLLM_TRY(launch_token_sums(sums, dtype, stream));
     }
-    const int64_t piece = layout.units * kUnit;
-    for (int64_t first = 0; first < s.vocabulary; first += piece) {
-        SoftmaxArgs a{};
-        a.s = s, a.hidden = hidden_operand<T>(s, b.hidden);
-        DLLM_TRY(weight_operand<T>(s, weight, b.weight, first, std::min(piece, s.vocabulary - first), a.weight, stream));
-        a.first = first, a.count = b.order.kept, a.terms = b.terms, a.out = b.softmax;
-        a.out_stride = piece * 2, a.out_plane = s.rows * a.out_stride;
-        const int64_t width = a.weight.count;
-        {
-            using Tile = LogitTile<T>;
-            const int64_t m = ceil_div(s.rows, Tile::kM), n = ceil_div(width, Tile::kN);
-            const dim3 grid = grid_of(m * n);
-            if (s.softcap != 0.0f)
-                softmax_kernel<T, true><<<grid, Tile::kThreads, 0, stream>>>(a, m, n);
-            else
-                softmax_kernel<T, false><<<grid, Tile::kThreads, 0, stream>>>(a, m, n);
-        }
-        const Operand softmax{b.softmax, a.out_stride, a.out_plane, kUnit * 2, s.rows};
-        if (dhidden) {
-            using Tile = HiddenTile<T>;
-            HiddenArgs h{};
-            h.softmax = softmax, h.weight = a.weight, h.weight.batch = kUnit * a.weight.stride;
-            h.count = b.order.kept, h.k = width, h.part = b.part, h.rows = s.rows, h.dim = s.dim;
-            const int64_t m = ceil_div(s.rows, Tile::kM), n = ceil_div(s.dim, Tile::kN), units = ceil_div(width, kUnit);
-            hidden_kernel<T><<<grid_of(m * n * units), Tile::kThreads, 0, stream>>>(h, m, n, units);
-            add_parts_kernel<<<static_cast<unsigned>(std::min<size_t>(ceil_div(s.rows * s.dim, 256), 4096)), 256, 0, stream>>>(
-                b.part, b.total, b.order.kept, s.rows, s.dim, static_cast<int>(units), first == 0);
-        }
-        if (dweight) {
-            using Tile = WeightTile<T>;
-            WeightArgs w{};
-            w.softmax = softmax, w.hidden = hidden_operand<T>(s, kHalf ? b.scaled : b.hidden);
-            w.count = b.order.kept, w.first = first, w.rows = width, w.dim = s.dim, w.sums = b.sums, w.at = b.at, w.largest = b.largest;
-            w.accumulate = accumulate;
-            const int64_t m = ceil_div(width, Tile::kM), n = ceil_div(s.dim, Tile::kN);
-            weight_kernel<T><<<grid_of(m * n), Tile::kThreads, 0, stream>>>(dweight, w, m, n);
-        }
-    }
+    const auto pieces = [&](auto tiles) { return run_pieces<T, decltype(tiles)>(s, b, layout, weight, dhidden != nullptr, dweight, accumulate, stream); };
+    if (s.rows <= 64)
+        DLLM_TRY(pieces(SmallTiles<T>{}));
+    else if (large_tiles(s, layout))
+        DLLM_TRY(pieces(LargeTiles<T>{}));
+    else
+        DLLM_TRY(pieces(MiddleTiles<T>{}));
     if (dhidden) {
         FinishArgs f{s, b.order, b.terms, b.total, b.coefficient};
         finish_hidden_kernel<T><<<grid_of(s.rows), 256, 0, stream>>>(weight, dhidden, f);
