@@ -4,14 +4,17 @@
 //
 // on the m x n matrix with m <= n (the transposed one where rows exceed columns: X p(X^T X) = p(X X^T) X). The singular values alone
 // change, each by the polynomial a s + b s^3 + c s^5; small ones grow by a in every step, so what a rounding of X adds in the
-// directions of small singular values grows with them. X is therefore held in float32, and what the products read is rounded
-// from it: an error of theirs is relative to the term b A X + c A A X, which for small singular values is far smaller than a X.
+// directions of small singular values grows with them. X is therefore held to 22 bits and more, as a pair of float16, and what
+// the products of 16-bit updates read is its first part: an error of theirs is relative to the term b A X + c A A X, which for
+// small singular values is far smaller than a X.
 //
 // The products' operands are float16, one plane for 16-bit updates (11 bits; bfloat16's 8 would cost its results two bits) and two
 // for float32 ones (22 bits, three products). All values are bounded by the singular values, which stay near one, so fixed
 // powers of two keep them in float16's range: X times 2^4 sqrt(n), A and B times 2^8.
 //
-// A and A A are symmetric: only tiles on and above the diagonal are formed, and stored twice.
+// A and A A are symmetric: only tiles on and above the diagonal are formed, and stored twice. Where they are few and long, X X^T is
+// formed in segments of its n columns at once, whose sums a launch of its own adds in order; where there are matrices enough, a
+// workgroup takes the segments in turn and adds them in the same order, so a matrix has the same bits alone and among others.
 #include <math.h>
 
 #include <algorithm>
@@ -26,15 +29,18 @@ using namespace dllm_hip;
 
 namespace {
 
-constexpr int kNormThreads = 256;
-constexpr int kNormParts = 64;  // workgroups that add up a matrix's squares
+constexpr int kThreads = 256;
+constexpr int64_t kNormElements = 1 << 12;  // at least, whose squares a workgroup adds
+constexpr int64_t kNormParts = 512;         // at most, of a matrix
 constexpr int kMaxSteps = 64;
 constexpr float kGramScale = 0x1p8f;
 
+// Planes that the products read.
 template <typename T>
-constexpr int kUpdatePlanes = sizeof(T) == 4 ? 2 : 1;
+constexpr int kProductPlanes = sizeof(T) == 4 ? 2 : 1;
 
 using Half = _Float16;
+using Half8 = Half __attribute__((ext_vector_type(8)));
 
 struct Matrices {
     int64_t batch, m, n, m_padded, n_padded;  // padded to whole chunks
@@ -45,91 +51,131 @@ struct Matrices {
     float out_scale;
 };
 
-// ---- norm and start ----
-
-template <typename T>
-__global__ __launch_bounds__(kNormThreads) void squares_kernel(const T* __restrict__ x, double* __restrict__ part, int64_t rows, int64_t cols,
-                                                               Matrices s) {
-    __shared__ double of_wave[kNormThreads / kWave];
-    const T* const matrix = x + static_cast<int64_t>(blockIdx.y) * s.in_batch;
-    double sum = 0.0;
-    for (int64_t r = blockIdx.x; r < rows; r += gridDim.x)
-        for (int64_t c = threadIdx.x; c < cols; c += kNormThreads) {
-            const double v = static_cast<double>(static_cast<float>(matrix[r * s.in_stride + c]));
-            sum = fma(v, v, sum);
-        }
-#pragma unroll
-    for (int i = 32; i > 0; i >>= 1) sum += __shfl_xor(sum, i);
-    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < kNormThreads / kWave; ++w) sum += of_wave[w];
-        part[static_cast<int64_t>(blockIdx.y) * gridDim.x + blockIdx.x] = sum;
-    }
-}
-
-// v as planes of float16 parts
+// v as a sum of float16 parts, in kPl planes
 template <int kPl>
-__device__ __forceinline__ void split_half(float v, Half (&parts)[kPl]) {
+__device__ __forceinline__ void store_parts(Half* out, int64_t plane, const float (&v)[8]) {
+    float left[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) left[e] = v[e];
 #pragma unroll
     for (int p = 0; p < kPl; ++p) {
-        parts[p] = static_cast<Half>(v);
-        v -= static_cast<float>(parts[p]);
+        Half8 part;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            part[e] = static_cast<Half>(left[e]);
+            left[e] -= static_cast<float>(part[e]);
+        }
+        *reinterpret_cast<Half8*>(out + p * plane) = part;
     }
 }
 
-// 64 x 64 of X: from x, or from its transposed.
-template <typename T>
-__global__ __launch_bounds__(256) void start_kernel(const T* __restrict__ x, const double* __restrict__ part, int parts, float* __restrict__ held,
-                                                    Half* __restrict__ planes, int64_t plane, Matrices s) {
-    constexpr int kPl = kUpdatePlanes<T>;
+// ---- norm and start ----
+
+__device__ __forceinline__ double add_over_threads(double v) {
+    __shared__ double of_wave[kThreads / kWave];
+#pragma unroll
+    for (int i = 32; i > 0; i >>= 1) v += __shfl_xor(v, i);
+    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0;
+    for (int w = 0; w < kThreads / kWave; ++w) v += of_wave[w];
+    return v;
+}
+
+// The sum of squares of `rows_each` rows, in double: the squares of float32 and bfloat16 values are more than float32 holds.
+template <typename T, int kWidth>
+__global__ __launch_bounds__(kThreads) void squares_kernel(const T* __restrict__ x, double* __restrict__ part, int64_t rows, int64_t cols,
+                                                           int64_t rows_each, int64_t parts, Matrices s) {
+    if (block_id() >= parts * s.batch) return;
+    const int64_t matrix = block_id() / parts, first = (block_id() - matrix * parts) * rows_each;
+    const int64_t chunks = cols / kWidth, items = (min(first + rows_each, rows) - first) * chunks;
+    const T* const from = x + matrix * s.in_batch + first * s.in_stride;
+    double sum = 0.0;
+    for (int64_t i = threadIdx.x; i < items; i += kThreads) {
+        const int64_t r = i / chunks;
+        float v[kWidth];
+        load_as_float<T, kWidth>(from + r * s.in_stride + (i - r * chunks) * kWidth, v);
+#pragma unroll
+        for (int e = 0; e < kWidth; ++e) sum = fma(static_cast<double>(v[e]), static_cast<double>(v[e]), sum);
+    }
+    sum = add_over_threads(sum);
+    if (threadIdx.x == 0) part[block_id()] = sum;
+}
+
+// 64 x 64 of X: from x, or from its transposed. kWide: x's rows are whole chunks of 8.
+template <typename T, bool kWide>
+__global__ __launch_bounds__(kThreads) void start_kernel(const T* __restrict__ x, const double* __restrict__ part, int64_t parts,
+                                                         Half* __restrict__ planes, int64_t plane, int64_t m_tiles, int64_t n_tiles, Matrices s) {
     __shared__ float tile[64][65];
-    const int64_t matrix = blockIdx.z, i0 = static_cast<int64_t>(blockIdx.y) * 64, j0 = static_cast<int64_t>(blockIdx.x) * 64;
+    if (block_id() >= m_tiles * n_tiles * s.batch) return;
+    const int64_t matrix = block_id() / (m_tiles * n_tiles), in_matrix = block_id() - matrix * m_tiles * n_tiles;
+    const int64_t i0 = in_matrix / n_tiles * 64, j0 = in_matrix % n_tiles * 64;
     double squares = 0.0;
-    for (int p = 0; p < parts; ++p) squares += part[matrix * parts + p];
-    const double norm = sqrt(squares) + s.eps;
+    for (int64_t p = threadIdx.x; p < parts; p += kThreads) squares += part[matrix * parts + p];
+    const double norm = sqrt(add_over_threads(squares)) + s.eps;
+    // the quotient's rounding is of X as a whole, which the steps forgive; a norm below float32's range, or above it, is not
+    const double inverse = 1.0 / norm;
     const T* const from = x + matrix * s.in_batch;
-    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-        const int slow = e >> 6, fast = e & 63;
-        const int64_t i = i0 + (s.turned ? fast : slow), j = j0 + (s.turned ? slow : fast);
-        float v = 0.0f;
-        if (i < s.m && j < s.n)
-            v = static_cast<float>(static_cast<double>(static_cast<float>(from[s.turned ? j * s.in_stride + i : i * s.in_stride + j])) / norm);
-        tile[s.turned ? fast : slow][s.turned ? slow : fast] = v;
+    // rows and columns of x
+    const int64_t r0 = s.turned ? j0 : i0, c0 = s.turned ? i0 : j0, rows = s.turned ? s.n : s.m, cols = s.turned ? s.m : s.n;
+#pragma unroll
+    for (int e = threadIdx.x; e < 64 * 8; e += kThreads) {
+        const int r = e >> 3, c = (e & 7) * 8;
+        float v[8] = {};
+        if (r0 + r < rows) {
+            const T* const at = from + (r0 + r) * s.in_stride + c0 + c;
+            if constexpr (kWide) {
+                if (c0 + c < cols) {
+#pragma unroll
+                    for (int q = 0; q < 8; q += kChunk<T>) {
+                        float w[kChunk<T>];
+                        load_as_float<T, kChunk<T>>(at + q, w);
+#pragma unroll
+                        for (int u = 0; u < kChunk<T>; ++u) v[q + u] = w[u];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int u = 0; u < 8; ++u)
+                    if (c0 + c + u < cols) v[u] = static_cast<float>(at[u]);
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            const float w = static_cast<float>(static_cast<double>(v[u]) * inverse) * s.x_scale;
+            if (s.turned)
+                tile[c + u][r] = w;
+            else
+                tile[r][c + u] = w;
+        }
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < 64 * 64; e += 256) {
-        const int64_t i = i0 + (e >> 6), j = j0 + (e & 63);
-        if (i >= s.m || j >= s.n_padded) continue;
-        const float v = tile[e >> 6][e & 63];
-        const int64_t at = (matrix * s.m + i) * s.n_padded + j;
-        held[at] = v;
-        Half parts16[kPl];
-        split_half<kPl>(v * s.x_scale, parts16);
 #pragma unroll
-        for (int p = 0; p < kPl; ++p) planes[p * plane + at] = parts16[p];
+    for (int e = threadIdx.x; e < 64 * 8; e += kThreads) {
+        const int64_t i = i0 + (e >> 3), j = j0 + (e & 7) * 8;
+        if (i >= s.m || j >= s.n_padded) continue;
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = tile[e >> 3][(e & 7) * 8 + u];
+        store_parts<2>(planes + (matrix * s.m + i) * s.n_padded + j, plane, v);
     }
 }
 
 // steps 0: out = scale X
 template <typename T>
-__global__ __launch_bounds__(256) void no_steps_kernel(const float* __restrict__ held, T* __restrict__ out, Matrices s) {
+__global__ __launch_bounds__(kThreads) void no_steps_kernel(const Half* __restrict__ planes, int64_t plane, T* __restrict__ out, Matrices s) {
     const int64_t rows = s.turned ? s.n : s.m, cols = s.turned ? s.m : s.n, matrix = blockIdx.y;
-    for (int64_t e = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; e < rows * cols; e += static_cast<int64_t>(gridDim.x) * 256) {
-        const int64_t r = e / cols, c = e - r * cols, i = s.turned ? c : r, j = s.turned ? r : c;
-        out[matrix * s.out_batch + r * s.out_stride + c] = static_cast<T>(held[(matrix * s.m + i) * s.n_padded + j] * s.out_scale);
+    for (int64_t e = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; e < rows * cols; e += static_cast<int64_t>(gridDim.x) * kThreads) {
+        const int64_t r = e / cols, c = e - r * cols, i = s.turned ? c : r, j = s.turned ? r : c, at = (matrix * s.m + i) * s.n_padded + j;
+        const float v = static_cast<float>(planes[at]) + static_cast<float>(planes[plane + at]);
+        out[matrix * s.out_batch + r * s.out_stride + c] = static_cast<T>(v * (s.out_scale / s.x_scale));
     }
 }
 
 // ---- products ----
 
-// Workgroup id -> matrix and tile on or above the diagonal, an XCD's tiles contiguous.
-__device__ __forceinline__ void triangle_of(int64_t id, int64_t tiles, int64_t batch, int64_t& matrix, int64_t& m, int64_t& n) {
-    const int64_t each = tiles * (tiles + 1) / 2;
-    int64_t one, t;
-    tile_of(id, each * batch, 1, t, one);
-    matrix = t / each;
-    t -= matrix * each;
+// Index -> tile on or above the diagonal.
+__device__ __forceinline__ void triangle_of(int64_t t, int64_t& m, int64_t& n) {
     n = static_cast<int64_t>((sqrtf(8.0f * static_cast<float>(t) + 1.0f) - 1.0f) * 0.5f);
     while (n * (n + 1) / 2 > t) --n;
     while ((n + 1) * (n + 2) / 2 <= t) ++n;
@@ -139,103 +185,198 @@ __device__ __forceinline__ void triangle_of(int64_t id, int64_t tiles, int64_t b
 struct GramArgs {
     Matrices s;
     Operand of;  // both sides
-    int64_t k;
+    int64_t k, segment, segments;  // of k
     Half* out;
     int64_t out_plane;
     float factor;       // of the product
     const Half* first;  // with it, plus first_factor times this
     float first_factor;
+    float* part;  // [matrix][segment][m][m_padded]: a workgroup forms one segment; NULL: all in turn
 };
 
-// value at (i, j) of a symmetric matrix and, above the diagonal's tiles, at (j, i); zero in the padding
+// What a row's 8 values from column j on are added to.
 template <int kPl>
-__device__ __forceinline__ void store_plane_values(Half* out, int64_t plane, int64_t at, float v) {
-    Half parts[kPl];
-    split_half<kPl>(v, parts);
+struct Held {
+    Half8 part[kPl];
+};
+
+template <int kPl>
+__device__ __forceinline__ Held<kPl> hold_parts(const Half* from, int64_t plane, bool inside) {
+    Held<kPl> h;
 #pragma unroll
-    for (int p = 0; p < kPl; ++p) out[p * plane + at] = parts[p];
+    for (int p = 0; p < kPl; ++p) h.part[p] = inside ? *reinterpret_cast<const Half8*>(from + p * plane) : Half8{};
+    return h;
+}
+
+template <int kPl>
+__device__ __forceinline__ float value_of(const Held<kPl>& h, int e) {
+    float v = 0.0f;
+#pragma unroll
+    for (int p = kPl - 1; p >= 0; --p) v += static_cast<float>(h.part[p][e]);
+    return v;
+}
+
+template <int kPl>
+__device__ __forceinline__ Held<kPl> hold_gram(const GramArgs& a, int64_t base, int64_t i, int64_t j) {
+    return hold_parts<kPl>(a.first + base + i * a.s.m_padded + j, a.out_plane, a.first && i < a.s.m && j < a.s.m_padded);
+}
+
+// 8 values of row i from column j on, finished; zero in the padding
+template <int kPl>
+__device__ __forceinline__ void finish_gram(const GramArgs& a, int64_t base, int64_t i, int64_t j, float (&v)[8], const Held<kPl>& first) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        v[e] *= a.factor;
+        if (a.first) v[e] = fmaf(a.first_factor, value_of(first, e), v[e]);
+        if (i >= a.s.m || j + e >= a.s.m) v[e] = 0.0f;
+    }
+    if (i < a.s.m && j < a.s.m_padded) store_parts<kPl>(a.out + base + i * a.s.m_padded + j, a.out_plane, v);
 }
 
 template <typename T, typename Tile>
 __global__ __launch_bounds__(Tile::kThreads) void gram_kernel(GramArgs a, int64_t tiles) {
-    constexpr int kPl = kUpdatePlanes<T>;
+    constexpr int kPl = kProductPlanes<T>;
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
-    int64_t matrix, m, n;
-    triangle_of(blockIdx.x, tiles, a.s.batch, matrix, m, n);
-    typename Tile::Sums acc;
-    Tile::run(a.of, a.of, m * Tile::kM, n * Tile::kN, a.s.m, a.s.m, a.k, matrix, matrix, (LdsByte*)lds, acc);
+    const int64_t each = tiles * (tiles + 1) / 2, at_once = a.part ? a.segments : 1, total = each * a.s.batch * at_once;
+    if (block_id() >= total) return;
+    int64_t id, one, m, n;
+    tile_of(block_id(), total, 1, id, one);
+    const int64_t matrix = id / (each * at_once), in_matrix = id - matrix * each * at_once, only = in_matrix / each;
+    triangle_of(in_matrix - only * each, m, n);
     const int64_t i0 = m * Tile::kM + Tile::wave_m(), j0 = n * Tile::kN + Tile::wave_n(), base = matrix * a.s.m * a.s.m_padded;
-    Half* const out = a.out + base;
+    typename Tile::Sums acc;
+    if (a.part) {
+        Operand of = a.of;
+        of.base += only * a.segment * 2;
+        Tile::run(of, of, m * Tile::kM, n * Tile::kN, a.s.m, a.s.m, min(a.segment, a.k - only * a.segment), matrix, matrix, (LdsByte*)lds, acc);
+        float* const part = a.part + (matrix * a.segments + only) * a.s.m * a.s.m_padded;
+        by_rows<Tile>(acc, (LdsByte*)lds, [](int, int) { return Nothing{}; }, [&](int row, int column, float (&v)[8], Nothing) {
+            const int64_t i = i0 + row, j = j0 + column;
+            if (i < a.s.m && j < a.s.m_padded) store_from_float<float, 8>(part + i * a.s.m_padded + j, v);
+        });
+        return;
+    }
+    Tile::template run<true>(a.of, a.of, m * Tile::kM, n * Tile::kN, a.s.m, a.s.m, a.k, matrix, matrix, (LdsByte*)lds, acc, a.segment);
+    by_rows_and_columns<Tile>(
+        acc, (LdsByte*)lds, m != n, [&](int row, int column) { return hold_gram<kPl>(a, base, i0 + row, j0 + column); },
+        [&](int row, int column, float (&v)[8], const Held<kPl>& first) { finish_gram<kPl>(a, base, i0 + row, j0 + column, v, first); },
+        [&](int row, int column, float (&v)[8]) {
+            const int64_t i = i0 + row, j = j0 + column;
+            if (j < a.s.m && i < a.s.m_padded) store_parts<kPl>(a.out + base + j * a.s.m_padded + i, a.out_plane, v);
+        });
+}
+
+// Adds the segments' parts in order: 64 x 64 on or above the diagonal, of the `tiles` tiles of kTile that the parts were formed in.
+template <typename T, int kTile>
+__global__ __launch_bounds__(kThreads) void join_segments_kernel(GramArgs a, int64_t tiles) {
+    constexpr int kPl = kProductPlanes<T>, kSub = kTile / 64;
+    __shared__ float tile[64][65];
+    const int64_t each = tiles * (tiles + 1) / 2 * kSub * kSub;
+    if (block_id() >= each * a.s.batch) return;
+    const int64_t matrix = block_id() / each, id = block_id() - matrix * each;
+    const int sub = static_cast<int>(id % (kSub * kSub));
+    int64_t m, n;
+    triangle_of(id / (kSub * kSub), m, n);
+    const int64_t i0 = m * kTile + sub / kSub * 64, j0 = n * kTile + sub % kSub * 64, base = matrix * a.s.m * a.s.m_padded;
+    const int64_t next = a.s.m * a.s.m_padded;
 #pragma unroll
-    for (int bi = 0; bi < Tile::kBlocksM; ++bi)
+    for (int e = threadIdx.x; e < 64 * 8; e += kThreads) {
+        const int64_t i = i0 + (e >> 3), j = j0 + (e & 7) * 8;
+        float v[8] = {};
+        if (i < a.s.m && j < a.s.m_padded) {
+            const float* from = a.part + matrix * a.segments * next + i * a.s.m_padded + j;
+            load_as_float<float, 8>(from, v);
+            for (int64_t which = 1; which < a.segments; ++which) {
+                float w[8];
+                load_as_float<float, 8>(from + which * next, w);
 #pragma unroll
-        for (int bj = 0; bj < Tile::kBlocksN; ++bj) {
-            const int64_t j = j0 + 32 * bj + lane_column();
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t i = i0 + 32 * bi + block_row(r), at = i * a.s.m_padded + j;
-                const bool inside = i < a.s.m && j < a.s.m;
-                float v = inside ? acc[bi][bj][r] * a.factor : 0.0f;
-                if (a.first && inside) {
-                    float w = 0.0f;
-#pragma unroll
-                    for (int p = kPl - 1; p >= 0; --p) w += static_cast<float>(a.first[base + p * a.out_plane + at]);
-                    v = fmaf(a.first_factor, w, v);
-                }
-                if (i < a.s.m && j < a.s.m_padded) store_plane_values<kPl>(out, a.out_plane, at, v);
-                if (m != n && j < a.s.m && i < a.s.m_padded) store_plane_values<kPl>(out, a.out_plane, j * a.s.m_padded + i, v);
+                for (int u = 0; u < 8; ++u) v[u] += w[u];
             }
         }
+        finish_gram<kPl>(a, base, i, j, v, hold_gram<kPl>(a, base, i, j));
+#pragma unroll
+        for (int u = 0; u < 8; ++u) tile[(e & 7) * 8 + u][e >> 3] = v[u];
+    }
+    if (m == n) return;
+    __syncthreads();
+#pragma unroll
+    for (int e = threadIdx.x; e < 64 * 8; e += kThreads) {
+        const int64_t j = j0 + (e >> 3), i = i0 + (e & 7) * 8;
+        if (j >= a.s.m || i >= a.s.m_padded) continue;
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = tile[e >> 3][(e & 7) * 8 + u];
+        store_parts<kPl>(a.out + base + j * a.s.m_padded + i, a.out_plane, v);
+    }
 }
 
 struct UpdateArgs {
     Matrices s;
     Operand left, x;
-    float* held;
-    Half* planes;  // of the new X; NULL in the last step
+    const Half* from;  // X's planes
+    Half* to;          // the new X's; NULL in the last step
     int64_t plane;
     float keep, factor;
+    bool whole;  // the result's rows are whole chunks of 8
 };
+
+template <typename T>
+__device__ __forceinline__ void store_result(T* to, int64_t left, bool whole, const float (&v)[8]) {
+    if (whole) {
+        if (left <= 0) return;
+        if constexpr (sizeof(T) == 4) {
+            *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+            *reinterpret_cast<float4*>(to + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+            store_from_float<T, 8>(to, v);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            if (e < left) to[e] = static_cast<T>(v[e]);
+    }
+}
 
 template <typename T, typename Tile>
 __global__ __launch_bounds__(Tile::kThreads) void update_kernel(T* __restrict__ result, UpdateArgs a, int64_t m_tiles, int64_t n_tiles) {
-    constexpr int kPl = kUpdatePlanes<T>;
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
+    if (block_id() >= m_tiles * n_tiles * a.s.batch) return;
     int64_t m, n;
-    tile_of(blockIdx.x, m_tiles, n_tiles * a.s.batch, m, n);
+    tile_of(block_id(), m_tiles, n_tiles * a.s.batch, m, n);
     const int64_t matrix = n / n_tiles;
     n -= matrix * n_tiles;
     typename Tile::Sums acc;
     Tile::run(a.left, a.x, m * Tile::kM, n * Tile::kN, a.s.m, a.s.n_padded, a.s.m, matrix, matrix, (LdsByte*)lds, acc);
     const int64_t i0 = m * Tile::kM + Tile::wave_m(), j0 = n * Tile::kN + Tile::wave_n();
+    T* const out = result + matrix * a.s.out_batch;
+    by_rows_and_columns<Tile>(
+        acc, (LdsByte*)lds, !a.to && a.s.turned,
+        [&](int row, int column) {
+            const int64_t i = i0 + row, j = j0 + column;
+            return hold_parts<2>(a.from + (matrix * a.s.m + i) * a.s.n_padded + j, a.plane, i < a.s.m && j < a.s.n_padded);
+        },
+        [&](int row, int column, float (&v)[8], const Held<2>& x) {
+            const int64_t i = i0 + row, j = j0 + column;
+            if (i >= a.s.m || j >= a.s.n_padded) return;
 #pragma unroll
-    for (int bi = 0; bi < Tile::kBlocksM; ++bi)
-#pragma unroll
-        for (int bj = 0; bj < Tile::kBlocksN; ++bj) {
-            const int64_t j = j0 + 32 * bj + lane_column();
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const int64_t i = i0 + 32 * bi + block_row(r);
-                if (i >= a.s.m || j >= a.s.n_padded) continue;
-                const int64_t at = (matrix * a.s.m + i) * a.s.n_padded + j;
-                const float v = fmaf(a.keep, a.held[at], acc[bi][bj][r] * a.factor);
-                if (a.planes) {
-                    a.held[at] = v;
-                    store_plane_values<kPl>(a.planes, a.plane, at, v * a.s.x_scale);
-                } else if (j < a.s.n) {
-                    const int64_t to = a.s.turned ? j * a.s.out_stride + i : i * a.s.out_stride + j;
-                    result[matrix * a.s.out_batch + to] = static_cast<T>(v * a.s.out_scale);
-                }
-            }
-        }
+            for (int e = 0; e < 8; ++e) v[e] = fmaf(a.keep, value_of(x, e), v[e] * a.factor);
+            if (a.to)
+                store_parts<2>(a.to + (matrix * a.s.m + i) * a.s.n_padded + j, a.plane, v);
+            else if (!a.s.turned)
+                store_result(out + i * a.s.out_stride + j, a.s.n - j, a.whole, v);
+        },
+        [&](int row, int column, float (&v)[8]) {
+            const int64_t i = i0 + row, j = j0 + column;
+            if (j < a.s.n) store_result(out + j * a.s.out_stride + i, a.s.m - i, a.whole, v);
+        });
 }
 
 // ---- the call ----
 
-template <typename T, int kSize>
-using GramTile = TileProduct<Half, kUpdatePlanes<T>, kSize, kSize, 2, kSize / 64, false, false>;
-template <typename T, int kSize>
-using UpdateTile = TileProduct<Half, kUpdatePlanes<T>, kSize, kSize, 2, kSize / 64, false, true>;
+template <typename T, int kSize, int kStages>
+using GramTile = TileProduct<Half, kProductPlanes<T>, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, false, 64, kStages>;
+template <typename T, int kSize, int kStages>
+using UpdateTile = TileProduct<Half, kProductPlanes<T>, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, true, 64, kStages>;
 
 Matrices matrices_of(const dllm_hip_orthogonalize_shape& sh) {
     Matrices s;
@@ -253,69 +394,132 @@ Matrices matrices_of(const dllm_hip_orthogonalize_shape& sh) {
     return s;
 }
 
+int64_t triangle(const Matrices& s, int64_t size) {
+    const int64_t t = ceil_div(s.m, size);
+    return t * (t + 1) / 2;
+}
+
+// Of k: what one matrix's tiles of 128 need to be about 512 workgroups, at least 1024 k each. It goes by the matrix's size alone.
+int64_t segment_of(const Matrices& s, int64_t k) {
+    const int64_t segments = std::clamp<int64_t>(512 / triangle(s, 128), 1, std::max<int64_t>(k / 1024, 1));
+    return static_cast<int64_t>(round_up(ceil_div(k, segments), 64));
+}
+
+// Segments are formed at once where the matrices' tiles do not fill the CUs.
+bool segments_at_once(const Matrices& s, int64_t k) { return segment_of(s, k) < k && triangle(s, 128) * s.batch < 384; }
+
+int64_t norm_rows(const dllm_hip_orthogonalize_shape& sh) {
+    return std::max<int64_t>({kNormElements / sh.cols, static_cast<int64_t>(ceil_div(sh.rows, kNormParts)), 1});
+}
+
 struct UpdateLayout {
-    size_t norm, held, planes, gram, bytes;
-    UpdateLayout(const Matrices& s, int64_t dtype) {
-        const size_t pl = dtype == kFloat32 ? 2 : 1;
-        norm = static_cast<size_t>(s.batch) * kNormParts;
-        held = static_cast<size_t>(s.batch) * s.m * s.n_padded;
-        planes = pl * held;
-        gram = pl * s.batch * s.m * s.m_padded;
+    size_t norm, planes, gram, part, bytes;
+    UpdateLayout(const dllm_hip_orthogonalize_shape& sh, const Matrices& s) {
+        norm = static_cast<size_t>(s.batch) * ceil_div(sh.rows, norm_rows(sh));
+        planes = 2 * static_cast<size_t>(s.batch) * s.m * s.n_padded;
+        gram = static_cast<size_t>(sh.dtype == kFloat32 ? 2 : 1) * s.batch * s.m * s.m_padded;
+        part = 0;
+        for (const int64_t k : {s.n_padded, s.m})
+            if (segments_at_once(s, k)) part = std::max(part, static_cast<size_t>(s.batch) * ceil_div(k, segment_of(s, k)) * s.m * s.m_padded);
         Layout l;
         l.add<double>(norm);
-        l.add<float>(held);
         for (const size_t n : {planes, planes, gram, gram}) l.add<Half>(n);
+        l.add<float>(part);
         bytes = l.bytes;
     }
 };
 
 struct UpdateBuffers {
     double* norm;
-    float* held;
     Half *planes[2], *gram, *left;
+    float* part;
 };
 
-template <typename T, int kSize>
+template <typename T, typename Tile>
+void launch_gram_tiles(const GramArgs& g, bool at_once, hipStream_t stream) {
+    constexpr int kSize = Tile::kM;
+    const int64_t tiles = ceil_div(g.s.m, kSize), all = triangle(g.s, kSize) * g.s.batch;
+    gram_kernel<T, Tile><<<grid_of(all * (at_once ? g.segments : 1)), Tile::kThreads, 0, stream>>>(g, tiles);
+    if (at_once) join_segments_kernel<T, kSize><<<grid_of(all * (kSize / 64) * (kSize / 64)), kThreads, 0, stream>>>(g, tiles);
+}
+
+// Tiles of 128 where they are enough for the CUs, else of 64 with more of their copies under way: a lone workgroup on a CU waits for
+// them. (192 x 576 in float32: 16 us for X X^T with four stages of 64 x 64 tiles, 29 with two of 128 x 128.)
+template <typename T>
+void launch_gram(GramArgs g, float* part, hipStream_t stream) {
+    g.segment = segment_of(g.s, g.k), g.segments = ceil_div(g.k, g.segment);
+    const bool at_once = segments_at_once(g.s, g.k);
+    g.part = at_once ? part : nullptr;
+    const int64_t blocks = triangle(g.s, 128) * g.s.batch * (at_once ? g.segments : 1);
+    if (blocks >= 200) {
+        launch_gram_tiles<T, GramTile<T, 128, 2>>(g, at_once, stream);
+    } else if (triangle(g.s, 64) * g.s.batch * (at_once ? g.segments : 1) > 256) {
+        launch_gram_tiles<T, GramTile<T, 64, 4>>(g, at_once, stream);
+    } else {
+        launch_gram_tiles<T, GramTile<T, 64, 8>>(g, at_once, stream);
+    }
+}
+
+template <typename T, typename Tile>
+void launch_update(const UpdateArgs& u, T* out, hipStream_t stream) {
+    const int64_t m = ceil_div(u.s.m, Tile::kM), n = ceil_div(u.s.n, Tile::kN);
+    update_kernel<T, Tile><<<grid_of(m * n * u.s.batch), Tile::kThreads, 0, stream>>>(out, u, m, n);
+}
+
+template <typename T>
 int launch_step(const Matrices& s, const UpdateBuffers& b, const double* c, int from, bool last, T* out, hipStream_t stream) {
-    constexpr int kPl = kUpdatePlanes<T>;
-    using Gram = GramTile<T, kSize>;
-    using Update = UpdateTile<T, kSize>;
     const int64_t plane = s.batch * s.m * s.n_padded, gram_plane = s.batch * s.m * s.m_padded;
     const Operand x{reinterpret_cast<const char*>(b.planes[from]), s.n_padded * 2, plane * 2, s.m * s.n_padded * 2, s.m};
-    const int64_t tiles = ceil_div(s.m, kSize), each = tiles * (tiles + 1) / 2;
-    const dim3 grid(static_cast<unsigned>(each * s.batch));
     GramArgs g{};
     g.s = s, g.of = x, g.k = s.n_padded, g.out = b.gram, g.out_plane = gram_plane, g.factor = kGramScale / (s.x_scale * s.x_scale);
-    gram_kernel<T, Gram><<<grid, Gram::kThreads, 0, stream>>>(g, tiles);
+    launch_gram<T>(g, b.part, stream);
     const Operand gram{reinterpret_cast<const char*>(b.gram), s.m_padded * 2, gram_plane * 2, s.m * s.m_padded * 2, s.m};
     g.of = gram, g.k = s.m, g.out = b.left, g.factor = static_cast<float>(c[2]) / kGramScale, g.first = b.gram, g.first_factor = static_cast<float>(c[1]);
-    gram_kernel<T, Gram><<<grid, Gram::kThreads, 0, stream>>>(g, tiles);
+    launch_gram<T>(g, b.part, stream);
     UpdateArgs u{};
     u.s = s, u.left = gram, u.left.base = reinterpret_cast<const char*>(b.left), u.x = x;
-    u.held = b.held, u.planes = last ? nullptr : b.planes[1 - from], u.plane = plane;
-    u.keep = static_cast<float>(c[0]), u.factor = 1.0f / (kGramScale * s.x_scale);
-    const int64_t n_tiles = ceil_div(s.n, kSize);
-    update_kernel<T, Update><<<static_cast<unsigned>(tiles * n_tiles * s.batch), Update::kThreads, 0, stream>>>(out, u, tiles, n_tiles);
-    (void)kPl;
+    u.from = b.planes[from], u.to = last ? nullptr : b.planes[1 - from], u.plane = plane;
+    // the last step's result leaves the planes' scale
+    const float unit = last ? s.out_scale / s.x_scale : 1.0f;
+    u.keep = static_cast<float>(c[0]) * unit, u.factor = unit / kGramScale;
+    const int64_t length = s.turned ? s.m : s.n;
+    u.whole = length % 8 == 0 && s.out_stride % 8 == 0 && s.out_batch % 8 == 0 && aligned_to(out, 16);
+    const int64_t large = ceil_div(s.m, 256) * ceil_div(s.n, 256) * s.batch, middle = ceil_div(s.m, 128) * ceil_div(s.n, 128) * s.batch;
+    if (middle < 256 && ceil_div(s.m, 64) * ceil_div(s.n, 64) * s.batch <= 256)
+        launch_update<T, UpdateTile<T, 64, 8>>(u, out, stream);
+    else if (middle < 256)
+        launch_update<T, UpdateTile<T, 64, 4>>(u, out, stream);
+    else if (ceil_div(large, 256) * 2 <= ceil_div(middle, 512))
+        launch_update<T, UpdateTile<T, 256, 2>>(u, out, stream);
+    else
+        launch_update<T, UpdateTile<T, 128, 2>>(u, out, stream);
     return check_launch("orthogonalize");
 }
 
 template <typename T>
 int run(const dllm_hip_orthogonalize_shape& sh, const Matrices& s, const double* coefficients, const T* x, T* out, const UpdateBuffers& b,
         hipStream_t stream) {
-    const int parts = static_cast<int>(std::min<int64_t>(kNormParts, sh.rows));
-    squares_kernel<T><<<dim3(parts, static_cast<unsigned>(s.batch)), kNormThreads, 0, stream>>>(x, b.norm, sh.rows, sh.cols, s);
-    const dim3 tiles(static_cast<unsigned>(ceil_div(s.n_padded, 64)), static_cast<unsigned>(ceil_div(s.m, 64)), static_cast<unsigned>(s.batch));
-    start_kernel<T><<<tiles, 256, 0, stream>>>(x, b.norm, parts, b.held, b.planes[0], s.batch * s.m * s.n_padded, s);
+    const int64_t parts = ceil_div(sh.rows, norm_rows(sh)), plane = s.batch * s.m * s.n_padded;
+    constexpr int kWide = kChunk<T>;
+    const bool chunks = sh.cols % kWide == 0 && s.in_stride % kWide == 0 && s.in_batch % kWide == 0 && aligned_to(x, 16);
+    if (chunks)
+        squares_kernel<T, kWide><<<grid_of(parts * s.batch), kThreads, 0, stream>>>(x, b.norm, sh.rows, sh.cols, norm_rows(sh), parts, s);
+    else
+        squares_kernel<T, 1><<<grid_of(parts * s.batch), kThreads, 0, stream>>>(x, b.norm, sh.rows, sh.cols, norm_rows(sh), parts, s);
+    const int64_t m_tiles = ceil_div(s.m, 64), n_tiles = ceil_div(s.n_padded, 64);
+    if (chunks && sh.cols % 8 == 0)
+        start_kernel<T, true><<<grid_of(m_tiles * n_tiles * s.batch), kThreads, 0, stream>>>(x, b.norm, parts, b.planes[0], plane, m_tiles, n_tiles, s);
+    else
+        start_kernel<T, false><<<grid_of(m_tiles * n_tiles * s.batch), kThreads, 0, stream>>>(x, b.norm, parts, b.planes[0], plane, m_tiles, n_tiles, s);
     if (sh.steps == 0) {
-        const size_t blocks = std::min<size_t>(ceil_div(s.m * s.n, 256), 4096);
-        no_steps_kernel<T><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(s.batch)), 256, 0, stream>>>(b.held, out, s);
+        const size_t blocks = std::min<size_t>(ceil_div(s.m * s.n, kThreads), 4096);
+        no_steps_kernel<T><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(s.batch)), kThreads, 0, stream>>>(b.planes[0], plane, out, s);
         return check_launch("orthogonalize");
     }
     static constexpr double kQuintic[3] = {3.4445, -4.7750, 2.0315};
     for (int64_t i = 0; i < sh.steps; ++i) {
         const double* const c = coefficients ? coefficients + 3 * i : kQuintic;
-        DLLM_TRY((launch_step<T, 128>(s, b, c, static_cast<int>(i % 2), i == sh.steps - 1, out, stream)));
+        DLLM_TRY(launch_step<T>(s, b, c, static_cast<int>(i % 2), i == sh.steps - 1, out, stream));
     }
     return kOk;
 }
@@ -335,9 +539,8 @@ int check_shape(const dllm_hip_orthogonalize_shape* sh) {
         DLLM_REQUIRE(row <= INT64_MAX / (1 << 17), "a row stride is too large");
         DLLM_REQUIRE(s[1] == 0 || s[1] >= (sh->rows - 1) * row + sh->cols, "a batch stride must be 0 or at least a matrix");
     }
-    // a grid's x extent times its workgroup is below 2^32
-    const int64_t tiles = ceil_div(sh->rows, 128) * ceil_div(sh->cols, 128) + ceil_div(std::min(sh->rows, sh->cols), 128);
-    DLLM_REQUIRE(tiles * sh->batch < (1 << 23), "too many matrices for one call");
+    // (the workspace of more is no size that a GPU has)
+    DLLM_REQUIRE(sh->batch * sh->rows * sh->cols < (int64_t{1} << 40), "too many matrices for one call");
     return kOk;
 }
 
@@ -346,7 +549,7 @@ int check_shape(const dllm_hip_orthogonalize_shape* sh) {
 extern "C" {
 
 size_t dllm_hip_orthogonalize_workspace(const dllm_hip_orthogonalize_shape* sh) {
-    return check_shape(sh) == kOk ? UpdateLayout(matrices_of(*sh), sh->dtype).bytes : 0;
+    return check_shape(sh) == kOk ? UpdateLayout(*sh, matrices_of(*sh)).bytes : 0;
 }
 
 int dllm_hip_orthogonalize(const dllm_hip_orthogonalize_shape* sh, const double* coefficients, const void* x, void* out, void* workspace,
@@ -361,17 +564,17 @@ int dllm_hip_orthogonalize(const dllm_hip_orthogonalize_shape* sh, const double*
             DLLM_REQUIRE(std::isfinite(static_cast<float>(coefficients[i])), "coefficients must be finite in float32");
     const Matrices s = matrices_of(*sh);
     DLLM_REQUIRE(x != out || (s.in_stride == s.out_stride && s.in_batch == s.out_batch), "in place needs equal strides");
-    const UpdateLayout layout(s, sh->dtype);
+    const UpdateLayout layout(*sh, s);
     DLLM_REQUIRE(workspace && workspace_bytes >= layout.bytes, "workspace too small for orthogonalize");
     DLLM_REQUIRE(aligned_to(workspace, 16), "the workspace must be aligned to 16 bytes");
     Carve c(workspace, workspace_bytes);
     UpdateBuffers b;
     b.norm = c.take<double>(layout.norm);
-    b.held = c.take<float>(layout.held);
     b.planes[0] = c.take<Half>(layout.planes);
     b.planes[1] = c.take<Half>(layout.planes);
     b.gram = c.take<Half>(layout.gram);
     b.left = c.take<Half>(layout.gram);
+    b.part = c.take<float>(layout.part);
     auto st = static_cast<hipStream_t>(stream);
     switch (sh->dtype) {
         case kFloat32: return run<float>(*sh, s, coefficients, static_cast<const float*>(x), static_cast<float*>(out), b, st);

@@ -174,31 +174,48 @@ struct TileProduct {
     static __device__ __forceinline__ int wave_m() { return wave() / kWavesN * kWaveM; }
     static __device__ __forceinline__ int wave_n() { return wave() % kWavesN * kWaveN; }
 
-    // acc = the tile at (m0, n0); all of m0 < a_count, n0 < b_count. LDS: kLds bytes.
+    // acc = the tile at (m0, n0); all of m0 < a_count, n0 < b_count. LDS: kLds bytes. kSegments: k is summed in segments of `segment`
+    // (a multiple of kTileK), each from zero, which are added in order.
+    template <bool kSegments = false>
     static __device__ __forceinline__ void run(const Operand& a, const Operand& b, int64_t m0, int64_t n0, int64_t a_count, int64_t b_count,
-                                               int64_t k, int64_t batch_a, int64_t batch_b, LdsByte* lds, Sums& acc) {
+                                               int64_t k, int64_t batch_a, int64_t batch_b, LdsByte* lds, Sums& acc, int64_t segment = 0) {
+        constexpr int kPairs = PlanePairs<kPlanesOf>::kCount;
         ATile at;
         BTile bt;
         at.init(a, m0, a_count, batch_a);
         bt.init(b, n0, b_count, batch_b);
         const OperandView<kM, kTileK, kAColumns> av(wave_m());
         const OperandView<kN, kTileK, kBColumns> bv(wave_n());
+        const auto clear = [&] {
 #pragma unroll
-        for (int i = 0; i < kBlocksM; ++i)
+            for (int i = 0; i < kBlocksM; ++i)
 #pragma unroll
-            for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Acc{};
-        const int tiles = static_cast<int>((k + kTileK - 1) / kTileK), count = tiles * PlanePairs<kPlanesOf>::kCount;
+                for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Acc{};
+        };
+        clear();
+        const int tiles = static_cast<int>((k + kTileK - 1) / kTileK), count = tiles * kPairs;
         if (count == 0) return;
-        int pair = 0, tile = 0, into = 0;  // of the next copy
+        const int segment_tiles = kSegments ? static_cast<int>(segment / kTileK) : tiles;
+        int pair = 0, tile = 0, into = 0, first = 0, end = min(segment_tiles, tiles);  // of the next copy; first, end: of its segment
         auto copy = [&] {
             LdsByte* const to = lds + into * kStage;
             at.copy(static_cast<int64_t>(tile) * kTileK, k, PlanePairs<kPlanesOf>::a(pair), to);
             bt.copy(static_cast<int64_t>(tile) * kTileK, k, PlanePairs<kPlanesOf>::b(pair), to + ATile::kBytes);
-            if (++tile == tiles) tile = 0, ++pair;
+            if (++tile == end) {
+                if (++pair == kPairs && kSegments) pair = 0, first = end, end = min(end + segment_tiles, tiles);
+                tile = first;
+            }
             into = into + 1 == kStages ? 0 : into + 1;
         };
         for (int i = 0; i < kStages - 1 && i < count; ++i) copy();
-        int from = 0;
+        int from = 0, boundary = segment_tiles * kPairs;
+        Sums total;
+        if constexpr (kSegments) {
+#pragma unroll
+            for (int i = 0; i < kBlocksM; ++i)
+#pragma unroll
+                for (int j = 0; j < kBlocksN; ++j) total[i][j] = Acc{};
+        }
         for (int i = 0; i < count; ++i) {
             // stage i has arrived, and the one that the next copy goes to is read
             if (kStages > 2 && i + kStages - 2 < count)
@@ -206,6 +223,14 @@ struct TileProduct {
             else
                 stage_barrier<0>();
             if (i + kStages - 1 < count) copy();
+            if (kSegments && i == boundary) {
+                boundary += segment_tiles * kPairs;
+#pragma unroll
+                for (int m = 0; m < kBlocksM; ++m)
+#pragma unroll
+                    for (int n = 0; n < kBlocksN; ++n) total[m][n] += acc[m][n];
+                clear();
+            }
             const LdsByte* const stage = lds + from * kStage;
             from = from + 1 == kStages ? 0 : from + 1;
 #pragma unroll
@@ -221,6 +246,12 @@ struct TileProduct {
                     for (int n = 0; n < kBlocksN; ++n) multiply<P>(x[m], y[n], acc[m][n]);
             }
         }
+        if constexpr (kSegments) {
+#pragma unroll
+            for (int m = 0; m < kBlocksM; ++m)
+#pragma unroll
+                for (int n = 0; n < kBlocksN; ++n) acc[m][n] = total[m][n] + acc[m][n];
+        }
     }
 };
 
@@ -232,37 +263,68 @@ __device__ __forceinline__ int block_row(int r) { return 8 * (r >> 2) + 4 * lane
 
 // A wave's sums by rows: f(row, column, v) with 8 consecutive columns' sums in each lane (row and column within the wave's part), for
 // wide stores. The blocks go through LDS, 32 rows at a time; its 16-byte chunks lie at places that keep both ways free of
-// conflicts on the 64 banks.
-template <typename Tile, typename F>
-__device__ __forceinline__ void by_rows(const typename Tile::Sums& acc, LdsByte* lds, F&& f) {
+// conflicts on the 64 banks. What f reads from memory is read by load(row, column), for a block at once and ahead of its way
+// through LDS, and handed to f. With columns, what f leaves in v goes by columns to g(row, column, v) with 8 consecutive rows of
+// one column.
+template <typename Tile, typename L, typename F, typename G>
+__device__ __forceinline__ void by_rows_and_columns(const typename Tile::Sums& acc, LdsByte* lds, bool columns, L&& load, F&& f, G&& g) {
     constexpr int kColumns = Tile::kWaveN, kRowBytes = kColumns * 4, kLanes = kColumns / 8, kRowsAtOnce = kWave / kLanes;
-    static_assert(Tile::kThreads / kWave * 32 * kRowBytes <= Tile::kLds);
+    static_assert(Tile::kThreads / kWave * 32 * kRowBytes <= Tile::kLds && (kColumns == 64 || kColumns == 32));
     using Four = float __attribute__((ext_vector_type(4)));
+    using LdsFour = __attribute__((address_space(3))) Four;
+    using LdsFloat = __attribute__((address_space(3))) float;
     const int lane = static_cast<int>(threadIdx.x) & 63;
     LdsByte* const area = lds + Tile::wave() * 32 * kRowBytes;
     const auto at = [](int row, int chunk) { return row * kRowBytes + ((chunk ^ (kColumns >= 64 ? ((row >> 2) & 1) << 3 | (row & 1) : row & 1)) << 4); };
+    constexpr int kTurns = 32 / kRowsAtOnce;
+    decltype(load(0, 0)) held[kTurns];
+    const auto load_block = [&](int i) {
+#pragma unroll
+        for (int t = 0; t < kTurns; ++t) held[t] = load(32 * i + t * kRowsAtOnce + lane / kLanes, lane % kLanes * 8);
+    };
+    load_block(0);
     __syncthreads();  // the products' stages are read
 #pragma unroll
     for (int i = 0; i < Tile::kBlocksM; ++i) {
+        if (i > 0) load_block(i);
 #pragma unroll
         for (int j = 0; j < Tile::kBlocksN; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 const int column = 32 * j + lane_column();
-                *(__attribute__((address_space(3))) float*)(area + at(block_row(r), column >> 2) + (column & 3) * 4) = acc[i][j][r];
+                *(LdsFloat*)(area + at(block_row(r), column >> 2) + (column & 3) * 4) = acc[i][j][r];
             }
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
-        for (int t = 0; t < 32 / kRowsAtOnce; ++t) {
+        for (int t = 0; t < kTurns; ++t) {
             const int row = t * kRowsAtOnce + lane / kLanes, chunk = 2 * (lane % kLanes);
-            const Four one = *(__attribute__((address_space(3))) Four*)(area + at(row, chunk)),
-                       two = *(__attribute__((address_space(3))) Four*)(area + at(row, chunk + 1));
+            LdsFour *const first = (LdsFour*)(area + at(row, chunk)), *const second = (LdsFour*)(area + at(row, chunk + 1));
+            const Four one = *first, two = *second;
             float v[8] = {one[0], one[1], one[2], one[3], two[0], two[1], two[2], two[3]};
-            f(32 * i + row, chunk * 4, v);
+            f(32 * i + row, chunk * 4, v, held[t]);
+            if (columns) *first = Four{v[0], v[1], v[2], v[3]}, *second = Four{v[4], v[5], v[6], v[7]};
         }
         __builtin_amdgcn_wave_barrier();
+        if (columns) {
+#pragma unroll
+            for (int t = 0; t < kColumns / 16; ++t) {
+                const int column = lane % kColumns, row = (kColumns == 64 ? t : 2 * t + lane / 32) * 8;
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = *(LdsFloat*)(area + at(row + e, column >> 2) + (column & 3) * 4);
+                g(32 * i + row, column, v);
+            }
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 }
+
+template <typename Tile, typename L, typename F>
+__device__ __forceinline__ void by_rows(const typename Tile::Sums& acc, LdsByte* lds, L&& load, F&& f) {
+    by_rows_and_columns<Tile>(acc, lds, false, load, f, [](int, int, float (&)[8]) {});
+}
+
+struct Nothing {};
 
 // Workgroup id -> tile, such that each XCD (workgroups are dealt over the 8 in turn) takes a contiguous range of tiles, and those
 // that run at once share panels: 8 tiles of n side by side, m after m.

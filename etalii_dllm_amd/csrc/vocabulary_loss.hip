@@ -384,18 +384,25 @@ __global__ __launch_bounds__(Tile::kThreads) void softmax_kernel(SoftmaxArgs a, 
     Tile::run(a.hidden, a.weight, m * Tile::kM, n * Tile::kN, count, a.weight.count, a.s.padded, 0, 0, (LdsByte*)lds, acc);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
     const Cap cap(a.s);
-    by_rows<Tile>(acc, (LdsByte*)lds, [&](int in_row, int in_column, float (&v)[8]) {
+    struct Row {
+        float lse, factor;
+        int32_t target;
+    };
+    const auto load = [&](int in_row, int) {
+        const int64_t row = min(m0 + in_row, count - 1);
+        return Row{a.terms.lse[row], a.terms.factor[row], a.terms.target[row]};
+    };
+    by_rows<Tile>(acc, (LdsByte*)lds, load, [&](int in_row, int in_column, float (&v)[8], const Row& of) {
         const int64_t row = m0 + in_row, column = n0 + in_column;
         if (row >= count) return;
-        const float lse = a.terms.lse[row], factor = a.terms.factor[row];
-        const int64_t target = a.terms.target[row] - a.first - column, left = a.weight.count - column;
+        const int64_t target = of.target - a.first - column, left = a.weight.count - column;
         using V = Part<T> __attribute__((ext_vector_type(8)));
         V out[kPlanes<T>];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float derivative;
             const float z = cap.logit<kCapped>(v[e], derivative);
-            float p = __builtin_amdgcn_exp2f((z - lse) * kLog2E) * factor;
+            float p = __builtin_amdgcn_exp2f((z - of.lse) * kLog2E) * of.factor;
             if constexpr (kCapped) p *= derivative;
             if (e >= left || e == target) p = 0.0f;
             Part<T> parts[kPlanes<T>];
@@ -442,20 +449,32 @@ __device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, L
         typename Tile::Sums acc;
         Tile::run(a.softmax, a.weight, m * Tile::kM, n * Tile::kN, count, a.dim, min(a.unit, a.width - unit * a.unit), unit, unit, lds, acc);
         const bool store = !a.in_turn || (a.begin && unit == 0);
-        by_rows<Tile>(acc, lds, [&](int in_row, int in_column, float (&v)[8]) {
+        struct Old {
+            float4 v[2];
+        };
+        const bool fours = a.dim % 4 == 0;
+        const auto load = [&](int in_row, int in_column) {
+            const int64_t row = m0 + in_row, column = n0 + in_column;
+            Old old = {};
+            if (fours && !store && row < count) {
+                const float* const from = out + row * a.dim + column;
+#pragma unroll
+                for (int q = 0; q < 2; ++q)
+                    if (column + 4 * q < a.dim) old.v[q] = *reinterpret_cast<const float4*>(from + 4 * q);
+            }
+            return old;
+        };
+        by_rows<Tile>(acc, lds, load, [&](int in_row, int in_column, float (&v)[8], const Old& old) {
             const int64_t row = m0 + in_row, column = n0 + in_column;
             if (row >= count) return;
             float* const to = out + row * a.dim + column;
-            if (a.dim % 4 == 0) {
+            if (fours) {
 #pragma unroll
-                for (int q = 0; q < 8; q += 4) {
-                    if (column + q >= a.dim) continue;
-                    float4 w = make_float4(v[q], v[q + 1], v[q + 2], v[q + 3]);
-                    if (!store) {
-                        const float4 old = *reinterpret_cast<const float4*>(to + q);
-                        w = make_float4(old.x + w.x, old.y + w.y, old.z + w.z, old.w + w.w);
-                    }
-                    *reinterpret_cast<float4*>(to + q) = w;
+                for (int q = 0; q < 2; ++q) {
+                    if (column + 4 * q >= a.dim) continue;
+                    float4 w = make_float4(v[4 * q], v[4 * q + 1], v[4 * q + 2], v[4 * q + 3]);
+                    if (!store) w = make_float4(old.v[q].x + w.x, old.v[q].y + w.y, old.v[q].z + w.z, old.v[q].w + w.w);
+                    *reinterpret_cast<float4*>(to + 4 * q) = w;
                 }
             } else {
 #pragma unroll
@@ -475,10 +494,23 @@ __device__ __forceinline__ void weight_tile(T* __restrict__ dweight, const Gradi
     Tile::run(a.softmax, a.hidden, m * Tile::kM, n * Tile::kN, a.width, a.dim, *a.count, 0, 0, lds, acc);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
     const int by = __is_same(T, _Float16) ? *a.largest - kHalfShift : 0;
-    by_rows<Tile>(acc, lds, [&](int in_row, int in_column, float (&v)[8]) {
+    struct Old {
+        int32_t at;
+        Pack<T, 8> v;
+    };
+    const auto load = [&](int in_row, int in_column) {
+        const int64_t row = m0 + in_row, column = n0 + in_column;
+        Old old = {-1, {}};
+        if (row < a.width && column < a.dim) {
+            old.at = a.at[a.first + row];
+            if (a.accumulate && a.whole) old.v = *reinterpret_cast<const Pack<T, 8>*>(dweight + (a.first + row) * a.dim + column);
+        }
+        return old;
+    };
+    by_rows<Tile>(acc, lds, load, [&](int in_row, int in_column, float (&v)[8], const Old& old) {
         const int64_t row = m0 + in_row, column = n0 + in_column;
         if (row >= a.width || column >= a.dim) return;
-        const int64_t at = a.at[a.first + row];
+        const int64_t at = old.at;
         T* const out = dweight + (a.first + row) * a.dim + column;
         if constexpr (__is_same(T, _Float16)) {
 #pragma unroll
@@ -492,10 +524,8 @@ __device__ __forceinline__ void weight_tile(T* __restrict__ dweight, const Gradi
                 for (int e = 0; e < 8; ++e) v[e] += w[e];
             }
             if (a.accumulate) {
-                float w[8];
-                load_as_float<T, 8>(out, w);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) v[e] += w[e];
+                for (int e = 0; e < 8; ++e) v[e] += static_cast<float>(old.v.v[e]);
             }
             store_from_float<T, 8>(out, v);
         } else {
