@@ -373,10 +373,10 @@ __global__ __launch_bounds__(Tile::kThreads) void update_kernel(T* __restrict__ 
 
 // ---- the call ----
 
-template <typename T, int kSize, int kStages>
-using GramTile = TileProduct<Half, kProductPlanes<T>, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, false, 64, kStages>;
-template <typename T, int kSize, int kStages>
-using UpdateTile = TileProduct<Half, kProductPlanes<T>, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, true, 64, kStages>;
+template <typename T, int kSize, int kStages, int kTileK = 64>
+using GramTile = TileProduct<Half, kProductPlanes<T>, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, false, kTileK, kStages>;
+template <typename T, int kSize, int kStages, int kTileK = 64>
+using UpdateTile = TileProduct<Half, kProductPlanes<T>, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, true, kTileK, kStages>;
 
 Matrices matrices_of(const dllm_hip_orthogonalize_shape& sh) {
     Matrices s;

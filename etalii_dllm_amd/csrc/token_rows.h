@@ -1,4 +1,4 @@
-// Rows gathered by token: a stable sort of positions by token, and the sums of the rows of each token in the order of their
+// Rows gathered by token: a stable grouping of positions by token, and the sums of the rows of each token in the order of their
 // positions. The embedding table's gradient is such a sum, and so is the targets' part of the vocabulary loss's.
 #pragma once
 
@@ -13,9 +13,9 @@ namespace dllm_hip {
 
 constexpr int64_t kMaxSortTokens = int64_t{1} << 27;  // the counts of larger sorts would be scanned by one workgroup for long
 
-// Positions 0 .. n - 1 in the order of their tokens, and what the sort needs beside them.
+// Positions 0 .. n - 1 grouped by token, and what the sort needs beside them.
 struct TokenOrder {
-    uint32_t* token;     // [n] ascending; tokens outside the vocabulary count as `vocabulary` and come last
+    uint32_t* token;     // [n] each token's together; tokens outside the vocabulary count as `vocabulary` and come last
     uint32_t* position;  // [n] ascending within a token
     uint32_t* kept;      // [1] how many are inside
     uint32_t* spare_token;

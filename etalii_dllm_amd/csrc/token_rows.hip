@@ -1,13 +1,13 @@
 // The sort and the sums of token_rows.h.
 //
-// Sort: least significant digits first, 9 bits at a time (a vocabulary of 2^18 takes two passes). A position's place is the
+// Sort by digits: least significant first, 9 bits at a time (a vocabulary of 2^18 takes two passes). A position's place is the
 // number of smaller digits, the same digits in earlier waves (counts of each wave and digit, scanned), and those before it
 // in its own wave, which 9 ballots per 64 positions give without any atomic operation, so the sort is stable and its result
-// the same every time. Up to 16384 positions stay in one workgroup's LDS for all passes; more go through memory, each
-// pass three launches. 16384 tokens of 2^18: see the figures at sort_kernel.
+// the same every time. Up to 16384 positions are first dealt to workgroups by a hash of the token, since one workgroup's ballots
+// over all of them took 39 us; more go through memory, each pass three launches.
 //
-// Sums: a wave takes 16 sorted positions and 16 bytes of columns to a lane, reads all 16 rows at once and adds them in order.
-// A token whose positions lie within the 16 is done; the sums of others are float32 parts, added in their order by a second
+// Sums: a wave takes 8 sorted positions and 16 bytes of columns to a lane, reads all 8 rows at once and adds them in order.
+// A token whose positions lie within the 8 is done; the sums of others are float32 parts, added in their order by a second
 // launch. Nothing depends on when a wave runs.
 #include "token_rows.h"
 
@@ -92,7 +92,7 @@ __device__ __forceinline__ uint32_t token_key(int64_t token, int64_t vocabulary)
     return static_cast<uint32_t>(token >= 0 && token < vocabulary ? token : vocabulary);
 }
 
-// word to every word of `bytes` bytes at `at` (aligned to 2), by workgroups `block` of `blocks`
+// word to every word of `bytes` bytes at `at` (aligned to 2), by workgroup `block` of `blocks`
 __device__ __forceinline__ void fill_part(char* at, size_t bytes, uint32_t word, size_t block, size_t blocks) {
     const size_t head = min(bytes, (16 - reinterpret_cast<uintptr_t>(at) % 16) % 16), chunks = (bytes - head) / 16;
     uint4* const body = reinterpret_cast<uint4*>(at + head);
@@ -109,50 +109,114 @@ __global__ __launch_bounds__(256) void fill_kernel(char* at, size_t bytes, uint3
     fill_part(at, bytes, word, blockIdx.x, gridDim.x);
 }
 
-// Workgroup 0 sorts, the others fill.
+// Up to kSortBlock positions. A workgroup to each of 2^bucket_bits parts of the tokens, by a hash, and one to those outside: it
+// lists its positions in their order, counts those of the parts before it, and sorts its own by token; short lists by counting
+// the smaller ones, longer ones by digits. The others fill. 16381 tokens of 49152 in 128 parts: 22 us (39 in one), most of
+// it the longest list's, a frequent token's. Beside a fill, which takes longer, few workgroups sort.
+constexpr int kBucketBits = 7, kBucketBitsWithFill = 4;
+constexpr int kCountedList = 256;
+
+__device__ __forceinline__ int bucket_of(uint32_t key, uint32_t outside, int bits) {
+    return key == outside ? 1 << bits : static_cast<int>((key * 2654435769u) >> (32 - bits));
+}
+
 __global__ __launch_bounds__(kSortThreads) void sort_kernel(const int64_t* __restrict__ tokens, int n, int64_t vocabulary, int passes,
-                                                            TokenOrder order, char* fill_at, size_t fill_bytes, uint32_t fill) {
+                                                            int bucket_bits, TokenOrder order, char* fill_at, size_t fill_bytes, uint32_t fill) {
     __shared__ SortCounts counts;
-    __shared__ uint32_t keys[kSortBlock];
+    __shared__ __attribute__((aligned(16))) uint32_t keys[kSortBlock];
     __shared__ uint16_t positions[kSortBlock], ranks[kSortBlock];
-    if (blockIdx.x > 0) {
-        fill_part(fill_at, fill_bytes, fill, blockIdx.x - 1, gridDim.x - 1);
+    __shared__ int mine_of[kSortWaves], before_of[kSortWaves];
+    const int bucket = static_cast<int>(blockIdx.x), buckets = 1 << bucket_bits;
+    if (bucket > buckets) {
+        fill_part(fill_at, fill_bytes, fill, bucket - buckets - 1, gridDim.x - buckets - 1);
         return;
     }
-    const int rounds = (n + kSortThreads - 1) / kSortThreads;
-    for (int i = threadIdx.x; i < n; i += kSortThreads) {
-        keys[i] = token_key(tokens[i], vocabulary);
-        positions[i] = static_cast<uint16_t>(i);
-    }
+    const uint32_t outside = static_cast<uint32_t>(vocabulary);
+    const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63;
+    const int rounds_all = (n + kSortThreads - 1) / kSortThreads;
+    uint32_t key[kSortRounds];
+    uint32_t in_bucket = 0;  // bit r: item r is this bucket's
+    int mine = 0, before = 0;
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r)
+        if (r < rounds_all) {
+            const int i = sort_item(rounds_all, r);
+            key[r] = i < n ? token_key(tokens[i], vocabulary) : ~0u;
+        }
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r)
+        if (r < rounds_all) {
+            const int of = key[r] == ~0u ? buckets + 1 : bucket_of(key[r], outside, bucket_bits);
+            mine += __popcll(__ballot(of == bucket));
+            before += __popcll(__ballot(of < bucket));
+            in_bucket |= (of == bucket ? 1u : 0u) << r;
+        }
+    if (lane == 0) mine_of[wave] = mine, before_of[wave] = before;
     __syncthreads();
+    int list = 0, base = 0, at = 0;
+    for (int w = 0; w < kSortWaves; ++w) {
+        if (w < wave) at += mine_of[w];
+        list += mine_of[w];
+        base += before_of[w];
+    }
+    if (bucket == buckets && threadIdx.x == 0) *order.kept = base;
+#pragma unroll
+    for (int r = 0; r < kSortRounds; ++r)
+        if (r < rounds_all) {
+            const uint64_t in = __ballot(in_bucket >> r & 1);
+            if (in >> lane & 1) {
+                const int to = at + __popcll(in & ((uint64_t{1} << lane) - 1));
+                keys[to] = key[r];
+                positions[to] = static_cast<uint16_t>(sort_item(rounds_all, r));
+            }
+            at += __popcll(in);
+        }
+    __syncthreads();
+    bool alike = true;
+    for (int i = threadIdx.x; i < list; i += kSortThreads) alike = alike && keys[i] == keys[0];
+    if (__syncthreads_and(alike)) {  // the positions' order is theirs already
+        for (int i = threadIdx.x; i < list; i += kSortThreads) order.token[base + i] = keys[i], order.position[base + i] = positions[i];
+        return;
+    }
+    if (list <= kCountedList) {
+        if (static_cast<int>(threadIdx.x) < list) {
+            const uint32_t own = keys[threadIdx.x];
+            const int self = static_cast<int>(threadIdx.x);
+            int rank = 0;
+#pragma unroll 4
+            for (int i = 0; i < list; i += 4) {  // (what is read past the list does not count)
+                const uint4 four = *reinterpret_cast<const uint4*>(keys + i);
+                const uint32_t k[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) rank += i + e < list && (k[e] < own || (k[e] == own && i + e < self));
+            }
+            order.token[base + rank] = own;
+            order.position[base + rank] = positions[threadIdx.x];
+        }
+        return;
+    }
+    const int rounds = (list + kSortThreads - 1) / kSortThreads;
     for (int pass = 0; pass < passes; ++pass) {
-        const int shift = pass * kDigitBits, wave = static_cast<int>(threadIdx.x) >> 6;
-        rank_digits(keys, rounds, n, shift, counts, ranks);
-        uint32_t key[kSortRounds], to[kSortRounds];
+        const int shift = pass * kDigitBits;
+        rank_digits(keys, rounds, list, shift, counts, ranks);
+        uint32_t moved[kSortRounds], to[kSortRounds];
         uint16_t position[kSortRounds];
 #pragma unroll
         for (int r = 0; r < kSortRounds; ++r) {
             const int i = sort_item(rounds, r);
-            if (r < rounds && i < n) {
-                key[r] = keys[i], position[r] = positions[i];
-                const uint32_t d = (key[r] >> shift) & (kDigits - 1);
+            if (r < rounds && i < list) {
+                moved[r] = keys[i], position[r] = positions[i];
+                const uint32_t d = (moved[r] >> shift) & (kDigits - 1);
                 to[r] = counts.digit[d] + counts.wave[wave][d] + ranks[i];
             }
         }
         __syncthreads();
 #pragma unroll
         for (int r = 0; r < kSortRounds; ++r)
-            if (r < rounds && sort_item(rounds, r) < n) keys[to[r]] = key[r], positions[to[r]] = position[r];
+            if (r < rounds && sort_item(rounds, r) < list) keys[to[r]] = moved[r], positions[to[r]] = position[r];
         __syncthreads();
     }
-    const uint32_t outside = static_cast<uint32_t>(vocabulary);
-    for (int i = threadIdx.x; i < n; i += kSortThreads) {
-        const uint32_t key = keys[i];
-        order.token[i] = key;
-        order.position[i] = positions[i];
-        if (key != outside && (i == n - 1 || keys[i + 1] == outside)) *order.kept = i + 1;
-        if (i == 0 && key == outside) *order.kept = 0;
-    }
+    for (int i = threadIdx.x; i < list; i += kSortThreads) order.token[base + i] = keys[i], order.position[base + i] = positions[i];
 }
 
 // One pass over more positions: this workgroup's number of each digit, by digit and workgroup ...
@@ -226,7 +290,7 @@ __global__ __launch_bounds__(256) void kept_kernel(const uint32_t* __restrict__ 
 
 // ---- sums ----
 
-constexpr int kSumRows = 16;  // sorted positions of a wave
+constexpr int kSumRows = 8;  // sorted positions of a wave
 
 struct SumArgs {
     const uint32_t* token;
@@ -343,7 +407,7 @@ __global__ __launch_bounds__(256) void token_parts_kernel(T* __restrict__ table,
     load_as_float<float, kWidth>(a.part + (2 * block + 1) * a.dim + column, acc);
     const float* part = a.part + 2 * (block + 1) * a.dim + column;
     int64_t i = 0;
-    constexpr int kAhead = 8;
+    constexpr int kAhead = 16;
     for (; i + kAhead <= more; i += kAhead) {
         float v[kAhead][kWidth];
 #pragma unroll
@@ -405,8 +469,10 @@ int sort_tokens(const int64_t* tokens, int64_t n, int64_t vocabulary, const Toke
     const int passes = (bits + kDigitBits - 1) / kDigitBits;
     char* const to = static_cast<char*>(fill_at);
     if (n <= kSortBlock) {
-        const size_t fills = std::min<size_t>(ceil_div(fill_bytes, kSortThreads * 16), 255);
-        sort_kernel<<<static_cast<unsigned>(1 + fills), kSortThreads, 0, stream>>>(tokens, static_cast<int>(n), vocabulary, passes, o, to,
+        const bool long_fill = fill_bytes > (size_t{64} << 20);  // of more than a sort's time
+        const int bits = long_fill ? kBucketBitsWithFill : kBucketBits, sorting = (1 << bits) + 1;
+        const size_t fills = std::min<size_t>(ceil_div(fill_bytes, kSortThreads * 16), 256 - sorting);
+        sort_kernel<<<static_cast<unsigned>(sorting + fills), kSortThreads, 0, stream>>>(tokens, static_cast<int>(n), vocabulary, passes, bits, o, to,
                                                                                     fill_bytes, fill);
         return check_launch("sort_tokens");
     }
