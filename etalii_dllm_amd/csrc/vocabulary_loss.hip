@@ -4,7 +4,12 @@
 //   g = (exp(z - lse) - onehot) dloss scale (1 - tanh^2)     dh = g W     dW = g^T h
 //
 // Only rows that count (a target inside the vocabulary) are worked on: they are listed first, and their hidden states gathered
-// into whole 16-byte chunks (float32 as three planes of bfloat16 parts), zeroes behind.
+// into whole 16-byte chunks, zeroes behind.
+//
+// Float32 values are multiplied as pairs of float16, three products: 22 bits and more of each value, off by 2^-39 of the largest
+// at most: hidden states are scaled by the power of two that brings their row's largest value to the top of float16's range,
+// weights by that of kScaleRows of them. (Three bfloat16 parts, six products, hold values of any size and take twice as long:
+// gradients of 1020 rows, 49152 x 576, 1.6 ms.)
 //
 // Forward: tiles of logits on the matrix cores, vocabulary by rows, so that a lane owns a row of the batch; a tile leaves each
 // row's largest logit and sum of exponentials of 128 of the vocabulary, which a second launch joins in a fixed order, and
@@ -36,6 +41,45 @@ constexpr int kStatRows = 128;        // of the vocabulary: one maximum and sum
 constexpr size_t kPieceBytes = size_t{1} << 28;
 constexpr int64_t kStrideSlack = 64;  // elements between the softmax's rows: their stride is no power of two, which would meet on few channels
 constexpr int kHalfShift = 14;  // float16 holds the softmax's part of g times 2^14, relative to the row's weight
+constexpr int kTop = 15;        // pairs of float16 hold values up to 2^15
+constexpr int64_t kScaleRows = 2048;  // of the vocabulary, that share a scale
+
+// What the products read of a type, in kLossPlanes planes.
+template <typename T>
+struct LossProduct {
+    using Part = T;
+};
+template <>
+struct LossProduct<float> {
+    using Part = _Float16;
+};
+template <typename T>
+using LossPart = typename LossProduct<T>::Part;
+template <typename T>
+constexpr int kLossPlanes = sizeof(T) == 4 ? 2 : 1;
+template <typename T>
+constexpr bool kHalfParts = __is_same(LossPart<T>, _Float16);
+template <typename T>
+constexpr bool kScaled = sizeof(T) == 4;
+
+// v's parts, 8 of them to each plane
+template <typename T>
+__device__ __forceinline__ void store_parts(char* to, int64_t plane, const float (&v)[8]) {
+    using V = LossPart<T> __attribute__((ext_vector_type(8)));
+    float left[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) left[e] = v[e];
+#pragma unroll
+    for (int q = 0; q < kLossPlanes<T>; ++q) {
+        V out;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            out[e] = static_cast<LossPart<T>>(left[e]);
+            left[e] -= static_cast<float>(out[e]);
+        }
+        *reinterpret_cast<V*>(to + q * plane) = out;
+    }
+}
 
 struct LossShape {
     int64_t rows, vocabulary, dim, padded;  // padded: dim in whole chunks
@@ -75,16 +119,72 @@ __global__ __launch_bounds__(1024) void keep_rows_kernel(const int64_t* __restri
 
 // ---- packing ----
 
-// Row list[j] (j itself without a list) of src as chunks of 8 parts, in kPlanes<T> planes; zeroes past dim. exponent: row j times
-// 2^(exponent[j] - *largest), as float16 allows.
+// The least e with |x| < 2^e for the float32 of these bits; 0 for zero.
+__device__ __forceinline__ int exponent_of(uint32_t bits) {
+    int e = 0;
+    if (bits != 0) frexpf(__builtin_bit_cast(float, bits), &e);
+    return e;
+}
+
+// The bits of x's size, which grow with it; zero for what is not finite.
+__device__ __forceinline__ uint32_t size_bits(float x) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, x) & 0x7fffffffu;
+    return bits < 0x7f800000u ? bits : 0;
+}
+
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#pragma unroll
+    for (int s = 32; s > 0; s >>= 1) v = max(v, static_cast<uint32_t>(__shfl_xor(static_cast<int>(v), s)));
+    return v;
+}
+
+// The exponent of each listed row's largest value, a wave to a row.
+__global__ __launch_bounds__(256) void row_exponents_kernel(const float* __restrict__ src, int64_t stride, int64_t dim, const uint32_t* __restrict__ list,
+                                                            const uint32_t* __restrict__ count, int32_t* __restrict__ exponent) {
+    const int64_t j = block_id() * 4 + (threadIdx.x >> 6);
+    if (j >= static_cast<int64_t>(*count)) return;
+    const int lane = static_cast<int>(threadIdx.x) & 63;
+    const float* const row = src + static_cast<int64_t>(list[j]) * stride;
+    uint32_t top = 0;
+    for (int64_t d = lane; d < dim; d += kWave) top = max(top, size_bits(row[d]));
+    top = wave_max(top);
+    if (lane == 0) exponent[j] = exponent_of(top);
+}
+
+// The bits of the largest size of each kScaleRows rows, which are zero before. (A maximum, so the order does not matter.)
+constexpr int kSizeRows = 64;
+template <int kWidth>
+__global__ __launch_bounds__(256) void unit_sizes_kernel(const float* __restrict__ src, int64_t rows, int64_t dim, uint32_t* __restrict__ sizes) {
+    __shared__ uint32_t of_wave[4];
+    const int64_t first = block_id() * kSizeRows;
+    if (first >= rows) return;
+    const int64_t n = min(rows - first, static_cast<int64_t>(kSizeRows)) * dim / kWidth;
+    const float* const from = src + first * dim;
+    uint32_t top = 0;
+    for (int64_t i = threadIdx.x; i < n; i += 256) {
+        float v[kWidth];
+        load_as_float<float, kWidth>(from + i * kWidth, v);
+#pragma unroll
+        for (int e = 0; e < kWidth; ++e) top = max(top, size_bits(v[e]));
+    }
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) atomicMax(sizes + first / kScaleRows, max(max(of_wave[0], of_wave[1]), max(of_wave[2], of_wave[3])));
+}
+
+// Row list[j] (j itself without a list) of src as chunks of 8 parts, in planes; zeroes past dim. Scaled by a power of two: of the row's
+// exponent (down), of its unit's size, or up by the row's exponent from the largest one.
+enum PackScale { kNoScale, kRowScale, kUnitScale, kWeightScale };
 struct PackArgs {
     const uint32_t *list, *count;
     int64_t n, dim, stride, chunks, plane;
     const int32_t *exponent, *largest;
+    const uint32_t* sizes;
 };
 
-template <typename T, bool kWhole>
-__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, Part<T>* __restrict__ dst, PackArgs a) {
+template <typename T, bool kWhole, PackScale kScale>
+__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, LossPart<T>* __restrict__ dst, PackArgs a) {
     const int64_t i = block_id() * 256 + threadIdx.x;
     const int64_t j = i / a.chunks, c = i - j * a.chunks;
     if (j >= (a.count ? static_cast<int64_t>(*a.count) : a.n)) return;
@@ -102,34 +202,27 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, Pa
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = c * 8 + e < a.dim ? static_cast<float>(row[e]) : 0.0f;
     }
-    if (a.exponent) {
-        const int by = a.exponent[j] - *a.largest;
+    if constexpr (kScale != kNoScale) {
+        int by;
+        if constexpr (kScale == kRowScale) by = kTop - a.exponent[j];
+        if constexpr (kScale == kUnitScale) by = kTop - exponent_of(a.sizes[j / kScaleRows]);
+        if constexpr (kScale == kWeightScale) by = a.exponent[j] - *a.largest + (kScaled<T> ? kTop : 0);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], by);
     }
-    using V = Part<T> __attribute__((ext_vector_type(8)));
-    V out[kPlanes<T>];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        Part<T> parts[kPlanes<T>];
-        split<T>(v[e], parts);
-#pragma unroll
-        for (int p = 0; p < kPlanes<T>; ++p) out[p][e] = parts[p];
-    }
-#pragma unroll
-    for (int p = 0; p < kPlanes<T>; ++p) *reinterpret_cast<V*>(dst + p * a.plane + i * 8) = out[p];
+    store_parts<T>(reinterpret_cast<char*>(dst + i * 8), a.plane * 2, v);
 }
 
-template <typename T>
-int launch_pack(const T* src, Part<T>* dst, const PackArgs& args, hipStream_t stream) {
+template <typename T, PackScale kScale>
+int launch_pack(const T* src, LossPart<T>* dst, const PackArgs& args, hipStream_t stream) {
     PackArgs a = args;
     a.chunks = static_cast<int64_t>(ceil_div(a.dim, 8));
     const bool whole = a.dim % 8 == 0 && a.stride % kChunk<T> == 0 && aligned_to(src, 16);
     const dim3 grid = grid_of(ceil_div(a.n * a.chunks, 256));
     if (whole)
-        pack_kernel<T, true><<<grid, 256, 0, stream>>>(src, dst, a);
+        pack_kernel<T, true, kScale><<<grid, 256, 0, stream>>>(src, dst, a);
     else
-        pack_kernel<T, false><<<grid, 256, 0, stream>>>(src, dst, a);
+        pack_kernel<T, false, kScale><<<grid, 256, 0, stream>>>(src, dst, a);
     return check_launch("vocabulary_loss packing");
 }
 
@@ -139,7 +232,7 @@ int launch_pack(const T* src, Part<T>* dst, const PackArgs& args, hipStream_t st
 // the large ones would leave CUs without work or pad much; and for up to 64 rows, whose products wait for the weights'
 // bytes, tiles of 64 rows. The forward's waves hold kStatRows of the vocabulary in all of them.
 template <typename T, bool kAColumns, bool kBColumns, int kM, int kN, int kWavesM, int kWavesN, int kStages = 2>
-using Product64 = TileProduct<Part<T>, kPlanes<T>, kM, kN, kWavesM, kWavesN, kAColumns, kBColumns, 64, kStages>;
+using Product64 = TileProduct<LossPart<T>, kLossPlanes<T>, kM, kN, kWavesM, kWavesN, kAColumns, kBColumns, 64, kStages>;
 
 template <typename T>
 struct LargeTiles {
@@ -198,6 +291,8 @@ struct ForwardArgs {
     const int64_t* targets;
     Stat* stats;  // [unit of kStatRows][rows]
     float* at_target;  // [rows]
+    const int32_t* exponent;  // float32: by the place in the list
+    const uint32_t* sizes;    // float32: of the piece, by kScaleRows
 };
 
 template <typename T, bool kCapped, typename Tile>
@@ -216,9 +311,12 @@ __global__ __launch_bounds__(Tile::kThreads) void forward_kernel(ForwardArgs a, 
     const int64_t unit = (a.first + m0) / kStatRows;
     const int valid = static_cast<int>(min(a.weight.count - m0, static_cast<int64_t>(kStatRows)));
     const Cap cap(a.s);
+    static_assert(kScaleRows % Tile::kM == 0);
+    const int weight_exponent = kScaled<T> ? exponent_of(a.sizes[m * Tile::kM / kScaleRows]) - 2 * kTop : 0;
 #pragma unroll
     for (int j = 0; j < Tile::kBlocksN; ++j) {
         const int64_t row = n0 + 32 * j + lane_column();
+        const int by = kScaled<T> ? weight_exponent + a.exponent[min(row, count - 1)] : 0;
         const int target = row < count ? static_cast<int>(a.targets[a.list[row]] - a.first - m0) : -1;
         const bool any = __ballot(target >= 0 && target < kStatRows) != 0;
         float top = -INFINITY;
@@ -226,8 +324,9 @@ __global__ __launch_bounds__(Tile::kThreads) void forward_kernel(ForwardArgs a, 
         for (int i = 0; i < Tile::kBlocksM; ++i) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
-                float unused;
-                acc[i][j][r] = cap.logit<kCapped>(acc[i][j][r], unused);
+                float unused, x = acc[i][j][r];
+                if constexpr (kScaled<T>) x = ldexpf(x, by);
+                acc[i][j][r] = cap.logit<kCapped>(x, unused);
             }
             __builtin_amdgcn_sched_barrier(0);  // one block's values at a time: all of them do not fit the registers
         }
@@ -292,7 +391,8 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const Stat* __restrict_
 struct RowTerms {
     float *lse, *factor;
     int32_t* target;
-    int32_t* exponent;  // float16: factor holds the weight's mantissa, this the power of two left out
+    int32_t* exponent;      // float16 parts: factor holds the weight's mantissa, this the power of two left out
+    int32_t* row_exponent;  // float32: of the hidden states
 };
 
 struct TargetArgs {
@@ -301,25 +401,28 @@ struct TargetArgs {
     const float *lse, *dloss;
     RowTerms terms;
     float* coefficient;  // by row
-    int32_t* largest;    // float16: the largest exponent
+    int32_t* largest;    // float16 parts: the largest exponent, of float32 with the row's added
 };
 
-// factor = mantissa 2^exponent, mantissa in [1, 2); an exponent no other is below, for zero
+// factor = mantissa 2^exponent, mantissa in [1, 2); for zero an exponent so far below all others that what it scales is zero
+constexpr int kNoWeight = -1000;
 __device__ __forceinline__ void take_apart(float factor, float& mantissa, int& exponent) {
     int e = 0;
     mantissa = factor;
     if (factor != 0.0f && isfinite(factor)) mantissa = 2.0f * frexpf(factor, &e), e -= 1;
-    exponent = factor == 0.0f ? -200 : e;
+    exponent = factor == 0.0f ? kNoWeight : e;
 }
 
+template <typename T>
 __global__ __launch_bounds__(1024) void largest_exponent_kernel(TargetArgs a) {
     __shared__ int of_wave[16];
-    int top = -200;
+    int top = -400;
     const int64_t n = *a.order.kept;
     for (int64_t j = threadIdx.x; j < n; j += 1024) {
         float mantissa;
         int e;
         take_apart(a.dloss[a.order.position[j]] * a.s.scale, mantissa, e);
+        if (kScaled<T> && e != kNoWeight) e += a.terms.row_exponent[j];
         top = max(top, e);
     }
 #pragma unroll
@@ -350,7 +453,7 @@ __global__ __launch_bounds__(256) void target_kernel(const T* __restrict__ hidde
     a.coefficient[row] = expm1f(z - lse) * derivative * factor;
     a.terms.lse[j] = lse;
     a.terms.target[j] = static_cast<int32_t>(target);
-    if constexpr (sizeof(Part<T>) == 2 && __is_same(Part<T>, _Float16)) {
+    if constexpr (kHalfParts<T>) {
         float mantissa;
         int e;
         take_apart(factor, mantissa, e);
@@ -369,6 +472,7 @@ struct SoftmaxArgs {
     RowTerms terms;
     char* out;  // [rows][piece] parts, in planes
     int64_t out_stride, out_plane;
+    const uint32_t* sizes;  // float32: of the piece, by kScaleRows
 };
 
 // The softmax's part of g, zero past the vocabulary's end and at the targets.
@@ -386,33 +490,28 @@ __global__ __launch_bounds__(Tile::kThreads) void softmax_kernel(SoftmaxArgs a, 
     const Cap cap(a.s);
     struct Row {
         float lse, factor;
-        int32_t target;
+        int32_t target, by;
     };
+    static_assert(kScaleRows % Tile::kN == 0);
+    const int weight_exponent = kScaled<T> ? exponent_of(a.sizes[n * Tile::kN / kScaleRows]) - 2 * kTop : 0;
     const auto load = [&](int in_row, int) {
         const int64_t row = min(m0 + in_row, count - 1);
-        return Row{a.terms.lse[row], a.terms.factor[row], a.terms.target[row]};
+        return Row{a.terms.lse[row], a.terms.factor[row], a.terms.target[row], kScaled<T> ? weight_exponent + a.terms.row_exponent[row] : 0};
     };
     by_rows<Tile>(acc, (LdsByte*)lds, load, [&](int in_row, int in_column, float (&v)[8], const Row& of) {
         const int64_t row = m0 + in_row, column = n0 + in_column;
         if (row >= count) return;
         const int64_t target = of.target - a.first - column, left = a.weight.count - column;
-        using V = Part<T> __attribute__((ext_vector_type(8)));
-        V out[kPlanes<T>];
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             float derivative;
+            if constexpr (kScaled<T>) v[e] = ldexpf(v[e], of.by);
             const float z = cap.logit<kCapped>(v[e], derivative);
             float p = __builtin_amdgcn_exp2f((z - of.lse) * kLog2E) * of.factor;
             if constexpr (kCapped) p *= derivative;
-            if (e >= left || e == target) p = 0.0f;
-            Part<T> parts[kPlanes<T>];
-            split<T>(p, parts);
-#pragma unroll
-            for (int q = 0; q < kPlanes<T>; ++q) out[q][e] = parts[q];
+            v[e] = e >= left || e == target ? 0.0f : p;
         }
-#pragma unroll
-        for (int q = 0; q < kPlanes<T>; ++q)
-            *reinterpret_cast<V*>(a.out + q * a.out_plane + row * a.out_stride + column * 2) = out[q];
+        store_parts<T>(a.out + row * a.out_stride + column * 2, a.out_plane, v);
     });
 }
 
@@ -431,12 +530,13 @@ struct GradientArgs {
     int64_t weight_m_tiles, weight_n_tiles;
     const float* sums;       // the targets' part, by the index in `at`
     const int32_t* at;       // by token, -1: none
-    const int32_t* largest;  // float16: the power of two left out
+    const int32_t* largest;  // float16 parts: the power of two left out
+    const uint32_t* sizes;   // float32: of the piece, by kScaleRows, which are its units
     bool accumulate;
     bool whole;  // dW's rows are whole 16-byte chunks
 };
 
-template <typename Tile>
+template <typename T, typename Tile>
 __device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, LdsByte* lds) {
     const int64_t count = *a.count, units = (a.width + a.unit - 1) / a.unit, each = a.m_tiles * a.n_tiles;
     const int64_t only = a.in_turn ? 0 : id / each, end = a.in_turn ? units : only + 1;
@@ -449,6 +549,7 @@ __device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, L
         typename Tile::Sums acc;
         Tile::run(a.softmax, a.weight, m * Tile::kM, n * Tile::kN, count, a.dim, min(a.unit, a.width - unit * a.unit), unit, unit, lds, acc);
         const bool store = !a.in_turn || (a.begin && unit == 0);
+        const int by = kScaled<T> ? exponent_of(a.sizes[unit]) - kTop : 0;
         struct Old {
             float4 v[2];
         };
@@ -468,6 +569,10 @@ __device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, L
             const int64_t row = m0 + in_row, column = n0 + in_column;
             if (row >= count) return;
             float* const to = out + row * a.dim + column;
+            if constexpr (kScaled<T>) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], by);
+            }
             if (fours) {
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
@@ -493,7 +598,7 @@ __device__ __forceinline__ void weight_tile(T* __restrict__ dweight, const Gradi
     typename Tile::Sums acc;
     Tile::run(a.softmax, a.hidden, m * Tile::kM, n * Tile::kN, a.width, a.dim, *a.count, 0, 0, lds, acc);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
-    const int by = __is_same(T, _Float16) ? *a.largest - kHalfShift : 0;
+    const int by = kHalfParts<T> ? *a.largest - kHalfShift - (kScaled<T> ? kTop : 0) : 0;
     struct Old {
         int32_t at;
         Pack<T, 8> v;
@@ -512,7 +617,7 @@ __device__ __forceinline__ void weight_tile(T* __restrict__ dweight, const Gradi
         if (row >= a.width || column >= a.dim) return;
         const int64_t at = old.at;
         T* const out = dweight + (a.first + row) * a.dim + column;
-        if constexpr (__is_same(T, _Float16)) {
+        if constexpr (kHalfParts<T>) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], by);
         }
@@ -546,7 +651,7 @@ __global__ __launch_bounds__(HiddenTile::kThreads) void gradient_kernel(T* __res
     __shared__ __attribute__((aligned(1024))) char lds[HiddenTile::kLds > WeightTile::kLds ? HiddenTile::kLds : WeightTile::kLds];
     const int64_t id = block_id();
     if (id < a.hidden_blocks)
-        hidden_tile<HiddenTile>(a, id, (LdsByte*)lds);
+        hidden_tile<T, HiddenTile>(a, id, (LdsByte*)lds);
     else if (id < a.hidden_blocks + a.weight_m_tiles * a.weight_n_tiles)
         weight_tile<T, WeightTile>(dweight, a, id - a.hidden_blocks, (LdsByte*)lds);
 }
@@ -581,10 +686,10 @@ __global__ __launch_bounds__(256) void finish_hidden_kernel(const T* __restrict_
     }
     const T* const w = weight + static_cast<int64_t>(a.order.token[j]) * a.s.dim;
     const float c = a.coefficient[row];
-    const int by = __is_same(T, _Float16) ? a.terms.exponent[j] - kHalfShift : 0;
+    const int by = kHalfParts<T> ? a.terms.exponent[j] - kHalfShift : 0;
     for (int64_t d = threadIdx.x; d < a.s.dim; d += 256) {
         float v = a.total[j * a.s.dim + d];
-        if constexpr (__is_same(T, _Float16)) v = ldexpf(v, by);
+        if constexpr (kHalfParts<T>) v = ldexpf(v, by);
         out[d] = static_cast<T>(fmaf(c, static_cast<float>(w[d]), v));
     }
 }
@@ -615,11 +720,11 @@ LossShape loss_shape(const dllm_hip_vocabulary_loss_shape& sh) {
     return s;
 }
 
-int planes_of(int64_t dtype) { return dtype == kFloat32 ? 3 : 1; }
+int planes_of(int64_t dtype) { return dtype == kFloat32 ? 2 : 1; }
 
 // Of the vocabulary: one addition to dh. It goes by the vocabulary and type alone, so that a row's bits are its own. Shorter units are
 // more workgroups where rows are few and more additions where they are many; float32's take six times as long.
-int64_t unit_of(const LossShape& s, int64_t dtype) { return dtype == kFloat32 ? 2048 : s.vocabulary <= 65536 ? 4096 : 8192; }
+int64_t unit_of(const LossShape& s, int64_t dtype) { return dtype == kFloat32 ? kScaleRows : s.vocabulary <= 65536 ? 4096 : 8192; }
 
 // Units of the backward's piece: as many as keep its softmax within kPieceBytes, at least one.
 int64_t piece_units(const LossShape& s, int64_t dtype) {
@@ -630,7 +735,7 @@ int64_t piece_units(const LossShape& s, int64_t dtype) {
 }
 
 struct LossLayout {
-    size_t hidden, scaled, weight, list, stats, at_target;                  // forward
+    size_t hidden, scaled, weight, list, stats, at_target, row_exponent, sizes;  // forward
     size_t terms, softmax, part, total, sums, sum_parts, at, coefficient;   // backward
     int64_t unit, units;
     size_t bytes;
@@ -639,11 +744,13 @@ struct LossLayout {
         unit = unit_of(s, dtype), units = piece_units(s, dtype);
         const size_t piece = backward ? std::min<size_t>(units * unit, s.vocabulary) : std::min<size_t>(kPackPiece, s.vocabulary);
         hidden = rows * s.padded * planes;
-        scaled = backward && dtype == kFloat16 ? hidden : 0;
+        scaled = backward && dtype != kBFloat16 ? hidden : 0;
         weight = piece * s.padded * planes;
         list = backward ? 0 : rows;
         stats = backward ? 0 : ceil_div(s.vocabulary, kStatRows) * rows;
         at_target = backward ? 0 : rows;
+        row_exponent = dtype == kFloat32 ? rows : 0;
+        sizes = dtype == kFloat32 ? ceil_div(s.vocabulary, kScaleRows) : 0;
         terms = backward ? round_up(rows, 256) : 0;
         softmax = backward ? rows * (units * unit + kStrideSlack) * planes : 0;
         part = backward ? units * rows * dim : 0;
@@ -660,6 +767,8 @@ struct LossLayout {
         l.add<uint32_t>(1);
         l.add<Stat>(stats);
         l.add<float>(at_target);
+        l.add<int32_t>(row_exponent);
+        l.add<uint32_t>(sizes);
         if (backward) {
             add_token_order(l, s.rows);
             for (int i = 0; i < 4; ++i) l.add<float>(terms);
@@ -672,10 +781,12 @@ struct LossLayout {
 
 template <typename T>
 struct Buffers {
-    Part<T>*hidden, *scaled, *weight;
+    LossPart<T>*hidden, *scaled, *weight;
     uint32_t *list, *count;
     Stat* stats;
     float* at_target;
+    int32_t* row_exponent;
+    uint32_t* sizes;
     TokenOrder order;
     RowTerms terms;
     char* softmax;
@@ -685,19 +796,22 @@ struct Buffers {
     int32_t* largest;
     Buffers(const LossLayout& l, const LossShape& s, bool backward, void* workspace, size_t bytes) {
         Carve c(workspace, bytes);
-        hidden = c.take<Part<T>>(l.hidden);
-        scaled = c.take<Part<T>>(l.scaled);
-        weight = c.take<Part<T>>(l.weight);
+        hidden = c.take<LossPart<T>>(l.hidden);
+        scaled = c.take<LossPart<T>>(l.scaled);
+        weight = c.take<LossPart<T>>(l.weight);
         list = c.take<uint32_t>(l.list);
         count = c.take<uint32_t>(1);
         stats = c.take<Stat>(l.stats);
         at_target = c.take<float>(l.at_target);
+        row_exponent = c.take<int32_t>(l.row_exponent);
+        sizes = c.take<uint32_t>(l.sizes);
         if (!backward) return;
         order = take_token_order(c, s.rows);
         terms.lse = c.take<float>(l.terms);
         terms.factor = c.take<float>(l.terms);
         terms.target = c.take<int32_t>(l.terms);
         terms.exponent = c.take<int32_t>(l.terms);
+        terms.row_exponent = row_exponent;
         softmax = reinterpret_cast<char*>(c.take<uint16_t>(l.softmax));
         part = c.take<float>(l.part);
         total = c.take<float>(l.total);
@@ -709,26 +823,54 @@ struct Buffers {
     }
 };
 
-// The weights of a piece as an operand: where they are, or packed.
 template <typename T>
-int weight_operand(const LossShape& s, const T* weight, Part<T>* packed, int64_t first, int64_t n, Operand& op, hipStream_t stream) {
-    const bool direct = sizeof(T) == 2 && s.dim % 8 == 0 && aligned_to(weight, 16);
+bool weights_direct(const LossShape& s, const T* weight) {
+    return sizeof(T) == 2 && s.dim % 8 == 0 && aligned_to(weight, 16);
+}
+
+// The weights of a piece as an operand: where they are, or packed. sizes: of the piece.
+template <typename T>
+int weight_operand(const LossShape& s, const T* weight, LossPart<T>* packed, uint32_t* sizes, int64_t first, int64_t n, Operand& op,
+                   hipStream_t stream) {
     op.count = n;
     op.batch = 0;
     op.stride = s.padded * 2;
     op.plane = n * s.padded * 2;
-    if (direct) {
+    if (weights_direct(s, weight)) {
         op.base = reinterpret_cast<const char*>(weight + first * s.dim);
         return kOk;
     }
     op.base = reinterpret_cast<const char*>(packed);
     PackArgs p{};
-    p.n = n, p.dim = s.dim, p.stride = s.dim, p.plane = n * s.padded;
-    return launch_pack<T>(weight + first * s.dim, packed, p, stream);
+    p.n = n, p.dim = s.dim, p.stride = s.dim, p.plane = n * s.padded, p.sizes = sizes;
+    if constexpr (kScaled<T>) {
+        const float* const from = weight + first * s.dim;
+        if (s.dim % 4 == 0 && aligned_to(from, 16))
+            unit_sizes_kernel<4><<<grid_of(ceil_div(n, kSizeRows)), 256, 0, stream>>>(from, n, s.dim, sizes);
+        else
+            unit_sizes_kernel<1><<<grid_of(ceil_div(n, kSizeRows)), 256, 0, stream>>>(from, n, s.dim, sizes);
+        return launch_pack<T, kUnitScale>(weight + first * s.dim, packed, p, stream);
+    } else {
+        return launch_pack<T, kNoScale>(weight + first * s.dim, packed, p, stream);
+    }
+}
+
+// The listed rows of the hidden states, packed; of float32, with their exponents.
+template <typename T>
+int pack_hidden(const LossShape& s, const T* hidden, const uint32_t* list, const uint32_t* count, LossPart<T>* packed, int32_t* exponent,
+                hipStream_t stream) {
+    PackArgs p{};
+    p.list = list, p.count = count, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride, p.plane = s.rows * s.padded, p.exponent = exponent;
+    if constexpr (kScaled<T>) {
+        row_exponents_kernel<<<grid_of(ceil_div(s.rows, 4)), 256, 0, stream>>>(hidden, s.hidden_stride, s.dim, list, count, exponent);
+        return launch_pack<T, kRowScale>(hidden, packed, p, stream);
+    } else {
+        return launch_pack<T, kNoScale>(hidden, packed, p, stream);
+    }
 }
 
 template <typename T>
-Operand hidden_operand(const LossShape& s, const Part<T>* packed) {
+Operand hidden_operand(const LossShape& s, const LossPart<T>* packed) {
     return {reinterpret_cast<const char*>(packed), s.padded * 2, s.rows * s.padded * 2, 0, s.rows};
 }
 
@@ -747,15 +889,14 @@ int run_forward(const LossShape& s, int64_t dtype, const T* hidden, const T* wei
     const LossLayout layout(s, dtype, false);
     const Buffers<T> b(layout, s, false, workspace, bytes);
     keep_rows_kernel<<<1, 1024, 0, stream>>>(targets, s.rows, s.vocabulary, b.list, b.count, loss, lse);
-    PackArgs p{};
-    p.list = b.list, p.count = b.count, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride, p.plane = s.rows * s.padded;
-    DLLM_TRY(launch_pack<T>(hidden, b.hidden, p, stream));
-    const bool direct = sizeof(T) == 2 && s.dim % 8 == 0 && aligned_to(weight, 16);
-    const int64_t piece = direct ? s.vocabulary : kPackPiece;
+    DLLM_TRY(pack_hidden<T>(s, hidden, b.list, b.count, b.hidden, b.row_exponent, stream));
+    if (kScaled<T>) DLLM_TRY(fill_words(b.sizes, layout.sizes * 4, 0, stream));
+    const int64_t piece = weights_direct(s, weight) ? s.vocabulary : kPackPiece;
     for (int64_t first = 0; first < s.vocabulary; first += piece) {
         ForwardArgs a{};
         a.s = s, a.hidden = hidden_operand<T>(s, b.hidden);
-        DLLM_TRY(weight_operand<T>(s, weight, b.weight, first, std::min(piece, s.vocabulary - first), a.weight, stream));
+        a.sizes = b.sizes + first / kScaleRows, a.exponent = b.row_exponent;
+        DLLM_TRY(weight_operand<T>(s, weight, b.weight, b.sizes + first / kScaleRows, first, std::min(piece, s.vocabulary - first), a.weight, stream));
         a.first = first, a.list = b.list, a.count = b.count, a.targets = targets, a.stats = b.stats, a.at_target = b.at_target;
         if (s.rows <= 64)
             launch_forward<T, typename SmallTiles<T>::Forward>(a, stream);
@@ -786,7 +927,6 @@ bool large_tiles(const LossShape& s, const LossLayout& l) {
 template <typename T, typename Tiles>
 int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout, const T* weight, bool dhidden, T* dweight, bool accumulate,
                hipStream_t stream) {
-    constexpr bool kHalf = __is_same(T, _Float16);
     using Logits = typename Tiles::Logits;
     using Hidden = typename Tiles::Hidden;
     using Weight = typename Tiles::Weight;
@@ -794,7 +934,8 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
     for (int64_t first = 0; first < s.vocabulary; first += piece) {
         SoftmaxArgs a{};
         a.s = s, a.hidden = hidden_operand<T>(s, b.hidden);
-        DLLM_TRY(weight_operand<T>(s, weight, b.weight, first, std::min(piece, s.vocabulary - first), a.weight, stream));
+        a.sizes = b.sizes + first / kScaleRows;
+        DLLM_TRY(weight_operand<T>(s, weight, b.weight, b.sizes + first / kScaleRows, first, std::min(piece, s.vocabulary - first), a.weight, stream));
         a.first = first, a.count = b.order.kept, a.terms = b.terms, a.out = b.softmax;
         a.out_stride = (piece + kStrideSlack) * 2, a.out_plane = s.rows * a.out_stride;
         const int64_t width = a.weight.count, m = ceil_div(s.rows, Logits::kM), n = ceil_div(width, Logits::kN);
@@ -805,8 +946,8 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
         GradientArgs g{};
         g.softmax = Operand{b.softmax, a.out_stride, a.out_plane, layout.unit * 2, s.rows};
         g.weight = a.weight, g.weight.batch = layout.unit * a.weight.stride;
-        g.hidden = hidden_operand<T>(s, kHalf ? b.scaled : b.hidden);
-        g.count = b.order.kept, g.rows = s.rows, g.dim = s.dim, g.first = first, g.width = width, g.unit = layout.unit;
+        g.hidden = hidden_operand<T>(s, kHalfParts<T> ? b.scaled : b.hidden);
+        g.sizes = a.sizes, g.count = b.order.kept, g.rows = s.rows, g.dim = s.dim, g.first = first, g.width = width, g.unit = layout.unit;
         const int64_t units = ceil_div(width, layout.unit);
         if (dhidden) {
             g.m_tiles = ceil_div(s.rows, Hidden::kM), g.n_tiles = ceil_div(s.dim, Hidden::kN);
@@ -831,25 +972,25 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
 template <typename T>
 int run_backward(const LossShape& s, int64_t dtype, const T* hidden, const T* weight, const int64_t* targets, const float* lse,
                  const float* dloss, T* dhidden, T* dweight, bool accumulate, void* workspace, size_t bytes, hipStream_t stream) {
-    constexpr bool kHalf = __is_same(T, _Float16);
     const LossLayout layout(s, dtype, true);
     const Buffers<T> b(layout, s, true, workspace, bytes);
     // at: -1 everywhere, until the sums say where they are
     DLLM_TRY(sort_tokens(targets, s.rows, s.vocabulary, b.order, b.at, dweight ? layout.at * 4 : 0, ~uint32_t{0}, stream));
     TargetArgs t{};
     t.s = s, t.order = b.order, t.lse = lse, t.dloss = dloss, t.terms = b.terms, t.coefficient = b.coefficient, t.largest = b.largest;
-    if (kHalf) largest_exponent_kernel<<<1, 1024, 0, stream>>>(t);
+    DLLM_TRY(pack_hidden<T>(s, hidden, b.order.position, b.order.kept, b.hidden, b.row_exponent, stream));
+    if (kScaled<T>) DLLM_TRY(fill_words(b.sizes, layout.sizes * 4, 0, stream));
+    if (kHalfParts<T>) largest_exponent_kernel<T><<<1, 1024, 0, stream>>>(t);
     const dim3 by_rows = grid_of(ceil_div(s.rows, 4));
     if (s.softcap != 0.0f)
         target_kernel<T, true><<<by_rows, 256, 0, stream>>>(hidden, weight, t);
     else
         target_kernel<T, false><<<by_rows, 256, 0, stream>>>(hidden, weight, t);
-    PackArgs p{};
-    p.list = b.order.position, p.count = b.order.kept, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride, p.plane = s.rows * s.padded;
-    DLLM_TRY(launch_pack<T>(hidden, b.hidden, p, stream));
-    if (kHalf && dweight) {
+    if constexpr (kHalfParts<T>) {
+        PackArgs p{};
+        p.list = b.order.position, p.count = b.order.kept, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride, p.plane = s.rows * s.padded;
         p.exponent = b.terms.exponent, p.largest = b.largest;
-        DLLM_TRY(launch_pack<T>(hidden, b.scaled, p, stream));
+        if (dweight) DLLM_TRY((launch_pack<T, kWeightScale>(hidden, b.scaled, p, stream)));
     }
     if (dweight) {
         TokenSums sums{};

@@ -392,7 +392,9 @@ int dllm_hip_token_embedding_backward(const dllm_hip_token_embedding_shape* shap
  * float32 before the one rounding. It forms the logits again, a piece of the vocabulary at a time. The softmax's part of a
  * gradient has the probabilities as operands in dtype, the target's part is float32's. float16 holds the probabilities times each
  * row's dloss relative to it, so that gradients of any size keep their bits; in dweight, rows whose dloss is below 2^-14
- * of the largest one's lose some of their softmax's part.
+ * of the largest one's lose some of their softmax's part. float32 has pairs of float16 as operands, 22 bits and more of each
+ * value: hidden states off by at most 2^-39 of their row's largest value (in dweight, of the largest one times its dloss), weights
+ * of 2048 rows' largest, so values far below those lose bits.
  * A row's loss, lse and dhidden are the same bits alone and in any batch. hidden_stride and dhidden_stride: elements between rows (0: dim).
  * Outputs do not overlap inputs. Limits: rows below 2^27, vocabulary below 2^31, their product below 2^48, dim at most 2^16, scale in
  * [2^-60, 2^60], softcap 0 or in [2^-64, 2^64]. */

@@ -34,12 +34,26 @@ def embedding_backward(tokens, dout, vocabulary, scale=1.0, old=None):
     return value, ((unit(dout.dtype) * value.abs() + err) * (1 + unit(dout.dtype)) + tiny(dout.dtype)) * seen
 
 
+def _floors(hidden, weight):
+    """Float32 values are multiplied as pairs of float16, scaled to below 2^15 by their row's (hidden states) or by 2048 rows'
+    (weights) largest: a pair's second part is off by half of float16's least step, 2^-25 there, so 2^-39 of the largest."""
+    if hidden.dtype != torch.float32:
+        return 0.0, 0.0
+    floor = lambda t: 2.0 ** -39 * t.abs().amax()  # noqa: E731
+    units = [floor(u).expand(len(u)) for u in weight.double().split(2048)]
+    return 2.0 ** -39 * hidden.double().abs().amax(dim=1, keepdim=True), torch.cat(units)[:, None]
+
+
 def _logits(hidden, weight, scale, softcap):
     """(z, bound, derivative, its bound)."""
     h, w = hidden.double(), weight.double()
     x = scale * (h @ w.T)
-    # a sum of dim products in any order, and the scale's two roundings; float32's parts leave out 2^-24 of a product each
-    err = (h.shape[1] + 8) * F * scale * (h.abs() @ w.abs().T)
+    # a sum of dim products in any order, and the scale's two roundings; a pair of float16 is off by 2 F at most, and the product
+    # of two pairs' second parts, 4 F, is left out: 8 F of a product
+    err = (h.shape[1] + 16) * F * scale * (h.abs() @ w.abs().T)
+    fh, fw = _floors(hidden, weight)
+    if hidden.dtype == torch.float32:
+        err = err + scale * (fh * w.abs().sum(dim=1) + h.abs().sum(dim=1, keepdim=True) * fw.T)
     slope, es = torch.ones_like(x), torch.zeros_like(x)
     if softcap:
         y = x / softcap
@@ -47,7 +61,7 @@ def _logits(hidden, weight, scale, softcap):
         # tanh to 6 F of itself and its argument's rounding (y F slope, at most F / 2 of the cap's size); the derivative to
         # about 12 F of itself, and twice the argument's error times it, as d slope / dy is at most 2 slope
         err = err * slope + softcap * (8 * F * torch.tanh(y).abs() + 2 * F * y.abs() * slope)
-        es = slope * (16 * F + 2 * (scale / softcap) * (h.shape[1] + 8) * F * (h.abs() @ w.abs().T) + 4 * F * y.abs())
+        es = slope * (16 * F + 2 * (scale / softcap) * (h.shape[1] + 16) * F * (h.abs() @ w.abs().T) + 4 * F * y.abs())
         x = softcap * torch.tanh(y)
     return x, err + 2 * F * x.abs(), slope, es
 
@@ -91,14 +105,22 @@ def loss_backward(hidden, weight, targets, lse, dloss, scale=1.0, softcap=0.0, o
     eg = factor.abs() * (esoft * slope + soft.abs() * es + 6 * F * soft.abs() * slope)
     rounded = (g.abs() + eg) * (1 - hot)  # the target's element stays in float32
     eg = eg + rounded * up
-    if dt == torch.float16:
-        # held times 2^14 relative to the row's weight: near zero off by half of 2^-24 of that
-        eg = eg + (1 - hot) * factor.abs() * 2.0 ** -39
+    if dt != torch.bfloat16:
+        # held times 2^14 relative to the row's weight: near zero off by half of 2^-24 of that; a pair
+        # (float32) by 2 F of itself too
+        eg = eg + (1 - hot) * factor.abs() * 2.0 ** -39 + (2 * F * rounded if dt == torch.float32 else 0.0)
     h, w = hidden.double(), weight.double()
     n = len(weight) + 16
     value, size = g @ w, g.abs() @ w.abs()
-    got = dict(dhidden=(value, eg @ w.abs() + n * F * size))
-    value, bound = g.T @ h, eg.T @ h.abs() + (len(h) + 16) * F * (g.abs().T @ h.abs())
+    got = dict(dhidden=(value, eg @ w.abs() + (n + 16) * F * size))
+    fh, fw = _floors(hidden, weight)
+    if dt == torch.float32:
+        got = dict(dhidden=(value, got["dhidden"][1] + g.abs() @ fw.expand(-1, w.shape[1])))
+    value, bound = g.T @ h, eg.T @ h.abs() + (len(h) + 32) * F * (g.abs().T @ h.abs())
+    if dt == torch.float32:
+        # the hidden states as operands here: below 2^15 by the largest row's, weighted
+        heavy = (factor.abs() * h.abs().amax(dim=1, keepdim=True)).max() * 2.0 ** -38
+        bound = bound + (soft.abs() * (1 - hot) * slope * (factor != 0)).sum(dim=0)[:, None] * heavy
     if dt == torch.float16:
         # the hidden states of light rows are held relative to the heaviest: off by half of 2^-24 there, times the weight
         soft16 = soft.abs() * (1 - hot) * slope * (factor.abs() > 0)
