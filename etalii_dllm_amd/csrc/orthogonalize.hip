@@ -8,8 +8,10 @@
 // the products of 16-bit updates read is its first part: an error of theirs is relative to the term b A X + c A A X, which for
 // small singular values is far smaller than a X.
 //
-// The products' operands are float16, one plane for 16-bit updates (11 bits; bfloat16's 8 would cost its results two bits) and two
-// for float32 ones (22 bits, three products). All values are bounded by the singular values, which stay near one, so fixed
+// The products' operands are float16 (bfloat16's 8 bits would cost results two of theirs): one plane of 11 bits for bfloat16 updates,
+// whose own 8 bits are coarser than what that adds (5e-4 of the result, by its 2-norm), two planes of 22 bits, three products, for
+// float32 and float16 ones, and for small matrices, whose few singular values average no rounding out (2 x 76: 2.5e-3 with
+// one). All values are bounded by the singular values, which stay near one, so fixed
 // powers of two keep them in float16's range: X times 2^4 sqrt(n), A and B times 2^8.
 //
 // A and A A are symmetric: only tiles on and above the diagonal are formed, and stored twice. Where they are few and long, X X^T is
@@ -35,9 +37,9 @@ constexpr int64_t kNormParts = 512;         // at most, of a matrix
 constexpr int kMaxSteps = 64;
 constexpr float kGramScale = 0x1p8f;
 
-// Planes that the products read.
-template <typename T>
-constexpr int kProductPlanes = sizeof(T) == 4 ? 2 : 1;
+// Planes that the products read: of a type and a smaller side m.
+constexpr int64_t kFewSingularValues = 64;
+inline int product_planes(int64_t dtype, int64_t m) { return dtype == kBFloat16 && m > kFewSingularValues ? 1 : 2; }
 
 using Half = _Float16;
 using Half8 = Half __attribute__((ext_vector_type(8)));
@@ -233,9 +235,8 @@ __device__ __forceinline__ void finish_gram(const GramArgs& a, int64_t base, int
     if (i < a.s.m && j < a.s.m_padded) store_parts<kPl>(a.out + base + i * a.s.m_padded + j, a.out_plane, v);
 }
 
-template <typename T, typename Tile>
+template <int kPl, typename Tile>
 __global__ __launch_bounds__(Tile::kThreads) void gram_kernel(GramArgs a, int64_t tiles) {
-    constexpr int kPl = kProductPlanes<T>;
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int64_t each = tiles * (tiles + 1) / 2, at_once = a.part ? a.segments : 1, total = each * a.s.batch * at_once;
     if (block_id() >= total) return;
@@ -267,9 +268,9 @@ __global__ __launch_bounds__(Tile::kThreads) void gram_kernel(GramArgs a, int64_
 }
 
 // Adds the segments' parts in order: 64 x 64 on or above the diagonal, of the `tiles` tiles of kTile that the parts were formed in.
-template <typename T, int kTile>
+template <int kPl, int kTile>
 __global__ __launch_bounds__(kThreads) void join_segments_kernel(GramArgs a, int64_t tiles) {
-    constexpr int kPl = kProductPlanes<T>, kSub = kTile / 64;
+    constexpr int kSub = kTile / 64;
     __shared__ float tile[64][65];
     const int64_t each = tiles * (tiles + 1) / 2 * kSub * kSub;
     if (block_id() >= each * a.s.batch) return;
@@ -373,10 +374,10 @@ __global__ __launch_bounds__(Tile::kThreads) void update_kernel(T* __restrict__ 
 
 // ---- the call ----
 
-template <typename T, int kSize, int kStages, int kTileK = 64>
-using GramTile = TileProduct<Half, kProductPlanes<T>, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, false, kTileK, kStages>;
-template <typename T, int kSize, int kStages, int kTileK = 64>
-using UpdateTile = TileProduct<Half, kProductPlanes<T>, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, true, kTileK, kStages>;
+template <int kPl, int kSize, int kStages>
+using GramTile = TileProduct<Half, kPl, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, false, 64, kStages>;
+template <int kPl, int kSize, int kStages>
+using UpdateTile = TileProduct<Half, kPl, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, true, 64, kStages>;
 
 Matrices matrices_of(const dllm_hip_orthogonalize_shape& sh) {
     Matrices s;
@@ -417,7 +418,7 @@ struct UpdateLayout {
     UpdateLayout(const dllm_hip_orthogonalize_shape& sh, const Matrices& s) {
         norm = static_cast<size_t>(s.batch) * ceil_div(sh.rows, norm_rows(sh));
         planes = 2 * static_cast<size_t>(s.batch) * s.m * s.n_padded;
-        gram = static_cast<size_t>(sh.dtype == kFloat32 ? 2 : 1) * s.batch * s.m * s.m_padded;
+        gram = static_cast<size_t>(product_planes(sh.dtype, s.m)) * s.batch * s.m * s.m_padded;
         part = 0;
         for (const int64_t k : {s.n_padded, s.m})
             if (segments_at_once(s, k)) part = std::max(part, static_cast<size_t>(s.batch) * ceil_div(k, segment_of(s, k)) * s.m * s.m_padded);
@@ -435,28 +436,28 @@ struct UpdateBuffers {
     float* part;
 };
 
-template <typename T, typename Tile>
+template <int kPl, typename Tile>
 void launch_gram_tiles(const GramArgs& g, bool at_once, hipStream_t stream) {
     constexpr int kSize = Tile::kM;
     const int64_t tiles = ceil_div(g.s.m, kSize), all = triangle(g.s, kSize) * g.s.batch;
-    gram_kernel<T, Tile><<<grid_of(all * (at_once ? g.segments : 1)), Tile::kThreads, 0, stream>>>(g, tiles);
-    if (at_once) join_segments_kernel<T, kSize><<<grid_of(all * (kSize / 64) * (kSize / 64)), kThreads, 0, stream>>>(g, tiles);
+    gram_kernel<kPl, Tile><<<grid_of(all * (at_once ? g.segments : 1)), Tile::kThreads, 0, stream>>>(g, tiles);
+    if (at_once) join_segments_kernel<kPl, kSize><<<grid_of(all * (kSize / 64) * (kSize / 64)), kThreads, 0, stream>>>(g, tiles);
 }
 
 // Tiles of 128 where they are enough for the CUs, else of 64 with more of their copies under way: a lone workgroup on a CU waits for
 // them. (192 x 576 in float32: 16 us for X X^T with four stages of 64 x 64 tiles, 29 with two of 128 x 128.)
-template <typename T>
+template <int kPl>
 void launch_gram(GramArgs g, float* part, hipStream_t stream) {
     g.segment = segment_of(g.s, g.k), g.segments = ceil_div(g.k, g.segment);
     const bool at_once = segments_at_once(g.s, g.k);
     g.part = at_once ? part : nullptr;
     const int64_t blocks = triangle(g.s, 128) * g.s.batch * (at_once ? g.segments : 1);
     if (blocks >= 200) {
-        launch_gram_tiles<T, GramTile<T, 128, 2>>(g, at_once, stream);
+        launch_gram_tiles<kPl, GramTile<kPl, 128, 2>>(g, at_once, stream);
     } else if (triangle(g.s, 64) * g.s.batch * (at_once ? g.segments : 1) > 256) {
-        launch_gram_tiles<T, GramTile<T, 64, 4>>(g, at_once, stream);
+        launch_gram_tiles<kPl, GramTile<kPl, 64, 4>>(g, at_once, stream);
     } else {
-        launch_gram_tiles<T, GramTile<T, 64, 8>>(g, at_once, stream);
+        launch_gram_tiles<kPl, GramTile<kPl, 64, 8>>(g, at_once, stream);
     }
 }
 
@@ -466,16 +467,16 @@ void launch_update(const UpdateArgs& u, T* out, hipStream_t stream) {
     update_kernel<T, Tile><<<grid_of(m * n * u.s.batch), Tile::kThreads, 0, stream>>>(out, u, m, n);
 }
 
-template <typename T>
+template <typename T, int kPl>
 int launch_step(const Matrices& s, const UpdateBuffers& b, const double* c, int from, bool last, T* out, hipStream_t stream) {
     const int64_t plane = s.batch * s.m * s.n_padded, gram_plane = s.batch * s.m * s.m_padded;
     const Operand x{reinterpret_cast<const char*>(b.planes[from]), s.n_padded * 2, plane * 2, s.m * s.n_padded * 2, s.m};
     GramArgs g{};
     g.s = s, g.of = x, g.k = s.n_padded, g.out = b.gram, g.out_plane = gram_plane, g.factor = kGramScale / (s.x_scale * s.x_scale);
-    launch_gram<T>(g, b.part, stream);
+    launch_gram<kPl>(g, b.part, stream);
     const Operand gram{reinterpret_cast<const char*>(b.gram), s.m_padded * 2, gram_plane * 2, s.m * s.m_padded * 2, s.m};
     g.of = gram, g.k = s.m, g.out = b.left, g.factor = static_cast<float>(c[2]) / kGramScale, g.first = b.gram, g.first_factor = static_cast<float>(c[1]);
-    launch_gram<T>(g, b.part, stream);
+    launch_gram<kPl>(g, b.part, stream);
     UpdateArgs u{};
     u.s = s, u.left = gram, u.left.base = reinterpret_cast<const char*>(b.left), u.x = x;
     u.from = b.planes[from], u.to = last ? nullptr : b.planes[1 - from], u.plane = plane;
@@ -486,13 +487,13 @@ int launch_step(const Matrices& s, const UpdateBuffers& b, const double* c, int 
     u.whole = length % 8 == 0 && s.out_stride % 8 == 0 && s.out_batch % 8 == 0 && aligned_to(out, 16);
     const int64_t large = ceil_div(s.m, 256) * ceil_div(s.n, 256) * s.batch, middle = ceil_div(s.m, 128) * ceil_div(s.n, 128) * s.batch;
     if (middle < 256 && ceil_div(s.m, 64) * ceil_div(s.n, 64) * s.batch <= 256)
-        launch_update<T, UpdateTile<T, 64, 8>>(u, out, stream);
+        launch_update<T, UpdateTile<kPl, 64, 8>>(u, out, stream);
     else if (middle < 256)
-        launch_update<T, UpdateTile<T, 64, 4>>(u, out, stream);
+        launch_update<T, UpdateTile<kPl, 64, 4>>(u, out, stream);
     else if (ceil_div(large, 256) * 2 <= ceil_div(middle, 512))
-        launch_update<T, UpdateTile<T, 256, 2>>(u, out, stream);
+        launch_update<T, UpdateTile<kPl, 256, 2>>(u, out, stream);
     else
-        launch_update<T, UpdateTile<T, 128, 2>>(u, out, stream);
+        launch_update<T, UpdateTile<kPl, 128, 2>>(u, out, stream);
     return check_launch("orthogonalize");
 }
 
@@ -519,7 +520,15 @@ int run(const dllm_hip_orthogonalize_shape& sh, const Matrices& s, const double*
     static constexpr double kQuintic[3] = {3.4445, -4.7750, 2.0315};
     for (int64_t i = 0; i < sh.steps; ++i) {
         const double* const c = coefficients ? coefficients + 3 * i : kQuintic;
-        DLLM_TRY(launch_step<T>(s, b, c, static_cast<int>(i % 2), i == sh.steps - 1, out, stream));
+        const int from = static_cast<int>(i % 2);
+        const bool last = i == sh.steps - 1;
+        if constexpr (__is_same(T, __bf16)) {
+            if (product_planes(sh.dtype, s.m) == 1) {
+                DLLM_TRY((launch_step<T, 1>(s, b, c, from, last, out, stream)));
+                continue;
+            }
+        }
+        DLLM_TRY((launch_step<T, 2>(s, b, c, from, last, out, stream)));
     }
     return kOk;
 }

@@ -221,11 +221,11 @@ __global__ __launch_bounds__(kSortThreads) void sort_kernel(const int64_t* __res
 
 // One pass over more positions: this workgroup's number of each digit, by digit and workgroup ...
 __global__ __launch_bounds__(kSortThreads) void digit_counts_kernel(const int64_t* __restrict__ tokens, const uint32_t* __restrict__ key,
-                                                                    int64_t n, int64_t vocabulary, int shift, uint32_t* __restrict__ counts) {
+                                                                    int64_t n, int64_t vocabulary, int shift, int64_t each, uint32_t* __restrict__ counts) {
     __shared__ uint32_t of[kDigits];
     for (int i = threadIdx.x; i < kDigits; i += kSortThreads) of[i] = 0;
     __syncthreads();
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortBlock, end = min(n, first + kSortBlock);
+    const int64_t first = static_cast<int64_t>(blockIdx.x) * each, end = min(n, first + each);
     for (int64_t i = first + threadIdx.x; i < end; i += kSortThreads)
         atomicAdd(&of[((key ? key[i] : token_key(tokens[i], vocabulary)) >> shift) & (kDigits - 1)], 1u);
     __syncthreads();
@@ -262,19 +262,19 @@ __global__ __launch_bounds__(kSortThreads) void scan_kernel(uint32_t* __restrict
 // ... and the positions to their places.
 __global__ __launch_bounds__(kSortThreads) void scatter_kernel(const int64_t* __restrict__ tokens, const uint32_t* __restrict__ key_in,
                                                                const uint32_t* __restrict__ position_in, int64_t n, int64_t vocabulary,
-                                                               int shift, const uint32_t* __restrict__ before, uint32_t* __restrict__ key_out,
+                                                               int shift, int rounds, const uint32_t* __restrict__ before, uint32_t* __restrict__ key_out,
                                                                uint32_t* __restrict__ position_out) {
     __shared__ SortCounts counts;
     __shared__ uint32_t keys[kSortBlock];
     __shared__ uint16_t ranks[kSortBlock];
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * kSortBlock;
-    const int here = static_cast<int>(min(n - first, static_cast<int64_t>(kSortBlock)));
+    const int64_t each = static_cast<int64_t>(rounds) * kSortThreads, first = static_cast<int64_t>(blockIdx.x) * each;
+    const int here = static_cast<int>(min(n - first, each));
     for (int i = threadIdx.x; i < here; i += kSortThreads) keys[i] = key_in ? key_in[first + i] : token_key(tokens[first + i], vocabulary);
     __syncthreads();
-    rank_digits(keys, kSortRounds, here, shift, counts, ranks);
+    rank_digits(keys, rounds, here, shift, counts, ranks);
     for (int i = threadIdx.x; i < here; i += kSortThreads) {
         const uint32_t key = keys[i], d = (key >> shift) & (kDigits - 1);
-        const int wave = i / (kWave * kSortRounds);  // the one that ranked it
+        const int wave = i / (kWave * rounds);  // the one that ranked it
         const uint32_t to = before[static_cast<size_t>(d) * gridDim.x + blockIdx.x] + counts.wave[wave][d] + ranks[i];
         key_out[to] = key;
         position_out[to] = position_in ? position_in[first + i] : static_cast<uint32_t>(first + i);
@@ -450,10 +450,16 @@ int launch_sums_of(const TokenSums& s, hipStream_t stream) {
 
 }  // namespace
 
+namespace {
+// Positions of a thread where the sort goes through memory: as many workgroups as one can scan the counts of (23234 tokens took
+// 109 us for the gradient of a small table with workgroups of 16384).
+int sort_rounds(int64_t n) { return static_cast<int>(std::clamp<int64_t>(static_cast<int64_t>(ceil_div(n, 64 * kSortThreads)), 1, kSortRounds)); }
+}  // namespace
+
 TokenOrderSizes::TokenOrderSizes(int64_t tokens) : n(static_cast<size_t>(tokens)) {
-    const size_t blocks = ceil_div(n, kSortBlock);
-    spare = blocks > 1 ? n : 0;
-    counts = blocks > 1 ? blocks * kDigits : 0;
+    const bool memory = tokens > kSortBlock;
+    spare = memory ? n : 0;
+    counts = memory ? ceil_div(n, sort_rounds(tokens) * kSortThreads) * kDigits : 0;
 }
 
 int fill_words(void* at, size_t bytes, uint32_t word, hipStream_t stream) {
@@ -477,16 +483,18 @@ int sort_tokens(const int64_t* tokens, int64_t n, int64_t vocabulary, const Toke
         return check_launch("sort_tokens");
     }
     if (fill_bytes) DLLM_TRY(fill_words(fill_at, fill_bytes, fill, stream));
-    const unsigned blocks = static_cast<unsigned>(ceil_div(n, kSortBlock));
+    const int rounds = sort_rounds(n);
+    const int64_t each = static_cast<int64_t>(rounds) * kSortThreads;
+    const unsigned blocks = static_cast<unsigned>(ceil_div(n, each));
     // the last pass ends in the order's own arrays
     uint32_t *key_in = nullptr, *position_in = nullptr;
     for (int pass = 0; pass < passes; ++pass) {
         const bool own = (passes - 1 - pass) % 2 == 0;
         uint32_t *const key_out = own ? o.token : o.spare_token, *const position_out = own ? o.position : o.spare_position;
         const int shift = pass * kDigitBits;
-        digit_counts_kernel<<<blocks, kSortThreads, 0, stream>>>(tokens, key_in, n, vocabulary, shift, o.counts);
+        digit_counts_kernel<<<blocks, kSortThreads, 0, stream>>>(tokens, key_in, n, vocabulary, shift, each, o.counts);
         scan_kernel<<<1, kSortThreads, 0, stream>>>(o.counts, static_cast<int64_t>(blocks) * kDigits);
-        scatter_kernel<<<blocks, kSortThreads, 0, stream>>>(tokens, key_in, position_in, n, vocabulary, shift, o.counts, key_out, position_out);
+        scatter_kernel<<<blocks, kSortThreads, 0, stream>>>(tokens, key_in, position_in, n, vocabulary, shift, rounds, o.counts, key_out, position_out);
         key_in = key_out, position_in = position_out;
     }
     kept_kernel<<<static_cast<unsigned>(ceil_div(n, 256)), 256, 0, stream>>>(o.token, n, static_cast<uint32_t>(vocabulary), o.kept);

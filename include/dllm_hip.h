@@ -419,8 +419,8 @@ int dllm_hip_vocabulary_loss_backward(const dllm_hip_vocabulary_loss_shape* shap
  *     A = X X^T,   X = a X + (b A + c A A) X
  * (on the transposed matrix where rows exceed cols, which is the same and smaller), and out = scale * X. coefficients: HOST, a, b
  * and c of each step; NULL: 3.4445, -4.7750, 2.0315 in all of them, which bring the singular values near one in about five
- * steps. 16-bit updates are multiplied in float16 with X itself held in float32; float32 ones in pairs of float16,
- * float32's accuracy. Strides in elements between rows and between matrices (0: packed). out may be x with the same strides;
+ * steps. X is held as pairs of float16, 22 bits; the products of bfloat16 updates with more than 64 singular values read float16,
+ * all others such pairs. Strides in elements between rows and between matrices (0: packed). out may be x with the same strides;
  * otherwise they do not overlap. Limits: rows and cols at most 2^16, batch at most 65535, steps in [0, 64], eps at least 0,
  * scale and coefficients finite. */
 typedef struct {

@@ -163,11 +163,11 @@ def halves(planes: int):
 def orthogonalize_limits(x, **options):
     """(value, how far in the 2-norm, relative). A rounding's way through the steps is no matter of a few factors (small
     singular values grow by 3.4 in each, errors with them), so the definition is computed with the operands rounded as they are
-    stated to be (float16, or pairs of it for float32), and the kernel may be twice as far away; what float32's sums add
+    stated to be (float16 for bfloat16 matrices with more than 64 on the smaller side, else pairs of it), and the kernel may be twice as far away; what float32's sums add
     (dim terms each, of random sign: the root of their number) is taken from the same steps in float32, twice too."""
     value = orthogonalize(x, **options)
     norm = torch.linalg.norm(value)
-    rounded = orthogonalize(x, rounding=halves(2 if x.dtype == torch.float32 else 1), **options)
+    rounded = orthogonalize(x, rounding=halves(1 if x.dtype == torch.bfloat16 and min(x.shape) > 64 else 2), **options)
     held = orthogonalize(x, rounding=lambda t: t.float().double(), **options)
     sums = steps_in_float32(x, **options)
     off = sum(torch.linalg.norm(t.double() - value) for t in (rounded, held, sums)) * 2 / norm if norm > 0 else 0.0
