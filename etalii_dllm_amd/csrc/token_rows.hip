@@ -232,15 +232,19 @@ __global__ __launch_bounds__(kSortThreads) void digit_counts_kernel(const int64_
     for (int i = threadIdx.x; i < kDigits; i += kSortThreads) counts[static_cast<size_t>(i) * gridDim.x + blockIdx.x] = of[i];
 }
 
-// ... their sums before each, by one workgroup ...
+// ... their sums before each, by one workgroup, 8 to a thread (n is a multiple of 8) ...
 __global__ __launch_bounds__(kSortThreads) void scan_kernel(uint32_t* __restrict__ counts, int64_t n) {
     __shared__ uint32_t carry[kSortWaves];
     const int wave = static_cast<int>(threadIdx.x) >> 6, lane = static_cast<int>(threadIdx.x) & 63;
     uint32_t before = 0;
-    for (int64_t base = 0; base < n; base += kSortThreads) {
-        const int64_t i = base + threadIdx.x;
-        const uint32_t c = i < n ? counts[i] : 0;
-        uint32_t sum = c;
+    for (int64_t base = 0; base < n; base += 8 * kSortThreads) {
+        const int64_t i = base + 8 * threadIdx.x;
+        Pack<uint32_t, 8> c = {};
+        if (i < n) c = *reinterpret_cast<const Pack<uint32_t, 8>*>(counts + i);
+        uint32_t own = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) own += c.v[e];
+        uint32_t sum = own;
 #pragma unroll
         for (int s = 1; s < kWave; s *= 2) {
             const uint32_t o = __shfl_up(sum, s);
@@ -248,13 +252,18 @@ __global__ __launch_bounds__(kSortThreads) void scan_kernel(uint32_t* __restrict
         }
         if (lane == kWave - 1) carry[wave] = sum;
         __syncthreads();
-        uint32_t earlier = 0, all = 0;
+        uint32_t earlier = before + sum - own;
         for (int w = 0; w < kSortWaves; ++w) {
             if (w < wave) earlier += carry[w];
-            all += carry[w];
+            before += carry[w];
         }
-        if (i < n) counts[i] = before + earlier + sum - c;
-        before += all;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const uint32_t one = c.v[e];
+            c.v[e] = earlier;
+            earlier += one;
+        }
+        if (i < n) *reinterpret_cast<Pack<uint32_t, 8>*>(counts + i) = c;
         __syncthreads();
     }
 }

@@ -119,8 +119,8 @@ __global__ __launch_bounds__(1024) void keep_rows_kernel(const int64_t* __restri
 
 // ---- packing ----
 
-// The least e with |x| < 2^e for the float32 of these bits; 0 for zero.
-__device__ __forceinline__ int exponent_of(uint32_t bits) {
+// The least e with |x| < 2^e for the float32 of these bits, x >= 0; 0 for zero.
+__device__ __forceinline__ int exponent_of(int32_t bits) {
     int e = 0;
     if (bits != 0) frexpf(__builtin_bit_cast(float, bits), &e);
     return e;
@@ -138,23 +138,10 @@ __device__ __forceinline__ uint32_t wave_max(uint32_t v) {
     return v;
 }
 
-// The exponent of each listed row's largest value, a wave to a row.
-__global__ __launch_bounds__(256) void row_exponents_kernel(const float* __restrict__ src, int64_t stride, int64_t dim, const uint32_t* __restrict__ list,
-                                                            const uint32_t* __restrict__ count, int32_t* __restrict__ exponent) {
-    const int64_t j = block_id() * 4 + (threadIdx.x >> 6);
-    if (j >= static_cast<int64_t>(*count)) return;
-    const int lane = static_cast<int>(threadIdx.x) & 63;
-    const float* const row = src + static_cast<int64_t>(list[j]) * stride;
-    uint32_t top = 0;
-    for (int64_t d = lane; d < dim; d += kWave) top = max(top, size_bits(row[d]));
-    top = wave_max(top);
-    if (lane == 0) exponent[j] = exponent_of(top);
-}
-
-// The bits of the largest size of each kScaleRows rows, which are zero before. (A maximum, so the order does not matter.)
+// The bits of the largest size of each kScaleRows rows, which are -1 before. (A maximum, so the order does not matter.)
 constexpr int kSizeRows = 64;
 template <int kWidth>
-__global__ __launch_bounds__(256) void unit_sizes_kernel(const float* __restrict__ src, int64_t rows, int64_t dim, uint32_t* __restrict__ sizes) {
+__global__ __launch_bounds__(256) void unit_sizes_kernel(const float* __restrict__ src, int64_t rows, int64_t dim, int32_t* __restrict__ sizes) {
     __shared__ uint32_t of_wave[4];
     const int64_t first = block_id() * kSizeRows;
     if (first >= rows) return;
@@ -170,43 +157,55 @@ __global__ __launch_bounds__(256) void unit_sizes_kernel(const float* __restrict
     top = wave_max(top);
     if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = top;
     __syncthreads();
-    if (threadIdx.x == 0) atomicMax(sizes + first / kScaleRows, max(max(of_wave[0], of_wave[1]), max(of_wave[2], of_wave[3])));
+    if (threadIdx.x == 0)
+        atomicMax(sizes + first / kScaleRows, static_cast<int>(max(max(of_wave[0], of_wave[1]), max(of_wave[2], of_wave[3]))));
 }
 
-// Row list[j] (j itself without a list) of src as chunks of 8 parts, in planes; zeroes past dim. Scaled by a power of two: of the row's
-// exponent (down), of its unit's size, or up by the row's exponent from the largest one.
-enum PackScale { kNoScale, kRowScale, kUnitScale, kWeightScale };
-struct PackArgs {
-    const uint32_t *list, *count;
-    int64_t n, dim, stride, chunks, plane;
-    const int32_t *exponent, *largest;
-    const uint32_t* sizes;
-};
-
-template <typename T, bool kWhole, PackScale kScale>
-__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, LossPart<T>* __restrict__ dst, PackArgs a) {
-    const int64_t i = block_id() * 256 + threadIdx.x;
-    const int64_t j = i / a.chunks, c = i - j * a.chunks;
-    if (j >= (a.count ? static_cast<int64_t>(*a.count) : a.n)) return;
-    const T* const row = src + (a.list ? static_cast<int64_t>(a.list[j]) : j) * a.stride + c * 8;
-    float v[8];
+// 8 elements of a row from column d on, zeroes past dim. kWhole: the row is whole 16-byte chunks.
+template <typename T, bool kWhole>
+__device__ __forceinline__ void load_eight(const T* row, int64_t d, int64_t dim, float (&v)[8]) {
     if constexpr (kWhole) {
 #pragma unroll
         for (int p = 0; p < 8; p += kChunk<T>) {
             float w[kChunk<T>];
-            load_as_float<T, kChunk<T>>(row + p, w);
+            load_as_float<T, kChunk<T>>(row + d + p, w);
 #pragma unroll
             for (int e = 0; e < kChunk<T>; ++e) v[p + e] = w[e];
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = c * 8 + e < a.dim ? static_cast<float>(row[e]) : 0.0f;
+        for (int e = 0; e < 8; ++e) v[e] = d + e < dim ? static_cast<float>(row[d + e]) : 0.0f;
     }
+}
+
+// What scales a row by a power of two: nothing, the size of its unit (weights), or its part in dW (hidden states): factor's exponent
+// and the row's from the largest, zero for none.
+enum PackScale { kNoScale, kUnitScale, kWeightScale };
+constexpr int kNoWeight = -1000;      // the exponent of a factor of zero
+constexpr int kExponentBase = 1000;  // the largest exponent is held with this added, -1 before any
+
+struct PackArgs {
+    const uint32_t *list, *count;
+    int64_t n, dim, stride, chunks, plane;
+    const int32_t *exponent, *largest, *sizes;
+};
+
+// Row list[j] (j itself without a list) of src as chunks of 8 parts, in planes.
+template <typename T, bool kWhole, PackScale kScale>
+__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, LossPart<T>* __restrict__ dst, PackArgs a) {
+    const int64_t i = block_id() * 256 + threadIdx.x;
+    const int64_t j = i / a.chunks, c = i - j * a.chunks;
+    if (j >= (a.count ? static_cast<int64_t>(*a.count) : a.n)) return;
+    float v[8];
+    load_eight<T, kWhole>(src + (a.list ? static_cast<int64_t>(a.list[j]) : j) * a.stride, c * 8, a.dim, v);
     if constexpr (kScale != kNoScale) {
         int by;
-        if constexpr (kScale == kRowScale) by = kTop - a.exponent[j];
-        if constexpr (kScale == kUnitScale) by = kTop - exponent_of(a.sizes[j / kScaleRows]);
-        if constexpr (kScale == kWeightScale) by = a.exponent[j] - *a.largest + (kScaled<T> ? kTop : 0);
+        if constexpr (kScale == kUnitScale) {
+            by = kTop - exponent_of(a.sizes[j / kScaleRows]);
+        } else {
+            const int e = a.exponent[j];
+            by = e == kNoWeight ? 2 * kNoWeight : e - (*a.largest - kExponentBase) + (kScaled<T> ? kTop : 0);
+        }
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], by);
     }
@@ -224,6 +223,163 @@ int launch_pack(const T* src, LossPart<T>* dst, const PackArgs& args, hipStream_
     else
         pack_kernel<T, false, kScale><<<grid, 256, 0, stream>>>(src, dst, a);
     return check_launch("vocabulary_loss packing");
+}
+
+// ---- logits ----
+
+// A logit from its product, and the cap's derivative.
+struct Cap {
+    float scale, softcap, in;
+    __device__ __forceinline__ explicit Cap(const LossShape& s) : scale(s.scale), softcap(s.softcap), in(0.0f) {
+        if (softcap != 0.0f) in = scale / softcap;
+    }
+    template <bool kCapped>
+    __device__ __forceinline__ float logit(float x, float& derivative) const {
+        derivative = 1.0f;
+        if constexpr (!kCapped) return x * scale;
+        return softcap * tanh_of_any_size(x * in, derivative);
+    }
+};
+
+// ---- the listed rows ----
+
+// What a row's gradient is formed from, by its place in the list.
+struct RowTerms {
+    float *lse, *factor;
+    int32_t* target;
+    int32_t* exponent;      // float16 parts: factor holds the weight's mantissa, this the power of two left out
+    int32_t* row_exponent;  // float32: of the hidden states
+};
+
+struct RowsArgs {
+    LossShape s;
+    uint32_t *list, *count;  // kFind: written here
+    char* packed;
+    int64_t plane;
+    int32_t* row_exponent;
+    // kFind
+    const int64_t* targets;
+    float *loss_out, *lse_out;
+    int32_t* sizes;  // set to -1
+    int64_t units;
+    // the backward's
+    TokenOrder order;
+    const float *lse, *dloss;
+    RowTerms terms;
+    float* coefficient;  // by row
+    int32_t* largest;    // float16 parts: kExponentBase and the largest exponent, of float32 with the row's added
+};
+
+// factor = mantissa 2^exponent, mantissa in [1, 2)
+__device__ __forceinline__ void take_apart(float factor, float& mantissa, int& exponent) {
+    int e = 0;
+    mantissa = factor;
+    if (factor != 0.0f && isfinite(factor)) mantissa = 2.0f * frexpf(factor, &e), e -= 1;
+    exponent = factor == 0.0f ? kNoWeight : e;
+}
+
+enum RowsOf { kListed, kFind, kBackward };
+template <RowsOf kOf>
+constexpr int kRowsThreads = kOf == kFind ? 1024 : 256;
+constexpr int64_t kFindRows = 16384;  // the most that every workgroup counts through for itself
+
+// A wave to a listed row: its hidden state in parts, and of the backward, its target's element (the product in float32) and what the
+// softmax's epilogue reads. kFind: the workgroup lists its 16 rows itself, by counting the rows before them.
+template <typename T, bool kWhole, bool kCapped, RowsOf kOf>
+__global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __restrict__ hidden, const T* __restrict__ weight, RowsArgs a) {
+    constexpr int kThreads = kRowsThreads<kOf>, kWaves = kThreads / kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(static_cast<int>(threadIdx.x) >> 6), lane = static_cast<int>(threadIdx.x) & 63;
+    const int64_t first = block_id() * kWaves;
+    int64_t j = first + wave, row;
+    if constexpr (kOf == kFind) {
+        const auto counts = [&](int64_t i) {
+            const int64_t t = i < a.s.rows ? a.targets[i] : -1;
+            return t >= 0 && t < a.s.vocabulary;
+        };
+        int64_t before = 0;
+        for (int64_t base = 0; base < first; base += kThreads) before += __syncthreads_count(base + threadIdx.x < first && counts(base + threadIdx.x));
+        const uint64_t mask = __ballot(lane < kWaves && counts(first + lane));
+        if (block_id() == 0)
+            for (int64_t i = threadIdx.x; i < a.units; i += kThreads) a.sizes[i] = -1;
+        if (first >= a.s.rows) return;
+        if (first + kWaves >= a.s.rows && threadIdx.x == 0) *a.count = static_cast<uint32_t>(before + __popcll(mask));
+        row = first + wave;
+        if (!(mask >> wave & 1)) {
+            if (row < a.s.rows && lane == 0) {
+                if (a.loss_out) a.loss_out[row] = 0.0f;
+                if (a.lse_out) a.lse_out[row] = 0.0f;
+            }
+            return;
+        }
+        j = before + __popcll(mask & ((uint64_t{1} << wave) - 1));
+        if (lane == 0) a.list[j] = static_cast<uint32_t>(row);
+    } else {
+        if (j >= static_cast<int64_t>(*a.count)) return;
+        row = a.list[j];
+    }
+    const T* const h = hidden + row * a.s.hidden_stride;
+    const T* w = nullptr;
+    if constexpr (kOf == kBackward) w = weight + static_cast<int64_t>(a.order.token[j]) * a.s.dim;
+    int exponent = 0;
+    if constexpr (kScaled<T>) {
+        uint32_t top = 0;
+        for (int64_t d = lane; d < a.s.dim; d += kWave) top = max(top, size_bits(h[d]));
+        exponent = exponent_of(static_cast<int32_t>(wave_max(top)));
+        if (lane == 0) a.row_exponent[j] = exponent;
+    }
+    float x = 0.0f;
+    for (int64_t d = lane * 8; d < a.s.padded; d += kWave * 8) {
+        float v[8];
+        load_eight<T, kWhole>(h, d, a.s.dim, v);
+        if constexpr (kOf == kBackward) {
+            float u[8];
+            load_eight<T, kWhole>(w, d, a.s.dim, u);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x = fmaf(v[e], u[e], x);
+        }
+        if constexpr (kScaled<T>) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], kTop - exponent);
+        }
+        store_parts<T>(a.packed + (j * a.s.padded + d) * 2, a.plane, v);
+    }
+    if constexpr (kOf == kBackward) {
+#pragma unroll
+        for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
+        if (lane != 0) return;
+        float derivative;
+        const float z = Cap(a.s).logit<kCapped>(x, derivative), lse = a.lse[row], factor = a.dloss[row] * a.s.scale;
+        a.coefficient[row] = expm1f(z - lse) * derivative * factor;
+        a.terms.lse[j] = lse;
+        a.terms.target[j] = static_cast<int32_t>(a.order.token[j]);
+        if constexpr (kHalfParts<T>) {
+            float mantissa;
+            int e;
+            take_apart(factor, mantissa, e);
+            a.terms.factor[j] = ldexpf(mantissa, kHalfShift);
+            a.terms.exponent[j] = e;
+            if (e != kNoWeight) atomicMax(a.largest, e + exponent + kExponentBase);  // (a maximum, so the order does not matter)
+        } else {
+            a.terms.factor[j] = factor;
+        }
+    }
+}
+
+template <typename T, RowsOf kOf>
+int launch_rows(const T* hidden, const T* weight, const RowsArgs& a, hipStream_t stream) {
+    constexpr int kThreads = kRowsThreads<kOf>;
+    const dim3 grid = grid_of(ceil_div(a.s.rows, kThreads / kWave));
+    const bool whole = a.s.dim % 8 == 0 && a.s.hidden_stride % kChunk<T> == 0 && aligned_to(hidden, 16) && (kOf != kBackward || aligned_to(weight, 16));
+    const bool capped = kOf == kBackward && a.s.softcap != 0.0f;
+    if (whole && capped)
+        rows_kernel<T, true, kOf == kBackward, kOf><<<grid, kThreads, 0, stream>>>(hidden, weight, a);
+    else if (whole)
+        rows_kernel<T, true, false, kOf><<<grid, kThreads, 0, stream>>>(hidden, weight, a);
+    else if (capped)
+        rows_kernel<T, false, kOf == kBackward, kOf><<<grid, kThreads, 0, stream>>>(hidden, weight, a);
+    else
+        rows_kernel<T, false, false, kOf><<<grid, kThreads, 0, stream>>>(hidden, weight, a);
+    return check_launch("vocabulary_loss rows");
 }
 
 // ---- tiles ----
@@ -256,22 +412,6 @@ struct SmallTiles {
     using Weight = Product64<T, true, true, 128, 128, 2, 2>;
 };
 
-// ---- logits ----
-
-// A logit from its product, and the cap's derivative.
-struct Cap {
-    float scale, softcap, in;
-    __device__ __forceinline__ explicit Cap(const LossShape& s) : scale(s.scale), softcap(s.softcap), in(0.0f) {
-        if (softcap != 0.0f) in = scale / softcap;
-    }
-    template <bool kCapped>
-    __device__ __forceinline__ float logit(float x, float& derivative) const {
-        derivative = 1.0f;
-        if constexpr (!kCapped) return x * scale;
-        return softcap * tanh_of_any_size(x * in, derivative);
-    }
-};
-
 // ---- forward ----
 
 struct Stat {
@@ -292,7 +432,7 @@ struct ForwardArgs {
     Stat* stats;  // [unit of kStatRows][rows]
     float* at_target;  // [rows]
     const int32_t* exponent;  // float32: by the place in the list
-    const uint32_t* sizes;    // float32: of the piece, by kScaleRows
+    const int32_t* sizes;     // float32: of the piece, by kScaleRows
 };
 
 template <typename T, bool kCapped, typename Tile>
@@ -372,7 +512,14 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const Stat* __restrict_
     const int part = static_cast<int>(threadIdx.x) >> 2, which = static_cast<int>(threadIdx.x) & 3;
     const int64_t row = min(first + which, n - 1);
     Stat s = {-INFINITY, 0.0f};
-    for (int64_t u = part; u < units; u += 64) s = join(s, stats[u * rows + row]);
+    constexpr int kAhead = 8;
+    for (int64_t u = part; u < units; u += 64 * kAhead) {
+        Stat v[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) v[k] = u + 64 * k < units ? stats[(u + 64 * k) * rows + row] : Stat{-INFINITY, 0.0f};
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) s = join(s, v[k]);
+    }
     of[part][which] = s;
     for (int step = 32; step > 0; step >>= 1) {
         __syncthreads();
@@ -387,83 +534,6 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const Stat* __restrict_
 
 // ---- backward ----
 
-// What a row's gradient is formed from, by its place in the list.
-struct RowTerms {
-    float *lse, *factor;
-    int32_t* target;
-    int32_t* exponent;      // float16 parts: factor holds the weight's mantissa, this the power of two left out
-    int32_t* row_exponent;  // float32: of the hidden states
-};
-
-struct TargetArgs {
-    LossShape s;
-    TokenOrder order;
-    const float *lse, *dloss;
-    RowTerms terms;
-    float* coefficient;  // by row
-    int32_t* largest;    // float16 parts: the largest exponent, of float32 with the row's added
-};
-
-// factor = mantissa 2^exponent, mantissa in [1, 2); for zero an exponent so far below all others that what it scales is zero
-constexpr int kNoWeight = -1000;
-__device__ __forceinline__ void take_apart(float factor, float& mantissa, int& exponent) {
-    int e = 0;
-    mantissa = factor;
-    if (factor != 0.0f && isfinite(factor)) mantissa = 2.0f * frexpf(factor, &e), e -= 1;
-    exponent = factor == 0.0f ? kNoWeight : e;
-}
-
-template <typename T>
-__global__ __launch_bounds__(1024) void largest_exponent_kernel(TargetArgs a) {
-    __shared__ int of_wave[16];
-    int top = -400;
-    const int64_t n = *a.order.kept;
-    for (int64_t j = threadIdx.x; j < n; j += 1024) {
-        float mantissa;
-        int e;
-        take_apart(a.dloss[a.order.position[j]] * a.s.scale, mantissa, e);
-        if (kScaled<T> && e != kNoWeight) e += a.terms.row_exponent[j];
-        top = max(top, e);
-    }
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) top = max(top, __shfl_xor(top, s));
-    if ((threadIdx.x & 63) == 0) of_wave[threadIdx.x >> 6] = top;
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) top = max(top, of_wave[w]);
-        *a.largest = top;
-    }
-}
-
-// The target's element of each row's gradient, a wave to a row: the product in float32.
-template <typename T, bool kCapped>
-__global__ __launch_bounds__(256) void target_kernel(const T* __restrict__ hidden, const T* __restrict__ weight, TargetArgs a) {
-    const int64_t j = block_id() * 4 + (threadIdx.x >> 6);
-    if (j >= static_cast<int64_t>(*a.order.kept)) return;
-    const int lane = static_cast<int>(threadIdx.x) & 63;
-    const int64_t row = a.order.position[j], target = a.order.token[j];
-    const T *const h = hidden + row * a.s.hidden_stride, *const w = weight + target * a.s.dim;
-    float x = 0.0f;
-    for (int64_t d = lane; d < a.s.dim; d += kWave) x = fmaf(static_cast<float>(h[d]), static_cast<float>(w[d]), x);
-#pragma unroll
-    for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
-    float derivative;
-    const float z = Cap(a.s).logit<kCapped>(x, derivative), lse = a.lse[row], factor = a.dloss[row] * a.s.scale;
-    if (lane != 0) return;
-    a.coefficient[row] = expm1f(z - lse) * derivative * factor;
-    a.terms.lse[j] = lse;
-    a.terms.target[j] = static_cast<int32_t>(target);
-    if constexpr (kHalfParts<T>) {
-        float mantissa;
-        int e;
-        take_apart(factor, mantissa, e);
-        a.terms.factor[j] = ldexpf(mantissa, kHalfShift);
-        a.terms.exponent[j] = e;
-    } else {
-        a.terms.factor[j] = factor;
-    }
-}
-
 struct SoftmaxArgs {
     LossShape s;
     Operand hidden, weight;
@@ -472,7 +542,7 @@ struct SoftmaxArgs {
     RowTerms terms;
     char* out;  // [rows][piece] parts, in planes
     int64_t out_stride, out_plane;
-    const uint32_t* sizes;  // float32: of the piece, by kScaleRows
+    const int32_t* sizes;  // float32: of the piece, by kScaleRows
 };
 
 // The softmax's part of g, zero past the vocabulary's end and at the targets.
@@ -531,7 +601,7 @@ struct GradientArgs {
     const float* sums;       // the targets' part, by the index in `at`
     const int32_t* at;       // by token, -1: none
     const int32_t* largest;  // float16 parts: the power of two left out
-    const uint32_t* sizes;   // float32: of the piece, by kScaleRows, which are its units
+    const int32_t* sizes;    // float32: of the piece, by kScaleRows, which are whole units
     bool accumulate;
     bool whole;  // dW's rows are whole 16-byte chunks
 };
@@ -549,7 +619,7 @@ __device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, L
         typename Tile::Sums acc;
         Tile::run(a.softmax, a.weight, m * Tile::kM, n * Tile::kN, count, a.dim, min(a.unit, a.width - unit * a.unit), unit, unit, lds, acc);
         const bool store = !a.in_turn || (a.begin && unit == 0);
-        const int by = kScaled<T> ? exponent_of(a.sizes[unit]) - kTop : 0;
+        const int by = kScaled<T> ? exponent_of(a.sizes[unit * a.unit / kScaleRows]) - kTop : 0;
         struct Old {
             float4 v[2];
         };
@@ -598,7 +668,7 @@ __device__ __forceinline__ void weight_tile(T* __restrict__ dweight, const Gradi
     typename Tile::Sums acc;
     Tile::run(a.softmax, a.hidden, m * Tile::kM, n * Tile::kN, a.width, a.dim, *a.count, 0, 0, lds, acc);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
-    const int by = kHalfParts<T> ? *a.largest - kHalfShift - (kScaled<T> ? kTop : 0) : 0;
+    const int by = kHalfParts<T> ? *a.largest - kExponentBase - kHalfShift - (kScaled<T> ? kTop : 0) : 0;
     struct Old {
         int32_t at;
         Pack<T, 8> v;
@@ -672,6 +742,7 @@ struct FinishArgs {
     TokenOrder order;
     RowTerms terms;
     const float *total, *coefficient;
+    int64_t parts;  // total: so many units' parts, added here
 };
 
 template <typename T>
@@ -689,6 +760,15 @@ __global__ __launch_bounds__(256) void finish_hidden_kernel(const T* __restrict_
     const int by = kHalfParts<T> ? a.terms.exponent[j] - kHalfShift : 0;
     for (int64_t d = threadIdx.x; d < a.s.dim; d += 256) {
         float v = a.total[j * a.s.dim + d];
+        constexpr int kAhead = 8;
+        for (int64_t u = 1; u < a.parts; u += kAhead) {
+            float w[kAhead];
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k) w[k] = u + k < a.parts ? a.total[((u + k) * a.s.rows + j) * a.s.dim + d] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (u + k < a.parts) v += w[k];
+        }
         if constexpr (kHalfParts<T>) v = ldexpf(v, by);
         out[d] = static_cast<T>(fmaf(c, static_cast<float>(w[d]), v));
     }
@@ -723,20 +803,28 @@ LossShape loss_shape(const dllm_hip_vocabulary_loss_shape& sh) {
 int planes_of(int64_t dtype) { return dtype == kFloat32 ? 2 : 1; }
 
 // Of the vocabulary: one addition to dh. It goes by the vocabulary and type alone, so that a row's bits are its own. Shorter units are
-// more workgroups where rows are few and more additions where they are many; float32's take six times as long.
-int64_t unit_of(const LossShape& s, int64_t dtype) { return dtype == kFloat32 ? kScaleRows : s.vocabulary <= 65536 ? 4096 : 8192; }
+// more workgroups where rows are few and more additions where they are many (94 rows, 5568 x 57: 81 us with 4096); float32's take
+// three times as long and share a scale.
+int64_t unit_of(const LossShape& s, int64_t dtype) {
+    const int64_t most = dtype == kFloat32 ? kScaleRows : s.vocabulary > 65536 ? 8192 : 4096;
+    int64_t unit = 512;
+    while (unit < most && unit * 24 <= s.vocabulary) unit *= 2;  // a dozen at least
+    return unit;
+}
 
-// Units of the backward's piece: as many as keep its softmax within kPieceBytes, at least one.
+// Units of the backward's piece: as many as keep its softmax, and half of its packed weights, within kPieceBytes, at least one.
 int64_t piece_units(const LossShape& s, int64_t dtype) {
     const int64_t unit = unit_of(s, dtype);
-    const size_t bytes = static_cast<size_t>(s.rows) * unit * 2 * planes_of(dtype);
-    const int64_t all = static_cast<int64_t>(ceil_div(s.vocabulary, unit));
-    return std::clamp<int64_t>(static_cast<int64_t>(kPieceBytes / std::max<size_t>(bytes, 1)), 1, all);
+    const size_t bytes = static_cast<size_t>(std::max(s.rows, s.padded / 2)) * unit * 2 * planes_of(dtype);
+    // float32's pieces are whole scales, so that those do not go by the rows either
+    const int64_t together = dtype == kFloat32 ? kScaleRows / unit : 1, groups = static_cast<int64_t>(kPieceBytes / std::max<size_t>(bytes, 1)) / together;
+    const int64_t all = static_cast<int64_t>(ceil_div(s.vocabulary, unit * together));
+    return std::clamp<int64_t>(groups, 1, all) * together;
 }
 
 struct LossLayout {
-    size_t hidden, scaled, weight, list, stats, at_target, row_exponent, sizes;  // forward
-    size_t terms, softmax, part, total, sums, sum_parts, at, coefficient;   // backward
+    size_t hidden, scaled, weight, list, stats, at_target, row_exponent, sizes;  // forward, sizes of both
+    size_t terms, softmax, part, total, sums, sum_parts, at, coefficient;       // backward
     int64_t unit, units;
     size_t bytes;
     LossLayout(const LossShape& s, int64_t dtype, bool backward) {
@@ -768,12 +856,12 @@ struct LossLayout {
         l.add<Stat>(stats);
         l.add<float>(at_target);
         l.add<int32_t>(row_exponent);
-        l.add<uint32_t>(sizes);
+        l.add<int32_t>(1 + sizes + at);  // filled with -1 at once
         if (backward) {
             add_token_order(l, s.rows);
             for (int i = 0; i < 4; ++i) l.add<float>(terms);
             l.add<uint16_t>(softmax);
-            for (const size_t n : {part, total, sums, sum_parts, at, coefficient, size_t{1}}) l.add<float>(n);
+            for (const size_t n : {part, total, sums, sum_parts, coefficient}) l.add<float>(n);
         }
         bytes = l.bytes;
     }
@@ -786,14 +874,11 @@ struct Buffers {
     Stat* stats;
     float* at_target;
     int32_t* row_exponent;
-    uint32_t* sizes;
+    int32_t *largest, *sizes, *at;
     TokenOrder order;
     RowTerms terms;
     char* softmax;
-    float *part, *total, *sums, *sum_parts;
-    int32_t* at;
-    float* coefficient;
-    int32_t* largest;
+    float *part, *total, *sums, *sum_parts, *coefficient;
     Buffers(const LossLayout& l, const LossShape& s, bool backward, void* workspace, size_t bytes) {
         Carve c(workspace, bytes);
         hidden = c.take<LossPart<T>>(l.hidden);
@@ -804,7 +889,8 @@ struct Buffers {
         stats = c.take<Stat>(l.stats);
         at_target = c.take<float>(l.at_target);
         row_exponent = c.take<int32_t>(l.row_exponent);
-        sizes = c.take<uint32_t>(l.sizes);
+        largest = c.take<int32_t>(1 + l.sizes + l.at);
+        sizes = largest + 1, at = sizes + l.sizes;
         if (!backward) return;
         order = take_token_order(c, s.rows);
         terms.lse = c.take<float>(l.terms);
@@ -817,9 +903,7 @@ struct Buffers {
         total = c.take<float>(l.total);
         sums = c.take<float>(l.sums);
         sum_parts = c.take<float>(l.sum_parts);
-        at = c.take<int32_t>(l.at);
         coefficient = c.take<float>(l.coefficient);
-        largest = c.take<int32_t>(1);
     }
 };
 
@@ -830,7 +914,7 @@ bool weights_direct(const LossShape& s, const T* weight) {
 
 // The weights of a piece as an operand: where they are, or packed. sizes: of the piece.
 template <typename T>
-int weight_operand(const LossShape& s, const T* weight, LossPart<T>* packed, uint32_t* sizes, int64_t first, int64_t n, Operand& op,
+int weight_operand(const LossShape& s, const T* weight, LossPart<T>* packed, int32_t* sizes, int64_t first, int64_t n, Operand& op,
                    hipStream_t stream) {
     op.count = n;
     op.batch = 0;
@@ -855,18 +939,11 @@ int weight_operand(const LossShape& s, const T* weight, LossPart<T>* packed, uin
     }
 }
 
-// The listed rows of the hidden states, packed; of float32, with their exponents.
 template <typename T>
-int pack_hidden(const LossShape& s, const T* hidden, const uint32_t* list, const uint32_t* count, LossPart<T>* packed, int32_t* exponent,
-                hipStream_t stream) {
-    PackArgs p{};
-    p.list = list, p.count = count, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride, p.plane = s.rows * s.padded, p.exponent = exponent;
-    if constexpr (kScaled<T>) {
-        row_exponents_kernel<<<grid_of(ceil_div(s.rows, 4)), 256, 0, stream>>>(hidden, s.hidden_stride, s.dim, list, count, exponent);
-        return launch_pack<T, kRowScale>(hidden, packed, p, stream);
-    } else {
-        return launch_pack<T, kNoScale>(hidden, packed, p, stream);
-    }
+RowsArgs rows_args(const LossShape& s, const Buffers<T>& b) {
+    RowsArgs a{};
+    a.s = s, a.packed = reinterpret_cast<char*>(b.hidden), a.plane = s.rows * s.padded * 2, a.row_exponent = b.row_exponent;
+    return a;
 }
 
 template <typename T>
@@ -888,9 +965,16 @@ int run_forward(const LossShape& s, int64_t dtype, const T* hidden, const T* wei
                 void* workspace, size_t bytes, hipStream_t stream) {
     const LossLayout layout(s, dtype, false);
     const Buffers<T> b(layout, s, false, workspace, bytes);
-    keep_rows_kernel<<<1, 1024, 0, stream>>>(targets, s.rows, s.vocabulary, b.list, b.count, loss, lse);
-    DLLM_TRY(pack_hidden<T>(s, hidden, b.list, b.count, b.hidden, b.row_exponent, stream));
-    if (kScaled<T>) DLLM_TRY(fill_words(b.sizes, layout.sizes * 4, 0, stream));
+    RowsArgs r = rows_args<T>(s, b);
+    r.list = b.list, r.count = b.count;
+    if (s.rows <= kFindRows) {
+        r.targets = targets, r.loss_out = loss, r.lse_out = lse, r.sizes = b.sizes, r.units = layout.sizes;
+        DLLM_TRY((launch_rows<T, kFind>(hidden, weight, r, stream)));
+    } else {
+        keep_rows_kernel<<<1, 1024, 0, stream>>>(targets, s.rows, s.vocabulary, b.list, b.count, loss, lse);
+        if (kScaled<T>) DLLM_TRY(fill_words(b.sizes, layout.sizes * 4, ~uint32_t{0}, stream));
+        DLLM_TRY((launch_rows<T, kListed>(hidden, weight, r, stream)));
+    }
     const int64_t piece = weights_direct(s, weight) ? s.vocabulary : kPackPiece;
     for (int64_t first = 0; first < s.vocabulary; first += piece) {
         ForwardArgs a{};
@@ -926,7 +1010,7 @@ bool large_tiles(const LossShape& s, const LossLayout& l) {
 
 template <typename T, typename Tiles>
 int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout, const T* weight, bool dhidden, T* dweight, bool accumulate,
-               hipStream_t stream) {
+               int64_t& parts, hipStream_t stream) {
     using Logits = typename Tiles::Logits;
     using Hidden = typename Tiles::Hidden;
     using Weight = typename Tiles::Weight;
@@ -954,6 +1038,7 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
             // with tiles for most CUs a tile takes the units in turn, which saves the parts' way through memory
             g.in_turn = g.m_tiles * g.n_tiles >= 160 || units == 1;
             g.hidden_blocks = g.m_tiles * g.n_tiles * (g.in_turn ? 1 : units);
+            if (!g.in_turn && piece >= s.vocabulary) parts = units;
             g.begin = first == 0, g.total = b.total, g.part = b.part;
         }
         if (dweight) {
@@ -962,7 +1047,7 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
             g.whole = s.dim % 8 == 0 && aligned_to(dweight, 16);
         }
         gradient_kernel<T, Hidden, Weight><<<grid_of(g.hidden_blocks + g.weight_m_tiles * g.weight_n_tiles), Hidden::kThreads, 0, stream>>>(dweight, g);
-        if (dhidden && !g.in_turn)
+        if (dhidden && !g.in_turn && piece < s.vocabulary)  // (one piece's parts are added at the end)
             add_parts_kernel<<<static_cast<unsigned>(std::min<size_t>(ceil_div(s.rows * s.dim, 256), 4096)), 256, 0, stream>>>(
                 b.part, b.total, b.order.kept, s.rows, s.dim, static_cast<int>(units), first == 0);
     }
@@ -974,18 +1059,12 @@ int run_backward(const LossShape& s, int64_t dtype, const T* hidden, const T* we
                  const float* dloss, T* dhidden, T* dweight, bool accumulate, void* workspace, size_t bytes, hipStream_t stream) {
     const LossLayout layout(s, dtype, true);
     const Buffers<T> b(layout, s, true, workspace, bytes);
-    // at: -1 everywhere, until the sums say where they are
-    DLLM_TRY(sort_tokens(targets, s.rows, s.vocabulary, b.order, b.at, dweight ? layout.at * 4 : 0, ~uint32_t{0}, stream));
-    TargetArgs t{};
-    t.s = s, t.order = b.order, t.lse = lse, t.dloss = dloss, t.terms = b.terms, t.coefficient = b.coefficient, t.largest = b.largest;
-    DLLM_TRY(pack_hidden<T>(s, hidden, b.order.position, b.order.kept, b.hidden, b.row_exponent, stream));
-    if (kScaled<T>) DLLM_TRY(fill_words(b.sizes, layout.sizes * 4, 0, stream));
-    if (kHalfParts<T>) largest_exponent_kernel<T><<<1, 1024, 0, stream>>>(t);
-    const dim3 by_rows = grid_of(ceil_div(s.rows, 4));
-    if (s.softcap != 0.0f)
-        target_kernel<T, true><<<by_rows, 256, 0, stream>>>(hidden, weight, t);
-    else
-        target_kernel<T, false><<<by_rows, 256, 0, stream>>>(hidden, weight, t);
+    // -1 everywhere: until the rows and weights say how large they are, and the sums where they are
+    DLLM_TRY(sort_tokens(targets, s.rows, s.vocabulary, b.order, b.largest, (1 + layout.sizes + (dweight ? layout.at : 0)) * 4, ~uint32_t{0}, stream));
+    RowsArgs r = rows_args<T>(s, b);
+    r.list = b.order.position, r.count = b.order.kept, r.order = b.order, r.lse = lse, r.dloss = dloss, r.terms = b.terms;
+    r.coefficient = b.coefficient, r.largest = b.largest;
+    DLLM_TRY((launch_rows<T, kBackward>(hidden, weight, r, stream)));
     if constexpr (kHalfParts<T>) {
         PackArgs p{};
         p.list = b.order.position, p.count = b.order.kept, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride, p.plane = s.rows * s.padded;
@@ -998,7 +1077,10 @@ int run_backward(const LossShape& s, int64_t dtype, const T* hidden, const T* we
         sums.rows = hidden, sums.coefficient = b.coefficient, sums.scale = 1.0f, sums.part = b.sum_parts, sums.sums = b.sums, sums.first = b.at;
         DLLM_TRY(launch_token_sums(sums, dtype, stream));
     }
-    const auto pieces = [&](auto tiles) { return run_pieces<T, decltype(tiles)>(s, b, layout, weight, dhidden != nullptr, dweight, accumulate, stream); };
+    int64_t parts = 1;
+    const auto pieces = [&](auto tiles) {
+        return run_pieces<T, decltype(tiles)>(s, b, layout, weight, dhidden != nullptr, dweight, accumulate, parts, stream);
+    };
     if (s.rows <= 64)
         DLLM_TRY(pieces(SmallTiles<T>{}));
     else if (large_tiles(s, layout))
@@ -1006,7 +1088,8 @@ int run_backward(const LossShape& s, int64_t dtype, const T* hidden, const T* we
     else
         DLLM_TRY(pieces(MiddleTiles<T>{}));
     if (dhidden) {
-        FinishArgs f{s, b.order, b.terms, b.total, b.coefficient};
+        FinishArgs f{s, b.order, b.terms, b.total, b.coefficient, 1};
+        if (parts > 1) f.total = b.part, f.parts = parts;
         finish_hidden_kernel<T><<<grid_of(s.rows), 256, 0, stream>>>(weight, dhidden, f);
     }
     return check_launch("vocabulary_loss_backward");

@@ -305,6 +305,21 @@ def test_a_row_alone_and_in_a_batch(K, dtype, vocabulary, dim):
         assert torch.equal(q.backward(dloss[rows].clone())[0], dhidden[rows]), n
 
 
+@pytest.mark.parametrize("dtype", R.DTYPES)
+def test_a_row_alone_and_in_a_batch_of_pieces(K, dtype):
+    """The same of a batch that goes over the vocabulary in several pieces, and lists its rows by a launch of its own."""
+    p, dloss = loss_problem(K, 25, R.DTYPES[dtype], 20000, 20000, 24)
+    loss, lse = (t.clone() for t in p.forward())
+    dhidden, _ = p.backward(dloss)
+    for first, n in [(0, 3), (7000, 90), (19700, 300)]:
+        rows = slice(first, first + n)
+        q = Loss(K, p.hidden[rows].clone(), p.weight, p.targets[rows].clone())
+        got = q.forward()
+        assert torch.equal(got[0], loss[rows]) and torch.equal(got[1], lse[rows]), n
+        assert torch.equal(q.backward(dloss[rows].clone())[0], dhidden[rows]), n
+    assert bool(torch.isfinite(dhidden).all())
+
+
 @pytest.mark.parametrize("size", [1e-6, 1e3])
 def test_float16_loss_gradients_of_any_size(K, size):
     """Upstream gradients far below and above one, and unequal ones."""
