@@ -196,6 +196,26 @@ struct GramArgs {
     float* part;  // [matrix][segment][m][m_padded]: a workgroup forms one segment; NULL: all in turn
 };
 
+// The values [first, end) of 8 alone.
+template <int kPl>
+__device__ __forceinline__ void store_some_parts(Half* out, int64_t plane, const float (&v)[8], int64_t first, int64_t end) {
+    if (first <= 0 && end >= 8) {
+        store_parts<kPl>(out, plane, v);
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        if (e < first || e >= end) continue;
+        float left = v[e];
+#pragma unroll
+        for (int p = 0; p < kPl; ++p) {
+            const Half part = static_cast<Half>(left);
+            out[p * plane + e] = part;
+            left -= static_cast<float>(part);
+        }
+    }
+}
+
 // What a row's 8 values from column j on are added to.
 template <int kPl>
 struct Held {
@@ -223,7 +243,8 @@ __device__ __forceinline__ Held<kPl> hold_gram(const GramArgs& a, int64_t base, 
     return hold_parts<kPl>(a.first + base + i * a.s.m_padded + j, a.out_plane, a.first && i < a.s.m && j < a.s.m_padded);
 }
 
-// 8 values of row i from column j on, finished; zero in the padding
+// 8 values of row i from column j on, finished; zero in the padding. What is left of the diagonal is stored from the right of it
+// (mirror_gram): two planes' products are added in another order there, and which tiles cross the diagonal goes by their size.
 template <int kPl>
 __device__ __forceinline__ void finish_gram(const GramArgs& a, int64_t base, int64_t i, int64_t j, float (&v)[8], const Held<kPl>& first) {
 #pragma unroll
@@ -232,7 +253,13 @@ __device__ __forceinline__ void finish_gram(const GramArgs& a, int64_t base, int
         if (a.first) v[e] = fmaf(a.first_factor, value_of(first, e), v[e]);
         if (i >= a.s.m || j + e >= a.s.m) v[e] = 0.0f;
     }
-    if (i < a.s.m && j < a.s.m_padded) store_parts<kPl>(a.out + base + i * a.s.m_padded + j, a.out_plane, v);
+    if (i < a.s.m && j < a.s.m_padded) store_some_parts<kPl>(a.out + base + i * a.s.m_padded + j, a.out_plane, v, i - j, 8);
+}
+
+// 8 values of column j from row i on, finished, to the row and columns across the diagonal
+template <int kPl>
+__device__ __forceinline__ void mirror_gram(const GramArgs& a, int64_t base, int64_t i, int64_t j, const float (&v)[8]) {
+    if (j < a.s.m && i < a.s.m_padded) store_some_parts<kPl>(a.out + base + j * a.s.m_padded + i, a.out_plane, v, 0, j - i);
 }
 
 template <int kPl, typename Tile>
@@ -259,12 +286,9 @@ __global__ __launch_bounds__(Tile::kThreads) void gram_kernel(GramArgs a, int64_
     }
     Tile::template run<true>(a.of, a.of, m * Tile::kM, n * Tile::kN, a.s.m, a.s.m, a.k, matrix, matrix, (LdsByte*)lds, acc, a.segment);
     by_rows_and_columns<Tile>(
-        acc, (LdsByte*)lds, m != n, [&](int row, int column) { return hold_gram<kPl>(a, base, i0 + row, j0 + column); },
+        acc, (LdsByte*)lds, true, [&](int row, int column) { return hold_gram<kPl>(a, base, i0 + row, j0 + column); },
         [&](int row, int column, float (&v)[8], const Held<kPl>& first) { finish_gram<kPl>(a, base, i0 + row, j0 + column, v, first); },
-        [&](int row, int column, float (&v)[8]) {
-            const int64_t i = i0 + row, j = j0 + column;
-            if (j < a.s.m && i < a.s.m_padded) store_parts<kPl>(a.out + base + j * a.s.m_padded + i, a.out_plane, v);
-        });
+        [&](int row, int column, float (&v)[8]) { mirror_gram<kPl>(a, base, i0 + row, j0 + column, v); });
 }
 
 // Adds the segments' parts in order: 64 x 64 on or above the diagonal, of the `tiles` tiles of kTile that the parts were formed in.
@@ -298,16 +322,14 @@ __global__ __launch_bounds__(kThreads) void join_segments_kernel(GramArgs a, int
 #pragma unroll
         for (int u = 0; u < 8; ++u) tile[(e & 7) * 8 + u][e >> 3] = v[u];
     }
-    if (m == n) return;
     __syncthreads();
 #pragma unroll
     for (int e = threadIdx.x; e < 64 * 8; e += kThreads) {
         const int64_t j = j0 + (e >> 3), i = i0 + (e & 7) * 8;
-        if (j >= a.s.m || i >= a.s.m_padded) continue;
         float v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[u] = tile[e >> 3][(e & 7) * 8 + u];
-        store_parts<kPl>(a.out + base + j * a.s.m_padded + i, a.out_plane, v);
+        mirror_gram<kPl>(a, base, i, j, v);
     }
 }
 
@@ -545,8 +567,9 @@ int check_shape(const dllm_hip_orthogonalize_shape* sh) {
     for (const auto& s : strides) {
         DLLM_REQUIRE(s[0] == 0 || s[0] >= sh->cols, "a row stride must be 0 or at least cols");
         const int64_t row = s[0] ? s[0] : sh->cols;
-        DLLM_REQUIRE(row <= INT64_MAX / (1 << 17), "a row stride is too large");
-        DLLM_REQUIRE(s[1] == 0 || s[1] >= (sh->rows - 1) * row + sh->cols, "a batch stride must be 0 or at least a matrix");
+        DLLM_REQUIRE(row < (int64_t{1} << 32), "a row stride must be below 2^32");
+        DLLM_REQUIRE(s[1] == 0 || (s[1] >= (sh->rows - 1) * row + sh->cols && s[1] < (int64_t{1} << 47)),
+                     "a batch stride must be 0 or at least a matrix, below 2^47");
     }
     // (the workspace of more is no size that a GPU has)
     DLLM_REQUIRE(sh->batch * sh->rows * sh->cols < (int64_t{1} << 40), "too many matrices for one call");

@@ -66,7 +66,7 @@ int check_shape(const dllm_hip_token_embedding_shape* sh) {
     DLLM_REQUIRE(sh->vocabulary >= 1 && sh->vocabulary < (int64_t{1} << 31), "vocabulary must be in [1, 2^31)");
     DLLM_REQUIRE(sh->dim >= 1 && sh->dim <= (1 << 20), "dim must be in [1, 2^20]");
     DLLM_REQUIRE(sh->tokens * sh->dim < (int64_t{1} << 40), "tokens * dim must be below 2^40");
-    DLLM_REQUIRE(sh->stride == 0 || sh->stride >= sh->dim, "a token stride must be 0 or at least dim");
+    DLLM_REQUIRE(sh->stride == 0 || (sh->stride >= sh->dim && sh->stride < (int64_t{1} << 32)), "a token stride must be 0 or at least dim, below 2^32");
     DLLM_REQUIRE(sh->scale >= -0x1p60 && sh->scale <= 0x1p60, "scale must be in [-2^60, 2^60]");
     return kOk;
 }

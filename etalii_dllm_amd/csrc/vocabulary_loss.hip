@@ -786,7 +786,8 @@ int check_shape(const dllm_hip_vocabulary_loss_shape* sh) {
     // in float32 the scale, the cap and their quotient are then ordinary numbers
     DLLM_REQUIRE(sh->softcap == 0.0 || (sh->softcap >= 0x1p-64 && sh->softcap <= 0x1p64), "softcap must be 0 or in [2^-64, 2^64]");
     DLLM_REQUIRE(sh->scale >= 0x1p-60 && sh->scale <= 0x1p60, "scale must be in [2^-60, 2^60]");
-    for (const int64_t s : {sh->hidden_stride, sh->dhidden_stride}) DLLM_REQUIRE(s == 0 || s >= sh->dim, "a row stride must be 0 or at least dim");
+    for (const int64_t s : {sh->hidden_stride, sh->dhidden_stride})
+        DLLM_REQUIRE(s == 0 || (s >= sh->dim && s < (int64_t{1} << 32)), "a row stride must be 0 or at least dim, below 2^32");
     return kOk;
 }
 

@@ -368,7 +368,8 @@ int dllm_hip_residual_norm_backward(const dllm_hip_residual_norm_shape* shape, c
  * zero. With accumulate the sum is added to what dtable holds, in float32 before the one rounding (the table of a model
  * whose embeddings are tied gathers its gradient from both ends), and rows of tokens that do not occur stay as they are.
  * Tokens outside the vocabulary count for nothing. out or dtable do not overlap inputs.
- * Limits: tokens below 2^27, vocabulary below 2^31, dim at most 2^20, tokens * dim below 2^40, scale in [-2^60, 2^60]. */
+ * Limits: tokens below 2^27, vocabulary below 2^31, dim at most 2^20, tokens * dim below 2^40, stride below
+ * 2^32, scale in [-2^60, 2^60]. */
 typedef struct {
     int64_t dtype;
     int64_t tokens, vocabulary, dim;
@@ -396,8 +397,8 @@ int dllm_hip_token_embedding_backward(const dllm_hip_token_embedding_shape* shap
  * value: hidden states off by at most 2^-39 of their row's largest value (in dweight, of the largest one times its dloss), weights
  * of 2048 rows' largest, so values far below those lose bits.
  * A row's loss, lse and dhidden are the same bits alone and in any batch. hidden_stride and dhidden_stride: elements between rows (0: dim).
- * Outputs do not overlap inputs. Limits: rows below 2^27, vocabulary below 2^31, their product below 2^48, dim at most 2^16, scale in
- * [2^-60, 2^60], softcap 0 or in [2^-64, 2^64]. */
+ * Outputs do not overlap inputs. Limits: rows below 2^27, vocabulary below 2^31, their product below 2^48, dim at most 2^16, strides
+ * below 2^32, scale in [2^-60, 2^60], softcap 0 or in [2^-64, 2^64]. */
 typedef struct {
     int64_t dtype;
     int64_t rows, vocabulary, dim;
@@ -421,8 +422,9 @@ int dllm_hip_vocabulary_loss_backward(const dllm_hip_vocabulary_loss_shape* shap
  * and c of each step; NULL: 3.4445, -4.7750, 2.0315 in all of them, which bring the singular values near one in about five
  * steps. X is held as pairs of float16, 22 bits; the products of bfloat16 updates with more than 64 singular values read float16,
  * all others such pairs. Strides in elements between rows and between matrices (0: packed). out may be x with the same strides;
- * otherwise they do not overlap. Limits: rows and cols at most 2^16, batch at most 65535, steps in [0, 64], eps at least 0,
- * scale and coefficients finite. */
+ * otherwise they do not overlap. Limits: rows and cols at most 2^16, batch at most 65535, batch * rows * cols below
+ * 2^40, strides below 2^32 between rows and 2^47 between matrices, steps in [0, 64], eps at least 0, scale and coefficients
+ * finite in float32. */
 typedef struct {
     int64_t dtype;
     int64_t batch, rows, cols;

@@ -204,6 +204,14 @@ def test_loss(K, dtype, rows, vocabulary, dim):
     p.check(dloss)
 
 
+# the largest tiles, tiles that add their units in turn, both at once
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize(("rows", "vocabulary", "dim"), [(1000, 32700, 508), (2100, 5000, 1200), (4096, 16384, 2560)])
+def test_loss_of_large_batches(K, dtype, rows, vocabulary, dim):
+    p, dloss = loss_problem(K, 26, R.DTYPES[dtype], rows, vocabulary, dim, masked=0.05)
+    p.check(dloss, randn(gen(27), vocabulary, dim, dtype=R.DTYPES[dtype], scale=1e-3))
+
+
 @pytest.mark.parametrize("dtype", R.DTYPES)
 @pytest.mark.parametrize("options", [dict(scale=0.25), dict(softcap=3.0), dict(scale=8.0, softcap=5.0), dict(softcap=1e6),
                                      dict(scale=2.0 ** -60, softcap=2.0 ** -64), dict(scale=100.0, softcap=30.0)])
@@ -383,6 +391,20 @@ def test_orthogonalize(K, dtype, batch, rows, cols):
     assert torch.equal(got, update(K, x, scale=0.7))
     one = update(K, x[batch - 1:].clone(), scale=0.7)  # a matrix alone has the bits that it has among others
     assert torch.equal(one[0], got[-1])
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize(("batch", "rows", "cols"), [(1, 130, 4200), (1, 1500, 8900), (65, 2100, 257), (3, 700, 3000)])
+def test_orthogonalize_long_sides(K, dtype, batch, rows, cols):
+    """Sums over a long side in segments, at once (few matrices) and in turn (many): the same bits; the largest tiles."""
+    x = momentum(gen(36), batch, rows, cols, R.DTYPES[dtype])
+    some = [0, batch // 2, batch - 1]
+    got = update(K, x, steps=3)
+    for i in sorted(set(some)):
+        value, limit = R.orthogonalize_limits(x[i], steps=3)
+        off = float(torch.linalg.norm(got[i].double() - value) / torch.linalg.norm(value))
+        assert off <= limit, (i, off, limit)
+        assert torch.equal(update(K, x[i:i + 1].clone(), steps=3)[0], got[i])
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES)

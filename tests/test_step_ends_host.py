@@ -33,7 +33,8 @@ EMBEDDING = dict(dtype=1, tokens=10, vocabulary=100, dim=16, accumulate=0, scale
 @pytest.mark.parametrize(("change", "message"), [
     (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(tokens=-1), "tokens"), (dict(tokens=1 << 27), "tokens"),
     (dict(vocabulary=0), "vocabulary"), (dict(vocabulary=1 << 31), "vocabulary"), (dict(dim=0), "dim"), (dict(dim=(1 << 20) + 1), "dim"),
-    (dict(tokens=1 << 26, dim=1 << 20), "2.40"), (dict(stride=15), "stride"), (dict(stride=-16), "stride"), (dict(scale=math.inf), "scale"),
+    (dict(tokens=1 << 26, dim=1 << 20), "2.40"), (dict(stride=15), "stride"), (dict(stride=-16), "stride"),
+    (dict(stride=1 << 32), "stride"), (dict(scale=math.inf), "scale"),
     (dict(scale=math.nan), "scale"), (dict(scale=2.0 ** 61), "scale"),
 ])
 def test_embedding_refuses_shapes(K, change, message):
@@ -76,6 +77,7 @@ LOSS = dict(dtype=1, rows=10, vocabulary=100, dim=16, accumulate=0, scale=1.0, s
     (dict(dtype=3), "dtype"), (dict(dtype=-1), "dtype"), (dict(rows=-1), "rows"), (dict(rows=1 << 27), "rows"),
     (dict(vocabulary=0), "vocabulary"), (dict(vocabulary=1 << 31), "vocabulary"), (dict(dim=0), "dim"), (dict(dim=(1 << 16) + 1), "dim"),
     (dict(rows=1 << 26, vocabulary=1 << 30), "2.48"), (dict(hidden_stride=15), "stride"), (dict(dhidden_stride=-1), "stride"),
+    (dict(hidden_stride=1 << 32), "stride"),
     (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=math.nan), "scale"), (dict(scale=math.inf), "scale"),
     (dict(scale=1e-40), "scale"), (dict(softcap=-1.0), "softcap"), (dict(softcap=math.nan), "softcap"), (dict(softcap=1e-30), "softcap"),
     (dict(softcap=1e30), "softcap"),
@@ -128,7 +130,7 @@ UPDATE = dict(dtype=1, batch=2, rows=10, cols=20, steps=5, eps=1e-7, scale=1.0, 
     (dict(rows=65537), "rows"), (dict(cols=65537), "cols"), (dict(steps=-1), "steps"), (dict(steps=65), "steps"), (dict(eps=-1e-9), "eps"),
     (dict(eps=math.nan), "eps"), (dict(eps=math.inf), "eps"), (dict(scale=math.nan), "scale"), (dict(scale=1e39), "scale"),
     (dict(x_stride=19), "row stride"), (dict(out_stride=-1), "row stride"), (dict(x_stride=1 << 62), "row stride"),
-    (dict(x_batch_stride=199), "batch stride"), (dict(out_stride=30, out_batch_stride=289), "batch stride"),
+    (dict(x_batch_stride=199), "batch stride"), (dict(x_batch_stride=1 << 47), "batch stride"), (dict(out_stride=30, out_batch_stride=289), "batch stride"),
     (dict(batch=65535, rows=65536, cols=65536), "too many"),
 ])
 def test_orthogonalize_refuses_shapes(K, change, message):
