@@ -53,22 +53,27 @@ struct Matrices {
     float out_scale;
 };
 
-// v as a sum of float16 parts, in kPl planes
+// Where X's values are. kPl 2: pairs as the products read them; kPl 1: the products read the first parts, the second ones are
+// `rest` further.
 template <int kPl>
-__device__ __forceinline__ void store_parts(Half* out, int64_t plane, const float (&v)[8]) {
-    float left[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) left[e] = v[e];
-#pragma unroll
-    for (int p = 0; p < kPl; ++p) {
-        Half8 part;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            part[e] = static_cast<Half>(left[e]);
-            left[e] -= static_cast<float>(part[e]);
-        }
-        *reinterpret_cast<Half8*>(out + p * plane) = part;
+struct Places {
+    int64_t row, rest;  // bytes
+    __host__ __device__ Places(const Matrices& s) : row(s.n_padded * 2 * kPl), rest(kPl == 2 ? kSecond : s.batch * s.m * s.n_padded * 2) {}
+    __device__ __forceinline__ int64_t at(const Matrices& s, int64_t matrix, int64_t i, int64_t j) const {
+        return (matrix * s.m + i) * row + value_at<kPl>(j);
     }
+};
+
+// 8 values as pairs, the second parts `rest` bytes further
+__device__ __forceinline__ void store_pairs(char* to, int64_t rest, const float (&v)[8]) {
+    Half8 first, second;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        first[e] = static_cast<Half>(v[e]);
+        second[e] = static_cast<Half>(v[e] - static_cast<float>(first[e]));
+    }
+    *reinterpret_cast<Half8*>(to) = first;
+    *reinterpret_cast<Half8*>(to + rest) = second;
 }
 
 // ---- norm and start ----
@@ -105,9 +110,9 @@ __global__ __launch_bounds__(kThreads) void squares_kernel(const T* __restrict__
 }
 
 // 64 x 64 of X: from x, or from its transposed. kWide: x's rows are whole chunks of 8.
-template <typename T, bool kWide>
+template <typename T, bool kWide, int kPl>
 __global__ __launch_bounds__(kThreads) void start_kernel(const T* __restrict__ x, const double* __restrict__ part, int64_t parts,
-                                                         Half* __restrict__ planes, int64_t plane, int64_t m_tiles, int64_t n_tiles, Matrices s) {
+                                                         char* __restrict__ out, int64_t m_tiles, int64_t n_tiles, Matrices s) {
     __shared__ float tile[64][65];
     if (block_id() >= m_tiles * n_tiles * s.batch) return;
     const int64_t matrix = block_id() / (m_tiles * n_tiles), in_matrix = block_id() - matrix * m_tiles * n_tiles;
@@ -159,17 +164,20 @@ __global__ __launch_bounds__(kThreads) void start_kernel(const T* __restrict__ x
         float v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[u] = tile[e >> 3][(e & 7) * 8 + u];
-        store_parts<2>(planes + (matrix * s.m + i) * s.n_padded + j, plane, v);
+        const Places<kPl> places(s);
+        store_pairs(out + places.at(s, matrix, i, j), places.rest, v);
     }
 }
 
 // steps 0: out = scale X
-template <typename T>
-__global__ __launch_bounds__(kThreads) void no_steps_kernel(const Half* __restrict__ planes, int64_t plane, T* __restrict__ out, Matrices s) {
+template <typename T, int kPl>
+__global__ __launch_bounds__(kThreads) void no_steps_kernel(const char* __restrict__ x, T* __restrict__ out, Matrices s) {
+    const Places<kPl> places(s);
     const int64_t rows = s.turned ? s.n : s.m, cols = s.turned ? s.m : s.n, matrix = blockIdx.y;
     for (int64_t e = static_cast<int64_t>(blockIdx.x) * kThreads + threadIdx.x; e < rows * cols; e += static_cast<int64_t>(gridDim.x) * kThreads) {
-        const int64_t r = e / cols, c = e - r * cols, i = s.turned ? c : r, j = s.turned ? r : c, at = (matrix * s.m + i) * s.n_padded + j;
-        const float v = static_cast<float>(planes[at]) + static_cast<float>(planes[plane + at]);
+        const int64_t r = e / cols, c = e - r * cols, i = s.turned ? c : r, j = s.turned ? r : c;
+        const char* const at = x + places.at(s, matrix, i, j);
+        const float v = static_cast<float>(*reinterpret_cast<const Half*>(at)) + static_cast<float>(*reinterpret_cast<const Half*>(at + places.rest));
         out[matrix * s.out_batch + r * s.out_stride + c] = static_cast<T>(v * (s.out_scale / s.x_scale));
     }
 }
@@ -188,19 +196,18 @@ struct GramArgs {
     Matrices s;
     Operand of;  // both sides
     int64_t k, segment, segments;  // of k
-    Half* out;
-    int64_t out_plane;
+    char* out;
     float factor;       // of the product
-    const Half* first;  // with it, plus first_factor times this
+    const char* first;  // with it, plus first_factor times this
     float first_factor;
     float* part;  // [matrix][segment][m][m_padded]: a workgroup forms one segment; NULL: all in turn
 };
 
 // The values [first, end) of 8 alone.
 template <int kPl>
-__device__ __forceinline__ void store_some_parts(Half* out, int64_t plane, const float (&v)[8], int64_t first, int64_t end) {
+__device__ __forceinline__ void store_some(char* out, const float (&v)[8], int64_t first, int64_t end) {
     if (first <= 0 && end >= 8) {
-        store_parts<kPl>(out, plane, v);
+        store_eight<Half, kPl>(out, v);
         return;
     }
 #pragma unroll
@@ -210,56 +217,62 @@ __device__ __forceinline__ void store_some_parts(Half* out, int64_t plane, const
 #pragma unroll
         for (int p = 0; p < kPl; ++p) {
             const Half part = static_cast<Half>(left);
-            out[p * plane + e] = part;
+            *reinterpret_cast<Half*>(out + p * kSecond + e * 2) = part;
             left -= static_cast<float>(part);
         }
     }
 }
 
-// What a row's 8 values from column j on are added to.
-template <int kPl>
+// 8 values' parts, of what a result is added to.
+template <int kParts>
 struct Held {
-    Half8 part[kPl];
+    Half8 part[kParts];
 };
 
-template <int kPl>
-__device__ __forceinline__ Held<kPl> hold_parts(const Half* from, int64_t plane, bool inside) {
-    Held<kPl> h;
+template <int kParts>
+__device__ __forceinline__ Held<kParts> hold(const char* from, int64_t rest, bool inside) {
+    Held<kParts> h;
 #pragma unroll
-    for (int p = 0; p < kPl; ++p) h.part[p] = inside ? *reinterpret_cast<const Half8*>(from + p * plane) : Half8{};
+    for (int p = 0; p < kParts; ++p) h.part[p] = inside ? *reinterpret_cast<const Half8*>(from + p * rest) : Half8{};
     return h;
 }
 
-template <int kPl>
-__device__ __forceinline__ float value_of(const Held<kPl>& h, int e) {
+template <int kParts>
+__device__ __forceinline__ float held_value(const Held<kParts>& h, int e) {
     float v = 0.0f;
 #pragma unroll
-    for (int p = kPl - 1; p >= 0; --p) v += static_cast<float>(h.part[p][e]);
+    for (int p = kParts - 1; p >= 0; --p) v += static_cast<float>(h.part[p][e]);
     return v;
 }
 
+// (i, j) of a symmetric matrix
 template <int kPl>
-__device__ __forceinline__ Held<kPl> hold_gram(const GramArgs& a, int64_t base, int64_t i, int64_t j) {
-    return hold_parts<kPl>(a.first + base + i * a.s.m_padded + j, a.out_plane, a.first && i < a.s.m && j < a.s.m_padded);
+__device__ __forceinline__ int64_t gram_at(const Matrices& s, int64_t matrix, int64_t i, int64_t j) {
+    return (matrix * s.m + i) * s.m_padded * 2 * kPl + value_at<kPl>(j);
+}
+
+template <int kPl>
+__device__ __forceinline__ Held<kPl> hold_gram(const GramArgs& a, int64_t matrix, int64_t i, int64_t j) {
+    return hold<kPl>(a.first + gram_at<kPl>(a.s, matrix, i, j), kSecond, a.first && i < a.s.m && j < a.s.m_padded);
 }
 
 // 8 values of row i from column j on, finished; zero in the padding. What is left of the diagonal is stored from the right of it
-// (mirror_gram): two planes' products are added in another order there, and which tiles cross the diagonal goes by their size.
+// (mirror_gram): pairs' products are added in another order there, and which tiles cross the diagonal goes by their size.
 template <int kPl>
-__device__ __forceinline__ void finish_gram(const GramArgs& a, int64_t base, int64_t i, int64_t j, float (&v)[8], const Held<kPl>& first) {
+__device__ __forceinline__ void finish_gram(const GramArgs& a, int64_t matrix, int64_t i, int64_t j, float (&v)[8], const Held<kPl>& first) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
         v[e] *= a.factor;
-        if (a.first) v[e] = fmaf(a.first_factor, value_of(first, e), v[e]);
+        if (a.first) v[e] = fmaf(a.first_factor, held_value(first, e), v[e]);
         if (i >= a.s.m || j + e >= a.s.m) v[e] = 0.0f;
     }
-    if (i < a.s.m && j < a.s.m_padded) store_some_parts<kPl>(a.out + base + i * a.s.m_padded + j, a.out_plane, v, i - j, 8);
+    if (i < a.s.m && j < a.s.m_padded) store_some<kPl>(a.out + gram_at<kPl>(a.s, matrix, i, j), v, i - j, 8);
 }
 
 // 8 values of column j from row i on, finished, to the row and columns across the diagonal
 template <int kPl>
-__device__ __forceinline__ void mirror_gram(const GramArgs& a, int64_t base, int64_t i, int64_t j, const float (&v)[8]) {
-    if (j < a.s.m && i < a.s.m_padded) store_some_parts<kPl>(a.out + base + j * a.s.m_padded + i, a.out_plane, v, 0, j - i);
+__device__ __forceinline__ void mirror_gram(const GramArgs& a, int64_t matrix, int64_t i, int64_t j, const float (&v)[8]) {
+    if (j < a.s.m && i < a.s.m_padded) store_some<kPl>(a.out + gram_at<kPl>(a.s, matrix, j, i), v, 0, j - i);
 }
 
 template <int kPl, typename Tile>
@@ -271,11 +284,11 @@ __global__ __launch_bounds__(Tile::kThreads) void gram_kernel(GramArgs a, int64_
     tile_of(block_id(), total, 1, id, one);
     const int64_t matrix = id / (each * at_once), in_matrix = id - matrix * each * at_once, only = in_matrix / each;
     triangle_of(in_matrix - only * each, m, n);
-    const int64_t i0 = m * Tile::kM + Tile::wave_m(), j0 = n * Tile::kN + Tile::wave_n(), base = matrix * a.s.m * a.s.m_padded;
+    const int64_t i0 = m * Tile::kM + Tile::wave_m(), j0 = n * Tile::kN + Tile::wave_n();
     typename Tile::Sums acc;
     if (a.part) {
         Operand of = a.of;
-        of.base += only * a.segment * 2;
+        of.base += value_at<kPl>(only * a.segment);
         Tile::run(of, of, m * Tile::kM, n * Tile::kN, a.s.m, a.s.m, min(a.segment, a.k - only * a.segment), matrix, matrix, (LdsByte*)lds, acc);
         float* const part = a.part + (matrix * a.segments + only) * a.s.m * a.s.m_padded;
         by_rows<Tile>(acc, (LdsByte*)lds, [](int, int) { return Nothing{}; }, [&](int row, int column, float (&v)[8], Nothing) {
@@ -286,9 +299,9 @@ __global__ __launch_bounds__(Tile::kThreads) void gram_kernel(GramArgs a, int64_
     }
     Tile::template run<true>(a.of, a.of, m * Tile::kM, n * Tile::kN, a.s.m, a.s.m, a.k, matrix, matrix, (LdsByte*)lds, acc, a.segment);
     by_rows_and_columns<Tile>(
-        acc, (LdsByte*)lds, true, [&](int row, int column) { return hold_gram<kPl>(a, base, i0 + row, j0 + column); },
-        [&](int row, int column, float (&v)[8], const Held<kPl>& first) { finish_gram<kPl>(a, base, i0 + row, j0 + column, v, first); },
-        [&](int row, int column, float (&v)[8]) { mirror_gram<kPl>(a, base, i0 + row, j0 + column, v); });
+        acc, (LdsByte*)lds, true, [&](int row, int column) { return hold_gram<kPl>(a, matrix, i0 + row, j0 + column); },
+        [&](int row, int column, float (&v)[8], const Held<kPl>& first) { finish_gram<kPl>(a, matrix, i0 + row, j0 + column, v, first); },
+        [&](int row, int column, float (&v)[8]) { mirror_gram<kPl>(a, matrix, i0 + row, j0 + column, v); });
 }
 
 // Adds the segments' parts in order: 64 x 64 on or above the diagonal, of the `tiles` tiles of kTile that the parts were formed in.
@@ -302,7 +315,7 @@ __global__ __launch_bounds__(kThreads) void join_segments_kernel(GramArgs a, int
     const int sub = static_cast<int>(id % (kSub * kSub));
     int64_t m, n;
     triangle_of(id / (kSub * kSub), m, n);
-    const int64_t i0 = m * kTile + sub / kSub * 64, j0 = n * kTile + sub % kSub * 64, base = matrix * a.s.m * a.s.m_padded;
+    const int64_t i0 = m * kTile + sub / kSub * 64, j0 = n * kTile + sub % kSub * 64;
     const int64_t next = a.s.m * a.s.m_padded;
 #pragma unroll
     for (int e = threadIdx.x; e < 64 * 8; e += kThreads) {
@@ -318,7 +331,7 @@ __global__ __launch_bounds__(kThreads) void join_segments_kernel(GramArgs a, int
                 for (int u = 0; u < 8; ++u) v[u] += w[u];
             }
         }
-        finish_gram<kPl>(a, base, i, j, v, hold_gram<kPl>(a, base, i, j));
+        finish_gram<kPl>(a, matrix, i, j, v, hold_gram<kPl>(a, matrix, i, j));
 #pragma unroll
         for (int u = 0; u < 8; ++u) tile[(e & 7) * 8 + u][e >> 3] = v[u];
     }
@@ -329,16 +342,15 @@ __global__ __launch_bounds__(kThreads) void join_segments_kernel(GramArgs a, int
         float v[8];
 #pragma unroll
         for (int u = 0; u < 8; ++u) v[u] = tile[e >> 3][(e & 7) * 8 + u];
-        mirror_gram<kPl>(a, base, i, j, v);
+        mirror_gram<kPl>(a, matrix, i, j, v);
     }
 }
 
 struct UpdateArgs {
     Matrices s;
     Operand left, x;
-    const Half* from;  // X's planes
-    Half* to;          // the new X's; NULL in the last step
-    int64_t plane;
+    const char* from;  // X
+    char* to;          // the new X; NULL in the last step
     float keep, factor;
     bool whole;  // the result's rows are whole chunks of 8
 };
@@ -360,7 +372,7 @@ __device__ __forceinline__ void store_result(T* to, int64_t left, bool whole, co
     }
 }
 
-template <typename T, typename Tile>
+template <typename T, int kPl, typename Tile>
 __global__ __launch_bounds__(Tile::kThreads) void update_kernel(T* __restrict__ result, UpdateArgs a, int64_t m_tiles, int64_t n_tiles) {
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     if (block_id() >= m_tiles * n_tiles * a.s.batch) return;
@@ -372,19 +384,20 @@ __global__ __launch_bounds__(Tile::kThreads) void update_kernel(T* __restrict__ 
     Tile::run(a.left, a.x, m * Tile::kM, n * Tile::kN, a.s.m, a.s.n_padded, a.s.m, matrix, matrix, (LdsByte*)lds, acc);
     const int64_t i0 = m * Tile::kM + Tile::wave_m(), j0 = n * Tile::kN + Tile::wave_n();
     T* const out = result + matrix * a.s.out_batch;
+    const Places<kPl> places(a.s);
     by_rows_and_columns<Tile>(
         acc, (LdsByte*)lds, !a.to && a.s.turned,
         [&](int row, int column) {
             const int64_t i = i0 + row, j = j0 + column;
-            return hold_parts<2>(a.from + (matrix * a.s.m + i) * a.s.n_padded + j, a.plane, i < a.s.m && j < a.s.n_padded);
+            return hold<2>(a.from + places.at(a.s, matrix, i, j), places.rest, i < a.s.m && j < a.s.n_padded);
         },
         [&](int row, int column, float (&v)[8], const Held<2>& x) {
             const int64_t i = i0 + row, j = j0 + column;
             if (i >= a.s.m || j >= a.s.n_padded) return;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = fmaf(a.keep, value_of(x, e), v[e] * a.factor);
+            for (int e = 0; e < 8; ++e) v[e] = fmaf(a.keep, held_value(x, e), v[e] * a.factor);
             if (a.to)
-                store_parts<2>(a.to + (matrix * a.s.m + i) * a.s.n_padded + j, a.plane, v);
+                store_pairs(a.to + places.at(a.s, matrix, i, j), places.rest, v);
             else if (!a.s.turned)
                 store_result(out + i * a.s.out_stride + j, a.s.n - j, a.whole, v);
         },
@@ -397,16 +410,17 @@ __global__ __launch_bounds__(Tile::kThreads) void update_kernel(T* __restrict__ 
 // ---- the call ----
 
 template <int kPl, int kSize, int kStages>
-using GramTile = TileProduct<Half, kPl, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, false, 64, kStages>;
+using GramTile = TileProduct<Half, kPl, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, false, kStages>;
 template <int kPl, int kSize, int kStages>
-using UpdateTile = TileProduct<Half, kPl, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, true, 64, kStages>;
+using UpdateTile = TileProduct<Half, kPl, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, true, kStages>;
 
 Matrices matrices_of(const dllm_hip_orthogonalize_shape& sh) {
     Matrices s;
     s.batch = sh.batch;
     s.turned = sh.rows > sh.cols;
     s.m = std::min(sh.rows, sh.cols), s.n = std::max(sh.rows, sh.cols);
-    s.m_padded = static_cast<int64_t>(round_up(s.m, 8)), s.n_padded = static_cast<int64_t>(round_up(s.n, 8));
+    const size_t multiple = product_planes(sh.dtype, s.m) == 1 ? kRowMultiple<1> : kRowMultiple<2>;
+    s.m_padded = static_cast<int64_t>(round_up(s.m, multiple)), s.n_padded = static_cast<int64_t>(round_up(s.n, multiple));
     s.in_stride = sh.x_stride ? sh.x_stride : sh.cols;
     s.out_stride = sh.out_stride ? sh.out_stride : sh.cols;
     s.in_batch = sh.x_batch_stride ? sh.x_batch_stride : sh.rows * s.in_stride;
@@ -454,7 +468,7 @@ struct UpdateLayout {
 
 struct UpdateBuffers {
     double* norm;
-    Half *planes[2], *gram, *left;
+    char *x[2], *gram, *left;
     float* part;
 };
 
@@ -483,46 +497,46 @@ void launch_gram(GramArgs g, float* part, hipStream_t stream) {
     }
 }
 
-template <typename T, typename Tile>
+template <typename T, int kPl, typename Tile>
 void launch_update(const UpdateArgs& u, T* out, hipStream_t stream) {
     const int64_t m = ceil_div(u.s.m, Tile::kM), n = ceil_div(u.s.n, Tile::kN);
-    update_kernel<T, Tile><<<grid_of(m * n * u.s.batch), Tile::kThreads, 0, stream>>>(out, u, m, n);
+    update_kernel<T, kPl, Tile><<<grid_of(m * n * u.s.batch), Tile::kThreads, 0, stream>>>(out, u, m, n);
 }
 
 template <typename T, int kPl>
 int launch_step(const Matrices& s, const UpdateBuffers& b, const double* c, int from, bool last, T* out, hipStream_t stream) {
-    const int64_t plane = s.batch * s.m * s.n_padded, gram_plane = s.batch * s.m * s.m_padded;
-    const Operand x{reinterpret_cast<const char*>(b.planes[from]), s.n_padded * 2, plane * 2, s.m * s.n_padded * 2, s.m};
+    const int64_t row = s.n_padded * 2 * kPl, gram_row = s.m_padded * 2 * kPl;
+    const Operand x{b.x[from], row, s.m * row, s.m};
     GramArgs g{};
-    g.s = s, g.of = x, g.k = s.n_padded, g.out = b.gram, g.out_plane = gram_plane, g.factor = kGramScale / (s.x_scale * s.x_scale);
+    g.s = s, g.of = x, g.k = s.n_padded, g.out = b.gram, g.factor = kGramScale / (s.x_scale * s.x_scale);
     launch_gram<kPl>(g, b.part, stream);
-    const Operand gram{reinterpret_cast<const char*>(b.gram), s.m_padded * 2, gram_plane * 2, s.m * s.m_padded * 2, s.m};
+    const Operand gram{b.gram, gram_row, s.m * gram_row, s.m};
     g.of = gram, g.k = s.m, g.out = b.left, g.factor = static_cast<float>(c[2]) / kGramScale, g.first = b.gram, g.first_factor = static_cast<float>(c[1]);
     launch_gram<kPl>(g, b.part, stream);
     UpdateArgs u{};
-    u.s = s, u.left = gram, u.left.base = reinterpret_cast<const char*>(b.left), u.x = x;
-    u.from = b.planes[from], u.to = last ? nullptr : b.planes[1 - from], u.plane = plane;
-    // the last step's result leaves the planes' scale
+    u.s = s, u.left = gram, u.left.base = b.left, u.x = x;
+    u.from = b.x[from], u.to = last ? nullptr : b.x[1 - from];
+    // the last step's result leaves X's scale
     const float unit = last ? s.out_scale / s.x_scale : 1.0f;
     u.keep = static_cast<float>(c[0]) * unit, u.factor = unit / kGramScale;
     const int64_t length = s.turned ? s.m : s.n;
     u.whole = length % 8 == 0 && s.out_stride % 8 == 0 && s.out_batch % 8 == 0 && aligned_to(out, 16);
     const int64_t large = ceil_div(s.m, 256) * ceil_div(s.n, 256) * s.batch, middle = ceil_div(s.m, 128) * ceil_div(s.n, 128) * s.batch;
     if (middle < 256 && ceil_div(s.m, 64) * ceil_div(s.n, 64) * s.batch <= 256)
-        launch_update<T, UpdateTile<kPl, 64, 8>>(u, out, stream);
+        launch_update<T, kPl, UpdateTile<kPl, 64, 8>>(u, out, stream);
     else if (middle < 256)
-        launch_update<T, UpdateTile<kPl, 64, 4>>(u, out, stream);
+        launch_update<T, kPl, UpdateTile<kPl, 64, 4>>(u, out, stream);
     else if (ceil_div(large, 256) * 2 <= ceil_div(middle, 512))
-        launch_update<T, UpdateTile<kPl, 256, 2>>(u, out, stream);
+        launch_update<T, kPl, UpdateTile<kPl, 256, 2>>(u, out, stream);
     else
-        launch_update<T, UpdateTile<kPl, 128, 2>>(u, out, stream);
+        launch_update<T, kPl, UpdateTile<kPl, 128, 2>>(u, out, stream);
     return check_launch("orthogonalize");
 }
 
-template <typename T>
-int run(const dllm_hip_orthogonalize_shape& sh, const Matrices& s, const double* coefficients, const T* x, T* out, const UpdateBuffers& b,
-        hipStream_t stream) {
-    const int64_t parts = ceil_div(sh.rows, norm_rows(sh)), plane = s.batch * s.m * s.n_padded;
+template <typename T, int kPl>
+int run_planes(const dllm_hip_orthogonalize_shape& sh, const Matrices& s, const double* coefficients, const T* x, T* out, const UpdateBuffers& b,
+               hipStream_t stream) {
+    const int64_t parts = ceil_div(sh.rows, norm_rows(sh));
     constexpr int kWide = kChunk<T>;
     const bool chunks = sh.cols % kWide == 0 && s.in_stride % kWide == 0 && s.in_batch % kWide == 0 && aligned_to(x, 16);
     if (chunks)
@@ -531,28 +545,29 @@ int run(const dllm_hip_orthogonalize_shape& sh, const Matrices& s, const double*
         squares_kernel<T, 1><<<grid_of(parts * s.batch), kThreads, 0, stream>>>(x, b.norm, sh.rows, sh.cols, norm_rows(sh), parts, s);
     const int64_t m_tiles = ceil_div(s.m, 64), n_tiles = ceil_div(s.n_padded, 64);
     if (chunks && sh.cols % 8 == 0)
-        start_kernel<T, true><<<grid_of(m_tiles * n_tiles * s.batch), kThreads, 0, stream>>>(x, b.norm, parts, b.planes[0], plane, m_tiles, n_tiles, s);
+        start_kernel<T, true, kPl><<<grid_of(m_tiles * n_tiles * s.batch), kThreads, 0, stream>>>(x, b.norm, parts, b.x[0], m_tiles, n_tiles, s);
     else
-        start_kernel<T, false><<<grid_of(m_tiles * n_tiles * s.batch), kThreads, 0, stream>>>(x, b.norm, parts, b.planes[0], plane, m_tiles, n_tiles, s);
+        start_kernel<T, false, kPl><<<grid_of(m_tiles * n_tiles * s.batch), kThreads, 0, stream>>>(x, b.norm, parts, b.x[0], m_tiles, n_tiles, s);
     if (sh.steps == 0) {
         const size_t blocks = std::min<size_t>(ceil_div(s.m * s.n, kThreads), 4096);
-        no_steps_kernel<T><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(s.batch)), kThreads, 0, stream>>>(b.planes[0], plane, out, s);
+        no_steps_kernel<T, kPl><<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(s.batch)), kThreads, 0, stream>>>(b.x[0], out, s);
         return check_launch("orthogonalize");
     }
     static constexpr double kQuintic[3] = {3.4445, -4.7750, 2.0315};
     for (int64_t i = 0; i < sh.steps; ++i) {
         const double* const c = coefficients ? coefficients + 3 * i : kQuintic;
-        const int from = static_cast<int>(i % 2);
-        const bool last = i == sh.steps - 1;
-        if constexpr (__is_same(T, __bf16)) {
-            if (product_planes(sh.dtype, s.m) == 1) {
-                DLLM_TRY((launch_step<T, 1>(s, b, c, from, last, out, stream)));
-                continue;
-            }
-        }
-        DLLM_TRY((launch_step<T, 2>(s, b, c, from, last, out, stream)));
+        DLLM_TRY((launch_step<T, kPl>(s, b, c, static_cast<int>(i % 2), i == sh.steps - 1, out, stream)));
     }
     return kOk;
+}
+
+template <typename T>
+int run(const dllm_hip_orthogonalize_shape& sh, const Matrices& s, const double* coefficients, const void* x, void* out, const UpdateBuffers& b,
+        hipStream_t stream) {
+    if constexpr (__is_same(T, __bf16))
+        if (product_planes(sh.dtype, s.m) == 1)
+            return run_planes<T, 1>(sh, s, coefficients, static_cast<const T*>(x), static_cast<T*>(out), b, stream);
+    return run_planes<T, 2>(sh, s, coefficients, static_cast<const T*>(x), static_cast<T*>(out), b, stream);
 }
 
 int check_shape(const dllm_hip_orthogonalize_shape* sh) {
@@ -602,16 +617,15 @@ int dllm_hip_orthogonalize(const dllm_hip_orthogonalize_shape* sh, const double*
     Carve c(workspace, workspace_bytes);
     UpdateBuffers b;
     b.norm = c.take<double>(layout.norm);
-    b.planes[0] = c.take<Half>(layout.planes);
-    b.planes[1] = c.take<Half>(layout.planes);
-    b.gram = c.take<Half>(layout.gram);
-    b.left = c.take<Half>(layout.gram);
+    for (char*& p : b.x) p = reinterpret_cast<char*>(c.take<Half>(layout.planes));
+    b.gram = reinterpret_cast<char*>(c.take<Half>(layout.gram));
+    b.left = reinterpret_cast<char*>(c.take<Half>(layout.gram));
     b.part = c.take<float>(layout.part);
     auto st = static_cast<hipStream_t>(stream);
     switch (sh->dtype) {
-        case kFloat32: return run<float>(*sh, s, coefficients, static_cast<const float*>(x), static_cast<float*>(out), b, st);
-        case kBFloat16: return run<__bf16>(*sh, s, coefficients, static_cast<const __bf16*>(x), static_cast<__bf16*>(out), b, st);
-        default: return run<_Float16>(*sh, s, coefficients, static_cast<const _Float16*>(x), static_cast<_Float16*>(out), b, st);
+        case kFloat32: return run<float>(*sh, s, coefficients, x, out, b, st);
+        case kBFloat16: return run<__bf16>(*sh, s, coefficients, x, out, b, st);
+        default: return run<_Float16>(*sh, s, coefficients, x, out, b, st);
     }
 }
 

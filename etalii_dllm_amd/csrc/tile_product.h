@@ -2,12 +2,19 @@
 // caller's on the tile in registers.
 //
 // Either operand lies in memory with k along its rows (kRows) or across them (kColumns: k is the row, m or n the column).
-// Tiles of 64 k go through LDS two buffers deep, copied without registers in 16-byte chunks; chunk c of LDS row r lies at place
+// Tiles of 64 k go through LDS in kStages buffers, copied without registers in 16-byte chunks; chunk c of LDS row r lies at place
 // c ^ swizzle(r), so that neither the row reads nor the transposing reads of kColumns tiles (4 rows of 16 columns by 16
 // lanes) meet on a bank. A wave holds a kWaveM x kWaveN part of the tile as blocks of 32 x 32.
 //
-// Float32 operands come as planes of 16-bit parts: three of bfloat16, six products, or two of float16, three products; the
-// smaller products first. The k loop runs once for each pair.
+// kPlanes 2: a value is a pair of 16-bit parts, multiplied as three products (second by first, first by second, first by first).
+// A row holds 32 values' first parts, then their second parts, and so on, so a tile of 32 k has the bytes, lines and LDS places of
+// one of 64 single values. (In planes of their own, multiplied pair after pair, the parts were read three times for two.)
+//
+// Measured, plain products of random bfloat16 values, 8192 x 8192: 1040 TFLOP/s over 1536 k and 1070 to 1230 over 8192 (256 x 256
+// tiles), 1020 and 1120 (128 x 128, two workgroups to a CU); a library product reaches 1148. The matrix cores are busy 60% of
+// the time at 1.86 GHz, to which power lowers the clock. Reading a step's operands ahead of the products before it, also over the
+// stages' barrier, gave nothing; shorter stages (32 k), three and four of them, are slower where rows of 64 bytes are
+// read, and wave priorities did not matter.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -18,86 +25,102 @@
 
 namespace dllm_hip {
 
-// Bytes; base and strides are multiples of 16. kRows: m or n rows of k elements. kColumns: k rows of m or n elements, each
-// readable up to the next multiple of 8 elements. `count`: how many m or n there are; indexes past it repeat others, what
-// they yield is not stored.
+// Bytes; base and strides are multiples of 16. kRows: m or n rows of k values. kColumns: k rows of m or n values, each readable up to
+// the next multiple of 8 values. `count`: how many m or n there are; indexes past it repeat others, what they yield is not
+// stored.
 struct Operand {
     const char* base;
-    int64_t stride, plane, batch;
+    int64_t stride, batch;
     int64_t count;
 };
 
 static __device__ const uint4 kZeroChunk = {0, 0, 0, 0};
 
-template <int kPlanesOf>
-struct PlanePairs {
-    static constexpr int kCount = kPlanesOf == 1 ? 1 : kPlanesOf == 2 ? 3 : 6;
-    // plane of A and of B in pair i
-    static __device__ __forceinline__ int a(int i) {
-        if constexpr (kPlanesOf == 1) return 0;
-        if constexpr (kPlanesOf == 2) return i == 0 ? 1 : 0;
-        return i == 0 ? 2 : i == 2 || i == 3 ? 1 : 0;
+// Where value c of a row begins, in bytes; a pair's second part is kSecond bytes further.
+template <int kPlanes>
+__host__ __device__ __forceinline__ int64_t value_at(int64_t c) {
+    return kPlanes == 1 ? c * 2 : (c >> 5) * 128 + (c & 31) * 2;
+}
+constexpr int kSecond = 64;
+// Values of a row that are there: whole chunks, or whole groups of pairs.
+template <int kPlanes>
+constexpr int kRowMultiple = kPlanes == 1 ? 8 : 32;
+
+// 8 values, from one that is a multiple of 8 in its row on, as parts of type P.
+template <typename P, int kPlanes>
+__device__ __forceinline__ void store_eight(char* to, const float (&v)[8]) {
+    using V = P __attribute__((ext_vector_type(8)));
+    float left[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) left[e] = v[e];
+#pragma unroll
+    for (int p = 0; p < kPlanes; ++p) {
+        V part;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            part[e] = static_cast<P>(left[e]);
+            left[e] -= static_cast<float>(part[e]);
+        }
+        *reinterpret_cast<V*>(to + p * kSecond) = part;
     }
-    static __device__ __forceinline__ int b(int i) {
-        if constexpr (kPlanesOf == 1) return 0;
-        if constexpr (kPlanesOf == 2) return i == 1 ? 1 : 0;
-        return i == 1 ? 2 : i == 2 || i == 4 ? 1 : 0;
-    }
-};
+}
 
 template <int kChunks>
 __device__ __forceinline__ int tile_swizzle(int row) {
     if constexpr (kChunks >= 16) return ((row & 3) << 2) | ((row >> 2) & 3);
-    if constexpr (kChunks == 4) return (row >> 2) & 3;
     return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
 }
 
-// One operand's tile of kSize m or n by kTileK k: its copy to LDS.
-template <int kSize, int kTileK, int kThreads, bool kColumns>
+// One operand's tile of kSize m or n: its copy to LDS.
+template <int kSize, int kPlanes, int kThreads, bool kColumns>
 struct OperandTile {
-    static constexpr int kChunks = kColumns ? kSize / 8 : kTileK / 8;  // of an LDS row
+    static constexpr int kTileK = 64 / kPlanes;
+    static constexpr int kChunks = kColumns ? kSize * kPlanes / 8 : 8;  // of an LDS row
     static constexpr int kRows = kColumns ? kTileK : kSize;
-    static constexpr int kRowBytes = kChunks * 16;
-    static constexpr int kBytes = kRows * kRowBytes;
+    static constexpr int kBytes = kRows * kChunks * 16;
     static constexpr int kTurns = kRows * kChunks / kThreads;
     static constexpr int kTurnRows = kThreads / kChunks;
     static_assert(kRows * kChunks % kThreads == 0 && kThreads % kChunks == 0);
 
     const char* base;  // of the tile's first m or n
-    int64_t stride, plane;
+    int64_t stride;
     uint32_t offset[kTurns];  // of the lane's chunk of each turn
 
     __device__ __forceinline__ static int lds_row(int turn) { return turn * kTurnRows + static_cast<int>(threadIdx.x) / kChunks; }
     __device__ __forceinline__ static int chunk(int turn) {
         return (static_cast<int>(threadIdx.x) % kChunks) ^ tile_swizzle<kChunks>(lds_row(turn));
     }
+    // the first value of a chunk
+    __device__ __forceinline__ static int value_of(int c) { return kPlanes == 1 ? c * 8 : c / 8 * 32 + (c & 3) * 8; }
 
     __device__ __forceinline__ void init(const Operand& op, int64_t first, int64_t count, int64_t batch) {
         stride = op.stride;
-        plane = op.plane;
         const int64_t left = count - first;  // at least 1
-        base = op.base + batch * op.batch + (kColumns ? first * 2 : first * stride);
+        base = op.base + batch * op.batch + (kColumns ? value_at<kPlanes>(first) : first * stride);
 #pragma unroll
         for (int t = 0; t < kTurns; ++t) {
-            const int64_t row = lds_row(t), c = chunk(t);
-            if constexpr (kColumns)
-                offset[t] = static_cast<uint32_t>(row * stride + min(c, (left - 1) / 8) * 16);
-            else
+            const int64_t row = lds_row(t);
+            int c = chunk(t);
+            if constexpr (kColumns) {
+                if (value_of(c) >= left) c = kPlanes == 1 ? static_cast<int>((left - 1) / 8) : static_cast<int>((left - 1) / 32 * 8) + (c & 4);
+                offset[t] = static_cast<uint32_t>(row * stride + c * 16);
+            } else {
                 offset[t] = static_cast<uint32_t>(min(row, left - 1) * stride + c * 16);
+            }
         }
     }
 
-    // The tile from k0 on of plane p to LDS; k at and past `k` are zero.
-    __device__ __forceinline__ void copy(int64_t k0, int64_t k, int p, LdsByte* lds) const {
+    // The tile from k0 on to LDS; k at and past `k` are zero.
+    __device__ __forceinline__ void copy(int64_t k0, int64_t k, LdsByte* lds) const {
         const char* to = (const char*)lds + (static_cast<int>(threadIdx.x) >> 6) * 1024;
-        const char* from = base + p * plane + (kColumns ? k0 * stride : k0 * 2);
+        const char* from = base + (kColumns ? k0 * stride : value_at<kPlanes>(k0));
         if (k0 + kTileK <= k) {
 #pragma unroll
             for (int t = 0; t < kTurns; ++t) copy16_to_lds_s(from, offset[t], to + t * (kThreads * 16));
         } else {
 #pragma unroll
             for (int t = 0; t < kTurns; ++t) {
-                const bool inside = kColumns ? k0 + lds_row(t) < k : k0 + chunk(t) * 8 < k;
+                const bool inside = kColumns ? k0 + lds_row(t) < k : k0 + value_of(chunk(t)) < k;
                 const char* src = inside ? from + offset[t] : reinterpret_cast<const char*>(&kZeroChunk);
                 copy16_to_lds(src, to + t * (kThreads * 16));
             }
@@ -106,11 +129,10 @@ struct OperandTile {
 };
 
 // A lane's reads of blocks of 32 m or n by 16 k from a tile.
-template <int kSize, int kTileK, bool kColumns>
+template <int kSize, int kPlanes, bool kColumns>
 struct OperandView {
-
-    static constexpr int kRowBytes = (kColumns ? kSize / 8 : kTileK / 8) * 16;
-    static constexpr int kChunks = kRowBytes / 16;
+    static constexpr int kChunks = kColumns ? kSize * kPlanes / 8 : 8;
+    static constexpr int kRowBytes = kChunks * 16;
     int at[2];
 
     __device__ __forceinline__ explicit OperandView(int first) {
@@ -125,15 +147,16 @@ struct OperandView {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int r = 8 * half + 4 * t + (i >> 2);
-                const int chunk = first / 8 + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+                const int chunk = first / 32 * (4 * kPlanes) + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
                 at[t] = r * kRowBytes + ((chunk ^ tile_swizzle<kChunks>(r)) << 4) + (i & 1) * 8;
             }
         }
     }
 
-    __device__ __forceinline__ Chunk16 read(const LdsByte* tile, int block, int step) const {
+    // (the places that step, block and plane change are whole bits of the chunk's number)
+    __device__ __forceinline__ Chunk16 read(const LdsByte* tile, int block, int step, int plane) const {
         if constexpr (!kColumns) {
-            return *(const __attribute__((address_space(3))) Chunk16*)(tile + ((at[0] ^ (step << 5)) + block * 32 * kRowBytes));
+            return *(const __attribute__((address_space(3))) Chunk16*)(tile + ((at[0] ^ (step << 5) ^ (plane << 6)) + block * 32 * kRowBytes));
         } else {
             using Half = short __attribute__((ext_vector_type(4)));
             union Both {
@@ -143,7 +166,7 @@ struct OperandView {
 #pragma unroll
             for (int t = 0; t < 2; ++t)
                 both.h[t] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                    (__attribute__((address_space(3))) Half*)(tile + ((at[t] ^ (block << 6)) + step * 16 * kRowBytes)));
+                    (__attribute__((address_space(3))) Half*)(tile + ((at[t] ^ (block << (5 + kPlanes)) ^ (plane << 6)) + step * 16 * kRowBytes)));
             return both.c;
         }
     }
@@ -156,15 +179,17 @@ __device__ __forceinline__ void stage_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kCount) : "memory");
 }
 
-// A tile of kM x kN by kWavesM x kWavesN waves, kTileK k to each of kStages buffers.
-template <typename P, int kPlanesOf, int kM_, int kN_, int kWavesM_, int kWavesN_, bool kAColumns, bool kBColumns, int kTileK = 64, int kStages = 2>
+// A tile of kM x kN by kWavesM x kWavesN waves, with kStages buffers.
+template <typename P, int kPlanesOf, int kM_, int kN_, int kWavesM_, int kWavesN_, bool kAColumns, bool kBColumns, int kStages = 2>
 struct TileProduct {
     static constexpr int kM = kM_, kN = kN_, kWavesM = kWavesM_, kWavesN = kWavesN_;
     static constexpr int kThreads = kWavesM * kWavesN * kWave;
     static constexpr int kWaveM = kM / kWavesM, kWaveN = kN / kWavesN;
     static constexpr int kBlocksM = kWaveM / 32, kBlocksN = kWaveN / 32;
-    using ATile = OperandTile<kM, kTileK, kThreads, kAColumns>;
-    using BTile = OperandTile<kN, kTileK, kThreads, kBColumns>;
+    static constexpr int kTileK = 64 / kPlanesOf;
+    static_assert(kPlanesOf == 1 || kPlanesOf == 2);
+    using ATile = OperandTile<kM, kPlanesOf, kThreads, kAColumns>;
+    using BTile = OperandTile<kN, kPlanesOf, kThreads, kBColumns>;
     static constexpr int kStage = ATile::kBytes + BTile::kBytes;
     static constexpr int kLds = kStages * kStage;
     static constexpr int kCopies = ATile::kTurns + BTile::kTurns;  // of a thread, for one stage
@@ -179,13 +204,12 @@ struct TileProduct {
     template <bool kSegments = false>
     static __device__ __forceinline__ void run(const Operand& a, const Operand& b, int64_t m0, int64_t n0, int64_t a_count, int64_t b_count,
                                                int64_t k, int64_t batch_a, int64_t batch_b, LdsByte* lds, Sums& acc, int64_t segment = 0) {
-        constexpr int kPairs = PlanePairs<kPlanesOf>::kCount;
         ATile at;
         BTile bt;
         at.init(a, m0, a_count, batch_a);
         bt.init(b, n0, b_count, batch_b);
-        const OperandView<kM, kTileK, kAColumns> av(wave_m());
-        const OperandView<kN, kTileK, kBColumns> bv(wave_n());
+        const OperandView<kM, kPlanesOf, kAColumns> av(wave_m());
+        const OperandView<kN, kPlanesOf, kBColumns> bv(wave_n());
         const auto clear = [&] {
 #pragma unroll
             for (int i = 0; i < kBlocksM; ++i)
@@ -193,22 +217,19 @@ struct TileProduct {
                 for (int j = 0; j < kBlocksN; ++j) acc[i][j] = Acc{};
         };
         clear();
-        const int tiles = static_cast<int>((k + kTileK - 1) / kTileK), count = tiles * kPairs;
+        const int count = static_cast<int>((k + kTileK - 1) / kTileK);
         if (count == 0) return;
-        const int segment_tiles = kSegments ? static_cast<int>(segment / kTileK) : tiles;
-        int pair = 0, tile = 0, into = 0, first = 0, end = min(segment_tiles, tiles);  // of the next copy; first, end: of its segment
+        int tile = 0, into = 0;  // of the next copy
         auto copy = [&] {
             LdsByte* const to = lds + into * kStage;
-            at.copy(static_cast<int64_t>(tile) * kTileK, k, PlanePairs<kPlanesOf>::a(pair), to);
-            bt.copy(static_cast<int64_t>(tile) * kTileK, k, PlanePairs<kPlanesOf>::b(pair), to + ATile::kBytes);
-            if (++tile == end) {
-                if (++pair == kPairs && kSegments) pair = 0, first = end, end = min(end + segment_tiles, tiles);
-                tile = first;
-            }
+            at.copy(static_cast<int64_t>(tile) * kTileK, k, to);
+            bt.copy(static_cast<int64_t>(tile) * kTileK, k, to + ATile::kBytes);
+            ++tile;
             into = into + 1 == kStages ? 0 : into + 1;
         };
         for (int i = 0; i < kStages - 1 && i < count; ++i) copy();
-        int from = 0, boundary = segment_tiles * kPairs;
+        const int segment_tiles = kSegments ? static_cast<int>(segment / kTileK) : count;
+        int from = 0, boundary = segment_tiles;
         Sums total;
         if constexpr (kSegments) {
 #pragma unroll
@@ -224,7 +245,7 @@ struct TileProduct {
                 stage_barrier<0>();
             if (i + kStages - 1 < count) copy();
             if (kSegments && i == boundary) {
-                boundary += segment_tiles * kPairs;
+                boundary += segment_tiles;
 #pragma unroll
                 for (int m = 0; m < kBlocksM; ++m)
 #pragma unroll
@@ -235,15 +256,20 @@ struct TileProduct {
             from = from + 1 == kStages ? 0 : from + 1;
 #pragma unroll
             for (int step = 0; step < kTileK / 16; ++step) {
-                Chunk16 x[kBlocksM], y[kBlocksN];
+                Chunk16 x[kPlanesOf][kBlocksM], y[kPlanesOf][kBlocksN];
 #pragma unroll
-                for (int m = 0; m < kBlocksM; ++m) x[m] = av.read(stage, m, step);
+                for (int p = 0; p < kPlanesOf; ++p) {
 #pragma unroll
-                for (int n = 0; n < kBlocksN; ++n) y[n] = bv.read(stage + ATile::kBytes, n, step);
+                    for (int m = 0; m < kBlocksM; ++m) x[p][m] = av.read(stage, m, step, p);
 #pragma unroll
-                for (int m = 0; m < kBlocksM; ++m)
+                    for (int n = 0; n < kBlocksN; ++n) y[p][n] = bv.read(stage + ATile::kBytes, n, step, p);
+                }
 #pragma unroll
-                    for (int n = 0; n < kBlocksN; ++n) multiply<P>(x[m], y[n], acc[m][n]);
+                for (int product = kPlanesOf == 1 ? 2 : 0; product < 3; ++product)
+#pragma unroll
+                    for (int m = 0; m < kBlocksM; ++m)
+#pragma unroll
+                        for (int n = 0; n < kBlocksN; ++n) multiply<P>(x[product == 0][m], y[product == 1][n], acc[m][n]);
             }
         }
         if constexpr (kSegments) {

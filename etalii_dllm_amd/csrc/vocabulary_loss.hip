@@ -62,27 +62,20 @@ constexpr bool kHalfParts = __is_same(LossPart<T>, _Float16);
 template <typename T>
 constexpr bool kScaled = sizeof(T) == 4;
 
-// v's parts, 8 of them to each plane
+// Bytes of a row of n values.
 template <typename T>
-__device__ __forceinline__ void store_parts(char* to, int64_t plane, const float (&v)[8]) {
-    using V = LossPart<T> __attribute__((ext_vector_type(8)));
-    float left[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) left[e] = v[e];
-#pragma unroll
-    for (int q = 0; q < kLossPlanes<T>; ++q) {
-        V out;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            out[e] = static_cast<LossPart<T>>(left[e]);
-            left[e] -= static_cast<float>(out[e]);
-        }
-        *reinterpret_cast<V*>(to + q * plane) = out;
-    }
+constexpr int64_t row_bytes(int64_t n) {
+    return static_cast<int64_t>(round_up(n, kRowMultiple<kLossPlanes<T>>)) * 2 * kLossPlanes<T>;
+}
+
+// 8 values of a row from column c on
+template <typename T>
+__device__ __forceinline__ void store_parts(char* row, int64_t c, const float (&v)[8]) {
+    store_eight<LossPart<T>, kLossPlanes<T>>(row + value_at<kLossPlanes<T>>(c), v);
 }
 
 struct LossShape {
-    int64_t rows, vocabulary, dim, padded;  // padded: dim in whole chunks
+    int64_t rows, vocabulary, dim, padded, row;  // padded: dim in whole chunks; row: bytes of a packed one
     int64_t hidden_stride, dhidden_stride;
     float scale, softcap;
 };
@@ -186,13 +179,13 @@ constexpr int kExponentBase = 1000;  // the largest exponent is held with this a
 
 struct PackArgs {
     const uint32_t *list, *count;
-    int64_t n, dim, stride, chunks, plane;
+    int64_t n, dim, stride, chunks, row;
     const int32_t *exponent, *largest, *sizes;
 };
 
 // Row list[j] (j itself without a list) of src as chunks of 8 parts, in planes.
 template <typename T, bool kWhole, PackScale kScale>
-__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, LossPart<T>* __restrict__ dst, PackArgs a) {
+__global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, char* __restrict__ dst, PackArgs a) {
     const int64_t i = block_id() * 256 + threadIdx.x;
     const int64_t j = i / a.chunks, c = i - j * a.chunks;
     if (j >= (a.count ? static_cast<int64_t>(*a.count) : a.n)) return;
@@ -209,12 +202,13 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, Lo
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], by);
     }
-    store_parts<T>(reinterpret_cast<char*>(dst + i * 8), a.plane * 2, v);
+    store_parts<T>(dst + j * a.row, c * 8, v);
 }
 
 template <typename T, PackScale kScale>
-int launch_pack(const T* src, LossPart<T>* dst, const PackArgs& args, hipStream_t stream) {
+int launch_pack(const T* src, char* dst, const PackArgs& args, hipStream_t stream) {
     PackArgs a = args;
+    a.row = row_bytes<T>(a.dim);
     a.chunks = static_cast<int64_t>(ceil_div(a.dim, 8));
     const bool whole = a.dim % 8 == 0 && a.stride % kChunk<T> == 0 && aligned_to(src, 16);
     const dim3 grid = grid_of(ceil_div(a.n * a.chunks, 256));
@@ -255,7 +249,6 @@ struct RowsArgs {
     LossShape s;
     uint32_t *list, *count;  // kFind: written here
     char* packed;
-    int64_t plane;
     int32_t* row_exponent;
     // kFind
     const int64_t* targets;
@@ -341,7 +334,7 @@ __global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __rest
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], kTop - exponent);
         }
-        store_parts<T>(a.packed + (j * a.s.padded + d) * 2, a.plane, v);
+        store_parts<T>(a.packed + j * a.s.row, d, v);
     }
     if constexpr (kOf == kBackward) {
 #pragma unroll
@@ -388,7 +381,7 @@ int launch_rows(const T* hidden, const T* weight, const RowsArgs& a, hipStream_t
 // the large ones would leave CUs without work or pad much; and for up to 64 rows, whose products wait for the weights'
 // bytes, tiles of 64 rows. The forward's waves hold kStatRows of the vocabulary in all of them.
 template <typename T, bool kAColumns, bool kBColumns, int kM, int kN, int kWavesM, int kWavesN, int kStages = 2>
-using Product64 = TileProduct<LossPart<T>, kLossPlanes<T>, kM, kN, kWavesM, kWavesN, kAColumns, kBColumns, 64, kStages>;
+using Product64 = TileProduct<LossPart<T>, kLossPlanes<T>, kM, kN, kWavesM, kWavesN, kAColumns, kBColumns, kStages>;
 
 template <typename T>
 struct LargeTiles {
@@ -540,8 +533,8 @@ struct SoftmaxArgs {
     int64_t first;  // of the piece, in the vocabulary
     const uint32_t* count;
     RowTerms terms;
-    char* out;  // [rows][piece] parts, in planes
-    int64_t out_stride, out_plane;
+    char* out;  // [rows][piece] parts
+    int64_t out_stride;
     const int32_t* sizes;  // float32: of the piece, by kScaleRows
 };
 
@@ -581,7 +574,7 @@ __global__ __launch_bounds__(Tile::kThreads) void softmax_kernel(SoftmaxArgs a, 
             if constexpr (kCapped) p *= derivative;
             v[e] = e >= left || e == target ? 0.0f : p;
         }
-        store_parts<T>(a.out + row * a.out_stride + column * 2, a.out_plane, v);
+        store_parts<T>(a.out + row * a.out_stride, column, v);
     });
 }
 
@@ -792,9 +785,10 @@ int check_shape(const dllm_hip_vocabulary_loss_shape* sh) {
 }
 
 LossShape loss_shape(const dllm_hip_vocabulary_loss_shape& sh) {
-    LossShape s;
+    LossShape s{};
     s.rows = sh.rows, s.vocabulary = sh.vocabulary, s.dim = sh.dim;
     s.padded = static_cast<int64_t>(round_up(sh.dim, 8));
+    s.row = sh.dtype == kFloat32 ? row_bytes<float>(sh.dim) : row_bytes<_Float16>(sh.dim);
     s.hidden_stride = sh.hidden_stride ? sh.hidden_stride : sh.dim;
     s.dhidden_stride = sh.dhidden_stride ? sh.dhidden_stride : sh.dim;
     s.scale = static_cast<float>(sh.scale), s.softcap = static_cast<float>(sh.softcap);
@@ -832,9 +826,9 @@ struct LossLayout {
         const size_t rows = static_cast<size_t>(s.rows), planes = planes_of(dtype), dim = static_cast<size_t>(s.dim);
         unit = unit_of(s, dtype), units = piece_units(s, dtype);
         const size_t piece = backward ? std::min<size_t>(units * unit, s.vocabulary) : std::min<size_t>(kPackPiece, s.vocabulary);
-        hidden = rows * s.padded * planes;
+        hidden = rows * s.row;
         scaled = backward && dtype != kBFloat16 ? hidden : 0;
-        weight = piece * s.padded * planes;
+        weight = piece * s.row;
         list = backward ? 0 : rows;
         stats = backward ? 0 : ceil_div(s.vocabulary, kStatRows) * rows;
         at_target = backward ? 0 : rows;
@@ -849,9 +843,9 @@ struct LossLayout {
         at = backward ? s.vocabulary : 0;
         coefficient = backward ? rows : 0;
         Layout l;
-        l.add<uint16_t>(hidden);
-        l.add<uint16_t>(scaled);
-        l.add<uint16_t>(weight);
+        l.add<char>(hidden);
+        l.add<char>(scaled);
+        l.add<char>(weight);
         l.add<uint32_t>(list);
         l.add<uint32_t>(1);
         l.add<Stat>(stats);
@@ -870,7 +864,7 @@ struct LossLayout {
 
 template <typename T>
 struct Buffers {
-    LossPart<T>*hidden, *scaled, *weight;
+    char *hidden, *scaled, *weight;
     uint32_t *list, *count;
     Stat* stats;
     float* at_target;
@@ -882,9 +876,9 @@ struct Buffers {
     float *part, *total, *sums, *sum_parts, *coefficient;
     Buffers(const LossLayout& l, const LossShape& s, bool backward, void* workspace, size_t bytes) {
         Carve c(workspace, bytes);
-        hidden = c.take<LossPart<T>>(l.hidden);
-        scaled = c.take<LossPart<T>>(l.scaled);
-        weight = c.take<LossPart<T>>(l.weight);
+        hidden = c.take<char>(l.hidden);
+        scaled = c.take<char>(l.scaled);
+        weight = c.take<char>(l.weight);
         list = c.take<uint32_t>(l.list);
         count = c.take<uint32_t>(1);
         stats = c.take<Stat>(l.stats);
@@ -915,19 +909,18 @@ bool weights_direct(const LossShape& s, const T* weight) {
 
 // The weights of a piece as an operand: where they are, or packed. sizes: of the piece.
 template <typename T>
-int weight_operand(const LossShape& s, const T* weight, LossPart<T>* packed, int32_t* sizes, int64_t first, int64_t n, Operand& op,
+int weight_operand(const LossShape& s, const T* weight, char* packed, int32_t* sizes, int64_t first, int64_t n, Operand& op,
                    hipStream_t stream) {
     op.count = n;
     op.batch = 0;
-    op.stride = s.padded * 2;
-    op.plane = n * s.padded * 2;
+    op.stride = s.row;
     if (weights_direct(s, weight)) {
         op.base = reinterpret_cast<const char*>(weight + first * s.dim);
         return kOk;
     }
-    op.base = reinterpret_cast<const char*>(packed);
+    op.base = packed;
     PackArgs p{};
-    p.n = n, p.dim = s.dim, p.stride = s.dim, p.plane = n * s.padded, p.sizes = sizes;
+    p.n = n, p.dim = s.dim, p.stride = s.dim, p.sizes = sizes;
     if constexpr (kScaled<T>) {
         const float* const from = weight + first * s.dim;
         if (s.dim % 4 == 0 && aligned_to(from, 16))
@@ -943,14 +936,11 @@ int weight_operand(const LossShape& s, const T* weight, LossPart<T>* packed, int
 template <typename T>
 RowsArgs rows_args(const LossShape& s, const Buffers<T>& b) {
     RowsArgs a{};
-    a.s = s, a.packed = reinterpret_cast<char*>(b.hidden), a.plane = s.rows * s.padded * 2, a.row_exponent = b.row_exponent;
+    a.s = s, a.packed = b.hidden, a.row_exponent = b.row_exponent;
     return a;
 }
 
-template <typename T>
-Operand hidden_operand(const LossShape& s, const LossPart<T>* packed) {
-    return {reinterpret_cast<const char*>(packed), s.padded * 2, s.rows * s.padded * 2, 0, s.rows};
-}
+Operand hidden_operand(const LossShape& s, const char* packed) { return {packed, s.row, 0, s.rows}; }
 
 template <typename T, typename Tile>
 void launch_forward(const ForwardArgs& a, hipStream_t stream) {
@@ -979,7 +969,7 @@ int run_forward(const LossShape& s, int64_t dtype, const T* hidden, const T* wei
     const int64_t piece = weights_direct(s, weight) ? s.vocabulary : kPackPiece;
     for (int64_t first = 0; first < s.vocabulary; first += piece) {
         ForwardArgs a{};
-        a.s = s, a.hidden = hidden_operand<T>(s, b.hidden);
+        a.s = s, a.hidden = hidden_operand(s, b.hidden);
         a.sizes = b.sizes + first / kScaleRows, a.exponent = b.row_exponent;
         DLLM_TRY(weight_operand<T>(s, weight, b.weight, b.sizes + first / kScaleRows, first, std::min(piece, s.vocabulary - first), a.weight, stream));
         a.first = first, a.list = b.list, a.count = b.count, a.targets = targets, a.stats = b.stats, a.at_target = b.at_target;
@@ -1018,20 +1008,20 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
     const int64_t piece = layout.units * layout.unit;
     for (int64_t first = 0; first < s.vocabulary; first += piece) {
         SoftmaxArgs a{};
-        a.s = s, a.hidden = hidden_operand<T>(s, b.hidden);
+        a.s = s, a.hidden = hidden_operand(s, b.hidden);
         a.sizes = b.sizes + first / kScaleRows;
         DLLM_TRY(weight_operand<T>(s, weight, b.weight, b.sizes + first / kScaleRows, first, std::min(piece, s.vocabulary - first), a.weight, stream));
         a.first = first, a.count = b.order.kept, a.terms = b.terms, a.out = b.softmax;
-        a.out_stride = (piece + kStrideSlack) * 2, a.out_plane = s.rows * a.out_stride;
+        a.out_stride = row_bytes<T>(piece + kStrideSlack);
         const int64_t width = a.weight.count, m = ceil_div(s.rows, Logits::kM), n = ceil_div(width, Logits::kN);
         if (s.softcap != 0.0f)
             softmax_kernel<T, true, Logits><<<grid_of(m * n), Logits::kThreads, 0, stream>>>(a, m, n);
         else
             softmax_kernel<T, false, Logits><<<grid_of(m * n), Logits::kThreads, 0, stream>>>(a, m, n);
         GradientArgs g{};
-        g.softmax = Operand{b.softmax, a.out_stride, a.out_plane, layout.unit * 2, s.rows};
+        g.softmax = Operand{b.softmax, a.out_stride, value_at<kLossPlanes<T>>(layout.unit), s.rows};
         g.weight = a.weight, g.weight.batch = layout.unit * a.weight.stride;
-        g.hidden = hidden_operand<T>(s, kHalfParts<T> ? b.scaled : b.hidden);
+        g.hidden = hidden_operand(s, kHalfParts<T> ? b.scaled : b.hidden);
         g.sizes = a.sizes, g.count = b.order.kept, g.rows = s.rows, g.dim = s.dim, g.first = first, g.width = width, g.unit = layout.unit;
         const int64_t units = ceil_div(width, layout.unit);
         if (dhidden) {
@@ -1068,7 +1058,7 @@ int run_backward(const LossShape& s, int64_t dtype, const T* hidden, const T* we
     DLLM_TRY((launch_rows<T, kBackward>(hidden, weight, r, stream)));
     if constexpr (kHalfParts<T>) {
         PackArgs p{};
-        p.list = b.order.position, p.count = b.order.kept, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride, p.plane = s.rows * s.padded;
+        p.list = b.order.position, p.count = b.order.kept, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride;
         p.exponent = b.terms.exponent, p.largest = b.largest;
         if (dweight) DLLM_TRY((launch_pack<T, kWeightScale>(hidden, b.scaled, p, stream)));
     }
