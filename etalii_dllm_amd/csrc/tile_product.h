@@ -1,4 +1,4 @@
-// Tiled products on the 16-bit matrix cores: C[m][n] = sum over k of A[m][k] B[n][k], float32 sums, with an epilogue of the
+// Tiled products on the matrix cores: C[m][n] = sum over k of A[m][k] B[n][k], float32 sums, with an epilogue of the
 // caller's on the tile in registers.
 //
 // Either operand lies in memory with k along its rows (kRows) or across them (kColumns: k is the row, m or n the column).
@@ -9,6 +9,9 @@
 // kPlanes 2: a value is a pair of 16-bit parts, multiplied as three products (second by first, first by second, first by first).
 // A row holds 32 values' first parts, then their second parts, and so on, so a tile of 32 k has the bytes, lines and LDS places of
 // one of 64 single values. (In planes of their own, multiplied pair after pair, the parts were read three times for two.)
+//
+// P float: values as they are, 32 k to a tile, only along the rows, on the float32 matrix instructions: a sixteenth of the 16-bit
+// ones' rate, for products that wait for their operands.
 //
 // Measured, plain products of random bfloat16 values, 8192 x 8192: 1040 TFLOP/s over 1536 k and 1070 to 1230 over 8192 (256 x 256
 // tiles), 1020 and 1120 (128 x 128, two workgroups to a CU); a library product reaches 1148. The matrix cores are busy 60% of
@@ -26,7 +29,7 @@
 namespace dllm_hip {
 
 // Bytes; base and strides are multiples of 16. kRows: m or n rows of k values. kColumns: k rows of m or n values, each readable up to
-// the next multiple of 8 values. `count`: how many m or n there are; indexes past it repeat others, what they yield is not
+// the next whole chunk. `count`: how many m or n there are; indexes past it repeat others, what they yield is not
 // stored.
 struct Operand {
     const char* base;
@@ -36,10 +39,10 @@ struct Operand {
 
 static __device__ const uint4 kZeroChunk = {0, 0, 0, 0};
 
-// Where value c of a row begins, in bytes; a pair's second part is kSecond bytes further.
-template <int kPlanes>
+// Where value c of a row begins, in bytes; a pair's second part is kSecond bytes further. kBytes: of a part.
+template <int kPlanes, int kBytes = 2>
 __host__ __device__ __forceinline__ int64_t value_at(int64_t c) {
-    return kPlanes == 1 ? c * 2 : (c >> 5) * 128 + (c & 31) * 2;
+    return kPlanes == 1 ? c * kBytes : (c >> 5) * 128 + (c & 31) * 2;
 }
 constexpr int kSecond = 64;
 // Values of a row that are there: whole chunks, or whole groups of pairs.
@@ -72,15 +75,15 @@ __device__ __forceinline__ int tile_swizzle(int row) {
 }
 
 // One operand's tile of kSize m or n: its copy to LDS.
-template <int kSize, int kPlanes, int kThreads, bool kColumns>
+template <int kSize, int kPlanes, int kPartBytes, int kThreads, bool kColumns>
 struct OperandTile {
-    static constexpr int kTileK = 64 / kPlanes;
+    static constexpr int kTileK = 128 / (kPlanes * kPartBytes);
     static constexpr int kChunks = kColumns ? kSize * kPlanes / 8 : 8;  // of an LDS row
     static constexpr int kRows = kColumns ? kTileK : kSize;
     static constexpr int kBytes = kRows * kChunks * 16;
     static constexpr int kTurns = kRows * kChunks / kThreads;
     static constexpr int kTurnRows = kThreads / kChunks;
-    static_assert(kRows * kChunks % kThreads == 0 && kThreads % kChunks == 0);
+    static_assert(kRows * kChunks % kThreads == 0 && kThreads % kChunks == 0 && (kPartBytes == 2 || !kColumns));
 
     const char* base;  // of the tile's first m or n
     int64_t stride;
@@ -91,7 +94,7 @@ struct OperandTile {
         return (static_cast<int>(threadIdx.x) % kChunks) ^ tile_swizzle<kChunks>(lds_row(turn));
     }
     // the first value of a chunk
-    __device__ __forceinline__ static int value_of(int c) { return kPlanes == 1 ? c * 8 : c / 8 * 32 + (c & 3) * 8; }
+    __device__ __forceinline__ static int value_of(int c) { return kPlanes == 1 ? c * (16 / kPartBytes) : c / 8 * 32 + (c & 3) * 8; }
 
     __device__ __forceinline__ void init(const Operand& op, int64_t first, int64_t count, int64_t batch) {
         stride = op.stride;
@@ -113,7 +116,7 @@ struct OperandTile {
     // The tile from k0 on to LDS; k at and past `k` are zero.
     __device__ __forceinline__ void copy(int64_t k0, int64_t k, LdsByte* lds) const {
         const char* to = (const char*)lds + (static_cast<int>(threadIdx.x) >> 6) * 1024;
-        const char* from = base + (kColumns ? k0 * stride : value_at<kPlanes>(k0));
+        const char* from = base + (kColumns ? k0 * stride : value_at<kPlanes, kPartBytes>(k0));
         if (k0 + kTileK <= k) {
 #pragma unroll
             for (int t = 0; t < kTurns; ++t) copy16_to_lds_s(from, offset[t], to + t * (kThreads * 16));
@@ -128,7 +131,7 @@ struct OperandTile {
     }
 };
 
-// A lane's reads of blocks of 32 m or n by 16 k from a tile.
+// A lane's reads of blocks of 32 m or n by 16 k (8 of float32) from a tile.
 template <int kSize, int kPlanes, bool kColumns>
 struct OperandView {
     static constexpr int kChunks = kColumns ? kSize * kPlanes / 8 : 8;
@@ -179,6 +182,19 @@ __device__ __forceinline__ void stage_barrier() {
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(kCount) : "memory");
 }
 
+// acc += x y: 16 k of a 16-bit type, 8 of float32, of which each instruction takes one of either half's chunk.
+template <typename P>
+__device__ __forceinline__ void multiply_chunks(const Chunk16& x, const Chunk16& y, Acc& acc) {
+    if constexpr (sizeof(P) == 4) {
+        using Four = float __attribute__((ext_vector_type(4)));
+        const Four a = __builtin_bit_cast(Four, x), b = __builtin_bit_cast(Four, y);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], acc, 0, 0, 0);
+    } else {
+        multiply<P>(x, y, acc);
+    }
+}
+
 // A tile of kM x kN by kWavesM x kWavesN waves, with kStages buffers.
 template <typename P, int kPlanesOf, int kM_, int kN_, int kWavesM_, int kWavesN_, bool kAColumns, bool kBColumns, int kStages = 2>
 struct TileProduct {
@@ -186,10 +202,11 @@ struct TileProduct {
     static constexpr int kThreads = kWavesM * kWavesN * kWave;
     static constexpr int kWaveM = kM / kWavesM, kWaveN = kN / kWavesN;
     static constexpr int kBlocksM = kWaveM / 32, kBlocksN = kWaveN / 32;
-    static constexpr int kTileK = 64 / kPlanesOf;
-    static_assert(kPlanesOf == 1 || kPlanesOf == 2);
-    using ATile = OperandTile<kM, kPlanesOf, kThreads, kAColumns>;
-    using BTile = OperandTile<kN, kPlanesOf, kThreads, kBColumns>;
+    static constexpr int kTileK = 128 / (kPlanesOf * static_cast<int>(sizeof(P)));
+    static_assert(kPlanesOf == 1 || (kPlanesOf == 2 && sizeof(P) == 2));
+    using Part = P;
+    using ATile = OperandTile<kM, kPlanesOf, sizeof(P), kThreads, kAColumns>;
+    using BTile = OperandTile<kN, kPlanesOf, sizeof(P), kThreads, kBColumns>;
     static constexpr int kStage = ATile::kBytes + BTile::kBytes;
     static constexpr int kLds = kStages * kStage;
     static constexpr int kCopies = ATile::kTurns + BTile::kTurns;  // of a thread, for one stage
@@ -255,7 +272,7 @@ struct TileProduct {
             const LdsByte* const stage = lds + from * kStage;
             from = from + 1 == kStages ? 0 : from + 1;
 #pragma unroll
-            for (int step = 0; step < kTileK / 16; ++step) {
+            for (int step = 0; step < 4 / kPlanesOf; ++step) {
                 Chunk16 x[kPlanesOf][kBlocksM], y[kPlanesOf][kBlocksN];
 #pragma unroll
                 for (int p = 0; p < kPlanesOf; ++p) {
@@ -269,7 +286,7 @@ struct TileProduct {
 #pragma unroll
                     for (int m = 0; m < kBlocksM; ++m)
 #pragma unroll
-                        for (int n = 0; n < kBlocksN; ++n) multiply<P>(x[product == 0][m], y[product == 1][n], acc[m][n]);
+                        for (int n = 0; n < kBlocksN; ++n) multiply_chunks<P>(x[product == 0][m], y[product == 1][n], acc[m][n]);
             }
         }
         if constexpr (kSegments) {

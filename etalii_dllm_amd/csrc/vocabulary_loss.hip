@@ -12,8 +12,8 @@
 // gradients of 1020 rows, 49152 x 576, 1.6 ms.)
 //
 // Forward: tiles of logits on the matrix cores, vocabulary by rows, so that a lane owns a row of the batch; a tile leaves each
-// row's largest logit and sum of exponentials of 128 of the vocabulary, which a second launch joins in a fixed order, and
-// the target's logit.
+// row's largest logit and sum of exponentials of 128 of the vocabulary, which a last launch joins in a fixed order. The target's
+// logit is formed where the rows are gathered, and goes into the sum as it is.
 //
 // Backward, a piece of the vocabulary at a time: the logits again, whose epilogue stores the softmax's part of g in the product's
 // type; then its products with the weights and with the hidden states. dh is added up in float32 over units of the vocabulary that
@@ -38,6 +38,7 @@ namespace {
 
 constexpr int64_t kPackPiece = 16384;  // of the vocabulary: weights packed at once, where they are
 constexpr int kStatRows = 128;        // of the vocabulary: one maximum and sum
+constexpr int64_t kFewRows = 256;
 constexpr size_t kPieceBytes = size_t{1} << 28;
 constexpr int64_t kStrideSlack = 64;  // elements between the softmax's rows: their stride is no power of two, which would meet on few channels
 constexpr int kHalfShift = 14;  // float16 holds the softmax's part of g times 2^14, relative to the row's weight
@@ -66,6 +67,12 @@ constexpr bool kScaled = sizeof(T) == 4;
 template <typename T>
 constexpr int64_t row_bytes(int64_t n) {
     return static_cast<int64_t>(round_up(n, kRowMultiple<kLossPlanes<T>>)) * 2 * kLossPlanes<T>;
+}
+
+// Float32 values as they are, 8 from column c on; a row takes as many bytes as one of pairs.
+__device__ __forceinline__ void store_as_they_are(char* row, int64_t c, const float (&v)[8]) {
+    float4* const to = reinterpret_cast<float4*>(row + c * 4);
+    to[0] = {v[0], v[1], v[2], v[3]}, to[1] = {v[4], v[5], v[6], v[7]};
 }
 
 // 8 values of a row from column c on
@@ -171,9 +178,9 @@ __device__ __forceinline__ void load_eight(const T* row, int64_t d, int64_t dim,
     }
 }
 
-// What scales a row by a power of two: nothing, the size of its unit (weights), or its part in dW (hidden states): factor's exponent
-// and the row's from the largest, zero for none.
-enum PackScale { kNoScale, kUnitScale, kWeightScale };
+// What scales a row by a power of two: nothing (kAsTheyAre: and float32 stays that), the size of its unit (weights), or its part in dW
+// (hidden states): factor's exponent and the row's from the largest, zero for none.
+enum PackScale { kNoScale, kAsTheyAre, kUnitScale, kWeightScale };
 constexpr int kNoWeight = -1000;      // the exponent of a factor of zero
 constexpr int kExponentBase = 1000;  // the largest exponent is held with this added, -1 before any
 
@@ -191,6 +198,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, ch
     if (j >= (a.count ? static_cast<int64_t>(*a.count) : a.n)) return;
     float v[8];
     load_eight<T, kWhole>(src + (a.list ? static_cast<int64_t>(a.list[j]) : j) * a.stride, c * 8, a.dim, v);
+    if constexpr (kScale == kAsTheyAre) return store_as_they_are(dst + j * a.row, c * 8, v);
     if constexpr (kScale != kNoScale) {
         int by;
         if constexpr (kScale == kUnitScale) {
@@ -249,9 +257,11 @@ struct RowsArgs {
     LossShape s;
     uint32_t *list, *count;  // kFind: written here
     char* packed;
-    int32_t* row_exponent;
-    // kFind
+    int32_t* row_exponent;  // float32: NULL: the values as they are
+    // the forward's
     const int64_t* targets;
+    float* at_target;  // by the place in the list
+    // kFind
     float *loss_out, *lse_out;
     int32_t* sizes;  // set to -1
     int64_t units;
@@ -276,8 +286,8 @@ template <RowsOf kOf>
 constexpr int kRowsThreads = kOf == kFind ? 1024 : 256;
 constexpr int64_t kFindRows = 16384;  // the most that every workgroup counts through for itself
 
-// A wave to a listed row: its hidden state in parts, and of the backward, its target's element (the product in float32) and what the
-// softmax's epilogue reads. kFind: the workgroup lists its 16 rows itself, by counting the rows before them.
+// A wave to a listed row: its hidden state in parts, and its target's logit, from a product in float32 added up by 64 lanes; of the
+// backward, the target's element and what the softmax's epilogue reads. kFind: the workgroup lists its 16 rows itself, by counting the rows before them.
 template <typename T, bool kWhole, bool kCapped, RowsOf kOf>
 __global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __restrict__ hidden, const T* __restrict__ weight, RowsArgs a) {
     constexpr int kThreads = kRowsThreads<kOf>, kWaves = kThreads / kWave;
@@ -311,10 +321,11 @@ __global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __rest
         row = a.list[j];
     }
     const T* const h = hidden + row * a.s.hidden_stride;
-    const T* w = nullptr;
-    if constexpr (kOf == kBackward) w = weight + static_cast<int64_t>(a.order.token[j]) * a.s.dim;
+    const int64_t target = kOf == kBackward ? static_cast<int64_t>(a.order.token[j]) : a.targets[row];
+    const T* const w = weight + target * a.s.dim;
     int exponent = 0;
-    if constexpr (kScaled<T>) {
+    const bool scaled = kScaled<T> && a.row_exponent;
+    if (scaled) {
         uint32_t top = 0;
         for (int64_t d = lane; d < a.s.dim; d += kWave) top = max(top, size_bits(h[d]));
         exponent = exponent_of(static_cast<int32_t>(wave_max(top)));
@@ -322,29 +333,33 @@ __global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __rest
     }
     float x = 0.0f;
     for (int64_t d = lane * 8; d < a.s.padded; d += kWave * 8) {
-        float v[8];
+        float v[8], u[8];
         load_eight<T, kWhole>(h, d, a.s.dim, v);
-        if constexpr (kOf == kBackward) {
-            float u[8];
-            load_eight<T, kWhole>(w, d, a.s.dim, u);
+        load_eight<T, kWhole>(w, d, a.s.dim, u);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x = fmaf(v[e], u[e], x);
-        }
+        for (int e = 0; e < 8; ++e) x = fmaf(v[e], u[e], x);
         if constexpr (kScaled<T>) {
+            if (!scaled) {
+                store_as_they_are(a.packed + j * a.s.row, d, v);
+                continue;
+            }
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], kTop - exponent);
         }
         store_parts<T>(a.packed + j * a.s.row, d, v);
     }
-    if constexpr (kOf == kBackward) {
 #pragma unroll
-        for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
-        if (lane != 0) return;
-        float derivative;
-        const float z = Cap(a.s).logit<kCapped>(x, derivative), lse = a.lse[row], factor = a.dloss[row] * a.s.scale;
+    for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
+    if (lane != 0) return;
+    float derivative;
+    const float z = Cap(a.s).logit<kCapped>(x, derivative);
+    if constexpr (kOf != kBackward) {
+        a.at_target[j] = z;
+    } else {
+        const float lse = a.lse[row], factor = a.dloss[row] * a.s.scale;
         a.coefficient[row] = expm1f(z - lse) * derivative * factor;
         a.terms.lse[j] = lse;
-        a.terms.target[j] = static_cast<int32_t>(a.order.token[j]);
+        a.terms.target[j] = static_cast<int32_t>(target);
         if constexpr (kHalfParts<T>) {
             float mantissa;
             int e;
@@ -362,14 +377,14 @@ template <typename T, RowsOf kOf>
 int launch_rows(const T* hidden, const T* weight, const RowsArgs& a, hipStream_t stream) {
     constexpr int kThreads = kRowsThreads<kOf>;
     const dim3 grid = grid_of(ceil_div(a.s.rows, kThreads / kWave));
-    const bool whole = a.s.dim % 8 == 0 && a.s.hidden_stride % kChunk<T> == 0 && aligned_to(hidden, 16) && (kOf != kBackward || aligned_to(weight, 16));
-    const bool capped = kOf == kBackward && a.s.softcap != 0.0f;
+    const bool whole = a.s.dim % 8 == 0 && a.s.hidden_stride % kChunk<T> == 0 && aligned_to(hidden, 16) && aligned_to(weight, 16);
+    const bool capped = a.s.softcap != 0.0f;
     if (whole && capped)
-        rows_kernel<T, true, kOf == kBackward, kOf><<<grid, kThreads, 0, stream>>>(hidden, weight, a);
+        rows_kernel<T, true, true, kOf><<<grid, kThreads, 0, stream>>>(hidden, weight, a);
     else if (whole)
         rows_kernel<T, true, false, kOf><<<grid, kThreads, 0, stream>>>(hidden, weight, a);
     else if (capped)
-        rows_kernel<T, false, kOf == kBackward, kOf><<<grid, kThreads, 0, stream>>>(hidden, weight, a);
+        rows_kernel<T, false, true, kOf><<<grid, kThreads, 0, stream>>>(hidden, weight, a);
     else
         rows_kernel<T, false, false, kOf><<<grid, kThreads, 0, stream>>>(hidden, weight, a);
     return check_launch("vocabulary_loss rows");
@@ -380,6 +395,9 @@ int launch_rows(const T* hidden, const T* weight, const RowsArgs& a, hipStream_t
 // The products' tiles by the number of rows. 256 x 256 by eight waves, one workgroup to a CU; 128 x 128 by four, two to a CU, where
 // the large ones would leave CUs without work or pad much; and for up to 64 rows, whose products wait for the weights'
 // bytes, tiles of 64 rows. The forward's waves hold kStatRows of the vocabulary in all of them.
+//
+// Float32's forward of up to kFewRows rows multiplies the values as they are (DirectTiles): packing the weights reads them
+// twice and stores them, which takes as long as the float32 products of some 250 rows.
 template <typename T, bool kAColumns, bool kBColumns, int kM, int kN, int kWavesM, int kWavesN, int kStages = 2>
 using Product64 = TileProduct<LossPart<T>, kLossPlanes<T>, kM, kN, kWavesM, kWavesN, kAColumns, kBColumns, kStages>;
 
@@ -405,6 +423,9 @@ struct SmallTiles {
     using Weight = Product64<T, true, true, 128, 128, 2, 2>;
 };
 
+template <int kN, int kWavesM, int kWavesN>
+using DirectTile = TileProduct<float, 1, kStatRows * kWavesM, kN, kWavesM, kWavesN, false, false>;
+
 // ---- forward ----
 
 struct Stat {
@@ -419,11 +440,12 @@ __device__ __forceinline__ Stat join(const Stat& a, const Stat& b) {
 struct ForwardArgs {
     LossShape s;
     Operand weight, hidden;
+    int64_t k;      // values of a row that are read
     int64_t first;  // of the piece, in the vocabulary; weight.count: of the piece
     const uint32_t *list, *count;
     const int64_t* targets;
     Stat* stats;  // [unit of kStatRows][rows]
-    float* at_target;  // [rows]
+    const float* at_target;  // by the place in the list
     const int32_t* exponent;  // float32: by the place in the list
     const int32_t* sizes;     // float32: of the piece, by kScaleRows
 };
@@ -431,6 +453,7 @@ struct ForwardArgs {
 template <typename T, bool kCapped, typename Tile>
 __global__ __launch_bounds__(Tile::kThreads) void forward_kernel(ForwardArgs a, int64_t m_tiles, int64_t n_tiles) {
     static_assert(Tile::kWaveM == kStatRows);
+    constexpr bool kScales = sizeof(T) != sizeof(typename Tile::Part);
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int64_t count = *a.count;
     int64_t m, n;
@@ -438,18 +461,18 @@ __global__ __launch_bounds__(Tile::kThreads) void forward_kernel(ForwardArgs a, 
     tile_of(block_id(), m_tiles, n_tiles, m, n);
     if (n * Tile::kN >= count) return;
     typename Tile::Sums acc;
-    Tile::run(a.weight, a.hidden, m * Tile::kM, n * Tile::kN, a.weight.count, count, a.s.padded, 0, 0, (LdsByte*)lds, acc);
+    Tile::run(a.weight, a.hidden, m * Tile::kM, n * Tile::kN, a.weight.count, count, a.k, 0, 0, (LdsByte*)lds, acc);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
     if (m0 >= a.weight.count) return;
     const int64_t unit = (a.first + m0) / kStatRows;
     const int valid = static_cast<int>(min(a.weight.count - m0, static_cast<int64_t>(kStatRows)));
     const Cap cap(a.s);
     static_assert(kScaleRows % Tile::kM == 0);
-    const int weight_exponent = kScaled<T> ? exponent_of(a.sizes[m * Tile::kM / kScaleRows]) - 2 * kTop : 0;
+    const int weight_exponent = kScales ? exponent_of(a.sizes[m * Tile::kM / kScaleRows]) - 2 * kTop : 0;
 #pragma unroll
     for (int j = 0; j < Tile::kBlocksN; ++j) {
         const int64_t row = n0 + 32 * j + lane_column();
-        const int by = kScaled<T> ? weight_exponent + a.exponent[min(row, count - 1)] : 0;
+        const int by = kScales ? weight_exponent + a.exponent[min(row, count - 1)] : 0;
         const int target = row < count ? static_cast<int>(a.targets[a.list[row]] - a.first - m0) : -1;
         const bool any = __ballot(target >= 0 && target < kStatRows) != 0;
         float top = -INFINITY;
@@ -458,7 +481,7 @@ __global__ __launch_bounds__(Tile::kThreads) void forward_kernel(ForwardArgs a, 
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
                 float unused, x = acc[i][j][r];
-                if constexpr (kScaled<T>) x = ldexpf(x, by);
+                if constexpr (kScales) x = ldexpf(x, by);
                 acc[i][j][r] = cap.logit<kCapped>(x, unused);
             }
             __builtin_amdgcn_sched_barrier(0);  // one block's values at a time: all of them do not fit the registers
@@ -470,12 +493,12 @@ __global__ __launch_bounds__(Tile::kThreads) void forward_kernel(ForwardArgs a, 
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 32 * i + block_row(r) < valid ? acc[i][j][r] : -INFINITY;
         }
         if (any) {
-            float wanted = 0.0f;
+            // the sum has the target's logit as the loss subtracts it: what is left where the model is sure is then not their rounding
+            const float known = a.at_target[min(row, count - 1)];
 #pragma unroll
             for (int i = 0; i < Tile::kBlocksM; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) wanted = 32 * i + block_row(r) == target ? acc[i][j][r] : wanted;
-            if (target >= 0 && target < kStatRows && lane_half() == (target >> 2 & 1)) a.at_target[row] = wanted;
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 32 * i + block_row(r) == target ? known : acc[i][j][r];
         }
 #pragma unroll
         for (int i = 0; i < Tile::kBlocksM; ++i)
@@ -519,9 +542,9 @@ __global__ __launch_bounds__(256) void join_stats_kernel(const Stat* __restrict_
         if (part < step) of[part][which] = s = join(s, of[part + step][which]);
     }
     if (part == 0 && first + which < n) {
-        const float l = s.top + kLn2 * __builtin_amdgcn_logf(s.sum);
-        if (lse) lse[list[row]] = l;
-        if (loss) loss[list[row]] = l - at_target[row];
+        const float rest = kLn2 * __builtin_amdgcn_logf(s.sum);
+        if (lse) lse[list[row]] = s.top + rest;
+        if (loss) loss[list[row]] = s.top - at_target[row] + rest;  // the large numbers' difference first, which is exact where they are near
     }
 }
 
@@ -902,19 +925,21 @@ struct Buffers {
     }
 };
 
+// Whether the weights are read where they are. as_they_are: values, not pairs.
 template <typename T>
-bool weights_direct(const LossShape& s, const T* weight) {
-    return sizeof(T) == 2 && s.dim % 8 == 0 && aligned_to(weight, 16);
+bool weights_direct(const LossShape& s, const T* weight, bool as_they_are) {
+    return as_they_are && s.dim % kChunk<T> == 0 && aligned_to(weight, 16);
 }
 
 // The weights of a piece as an operand: where they are, or packed. sizes: of the piece.
 template <typename T>
-int weight_operand(const LossShape& s, const T* weight, char* packed, int32_t* sizes, int64_t first, int64_t n, Operand& op,
+int weight_operand(const LossShape& s, const T* weight, bool as_they_are, char* packed, int32_t* sizes, int64_t first, int64_t n, Operand& op,
                    hipStream_t stream) {
     op.count = n;
     op.batch = 0;
     op.stride = s.row;
-    if (weights_direct(s, weight)) {
+    if (weights_direct(s, weight, as_they_are)) {
+        op.stride = s.dim * static_cast<int64_t>(sizeof(T));
         op.base = reinterpret_cast<const char*>(weight + first * s.dim);
         return kOk;
     }
@@ -922,6 +947,7 @@ int weight_operand(const LossShape& s, const T* weight, char* packed, int32_t* s
     PackArgs p{};
     p.n = n, p.dim = s.dim, p.stride = s.dim, p.sizes = sizes;
     if constexpr (kScaled<T>) {
+        if (as_they_are) return launch_pack<T, kAsTheyAre>(weight + first * s.dim, packed, p, stream);
         const float* const from = weight + first * s.dim;
         if (s.dim % 4 == 0 && aligned_to(from, 16))
             unit_sizes_kernel<4><<<grid_of(ceil_div(n, kSizeRows)), 256, 0, stream>>>(from, n, s.dim, sizes);
@@ -956,29 +982,43 @@ int run_forward(const LossShape& s, int64_t dtype, const T* hidden, const T* wei
                 void* workspace, size_t bytes, hipStream_t stream) {
     const LossLayout layout(s, dtype, false);
     const Buffers<T> b(layout, s, false, workspace, bytes);
+    const bool few = kScaled<T> && s.rows <= kFewRows, direct = weights_direct(s, weight, !kScaled<T> || few);
     RowsArgs r = rows_args<T>(s, b);
-    r.list = b.list, r.count = b.count;
+    r.list = b.list, r.count = b.count, r.targets = targets, r.at_target = b.at_target;
+    if (few) r.row_exponent = nullptr;
     if (s.rows <= kFindRows) {
-        r.targets = targets, r.loss_out = loss, r.lse_out = lse, r.sizes = b.sizes, r.units = layout.sizes;
+        r.loss_out = loss, r.lse_out = lse, r.sizes = b.sizes, r.units = layout.sizes;
         DLLM_TRY((launch_rows<T, kFind>(hidden, weight, r, stream)));
     } else {
         keep_rows_kernel<<<1, 1024, 0, stream>>>(targets, s.rows, s.vocabulary, b.list, b.count, loss, lse);
         if (kScaled<T>) DLLM_TRY(fill_words(b.sizes, layout.sizes * 4, ~uint32_t{0}, stream));
         DLLM_TRY((launch_rows<T, kListed>(hidden, weight, r, stream)));
     }
-    const int64_t piece = weights_direct(s, weight) ? s.vocabulary : kPackPiece;
+    const int64_t piece = direct ? s.vocabulary : kPackPiece;
     for (int64_t first = 0; first < s.vocabulary; first += piece) {
         ForwardArgs a{};
-        a.s = s, a.hidden = hidden_operand(s, b.hidden);
+        a.s = s, a.hidden = hidden_operand(s, b.hidden), a.k = direct ? s.dim : s.padded;
         a.sizes = b.sizes + first / kScaleRows, a.exponent = b.row_exponent;
-        DLLM_TRY(weight_operand<T>(s, weight, b.weight, b.sizes + first / kScaleRows, first, std::min(piece, s.vocabulary - first), a.weight, stream));
+        DLLM_TRY(weight_operand<T>(s, weight, !kScaled<T> || few, b.weight, b.sizes + first / kScaleRows, first,
+                                   std::min(piece, s.vocabulary - first), a.weight, stream));
         a.first = first, a.list = b.list, a.count = b.count, a.targets = targets, a.stats = b.stats, a.at_target = b.at_target;
-        if (s.rows <= 64)
-            launch_forward<T, typename SmallTiles<T>::Forward>(a, stream);
-        else if (s.rows <= 128)
-            launch_forward<T, typename MiddleTiles<T>::Forward>(a, stream);
-        else
-            launch_forward<T, typename LargeTiles<T>::Forward>(a, stream);
+        if constexpr (kScaled<T>) {
+            if (s.rows <= 32)
+                launch_forward<T, DirectTile<32, 1, 1>>(a, stream);
+            else if (s.rows <= 64)
+                launch_forward<T, DirectTile<64, 1, 2>>(a, stream);
+            else if (s.rows <= kFewRows)
+                launch_forward<T, DirectTile<128, 2, 4>>(a, stream);
+            else
+                launch_forward<T, typename LargeTiles<T>::Forward>(a, stream);
+        } else {
+            if (s.rows <= 64)
+                launch_forward<T, typename SmallTiles<T>::Forward>(a, stream);
+            else if (s.rows <= 128)
+                launch_forward<T, typename MiddleTiles<T>::Forward>(a, stream);
+            else
+                launch_forward<T, typename LargeTiles<T>::Forward>(a, stream);
+        }
     }
     join_stats_kernel<<<grid_of(ceil_div(s.rows, 4)), 256, 0, stream>>>(
         b.stats, b.at_target, static_cast<int64_t>(ceil_div(s.vocabulary, kStatRows)), s.rows, b.list, b.count, loss, lse);
@@ -1010,7 +1050,7 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
         SoftmaxArgs a{};
         a.s = s, a.hidden = hidden_operand(s, b.hidden);
         a.sizes = b.sizes + first / kScaleRows;
-        DLLM_TRY(weight_operand<T>(s, weight, b.weight, b.sizes + first / kScaleRows, first, std::min(piece, s.vocabulary - first), a.weight, stream));
+        DLLM_TRY(weight_operand<T>(s, weight, !kScaled<T>, b.weight, b.sizes + first / kScaleRows, first, std::min(piece, s.vocabulary - first), a.weight, stream));
         a.first = first, a.count = b.order.kept, a.terms = b.terms, a.out = b.softmax;
         a.out_stride = row_bytes<T>(piece + kStrideSlack);
         const int64_t width = a.weight.count, m = ceil_div(s.rows, Logits::kM), n = ceil_div(width, Logits::kN);

@@ -396,7 +396,8 @@ int dllm_hip_token_embedding_backward(const dllm_hip_token_embedding_shape* shap
  * of the largest one's lose some of their softmax's part. float32 has pairs of float16 as operands, 22 bits and more of each
  * value: hidden states off by at most 2^-39 of their row's largest value (in dweight, of the largest one times its dloss), weights
  * of 2048 rows' largest, so values far below those lose bits.
- * A row's loss, lse and dhidden are the same bits alone and in any batch. hidden_stride and dhidden_stride: elements between rows (0: dim).
+ * A row's loss, lse and dhidden are the same bits alone and in any batch (dhidden: from the same lse); float32's loss and lse are where
+ * the batches have at most 256 rows, and where they have more: few rows are multiplied by the weights as they are. hidden_stride and dhidden_stride: elements between rows (0: dim).
  * Outputs do not overlap inputs. Limits: rows below 2^27, vocabulary below 2^31, their product below 2^48, dim at most 2^16, strides
  * below 2^32, scale in [2^-60, 2^60], softcap 0 or in [2^-64, 2^64]. */
 typedef struct {

@@ -296,20 +296,38 @@ def test_loss_results_alone(K):
         assert torch.equal(getattr(q, keep), loss if keep == "loss" else lse)
 
 
+# odd and short rows, whose weights are packed also where rows are few
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize(("rows", "vocabulary", "dim"), [(1, 3, 2), (5, 700, 33), (40, 2100, 33), (100, 700, 67), (256, 5000, 7)])
+def test_loss_of_few_rows_packed(K, dtype, rows, vocabulary, dim):
+    p, dloss = loss_problem(K, 28, R.DTYPES[dtype], rows, vocabulary, dim)
+    p.check(dloss)
+
+
+def in_few_rows(K, p):
+    """The results of a batch's rows, 256 at once."""
+    few = [Loss(K, p.hidden[i:i + 256].clone(), p.weight, p.targets[i:i + 256].clone()).forward() for i in range(0, p.rows, 256)]
+    return torch.cat([f[0] for f in few]), torch.cat([f[1] for f in few])
+
+
 @pytest.mark.parametrize("dtype", R.DTYPES)
 @pytest.mark.parametrize(("vocabulary", "dim"), [(20000, 96), (9000, 130)])
 def test_a_row_alone_and_in_a_batch(K, dtype, vocabulary, dim):
-    """A row's loss, lse and dhidden are the same bits in batches of any size, and every call gives the same bits."""
+    """A row's loss, lse and dhidden are the same bits in batches of any size, and every call gives the same bits. (float32's loss
+    and lse: in all of at most 256 rows, and in all of more.)"""
     p, dloss = loss_problem(K, 21, R.DTYPES[dtype], 700, vocabulary, dim, masked=0.1)
     loss, lse = (t.clone() for t in p.forward())
     dhidden, dweight = p.backward(dloss)
     again = p.backward(dloss)
     assert torch.equal(again[0], dhidden) and torch.equal(again[1], dweight)
+    few = in_few_rows(K, p)
+    assert dtype == "float32" or (torch.equal(few[0], loss) and torch.equal(few[1], lse))
     for first, n in [(0, 1), (5, 30), (64, 64), (100, 65), (300, 129), (13, 257), (1, 600)]:
         rows = slice(first, first + n)
         q = Loss(K, p.hidden[rows].clone(), p.weight, p.targets[rows].clone())
-        got = q.forward()
-        assert torch.equal(got[0], loss[rows]) and torch.equal(got[1], lse[rows]), n
+        got, want = q.forward(), few if n <= 256 else (loss, lse)
+        assert torch.equal(got[0], want[0][rows]) and torch.equal(got[1], want[1][rows]), n
+        q.lse.copy_(lse[rows])
         assert torch.equal(q.backward(dloss[rows].clone())[0], dhidden[rows]), n
 
 
@@ -319,11 +337,13 @@ def test_a_row_alone_and_in_a_batch_of_pieces(K, dtype):
     p, dloss = loss_problem(K, 25, R.DTYPES[dtype], 20000, 20000, 24)
     loss, lse = (t.clone() for t in p.forward())
     dhidden, _ = p.backward(dloss)
+    few = in_few_rows(K, p)
     for first, n in [(0, 3), (7000, 90), (19700, 300)]:
         rows = slice(first, first + n)
         q = Loss(K, p.hidden[rows].clone(), p.weight, p.targets[rows].clone())
-        got = q.forward()
-        assert torch.equal(got[0], loss[rows]) and torch.equal(got[1], lse[rows]), n
+        got, want = q.forward(), few if n <= 256 else (loss, lse)
+        assert torch.equal(got[0], want[0][rows]) and torch.equal(got[1], want[1][rows]), n
+        q.lse.copy_(lse[rows])
         assert torch.equal(q.backward(dloss[rows].clone())[0], dhidden[rows]), n
     assert bool(torch.isfinite(dhidden).all())
 
