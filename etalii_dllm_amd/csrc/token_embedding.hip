@@ -3,7 +3,9 @@
 //   out[t] = scale * table[token t]          dtable[v] = (dtable[v] +) scale * sum over t with token v of dout[t]
 //
 // Bound: HBM. The lookup reads and writes each element once, a thread 16 bytes. The gradient writes the whole table, or with
-// accumulate reads and writes the rows of tokens that occur; its sums are token_rows.hip's.
+// accumulate reads and writes the rows of tokens that occur; its sums are token_rows.hip's. Measured: 16384 tokens of 2304 in
+// bfloat16 27 us, 5.5 TB/s (tokens that come again are read from the caches); the gradient of 8192 tokens onto 151936 x 1536
+// 108 us, 78 of them the table's zeroes at 6.0 TB/s with the sort beside them. One token is a launch, 6.7 us.
 #include "common.h"
 #include "dllm_hip.h"
 #include "element.h"

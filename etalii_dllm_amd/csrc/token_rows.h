@@ -48,7 +48,7 @@ inline TokenOrder take_token_order(Carve& c, int64_t n) {
 // Writes `word`, whose halves are alike, to every word of `bytes` bytes (an even number) at `at`, aligned to 2.
 int fill_words(void* at, size_t bytes, uint32_t word, hipStream_t stream);
 
-// Sorts n >= 1 tokens and fills fill_bytes bytes at fill_at as fill_words, in the same launch where one workgroup sorts.
+// Sorts n >= 1 tokens and fills fill_bytes bytes at fill_at as fill_words, in the sort's launch where that is one.
 int sort_tokens(const int64_t* tokens, int64_t n, int64_t vocabulary, const TokenOrder& order, void* fill_at, size_t fill_bytes,
                 uint32_t fill, hipStream_t stream);
 
@@ -63,7 +63,7 @@ struct TokenSums {
     // either the table's rows, of the rows' type, ...
     void* table;
     bool accumulate;
-    // ... or float32 rows by the sorted index of a token's first position, and that index by token
+    // ... or float32 rows by the index in the order of a token's first position, and that index by token
     float* sums;
     int32_t* first;
 };

@@ -8,7 +8,8 @@
 //
 // Sums: a wave takes 8 sorted positions and 16 bytes of columns to a lane, reads all 8 rows at once and adds them in order.
 // A token whose positions lie within the 8 is done; the sums of others are float32 parts, added in their order by a second
-// launch. Nothing depends on when a wave runs.
+// launch. Nothing depends on when a wave runs. 16381 rows of 576 in float32 onto a table that is added to: sort 22 us, sums 14
+// (2.7 TB/s of rows read), parts 9, a chain of additions as long as the most frequent token's; 16 positions to a wave were no faster.
 #include "token_rows.h"
 
 #include <algorithm>
