@@ -223,6 +223,16 @@ def test_loss_bends(K, dtype, options):
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize("counted", [1, 255, 257, 700, 2099])
+@pytest.mark.parametrize(("vocabulary", "dim"), [(20000, 96), (3000, 1100)])
+def test_loss_of_a_batch_of_which_few_rows_count(K, dtype, counted, vocabulary, dim):
+    """The tiles are those of the rows that count: at a tile's edge, in few of the launch's, behind many that do not."""
+    p, dloss = loss_problem(K, 29, R.DTYPES[dtype], 2100, vocabulary, dim, masked=0.0)
+    p.targets[:2100 - counted] = -1
+    p.check(dloss, randn(gen(30), vocabulary, dim, dtype=R.DTYPES[dtype], scale=1e-3))
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
 def test_loss_of_rows_that_do_not_count(K, dtype):
     """What they hold reaches nothing, and their rows of the results are zero; none at all, and all but none."""
     dt = R.DTYPES[dtype]
