@@ -624,9 +624,8 @@ struct GradientArgs {
     const uint32_t* count;
     int64_t rows, dim, first, width, unit;  // first and width: of the piece
     // dh
-    int64_t hidden_blocks, m_tiles, n_tiles;
-    bool in_turn;  // a tile adds its units to the total itself, else each unit has a part
-    bool begin;    // the total begins here
+    int64_t m_tiles, n_tiles;  // none without dh
+    bool begin;  // the total begins here
     float *total, *part;
     // dW
     int64_t weight_m_tiles, weight_n_tiles;
@@ -638,18 +637,25 @@ struct GradientArgs {
     bool whole;  // dW's rows are whole 16-byte chunks
 };
 
+// Whether a tile of dh adds the piece's units to the total itself; else each unit has a part. With tiles for most CUs that saves the
+// parts' way through memory; with fewer, the others would wait for them (8192 rows, 151936 x 1536, of which 3277 count: 78
+// tiles; 5.8 ms in turn, 5.0 with parts). The additions and their order are the same.
+constexpr int64_t kTurnTiles = 160;
+__host__ __device__ __forceinline__ bool in_turn(int64_t tiles, int64_t units) { return units == 1 || tiles >= kTurnTiles; }
+
 template <typename T, typename Tile>
-__device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, LdsByte* lds) {
-    const int64_t count = *a.count, units = (a.width + a.unit - 1) / a.unit, m_tiles = tiles_that_count<Tile::kM>(count, a.m_tiles);
-    const int64_t each = m_tiles * a.n_tiles, only = a.in_turn ? 0 : id / each, end = a.in_turn ? units : only + 1;
+__device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, int64_t m_tiles, int64_t units, LdsByte* lds) {
+    const int64_t count = *a.count, each = m_tiles * a.n_tiles;
+    const bool turns = in_turn(each, units);
+    const int64_t only = turns ? 0 : id / each, end = turns ? units : only + 1;
     int64_t m, n;
     tile_of(id - only * each, m_tiles, a.n_tiles, m, n);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
-    float* const out = a.in_turn ? a.total : a.part + only * a.rows * a.dim;
+    float* const out = turns ? a.total : a.part + only * a.rows * a.dim;
     for (int64_t unit = only; unit < end; ++unit) {
         typename Tile::Sums acc;
         Tile::run(a.softmax, a.weight, m * Tile::kM, n * Tile::kN, count, a.dim, min(a.unit, a.width - unit * a.unit), unit, unit, lds, acc);
-        const bool store = !a.in_turn || (a.begin && unit == 0);
+        const bool store = !turns || (a.begin && unit == 0);
         const int by = kScaled<T> ? exponent_of(a.sizes[unit * a.unit / kScaleRows]) - kTop : 0;
         struct Old {
             float4 v[2];
@@ -750,17 +756,20 @@ template <typename T, typename HiddenTile, typename WeightTile>
 __global__ __launch_bounds__(HiddenTile::kThreads) void gradient_kernel(T* __restrict__ dweight, GradientArgs a) {
     static_assert(HiddenTile::kThreads == WeightTile::kThreads);
     __shared__ __attribute__((aligned(1024))) char lds[HiddenTile::kLds > WeightTile::kLds ? HiddenTile::kLds : WeightTile::kLds];
-    const int64_t id = block_id(), hidden_tiles = a.hidden_blocks / max(a.m_tiles, int64_t{1}) * tiles_that_count<HiddenTile::kM>(*a.count, a.m_tiles);
+    const int64_t id = block_id(), m_tiles = tiles_that_count<HiddenTile::kM>(*a.count, a.m_tiles), units = (a.width + a.unit - 1) / a.unit;
+    const int64_t each = m_tiles * a.n_tiles, hidden_tiles = in_turn(each, units) ? each : each * units;
     if (id < hidden_tiles)
-        hidden_tile<T, HiddenTile>(a, id, (LdsByte*)lds);
+        hidden_tile<T, HiddenTile>(a, id, m_tiles, units, (LdsByte*)lds);
     else if (id < hidden_tiles + a.weight_m_tiles * a.weight_n_tiles)
         weight_tile<T, WeightTile>(dweight, a, id - hidden_tiles, (LdsByte*)lds);
 }
 
-// total (+)= the units' parts, in their order
+// total (+)= the units' parts, in their order, where there are parts (kSize: of dh's tiles)
+template <int kSize>
 __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, float* __restrict__ total, const uint32_t* __restrict__ count,
-                                                        int64_t rows, int64_t dim, int units, bool begin) {
+                                                        int64_t rows, int64_t dim, int64_t n_tiles, int units, bool begin) {
     const int64_t n = static_cast<int64_t>(*count) * dim;
+    if (in_turn((static_cast<int64_t>(*count) + kSize - 1) / kSize * n_tiles, units)) return;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
         float v = begin ? part[i] : total[i] + part[i];
         for (int u = 1; u < units; ++u) v += part[u * rows * dim + i];
@@ -1086,12 +1095,15 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
         g.hidden = hidden_operand(s, kHalfParts<T> ? b.scaled : b.hidden);
         g.sizes = a.sizes, g.count = b.order.kept, g.rows = s.rows, g.dim = s.dim, g.first = first, g.width = width, g.unit = layout.unit;
         const int64_t units = ceil_div(width, layout.unit);
+        int64_t hidden_blocks = 0;
+        bool add_parts = false;
         if (dhidden) {
             g.m_tiles = ceil_div(s.rows, Hidden::kM), g.n_tiles = ceil_div(s.dim, Hidden::kN);
-            // with tiles for most CUs a tile takes the units in turn, which saves the parts' way through memory
-            g.in_turn = g.m_tiles * g.n_tiles >= 160 || units == 1;
-            g.hidden_blocks = g.m_tiles * g.n_tiles * (g.in_turn ? 1 : units);
-            if (!g.in_turn && piece >= s.vocabulary) parts = units;
+            // (how many tiles there are is known where the rows that count are: either way's workgroups)
+            const int64_t tiles = g.m_tiles * g.n_tiles;
+            hidden_blocks = units == 1 ? tiles : std::max(tiles, std::min(tiles, kTurnTiles - 1) * units);
+            add_parts = units > 1;
+            if (add_parts && tiles < kTurnTiles && piece >= s.vocabulary) parts = units, add_parts = false;  // one piece's: at the end
             g.begin = first == 0, g.total = b.total, g.part = b.part;
         }
         if (dweight) {
@@ -1099,10 +1111,10 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
             g.sums = b.sums, g.at = b.at, g.largest = b.largest, g.accumulate = accumulate;
             g.whole = s.dim % 8 == 0 && aligned_to(dweight, 16);
         }
-        gradient_kernel<T, Hidden, Weight><<<grid_of(g.hidden_blocks + g.weight_m_tiles * g.weight_n_tiles), Hidden::kThreads, 0, stream>>>(dweight, g);
-        if (dhidden && !g.in_turn && piece < s.vocabulary)  // (one piece's parts are added at the end)
-            add_parts_kernel<<<static_cast<unsigned>(std::min<size_t>(ceil_div(s.rows * s.dim, 256), 4096)), 256, 0, stream>>>(
-                b.part, b.total, b.order.kept, s.rows, s.dim, static_cast<int>(units), first == 0);
+        gradient_kernel<T, Hidden, Weight><<<grid_of(hidden_blocks + g.weight_m_tiles * g.weight_n_tiles), Hidden::kThreads, 0, stream>>>(dweight, g);
+        if (add_parts)
+            add_parts_kernel<Hidden::kM><<<static_cast<unsigned>(std::min<size_t>(ceil_div(s.rows * s.dim, 256), 4096)), 256, 0, stream>>>(
+                b.part, b.total, b.order.kept, s.rows, s.dim, g.n_tiles, static_cast<int>(units), first == 0);
     }
     return check_launch("vocabulary_loss_backward");
 }

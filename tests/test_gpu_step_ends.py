@@ -233,6 +233,19 @@ def test_loss_of_a_batch_of_which_few_rows_count(K, dtype, counted, vocabulary, 
 
 
 @pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize("counted", [1000, 3900])
+def test_loss_of_a_wide_batch_of_which_some_rows_count(K, dtype, counted):
+    """Enough tiles for each to take the vocabulary's units in turn, and, of the rows that count, too few; the same bits either way."""
+    p, dloss = loss_problem(K, 31, R.DTYPES[dtype], 4096, 16384, 2560, masked=0.0)
+    p.targets[:4096 - counted] = -1
+    p.check(dloss, randn(gen(32), 16384, 2560, dtype=R.DTYPES[dtype], scale=1e-3))
+    lse, dhidden = p.lse.clone(), p.backward(dloss)[0]
+    q = Loss(K, p.hidden[-300:].clone(), p.weight, p.targets[-300:].clone())
+    q.lse.copy_(lse[-300:])
+    assert torch.equal(q.backward(dloss[-300:].clone())[0], dhidden[-300:])
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
 def test_loss_of_rows_that_do_not_count(K, dtype):
     """What they hold reaches nothing, and their rows of the results are zero; none at all, and all but none."""
     dt = R.DTYPES[dtype]
