@@ -640,13 +640,17 @@ struct GradientArgs {
 // Whether a tile of dh adds the piece's units to the total itself; else each unit has a part. With tiles for most CUs that saves the
 // parts' way through memory; with fewer, the others would wait for them (8192 rows, 151936 x 1536, of which 3277 count: 78
 // tiles; 5.8 ms in turn, 5.0 with parts). The additions and their order are the same.
-constexpr int64_t kTurnTiles = 160;
-__host__ __device__ __forceinline__ bool in_turn(int64_t tiles, int64_t units) { return units == 1 || tiles >= kTurnTiles; }
+template <typename Tile>
+constexpr int64_t kTurnTiles = Tile::kM == 256 ? 160 : 320;
+template <typename Tile>
+__host__ __device__ __forceinline__ bool in_turn(int64_t tiles, int64_t units) {
+    return units == 1 || tiles >= kTurnTiles<Tile>;
+}
 
 template <typename T, typename Tile>
 __device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, int64_t m_tiles, int64_t units, LdsByte* lds) {
     const int64_t count = *a.count, each = m_tiles * a.n_tiles;
-    const bool turns = in_turn(each, units);
+    const bool turns = in_turn<Tile>(each, units);
     const int64_t only = turns ? 0 : id / each, end = turns ? units : only + 1;
     int64_t m, n;
     tile_of(id - only * each, m_tiles, a.n_tiles, m, n);
@@ -757,19 +761,19 @@ __global__ __launch_bounds__(HiddenTile::kThreads) void gradient_kernel(T* __res
     static_assert(HiddenTile::kThreads == WeightTile::kThreads);
     __shared__ __attribute__((aligned(1024))) char lds[HiddenTile::kLds > WeightTile::kLds ? HiddenTile::kLds : WeightTile::kLds];
     const int64_t id = block_id(), m_tiles = tiles_that_count<HiddenTile::kM>(*a.count, a.m_tiles), units = (a.width + a.unit - 1) / a.unit;
-    const int64_t each = m_tiles * a.n_tiles, hidden_tiles = in_turn(each, units) ? each : each * units;
+    const int64_t each = m_tiles * a.n_tiles, hidden_tiles = in_turn<HiddenTile>(each, units) ? each : each * units;
     if (id < hidden_tiles)
         hidden_tile<T, HiddenTile>(a, id, m_tiles, units, (LdsByte*)lds);
     else if (id < hidden_tiles + a.weight_m_tiles * a.weight_n_tiles)
         weight_tile<T, WeightTile>(dweight, a, id - hidden_tiles, (LdsByte*)lds);
 }
 
-// total (+)= the units' parts, in their order, where there are parts (kSize: of dh's tiles)
-template <int kSize>
+// total (+)= the units' parts, in their order, where there are parts
+template <typename HiddenTile>
 __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, float* __restrict__ total, const uint32_t* __restrict__ count,
                                                         int64_t rows, int64_t dim, int64_t n_tiles, int units, bool begin) {
     const int64_t n = static_cast<int64_t>(*count) * dim;
-    if (in_turn((static_cast<int64_t>(*count) + kSize - 1) / kSize * n_tiles, units)) return;
+    if (in_turn<HiddenTile>((static_cast<int64_t>(*count) + HiddenTile::kM - 1) / HiddenTile::kM * n_tiles, units)) return;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
         float v = begin ? part[i] : total[i] + part[i];
         for (int u = 1; u < units; ++u) v += part[u * rows * dim + i];
@@ -1101,9 +1105,9 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
             g.m_tiles = ceil_div(s.rows, Hidden::kM), g.n_tiles = ceil_div(s.dim, Hidden::kN);
             // (how many tiles there are is known where the rows that count are: either way's workgroups)
             const int64_t tiles = g.m_tiles * g.n_tiles;
-            hidden_blocks = units == 1 ? tiles : std::max(tiles, std::min(tiles, kTurnTiles - 1) * units);
+            hidden_blocks = units == 1 ? tiles : std::max(tiles, std::min(tiles, kTurnTiles<Hidden> - 1) * units);
             add_parts = units > 1;
-            if (add_parts && tiles < kTurnTiles && piece >= s.vocabulary) parts = units, add_parts = false;  // one piece's: at the end
+            if (add_parts && tiles < kTurnTiles<Hidden> && piece >= s.vocabulary) parts = units, add_parts = false;  // one piece's: at the end
             g.begin = first == 0, g.total = b.total, g.part = b.part;
         }
         if (dweight) {
@@ -1113,7 +1117,7 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
         }
         gradient_kernel<T, Hidden, Weight><<<grid_of(hidden_blocks + g.weight_m_tiles * g.weight_n_tiles), Hidden::kThreads, 0, stream>>>(dweight, g);
         if (add_parts)
-            add_parts_kernel<Hidden::kM><<<static_cast<unsigned>(std::min<size_t>(ceil_div(s.rows * s.dim, 256), 4096)), 256, 0, stream>>>(
+            add_parts_kernel<Hidden><<<static_cast<unsigned>(std::min<size_t>(ceil_div(s.rows * s.dim, 256), 4096)), 256, 0, stream>>>(
                 b.part, b.total, b.order.kept, s.rows, s.dim, g.n_tiles, static_cast<int>(units), first == 0);
     }
     return check_launch("vocabulary_loss_backward");
