@@ -330,12 +330,13 @@ __global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __rest
     const T* const h = hidden + row * a.s.hidden_stride;
     const int64_t target = kOf == kBackward ? static_cast<int64_t>(a.order.token[j]) : a.targets[row];
     const T* const w = weight + target * a.s.dim;
+    uint32_t size = 0;  // of the row's largest value
     int exponent = 0;
     const bool scaled = kScaled<T> && a.row_exponent;
     if (scaled) {
-        uint32_t top = 0;
-        for (int64_t d = lane; d < a.s.dim; d += kWave) top = max(top, size_bits(h[d]));
-        exponent = exponent_of(static_cast<int32_t>(wave_max(top)));
+        for (int64_t d = lane; d < a.s.dim; d += kWave) size = max(size, size_bits(h[d]));
+        size = wave_max(size);
+        exponent = exponent_of(static_cast<int32_t>(size));
         if (lane == 0) a.row_exponent[j] = exponent;
     }
     float x = 0.0f;
@@ -373,7 +374,8 @@ __global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __rest
             take_apart(factor, mantissa, e);
             a.terms.factor[j] = ldexpf(mantissa, kHalfShift);
             a.terms.exponent[j] = e;
-            if (e != kNoWeight) atomicMax(a.largest, e + exponent + kExponentBase);  // (a maximum, so the order does not matter)
+            // a row of zeroes is zeroes by any power, and does not take the others' bits. (A maximum, so the order does not matter.)
+            if (e != kNoWeight && (!kScaled<T> || size != 0)) atomicMax(a.largest, e + exponent + kExponentBase);
         } else {
             a.terms.factor[j] = factor;
         }
