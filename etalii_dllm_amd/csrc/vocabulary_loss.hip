@@ -186,7 +186,7 @@ __device__ __forceinline__ void load_eight(const T* row, int64_t d, int64_t dim,
 }
 
 // What scales a row by a power of two: nothing (kAsTheyAre: and float32 stays that), the size of its unit (weights), or its part in dW
-// (hidden states): factor's exponent and the row's from the largest, zero for none.
+// (hidden states): factor's exponent from the largest of that and the row's, so that the largest values are below 2^kTop; zero for none.
 enum PackScale { kNoScale, kAsTheyAre, kUnitScale, kWeightScale };
 constexpr int kNoWeight = -1000;      // the exponent of a factor of zero
 constexpr int kExponentBase = 1000;  // the largest exponent is held with this added, -1 before any
@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, ch
             by = kTop - exponent_of(a.sizes[j / kScaleRows]);
         } else {
             const int e = a.exponent[j];
-            by = e == kNoWeight ? 2 * kNoWeight : e - (*a.largest - kExponentBase) + (kScaled<T> ? kTop : 0);
+            by = e == kNoWeight ? 2 * kNoWeight : e - (*a.largest - kExponentBase) + kTop;
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], by);
@@ -277,7 +277,7 @@ struct RowsArgs {
     const float *lse, *dloss;
     RowTerms terms;
     float* coefficient;  // by row
-    int32_t* largest;    // float16 parts: kExponentBase and the largest exponent, of float32 with the row's added
+    int32_t* largest;    // float16 parts: kExponentBase and the largest exponent of a factor and its row together
 };
 
 // factor = mantissa 2^exponent, mantissa in [1, 2)
@@ -346,6 +346,10 @@ __global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __rest
         load_eight<T, kWhole>(w, d, a.s.dim, u);
 #pragma unroll
         for (int e = 0; e < 8; ++e) x = fmaf(v[e], u[e], x);
+        if constexpr (kOf == kBackward && kHalfParts<T> && !kScaled<T>) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) size = max(size, size_bits(v[e]));
+        }
         if constexpr (kScaled<T>) {
             if (!scaled) {
                 store_as_they_are(a.packed + j * a.s.row, d, v);
@@ -358,6 +362,10 @@ __global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __rest
     }
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
+    if constexpr (kOf == kBackward && kHalfParts<T> && !kScaled<T>) {
+        size = wave_max(size);
+        exponent = exponent_of(static_cast<int32_t>(size));
+    }
     if (lane != 0) return;
     float derivative;
     const float z = Cap(a.s).logit<kCapped>(x, derivative);
@@ -375,7 +383,7 @@ __global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __rest
             a.terms.factor[j] = ldexpf(mantissa, kHalfShift);
             a.terms.exponent[j] = e;
             // a row of zeroes is zeroes by any power, and does not take the others' bits. (A maximum, so the order does not matter.)
-            if (e != kNoWeight && (!kScaled<T> || size != 0)) atomicMax(a.largest, e + exponent + kExponentBase);
+            if (e != kNoWeight && size != 0) atomicMax(a.largest, e + exponent + kExponentBase);
         } else {
             a.terms.factor[j] = factor;
         }
@@ -711,7 +719,7 @@ __device__ __forceinline__ void weight_tile(T* __restrict__ dweight, const Gradi
     typename Tile::Sums acc;
     Tile::run(a.softmax, a.hidden, m * Tile::kM, n * Tile::kN, a.width, a.dim, *a.count, 0, 0, lds, acc);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
-    const int by = kHalfParts<T> ? *a.largest - kExponentBase - kHalfShift - (kScaled<T> ? kTop : 0) : 0;
+    const int by = kHalfParts<T> ? *a.largest - kExponentBase - kHalfShift - kTop : 0;
     struct Old {
         int32_t at;
         Pack<T, 8> v;

@@ -392,9 +392,10 @@ int dllm_hip_token_embedding_backward(const dllm_hip_token_embedding_shape* shap
  * writes dhidden (zero where a row does not count) and dweight; either may be NULL. accumulate adds to what dweight holds, in
  * float32 before the one rounding. It forms the logits again, a piece of the vocabulary at a time. The softmax's part of a
  * gradient has the probabilities as operands in dtype, the target's part is float32's. float16 holds the probabilities times each
- * row's dloss relative to it, so that gradients of any size keep their bits; in dweight, rows whose dloss is below 2^-14
- * of the largest one's lose some of their softmax's part. float32 has pairs of float16 as operands, 22 bits and more of each
- * value: hidden states off by at most 2^-39 of their row's largest value (in dweight, of the largest one times its dloss), weights
+ * row's dloss relative to it, so that gradients of any size keep their bits, and in dweight the hidden states times the power of two
+ * of their dloss: both together are off by at most 2^-38 of the largest one times its dloss, so those below 2^-28 of it
+ * lose bits. float32 has pairs of float16 as operands, 22 bits and more of each
+ * value: hidden states off by at most 2^-39 of their row's largest value (in dweight, 2^-38 of the largest one times its dloss), weights
  * of 2048 rows' largest, so values far below those lose bits.
  * A row's loss, lse and dhidden are the same bits alone and in any batch (dhidden: from the same lse); float32's loss and lse are where
  * the batches have at most 256 rows, and where they have more: few rows are multiplied by the weights as they are. hidden_stride and dhidden_stride: elements between rows (0: dim).

@@ -192,3 +192,20 @@ def finite_difference(f, x, d, step=1e-6):
 
 
 assert math.isfinite(F)
+
+
+def light_rows(hidden, weight, targets, lse, dloss, scale=1.0, softcap=0.0, old=None):
+    """loss_backward of float16 with what dweight's hidden states are held to as operands: times the power of two of their dloss,
+    below 2^15 by the largest such product, so off by half of 2^-24 there, 2^-40 of it, and twice that for each of the two powers."""
+    assert hidden.dtype == torch.float16
+    got = loss_backward(hidden, weight, targets, lse, dloss, scale, softcap, old)
+    inside = (targets >= 0) & (targets < len(weight))
+    factor = torch.where(inside, dloss.double().abs() * scale, torch.zeros_like(dloss, dtype=torch.float64))[:, None]
+    counted = torch.where(inside[:, None], hidden, torch.zeros_like(hidden))
+    z, _, slope, _ = _logits(counted, weight, scale, softcap)
+    hot = torch.zeros_like(z).scatter_(1, targets.clamp(0, len(weight) - 1)[:, None], 1.0)
+    soft = torch.exp(z - torch.where(inside, lse, torch.zeros_like(lse)).double()[:, None]) * (1 - hot) * slope * (factor > 0)
+    stated = soft.T @ (2.0 ** -24 * (counted != 0).double()) * factor.max()  # loss_backward's bound of the same
+    held = soft.sum(dim=0)[:, None] * (factor * counted.double().abs().amax(dim=1, keepdim=True)).max() * 2.0 ** -38
+    value, bound = got["dweight"]
+    return dict(got, dweight=(value, bound + (held - stated) * (1 + unit(hidden.dtype))))
