@@ -6,14 +6,16 @@
 // the same every time. Up to 16384 positions are first dealt to workgroups by a hash of the token, since one workgroup's ballots
 // over all of them took 39 us; more go through memory, each pass three launches.
 //
-// Sums: a wave takes 8 sorted positions and 16 bytes of columns to a lane, reads all 8 rows at once and adds them in order.
-// A token whose positions lie within the 8 is done; the sums of others are float32 parts, added in their order by a second
-// launch. Nothing depends on when a wave runs. 16381 rows of 576 in float32 onto a table that is added to: sort 22 us, sums 14
+// Sums: a token's positions are added 8 at a time from its first one on, whatever tokens lie beside it, so a row of the sums is the
+// same bits in any batch that has its positions. A wave takes the groups of 8 that begin among 8 sorted positions, and
+// 16 bytes of columns to a lane; it reads all their rows (up to 15) at once and adds them in order. A token of at most 8 is done; the
+// groups of others are float32 parts, added in their order by a second launch. Nothing depends on when a wave runs. 16381 rows of 576 in float32 onto a table that is added to: sort 22 us, sums 14
 // (2.7 TB/s of rows read), parts 9, a chain of additions as long as the most frequent token's; 16 positions to a wave were no faster.
 #include "token_rows.h"
 
 #include <algorithm>
 #include <initializer_list>
+#include <type_traits>
 
 namespace dllm_hip {
 
@@ -334,83 +336,129 @@ __device__ __forceinline__ void finish_sum(const SumArgs& a, T* table, uint32_t 
     store_from_float<T, kWidth>(row, acc);
 }
 
-// part[block][0]: what the block's first token has here, if it began earlier; part[block][1]: what its last one has here, if it
-// begins here and goes on.
+// What a wave makes of the positions first .. first + 15, a lane each (16 lanes count): bit masks.
+struct Runs {
+    uint32_t inside;  // there is a position, of a token inside the vocabulary
+    uint32_t starts;  // a token's first position
+    uint32_t groups;  // the first of a token's 8
+    int earlier;      // positions of the first one's token before it
+};
+
+// The start of the run of t that reaches up to `first` from below, where token[first - 1] is t: 64 probes at a time, since
+// whether a position before `first` is the run's goes from no to yes once.
+__device__ __forceinline__ int64_t run_start(const uint32_t* token, int64_t first, uint32_t t, int lane) {
+    int64_t low = 0, high = first - 1;  // the start is in [low, high], and high is the run's
+    {
+        const int64_t at = first - 1 - lane;  // most runs are short
+        const uint64_t in = __ballot(at >= 0 && token[at >= 0 ? at : 0] == t);
+        if (~in) return first - (__ffsll(static_cast<unsigned long long>(~in)) - 1);
+        high = first - kWave;
+    }
+    while (low < high) {
+        const int64_t step = (high - low + kWave - 1) / kWave;
+        const int64_t at = min(low + lane * step, high);
+        const int in = __ffsll(static_cast<unsigned long long>(__ballot(token[at] == t))) - 1;
+        if (in < 0) {  // (between the last probe and high)
+            low = min(low + (kWave - 1) * step, high) + 1;
+        } else {
+            high = min(low + in * step, high);
+            if (in > 0) low = min(low + (in - 1) * step, high - 1) + 1;
+            else low = high;
+        }
+    }
+    return low;
+}
+
+__device__ __forceinline__ Runs runs_of(const uint32_t* token, int64_t n, uint32_t outside, int64_t first, int lane, uint32_t own) {
+    const uint32_t t0 = __builtin_amdgcn_readfirstlane(own), previous = first > 0 ? token[first - 1] : outside;
+    const uint32_t before = __shfl_up(own, 1);
+    Runs r;
+    r.inside = static_cast<uint32_t>(__ballot(lane < 2 * kSumRows && first + lane < n && own != outside));
+    r.starts = static_cast<uint32_t>(__ballot(lane < 2 * kSumRows && own != (lane == 0 ? previous : before))) & r.inside;
+    r.earlier = 0;
+    if (first > 0 && t0 != outside && t0 == previous) r.earlier = static_cast<int>((first - run_start(token, first, t0, lane)) & (kSumRows - 1));
+    const uint32_t below = r.starts & ((2u << (lane & 31)) - 1);
+    const int rank = below ? lane - (31 - __clz(below)) : lane + r.earlier;
+    r.groups = static_cast<uint32_t>(__ballot(lane < 2 * kSumRows && (rank & (kSumRows - 1)) == 0)) & r.inside;
+    return r;
+}
+
+// A wave forms the sums of the groups of 8 that begin among its 8 positions. part[block][0]: of a token that began earlier;
+// part[block][1]: the first 8 of one that begins here and has more.
 template <typename T, int kWidth>
 __global__ __launch_bounds__(256) void token_sums_kernel(const T* __restrict__ rows, T* __restrict__ table, SumArgs a) {
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int64_t block = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)));
     if (block >= a.blocks) return;
     const int64_t first = block * kSumRows, column = (static_cast<int64_t>(blockIdx.y) * kWave + lane) * kWidth;
-    const int count = static_cast<int>(min(a.n - first, static_cast<int64_t>(kSumRows)));
-    // lane 0: the position before; lanes 1 .. count: the block's; lane count + 1: the one after
     uint32_t token = a.outside, position = 0;
-    const int64_t at = first + lane - 1;
-    if (lane <= count + 1 && at >= 0 && at < a.n) token = a.token[at], position = a.position[at];
-    float mine = 1.0f;
-    if (a.coefficient && lane >= 1 && lane <= count && token != a.outside) mine = a.coefficient[position];
+    if (lane < 2 * kSumRows && first + lane < a.n) token = a.token[first + lane], position = a.position[first + lane];
+    const Runs r = runs_of(a.token, a.n, a.outside, first, lane, token);
+    // from the first group that begins here to the end of the last one
+    const uint32_t here = r.groups & ((1u << kSumRows) - 1), past = (r.groups | ~r.inside) >> kSumRows;
+    if (!here) return;
+    const int begin = __ffs(here) - 1, end = kSumRows + __ffs(past | (1u << kSumRows)) - 1;
+    const uint32_t mine = r.inside & ((1u << end) - 1) & ~((1u << begin) - 1);
+    float weight = 1.0f;
+    if (a.coefficient && mine >> (lane & 31) & 1 && lane < 2 * kSumRows) weight = a.coefficient[position];
     const bool inside = column < a.dim;
-    Pack<T, kWidth> row[kSumRows] = {};
+    constexpr int kMost = 2 * kSumRows - 1;
+    using Words = uint32_t __attribute__((ext_vector_type(kWidth * sizeof(T) >= 8 ? kWidth * sizeof(T) / 4 : 2)));
+    using Row = std::conditional_t<kWidth == 1, T, Words>;  // (16-bit elements one by one would take a register each)
+    Row row[kMost] = {};
 #pragma unroll
-    for (int i = 0; i < kSumRows; ++i) {
-        const uint32_t t = __builtin_amdgcn_readlane(token, i + 1);
-        const uint32_t p = __builtin_amdgcn_readlane(position, i + 1);
-        if (i < count && t != a.outside && inside)
-            row[i] = *reinterpret_cast<const Pack<T, kWidth>*>(rows + static_cast<int64_t>(p) * a.stride + column);
+    for (int i = 0; i < kMost; ++i) {
+        const uint32_t p = __builtin_amdgcn_readlane(position, i);
+        if (mine >> i & 1 && inside) row[i] = *reinterpret_cast<const Row*>(rows + static_cast<int64_t>(p) * a.stride + column);
     }
     // (all lanes stay: the tokens are read from lanes whose columns are past the row too)
     float acc[kWidth] = {};
-    int begin = 0;
-    bool earlier = false;
+    int group = begin;
 #pragma unroll
-    for (int i = 0; i < kSumRows; ++i) {
-        const uint32_t t = __builtin_amdgcn_readlane(token, i + 1), previous = __builtin_amdgcn_readlane(token, i),
-                       next = __builtin_amdgcn_readlane(token, i + 2);
-        if (i >= count || t == a.outside) break;
-        if (i == 0) earlier = previous == t && first > 0;
-        const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, mine), i + 1));
+    for (int i = 0; i < kMost; ++i) {
+        if (!(mine >> i & 1)) continue;
+        const float c = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, weight), i));
+        const Pack<T, kWidth> v = __builtin_bit_cast(Pack<T, kWidth>, row[i]);
 #pragma unroll
-        for (int j = 0; j < kWidth; ++j) acc[j] = fmaf(c, static_cast<float>(row[i].v[j]), acc[j]);
-        const bool last = i == count - 1, goes_on = next == t;
-        if (!last && goes_on) continue;
+        for (int j = 0; j < kWidth; ++j) acc[j] = fmaf(c, static_cast<float>(v.v[j]), acc[j]);
+        if (!((r.groups | ~r.inside) >> (i + 1) & 1)) continue;
         if (inside) {
-            if (!earlier && !goes_on)
-                finish_sum<T, kWidth>(a, table, t, first + begin, column, acc);
+            const bool begins = r.starts >> group & 1, ends = (r.starts | ~r.inside) >> (i + 1) & 1;
+            if (begins && ends)
+                finish_sum<T, kWidth>(a, table, __builtin_amdgcn_readlane(token, i), first + group, column, acc);
             else
-                store_from_float<float, kWidth>(a.part + (2 * block + (earlier ? 0 : 1)) * a.dim + column, acc);
+                store_from_float<float, kWidth>(a.part + (2 * block + (begins ? 1 : 0)) * a.dim + column, acc);
         }
 #pragma unroll
         for (int j = 0; j < kWidth; ++j) acc[j] = 0.0f;
-        begin = i + 1;
-        earlier = false;
+        group = i + 1;
     }
 }
 
-// Adds the parts of a token whose positions begin in this block and go on.
+// Adds the groups' parts of a token that begins among this wave's positions and has more than 8.
 template <typename T, int kWidth>
 __global__ __launch_bounds__(256) void token_parts_kernel(T* __restrict__ table, SumArgs a) {
     const int lane = static_cast<int>(threadIdx.x) & 63;
     const int64_t block = __builtin_amdgcn_readfirstlane(static_cast<int>(static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6)));
-    if (block >= a.blocks - 1) return;  // the last block's tokens end there
-    const int64_t first = block * kSumRows, end = first + kSumRows;
-    const uint32_t t = a.token[end - 1];
-    if (t == a.outside || a.token[end] != t) return;
-    if (a.token[first] == t && first > 0 && a.token[first - 1] == t) return;  // began earlier
-    // the sorted index of its first position
-    const uint64_t same = __ballot(lane < kSumRows && a.token[first + (lane < kSumRows ? lane : 0)] == t);
-    const int64_t index = first + (__ffsll(static_cast<unsigned long long>(same)) - 1);
-    // further blocks that it reaches into
+    if (block >= a.blocks - 1) return;  // what begins in the last block has at most 8
+    const int64_t first = block * kSumRows;
+    const uint32_t own = lane < kSumRows ? a.token[first + lane] : a.outside;
+    const uint32_t previous = lane > 0 ? a.token[first + min(lane, kSumRows) - 1] : first > 0 ? a.token[first - 1] : a.outside;
+    const uint32_t starts = static_cast<uint32_t>(__ballot(lane < kSumRows && own != a.outside && own != previous));
+    if (!starts) return;
+    const int64_t index = first + 31 - __clz(starts);  // the last one alone can have more
+    const uint32_t t = a.token[index];
+    // further groups
     int64_t more = 0;
-    for (int64_t b = block + 1;; b += kWave) {
-        const int64_t last = (b + lane + 1) * kSumRows;  // the position after block b + lane
-        const bool goes_on = last < a.n && a.token[last - 1] == t && a.token[last] == t;
-        const uint64_t stops = ~__ballot(goes_on);
+    for (;; more += kWave) {
+        const int64_t at = index + (more + lane + 1) * kSumRows;
+        const uint64_t stops = ~__ballot(at < a.n && a.token[min(at, a.n - 1)] == t);
         if (stops) {
-            more += __ffsll(static_cast<unsigned long long>(stops));
+            more += __ffsll(static_cast<unsigned long long>(stops)) - 1;
             break;
         }
-        more += kWave;
     }
+    if (more == 0) return;
     const int64_t column = (static_cast<int64_t>(blockIdx.y) * kWave + lane) * kWidth;
     if (column >= a.dim) return;
     float acc[kWidth];

@@ -364,7 +364,8 @@ int dllm_hip_residual_norm_backward(const dllm_hip_residual_norm_shape* shape, c
 
 /* Embedding lookup: out[t] = scale * table[tokens[t]], table[vocabulary, dim], tokens[tokens] (int64, device). A token outside the
  * vocabulary (padding) gives a row of zeroes. stride: elements between the rows of out, and of dout (0: dim).
- * The backward: dtable[v] = scale * sum of dout[t] over the t with token v, added in order of t in float32; all other rows are
+ * The backward: dtable[v] = scale * sum of dout[t] over the t with token v, in float32: in order of t, 8 at a time from the first
+ * on, and those sums in order, so a row's bits are its own whatever the other tokens are; all other rows are
  * zero. With accumulate the sum is added to what dtable holds, in float32 before the one rounding (the table of a model
  * whose embeddings are tied gathers its gradient from both ends), and rows of tokens that do not occur stay as they are.
  * Tokens outside the vocabulary count for nothing. out or dtable do not overlap inputs.

@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import ends_reference as R
-from test_gpu_step_ends import K, Loss, gen, randn  # noqa: F401
+from test_gpu_step_ends import K, Loss, embed_backward, gen, randn, some_tokens  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -74,3 +74,60 @@ def test_float16_gradients_of_unequal_rows(K):  # noqa: F811
     got, want = p.backward(dloss), R.light_rows(hidden, weight, targets, lse, dloss, softcap=9.0)
     R.assert_within(got[0], want["dhidden"], "dhidden")
     R.assert_within(got[1], want["dweight"], "dweight")
+
+
+# ---- the table's gradient ----
+
+
+def in_groups(ids, dout, vocabulary, scale):
+    """The sums in the order that is promised, in float32: each token's positions 8 at a time, then those sums."""
+    total = torch.zeros(vocabulary, dout.shape[1])
+    order = torch.argsort(ids, stable=True)
+    tokens, counts = torch.unique_consecutive(ids[order], return_counts=True)
+    for token, rows in zip(tokens.tolist(), order.split(counts.tolist())):
+        if not 0 <= token < vocabulary:
+            continue
+        parts = []
+        for some in rows.split(8):
+            acc = dout[some[0]].float()
+            for i in some[1:]:
+                acc = acc + dout[i].float()
+            parts.append(acc)
+        acc = parts[0]
+        for part in parts[1:]:
+            acc = acc + part
+        total[token] = acc * scale
+    return total
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize(("tokens", "vocabulary", "dim"), [(7, 3, 8), (9, 1, 4), (100, 9, 16), (1000, 70, 24), (3000, 40, 3), (16384, 3000, 8), (16385, 5, 8),
+                                                           (30000, 20000, 4)])
+def test_embedding_gradient_adds_in_its_order(K, dtype, tokens, vocabulary, dim):  # noqa: F811
+    g, dt = gen(80), R.DTYPES[dtype]
+    ids = some_tokens(g, tokens, vocabulary)
+    dout = randn(g, tokens, dim, dtype=dt)
+    want = in_groups(ids.cpu(), dout.cpu(), vocabulary, 0.5).to(dt)  # (a power of two: no rounding of its own)
+    assert torch.equal(embed_backward(K, ids, dout, vocabulary, 0.5).cpu(), want)
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
+def test_embedding_gradient_of_a_token_in_other_company(K, dtype):  # noqa: F811
+    """A token's row has the same bits whatever other tokens a batch has."""
+    g, dt = gen(81), R.DTYPES[dtype]
+    counts = [1, 2, 7, 8, 9, 15, 16, 17, 24, 63, 65, 200, 1000, 6000]
+    ids = torch.cat([torch.full((c,), 3 * i + 40, device="cuda") for i, c in enumerate(counts)])
+    ids = ids[torch.randperm(len(ids), generator=g, device="cuda")]
+    dout = randn(g, len(ids), 40, dtype=dt)
+    alone = embed_backward(K, ids, dout, 100)
+    seen = torch.unique(ids)
+    for others in (1, 3, 500, 9000, 40000):
+        more = torch.randint(0, 40, (others,), generator=g, device="cuda")
+        if others > 500:  # between them too
+            more = torch.where(torch.rand(others, generator=g, device="cuda") < 0.5, more, 41 + 3 * (more % 14))
+        keep = torch.rand(len(ids) + others, generator=g, device="cuda").argsort()[:len(ids)].sort().values
+        mixed, rows = torch.empty(len(ids) + others, dtype=torch.int64, device="cuda"), randn(g, len(ids) + others, 40, dtype=dt)
+        rest = torch.ones(len(mixed), dtype=torch.bool, device="cuda")
+        rest[keep] = False
+        mixed[keep], mixed[rest], rows[keep] = ids, more, dout
+        assert torch.equal(embed_backward(K, mixed, rows, 100)[seen], alone[seen]), others
