@@ -632,11 +632,11 @@ __global__ __launch_bounds__(Tile::kThreads) void softmax_kernel(SoftmaxArgs a, 
 struct GradientArgs {
     Operand softmax, weight, hidden;  // softmax.batch, weight.batch: a unit
     const uint32_t* count;
-    int64_t rows, dim, first, width, unit;  // first and width: of the piece
+    int64_t dim, first, width, unit;  // first and width: of the piece
     // dh
     int64_t m_tiles, n_tiles;  // none without dh
     bool begin;  // the total begins here
-    float *total, *part;
+    float *total, *part;  // [row], [unit][row] of those that count
     // dW
     int64_t weight_m_tiles, weight_n_tiles;
     const float* sums;       // the targets' part, by the index in `at`
@@ -649,23 +649,26 @@ struct GradientArgs {
 
 // Whether a tile of dh adds the piece's units to the total itself; else each unit has a part. With tiles for most CUs that saves the
 // parts' way through memory; with fewer, the others would wait for them (8192 rows, 151936 x 1536, of which 3277 count: 78
-// tiles; 5.8 ms in turn, 5.0 with parts). The additions and their order are the same.
+// tiles; 5.8 ms in turn, 5.0 with parts). Parts are kPartFloats at most: to write and read more takes as long as the tiles in turn, beside
+// dW's (12287 of the vocabulary: 1000 rows of 2900, 0.26 GiB of parts, 0.54 ms and 0.76 in turn; 2000 of 2304, 0.41 GiB, 0.64 and 0.53; 2458 of
+// 2304, 0.51 GiB, 0.76 and 0.77). The additions and their order are the same.
 template <typename Tile>
 constexpr int64_t kTurnTiles = Tile::kM == 256 ? 160 : 320;
+constexpr int64_t kPartFloats = int64_t{96} << 20;
 template <typename Tile>
-__host__ __device__ __forceinline__ bool in_turn(int64_t tiles, int64_t units) {
-    return units == 1 || tiles >= kTurnTiles<Tile>;
+__host__ __device__ __forceinline__ bool in_turn(int64_t rows, int64_t dim, int64_t n_tiles, int64_t units) {
+    return units == 1 || (rows + Tile::kM - 1) / Tile::kM * n_tiles >= kTurnTiles<Tile> || rows * dim * units > kPartFloats;
 }
 
 template <typename T, typename Tile>
 __device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, int64_t m_tiles, int64_t units, LdsByte* lds) {
     const int64_t count = *a.count, each = m_tiles * a.n_tiles;
-    const bool turns = in_turn<Tile>(each, units);
+    const bool turns = in_turn<Tile>(count, a.dim, a.n_tiles, units);
     const int64_t only = turns ? 0 : id / each, end = turns ? units : only + 1;
     int64_t m, n;
     tile_of(id - only * each, m_tiles, a.n_tiles, m, n);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
-    float* const out = turns ? a.total : a.part + only * a.rows * a.dim;
+    float* const out = turns ? a.total : a.part + only * count * a.dim;
     for (int64_t unit = only; unit < end; ++unit) {
         typename Tile::Sums acc;
         Tile::run(a.softmax, a.weight, m * Tile::kM, n * Tile::kN, count, a.dim, min(a.unit, a.width - unit * a.unit), unit, unit, lds, acc);
@@ -770,8 +773,8 @@ template <typename T, typename HiddenTile, typename WeightTile>
 __global__ __launch_bounds__(HiddenTile::kThreads) void gradient_kernel(T* __restrict__ dweight, GradientArgs a) {
     static_assert(HiddenTile::kThreads == WeightTile::kThreads);
     __shared__ __attribute__((aligned(1024))) char lds[HiddenTile::kLds > WeightTile::kLds ? HiddenTile::kLds : WeightTile::kLds];
-    const int64_t id = block_id(), m_tiles = tiles_that_count<HiddenTile::kM>(*a.count, a.m_tiles), units = (a.width + a.unit - 1) / a.unit;
-    const int64_t each = m_tiles * a.n_tiles, hidden_tiles = in_turn<HiddenTile>(each, units) ? each : each * units;
+    const int64_t id = block_id(), count = *a.count, m_tiles = tiles_that_count<HiddenTile::kM>(count, a.m_tiles), units = (a.width + a.unit - 1) / a.unit;
+    const int64_t each = m_tiles * a.n_tiles, hidden_tiles = in_turn<HiddenTile>(count, a.dim, a.n_tiles, units) ? each : each * units;
     if (id < hidden_tiles)
         hidden_tile<T, HiddenTile>(a, id, m_tiles, units, (LdsByte*)lds);
     else if (id < hidden_tiles + a.weight_m_tiles * a.weight_n_tiles)
@@ -781,12 +784,12 @@ __global__ __launch_bounds__(HiddenTile::kThreads) void gradient_kernel(T* __res
 // total (+)= the units' parts, in their order, where there are parts
 template <typename HiddenTile>
 __global__ __launch_bounds__(256) void add_parts_kernel(const float* __restrict__ part, float* __restrict__ total, const uint32_t* __restrict__ count,
-                                                        int64_t rows, int64_t dim, int64_t n_tiles, int units, bool begin) {
+                                                        int64_t dim, int64_t n_tiles, int units, bool begin) {
     const int64_t n = static_cast<int64_t>(*count) * dim;
-    if (in_turn<HiddenTile>((static_cast<int64_t>(*count) + HiddenTile::kM - 1) / HiddenTile::kM * n_tiles, units)) return;
+    if (in_turn<HiddenTile>(*count, dim, n_tiles, units)) return;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < n; i += static_cast<int64_t>(gridDim.x) * 256) {
         float v = begin ? part[i] : total[i] + part[i];
-        for (int u = 1; u < units; ++u) v += part[u * rows * dim + i];
+        for (int u = 1; u < units; ++u) v += part[u * n + i];
         total[i] = v;
     }
 }
@@ -801,11 +804,11 @@ struct FinishArgs {
 
 template <typename T>
 __global__ __launch_bounds__(256) void finish_hidden_kernel(const T* __restrict__ weight, T* __restrict__ dhidden, FinishArgs a) {
-    const int64_t j = block_id();
+    const int64_t j = block_id(), count = *a.order.kept;
     if (j >= a.s.rows) return;
     const int64_t row = a.order.position[j];
     T* const out = dhidden + row * a.s.dhidden_stride;
-    if (j >= static_cast<int64_t>(*a.order.kept)) {
+    if (j >= count) {
         for (int64_t d = threadIdx.x; d < a.s.dim; d += 256) out[d] = static_cast<T>(0.0f);
         return;
     }
@@ -818,7 +821,7 @@ __global__ __launch_bounds__(256) void finish_hidden_kernel(const T* __restrict_
         for (int64_t u = 1; u < a.parts; u += kAhead) {
             float w[kAhead];
 #pragma unroll
-            for (int k = 0; k < kAhead; ++k) w[k] = u + k < a.parts ? a.total[((u + k) * a.s.rows + j) * a.s.dim + d] : 0.0f;
+            for (int k = 0; k < kAhead; ++k) w[k] = u + k < a.parts ? a.total[((u + k) * count + j) * a.s.dim + d] : 0.0f;
 #pragma unroll
             for (int k = 0; k < kAhead; ++k)
                 if (u + k < a.parts) v += w[k];
@@ -897,7 +900,7 @@ struct LossLayout {
         sizes = dtype == kFloat32 ? ceil_div(s.vocabulary, kScaleRows) : 0;
         terms = backward ? round_up(rows, 256) : 0;
         softmax = backward ? rows * (units * unit + kStrideSlack) * planes : 0;
-        part = backward ? units * rows * dim : 0;
+        part = backward && units > 1 ? std::min<size_t>(units * rows * dim, kPartFloats) : 0;
         total = backward ? rows * dim : 0;
         sums = total;
         sum_parts = backward ? token_sums_part_floats(s.rows, s.dim) : 0;
@@ -1107,7 +1110,7 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
         g.softmax = Operand{b.softmax, a.out_stride, value_at<kLossPlanes<T>>(layout.unit), s.rows};
         g.weight = a.weight, g.weight.batch = layout.unit * a.weight.stride;
         g.hidden = hidden_operand(s, kHalfParts<T> ? b.scaled : b.hidden);
-        g.sizes = a.sizes, g.count = b.order.kept, g.rows = s.rows, g.dim = s.dim, g.first = first, g.width = width, g.unit = layout.unit;
+        g.sizes = a.sizes, g.count = b.order.kept, g.dim = s.dim, g.first = first, g.width = width, g.unit = layout.unit;
         const int64_t units = ceil_div(width, layout.unit);
         int64_t hidden_blocks = 0;
         bool add_parts = false;
@@ -1117,7 +1120,7 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
             const int64_t tiles = g.m_tiles * g.n_tiles;
             hidden_blocks = units == 1 ? tiles : std::max(tiles, std::min(tiles, kTurnTiles<Hidden> - 1) * units);
             add_parts = units > 1;
-            if (add_parts && tiles < kTurnTiles<Hidden> && piece >= s.vocabulary) parts = units, add_parts = false;  // one piece's: at the end
+            if (add_parts && !in_turn<Hidden>(s.rows, s.dim, g.n_tiles, units) && piece >= s.vocabulary) parts = units, add_parts = false;  // one piece's: at the end
             g.begin = first == 0, g.total = b.total, g.part = b.part;
         }
         if (dweight) {
@@ -1128,7 +1131,7 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
         gradient_kernel<T, Hidden, Weight><<<grid_of(hidden_blocks + g.weight_m_tiles * g.weight_n_tiles), Hidden::kThreads, 0, stream>>>(dweight, g);
         if (add_parts)
             add_parts_kernel<Hidden><<<static_cast<unsigned>(std::min<size_t>(ceil_div(s.rows * s.dim, 256), 4096)), 256, 0, stream>>>(
-                b.part, b.total, b.order.kept, s.rows, s.dim, g.n_tiles, static_cast<int>(units), first == 0);
+                b.part, b.total, b.order.kept, s.dim, g.n_tiles, static_cast<int>(units), first == 0);
     }
     return check_launch("vocabulary_loss_backward");
 }

@@ -131,3 +131,24 @@ def test_embedding_gradient_of_a_token_in_other_company(K, dtype):  # noqa: F811
         rest[keep] = False
         mixed[keep], mixed[rest], rows[keep] = ids, more, dout
         assert torch.equal(embed_backward(K, mixed, rows, 100)[seen], alone[seen]), others
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
+def test_loss_gradients_whose_parts_would_be_many(K, dtype):  # noqa: F811
+    """Few tiles of dhidden, and so much of it that they take the vocabulary's units in turn; the same bits as in parts."""
+    g, dt = gen(74), R.DTYPES[dtype]
+    weight = randn(g, 12287, 2900, dtype=dt, scale=2.0 / math.sqrt(2900))
+    hidden = randn(g, 1600, 2900, dtype=dt)
+    targets = torch.randint(0, 12287, (1600,), generator=g, device="cuda")
+    dloss = torch.rand(1600, generator=g, device="cuda") / 1600
+    p = Loss(K, hidden, weight, targets)
+    p.check(dloss)
+    dhidden = p.backward(dloss)[0]
+    p.targets = targets.clone()
+    p.targets[:500] = -1  # in parts
+    some = p.backward(dloss)[0]
+    assert torch.equal(some[500:], dhidden[500:]) and bool((some[:500] == 0).all())
+    for first, n in ((0, 1000), (300, 50)):
+        q = Loss(K, hidden[first:first + n].clone(), weight, targets[first:first + n].clone())
+        q.lse.copy_(p.lse[first:first + n])
+        assert torch.equal(q.backward(dloss[first:first + n].clone())[0], dhidden[first:first + n])

@@ -223,3 +223,20 @@ def test_orthogonalize_definition():
     assert (R.orthogonalize(x.T) - R.orthogonalize(x).T).abs().max() < 1e-12
     rounded = R.orthogonalize(x, rounding=R.halves(1)) - R.orthogonalize(x)
     assert 1e-6 < rounded.abs().max() < 1e-2 and (R.orthogonalize(x, rounding=R.halves(2)) - R.orthogonalize(x)).abs().max() < 1e-5
+
+
+@needs_library
+@pytest.mark.parametrize("dtype", [0, 1, 2])
+@pytest.mark.parametrize(("rows", "vocabulary", "dim"), [
+    (8192, 12287, 2304), (8192, 12287, 8192), (8192, 151936, 1536), (131072, 151936, 4096), (131072, 300, 4096), (100, 12287, 65536),
+    (3000, 700, 65536), (16384, 256000, 2304), (1, 1, 1), (1, 2 ** 31 - 1, 8), (64, 2 ** 30, 65536)])
+def test_loss_workspace_is_what_is_said_of_it(K, dtype, rows, vocabulary, dim):
+    """256 MB of softmax, or a unit of 8192 (float32: 2048) of the vocabulary; half as much again at most of packed weights, by its
+    own rule; 384 MB of dhidden's parts; rows of hidden and of float32."""
+    size = 4 if dtype == 0 else 2
+    need = K.lib.dllm_hip_vocabulary_loss_backward_workspace(K.VocabularyLoss(**{**LOSS, "dtype": dtype, "rows": rows, "vocabulary": vocabulary, "dim": dim}))
+    unit, padded = 2048 if dtype == 0 else 8192, (dim + 31) // 32 * 32
+    softmax = max(2 ** 28, rows * unit * size) + 64 * rows * size
+    weight = max(2 ** 29, unit * padded * size)
+    others = rows * padded * (2 * size + 4 + 4 + 1) + 8 * padded + rows * 64 + 5 * vocabulary + 2 ** 23
+    assert 0 < need <= softmax + weight + 3 * 2 ** 27 + others, need
