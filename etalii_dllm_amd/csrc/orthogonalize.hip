@@ -9,9 +9,11 @@
 // small singular values is far smaller than a X.
 //
 // The products' operands are float16 (bfloat16's 8 bits would cost results two of theirs): one part of 11 bits for bfloat16 updates,
-// whose own 8 bits are coarser than what that adds (of the result, by its 2-norm: 5e-4 after five steps and 1.4e-3 after six, where
+// whose own 8 bits are coarser than what that adds (of the result, by its 2-norm: 5e-4 after five steps, where
 // rounding it once is 1.7e-3), pairs of 22 bits, three products, for float32 and float16 ones, and for small matrices, whose few
-// singular values average no rounding out (2 x 76: 2.5e-3 with one part). All values are bounded by the singular values, which stay near one, so fixed
+// singular values average no rounding out (2 x 76: 2.5e-3 with one part). From the fifth step on singular values are near one, the term is
+// as large as a X, and its error stays: calls of more than five steps multiply pairs from there on (256 x 1024, six steps: off by 1.3e-3 before the result's
+// rounding with one part, 1e-4 so; ten steps 3.4e-3 and 2e-4), at 1.9 times the time of such a step (24 of 896 x 4864, six steps: 3.33 to 4.28 ms). All values are bounded by the singular values, which stay near one, so fixed
 // powers of two keep them in float16's range: X times 2^4 sqrt(n), A and B times 2^8.
 //
 // A and A A are symmetric: only tiles on and above the diagonal are formed, and stored twice. Where they are few and long, X X^T is
@@ -46,6 +48,13 @@ constexpr float kGramScale = 0x1p8f;
 // Parts of a value that the products read: of a type and a smaller side m.
 constexpr int64_t kFewSingularValues = 64;
 inline int product_planes(int64_t dtype, int64_t m) { return dtype == kBFloat16 && m > kFewSingularValues ? 1 : 2; }
+
+// The step from which on all multiply pairs.
+constexpr int64_t kCoarseSteps = 4;
+inline int64_t pairs_from(const dllm_hip_orthogonalize_shape& sh) {
+    if (product_planes(sh.dtype, std::min(sh.rows, sh.cols)) == 2) return 0;
+    return sh.steps > kCoarseSteps + 1 ? kCoarseSteps : sh.steps;
+}
 
 using Half = _Float16;
 using Half8 = Half __attribute__((ext_vector_type(8)));
@@ -378,7 +387,8 @@ __device__ __forceinline__ void store_result(T* to, int64_t left, bool whole, co
     }
 }
 
-template <typename T, int kPl, typename Tile>
+// kTo: the new X's parts, of the products that read it next.
+template <typename T, int kPl, int kTo, typename Tile>
 __global__ __launch_bounds__(Tile::kThreads) void update_kernel(T* __restrict__ result, UpdateArgs a, int64_t m_tiles, int64_t n_tiles) {
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     if (block_id() >= m_tiles * n_tiles * a.s.batch) return;
@@ -391,6 +401,7 @@ __global__ __launch_bounds__(Tile::kThreads) void update_kernel(T* __restrict__ 
     const int64_t i0 = m * Tile::kM + Tile::wave_m(), j0 = n * Tile::kN + Tile::wave_n();
     T* const out = result + matrix * a.s.out_batch;
     const Places<kPl> places(a.s);
+    const Places<kTo> next(a.s);
     by_rows_and_columns<Tile>(
         acc, (LdsByte*)lds, !a.to && a.s.turned,
         [&](int row, int column) {
@@ -403,7 +414,7 @@ __global__ __launch_bounds__(Tile::kThreads) void update_kernel(T* __restrict__ 
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[e] = fmaf(a.keep, held_value(x, e), v[e] * a.factor);
             if (a.to)
-                store_pairs(a.to + places.at(a.s, matrix, i, j), places.rest, v);
+                store_pairs(a.to + next.at(a.s, matrix, i, j), next.rest, v);
             else if (!a.s.turned)
                 store_result(out + i * a.s.out_stride + j, a.s.n - j, a.whole, v);
         },
@@ -425,7 +436,7 @@ Matrices matrices_of(const dllm_hip_orthogonalize_shape& sh) {
     s.batch = sh.batch;
     s.turned = sh.rows > sh.cols;
     s.m = std::min(sh.rows, sh.cols), s.n = std::max(sh.rows, sh.cols);
-    const size_t multiple = product_planes(sh.dtype, s.m) == 1 ? kRowMultiple<1> : kRowMultiple<2>;
+    const size_t multiple = pairs_from(sh) == sh.steps && sh.steps > 0 ? kRowMultiple<1> : kRowMultiple<2>;
     s.m_padded = static_cast<int64_t>(round_up(s.m, multiple)), s.n_padded = static_cast<int64_t>(round_up(s.n, multiple));
     s.in_stride = sh.x_stride ? sh.x_stride : sh.cols;
     s.out_stride = sh.out_stride ? sh.out_stride : sh.cols;
@@ -460,7 +471,7 @@ struct UpdateLayout {
     UpdateLayout(const dllm_hip_orthogonalize_shape& sh, const Matrices& s) {
         norm = static_cast<size_t>(s.batch) * ceil_div(sh.rows, norm_rows(sh));
         planes = 2 * static_cast<size_t>(s.batch) * s.m * s.n_padded;
-        gram = static_cast<size_t>(product_planes(sh.dtype, s.m)) * s.batch * s.m * s.m_padded;
+        gram = static_cast<size_t>(pairs_from(sh) < sh.steps ? 2 : 1) * s.batch * s.m * s.m_padded;
         part = 0;
         for (const int64_t k : {s.n_padded, s.m})
             if (segments_at_once(s, k)) part = std::max(part, static_cast<size_t>(s.batch) * ceil_div(k, segment_of(s, k)) * s.m * s.m_padded);
@@ -503,13 +514,13 @@ void launch_gram(GramArgs g, float* part, hipStream_t stream) {
     }
 }
 
-template <typename T, int kPl, typename Tile>
+template <typename T, int kPl, int kTo, typename Tile>
 void launch_update(const UpdateArgs& u, T* out, hipStream_t stream) {
     const int64_t m = ceil_div(u.s.m, Tile::kM), n = ceil_div(u.s.n, Tile::kN);
-    update_kernel<T, kPl, Tile><<<grid_of(m * n * u.s.batch), Tile::kThreads, 0, stream>>>(out, u, m, n);
+    update_kernel<T, kPl, kTo, Tile><<<grid_of(m * n * u.s.batch), Tile::kThreads, 0, stream>>>(out, u, m, n);
 }
 
-template <typename T, int kPl>
+template <typename T, int kPl, int kTo>
 int launch_step(const Matrices& s, const UpdateBuffers& b, const double* c, int from, bool last, T* out, hipStream_t stream) {
     const int64_t row = s.n_padded * 2 * kPl, gram_row = s.m_padded * 2 * kPl;
     const Operand x{b.x[from], row, s.m * row, s.m};
@@ -529,13 +540,13 @@ int launch_step(const Matrices& s, const UpdateBuffers& b, const double* c, int 
     u.whole = length % 8 == 0 && s.out_stride % 8 == 0 && s.out_batch % 8 == 0 && aligned_to(out, 16);
     const int64_t large = ceil_div(s.m, 256) * ceil_div(s.n, 256) * s.batch, middle = ceil_div(s.m, 128) * ceil_div(s.n, 128) * s.batch;
     if (middle < 256 && ceil_div(s.m, 64) * ceil_div(s.n, 64) * s.batch <= 256)
-        launch_update<T, kPl, UpdateTile<kPl, 64, 8>>(u, out, stream);
+        launch_update<T, kPl, kTo, UpdateTile<kPl, 64, 8>>(u, out, stream);
     else if (middle < 256)
-        launch_update<T, kPl, UpdateTile<kPl, 64, 4>>(u, out, stream);
+        launch_update<T, kPl, kTo, UpdateTile<kPl, 64, 4>>(u, out, stream);
     else if (ceil_div(large, 256) * 2 <= ceil_div(middle, 512))
-        launch_update<T, kPl, UpdateTile<kPl, 256, 2>>(u, out, stream);
+        launch_update<T, kPl, kTo, UpdateTile<kPl, 256, 2>>(u, out, stream);
     else
-        launch_update<T, kPl, UpdateTile<kPl, 128, 2>>(u, out, stream);
+        launch_update<T, kPl, kTo, UpdateTile<kPl, 128, 2>>(u, out, stream);
     return check_launch("orthogonalize");
 }
 
@@ -562,7 +573,19 @@ int run_planes(const dllm_hip_orthogonalize_shape& sh, const Matrices& s, const 
     static constexpr double kQuintic[3] = {3.4445, -4.7750, 2.0315};
     for (int64_t i = 0; i < sh.steps; ++i) {
         const double* const c = coefficients ? coefficients + 3 * i : kQuintic;
-        DLLM_TRY((launch_step<T, kPl>(s, b, c, static_cast<int>(i % 2), i == sh.steps - 1, out, stream)));
+        const int from = static_cast<int>(i % 2);
+        const bool last = i == sh.steps - 1;
+        if constexpr (kPl == 1) {
+            if (i >= pairs_from(sh)) {
+                DLLM_TRY((launch_step<T, 2, 2>(s, b, c, from, last, out, stream)));
+                continue;
+            }
+            if (!last && i + 1 == pairs_from(sh)) {
+                DLLM_TRY((launch_step<T, 1, 2>(s, b, c, from, last, out, stream)));
+                continue;
+            }
+        }
+        DLLM_TRY((launch_step<T, kPl, kPl>(s, b, c, from, last, out, stream)));
     }
     return kOk;
 }

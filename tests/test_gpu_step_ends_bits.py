@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import ends_reference as R
-from test_gpu_step_ends import K, Loss, embed_backward, gen, randn, some_tokens  # noqa: F401
+from test_gpu_step_ends import K, Loss, embed_backward, gen, momentum, randn, some_tokens, update  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +152,34 @@ def test_loss_gradients_whose_parts_would_be_many(K, dtype):  # noqa: F811
         q = Loss(K, hidden[first:first + n].clone(), weight, targets[first:first + n].clone())
         q.lse.copy_(p.lse[first:first + n])
         assert torch.equal(q.backward(dloss[first:first + n].clone())[0], dhidden[first:first + n])
+
+
+# ---- orthogonalisation ----
+
+
+@pytest.mark.parametrize("steps", [6, 7, 8, 10])
+@pytest.mark.parametrize(("batch", "rows", "cols"), [(1, 256, 1024), (3, 576, 576), (2, 1000, 130), (1, 2050, 300)])
+def test_bfloat16_updates_of_many_steps(K, steps, batch, rows, cols):  # noqa: F811
+    """Singular values near one keep a product's error, so from the fifth step on the operands are pairs: what the kernel adds to the
+    result's own rounding (1.66e-3 in the 2-norm, as of any values) is at most 4.5e-4 of it, as the definition with float32's sums and
+    those operands has it, a factor of sqrt(1 + 0.27^2) = 1.04; the plain form in float32 is the measure."""
+    x = momentum(gen(90), batch, rows, cols, torch.bfloat16)
+    got = update(K, x, steps=steps, scale=0.7)
+    for i in range(batch):
+        value = R.orthogonalize(x[i], steps=steps, scale=0.7)
+        plain = R.steps_in_float32(x[i], steps=steps, scale=0.7).bfloat16()
+        off, of_plain = (float(torch.linalg.norm(t.double() - value)) for t in (got[i], plain))
+        assert off <= 1.05 * of_plain, (i, off / of_plain)
+        assert torch.equal(update(K, x[i:i + 1].clone(), steps=steps, scale=0.7)[0], got[i])
+
+
+def test_bfloat16_updates_of_many_steps_in_place_and_strided(K):  # noqa: F811
+    for m, n in ((100, 170), (170, 100)):
+        x = momentum(gen(91), 2, m, n, torch.bfloat16)
+        want = update(K, x, steps=7)
+        wide = torch.full((2, m + 3, n + 11), 5.0, dtype=x.dtype, device="cuda")
+        into = wide[:, 1:m + 1, 3:n + 3]
+        into.copy_(x)
+        assert torch.equal(update(K, into, steps=7, out=into), want)
+        into[:] = 5.0
+        assert bool((wide == 5.0).all())
