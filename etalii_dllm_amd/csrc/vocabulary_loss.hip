@@ -16,7 +16,9 @@
 // logit is formed where the rows are gathered, and goes into the sum as it is.
 //
 // Backward, a piece of the vocabulary at a time: the logits again, whose epilogue stores the softmax's part of g in the product's
-// type; then its products with the weights and with the hidden states. dh is added up in float32 over units of the vocabulary that
+// type; then its products with the weights and with the hidden states. (For that rounding dW's rows of tokens that are no target are off by
+// 1.3 to 1.4 times their own. Up to kPairedRows rows, whose products wait for the weights' bytes, have what it leaves too, as
+// further rows of the softmax, beside the hidden states once more: 37 rows, 151936 x 896, 265 to 286 us.) dh is added up in float32 over units of the vocabulary that
 // go by its size alone, whatever the batch, so a row's bits are its own. The target's element c = expm1(z - lse) ... stays out of the
 // 16-bit products: p - 1 is what is left of two near numbers where the model is sure, and with a uniform dloss its rounding would
 // not average out. c W[target] is added to dh in float32, and the sums of c h by target (token_rows.h) to dW in the epilogue.
@@ -69,6 +71,9 @@ template <typename T>
 constexpr bool kHalfParts = __is_same(LossPart<T>, _Float16);
 template <typename T>
 constexpr bool kScaled = sizeof(T) == 4;
+
+constexpr int64_t kPairedRows = 64;
+inline bool paired_rows(int64_t rows, int64_t dtype) { return rows <= kPairedRows && dtype != kFloat32; }
 
 // Bytes of a row of n values.
 template <typename T>
@@ -195,6 +200,7 @@ struct PackArgs {
     const uint32_t *list, *count;
     int64_t n, dim, stride, chunks, row;
     const int32_t *exponent, *largest, *sizes;
+    bool twice;  // the rows once more behind the last one
 };
 
 // Row list[j] (j itself without a list) of src as chunks of 8 values' parts.
@@ -202,7 +208,8 @@ template <typename T, bool kWhole, PackScale kScale>
 __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, char* __restrict__ dst, PackArgs a) {
     const int64_t i = block_id() * 256 + threadIdx.x;
     const int64_t j = i / a.chunks, c = i - j * a.chunks;
-    if (j >= (a.count ? static_cast<int64_t>(*a.count) : a.n)) return;
+    const int64_t n = a.count ? static_cast<int64_t>(*a.count) : a.n;
+    if (j >= n) return;
     float v[8];
     load_eight<T, kWhole>(src + (a.list ? static_cast<int64_t>(a.list[j]) : j) * a.stride, c * 8, a.dim, v);
     if constexpr (kScale == kAsTheyAre) return store_as_they_are(dst + j * a.row, c * 8, v);
@@ -218,6 +225,7 @@ __global__ __launch_bounds__(256) void pack_kernel(const T* __restrict__ src, ch
         for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], by);
     }
     store_parts<T>(dst + j * a.row, c * 8, v);
+    if (kScale == kWeightScale && a.twice) store_parts<T>(dst + (n + j) * a.row, c * 8, v);
 }
 
 template <typename T, PackScale kScale>
@@ -264,6 +272,7 @@ struct RowsArgs {
     LossShape s;
     uint32_t *list, *count;  // kFind: written here
     char* packed;
+    bool twice;  // packed: the rows once more behind the last one
     int32_t* row_exponent;  // float32: NULL: the values as they are
     // the forward's
     const int64_t* targets;
@@ -359,6 +368,7 @@ __global__ __launch_bounds__(kRowsThreads<kOf>) void rows_kernel(const T* __rest
             for (int e = 0; e < 8; ++e) v[e] = ldexpf(v[e], kTop - exponent);
         }
         store_parts<T>(a.packed + j * a.s.row, d, v);
+        if (kOf == kBackward && !kHalfParts<T> && a.twice) store_parts<T>(a.packed + (*a.count + j) * a.s.row, d, v);
     }
 #pragma unroll
     for (int s = 32; s > 0; s >>= 1) x += __shfl_xor(x, s);
@@ -582,13 +592,13 @@ struct SoftmaxArgs {
     int64_t first;  // of the piece, in the vocabulary
     const uint32_t* count;
     RowTerms terms;
-    char* out;  // [rows][piece] parts
+    char* out;  // [rows][piece] parts; kPaired: behind the last row what their rounding left, by the same rows
     int64_t out_stride;
     const int32_t* sizes;  // float32: of the piece, by kScaleRows
 };
 
 // The softmax's part of g, zero past the vocabulary's end and at the targets.
-template <typename T, bool kCapped, typename Tile>
+template <typename T, bool kCapped, bool kPaired, typename Tile>
 __global__ __launch_bounds__(Tile::kThreads) void softmax_kernel(SoftmaxArgs a, int64_t m_tiles, int64_t n_tiles) {
     __shared__ __attribute__((aligned(1024))) char lds[Tile::kLds];
     const int64_t count = *a.count;
@@ -621,9 +631,17 @@ __global__ __launch_bounds__(Tile::kThreads) void softmax_kernel(SoftmaxArgs a, 
             const float z = cap.logit<kCapped>(v[e], derivative);
             float p = __builtin_amdgcn_exp2f((z - of.lse) * kLog2E) * of.factor;
             if constexpr (kCapped) p *= derivative;
+            // float32's rounding first, in every kernel: a product that float16 alone takes would be rounded to that at once, and
+            // kPaired takes it in float32 too
+            if constexpr (__is_same(T, _Float16)) asm("" : "+v"(p));
             v[e] = e >= left || e == target ? 0.0f : p;
         }
         store_parts<T>(a.out + row * a.out_stride, column, v);
+        if constexpr (kPaired) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] -= static_cast<float>(static_cast<T>(v[e]));
+            store_parts<T>(a.out + (count + row) * a.out_stride, column, v);
+        }
     });
 }
 
@@ -715,12 +733,12 @@ __device__ __forceinline__ void hidden_tile(const GradientArgs& a, int64_t id, i
     }
 }
 
-template <typename T, typename Tile>
+template <typename T, bool kPaired, typename Tile>
 __device__ __forceinline__ void weight_tile(T* __restrict__ dweight, const GradientArgs& a, int64_t id, LdsByte* lds) {
     int64_t m, n;
     tile_of(id, a.weight_m_tiles, a.weight_n_tiles, m, n);
     typename Tile::Sums acc;
-    Tile::run(a.softmax, a.hidden, m * Tile::kM, n * Tile::kN, a.width, a.dim, *a.count, 0, 0, lds, acc);
+    Tile::run(a.softmax, a.hidden, m * Tile::kM, n * Tile::kN, a.width, a.dim, static_cast<int64_t>(*a.count) * (kPaired ? 2 : 1), 0, 0, lds, acc);
     const int64_t m0 = m * Tile::kM + Tile::wave_m(), n0 = n * Tile::kN + Tile::wave_n();
     const int by = kHalfParts<T> ? *a.largest - kExponentBase - kHalfShift - kTop : 0;
     struct Old {
@@ -769,7 +787,7 @@ __device__ __forceinline__ void weight_tile(T* __restrict__ dweight, const Gradi
     });
 }
 
-template <typename T, typename HiddenTile, typename WeightTile>
+template <typename T, bool kPaired, typename HiddenTile, typename WeightTile>
 __global__ __launch_bounds__(HiddenTile::kThreads) void gradient_kernel(T* __restrict__ dweight, GradientArgs a) {
     static_assert(HiddenTile::kThreads == WeightTile::kThreads);
     __shared__ __attribute__((aligned(1024))) char lds[HiddenTile::kLds > WeightTile::kLds ? HiddenTile::kLds : WeightTile::kLds];
@@ -778,7 +796,7 @@ __global__ __launch_bounds__(HiddenTile::kThreads) void gradient_kernel(T* __res
     if (id < hidden_tiles)
         hidden_tile<T, HiddenTile>(a, id, m_tiles, units, (LdsByte*)lds);
     else if (id < hidden_tiles + a.weight_m_tiles * a.weight_n_tiles)
-        weight_tile<T, WeightTile>(dweight, a, id - hidden_tiles, (LdsByte*)lds);
+        weight_tile<T, kPaired, WeightTile>(dweight, a, id - hidden_tiles, (LdsByte*)lds);
 }
 
 // total (+)= the units' parts, in their order, where there are parts
@@ -874,7 +892,8 @@ int64_t unit_of(const LossShape& s, int64_t dtype) {
 // Units of the backward's piece: as many as keep its softmax, and half of its packed weights, within kPieceBytes, at least one.
 int64_t piece_units(const LossShape& s, int64_t dtype) {
     const int64_t unit = unit_of(s, dtype);
-    const size_t bytes = static_cast<size_t>(std::max(s.rows, s.padded / 2)) * unit * 2 * planes_of(dtype);
+    const int64_t rows = paired_rows(s.rows, dtype) ? 2 * s.rows : s.rows;
+    const size_t bytes = static_cast<size_t>(std::max(rows, s.padded / 2)) * unit * 2 * planes_of(dtype);
     // float32's pieces are whole scales, so that those do not go by the rows either
     const int64_t together = dtype == kFloat32 ? kScaleRows / unit : 1, groups = static_cast<int64_t>(kPieceBytes / std::max<size_t>(bytes, 1)) / together;
     const int64_t all = static_cast<int64_t>(ceil_div(s.vocabulary, unit * together));
@@ -890,8 +909,9 @@ struct LossLayout {
         const size_t rows = static_cast<size_t>(s.rows), planes = planes_of(dtype), dim = static_cast<size_t>(s.dim);
         unit = unit_of(s, dtype), units = piece_units(s, dtype);
         const size_t piece = backward ? std::min<size_t>(units * unit, s.vocabulary) : std::min<size_t>(kPackPiece, s.vocabulary);
-        hidden = rows * s.row;
-        scaled = backward && dtype != kBFloat16 ? hidden : 0;
+        const size_t times = backward && paired_rows(s.rows, dtype) ? 2 : 1;
+        hidden = rows * s.row * (dtype == kBFloat16 ? times : 1);
+        scaled = backward && dtype != kBFloat16 ? rows * s.row * times : 0;
         weight = piece * s.row;
         list = backward ? 0 : rows;
         stats = backward ? 0 : ceil_div(s.vocabulary, kStatRows) * rows;
@@ -899,7 +919,7 @@ struct LossLayout {
         row_exponent = dtype == kFloat32 ? rows : 0;
         sizes = dtype == kFloat32 ? ceil_div(s.vocabulary, kScaleRows) : 0;
         terms = backward ? round_up(rows, 256) : 0;
-        softmax = backward ? rows * (units * unit + kStrideSlack) * planes : 0;
+        softmax = backward ? rows * (units * unit + kStrideSlack) * planes * times : 0;
         part = backward && units > 1 ? std::min<size_t>(units * rows * dim, kPartFloats) : 0;
         total = backward ? rows * dim : 0;
         sums = total;
@@ -1093,6 +1113,7 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
     using Logits = typename Tiles::Logits;
     using Hidden = typename Tiles::Hidden;
     using Weight = typename Tiles::Weight;
+    constexpr bool kPaired = std::is_same_v<Tiles, SmallTiles<T>> && !kScaled<T>;
     const int64_t piece = layout.units * layout.unit;
     for (int64_t first = 0; first < s.vocabulary; first += piece) {
         SoftmaxArgs a{};
@@ -1103,9 +1124,9 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
         a.out_stride = row_bytes<T>(piece + kStrideSlack);
         const int64_t width = a.weight.count, m = ceil_div(s.rows, Logits::kM), n = ceil_div(width, Logits::kN);
         if (s.softcap != 0.0f)
-            softmax_kernel<T, true, Logits><<<grid_of(m * n), Logits::kThreads, 0, stream>>>(a, m, n);
+            softmax_kernel<T, true, kPaired, Logits><<<grid_of(m * n), Logits::kThreads, 0, stream>>>(a, m, n);
         else
-            softmax_kernel<T, false, Logits><<<grid_of(m * n), Logits::kThreads, 0, stream>>>(a, m, n);
+            softmax_kernel<T, false, kPaired, Logits><<<grid_of(m * n), Logits::kThreads, 0, stream>>>(a, m, n);
         GradientArgs g{};
         g.softmax = Operand{b.softmax, a.out_stride, value_at<kLossPlanes<T>>(layout.unit), s.rows};
         g.weight = a.weight, g.weight.batch = layout.unit * a.weight.stride;
@@ -1128,7 +1149,7 @@ int run_pieces(const LossShape& s, const Buffers<T>& b, const LossLayout& layout
             g.sums = b.sums, g.at = b.at, g.largest = b.largest, g.accumulate = accumulate;
             g.whole = s.dim % 8 == 0 && aligned_to(dweight, 16);
         }
-        gradient_kernel<T, Hidden, Weight><<<grid_of(hidden_blocks + g.weight_m_tiles * g.weight_n_tiles), Hidden::kThreads, 0, stream>>>(dweight, g);
+        gradient_kernel<T, kPaired, Hidden, Weight><<<grid_of(hidden_blocks + g.weight_m_tiles * g.weight_n_tiles), Hidden::kThreads, 0, stream>>>(dweight, g);
         if (add_parts)
             add_parts_kernel<Hidden><<<static_cast<unsigned>(std::min<size_t>(ceil_div(s.rows * s.dim, 256), 4096)), 256, 0, stream>>>(
                 b.part, b.total, b.order.kept, s.dim, g.n_tiles, static_cast<int>(units), first == 0);
@@ -1145,12 +1166,12 @@ int run_backward(const LossShape& s, int64_t dtype, const T* hidden, const T* we
     DLLM_TRY(sort_tokens(targets, s.rows, s.vocabulary, b.order, b.largest, (1 + layout.sizes + (dweight ? layout.at : 0)) * 4, ~uint32_t{0}, stream));
     RowsArgs r = rows_args<T>(s, b);
     r.list = b.order.position, r.count = b.order.kept, r.order = b.order, r.lse = lse, r.dloss = dloss, r.terms = b.terms;
-    r.coefficient = b.coefficient, r.largest = b.largest;
+    r.coefficient = b.coefficient, r.largest = b.largest, r.twice = paired_rows(s.rows, dtype);
     DLLM_TRY((launch_rows<T, kBackward>(hidden, weight, r, stream)));
     if constexpr (kHalfParts<T>) {
         PackArgs p{};
         p.list = b.order.position, p.count = b.order.kept, p.n = s.rows, p.dim = s.dim, p.stride = s.hidden_stride;
-        p.exponent = b.terms.exponent, p.largest = b.largest;
+        p.exponent = b.terms.exponent, p.largest = b.largest, p.twice = paired_rows(s.rows, dtype);
         if (dweight) DLLM_TRY((launch_pack<T, kWeightScale>(hidden, b.scaled, p, stream)));
     }
     if (dweight) {
@@ -1163,7 +1184,7 @@ int run_backward(const LossShape& s, int64_t dtype, const T* hidden, const T* we
     const auto pieces = [&](auto tiles) {
         return run_pieces<T, decltype(tiles)>(s, b, layout, weight, dhidden != nullptr, dweight, accumulate, parts, stream);
     };
-    if (s.rows <= 64)
+    if (s.rows <= kPairedRows)
         DLLM_TRY(pieces(SmallTiles<T>{}));
     else if (large_tiles(s, layout))
         DLLM_TRY(pieces(LargeTiles<T>{}));

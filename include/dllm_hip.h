@@ -392,7 +392,8 @@ int dllm_hip_token_embedding_backward(const dllm_hip_token_embedding_shape* shap
  * The backward takes the forward's lse and the upstream gradients dloss (float32[rows]; the caller's weights, 1 / count for a mean) and
  * writes dhidden (zero where a row does not count) and dweight; either may be NULL. accumulate adds to what dweight holds, in
  * float32 before the one rounding. It forms the logits again, a piece of the vocabulary at a time. The softmax's part of a
- * gradient has the probabilities as operands in dtype, the target's part is float32's. float16 holds the probabilities times each
+ * gradient has the probabilities as operands in dtype (in dweight of up to 64 rows, with what that rounding left), the target's
+ * part is float32's. float16 holds the probabilities times each
  * row's dloss relative to it, so that gradients of any size keep their bits, and in dweight the hidden states times the power of two
  * of their dloss: both together are off by at most 2^-38 of the largest one times its dloss, so those below 2^-28 of it
  * lose bits. float32 has pairs of float16 as operands, 22 bits and more of each

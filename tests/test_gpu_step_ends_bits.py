@@ -76,6 +76,36 @@ def test_float16_gradients_of_unequal_rows(K):  # noqa: F811
     R.assert_within(got[1], want["dweight"], "dweight")
 
 
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+@pytest.mark.parametrize("softcap", [0.0, 4.0])
+@pytest.mark.parametrize(("rows", "vocabulary", "dim"), [(1, 5000, 96), (2, 300, 33), (37, 5000, 200), (64, 20001, 72)])
+def test_gradients_of_few_rows_for_tokens_that_are_no_target(K, dtype, softcap, rows, vocabulary, dim):  # noqa: F811
+    """dweight's rows that the softmax alone reaches are off by their own rounding, as from products in float32: what a pair leaves of
+    an operand is 2^-16 (bfloat16) or 2^-22 of it, and the factor below is for that and float32's sums."""
+    g, dt = gen(75), R.DTYPES[dtype]
+    weight, hidden = randn(g, vocabulary, dim, dtype=dt, scale=dim ** -0.5), randn(g, rows, dim, dtype=dt)
+    targets = torch.randint(0, vocabulary, (rows,), generator=g, device="cuda")
+    dloss = torch.exp2(4.0 * torch.rand(rows, generator=g, device="cuda")) * 100.0
+    if rows > 2:
+        targets[1] = -1
+    p = Loss(K, hidden, weight, targets, softcap=softcap)
+    _, lse = p.forward()
+    counts = targets >= 0
+    got = p.backward(dloss, want=(False, True))[1]
+    value = R.loss_backward(hidden, weight, targets, lse, dloss, softcap=softcap)["dweight"][0]
+    z = hidden.float() @ weight.float().T
+    slope = torch.ones_like(z)
+    if softcap:
+        z = softcap * torch.tanh(z / softcap)
+        slope = 1.0 - (z / softcap).square()
+    plain = ((torch.exp(z - lse[:, None]) * slope * (dloss * counts)[:, None]).T @ hidden.float()).to(dt)
+    others = torch.ones(vocabulary, dtype=torch.bool, device="cuda")
+    others[targets[counts]] = False
+    off, of_plain = (float(torch.linalg.norm((t.double() - value)[others])) for t in (got, plain))
+    assert off <= 1.02 * of_plain, off / of_plain
+    assert torch.equal(p.backward(dloss)[1], got)
+
+
 # ---- the table's gradient ----
 
 
