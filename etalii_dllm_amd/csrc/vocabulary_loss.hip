@@ -8,7 +8,9 @@
 //
 // Float32 values are multiplied as pairs of float16, three products: 22 bits and more of each value, off by 2^-39 of the largest
 // at most: hidden states are scaled by the power of two that brings their row's largest value to the top of float16's range,
-// weights by that of kScaleRows of them. (Three bfloat16 parts, six products, hold values of any size and take twice as long:
+// weights by that of kScaleRows of them. Probabilities, times 2^14, are off by 2^-39 at most whatever their size, which leaves those of 2^-17 their
+// 22 bits, those of 1e-8 12 and those below 2^-39 none: a power of two for each of the vocabulary, from its largest probability, would take the logits
+// twice. (Three bfloat16 parts, six products, hold values of any size and take twice as long:
 // gradients of 1020 rows, 49152 x 576, 1.6 ms.)
 //
 // Forward: tiles of logits on the matrix cores, vocabulary by rows, so that a lane owns a row of the batch; a tile leaves each

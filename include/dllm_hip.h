@@ -398,7 +398,9 @@ int dllm_hip_token_embedding_backward(const dllm_hip_token_embedding_shape* shap
  * of their dloss: both together are off by at most 2^-38 of the largest one times its dloss, so those below 2^-28 of it
  * lose bits. float32 has pairs of float16 as operands, 22 bits and more of each
  * value: hidden states off by at most 2^-39 of their row's largest value (in dweight, 2^-38 of the largest one times its dloss), weights
- * of 2048 rows' largest, so values far below those lose bits.
+ * of 2048 rows' largest, so values far below those lose bits. In both types a probability in the softmax's part is off by at most
+ * 2^-39 besides: in float32 one below 2^-17 has fewer than 22 bits (1e-8: 12, 1e-10: 6) and one below 2^-39 counts as zero, so dweight's
+ * rows of tokens that no row of the batch finds likelier than that are coarse or zero.
  * A row's loss, lse and dhidden are the same bits alone and in any batch (dhidden: from the same lse); float32's loss and lse are where
  * the batches have at most 256 rows, and where they have more: few rows are multiplied by the weights as they are. hidden_stride and dhidden_stride: elements between rows (0: dim).
  * Outputs do not overlap inputs. Limits: rows below 2^27, vocabulary below 2^31, their product below 2^48, dim at most 2^16, strides

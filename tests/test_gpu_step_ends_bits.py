@@ -76,6 +76,25 @@ def test_float16_gradients_of_unequal_rows(K):  # noqa: F811
     R.assert_within(got[1], want["dweight"], "dweight")
 
 
+def test_float32_gradients_of_unlikely_tokens(K):  # noqa: F811
+    """Probabilities from one half to 1e-13 in dweight's rows: off by 2^-39 as float16 pairs, and by what the logits' sums of 64 terms, 80 F of
+    at most 30, make of them."""
+    g = gen(76)
+    likely = torch.linspace(0.0, -30.0, 400, device="cuda")
+    weight = torch.zeros(400, 64, device="cuda")
+    weight[:, 0] = likely
+    hidden = randn(g, 100, 64)
+    hidden[:, 0] = 1.0
+    targets = torch.zeros(100, dtype=torch.int64, device="cuda")
+    p = Loss(K, hidden, weight, targets)
+    dloss = torch.full((100,), 0.01, device="cuda")
+    p.check(dloss)
+    value = R.loss_backward(hidden, weight, targets, p.lse, dloss)["dweight"][0][1:, 0]  # of hidden states of one
+    off = (p.backward(dloss)[1][1:, 0].double() / value - 1).abs()
+    assert float(value.max()) > 0.05 and float(value.min()) < 1e-13
+    assert bool((off <= 1.01 * 2.0 ** -39 / value + 80 * R.F * 30 + 1e-5).all())
+
+
 @pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
 @pytest.mark.parametrize("softcap", [0.0, 4.0])
 @pytest.mark.parametrize(("rows", "vocabulary", "dim"), [(1, 5000, 96), (2, 300, 33), (37, 5000, 200), (64, 20001, 72)])
