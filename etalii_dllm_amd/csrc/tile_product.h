@@ -49,7 +49,7 @@ constexpr int kSecond = 64;
 template <int kPlanes>
 constexpr int kRowMultiple = kPlanes == 1 ? 8 : 32;
 
-// 8 values, from one that is a multiple of 8 in its row on, as parts of type P.
+// 8 values, from one that is a multiple of 8 in its row on, as parts of type P. (A pair of an infinity is that and NaN, so products are NaN.)
 template <typename P, int kPlanes>
 __device__ __forceinline__ void store_eight(char* to, const float (&v)[8]) {
     using V = P __attribute__((ext_vector_type(8)));

@@ -401,6 +401,8 @@ int dllm_hip_token_embedding_backward(const dllm_hip_token_embedding_shape* shap
  * of 2048 rows' largest, so values far below those lose bits. In both types a probability in the softmax's part is off by at most
  * 2^-39 besides: in float32 one below 2^-17 has fewer than 22 bits (1e-8: 12, 1e-10: 6) and one below 2^-39 counts as zero, so dweight's
  * rows of tokens that no row of the batch finds likelier than that are coarse or zero.
+ * NaN and infinities of a counted row's hidden state, or of weights, are what arithmetic makes of them, but for float32's pairs (all gradients,
+ * and losses of more than 256 rows), where an infinity is NaN: it makes NaN of the row's results, or of all rows'.
  * A row's loss, lse and dhidden are the same bits alone and in any batch (dhidden: from the same lse); float32's loss and lse are where
  * the batches have at most 256 rows, and where they have more: few rows are multiplied by the weights as they are. hidden_stride and dhidden_stride: elements between rows (0: dim).
  * Outputs do not overlap inputs. Limits: rows below 2^27, vocabulary below 2^31, their product below 2^48, dim at most 2^16, strides

@@ -125,6 +125,34 @@ def test_gradients_of_few_rows_for_tokens_that_are_no_target(K, dtype, softcap, 
     assert torch.equal(p.backward(dloss)[1], got)
 
 
+@pytest.mark.parametrize("value", [math.inf, -math.inf])
+@pytest.mark.parametrize("rows", [5, 300])
+@pytest.mark.parametrize("dtype", R.DTYPES)
+def test_loss_of_infinities(K, dtype, rows, value):  # noqa: F811
+    """An infinite weight: rows that it gives a logit of minus infinity have their loss without it, others none, and in float32's
+    pairs no row has one. An infinite hidden state is its row's own."""
+    g, dt = gen(77), R.DTYPES[dtype]
+    weight, hidden = randn(g, 500, 40, dtype=dt), randn(g, rows, 40, dtype=dt)
+    targets = torch.randint(0, 77, (rows,), generator=g, device="cuda")
+    dloss = torch.full((rows,), 0.1, device="cuda")
+    weight[400, 7] = value
+    p = Loss(K, hidden, weight, targets)
+    loss, lse = p.forward()
+    pairs = dtype == "float32" and rows > 256
+    gone = (hidden[:, 7].float() * value < 0) & (not pairs)
+    assert not bool(torch.isfinite(loss[~gone]).any()) and not bool(torch.isfinite(lse[~gone]).any())
+    want = R.loss(hidden[gone], torch.cat([weight[:400], weight[401:]]), targets[gone])
+    R.assert_within(loss[gone], want["loss"], "loss")
+    R.assert_within(lse[gone], want["lse"], "lse")
+    weight[400], hidden[3, 5] = 0.25, value
+    p = Loss(K, hidden, weight, targets)
+    got = [t.clone() for t in p.forward()]
+    dhidden = p.backward(dloss)[0]
+    others = torch.arange(rows, device="cuda") != 3
+    assert not bool(torch.isfinite(got[0][3])) and bool(dhidden[3].isnan().all())
+    assert bool(torch.isfinite(got[0][others]).all()) and bool(torch.isfinite(dhidden[others]).all())
+
+
 # ---- the table's gradient ----
 
 
