@@ -9,7 +9,7 @@ import pytest
 import torch
 
 import ends_reference as R
-from test_gpu_step_ends import K, Loss, embed_backward, gen, momentum, randn, some_tokens, update  # noqa: F401
+from test_gpu_step_ends import K, Loss, Step, embed_backward, gen, momentum, randn, some_tokens, update  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -260,3 +260,69 @@ def test_bfloat16_updates_of_many_steps_in_place_and_strided(K):  # noqa: F811
         assert torch.equal(update(K, into, steps=7, out=into), want)
         into[:] = 5.0
         assert bool((wide == 5.0).all())
+
+
+def element_limits(x, **options):
+    """(value, how far one element may be, how far a row, how far a column, in the 2-norm) as orthogonalize_limits has it for the whole:
+    the definition with the operands rounded as they are stated to be is off by so much at most in any element (row, column), and the
+    kernel, whose errors are of that kind and as many, may be twice as far; float32's sums too; the result's rounding is added."""
+    value = R.orthogonalize(x, **options)
+    coarse = x.dtype == torch.bfloat16 and min(x.shape) > 64 and options.get("steps", 5) <= 5
+    errors = [R.orthogonalize(x, rounding=R.halves(1 if coarse else 2), **options) - value, R.steps_in_float32(x, **options).double() - value]
+    u = R.unit(x.dtype)
+    one, row, column = (sum(2 * f(e) for e in errors) for f in (
+        lambda e: e.abs().max(), lambda e: e.norm(dim=1).max(), lambda e: e.norm(dim=0).max()))
+    return (value, one + 2 * u * value.abs() + R.tiny(x.dtype), row + 2 * u * value.norm(dim=1), column + 2 * u * value.norm(dim=0))
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize(("batch", "rows", "cols"), [(1, 1, 9), (2, 7, 3), (2, 33, 31), (3, 65, 130), (1, 129, 257), (3, 100, 24), (1, 70, 4200), (65, 2100, 257),
+                                                     (1, 1500, 8900), (2, 300, 1001)])
+def test_every_element_of_an_update(K, dtype, batch, rows, cols):  # noqa: F811
+    """The largest error of an element, and of a row and a column by itself: at the tiles' edges and remainders too."""
+    x = momentum(gen(92), batch, rows, cols, R.DTYPES[dtype])
+    got = update(K, x, steps=4)
+    for i in sorted({0, batch - 1}):
+        value, one, row, column = element_limits(x[i], steps=4)
+        off = got[i].double() - value
+        assert bool((off.abs() <= one).all()), (i, torch.nonzero(off.abs() > one)[0].tolist())
+        assert bool((off.norm(dim=1) <= row).all()), (i, torch.nonzero(off.norm(dim=1) > row)[0].tolist())
+        assert bool((off.norm(dim=0) <= column).all()), (i, torch.nonzero(off.norm(dim=0) > column)[0].tolist())
+
+
+# ---- together ----
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16"])
+def test_a_step_with_its_roundings(K, dtype):  # noqa: F811
+    """The whole step in 16 bits, within twice of what the same step in 64 bits is off by with its results rounded to the type on the
+    way (each rounding is one of as many, of random sign), and the last rounding."""
+    dt = R.DTYPES[dtype]
+    s = Step(K, 42, dt)
+    got, want = s.step(), s.reference()
+
+    def rounded(t):
+        return t + (t.detach().to(dt).double() - t.detach())
+
+    def rounding(t):
+        t.register_hook(lambda g: g.to(dt).double())
+        return t
+
+    proj, norm = (t.double().requires_grad_() for t in (s.proj, s.norm))
+    ends = [s.table.double().requires_grad_() for _ in range(2)]  # the table's two parts
+    x = rounding(rounded(s.scale * ends[0][s.tokens.clamp(min=0)] * (s.tokens >= 0)[:, None]))
+    h = rounding(rounded(x + rounded(x @ proj)))
+    n = rounding(rounded(h / torch.sqrt(h.square().mean(dim=1, keepdim=True) + 1e-5) * norm))
+    logits = n @ ends[1].T
+    counts, at = s.targets >= 0, s.targets.clamp(min=0)[:, None]
+    hot = torch.zeros_like(logits, dtype=torch.bool).scatter_(1, at, True)
+    # the softmax's part is an operand in the type, relative to its row; the target's is not
+    logits.register_hook(lambda g: torch.where(hot, g, (g * 2.0 ** 20).to(dt).double() / 2.0 ** 20))
+    z = 20.0 * torch.tanh(logits / 20.0)
+    loss = (torch.logsumexp(z, dim=1) - z.gather(1, at)[:, 0]) * counts
+    first, last, dnorm, dproj = torch.autograd.grad((loss * s.dloss.double()).sum(), [*ends, norm, proj])
+    close = dict(loss=loss, dtable=(last.to(dt).double() + first).to(dt).double(), dnorm=dnorm, dproj=dproj.to(dt).double())
+    for name, value in want.items():
+        value = value.detach()
+        off, limit = (float((t.detach().double() - value).norm() / value.norm()) for t in (got[name], close[name]))
+        assert off <= 2 * limit + R.unit(dt), (name, off, limit)
