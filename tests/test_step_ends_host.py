@@ -4,6 +4,7 @@ tests compare with against differences."""
 from __future__ import annotations
 
 import math
+import shutil
 from pathlib import Path
 
 import numpy as np
@@ -11,6 +12,7 @@ import pytest
 import torch
 
 import ends_reference as R
+import test_dpp_hazards as H
 
 LIBRARY = Path(__file__).resolve().parents[1] / "etalii_dllm_amd" / "libdllm_hip.so"
 needs_library = pytest.mark.skipif(not LIBRARY.exists(), reason="libdllm_hip.so not built")
@@ -240,3 +242,14 @@ def test_loss_workspace_is_what_is_said_of_it(K, dtype, rows, vocabulary, dim):
     weight = max(2 ** 29, unit * padded * size)
     others = rows * padded * (2 * size + 4 + 4 + 1) + 8 * padded + rows * 64 + 5 * vocabulary + 2 ** 23
     assert 0 < need <= softmax + weight + 3 * 2 ** 27 + others, need
+
+
+@pytest.mark.skipif(not Path(H.B.HIPCC).exists() and shutil.which("hipcc") is None, reason="hipcc not available")
+@pytest.mark.parametrize("source", ["vocabulary_loss.hip", "orthogonalize.hip"])
+def test_tiled_products_copies_respect_their_wait_states(tmp_path, source):
+    """The tiled products' copies to LDS are inline statements whose base is in scalar registers."""
+    asm = H._device_asm(tmp_path, source)
+    copies = asm.count("global_load_lds_dwordx4")
+    checked, bad = H.sgpr_base_hazards(asm)
+    assert not bad, f"{len(bad)} SGPR-base hazards, e.g. {bad[:3]}"
+    assert checked >= copies // 2 > 0
