@@ -136,7 +136,8 @@ __global__ __launch_bounds__(kThreads) void start_kernel(const T* __restrict__ x
     for (int64_t p = threadIdx.x; p < parts; p += kThreads) squares += part[matrix * parts + p];
     const double norm = sqrt(add_over_threads(squares)) + s.eps;
     // the quotient's rounding is of X as a whole, which the steps forgive; a norm below float32's range, or above it, is not
-    const double inverse = 1.0 / norm;
+    // (zeroes beside an eps whose inverse is none are zeroes)
+    const double inverse = norm > 0.0 ? fmin(1.0 / norm, 0x1p1023) : NAN;
     const T* const from = x + matrix * s.in_batch;
     // rows and columns of x
     const int64_t r0 = s.turned ? j0 : i0, c0 = s.turned ? i0 : j0, rows = s.turned ? s.n : s.m, cols = s.turned ? s.m : s.n;

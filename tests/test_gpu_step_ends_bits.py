@@ -262,6 +262,19 @@ def test_bfloat16_updates_of_many_steps_in_place_and_strided(K):  # noqa: F811
         assert bool((wide == 5.0).all())
 
 
+@pytest.mark.parametrize("dtype", R.DTYPES)
+def test_updates_of_zeroes(K, dtype):  # noqa: F811
+    """Zeroes beside any eps; NaN, alone in its batch, without one."""
+    x = momentum(gen(93), 2, 20, 70, R.DTYPES[dtype])
+    want = update(K, x, eps=0.0)
+    x[0] = 0
+    for eps in (1e-7, 1e-300, 1e-320):
+        assert bool((update(K, x, eps=eps)[0] == 0).all()), eps
+    got = update(K, x, eps=0.0)
+    assert bool(got[0].isnan().all()) and torch.equal(got[1], want[1])
+    assert torch.equal(update(K, x, eps=1e-320)[1], want[1])
+
+
 def element_limits(x, **options):
     """(value, how far one element may be, how far a row, how far a column, in the 2-norm) as orthogonalize_limits has it for the whole:
     the definition with the operands rounded as they are stated to be is off by so much at most in any element (row, column), and the
