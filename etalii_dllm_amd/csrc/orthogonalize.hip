@@ -9,12 +9,16 @@
 // small singular values is far smaller than a X.
 //
 // The products' operands are float16 (bfloat16's 8 bits would cost results two of theirs): one part of 11 bits for bfloat16 updates,
-// whose own 8 bits are coarser than what that adds (of the result, by its 2-norm: 5e-4 after five steps, where
-// rounding it once is 1.7e-3), pairs of 22 bits, three products, for float32 and float16 ones, and for small matrices, whose few
-// singular values average no rounding out (2 x 76: 2.5e-3 with one part). From the fifth step on singular values are near one, the term is
-// as large as a X, and its error stays: calls of more than five steps multiply pairs from there on (256 x 1024, six steps: off by 1.3e-3 before the result's
-// rounding with one part, 1e-4 so; ten steps 3.4e-3 and 2e-4), at 1.9 times the time of such a step (24 of 896 x 4864, six steps: 3.33 to 4.28 ms). All values are bounded by the singular values, which stay near one, so fixed
-// powers of two keep them in float16's range: X times 2^4 sqrt(n), A and B times 2^8.
+// whose own 8 bits are coarser than what that adds: after five steps results are off by 1.00 (896 x 4864) to 1.2 times (70 x 500) what their
+// rounding alone is, 1.7e-3 in the 2-norm, where a few directions are strong as in a momentum; by 1.4 to 1.5 times where all
+// singular values are alike, which then are near one two steps earlier. Pairs of 22 bits, three products, for float32 and float16 ones, and for small
+// matrices, whose few singular values average no rounding out (2 x 76: 2.5e-3 with one part). With singular values near one the term is as
+// large as a X, and its error stays: calls of more than five steps multiply pairs from the fifth on (256 x 1024, six steps: 1.3 times with one
+// part, 1.00 so; ten steps 2.3 and 1.01), at 1.9 times the time of such a step (24 of 896 x 4864, six steps: 3.33 to 4.28 ms; from the third step on
+// singular values that are all alike would have 1.00 too, instead of 1.4 to 1.6, for another 1 ms).
+//
+// All values are bounded by the singular values, which stay near one, so fixed powers of two keep them in float16's range: X times
+// 2^4 sqrt(n), A and B times 2^8.
 //
 // A and A A are symmetric: only tiles on and above the diagonal are formed, and stored twice. Where they are few and long, X X^T is
 // formed in segments of its n columns at once, whose sums a launch of its own adds in order; where there are matrices enough, a
@@ -428,7 +432,7 @@ __global__ __launch_bounds__(Tile::kThreads) void update_kernel(T* __restrict__ 
 // ---- the call ----
 
 template <int kPl, int kSize, int kStages>
-using GramTile = TileProduct<Half, kPl, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, false, kStages>;
+using GramTile = TileProduct<Half, kPl, kSize, kSize, 2, 2, false, false, kStages>;
 template <int kPl, int kSize, int kStages>
 using UpdateTile = TileProduct<Half, kPl, kSize, kSize, 2, kSize == 256 ? 4 : 2, false, true, kStages>;
 

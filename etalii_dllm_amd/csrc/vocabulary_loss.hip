@@ -423,7 +423,8 @@ int launch_rows(const T* hidden, const T* weight, const RowsArgs& a, hipStream_t
 
 // The products' tiles by the number of rows. 256 x 256 by eight waves, one workgroup to a CU; 128 x 128 by four, two to a CU, where
 // the large ones would leave CUs without work or pad much; and for up to 64 rows, whose products wait for the weights'
-// bytes, tiles of 64 rows. The forward's waves hold kStatRows of the vocabulary in all of them.
+// bytes, tiles of 64 rows. The forward's waves hold kStatRows of the vocabulary in all of them. (The gradients' large tiles of float32 spill
+// three registers, outside their loop over k.)
 //
 // Float32's forward of up to kFewRows rows multiplies the values as they are (DirectTile): packing the weights reads them
 // twice and stores them, which takes as long as the float32 products of some 250 rows (3 rows, 151936 x 1536: 257 us instead of 1240).
@@ -1096,7 +1097,7 @@ int run_forward(const LossShape& s, int64_t dtype, const T* hidden, const T* wei
 }
 
 // Whether 256 x 256 tiles take less time for a piece's products than 128 x 128 ones: a large tile takes as long as four small ones at
-// two to a CU would, or a little less, so rounds and padding decide.
+// two to a CU would, or a little less, so rounds and padding decide. It goes by all rows: how many count is not known here.
 bool large_tiles(const LossShape& s, const LossLayout& l) {
     const auto time = [&](int64_t size, int64_t slots, double round) {
         const int64_t width = std::min(l.units * l.unit, s.vocabulary);

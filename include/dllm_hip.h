@@ -429,7 +429,8 @@ int dllm_hip_vocabulary_loss_backward(const dllm_hip_vocabulary_loss_shape* shap
  * (on the transposed matrix where rows exceed cols, which is the same and smaller), and out = scale * X. coefficients: HOST, a, b
  * and c of each step; NULL: 3.4445, -4.7750, 2.0315 in all of them, which bring the singular values near one in about five
  * steps. X is held as pairs of float16, 22 bits; the products of bfloat16 updates with more than 64 singular values read float16
- * in calls of up to five steps and in the first four of more, all others such pairs. Singular values have to stay where float16 holds all three: X below 15, A and b A + c A A below 255
+ * in calls of up to five steps and in the first four of more, all others such pairs. (A bfloat16 result is off by 1.0 to 1.2 times what its
+ * rounding alone is, by the 2-norm, and by 1.6 at most where all singular values are alike.) Singular values have to stay where float16 holds all three: X below 15, A and b A + c A A below 255
  * (the default coefficients keep X below 1.3); others give infinities. Zeroes stay zeroes, without an eps they give NaN. Strides in elements between rows and between matrices (0: packed). out may be x with the same strides;
  * otherwise they do not overlap. Limits: rows and cols at most 2^16, batch at most 65535, batch * rows * cols below
  * 2^40, strides below 2^32 between rows and 2^47 between matrices, steps in [0, 64], eps at least 0, scale and coefficients
