@@ -440,7 +440,7 @@ struct LargeTiles {
 };
 template <typename T>
 struct MiddleTiles {
-    using Forward = Product64<T, false, false, 256, 128, 2, 4>;
+    using Forward = Product64<T, false, false, 256, 128, 2, 4>;  // of 16-bit types, as SmallTiles'
     using Logits = Product64<T, false, false, 128, 128, 2, 2>;
     using Hidden = Product64<T, false, true, 128, 128, 2, 2>;
     using Weight = Product64<T, true, true, 128, 128, 2, 2>;

@@ -9,7 +9,8 @@ import pytest
 import torch
 
 import ends_reference as R
-from test_gpu_step_ends import K, Loss, Step, embed_backward, gen, momentum, randn, some_tokens, update  # noqa: F401
+from test_gpu_step_ends import (  # noqa: F401
+    K, Loss, Step, embed_backward, gen, loss_problem, momentum, moved, ptr, randn, some_tokens, stream, update)
 
 pytestmark = pytest.mark.gpu
 
@@ -123,6 +124,25 @@ def test_gradients_of_few_rows_for_tokens_that_are_no_target(K, dtype, softcap, 
     off, of_plain = (float(torch.linalg.norm((t.double() - value)[others])) for t in (got, plain))
     assert off <= 1.02 * of_plain, off / of_plain
     assert torch.equal(p.backward(dloss)[1], got)
+
+
+@pytest.mark.parametrize("dtype", R.DTYPES)
+@pytest.mark.parametrize(("rows", "dim"), [(64, 8), (33, 5)])
+def test_gradients_of_few_rows_in_pieces(K, dtype, rows, dim):  # noqa: F811
+    """So large a vocabulary that few rows go over it in pieces, added to what dweight holds; rows that do not count, and one alone; dweight
+    that is not aligned."""
+    p, dloss = loss_problem(K, 78, R.DTYPES[dtype], rows, 2200000, dim, masked=0.2)
+    old = randn(gen(79), 2200000, dim, dtype=R.DTYPES[dtype], scale=1e-3)
+    p.check(dloss, old)
+    dhidden, dweight = (t.clone() for t in p.backward(dloss, old))
+    q = Loss(K, p.hidden[9:10].clone(), p.weight, p.targets[9:10].clone())
+    q.lse.copy_(p.lse[9:10])
+    assert torch.equal(q.backward(dloss[9:10].clone())[0], dhidden[9:10])
+    p.shape.accumulate = 1
+    into = moved(old)
+    K.check(K.lib.dllm_hip_vocabulary_loss_backward(p.shape, *map(ptr, (p.hidden, p.weight, p.targets, p.lse, dloss)), None, ptr(into), ptr(p.workspace),
+                                                    p.workspace.numel(), stream()))
+    assert torch.equal(into, dweight)
 
 
 @pytest.mark.parametrize("value", [math.inf, -math.inf])
