@@ -8,14 +8,15 @@
 // the products of 16-bit updates read is its first part: an error of theirs is relative to the term b A X + c A A X, which for
 // small singular values is far smaller than a X.
 //
-// The products' operands are float16 (bfloat16's 8 bits would cost results two of theirs): one part of 11 bits for bfloat16 updates,
-// whose own 8 bits are coarser than what that adds: after five steps results are off by 1.00 (896 x 4864) to 1.2 times (70 x 500) what their
-// rounding alone is, 1.7e-3 in the 2-norm, where a few directions are strong as in a momentum; by 1.4 to 1.5 times where all
-// singular values are alike, which then are near one two steps earlier. Pairs of 22 bits, three products, for float32 and float16 ones, and for small
-// matrices, whose few singular values average no rounding out (2 x 76: 2.5e-3 with one part). With singular values near one the term is as
-// large as a X, and its error stays: calls of more than five steps multiply pairs from the fifth on (256 x 1024, six steps: 1.3 times with one
-// part, 1.00 so; ten steps 2.3 and 1.01), at 1.9 times the time of such a step (24 of 896 x 4864, six steps: 3.33 to 4.28 ms; from the third step on
-// singular values that are all alike would have 1.00 too, instead of 1.4 to 1.6, for another 1 ms).
+// The products' operands are float16 (bfloat16's 8 bits would cost results two of theirs): one part of 11 bits for bfloat16
+// updates, whose own 8 bits are coarser than what that adds: after five steps results are off by 1.00 (896 x 4864) to 1.2 times (70
+// x 500) what their rounding alone is, 1.7e-3 in the 2-norm, where a few directions are strong as in a momentum; by 1.4 to 1.5
+// times where all singular values are alike, which then are near one two steps earlier. Pairs of 22 bits, three products, for
+// float32 and float16 ones, and for small matrices, whose few singular values average no rounding out (2 x 76: 2.5e-3 with one
+// part). With singular values near one the term is as large as a X, and its error stays: calls of more than five steps multiply
+// pairs from the fifth on (256 x 1024, six steps: 1.3 times with one part, 1.00 so; ten steps 2.3 and 1.01), at 1.9 times the time
+// of such a step (24 of 896 x 4864, six steps: 3.33 to 4.28 ms; from the third step on singular values that are all alike would
+// have 1.00 too, instead of 1.4 to 1.6 and 2.1 after ten steps, for another 1 ms).
 //
 // All values are bounded by the singular values, which stay near one, so fixed powers of two keep them in float16's range: X times
 // 2^4 sqrt(n), A and B times 2^8.

@@ -7,10 +7,11 @@
 // over all of them took 39 us; more go through memory, each pass three launches.
 //
 // Sums: a token's positions are added 8 at a time from its first one on, whatever tokens lie beside it, so a row of the sums is the
-// same bits in any batch that has its positions. A wave takes the groups of 8 that begin among 8 sorted positions, and
-// 16 bytes of columns to a lane; it reads all their rows (up to 15) at once and adds them in order. A token of at most 8 is done; the
-// groups of others are float32 parts, added in their order by a second launch. Nothing depends on when a wave runs. 16381 rows of 576 in float32 onto a table that is added to: sort 22 us, sums 14
-// (2.7 TB/s of rows read), parts 9, a chain of additions as long as the most frequent token's; 16 positions to a wave were no faster.
+// same bits in any batch that has its positions. A wave takes the groups of 8 that begin among 8 sorted positions, and 16 bytes of
+// columns to a lane; it reads all their rows (up to 15) at once and adds them in order. A token of at most 8 is done; the groups of
+// others are float32 parts, added in their order by a second launch. Nothing depends on when a wave runs. 16381 rows of 576 in
+// float32 onto a table that is added to: sort 22 us, sums 14 (2.7 TB/s of rows read), parts 9, a chain of additions as long as the
+// most frequent token's; 16 positions to a wave were no faster.
 #include "token_rows.h"
 
 #include <algorithm>

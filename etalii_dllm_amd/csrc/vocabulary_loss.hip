@@ -6,11 +6,11 @@
 // Only rows that count (a target inside the vocabulary) are worked on: they are listed first, and their hidden states gathered
 // into whole 16-byte chunks, zeroes behind.
 //
-// Float32 values are multiplied as pairs of float16, three products: 22 bits and more of each value, off by 2^-39 of the largest
-// at most: hidden states are scaled by the power of two that brings their row's largest value to the top of float16's range,
-// weights by that of kScaleRows of them. Probabilities, times 2^14, are off by 2^-39 at most whatever their size, which leaves those of 2^-17 their
-// 22 bits, those of 1e-8 12 and those below 2^-39 none: a power of two for each of the vocabulary, from its largest probability, would take the logits
-// twice. (Three bfloat16 parts, six products, hold values of any size and take twice as long:
+// Float32 values are multiplied as pairs of float16, three products: 22 bits and more of each value, off by 2^-39 of the largest at
+// most: hidden states are scaled by the power of two that brings their row's largest value to the top of float16's range, weights
+// by that of kScaleRows of them. Probabilities, times 2^14, are off by 2^-39 at most whatever their size, which leaves those of
+// 2^-17 their 22 bits, those of 1e-8 12 and those below 2^-39 none: a power of two for each of the vocabulary, from its largest
+// probability, would take the logits twice. (Three bfloat16 parts, six products, hold values of any size and take twice as long:
 // gradients of 1020 rows, 49152 x 576, 1.6 ms.)
 //
 // Forward: tiles of logits on the matrix cores, vocabulary by rows, so that a lane owns a row of the batch; a tile leaves each
@@ -18,12 +18,13 @@
 // logit is formed where the rows are gathered, and goes into the sum as it is.
 //
 // Backward, a piece of the vocabulary at a time: the logits again, whose epilogue stores the softmax's part of g in the product's
-// type; then its products with the weights and with the hidden states. (For that rounding dW's rows of tokens that are no target are off by
-// 1.3 to 1.4 times their own. Up to kPairedRows rows, whose products wait for the weights' bytes, have what it leaves too, as
-// further rows of the softmax, beside the hidden states once more: 37 rows, 151936 x 896, 265 to 286 us.) dh is added up in float32 over units of the vocabulary that
-// go by its size alone, whatever the batch, so a row's bits are its own. The target's element c = expm1(z - lse) ... stays out of the
-// 16-bit products: p - 1 is what is left of two near numbers where the model is sure, and with a uniform dloss its rounding would
-// not average out. c W[target] is added to dh in float32, and the sums of c h by target (token_rows.h) to dW in the epilogue.
+// type; then its products with the weights and with the hidden states. (For that rounding dW's rows of tokens that are no target
+// are off by 1.3 to 1.4 times their own. Up to kPairedRows rows, whose products wait for the weights' bytes, have what it leaves
+// too, as further rows of the softmax, beside the hidden states once more: 37 rows, 151936 x 896, 265 to 286 us.) dh is added up in
+// float32 over units of the vocabulary that go by its size alone, whatever the batch, so a row's bits are its own. The target's
+// element c = expm1(z - lse) ... stays out of the 16-bit products: p - 1 is what is left of two near numbers where the model is
+// sure, and with a uniform dloss its rounding would not average out. c W[target] is added to dh in float32, and the sums of c h by
+// target (token_rows.h) to dW in the epilogue.
 //
 // Bound and measured. 8192 rows, 151936 x 1536 in bfloat16, forward 3.5 ms: 1090 TFLOP/s, matrix cores 52% busy at 1.7 GHz, to which
 // power lowers the clock; gradients 11.5 ms: the logits again and their epilogue 0.43 ms for 16384 of the vocabulary (890

@@ -389,20 +389,20 @@ int dllm_hip_token_embedding_backward(const dllm_hip_token_embedding_shape* shap
  *     lse[t] = log sum over v of exp z[t, v],   loss[t] = lse[t] - z[t, targets[t]]   (float32[rows] each).
  * A row whose target is outside the vocabulary (a prompt's, padding) does not count: its loss and lse are 0, and whatever its
  * hidden state holds reaches nothing. loss is minus the target's log-probability. Either of loss and lse may be NULL.
- * The backward takes the forward's lse and the upstream gradients dloss (float32[rows]; the caller's weights, 1 / count for a mean) and
- * writes dhidden (zero where a row does not count) and dweight; either may be NULL. accumulate adds to what dweight holds, in
- * float32 before the one rounding. It forms the logits again, a piece of the vocabulary at a time. The softmax's part of a
- * gradient has the probabilities as operands in dtype (in dweight of up to 64 rows, with what that rounding left), the target's
- * part is float32's. float16 holds the probabilities times each
- * row's dloss relative to it, so that gradients of any size keep their bits, and in dweight the hidden states times the power of two
- * of their dloss: both together are off by at most 2^-38 of the largest one times its dloss, so those below 2^-28 of it
- * lose bits. float32 has pairs of float16 as operands, 22 bits and more of each
- * value: hidden states off by at most 2^-39 of their row's largest value (in dweight, 2^-38 of the largest one times its dloss), weights
- * of 2048 rows' largest, so values far below those lose bits. In both types a probability in the softmax's part is off by at most
- * 2^-39 besides: in float32 one below 2^-17 has fewer than 22 bits (1e-8: 12, 1e-10: 6) and one below 2^-39 counts as zero, so dweight's
- * rows of tokens that no row of the batch finds likelier than that are coarse or zero.
- * NaN and infinities of a counted row's hidden state, or of weights, are what arithmetic makes of them, but for float32's pairs (all gradients,
- * and losses of more than 256 rows), where an infinity is NaN: it makes NaN of the row's results, or of all rows'.
+ * The backward takes the forward's lse and the upstream gradients dloss (float32[rows]; the caller's weights, 1 / count for a
+ * mean) and writes dhidden (zero where a row does not count) and dweight; either may be NULL. accumulate adds to what dweight
+ * holds, in float32 before the one rounding. It forms the logits again, a piece of the vocabulary at a time. The softmax's
+ * part of a gradient has the probabilities as operands in dtype (in dweight of up to 64 rows, with what that rounding left),
+ * the target's part is float32's. float16 holds the probabilities times each row's dloss relative to it, so that gradients of
+ * any size keep their bits, and in dweight the hidden states times the power of two of their dloss: both together are off by
+ * at most 2^-38 of the largest one times its dloss, so those below 2^-28 of it lose bits. float32 has pairs of float16 as
+ * operands, 22 bits and more of each value: hidden states off by at most 2^-39 of their row's largest value (in dweight,
+ * 2^-38 of the largest one times its dloss), weights of 2048 rows' largest, so values far below those lose bits. In these two
+ * types a probability in the softmax's part is off by at most 2^-39 besides: in float32 one below 2^-17 has fewer than 22
+ * bits (1e-8: 12, 1e-10: 6) and one below 2^-39 counts as zero, so dweight's rows of tokens that no row of the batch finds
+ * likelier than that are coarse or zero. NaN and infinities of a counted row's hidden state, or of weights, are what
+ * arithmetic makes of them, but for float32's pairs (all gradients, and losses of more than 256 rows), where an infinity is
+ * NaN: it makes NaN of the row's results, or of all rows'.
  * A row's loss, lse and dhidden are the same bits alone and in any batch (dhidden: from the same lse); float32's loss and lse are where
  * the batches have at most 256 rows, and where they have more: few rows are multiplied by the weights as they are. hidden_stride and dhidden_stride: elements between rows (0: dim).
  * Outputs do not overlap inputs. Limits: rows below 2^27, vocabulary below 2^31, their product below 2^48, dim at most 2^16, strides
@@ -428,13 +428,14 @@ int dllm_hip_vocabulary_loss_backward(const dllm_hip_vocabulary_loss_shape* shap
  *     A = X X^T,   X = a X + (b A + c A A) X
  * (on the transposed matrix where rows exceed cols, which is the same and smaller), and out = scale * X. coefficients: HOST, a, b
  * and c of each step; NULL: 3.4445, -4.7750, 2.0315 in all of them, which bring the singular values near one in about five
- * steps. X is held as pairs of float16, 22 bits; the products of bfloat16 updates with more than 64 singular values read float16
- * in calls of up to five steps and in the first four of more, all others such pairs. (A bfloat16 result is off by 1.0 to 1.2 times what its
- * rounding alone is, by the 2-norm, and by 1.6 at most where all singular values are alike.) Singular values have to stay where float16 holds all three: X below 15, A and b A + c A A below 255
- * (the default coefficients keep X below 1.3); others give infinities. Zeroes stay zeroes, without an eps they give NaN. Strides in elements between rows and between matrices (0: packed). out may be x with the same strides;
- * otherwise they do not overlap. Limits: rows and cols at most 2^16, batch at most 65535, batch * rows * cols below
- * 2^40, strides below 2^32 between rows and 2^47 between matrices, steps in [0, 64], eps at least 0, scale and coefficients
- * finite in float32. */
+ * steps. X is held as pairs of float16, 22 bits; the products of bfloat16 updates with more than 64 singular values read
+ * float16 in calls of up to five steps and in the first four of more, all others such pairs. (A bfloat16 result is off by 1.0
+ * to 1.2 times what its rounding alone is, by the 2-norm; where all singular values are alike by 1.4 to 1.6, and 2.1 after
+ * ten steps.) Singular values have to stay where float16 holds all three: X below 15, A and b A + c A A below 255 (the
+ * default coefficients keep X below 1.3); others give infinities. Zeroes stay zeroes, without an eps they give NaN. Strides
+ * in elements between rows and between matrices (0: packed). out may be x with the same strides; otherwise they do not
+ * overlap. Limits: rows and cols at most 2^16, batch at most 65535, batch * rows * cols below 2^40, strides below 2^32
+ * between rows and 2^47 between matrices, steps in [0, 64], eps at least 0, scale and coefficients finite in float32. */
 typedef struct {
     int64_t dtype;
     int64_t batch, rows, cols;
